@@ -10,8 +10,16 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from .. import _native
 from . import runtime as rt
 from .gemm import EPI_ATOMIC, gemm, main_grad_of, main_grads
+
+_vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
+_native.register_cuda_sigs({
+    "inv_qk_norm_fwd": [_vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _i, _vp] + [_i] * 6 + [_f, _i, _vp, _vp],
+    "inv_qk_norm_bwd_grid": [_i] * 4,
+    "inv_qk_norm_bwd": [_vp, _l, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp] + [_i] * 6 + [_f, _i, _vp, _vp],
+})
 
 
 def _acc_grad(param, g32):
@@ -278,6 +286,132 @@ def rope_qk(qkv, cos, sin, n_q_heads, n_kv_heads, head_dim, positions=None):
         rot = torch.cat([x1 * c - x2 * s, x1 * s + x2 * c], dim=-1).reshape(*lead, n_rot * head_dim)
         return torch.cat([rot, qkv[..., n_rot * head_dim:]], dim=-1)
     return _RopeFn.apply(qkv, cos, sin, positions, S, n_rot, head_dim)
+
+
+# --------------------------------------------------------------------------------------------
+# Norms of query and key heads, with the rotation in the same pass
+# --------------------------------------------------------------------------------------------
+def check_rope(cos, sin, head_dim, device):
+    """The tables of a rotation, fp32 [positions, pairs], of at most ``head_dim`` values, or None twice -> rotated values of a head."""
+    if cos is None and sin is None:
+        return 0
+    if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError("cos and sin are fp32 tables [positions, pairs], both or neither")
+    rot = 2 * cos.shape[1]
+    if not 0 < rot <= head_dim or cos.shape[0] < 1:
+        raise ValueError(f"tables {tuple(cos.shape)} for heads of {head_dim}")
+    if cos.device != device or sin.device != device:
+        raise ValueError(f"rotation tables on {cos.device}, heads on {device}")
+    return rot
+
+
+def _head_norm_rope(x, weight, eps, cos, sin):
+    """x [T, heads, D] in fp32 or 64 bits; weight [D] or None; cos, sin [T, 1, pairs] or None."""
+    if weight is not None:
+        x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps) * weight.to(x.dtype)
+    if cos is None:
+        return x
+    half = cos.shape[-1]
+    a, b = x[..., :half], x[..., half:2 * half]
+    return torch.cat([a * cos - b * sin, a * sin + b * cos, x[..., 2 * half:]], dim=-1)
+
+
+def _rows16(x, width):
+    """x as rows [T, width] that start on 16-byte boundaries: a view where it is one, else a copy."""
+    x = x.reshape(-1, width)
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) * x.element_size() % 16) or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _ld(x):
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]          # the stride of a single row says nothing
+
+
+class _QkNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, wq, wk, cos, sin, positions, seq_len, heads, kv_heads, dim, eps):
+        x = _rows16(qkv, qkv.shape[-1])
+        T, W = x.shape
+        y = torch.empty(qkv.shape, dtype=x.dtype, device=x.device)
+        rot, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
+        ctx.rows, ctx.sizes = rows, (T, seq_len, heads, kv_heads, dim, rot, float(eps), int(x.dtype == torch.float32),
+                                     rt.status_tensor(x.device).data_ptr())
+        rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), _ld(x), y.data_ptr(), W, wq.data_ptr(), wk.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
+                                          rt.ptr(positions), *ctx.sizes, rt.stream_ptr()), "inv_qk_norm_fwd")
+        ctx.main_grads = main_grads(wq, wk)
+        ctx.save_for_backward(x, wq, wk, cos, sin, positions)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, wq, wk, cos, sin, positions = ctx.saved_tensors
+        T, _, H, G, D = ctx.sizes[:5]
+        d = _rows16(dy, x.shape[1])
+        dx = torch.empty(dy.shape, dtype=x.dtype, device=x.device)
+        mg_q, mg_k = (main_grad_of(w, kept) for w, kept in zip((wq, wk), ctx.main_grads))
+        shared = None
+        if mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr():     # one weight for both norms: added one after the other
+            shared = mg_k = torch.zeros_like(mg_q)
+        grads = [None if mg is not None else torch.empty_like(w) for w, mg in ((wq, mg_q), (wk, mg_k))]
+        outs = []
+        for g, mg in zip(grads, (mg_q, mg_k)):
+            outs += [mg.data_ptr(), 2] if mg is not None else [g.data_ptr(), int(g.dtype == torch.float32)]
+        grid = rt.lib().inv_qk_norm_bwd_grid(T, H, G, D)
+        part = torch.empty(max(grid, 1) * 2 * D, dtype=torch.float32, device=x.device)
+        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), _ld(x), d.data_ptr(), _ld(d), dx.data_ptr(), x.shape[1], wq.data_ptr(), wk.data_ptr(),
+                                          rt.ptr(cos), rt.ptr(sin), ctx.rows, rt.ptr(positions), *outs, part.data_ptr(), *ctx.sizes,
+                                          rt.stream_ptr()), "inv_qk_norm_bwd")
+        rt.count_launches(1)
+        if shared is not None:
+            mg_q.add_(shared)
+        return (dx, *grads, None, None, None, None, None, None, None, None)
+
+
+def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_dim, positions=None, eps=1e-6):
+    """RMS norm of every query and key head with a weight of its own kind ([head_dim], shared by the heads), then the rotation of ``rope_qk``, in one
+    pass over qkv [..., S, (n_q + 2 n_kv) * head_dim]; the value heads are carried over. Returns a new tensor. The tables [positions, pairs] may turn
+    the first 2 * pairs values of a head only, or be None for norms alone. ``positions``: one per token, inside the tables (on a GPU one outside takes
+    the nearest row and ``check_status`` raises); None: 0 to S - 1. bf16 or fp32, weights in the same type; differentiable in qkv and the weights,
+    whose gradients are summed in an order that the sizes alone decide. On a GPU head_dim and the rotated values are multiples of 16, head_dim at
+    most 256."""
+    S, width = qkv.shape[-2] if qkv.dim() > 1 else 1, (n_q_heads + 2 * n_kv_heads) * head_dim
+    if qkv.dim() < 2 or qkv.shape[-1] != width or n_q_heads < 1 or n_kv_heads < 1:
+        raise ValueError(f"qkv of {tuple(qkv.shape)} for {n_q_heads} query and {n_kv_heads} key heads of {head_dim}")
+    for w in (q_weight, k_weight):
+        if w.shape != (head_dim,) or w.dtype != qkv.dtype or w.device != qkv.device:
+            raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {qkv.dtype} heads of {head_dim} on {qkv.device}")
+    rot = check_rope(cos, sin, head_dim, qkv.device)
+    tokens = qkv.numel() // width
+    if positions is not None and (positions.numel() != tokens or positions.dtype.is_floating_point or positions.device != qkv.device):
+        raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)} on {positions.device} for {tokens} tokens on {qkv.device}")
+    if rot and positions is None and S > cos.shape[0]:
+        raise ValueError(f"{S} positions, tables of {cos.shape[0]}")
+    if not qkv.is_cuda:
+        c = s = None
+        if rot:
+            pos = torch.arange(S).repeat(tokens // S if S else 0) if positions is None else positions.reshape(-1).long()
+            if tokens and not (0 <= int(pos.min()) and int(pos.max()) < cos.shape[0]):
+                raise ValueError(f"a position outside the tables of {cos.shape[0]}")
+            c, s = cos[pos].unsqueeze(1), sin[pos].unsqueeze(1)
+        x = qkv.reshape(tokens, -1, head_dim)
+        x = x if x.dtype == torch.float64 else x.float()
+        q, k, v = x.split([n_q_heads, n_kv_heads, n_kv_heads], dim=1)
+        y = torch.cat([_head_norm_rope(q, q_weight, eps, c, s), _head_norm_rope(k, k_weight, eps, c, s), v], dim=1)
+        return y.reshape(qkv.shape).to(qkv.dtype)
+    if qkv.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"qk_norm_rope takes bf16 or fp32 on a GPU, not {qkv.dtype}")
+    if head_dim % 16 or head_dim > 256 or rot % 16:
+        raise ValueError(f"heads of {head_dim} with {rot} rotated values: multiples of 16 up to 256 on a GPU")
+    if positions is not None:
+        positions = positions.reshape(-1).to(torch.int32).contiguous()
+    if rot:
+        cos, sin = cos.contiguous(), sin.contiguous()
+    q_weight, k_weight = (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+                          for w in (q_weight, k_weight))
+    with rt.device_of(qkv):
+        return _QkNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, positions, max(S, 1), n_q_heads, n_kv_heads, head_dim, eps)
 
 
 # --------------------------------------------------------------------------------------------

@@ -1,0 +1,312 @@
+"""Paged cache of keys and values in 8 bits (float8 e4m3) with a scale for each page of 16 tokens and key head (``csrc/paged_fp8.cu``).
+
+``qkv_append`` is everything between a fused projection and the attention: norms of the query and key heads, rotation, append of keys and values to
+the pages. ``kv_attend`` is the attention of the same new tokens over all that the pages hold, one token a sequence or many, causal, with or without a
+sliding window; ``tree_attend`` that of single rows with masks of their own. ``inference.kv_cache.PagedKVCache`` with ``fmt="fp8"`` calls them.
+
+The scale of a page and head is the smallest power of two 2^e, at least 2^-64, with |x| <= 448 * 2^e for every token in it. Later tokens can raise it;
+the codes that are there are then rounded to the new scale, which changes nothing but their exponent unless they fall under 2^-6. A value that is not
+finite makes a page of its head read as NaN until its first slot is written again."""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+
+from .. import _native
+from . import runtime as rt
+from .functional import _head_norm_rope, check_rope
+
+_vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
+_native.register_cuda_sigs({
+    "inv_fp8_append": [_vp, _l, _vp, _l, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _i, _i, _vp] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i, _i, _vp, _vp],
+    "inv_fp8_attend_splits": [_i] * 6,
+    "inv_fp8_attend": [_vp, _l, _vp, _l, _i, _i, _i, _f, _i] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i] * 4 + [_vp] * 4,
+    "inv_fp8_attend_tree": [_vp, _l, _vp, _l, _i, _i, _i, _f] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 4 + [_i, _i] + [_vp] * 4,
+})
+
+PAGE, TOP, MIN_EXP = 16, 448.0, -64
+
+
+class Fp8Pages(NamedTuple):
+    """The pools of one layer, contiguous."""
+    k: torch.Tensor          # [pages, kv_heads, 16, dim] float8_e4m3fn
+    v: torch.Tensor
+    k_scale: torch.Tensor    # [pages, kv_heads] fp32
+    v_scale: torch.Tensor
+
+
+class NewTokens(NamedTuple):
+    """Where a step's packed tokens belong: tokens [cu[i], cu[i + 1]) are the next ones of page table row ``rows[i]``, whose first ``start[i]`` positions
+    are cached already. int32 on the pools' device; ``rows`` are distinct. The bounds size the launches, so a captured step is given the largest that it
+    will be replayed with: no sequence has more than ``max_new`` tokens here, or ``max_len`` positions with them."""
+    rows: torch.Tensor       # [n]
+    cu: torch.Tensor         # [n + 1]
+    start: torch.Tensor      # [n]
+    max_new: int
+    max_len: int
+
+
+def new_pages(num_pages: int, kv_heads: int, dim: int, device) -> Fp8Pages:
+    def codes():
+        return torch.zeros(num_pages, kv_heads, PAGE, dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+
+    def scales():
+        return torch.zeros(num_pages, kv_heads, dtype=torch.float32, device=device)
+    return Fp8Pages(codes(), codes(), scales(), scales())
+
+
+def _check(x, what, heads, pages: Fp8Pages, page_table, kv_heads=None):
+    k = pages.k
+    N, G, P, D = k.shape if k.dim() == 4 else (0, 0, 0, 0)
+    if P != PAGE or pages.v.shape != k.shape or k.dtype != torch.float8_e4m3fn or pages.v.dtype != k.dtype:
+        raise ValueError(f"pages of {k.dtype} {tuple(k.shape)} and {pages.v.dtype} {tuple(pages.v.shape)}: [pages, heads, {PAGE}, dim] of float8_e4m3fn")
+    for s in (pages.k_scale, pages.v_scale):
+        if s.shape != (N, G) or s.dtype != torch.float32:
+            raise ValueError(f"page scales of {s.dtype} {tuple(s.shape)}: fp32 {(N, G)}")
+    if not all(t.is_contiguous() for t in pages):
+        raise ValueError("pages and their scales are contiguous")
+    if heads < 1 or G < 1 or heads % G or (kv_heads is not None and kv_heads != G):
+        raise ValueError(f"{heads} query heads on pages of {G}")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.is_contiguous() or page_table.numel() == 0:
+        raise ValueError(f"page table of {page_table.dtype} {tuple(page_table.shape)}: contiguous int32 [rows, pages]")
+    if x.dim() != 2 or x.stride(1) != 1:
+        raise ValueError(f"{what} of {tuple(x.shape)}: rows of tokens with unit stride")
+    dev = x.device
+    if any(t.device != dev for t in (*pages, page_table)):
+        raise ValueError(f"{what} on {dev}, pages on {k.device}, page table on {page_table.device}")
+    if x.is_cuda:
+        if x.dtype != torch.bfloat16:
+            raise TypeError(f"{what} in bf16 on a GPU, not {x.dtype}")
+        if D not in (64, 128):
+            raise ValueError(f"heads of {D}: 64 or 128 on a GPU")
+    return N, G, D
+
+
+def _check_new(new: NewTokens, dev):
+    n = new.rows.numel()
+    for t, size in ((new.rows, n), (new.cu, n + 1), (new.start, n)):
+        if t.dtype != torch.int32 or t.numel() != size or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"rows, cu and start of {n} sequences: contiguous int32 on {dev}")
+    if n and (new.max_new < 1 or new.max_len < new.max_new):
+        raise ValueError(f"max_new {new.max_new}, max_len {new.max_len}")
+    return n
+
+
+def _aligned(x):
+    """x with rows on 16-byte boundaries."""
+    if x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) % 8):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _ld(x):
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def scale_of(amax: torch.Tensor) -> torch.Tensor:
+    """The scale of pages with these largest values."""
+    m, e = torch.frexp(amax.float())                           # amax = m 2^e, m in [1/2, 1); 448 = 7/8 2^9
+    e = torch.where(m > 0.875, e - 8, e - 9).clamp(MIN_EXP, 120)
+    return torch.where(torch.isfinite(amax), torch.ldexp(torch.ones_like(m), e), torch.nan)
+
+
+def _write(x, codes, scales, page, slot):
+    """x [tokens, kv_heads, dim] into slots [slot, slot + tokens) of one page, behind what is there."""
+    new = scale_of(x.abs().amax((0, 2)))
+    raw = codes.view(torch.uint8)
+    if slot:
+        old = scales[page].clone()
+        new = torch.maximum(new, old)                          # NaN stays
+        for h in torch.nonzero(new > old).flatten().tolist():
+            raw[page, h, :slot] = (codes[page, h, :slot].float() * (old[h] / new[h])).to(codes.dtype).view(torch.uint8)
+    y = (x.transpose(0, 1) / new.view(-1, 1, 1)).to(codes.dtype).view(torch.uint8)
+    raw[page, :, slot:slot + x.shape[0]] = torch.where(torch.isnan(new).view(-1, 1, 1), torch.zeros_like(y), y)
+    scales[page] = new
+
+
+def _places(new: NewTokens, page_table, pages: int, T: int):
+    """(first token, tokens, first position, page ids) of every sequence, on the CPU."""
+    cu = new.cu.tolist()
+    for i, (row, start) in enumerate(zip(new.rows.tolist(), new.start.tolist())):
+        n = cu[i + 1] - cu[i]
+        need = -(-(start + n) // PAGE)
+        if not (0 <= cu[i] <= cu[i + 1] <= T and start >= 0 and 0 <= row < page_table.shape[0] and need <= page_table.shape[1] and n <= new.max_new):
+            raise ValueError(f"sequence {i}: tokens [{cu[i]}, {cu[i + 1]}) of {T} at position {start} of row {row}")
+        ids = page_table[row, :need].tolist()
+        if n and not all(0 <= p < pages for p in ids):
+            raise ValueError(f"row {row} lists a page outside the pool of {pages}")
+        yield cu[i], n, start, ids
+
+
+def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_table, new: NewTokens, cos=None, sin=None, positions=None, q_weight=None,
+               k_weight=None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qkv [T, (heads + 2 kv_heads) * dim]: packed tokens from the fused projection, bias included. Query and key heads are normed (``q_weight`` and
+    ``k_weight`` [dim], or neither) and rotated (tables ``cos`` and ``sin`` [positions, pairs], of the first 2 * pairs values of a head, or neither) in
+    fp32; keys and values go to the pages, whose other slots stay as they are. ``positions`` [T] int32: the rotation's, where they are not the
+    tokens' places in their sequences. Returns the queries [T, heads * dim]. On a GPU an entry that points outside the tables or the pool is reported
+    (``check_status`` raises) and its keys and values are not written."""
+    N, G, D = _check(qkv, "qkv", heads, pages, page_table, kv_heads)
+    T = qkv.shape[0]
+    if D != dim or qkv.shape[1] != (heads + 2 * G) * D:
+        raise ValueError(f"qkv of {tuple(qkv.shape)} for {heads} query and {kv_heads} key heads of {dim} on pages of {D}")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError("norm weights of queries and keys, both or neither")
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (D,) or w.dtype != qkv.dtype or w.device != qkv.device):
+            raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {qkv.dtype} heads of {D} on {qkv.device}")
+    rot = check_rope(cos, sin, D, qkv.device)
+    n = _check_new(new, qkv.device)
+    if positions is not None and (positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous() or positions.device != qkv.device):
+        raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)}: contiguous int32, one for each of {T} tokens")
+    if q_out is None:
+        q_out = torch.empty(T, heads * D, dtype=qkv.dtype, device=qkv.device)
+    elif q_out.shape != (T, heads * D) or q_out.dtype != qkv.dtype or q_out.device != qkv.device or q_out.stride(1) != 1:
+        raise ValueError(f"q_out of {q_out.dtype} {tuple(q_out.shape)} for {T} tokens of {heads} heads of {D}")
+    if not qkv.is_cuda:
+        x = qkv.float().view(T, heads + 2 * G, D)
+        for t0, m, start, ids in _places(new, page_table, N, T):
+            if not m:
+                continue
+            pos = torch.arange(start, start + m) if positions is None else positions[t0:t0 + m].long()
+            c = s = None
+            if rot:
+                if not (0 <= int(pos.min()) and int(pos.max()) < cos.shape[0]):
+                    raise ValueError(f"a position outside the tables of {cos.shape[0]}")
+                c, s = cos[pos].unsqueeze(1), sin[pos].unsqueeze(1)
+            part = x[t0:t0 + m]
+            q_out[t0:t0 + m] = _head_norm_rope(part[:, :heads], q_weight, eps, c, s).reshape(m, -1).to(qkv.dtype)
+            k, v = _head_norm_rope(part[:, heads:heads + G], k_weight, eps, c, s), part[:, heads + G:]
+            at = start
+            while at < start + m:
+                end = min(start + m, (at // PAGE + 1) * PAGE)
+                for src, codes, scales in ((k, pages.k, pages.k_scale), (v, pages.v, pages.v_scale)):
+                    _write(src[at - start:end - start], codes, scales, ids[at // PAGE], at % PAGE)
+                at = end
+        return q_out
+    if rot % 16:
+        raise ValueError(f"{rot} rotated values: a multiple of 16 on a GPU")
+    if _ld(q_out) % 8 or q_out.data_ptr() % 16:
+        raise ValueError("q_out starts and steps on 16-byte boundaries")
+    if T == 0 or n == 0:
+        return q_out
+    qkv = _aligned(qkv)
+    if q_weight is not None:
+        q_weight, k_weight = (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
+                              for w in (q_weight, k_weight))
+    if rot:
+        cos, sin = cos.contiguous(), sin.contiguous()
+    with rt.device_of(qkv):
+        rt.check(rt.lib().inv_fp8_append(qkv.data_ptr(), _ld(qkv), q_out.data_ptr(), _ld(q_out), heads, G, D, rt.ptr(q_weight), rt.ptr(k_weight),
+                                         float(eps), rt.ptr(cos), rt.ptr(sin), cos.shape[0] if rot else 0, rot, rt.ptr(positions), pages.k.data_ptr(),
+                                         pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), N, page_table.data_ptr(),
+                                         page_table.shape[0], page_table.shape[1], new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
+                                         rt.status_tensor(qkv.device).data_ptr(), rt.stream_ptr()), "inv_fp8_append")
+    return q_out
+
+
+def read(pages: Fp8Pages, ids: torch.Tensor, length: int):
+    """Keys and values [length, kv_heads, dim] in fp32 of a sequence in pages ``ids``."""
+    out = []
+    for codes, scales in ((pages.k, pages.k_scale), (pages.v, pages.v_scale)):
+        x = codes.view(torch.uint8)[ids.long()].view(codes.dtype).float() * scales[ids.long()][..., None, None]
+        out.append(x.transpose(1, 2).reshape(-1, x.shape[1], x.shape[3])[:length])
+    return out[0], out[1]
+
+
+def _softmax_rows(q, k, v, scale, seen):
+    """q [rows, heads, dim], k and v [keys, kv_heads, dim], seen [rows, keys] -> [rows, heads * dim] fp32; a row that sees nothing gives zeros."""
+    G = k.shape[1]
+    s = torch.einsum("tghd,jgd->ghtj", q.float().view(q.shape[0], G, -1, q.shape[2]), k) * scale
+    p = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
+    p = torch.where(seen.any(-1, keepdim=True), p, torch.zeros_like(p))
+    v = torch.where(seen.any(0).view(-1, 1, 1), v, torch.zeros_like(v))
+    return torch.einsum("ghtj,jgd->tghd", p, v).reshape(q.shape[0], -1)
+
+
+def _check_out(out, q, width):
+    if out is None:
+        return torch.empty(q.shape[0], width, dtype=q.dtype, device=q.device)
+    if out.shape != (q.shape[0], width) or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1:
+        raise ValueError(f"out of {out.dtype} {tuple(out.shape)} for {q.shape[0]} rows of {width}")
+    return out
+
+
+def _workspace(T, heads, splits, dim, dev):
+    """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
+    if splits == 1:
+        return None, None
+    return (torch.empty(T * heads * splits * (dim + 2), dtype=torch.float32, device=dev), torch.empty(T * heads, dtype=torch.int32, device=dev))
+
+
+def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale: Optional[float] = None, window: int = 0,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """q [T, heads * dim]: the queries of ``new``'s tokens, whose keys and values are in the pages already. The token at position p of its sequence
+    sees the positions up to p, or with ``window`` > 0 the latest ``window`` of them, its own included; query head h uses key head
+    h // (heads / kv_heads). Returns [T, heads * dim]."""
+    N, G, D = _check(q, "q", heads, pages, page_table)
+    T = q.shape[0]
+    if q.shape[1] != heads * D or window < 0:
+        raise ValueError(f"q of {tuple(q.shape)} for {heads} heads of {D}, window {window}")
+    n = _check_new(new, q.device)
+    scale = D ** -0.5 if scale is None else float(scale)
+    out = _check_out(out, q, heads * D)
+    if not q.is_cuda:
+        for t0, m, start, ids in _places(new, page_table, N, T):
+            if m:
+                k, v = read(pages, torch.tensor(ids), start + m)
+                p, j = torch.arange(start, start + m).view(-1, 1), torch.arange(start + m)
+                seen = (j <= p) & (j > p - window) if window else j <= p
+                out[t0:t0 + m] = _softmax_rows(q[t0:t0 + m].view(m, heads, D), k, v, scale, seen).to(q.dtype)
+        return out
+    if T == 0 or n == 0:
+        return out
+    q = _aligned(q)
+    with rt.device_of(q):
+        splits = rt.lib().inv_fp8_attend_splits(n, G, heads // G, new.max_new, new.max_len, window)
+        part, used = _workspace(T, heads, splits, D, q.device)
+        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, window, pages.k.data_ptr(),
+                                         pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), N, page_table.data_ptr(),
+                                         page_table.shape[0], page_table.shape[1], new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
+                                         new.max_new, new.max_len, rt.ptr(part), rt.ptr(used), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
+                 "inv_fp8_attend")
+    return out
+
+
+def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, max_len: int, scale: Optional[float] = None, tail_start=None,
+                tail_mask=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rows with masks of their own: row t of q [T, heads * dim] belongs to page table row ``row_seq[t]``, which holds ``seq_lens[row_seq[t]]`` tokens,
+    and sees those below ``tail_start[t]`` and token ``tail_start[t] + i``, i < 64, iff bit i of ``tail_mask[t]`` (int64) is set; all of them without a
+    tail. A row that sees nothing gives zeros. No row of the page table holds more than ``max_len`` tokens."""
+    N, G, D = _check(q, "q", heads, pages, page_table)
+    T = q.shape[0]
+    if q.shape[1] != heads * D or max_len < 1 or (tail_start is None) != (tail_mask is None):
+        raise ValueError(f"q of {tuple(q.shape)} for {heads} heads of {D}, max_len {max_len}, tail_start and tail_mask both or neither")
+    for t, size, dt in ((seq_lens, page_table.shape[0], torch.int32), (row_seq, T, torch.int32), (tail_start, T, torch.int32), (tail_mask, T, torch.int64)):
+        if t is not None and (t.dtype != dt or t.numel() != size or not t.is_contiguous() or t.device != q.device):
+            raise ValueError(f"{tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dt} [{size}] on {q.device}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    out = _check_out(out, q, heads * D)
+    if not q.is_cuda:
+        lens, starts, masks = seq_lens.tolist(), tail_start.tolist() if tail_start is not None else None, tail_mask.tolist() if tail_mask is not None else None
+        for t, row in enumerate(row_seq.tolist()):
+            k, v = read(pages, page_table[row, : -(-lens[row] // PAGE)], lens[row])
+            j = torch.arange(lens[row])
+            seen = torch.ones(lens[row], dtype=torch.bool)
+            if starts is not None:
+                bits = torch.tensor([(masks[t] >> i) & 1 for i in range(64)] + [0], dtype=torch.bool)
+                seen = (j < starts[t]) | bits[(j - starts[t]).clamp(0, 64)]
+            out[t] = _softmax_rows(q[t].view(1, heads, D), k, v, scale, seen.view(1, -1))[0].to(q.dtype)
+        return out
+    if T == 0:
+        return out
+    q = _aligned(q)
+    with rt.device_of(q):
+        splits = rt.lib().inv_fp8_attend_splits(T, G, heads // G, 1, max_len, 0)
+        part, used = _workspace(T, heads, splits, D, q.device)
+        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, pages.k.data_ptr(), pages.v.data_ptr(),
+                                              pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), N, page_table.data_ptr(), page_table.shape[0],
+                                              page_table.shape[1], row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
+                                              max_len, rt.ptr(part), rt.ptr(used), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
+                 "inv_fp8_attend_tree")
+    return out

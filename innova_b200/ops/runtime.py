@@ -17,6 +17,22 @@ def stream_ptr() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())   # no Stream object made for every launch
 
 
+class device_of:
+    """``with device_of(t)``: launches go to the device of ``t`` and its current stream. Costs nothing where that device is current."""
+
+    def __init__(self, t: torch.Tensor):
+        self.index, self.back = t.device.index, None
+
+    def __enter__(self):
+        if self.index is not None and self.index != torch.cuda.current_device():
+            self.back = torch.cuda.current_device()
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+
+
 def status_tensor(device=None) -> torch.Tensor:
     """One int32 word per device into which kernels write a code when a bounded wait runs out."""
     if device is None:
