@@ -62,11 +62,11 @@ __device__ __forceinline__ int pool_page(const Fp8Tokens& t, int pages, int row,
 
 // ---------------------------------------------------------------------------------------------- append
 struct Fp8Append {
-  const __nv_bfloat16 *qkv, *wq, *wk;   // weights null: no norm
+  const __nv_bfloat16 *q_in, *k_in, *v_in, *wq, *wk;   // rows ld_in apart, H, Hkv and Hkv heads side by side; weights null: no norm
   const float *cos_t, *sin_t;           // null: no rotation
   const int* pos;                       // positions of the rotation, per token; null: the token's place in its sequence
   __nv_bfloat16* q;
-  long ld, ld_q;
+  long ld_in, ld_v, ld_q;
   int H, rot, table_rows;
   float eps;
 };
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256) fp8_append_kernel(const __grid_constant__
   const int page = pool_page(tk, pool.pages, tk.rows[seq], pg);
   const HeadUnit h(u, D, a.rot);
   // queries: (group of tokens, a run of heads)
-  const int run = max(1, (h1 - h0) * groups / 16), runs = (h1 - h0 + run - 1) / run;
+  const int run = max(1, (h1 - h0) * groups / 16), runs = (h1 - h0 + run - 1) / run;      // none without query heads
   const int n_kv = page < 0 ? 0 : g1 - g0;
   for (int item = warp; item < n_kv + groups * runs; item += 8) {
     if (item >= n_kv) {
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) fp8_append_kernel(const __grid_constant__
       if (a.rot) turn.load(a.cos_t, a.sin_t, a.rot, table_row(a.pos ? a.pos[t] : at, a.table_rows, tk.status), u, h);
       float w[16];
       if (a.wq) load_unit(a.wq, h, w);
-      const __nv_bfloat16* src = a.qkv + t * a.ld;
+      const __nv_bfloat16* src = a.q_in + t * a.ld_in;
       __nv_bfloat16* dst = a.q + t * a.ld_q;
 #pragma unroll 2
       for (int hd = hq; hd < min(h1, hq + run); ++hd) {
@@ -136,14 +136,15 @@ __global__ void __launch_bounds__(256) fp8_append_kernel(const __grid_constant__
       continue;
     }
     const int g = g0 + item, hk = g >> 1, which = g & 1;         // 0 keys, 1 values
-    const __nv_bfloat16* src = a.qkv + (a.H + which * pool.Hkv + hk) * D;
+    const __nv_bfloat16* src = (which ? a.v_in : a.k_in) + hk * D;
+    const long ld = which ? a.ld_v : a.ld_in;
     float x[NIT][16];
     uint32_t amax = 0;
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
       if (it >= groups) break;
       const int at = lo + min(it * HPW + sub, m - 1), t = t0 + at - start;      // lanes past the last token repeat it
-      load_unit(src + t * a.ld, h, x[it]);
+      load_unit(src + t * ld, h, x[it]);
       if (!which) {
         if (a.wk) {
           float w[16];
@@ -580,18 +581,18 @@ static bool off16(const void* a, const void* b = nullptr, const void* c = nullpt
   return ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16 != 0;
 }
 
-// qkv [T, (H + 2 Hkv) D] bf16, rows ld apart -> q [T, H D] normed and rotated, rows ld_q apart, and the pools. wq, wk [D] bf16 or null; cos_t, sin_t
-// [table_rows, rot / 2] fp32 or null with rot 0; pos [T] or null.
-extern "C" int inv_fp8_append(const void* qkv, long ld, void* q, long ld_q, int H, int Hkv, int D, const void* wq, const void* wk, float eps,
-                              const float* cos_t, const float* sin_t, int rope_rows, int rot, const int* pos, void* k_pool, void* v_pool, float* k_scale,
-                              float* v_scale, int pages, const int* page_table, int table_rows, int max_pages, const int* rows, const int* cu,
-                              const int* start, int n, int T, int* status, void* stream) {
-  if (fp8_bad_shape(H, Hkv, D, pages, n, T, table_rows, max_pages) || rot < 0 || rot > D || rot % 16 || (rot && (!cos_t || !sin_t || rope_rows < 1)))
-    return -ERR_BAD_ARG;
-  if (ld % 8 || ld_q % 8 || off16(qkv, q, wq, wk) || off16(cos_t, sin_t, k_pool, v_pool)) return -ERR_BAD_ARG;
+// q_in [T, H D], k_in, v_in [T, Hkv D] bf16 -> q [T, H D] normed and rotated, and the pools. Queries and keys have rows ld_in apart, values ld_v, q
+// ld_q; H may be 0. wq, wk [D] bf16 or null; cos_t, sin_t [rope_rows, rot / 2] fp32 or null with rot 0; pos [T] or null.
+extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, const void* v_in, long ld_v, void* q, long ld_q, int H, int Hkv, int D,
+                              const void* wq, const void* wk, float eps, const float* cos_t, const float* sin_t, int rope_rows, int rot, const int* pos,
+                              void* k_pool, void* v_pool, float* k_scale, float* v_scale, int pages, const int* page_table, int table_rows,
+                              int max_pages, const int* rows, const int* cu, const int* start, int n, int T, int* status, void* stream) {
+  if (fp8_bad_shape(H ? H : Hkv, Hkv, D, pages, n, T, table_rows, max_pages) || rot < 0 || rot > D || rot % 16) return -ERR_BAD_ARG;
+  if (rot && (!cos_t || !sin_t || rope_rows < 1)) return -ERR_BAD_ARG;
+  if (ld_in % 8 || ld_v % 8 || ld_q % 8 || off16(q_in, k_in, v_in, q) || off16(wq, wk) || off16(cos_t, sin_t, k_pool, v_pool)) return -ERR_BAD_ARG;
   if (n == 0 || T == 0) return 0;
-  const Fp8Append a{(const __nv_bfloat16*)qkv, (const __nv_bfloat16*)wq, (const __nv_bfloat16*)wk, cos_t, sin_t, pos, (__nv_bfloat16*)q, ld, ld_q, H, rot,
-                    rope_rows, eps};
+  const Fp8Append a{(const __nv_bfloat16*)q_in, (const __nv_bfloat16*)k_in, (const __nv_bfloat16*)v_in, (const __nv_bfloat16*)wq,
+                    (const __nv_bfloat16*)wk, cos_t, sin_t, pos, (__nv_bfloat16*)q, ld_in, ld_v, ld_q, H, rot, rope_rows, eps};
   const Fp8Pool pool{(uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, pages, Hkv};
   const Fp8Tokens tk{rows, cu, start, page_table, n, T, table_rows, max_pages, status};
   const unsigned ctas = (unsigned)(T / FP8_PAGE + 2 * n);

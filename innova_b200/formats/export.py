@@ -47,6 +47,7 @@ def parse_config(blob: bytes, tensor_names=()) -> Optional[TransformerConfig]:
     cfg.positions = "learned" if "pos_embeddings.weight" in names else "rope"
     cfg.norm = "layernorm" if "layers.0.attention_norm.bias" in names else "rmsnorm"
     cfg.bias = "layers.0.attention.q_proj.bias" in names
+    cfg.qk_norm = "layers.0.attention.q_norm.weight" in names
     if "layers.0.ffn.gate_proj.weight" not in names and cfg.activation == "silu":
         cfg.activation = "gelu"
     cfg.vocab_pad_to = 1

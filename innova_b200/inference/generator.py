@@ -4,7 +4,8 @@ Covers the reference's Generator / StreamingGenerator (src/generator.cpp:14-63 p
 KV cache, :129-144 stats, :149-353 per-token callbacks, stop tokens, cooperative stop) and the
 InferenceEngine generate / stream / batch entry points (engines/inference/inference.cpp:72-145).
 Prefill runs the flash-attention kernel on the whole prompt and appends K/V to the cache; every decode
-step runs the projections as skinny GEMMs and ``paged_decode`` attention over the (OIL4 or bf16) cache.
+step runs the projections as skinny GEMMs and ``paged_decode`` attention over the (OIL4 or bf16) cache, or over an
+fp8 cache (``kv_format="fp8"``) one launch from the projection to the pages and one attention for any number of new tokens.
 """
 from __future__ import annotations
 
@@ -78,14 +79,20 @@ class Generator:
         pos32 = pos.reshape(-1).to(torch.int32).contiguous()
         prefill = S > 1 and all(s == 0 for s in start)
         scale = D ** -0.5
+        packed = cache.new_tokens(batch_ids, list(start), [S] * B) if cache.fmt == "fp8" else None
         for li, blk in enumerate(m.layers):
             h = blk.attention_norm(x)
             qkv = self.linear(h, blk.attention.qkv_proj)
-            if rope is not None:
-                qkv = ops.rope_qk(qkv, rope[0], rope[1], H, Hkv, D, pos32)
+            if packed is not None and not prefill:
+                q = cache.append_rope(li, qkv.reshape(B * S, -1), H, packed, rope, None, *blk.attention.head_norms())
+                if li == 0:
+                    cache.commit(batch_ids, [s + S for s in start])
+                x = self._after_attention(blk, x, cache.attend(li, q, packed, H, scale).view(B, S, -1))
+                continue
+            qkv = blk.attention.turn(qkv, rope, pos32)
             k = qkv[..., H * D:(H + Hkv) * D]
             v = qkv[..., (H + Hkv) * D:]
-            cache.append(li, k, v, batch_ids, start)
+            cache.append(li, k, v, batch_ids, start, packed)
             if prefill:
                 a = ops.flash_attention(qkv.contiguous(), H, Hkv, D, causal=True)
             else:
@@ -106,15 +113,10 @@ class Generator:
                         outs.append(cache.decode_attention(li, qkv[:, s], H, scale))
                     a = torch.stack(outs, dim=1).to(x.dtype)
                     cache.commit(batch_ids, [start[b] + S for b in range(B)])
-            att = self.linear(a, blk.attention.o_proj)
-            if cfg.use_parallel_residual:
-                x = x + att + self._ffn(blk, blk.ffn_norm(x))
-            else:
-                x = x + att
-                x = x + self._ffn(blk, blk.ffn_norm(x))
+            x = self._after_attention(blk, x, a)
         if prefill:
             cache.commit(batch_ids, [S] * B)
-        assert prefill or slots is None, "decoding runs on cache rows 0..B-1"
+        assert prefill or slots is None or packed is not None, "decoding runs on cache rows 0..B-1"
         last = m.norm(x if all_logits else x[:, -1])
         logits = ops.linear(last, m.lm_head.weight)
         return logits[..., : cfg.vocab_size]
@@ -192,23 +194,30 @@ class Generator:
         rope = m.rope(dev)
         pos32 = pos.reshape(-1).to(torch.int32).contiguous()
         scale = D ** -0.5
+        packed = cache.new_tokens([row], [start], [T]) if cache.fmt == "fp8" else None
         for li, blk in enumerate(m.layers):
             h = blk.attention_norm(x)
             qkv = self.linear(h, blk.attention.qkv_proj)
-            if rope is not None:
-                qkv = ops.rope_qk(qkv, rope[0], rope[1], H, Hkv, D, pos32)
-            cache.append(li, qkv[..., H * D:(H + Hkv) * D], qkv[..., (H + Hkv) * D:], [row], [start])
+            if packed is not None:
+                q = cache.append_rope(li, qkv.view(T, -1), H, packed, rope, pos32, *blk.attention.head_norms())
+            else:
+                qkv = blk.attention.turn(qkv, rope, pos32)
+                cache.append(li, qkv[..., H * D:(H + Hkv) * D], qkv[..., (H + Hkv) * D:], [row], [start])
+                q = qkv.view(T, -1)
             if li == 0:
                 cache.commit([row], [start + T])
-            a = cache.tree_attention(li, qkv.view(T, -1), H, scale, row_seq, tail_start, tail_mask).view(1, T, -1).to(x.dtype)
-            att = self.linear(a, blk.attention.o_proj)
-            if cfg.use_parallel_residual:
-                x = x + att + self._ffn(blk, blk.ffn_norm(x))
-            else:
-                x = x + att
-                x = x + self._ffn(blk, blk.ffn_norm(x))
+            a = cache.tree_attention(li, q, H, scale, row_seq, tail_start, tail_mask).view(1, T, -1).to(x.dtype)
+            x = self._after_attention(blk, x, a)
         logits = ops.linear(m.norm(x[0]), m.lm_head.weight)
         return logits[..., : cfg.vocab_size]
+
+    def _after_attention(self, blk, x, a):
+        """The rest of a block behind its attention's output ``a``."""
+        att = self.linear(a, blk.attention.o_proj)
+        if self.cfg.use_parallel_residual:
+            return x + att + self._ffn(blk, blk.ffn_norm(x))
+        x = x + att
+        return x + self._ffn(blk, blk.ffn_norm(x))
 
     def _ffn(self, blk, h):
         f = blk.ffn

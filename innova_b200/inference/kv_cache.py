@@ -1,8 +1,9 @@
 """KV caches for generation.
 
-``PagedKVCache``: pools of 16-token pages per layer with a page table per sequence, in bf16 or in
+``PagedKVCache``: pools of 16-token pages per layer with a page table per sequence, in bf16, in
 the OIL4 KV format (4-bit indices + fp16 scale per 32 values), appended and read by
-``csrc/paged_attn.cu`` on the GPU and by the PyTorch code below on the CPU. Covers the reference's
+``csrc/paged_attn.cu`` on the GPU and by the PyTorch code below on the CPU, or in float8 with a scale
+per page and head (``ops/paged_fp8.py``). Covers the reference's
 KVCache (src/kv_cache.cpp:85-280), PagedKVCacheBase / block tables with a physical-memory cap and
 LRU page eviction (include/oil/kv_cache.h:73-238, src/kv_cache.cpp:286-569), OIL4KVCache
 (src/kv_cache_oil4.cpp:207-362) and the checkpoint / rewind used by speculative decoding.
@@ -15,6 +16,7 @@ from typing import List, Optional
 import torch
 
 from .. import _native
+from ..ops import paged_fp8
 from ..ops import runtime as rt
 
 _native.register_cuda_sigs({
@@ -149,9 +151,16 @@ class PagedRows:
 class PagedKVCache(PagedRows):
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, max_batch: int, max_seq: int, device, fmt: str = "oil4",
                  num_pages: Optional[int] = None):
-        assert fmt in ("oil4", "bf16") and (fmt == "bf16" or head_dim % 32 == 0)
+        assert fmt in ("oil4", "bf16", "fp8") and (fmt != "oil4" or head_dim % 32 == 0)
+        if fmt == "fp8" and torch.device(device).type == "cuda" and head_dim not in (64, 128):
+            raise ValueError(f"an fp8 cache on a GPU holds heads of 64 or 128, not {head_dim}")
         super().__init__(max_batch, max_seq, device, num_pages)
         self.L, self.Hkv, self.D, self.fmt = num_layers, num_kv_heads, head_dim, fmt
+        if fmt == "fp8":
+            self.pages = [paged_fp8.new_pages(self.num_pages, num_kv_heads, head_dim, self.device) for _ in range(num_layers)]
+            self.k_pool, self.v_pool, self.k_scale, self.v_scale = map(list, zip(*self.pages))
+            self._all_rows = torch.arange(max_batch, dtype=torch.int32, device=self.device)
+            return
         row = head_dim // 2 if fmt == "oil4" else head_dim * 2  # bytes per token per head
         self.k_pool = [torch.zeros(self.num_pages, num_kv_heads, PAGE, row, dtype=torch.uint8, device=self.device) for _ in range(num_layers)]
         self.v_pool = [torch.zeros_like(self.k_pool[0]) for _ in range(num_layers)]
@@ -163,13 +172,49 @@ class PagedKVCache(PagedRows):
             self.k_scale = self.v_scale = [None] * num_layers
 
     def bytes_per_token(self) -> int:
+        if self.fmt == "fp8":
+            return 2 * self.L * self.Hkv * (self.D * PAGE + 4) // PAGE
         per = self.D // 2 + (self.D // 32) * 2 if self.fmt == "oil4" else self.D * 2
         return 2 * self.L * self.Hkv * per
 
+    # ------------------------------------------------------------------ steps over an fp8 cache
+    def new_tokens(self, batch_ids: List[int], start: List[int], counts: List[int]) -> paged_fp8.NewTokens:
+        """Where ``counts[i]`` new tokens of sequence ``batch_ids[i]`` go, which holds ``start[i]`` already and owns the pages for them (``reserve``):
+        made once a step, used by every layer's ``append_rope`` and ``attend``."""
+        if self.fmt != "fp8":
+            raise NotImplementedError(f"packed steps over a cache of {self.fmt}")
+        n = len(batch_ids)
+        if len(start) != n or len(counts) != n or len(set(batch_ids)) != n:
+            raise ValueError(f"rows {list(batch_ids)} with {len(start)} starts and {len(counts)} counts: one of each a row, no row twice")
+        cu = [0]
+        for b, s, c in zip(batch_ids, start, counts):
+            if not 0 <= b < self.max_batch or s < 0 or c < 0 or s + c > PAGE * len(self._host_pages[b]) or s // PAGE < self._released[b] and c:
+                raise ValueError(f"{c} tokens at position {s} of row {b}: outside its pages")
+            cu.append(cu[-1] + c)
+        buf = torch.tensor([*batch_ids, *start, *cu], dtype=torch.int32).to(self.device)
+        return paged_fp8.NewTokens(buf[:n], buf[2 * n:], buf[n:2 * n], max([1, *counts]), max([1, *(s + c for s, c in zip(start, counts))]))
+
+    def append_rope(self, layer: int, qkv: torch.Tensor, num_heads: int, new: paged_fp8.NewTokens, rope=None, positions=None, q_weight=None,
+                    k_weight=None, eps: float = 1e-6) -> torch.Tensor:
+        """qkv [T, (num_heads + 2 kv_heads) * D] of the step's tokens: keys and values go to the pages, query and key heads normed and rotated on the way
+        (``rope``: tables of cosines and sines; ``positions``: the rotation's, where tokens are stored elsewhere) -> queries [T, num_heads * D]."""
+        cos, sin = rope if rope is not None else (None, None)
+        return paged_fp8.qkv_append(qkv, num_heads, self.Hkv, self.D, self.pages[layer], self.page_table, new, cos, sin, positions, q_weight, k_weight, eps)
+
+    def attend(self, layer: int, q: torch.Tensor, new: paged_fp8.NewTokens, num_heads: int, scale: float, window: int = 0,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Causal attention of the step's tokens, which are in the pages, over their sequences. q [T, num_heads * D] -> the same shape."""
+        return paged_fp8.kv_attend(q, self.pages[layer], self.page_table, new, num_heads, scale, window, out)
+
     # ------------------------------------------------------------------ append / attend
-    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch_ids: List[int], start: List[int]):
-        """k, v: [B, S_new, Hkv*D] views (token-major, unit inner stride) for the listed sequences."""
+    def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch_ids: List[int], start: List[int],
+               new: Optional[paged_fp8.NewTokens] = None):
+        """k, v: [B, S_new, Hkv*D] views (token-major, unit inner stride) for the listed sequences. ``new``: the step's, where the cache is fp8 and it
+        is made already."""
         B, S_new = k.shape[0], k.shape[1]
+        if self.fmt == "fp8":
+            k, v = (x.reshape(B * S_new, x.shape[-1]) for x in (k, v))
+            return paged_fp8.kv_append(k, v, self.pages[layer], self.page_table, new or self.new_tokens(batch_ids, start, [S_new] * B))
         if k.is_cuda:
             # the kernel walks consecutive cache rows from the row its page-table pointer starts at: one launch per run of
             # consecutive rows (a running batch is one run; a request admitted into row r is a run of one)
@@ -209,6 +254,8 @@ class PagedKVCache(PagedRows):
         """Dequantised K, V of one sequence: [len, Hkv, D] fp32 (CPU path and tests)."""
         n = self._host_lens[b]
         pages = torch.tensor(self._host_pages[b], dtype=torch.long, device=self.device)
+        if self.fmt == "fp8":
+            return paged_fp8.read(self.pages[layer], pages, n)
         out = []
         for pool, scale in ((self.k_pool[layer], self.k_scale[layer]), (self.v_pool[layer], self.v_scale[layer])):
             raw = pool[pages]  # [P, Hkv, 16, row]
@@ -226,6 +273,9 @@ class PagedKVCache(PagedRows):
         """q: [B, >= H*D] token-major rows (one new token per sequence, already appended) -> [B, H*D]."""
         B = q.shape[0]
         H, D = num_heads, self.D
+        if self.fmt == "fp8":
+            return paged_fp8.tree_attend(q[:, : H * D], self.pages[layer], self.page_table, self.seq_lens, self._all_rows[:B], H,
+                                         max([1, *self._host_lens[:B]]), scale, out=out)
         if q.is_cuda:
             out = out if out is not None else torch.empty(B, H * D, dtype=torch.bfloat16, device=q.device)
             max_len = max(self._host_lens[:B]) if B else 0
@@ -257,6 +307,9 @@ class PagedKVCache(PagedRows):
         ``(1 << (s + 1)) - 1``; a tree row sets the bits of its ancestors and its own (include/oil/inference_opt.h:262-298)."""
         T = q.shape[0]
         H, D = num_heads, self.D
+        if self.fmt == "fp8":
+            return paged_fp8.tree_attend(q[:, : H * D], self.pages[layer], self.page_table, self.seq_lens, row_seq, H, max([1, *self._host_lens]), scale,
+                                         tail_start, tail_mask, out)
         if q.is_cuda:
             out = out if out is not None else torch.empty(T, H * D, dtype=torch.bfloat16, device=q.device)
             max_len = max(self._host_lens) if self._host_lens else 0

@@ -34,6 +34,7 @@ class TransformerConfig:
     norm: str = "rmsnorm"             # "rmsnorm" | "layernorm"
     positions: str = "rope"           # "rope" | "learned"
     bias: bool = False
+    qk_norm: bool = False             # RMS norm of every query and key head before the rotation
     tie_embeddings: bool = False
     # MoE (0 experts = dense)
     num_experts: int = 0

@@ -42,6 +42,27 @@ class Norm(nn.Module):
         return ops.norm_residual(x, self.weight, self.bias, self.eps, rms=self.kind != "layernorm")
 
 
+class HeadNorm(nn.Module):
+    """Weight of an RMS norm over each head, applied by ``ops.qk_norm_rope``."""
+
+    def __init__(self, dim, eps, dtype):
+        super().__init__()
+        self.eps = eps
+        self.weight = nn.Parameter(torch.ones(dim, dtype=dtype))
+
+
+def head_norm_state(out, pre, att):
+    """The head norms of a block under ``pre`` in a flat state."""
+    if att.q_norm is not None:
+        out[pre + "attention.q_norm.weight"], out[pre + "attention.k_norm.weight"] = att.q_norm.weight, att.k_norm.weight
+
+
+def load_head_norms(tensors, pre, att):
+    if att.q_norm is not None:
+        for norm, name in ((att.q_norm, "q_norm"), (att.k_norm, "k_norm")):
+            norm.weight.copy_(tensors[pre + f"attention.{name}.weight"].view(-1))
+
+
 class Attention(nn.Module):
     def __init__(self, cfg: TransformerConfig, dtype):
         super().__init__()
@@ -49,12 +70,27 @@ class Attention(nn.Module):
         H, Hkv, D, E = cfg.num_heads, cfg.kv_heads, cfg.head_dim, cfg.hidden_size
         self.qkv_proj = nn.Linear(E, (H + 2 * Hkv) * D, bias=cfg.bias, dtype=dtype)
         self.o_proj = nn.Linear(H * D, E, bias=cfg.bias, dtype=dtype)
+        self.q_norm = HeadNorm(D, cfg.norm_eps, dtype) if cfg.qk_norm else None
+        self.k_norm = HeadNorm(D, cfg.norm_eps, dtype) if cfg.qk_norm else None
+
+    def head_norms(self):
+        """(weight of the query heads' norm, of the key heads', eps)."""
+        return (None, None, self.cfg.norm_eps) if self.q_norm is None else (self.q_norm.weight, self.k_norm.weight, self.q_norm.eps)
+
+    def turn(self, qkv, rope, positions=None):
+        """The norms and the rotation of the query and key heads in qkv."""
+        cfg = self.cfg
+        if self.q_norm is not None:
+            cos, sin = rope if rope is not None else (None, None)
+            wq, wk, eps = self.head_norms()
+            return ops.qk_norm_rope(qkv, wq, wk, cos, sin, cfg.num_heads, cfg.kv_heads, cfg.head_dim, positions, eps)
+        if rope is not None:
+            return ops.rope_qk(qkv, rope[0], rope[1], cfg.num_heads, cfg.kv_heads, cfg.head_dim, positions)
+        return qkv
 
     def forward(self, h, residual, rope, positions=None):
         cfg = self.cfg
-        qkv = ops.linear(h, _ste(self.qkv_proj.weight, cfg), self.qkv_proj.bias)
-        if rope is not None:
-            qkv = ops.rope_qk(qkv, rope[0], rope[1], cfg.num_heads, cfg.kv_heads, cfg.head_dim, positions)
+        qkv = self.turn(ops.linear(h, _ste(self.qkv_proj.weight, cfg), self.qkv_proj.bias), rope, positions)
         a = ops.flash_attention(qkv, cfg.num_heads, cfg.kv_heads, cfg.head_dim, causal=True)
         return ops.linear(a, _ste(self.o_proj.weight, cfg), self.o_proj.bias, residual=residual, mode="add")
 
@@ -216,6 +252,7 @@ class DenseModel(nn.Module):
             q, k, v = blk.attention.qkv_proj.weight.split([H * D, Hkv * D, Hkv * D], dim=0)
             out[pre + "attention.q_proj.weight"], out[pre + "attention.k_proj.weight"], out[pre + "attention.v_proj.weight"] = q, k, v
             out[pre + "attention.o_proj.weight"] = blk.attention.o_proj.weight
+            head_norm_state(out, pre, blk.attention)
             if cfg.bias:
                 qb, kb, vb = blk.attention.qkv_proj.bias.split([H * D, Hkv * D, Hkv * D], dim=0)
                 out[pre + "attention.q_proj.bias"], out[pre + "attention.k_proj.bias"], out[pre + "attention.v_proj.bias"] = qb, kb, vb
@@ -268,6 +305,7 @@ class DenseModel(nn.Module):
             v = mat(pre + "attention.v_proj.weight", Hkv * D, E)
             blk.attention.qkv_proj.weight.copy_(torch.cat([q, k, v], dim=0))
             blk.attention.o_proj.weight.copy_(mat(pre + "attention.o_proj.weight", E, H * D))
+            load_head_norms(tensors, pre, blk.attention)
             if cfg.bias and pre + "attention.q_proj.bias" in tensors:
                 blk.attention.qkv_proj.bias.copy_(torch.cat([tensors[pre + f"attention.{n}_proj.bias"].view(-1) for n in "qkv"]))
                 blk.attention.o_proj.bias.copy_(tensors[pre + "attention.o_proj.bias"].view(-1))

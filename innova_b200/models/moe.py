@@ -16,7 +16,7 @@ import torch.nn as nn
 from .. import ops
 from ..ops.moe import moe_ffn
 from .config import TransformerConfig
-from .dense import Attention, FFN, Norm, _ste
+from .dense import Attention, FFN, Norm, _ste, head_norm_state, load_head_norms
 
 
 class MoELayer(nn.Module):
@@ -154,6 +154,7 @@ class MoEModel(nn.Module):
             q, k, v = blk.attention.qkv_proj.weight.split([H * D, Hkv * D, Hkv * D], dim=0)
             out[pre + "attention.q_proj.weight"], out[pre + "attention.k_proj.weight"], out[pre + "attention.v_proj.weight"] = q, k, v
             out[pre + "attention.o_proj.weight"] = blk.attention.o_proj.weight
+            head_norm_state(out, pre, blk.attention)
             out[pre + "moe.router.weight"] = blk.moe.router.weight
             for e in range(cfg.num_experts):
                 g, u = blk.moe.w_gate_up[e].chunk(2, dim=0)
@@ -187,6 +188,7 @@ class MoEModel(nn.Module):
             blk.attention.qkv_proj.weight.copy_(torch.cat([mat(pre + "attention.q_proj.weight", H * D, E), mat(pre + "attention.k_proj.weight", Hkv * D, E),
                                                            mat(pre + "attention.v_proj.weight", Hkv * D, E)], dim=0))
             blk.attention.o_proj.weight.copy_(mat(pre + "attention.o_proj.weight", E, H * D))
+            load_head_norms(tensors, pre, blk.attention)
             blk.moe.router.weight.copy_(mat(pre + "moe.router.weight", cfg.num_experts, E))
             for e in range(cfg.num_experts):
                 blk.moe.w_gate_up[e].copy_(torch.cat([mat(pre + f"moe.expert.{e}.gate_proj.weight", Fh, E),

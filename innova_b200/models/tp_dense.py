@@ -98,6 +98,8 @@ class TPDenseModel(nn.Module):
     def __init__(self, cfg: TransformerConfig, tp_group=None, dtype=torch.bfloat16, device="cuda", seed: int = 0, comm: Optional[FusedGemmComm] = None,
                  cache_ste: bool = False):
         super().__init__()
+        if cfg.qk_norm:
+            raise NotImplementedError("the tensor-parallel decoder has no norms of query and key heads")
         self.cfg = cfg
         self.tp_group = tp_group
         dev = torch.device(device)

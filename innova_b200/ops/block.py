@@ -124,7 +124,7 @@ def block_forward(blk, x, rope, positions):
     Looked at in every call."""
     cfg, att, ffn, n1, n2 = blk.cfg, blk.attention, blk.ffn, blk.attention_norm, blk.ffn_norm
     gated = ffn.gated
-    if (x.dim() != 3 or not _plain(x) or x.numel() == 0 or cfg.use_parallel_residual or ffn.adapter is not None
+    if (x.dim() != 3 or not _plain(x) or x.numel() == 0 or cfg.use_parallel_residual or att.q_norm is not None or ffn.adapter is not None
             or not (gated or cfg.activation == "gelu") or cfg.head_dim not in (64, 128) or _gemm._side_job_provider is not None
             or (cfg.ste_format and (cfg.ste_format not in MODES or cfg.ste_block != BLOCK)) or n1.kind != n2.kind):
         return None

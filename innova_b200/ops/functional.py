@@ -324,6 +324,11 @@ def _rows16(x, width):
     return x
 
 
+def _weights16(*weights):
+    """Norm weights as the kernels read them: dense, on 16-byte boundaries."""
+    return [w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.detach().clone(memory_format=torch.contiguous_format) for w in weights]
+
+
 def _ld(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]          # the stride of a single row says nothing
 
@@ -335,9 +340,10 @@ class _QkNormRopeFn(torch.autograd.Function):
         T, W = x.shape
         y = torch.empty(qkv.shape, dtype=x.dtype, device=x.device)
         rot, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
+        a, b = _weights16(wq, wk)
         ctx.rows, ctx.sizes = rows, (T, seq_len, heads, kv_heads, dim, rot, float(eps), int(x.dtype == torch.float32),
                                      rt.status_tensor(x.device).data_ptr())
-        rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), _ld(x), y.data_ptr(), W, wq.data_ptr(), wk.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
+        rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), _ld(x), y.data_ptr(), W, a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
                                           rt.ptr(positions), *ctx.sizes, rt.stream_ptr()), "inv_qk_norm_fwd")
         ctx.main_grads = main_grads(wq, wk)
         ctx.save_for_backward(x, wq, wk, cos, sin, positions)
@@ -348,19 +354,19 @@ class _QkNormRopeFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, wq, wk, cos, sin, positions = ctx.saved_tensors
         T, _, H, G, D = ctx.sizes[:5]
-        d = _rows16(dy, x.shape[1])
+        d, (a, b) = _rows16(dy, x.shape[1]), _weights16(wq, wk)
         dx = torch.empty(dy.shape, dtype=x.dtype, device=x.device)
         mg_q, mg_k = (main_grad_of(w, kept) for w, kept in zip((wq, wk), ctx.main_grads))
         shared = None
         if mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr():     # one weight for both norms: added one after the other
             shared = mg_k = torch.zeros_like(mg_q)
-        grads = [None if mg is not None else torch.empty_like(w) for w, mg in ((wq, mg_q), (wk, mg_k))]
+        grads = [None if mg is not None else torch.empty(w.shape, dtype=w.dtype, device=w.device) for w, mg in ((wq, mg_q), (wk, mg_k))]
         outs = []
         for g, mg in zip(grads, (mg_q, mg_k)):
             outs += [mg.data_ptr(), 2] if mg is not None else [g.data_ptr(), int(g.dtype == torch.float32)]
         grid = rt.lib().inv_qk_norm_bwd_grid(T, H, G, D)
         part = torch.empty(max(grid, 1) * 2 * D, dtype=torch.float32, device=x.device)
-        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), _ld(x), d.data_ptr(), _ld(d), dx.data_ptr(), x.shape[1], wq.data_ptr(), wk.data_ptr(),
+        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), _ld(x), d.data_ptr(), _ld(d), dx.data_ptr(), x.shape[1], a.data_ptr(), b.data_ptr(),
                                           rt.ptr(cos), rt.ptr(sin), ctx.rows, rt.ptr(positions), *outs, part.data_ptr(), *ctx.sizes,
                                           rt.stream_ptr()), "inv_qk_norm_bwd")
         rt.count_launches(1)
@@ -408,8 +414,6 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
         positions = positions.reshape(-1).to(torch.int32).contiguous()
     if rot:
         cos, sin = cos.contiguous(), sin.contiguous()
-    q_weight, k_weight = (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
-                          for w in (q_weight, k_weight))
     with rt.device_of(qkv):
         return _QkNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, positions, max(S, 1), n_q_heads, n_kv_heads, head_dim, eps)
 

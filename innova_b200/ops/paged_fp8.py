@@ -15,11 +15,11 @@ import torch
 
 from .. import _native
 from . import runtime as rt
-from .functional import _head_norm_rope, check_rope
+from .functional import _head_norm_rope, _weights16, check_rope
 
 _vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
 _native.register_cuda_sigs({
-    "inv_fp8_append": [_vp, _l, _vp, _l, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _i, _i, _vp] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i, _i, _vp, _vp],
+    "inv_fp8_append": [_vp, _vp, _l, _vp, _l, _vp, _l, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _i, _i, _vp] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i, _i, _vp, _vp],
     "inv_fp8_attend_splits": [_i] * 6,
     "inv_fp8_attend": [_vp, _l, _vp, _l, _i, _i, _i, _f, _i] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i] * 4 + [_vp] * 4,
     "inv_fp8_attend_tree": [_vp, _l, _vp, _l, _i, _i, _i, _f] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 4 + [_i, _i] + [_vp] * 4,
@@ -107,7 +107,7 @@ def _ld(x):
 def scale_of(amax: torch.Tensor) -> torch.Tensor:
     """The scale of pages with these largest values."""
     m, e = torch.frexp(amax.float())                           # amax = m 2^e, m in [1/2, 1); 448 = 7/8 2^9
-    e = torch.where(m > 0.875, e - 8, e - 9).clamp(MIN_EXP, 120)
+    e = torch.where(m == 0, MIN_EXP, torch.where(m > 0.875, e - 8, e - 9)).clamp(MIN_EXP, 120)
     return torch.where(torch.isfinite(amax), torch.ldexp(torch.ones_like(m), e), torch.nan)
 
 
@@ -123,6 +123,20 @@ def _write(x, codes, scales, page, slot):
     y = (x.transpose(0, 1) / new.view(-1, 1, 1)).to(codes.dtype).view(torch.uint8)
     raw[page, :, slot:slot + x.shape[0]] = torch.where(torch.isnan(new).view(-1, 1, 1), torch.zeros_like(y), y)
     scales[page] = new
+
+
+def _write_tokens(k, v, pages: Fp8Pages, ids, start: int):
+    at, last = start, start + k.shape[0]
+    while at < last:
+        end = min(last, (at // PAGE + 1) * PAGE)
+        for src, codes, scales in ((k, pages.k, pages.k_scale), (v, pages.v, pages.v_scale)):
+            _write(src[at - start:end - start], codes, scales, ids[at // PAGE], at % PAGE)
+        at = end
+
+
+def _pool_args(pages: Fp8Pages, page_table):
+    return (pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), pages.k.shape[0], page_table.data_ptr(),
+            *page_table.shape)
 
 
 def _places(new: NewTokens, page_table, pages: int, T: int):
@@ -177,12 +191,7 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
             part = x[t0:t0 + m]
             q_out[t0:t0 + m] = _head_norm_rope(part[:, :heads], q_weight, eps, c, s).reshape(m, -1).to(qkv.dtype)
             k, v = _head_norm_rope(part[:, heads:heads + G], k_weight, eps, c, s), part[:, heads + G:]
-            at = start
-            while at < start + m:
-                end = min(start + m, (at // PAGE + 1) * PAGE)
-                for src, codes, scales in ((k, pages.k, pages.k_scale), (v, pages.v, pages.v_scale)):
-                    _write(src[at - start:end - start], codes, scales, ids[at // PAGE], at % PAGE)
-                at = end
+            _write_tokens(k, v, pages, ids, start)
         return q_out
     if rot % 16:
         raise ValueError(f"{rot} rotated values: a multiple of 16 on a GPU")
@@ -191,18 +200,36 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
     if T == 0 or n == 0:
         return q_out
     qkv = _aligned(qkv)
-    if q_weight is not None:
-        q_weight, k_weight = (w if w.is_contiguous() and w.data_ptr() % 16 == 0 else w.clone(memory_format=torch.contiguous_format)
-                              for w in (q_weight, k_weight))
+    q_weight, k_weight = _weights16(q_weight, k_weight)
     if rot:
         cos, sin = cos.contiguous(), sin.contiguous()
+    at, size, ld = qkv.data_ptr(), D * qkv.element_size(), _ld(qkv)
     with rt.device_of(qkv):
-        rt.check(rt.lib().inv_fp8_append(qkv.data_ptr(), _ld(qkv), q_out.data_ptr(), _ld(q_out), heads, G, D, rt.ptr(q_weight), rt.ptr(k_weight),
-                                         float(eps), rt.ptr(cos), rt.ptr(sin), cos.shape[0] if rot else 0, rot, rt.ptr(positions), pages.k.data_ptr(),
-                                         pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), N, page_table.data_ptr(),
-                                         page_table.shape[0], page_table.shape[1], new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
-                                         rt.status_tensor(qkv.device).data_ptr(), rt.stream_ptr()), "inv_fp8_append")
+        rt.check(rt.lib().inv_fp8_append(at, at + heads * size, ld, at + (heads + G) * size, ld, q_out.data_ptr(), _ld(q_out), heads, G, D,
+                                         rt.ptr(q_weight), rt.ptr(k_weight), float(eps), rt.ptr(cos), rt.ptr(sin), cos.shape[0] if rot else 0, rot,
+                                         rt.ptr(positions), *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(),
+                                         new.start.data_ptr(), n, T, rt.status_tensor(qkv.device).data_ptr(), rt.stream_ptr()), "inv_fp8_append")
     return q_out
+
+
+def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens):
+    """Keys and values [T, kv_heads * dim] of packed tokens, as they are, into the pages: ``qkv_append`` for heads that were normed and rotated before."""
+    N, G, D = _check(k, "k", 1 if pages.k.dim() != 4 else pages.k.shape[1], pages, page_table)
+    T = k.shape[0]
+    if k.shape[1] != G * D or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or v.stride(1) != 1:
+        raise ValueError(f"k of {k.dtype} {tuple(k.shape)}, v of {v.dtype} {tuple(v.shape)} for {G} heads of {D}")
+    n = _check_new(new, k.device)
+    if not k.is_cuda:
+        for t0, m, start, ids in _places(new, page_table, N, T):
+            _write_tokens(k[t0:t0 + m].float().view(m, G, D), v[t0:t0 + m].float().view(m, G, D), pages, ids, start)
+        return
+    if T == 0 or n == 0:
+        return
+    k, v = _aligned(k), _aligned(v)
+    with rt.device_of(k):
+        rt.check(rt.lib().inv_fp8_append(0, k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), 0, 0, 0, G, D, 0, 0, 0.0, 0, 0, 0, 0, 0,
+                                         *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
+                                         rt.status_tensor(k.device).data_ptr(), rt.stream_ptr()), "inv_fp8_append")
 
 
 def read(pages: Fp8Pages, ids: torch.Tensor, length: int):
@@ -220,8 +247,9 @@ def _softmax_rows(q, k, v, scale, seen):
     s = torch.einsum("tghd,jgd->ghtj", q.float().view(q.shape[0], G, -1, q.shape[2]), k) * scale
     p = torch.softmax(s.masked_fill(~seen, float("-inf")), -1)
     p = torch.where(seen.any(-1, keepdim=True), p, torch.zeros_like(p))
-    v = torch.where(seen.any(0).view(-1, 1, 1), v, torch.zeros_like(v))
-    return torch.einsum("ghtj,jgd->tghd", p, v).reshape(q.shape[0], -1)
+    o = torch.einsum("ghtj,jgd->tghd", p, torch.nan_to_num(v, nan=0.0, posinf=0.0, neginf=0.0))
+    lost = torch.einsum("tj,jgd->tgd", seen.float(), (~torch.isfinite(v)).float()) > 0        # a hidden value is nothing, whatever it holds
+    return o.masked_fill(lost.unsqueeze(2), float("nan")).reshape(q.shape[0], -1)
 
 
 def _check_out(out, q, width):
@@ -265,9 +293,8 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
     with rt.device_of(q):
         splits = rt.lib().inv_fp8_attend_splits(n, G, heads // G, new.max_new, new.max_len, window)
         part, used = _workspace(T, heads, splits, D, q.device)
-        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, window, pages.k.data_ptr(),
-                                         pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), N, page_table.data_ptr(),
-                                         page_table.shape[0], page_table.shape[1], new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
+        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, window,
+                                         *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
                                          new.max_new, new.max_len, rt.ptr(part), rt.ptr(used), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
                  "inv_fp8_attend")
     return out
@@ -304,9 +331,8 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
     with rt.device_of(q):
         splits = rt.lib().inv_fp8_attend_splits(T, G, heads // G, 1, max_len, 0)
         part, used = _workspace(T, heads, splits, D, q.device)
-        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, pages.k.data_ptr(), pages.v.data_ptr(),
-                                              pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), N, page_table.data_ptr(), page_table.shape[0],
-                                              page_table.shape[1], row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
+        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, *_pool_args(pages, page_table),
+                                              row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
                                               max_len, rt.ptr(part), rt.ptr(used), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
                  "inv_fp8_attend_tree")
     return out

@@ -163,6 +163,9 @@ class TPDecoder:
 
     def __init__(self, cfg: TransformerConfig, group=None, fmt: str = "oil4", max_batch: int = 64, max_seq: int = 1024, seed: int = 0,
                  kv_format: str = "oil4", device=None, single: bool = False):
+        if cfg.qk_norm or kv_format not in ("oil4", "bf16"):
+            raise NotImplementedError(f"a tensor-parallel decoder has no norms of query and key heads and caches in oil4 or bf16 (qk_norm {cfg.qk_norm}, "
+                                      f"kv_format {kv_format!r})")
         self.cfg = cfg
         self.dev = device or torch.device("cuda", torch.cuda.current_device())
         multi = dist.is_initialized() and not single  # single=True: the whole model on this GPU (reference for tests)

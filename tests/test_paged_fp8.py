@@ -1,0 +1,576 @@
+"""Paged cache of 8-bit keys and values: append with norms and rotation on the way and attention over the pages, against the formulas in 64 bits; refusals;
+what is left alone; runs of them together, up to a decoder's generation."""
+import pytest
+import torch
+
+from innova_b200 import ops
+from innova_b200.inference.generator import Generator
+from innova_b200.inference.kv_cache import PagedKVCache
+from innova_b200.inference.sampler import SamplingParams
+from innova_b200.models import DenseModel, TransformerConfig
+from innova_b200.ops import paged_fp8 as pf
+from innova_b200.ops import runtime as rt
+
+GPU = pytest.param("cuda", marks=pytest.mark.gpu)
+DEVS = ["cpu", GPU]
+EPS = 1e-6
+
+
+def dtype_of(dev):
+    return torch.float32 if dev == "cpu" else torch.bfloat16
+
+
+def i32(x, dev):
+    return torch.tensor(x, dtype=torch.int32, device=dev)
+
+
+class Setup:
+    """Sequences of given lengths in shuffled pages. Codes and scales that no sequence owns are NaN, as are the slots behind each sequence's end."""
+
+    def __init__(self, ctx, new, H, G, D, dev, seed=0, spread=4.0):
+        g = torch.Generator().manual_seed(seed)
+        self.ctx, self.new, self.H, self.G, self.D, self.dev, self.n = ctx, new, H, G, D, dev, len(ctx)
+        need = [-(-(a + b) // 16) for a, b in zip(ctx, new)]
+        rows = self.n + 2
+        self.pages = sum(need) + 3
+        order = torch.randperm(self.pages, generator=g).tolist()
+        self.owner = torch.randperm(rows, generator=g)[: self.n].tolist()              # page table row of each sequence
+        table = torch.full((rows, max([1, *need]) + 1), -7, dtype=torch.int32)         # entries that nothing may read
+        self.ids, at = [], 0
+        for r, m in zip(self.owner, need):
+            self.ids.append(order[at:at + m])
+            table[r, :m] = torch.tensor(order[at:at + m], dtype=torch.int32)
+            at += m
+        self.page_table = table.to(dev)
+        codes = [torch.full((self.pages, G, 16, D), 0x7f, dtype=torch.uint8) for _ in "kv"]
+        scales = [torch.full((self.pages, G), float("nan")) for _ in "kv"]
+        self.filled = torch.zeros(self.pages, 16, dtype=torch.bool)
+        for ids, n in zip(self.ids, [a + (b if seed >= 0 else 0) for a, b in zip(ctx, new)]):
+            for j, p in enumerate(ids):
+                m = min(16, n - 16 * j)
+                if m <= 0:
+                    break
+                x = torch.randn(2, G, m, D, generator=g) * torch.exp(spread * torch.rand(2, G, 1, 1, generator=g) - spread / 2)
+                for c, s, v in zip(codes, scales, x):
+                    s[p] = pf.scale_of(v.abs().amax((1, 2)))
+                    c[p, :, :m] = (v / s[p].view(-1, 1, 1)).to(torch.float8_e4m3fn).view(torch.uint8)
+                self.filled[p, :m] = True
+        self.pool = pf.Fp8Pages(*(c.view(torch.float8_e4m3fn).to(dev) for c in codes), *(s.to(dev) for s in scales))
+        cu = [sum(new[:i]) for i in range(self.n + 1)]
+        self.T = cu[-1]
+        self.tokens = pf.NewTokens(i32(self.owner, dev), i32(cu, dev), i32(ctx, dev), max([1, *new]), max([1, *(a + b for a, b in zip(ctx, new))]))
+        self.cu, self.g = cu, g
+
+    def q(self):
+        x = torch.randn(self.T, self.H * self.D, generator=self.g)
+        return (x * torch.exp(3 * torch.rand(self.T, 1, generator=self.g) - 2)).to(dtype_of(self.dev)).to(self.dev)
+
+    def values(self, i, n):
+        """Keys and values of sequence i's first n tokens in 64 bits."""
+        out = []
+        for c, s in zip(self.pool[:2], self.pool[2:]):
+            ids = torch.tensor(self.ids[i], dtype=torch.long)
+            x = c.cpu()[ids].double() * s.cpu()[ids].double()[..., None, None]
+            out.append(x.transpose(1, 2).reshape(-1, self.G, self.D)[:n])
+        return out
+
+
+def attention(q, k, v, seen, scale):
+    """q [H, D], k and v [n, G, D] in 64 bits, seen [n] -> (o, sum of weights times |v|), both [H, D]."""
+    G = k.shape[1]
+    k, v = k[seen], v[seen]
+    if not len(k):
+        return torch.zeros_like(q), torch.zeros_like(q)
+    s = torch.einsum("ghd,jgd->ghj", q.view(G, -1, q.shape[1]), k) * scale
+    p = torch.softmax(s, -1)
+    return (torch.einsum("ghj,jgd->ghd", p, x).reshape(q.shape) for x in (v, v.abs()))
+
+
+def close_attention(got, o, size, dtype):
+    """Weights are rounded to fp16 (2^-11), their scores are off by under 2^-12 of an exponent, the exponential by 2^-21: 2^-9 of the sum of weighted sizes,
+    and one rounding to the type."""
+    bound = torch.finfo(dtype).eps / 2 * o.abs() + 2.0 ** -9 * size
+    assert bool(((got.double() - o).abs() <= bound).all()), float(((got.double() - o).abs() / (bound + 1e-300)).max())
+
+
+def check_attend(s, window=0, q=None, out=None):
+    q = s.q() if q is None else q
+    got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H, s.D ** -0.5, window, out).cpu()
+    for i, (a, b) in enumerate(zip(s.ctx, s.new)):
+        k, v = s.values(i, a + b)
+        j = torch.arange(a + b)
+        for t in range(b) if b < 40 else [*range(0, b, max(1, b // 13)), b - 1]:
+            seen = (j <= a + t) & (j > a + t - window) if window else j <= a + t
+            o, size = attention(q[s.cu[i] + t].cpu().double().view(s.H, s.D), k, v, seen, s.D ** -0.5)
+            close_attention(got[s.cu[i] + t].view(s.H, s.D), o, size, q.dtype)
+    return got
+
+
+ATTEND = [
+    # cached, new, query heads, key heads, dim, window
+    ([0], [1], 1, 1, 64, 0),
+    ([0, 15, 16, 17, 31], [1, 1, 1, 1, 1], 4, 2, 64, 0),
+    ([3, 0, 40, 700], [1, 17, 0, 5], 6, 2, 128, 0),
+    ([500], [1], 8, 8, 64, 0),
+    ([1, 900, 33], [3, 1, 2], 32, 2, 128, 0),
+    ([0, 7], [40, 33], 3, 1, 64, 0),
+    ([5000, 12], [1, 1], 8, 2, 128, 0),
+    ([2100, 0, 4999], [1, 1, 2], 5, 1, 64, 0),
+    ([300, 5, 0], [1, 9, 20], 4, 2, 128, 16),
+    ([2000, 64], [5, 1], 4, 1, 64, 1),
+    ([3000, 100], [1, 30], 8, 4, 64, 1000),
+    ([129], [150], 4, 1, 128, 0),
+    ([0, 300, 45], [300, 131, 1], 8, 2, 64, 100),
+    ([1000, 0], [257, 3], 16, 4, 128, 0),
+]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("case", ATTEND)
+def test_attend_matches_the_formula(case, dev):
+    ctx, new, H, G, D, window = case
+    check_attend(Setup(ctx, new, H, G, D, dev), window)
+    if dev == "cuda":
+        rt.check_status()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_attend_strides(dev):
+    s = Setup([20, 3], [2, 1], 4, 2, 64, dev)
+    q = s.q()
+    want = check_attend(s, q=q)
+    for off in (0, 8, 3):                                # a projection's columns; off 16 bytes
+        wide = torch.zeros(s.T, 4 * 64 + 24, dtype=q.dtype, device=dev)
+        wide[:, off:off + 256] = q
+        res = torch.full((s.T, 300), 7.0, dtype=q.dtype, device=dev)
+        got = pf.kv_attend(wide[:, off:off + 256], s.pool, s.page_table, s.tokens, 4, out=res[:, off:off + 256])
+        assert torch.equal(got.cpu(), want) and bool((res[:, :off] == 7).all()) and bool((res[:, off + 256:] == 7).all())
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_attend_values_that_are_no_numbers(dev):
+    """A page of NaN poisons the rows that see it, and no others; so does a query of its row."""
+    s = Setup([100, 40], [30, 2], 4, 2, 64, dev)
+    q = s.q()
+    clean = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 4).cpu()
+    s.pool.v_scale[s.ids[0][7], 1] = float("nan")                                     # positions 112 to 127 of sequence 0, key head 1
+    got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 4).cpu()
+    assert bool(got[12:30, 128:].isnan().all())                                        # positions 112 and on
+    assert torch.equal(got[:12], clean[:12]) and torch.equal(got[12:, :128], clean[12:, :128]) and torch.equal(got[30:], clean[30:])
+    windowed = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 4, window=2).cpu()
+    assert not bool(windowed[29:].isnan().any()) and bool(windowed[13, 128:].isnan().all())      # 128 sees 127 and is lost, 129 is not
+    s.pool.v_scale[s.ids[0][7], 1] = 1.0
+    s.pool.k_scale[s.ids[1][0], 0] = float("nan")
+    q[3] = float("nan")
+    got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 4).cpu()
+    assert bool(got[3].isnan().all()) and torch.equal(got[:3], clean[:3]) and torch.equal(got[4:12], clean[4:12])
+    assert bool(got[30:, :128].isnan().all()) and torch.equal(got[30:, 128:], clean[30:, 128:])
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_attend_extreme_values(dev):
+    """Queries and pages far from one: no overflow where the result is finite, and large scores pick their key."""
+    s = Setup([200], [2], 2, 1, 64, dev, spread=40.0)                                # page scales over 2^-29 ... 2^29
+    check_attend(s, q=(s.q().float() * 2.0 ** -30).to(dtype_of(dev)))
+    s = Setup([50], [1], 2, 1, 64, dev)
+    q = s.q()
+    q.zero_()
+    check_attend(s, q=q)                                                              # equal weights
+    s.pool.k_scale.nan_to_num_().mul_(2.0 ** 40)
+    q.fill_(2.0 ** -40)
+    check_attend(s, q=q)
+
+
+TREE = [([30, 5, 0], 4, 2, 64, [0, 0, 1, 2, 1, 0]), ([3000, 17], 8, 1, 128, [1, 0, 0])]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("case", TREE)
+def test_tree_rows(case, dev):
+    lens, H, G, D, row_seq = case
+    s = Setup(lens, [0] * len(lens), H, G, D, dev)
+    T = len(row_seq)
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(T, H * D + 40, generator=g).to(dtype_of(dev)).to(dev)[:, : H * D]
+    seq_lens = torch.zeros(s.page_table.shape[0], dtype=torch.int32)
+    for r, n in zip(s.owner, lens):
+        seq_lens[r] = n
+    tail = [max(0, lens[i] - 9) for i in row_seq]
+    mask = [int(torch.randint(0, 2 ** 62, (1,), generator=g)) for _ in row_seq]
+    mask[0] = 0
+    mask[-1] = -1                                                                     # all 64 bits
+    if lens[row_seq[1]] <= 64:
+        tail[1], mask[1] = 0, 0                                                       # sees nothing
+    rows = i32([s.owner[i] for i in row_seq], dev)
+    args = (q, s.pool, s.page_table, seq_lens.to(dev), rows, H, max(lens))
+    for with_tail in (False, True):
+        more = dict(tail_start=i32(tail, dev), tail_mask=torch.tensor(mask, dtype=torch.int64, device=dev)) if with_tail else {}
+        got = pf.tree_attend(*args, **more).cpu()
+        for t, i in enumerate(row_seq):
+            k, v = s.values(i, lens[i])
+            j = torch.arange(lens[i])
+            seen = torch.ones(lens[i], dtype=torch.bool)
+            if with_tail:
+                bits = torch.tensor([(mask[t] >> b) & 1 for b in range(64)] + [0], dtype=torch.bool)
+                seen = (j < tail[t]) | bits[(j - tail[t]).clamp(0, 64)]
+            o, size = attention(q[t].cpu().double().view(H, D), k, v, seen, D ** -0.5)
+            close_attention(got[t].view(H, D), o, size, q.dtype)
+
+
+# ---------------------------------------------------------------------------------------------- append
+def heads64(x, w, pos, cos, sin):
+    x = x.double()
+    if w is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS) * w.cpu().double()
+    if cos is None:
+        return x
+    n = cos.shape[1]
+    c, s = cos.cpu().double()[pos].unsqueeze(1), sin.cpu().double()[pos].unsqueeze(1)
+    a, b = x[..., :n], x[..., n:2 * n]
+    return torch.cat([a * c - b * s, a * s + b * c, x[..., 2 * n:]], -1)
+
+
+def check_append(ctx, new, H, G, D, dev, rot, norm, positions=False, seed=0):
+    s = Setup(ctx, [0] * len(ctx), H, G, D, dev, seed)                               # pages that hold the cached tokens only
+    t = Setup(ctx, new, H, G, D, dev, seed)
+    # the same tables as t's, with s's contents where the cached tokens are
+    pool = pf.new_pages(t.pages, G, D, dev)
+    for i, a in enumerate(ctx):
+        for j in range(-(-a // 16)):
+            for x, y in zip(pool, s.pool):
+                x.view(torch.uint8 if x.element_size() == 1 else x.dtype)[t.ids[i][j]] = y.view(torch.uint8 if y.element_size() == 1 else y.dtype)[s.ids[i][j]]
+    before = [x.clone() for x in pool]
+    g = torch.Generator().manual_seed(seed + 1)
+    qkv = (torch.randn(t.T, (H + 2 * G) * D, generator=g) * torch.exp(2 * torch.rand(t.T, 1, generator=g))).to(dtype_of(dev)).to(dev)
+    cos, sin = ops.rope_tables(t.tokens.max_len + 70, rot, device=dev) if rot else (None, None)
+    w = [(1 + 0.3 * torch.randn(D, generator=g)).to(dtype_of(dev)).to(dev) for _ in "qk"] if norm else [None, None]
+    pos = torch.cat([torch.arange(a, a + b) for a, b in zip(ctx, new)])
+    if positions:
+        pos = torch.randint(0, t.tokens.max_len + 70, (t.T,), generator=g)
+    got = pf.qkv_append(qkv, H, G, D, pool, t.page_table, t.tokens, cos, sin, pos.int().to(dev) if positions else None, *w, EPS)
+    x = qkv.cpu().view(t.T, -1, D)
+    q, k, v = heads64(x[:, :H], w[0], pos, cos, sin), heads64(x[:, H:H + G], w[1], pos, cos, sin), x[:, H + G:].double()
+    # fp32 on the way (2^-18 of a head's largest value), one rounding at its end
+    size = q.abs().amax(-1, keepdim=True)
+    err = (got.cpu().double().view_as(q) - q).abs()
+    assert bool((err <= torch.finfo(qkv.dtype).eps / 2 * q.abs() + 2.0 ** -18 * size).all())
+    written = torch.zeros(t.pages, 16, dtype=torch.bool)
+    for i, (a, b) in enumerate(zip(ctx, new)):
+        for j in range(a // 16, -(-(a + b) // 16) if b else 0):
+            p, lo, hi = t.ids[i][j], max(a, 16 * j), min(a + b, 16 * j + 16)
+            written[p, lo - 16 * j:hi - 16 * j] = True
+            for src, codes, scales, was, was_s in ((k, pool.k, pool.k_scale, before[0], before[2]), (v, pool.v, pool.v_scale, before[1], before[3])):
+                part = src[t.cu[i] + lo - a:t.cu[i] + hi - a].transpose(0, 1)            # [G, m, D]
+                amax, sc = part.abs().amax((1, 2)), scales[p].cpu().double()
+                kept = lo - 16 * j
+                old = was_s[p].cpu().double() if kept else torch.zeros(G, dtype=torch.float64)
+                want = torch.maximum(pf.scale_of(amax.float()).double(), old)
+                edge = ((torch.log2(amax / 448) - torch.log2(amax / 448).round()).abs() < 1e-5) & (src is k)       # either power of two is right
+                assert bool(((sc == want) | edge).all()), (sc, want)
+                m = codes[p].cpu().double()[:, lo - 16 * j:hi - 16 * j] * sc.view(-1, 1, 1)
+                bound = torch.maximum(2.0 ** -4 * part.abs(), 2.0 ** -10 * sc.view(-1, 1, 1)) + 2.0 ** -18 * amax.view(-1, 1, 1)
+                assert bool(((m - part).abs() <= bound).all())
+                if kept:                                                                  # earlier tokens: moved to the new scale
+                    w0, now = was[p].cpu().double()[:, :kept] * old.view(-1, 1, 1), codes[p].cpu().double()[:, :kept] * sc.view(-1, 1, 1)
+                    exact = (w0.abs() >= 2.0 ** -6 * sc.view(-1, 1, 1)) | (sc == old).view(-1, 1, 1)
+                    assert torch.equal(now[exact], w0[exact]) and bool(((now - w0).abs() <= 2.0 ** -10 * sc.view(-1, 1, 1))[~exact].all())
+    for x, y in zip(pool[:2], before[:2]):                       # slots that hold no token of these sequences keep their bytes
+        free = ~written
+        for i, a in enumerate(ctx):
+            for j in range(-(-a // 16)):
+                free[t.ids[i][j], : a - 16 * j] = False
+        keep = free.view(-1, 1, 16, 1).expand(x.shape)
+        assert torch.equal(x.cpu().view(torch.uint8)[keep], y.cpu().view(torch.uint8)[keep])
+    touched = written.any(-1)
+    for x, y in zip(pool[2:], before[2:]):
+        assert torch.equal(x.cpu()[~touched], y.cpu()[~touched])
+
+
+APPEND = [
+    ([0], [1], 1, 1, 64, 64, False),
+    ([15, 16, 17, 0], [1, 1, 1, 1], 4, 2, 128, 128, False),
+    ([5, 0, 40, 31], [1, 40, 0, 18], 6, 2, 64, 64, True),
+    ([333], [200], 8, 1, 128, 32, True),
+    ([7, 100], [30, 3], 3, 3, 64, 0, False),
+    ([9] * 21, [2] * 21, 4, 4, 64, 16, True),
+    ([0] * 300, [1] * 300, 2, 1, 64, 64, False),
+]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("case", APPEND)
+def test_append_matches_the_formula(case, dev):
+    ctx, new, H, G, D, rot, norm = case
+    check_append(ctx, new, H, G, D, dev, rot, norm)
+    check_append(ctx, new, H, G, D, dev, rot, norm, positions=True, seed=5)
+    if dev == "cuda":
+        rt.check_status()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_append_in_portions_reads_the_same(dev):
+    """Scales grow by powers of two, so the portions that a sequence arrives in leave no mark (but on what falls under 2^-6 of a scale, absent here)."""
+    g = torch.Generator().manual_seed(0)
+    T, H, G, D = 77, 4, 2, 64
+    sign = torch.where(torch.rand(T, (H + 2 * G) * D, generator=g) < 0.5, -1.0, 1.0)
+    qkv = (sign * (1 + torch.rand(T, (H + 2 * G) * D, generator=g)) * torch.exp2(torch.randint(0, 7, (T, 1), generator=g).float())).to(dtype_of(dev)).to(dev)
+    table = torch.randperm(6, generator=g).int().view(1, 6).to(dev)
+    pools = []
+    for cuts in ([0, 77], list(range(78)), [0, 5, 6, 30, 48, 77]):
+        pool = pf.new_pages(6, G, D, dev)
+        for a, b in zip(cuts, cuts[1:]):
+            pf.qkv_append(qkv[a:b], H, G, D, pool, table, pf.NewTokens(i32([0], dev), i32([0, b - a], dev), i32([a], dev), b - a, b))
+        pools.append(pool)
+    for other in pools[1:]:
+        for a, b in zip(pools[0], other):
+            assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+    alone = pf.new_pages(6, G, D, dev)
+    pf.kv_append(qkv[:, H * D:(H + G) * D], qkv[:, (H + G) * D:], alone, table, pf.NewTokens(i32([0], dev), i32([0, T], dev), i32([0], dev), T, T))
+    for a, b in zip(pools[0], alone):
+        assert torch.equal(a.view(torch.uint8) if a.element_size() == 1 else a, b.view(torch.uint8) if b.element_size() == 1 else b)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_append_values_at_the_edges(dev):
+    """Zeros, values below the smallest scale, the largest ones, infinities and NaN; a page starts over with its first slot."""
+    D, table = 64, torch.zeros(1, 1, dtype=torch.int32, device=dev)
+    pool = pf.new_pages(1, 1, D, dev)
+
+    def put(at, *values):
+        x = torch.zeros(len(values), D)
+        x[:, 3] = torch.tensor(values)
+        x = x.to(dtype_of(dev)).to(dev)
+        n = len(values)
+        pf.kv_append(x, x, pool, table, pf.NewTokens(i32([0], dev), i32([0, n], dev), i32([at], dev), n, at + n))
+        k, v = pf.read(pool, table[0], at + n)
+        assert torch.equal(k.nan_to_num(nan=-9), v.nan_to_num(nan=-9))
+        return float(pool.k_scale[0, 0]), k[:, 0, 3].tolist()
+    assert put(0, 0.0, 0.0) == (2.0 ** -64, [0.0, 0.0])
+    assert put(0, 2.0 ** -75, 2.0 ** -72) == (2.0 ** -64, [0.0, 2.0 ** -72])
+    assert put(0, 448.0) == (1.0, [448.0])
+    assert put(1, 450.0) == (2.0, [448.0, 448.0])                                     # 450 / 2 rounds to 224; 448 moves with its bits
+    assert put(2, 1.0) == (2.0, [448.0, 448.0, 1.0])
+    top = 2.0 ** 127 * 1.9921875
+    assert put(0, top)[0] == 2.0 ** 120                                                # the largest bf16 value, 255 * 2^120
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        put(0, 5.0)
+        scale, x = put(1, bad, 7.0)
+        assert scale != scale and all(v != v for v in x)
+        scale, x = put(3, 1.0)                                                         # the page stays lost ...
+        assert scale != scale and all(v != v for v in x)
+        raw = pool.k.view(torch.uint8)
+        assert not bool(((raw & 0x7f) == 0x7f).any())                                 # ... by its scale: no code is NaN
+    assert put(0, 3.0) == (2.0 ** -7, [3.0])                                          # ... until it starts over
+
+
+# ---------------------------------------------------------------------------------------------- refusals and bad tables
+@pytest.mark.parametrize("dev", DEVS)
+def test_refusals(dev):
+    s = Setup([5, 20], [2, 1], 4, 2, 64, dev)
+    q = s.q()
+    ok = dict(q=q, pages=s.pool, page_table=s.page_table, new=s.tokens, heads=4)
+    pf.kv_attend(**ok)
+    P, N = s.pool, s.tokens
+    for bad in (dict(q=q[:, :100]), dict(q=q.view(3, 4, 64)), dict(q=q.t()), dict(heads=3), dict(heads=8), dict(heads=0), dict(window=-1),
+                dict(page_table=s.page_table.long()), dict(page_table=s.page_table.t()), dict(page_table=s.page_table[0]),
+                dict(pages=P._replace(k=P.k.view(torch.uint8))), dict(pages=P._replace(k=P.k[1:])), dict(pages=P._replace(k_scale=P.k_scale[:, :1])),
+                dict(pages=P._replace(v_scale=P.v_scale.double())), dict(pages=P._replace(v=P.v.transpose(2, 3))),
+                dict(pages=pf.Fp8Pages(P.k[:, :, :8], P.v[:, :, :8], P.k_scale, P.v_scale)), dict(new=N._replace(cu=N.cu[:2])),
+                dict(new=N._replace(start=N.start.long())), dict(new=N._replace(max_new=0)), dict(new=N._replace(max_len=1)),
+                dict(out=q[:, :128]), dict(out=q[:2]), dict(out=q.double())):
+        with pytest.raises((ValueError, TypeError)):
+            pf.kv_attend(**{**ok, **bad})
+    qkv = torch.randn(3, 8 * 64, device=dev).to(q.dtype)
+    cos, sin = ops.rope_tables(40, 64, device=dev)
+    w = torch.ones(64, dtype=q.dtype, device=dev)
+    ok = dict(qkv=qkv, heads=4, kv_heads=2, dim=64, pages=s.pool, page_table=s.page_table, new=s.tokens, cos=cos, sin=sin)
+    pf.qkv_append(**ok)
+    for bad in (dict(qkv=qkv[:, 64:]), dict(kv_heads=4), dict(dim=128), dict(q_weight=w), dict(q_weight=w[:32], k_weight=w),
+                dict(q_weight=w.double(), k_weight=w.double()), dict(sin=None), dict(cos=cos[:, :20]), dict(q_out=q[:, :128]),
+                dict(cos=torch.ones(40, 40, device=dev), sin=torch.ones(40, 40, device=dev)), dict(positions=torch.zeros(3, device=dev, dtype=torch.int64)),
+                dict(positions=torch.zeros(2, device=dev, dtype=torch.int32))):
+        with pytest.raises((ValueError, TypeError)):
+            pf.qkv_append(**{**ok, **bad})
+    k = qkv[:, :128]
+    for args in ((k, k[:, :64]), (k, k.double()), (k[:, :64], k[:, :64])):
+        with pytest.raises((ValueError, TypeError)):
+            pf.kv_append(*args, s.pool, s.page_table, s.tokens)
+    lens = torch.zeros(s.page_table.shape[0], dtype=torch.int32, device=dev)
+    rows = i32([0, 0, 0], dev)
+    for bad in (dict(max_len=0), dict(row_seq=rows[:2]), dict(seq_lens=lens[:1]), dict(tail_start=rows), dict(row_seq=rows.long())):
+        with pytest.raises((ValueError, TypeError)):
+            pf.tree_attend(**{**dict(q=q, pages=s.pool, page_table=s.page_table, seq_lens=lens, row_seq=rows, heads=4, max_len=9), **bad})
+    if dev == "cuda":
+        for bad in (dict(q=q.half()), dict(q=q.float()), dict(q=q.cpu()), dict(page_table=s.page_table.cpu())):
+            with pytest.raises((ValueError, TypeError)):
+                pf.kv_attend(**{**dict(q=q, pages=s.pool, page_table=s.page_table, new=s.tokens, heads=4), **bad})
+        small = pf.new_pages(4, 2, 32, dev)
+        with pytest.raises(ValueError):
+            pf.kv_attend(q[:, :128], small, s.page_table, s.tokens, 4)
+        with pytest.raises(ValueError):
+            PagedKVCache(1, 2, 32, 1, 64, dev, "fp8")
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_entries_outside_the_pool(dev):
+    """Pages, rows and positions that point outside: an error on the CPU; on the GPU nothing outside is touched, what is right is done, and the status word
+    says so."""
+    for what in ("page", "row", "start"):
+        s = Setup([40, 33], [1, 2], 4, 2, 64, dev)
+        q, new, table = s.q(), s.tokens, s.page_table.clone()
+        want = pf.kv_attend(q, s.pool, s.page_table, new, 4)
+        if what == "page":
+            table[s.owner[0], 1] = s.pages
+        elif what == "row":
+            new = new._replace(rows=i32([table.shape[0], s.owner[1]], dev))
+        else:
+            new = new._replace(start=i32([-1, 33], dev))
+        qkv = torch.randn(3, 8 * 64, device=dev).to(q.dtype)
+        if dev == "cpu":
+            with pytest.raises(ValueError):
+                pf.kv_attend(q, s.pool, table, new, 4)
+            with pytest.raises(ValueError):
+                pf.qkv_append(qkv, 4, 2, 64, s.pool, table, new)
+            continue
+        got = pf.kv_attend(q, s.pool, table, new, 4)
+        with pytest.raises(RuntimeError):
+            rt.check_status()
+        assert torch.equal(got[1:], want[1:])
+        if what == "page":
+            table = s.page_table.clone()
+            table[s.owner[0], 2] = -1                                                 # where the new token goes
+        before = [x.clone() for x in s.pool]
+        pf.qkv_append(qkv, 4, 2, 64, s.pool, table, new)
+        with pytest.raises(RuntimeError):
+            rt.check_status()
+        own = torch.zeros(s.pages, dtype=torch.bool)
+        own[s.ids[1]] = True
+        for x, y in zip(s.pool, before):
+            codes = x.element_size() == 1
+            x, y = (z.cpu().view(torch.uint8 if codes else torch.int32) for z in (x, y))
+            assert torch.equal(x[~own], y[~own]) and not (codes and torch.equal(x[own], y[own]))
+
+
+@pytest.mark.gpu
+def test_gpu_more_tokens_than_the_bounds_say():
+    """Sequences longer than max_len are still read whole; more new tokens than max_new are reported."""
+    s = Setup([5000], [1], 8, 1, 64, "cuda")
+    q = s.q()
+    want = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 8)
+    for n in (1, 40, 3000):
+        got = pf.kv_attend(q, s.pool, s.page_table, s.tokens._replace(max_len=n), 8)
+        assert torch.allclose(got.float(), want.float(), rtol=2.0 ** -7, atol=1e-2)
+    rt.check_status()
+    s = Setup([50], [40], 8, 1, 64, "cuda")
+    pf.kv_attend(s.q(), s.pool, s.page_table, s.tokens._replace(max_new=3), 8)
+    with pytest.raises(RuntimeError):
+        rt.check_status()
+
+
+# ---------------------------------------------------------------------------------------------- streams, graphs, runs together
+def decode_step(s, qkv, cos, sin):
+    q = pf.qkv_append(qkv, s.H, s.G, s.D, s.pool, s.page_table, s.tokens, cos, sin)
+    return pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H)
+
+
+@pytest.mark.gpu
+def test_gpu_two_captured_steps_share_nothing():
+    """Graphs of two batches, split over many CTAs, replayed in turn and at once, with lengths that grew since the capture."""
+    dev, steps = "cuda", []
+    for seed, ctx in ((0, [4000, 100]), (1, [3000, 5])):
+        s = Setup([c + 64 for c in ctx], [1, 1], 8, 2, 64, dev, seed)                 # pages for 64 more tokens
+        s.tokens = s.tokens._replace(start=i32(ctx, dev))
+        s.pool.k_scale.nan_to_num_(1.0)
+        s.pool.v_scale.nan_to_num_(1.0)
+        qkv = torch.randn(2, 12 * 64, device=dev).bfloat16()
+        cos, sin = ops.rope_tables(5000, 64, device=dev)
+        decode_step(s, qkv, cos, sin)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = decode_step(s, qkv, cos, sin)
+        steps.append((s, qkv, cos, sin, graph, out))
+    for n in range(3):
+        for s, qkv, *_ in steps:
+            s.tokens.start.add_(1)
+            qkv.normal_()
+        streams = [torch.cuda.Stream() for _ in steps]
+        for st, (s, qkv, cos, sin, graph, out) in zip(streams, steps):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        got = [out.clone() for *_, out in steps]
+        for g, (s, qkv, cos, sin, *_) in zip(got, steps):
+            assert torch.equal(g, decode_step(s, qkv, cos, sin))                      # the append writes the same again
+    rt.check_status()
+
+
+def tiny(**kw):
+    return TransformerConfig(**{**dict(vocab_size=300, hidden_size=256, num_layers=2, num_heads=4, head_dim=64, ffn_hidden_size=256, num_kv_heads=2,
+                                       max_seq_len=512, qk_norm=True, vocab_pad_to=8), **kw})
+
+
+def full_logits(model, ids):
+    with torch.no_grad():
+        return model(ids)[:, -1].float()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("kw", [{}, dict(qk_norm=False), dict(positions="learned", bias=True, norm="layernorm", activation="gelu")])
+def test_generator_over_an_fp8_cache(kw, dev):
+    """Prompt, single tokens, a chain of drafts and a longer portion, sequence by sequence and row by row, against the whole model."""
+    torch.manual_seed(0)
+    m = DenseModel(tiny(**kw), dtype=dtype_of(dev), device=dev).eval()
+    with torch.no_grad():
+        for p in m.parameters():
+            p.mul_(3.0 if p.dim() == 2 else 1.0)                                    # logits that depend on the context
+    gen = Generator(m, kv_format="fp8", max_batch=3, max_seq=400)
+    ids = torch.randint(0, 300, (2, 260), device=dev)
+    at = 0
+    for n in (37, 1, 1, 5, 100, 64, 1):
+        logits = gen._forward(ids[:, at:at + n], [at, at])
+        at += n
+        want = full_logits(m, ids[:, :at])
+        # keys and values in e4m3 are off by up to 2^-4 of their size (3.6 % as a rule); what attention adds to the stream carries that, averaged over keys
+        assert float((logits.float() - want).norm() / want.norm()) < 0.06
+    if dev == "cuda":
+        rt.check_status()
+    tree = gen._forward_tree([5, 6, 7], [-1, 0, 0], at, row=0)
+    gen.cache.truncate(0, at)
+    for t, path in enumerate(([5], [5, 6], [5, 7])):
+        want = full_logits(m, torch.cat([ids[:1, :at], torch.tensor([path], device=dev)], 1))
+        assert float((tree[t].float() - want[0]).norm() / want.norm()) < 0.06
+    out = Generator(m, kv_format="fp8", max_batch=2).generate_tokens(ids[:, :30], 8, SamplingParams())
+    assert len(out) == 2 and all(len(o) == 8 for o in out)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_continuous_batching_over_an_fp8_cache(dev):
+    from innova_b200.inference.serving import ContinuousBatching, Request
+    torch.manual_seed(0)
+    m = DenseModel(tiny(num_layers=1), dtype=dtype_of(dev), device=dev).eval()
+    cb = ContinuousBatching(Generator(m, kv_format="fp8", max_batch=2, max_seq=128))
+    prompts = [[1, 2, 3], list(range(40)), [7] * 17]
+    for i, p in enumerate(prompts):
+        cb.add_request(Request(id=i, tokens=p, max_tokens=5))
+    for _ in range(30):
+        if not cb.step() and not cb.sched.pending_count():
+            break
+    alone = Generator(m, kv_format="fp8", max_batch=1, max_seq=128)
+    for i, p in enumerate(prompts):
+        assert cb.finished[i] == alone.generate_tokens([p], 5)[0]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_cache_steps_refuse_what_is_outside(dev):
+    c = PagedKVCache(1, 2, 64, 3, 64, dev, "fp8")
+    c.reserve(0, 20)
+    c.reserve(2, 5)
+    c.new_tokens([2, 0], [0, 16], [5, 4])
+    for args in (([0, 0], [0, 0], [1, 1]), ([3], [0], [1]), ([0], [33], [1]), ([0], [-1], [1]), ([1], [0], [1]), ([0], [0, 1], [1])):
+        with pytest.raises(ValueError):
+            c.new_tokens(*args)
+    with pytest.raises(NotImplementedError):
+        PagedKVCache(1, 2, 64, 1, 64, dev, "bf16").new_tokens([0], [0], [1])
+    assert c.bytes_per_token() == 2 * 2 * (64 * 16 + 4) // 16
