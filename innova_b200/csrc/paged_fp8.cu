@@ -12,6 +12,8 @@
 
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 namespace inv {
 
 constexpr int FP8_PAGE = 16;
@@ -210,7 +212,7 @@ struct Fp8Attend {
   float scale;
   int per_split;        // pages of a CTA
   int splits, tiles;
-  float* part;          // splits > 1: [T, H, splits, D + 2] (maximum, sum, values)
+  float *part, *part_ml;  // splits > 1: [T, H, splits, D] values, [T, H, splits, 2] maximum and sum
   int* used;            // splits > 1: [T, H] splits that a row has
   // Rows of a token tree (or null): row t is of table row row_seq[t], which holds seq_lens[.] tokens, and sees those below tail_start[t] and of the 64
   // from there on the ones whose bit is set.
@@ -218,16 +220,12 @@ struct Fp8Attend {
   const unsigned long long* tail_mask;
 };
 
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 load_stream2(const void* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -244,36 +242,24 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// A lane's codes of one page: of the keys, tokens 4 (n / 2) + n % 2 and that + 2 (n = lane / 4), dimensions 64 j + 16 c on (c = lane % 4);
-// of the values, tokens 4 c to 4 c + 3, dimensions n D / 8 on.
+// Where the codes of a page lie in a warp's ring, and which of them a lane takes. In shared memory a page's keys (and values) are lines of 128 bytes whose
+// 16-byte pieces are exchanged by the line's number, so that the eight lanes of a read meet all banks. n = lane / 4, c = lane % 4. Column n of block j of
+// a score product is token slot(j, n); a lane's scores are those of columns 2 c and 2 c + 1 of both blocks, and its values those four tokens'. Column n of
+// block b of the value product is dimension col(n) + b.
 template <int D>
-struct PageCodes {
-  static constexpr int KP = D / 64, VW = D / 32;
-  uint4 k[2][KP];
-  uint32_t v[4][VW];
-  __device__ __forceinline__ void load(const Fp8Pool& pool, int id, int hk, int lane) {
-    const int n = lane >> 2, c = lane & 3;
-    const long base = ((long)id * pool.Hkv + hk) * FP8_PAGE * D;
-    const uint8_t* kp = pool.k + base + (4 * (n >> 1) + (n & 1)) * D + c * 16;
-    const uint8_t* vp = pool.v + base + 4 * c * D + n * (D / 8);
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int i = 0; i < KP; ++i) k[j][i] = load_stream(kp + 2 * j * D + i * 64);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      if (D == 128) {
-        const uint4 w = load_stream(vp + r * D);
-        v[r][0] = w.x; v[r][1] = w.y; v[r][VW - 2] = w.z; v[r][VW - 1] = w.w;
-      } else {
-        const uint2 w = load_stream2(vp + r * D);
-        v[r][0] = w.x; v[r][1] = w.y;
-      }
-    }
+struct PageMap {
+  static constexpr int KP = D / 64, VW = D / 32, BYTES = 2 * FP8_PAGE * D;
+  static __device__ __forceinline__ int at(int byte) {                            // of 16 * D, a multiple of 8
+    const int line = byte >> 7;
+    return (line << 7) + ((((byte >> 4) ^ line) & 7) << 4) + (byte & 15);
   }
+  static __device__ __forceinline__ int slot(int j, int n) { return D == 128 ? (n >> 1) + 4 * (n & 1) + 8 * j : n + 8 * j; }
+  static __device__ __forceinline__ int col(int n) { return D == 128 ? ((n >> 1) + 4 * (n & 1)) * 16 : n * 8; }
 };
 
-// Sixteen rows (query tokens times the heads that share a key head) against a run of pages: grid = sequences x key heads x splits x row tiles, four warps
+constexpr int FP8_STAGES = 4;
+
+// Sixteen rows (query tokens times the heads that share a key head) against a run of pages: grid = sequences x key heads x splits x row tiles, NW warps
 // that take a page in turn, each with a softmax of its own; they join at the end.
 //
 // Scores and values are products on m16n8k16 tensor instructions in fp16: a code is exact there, and so is a query up to 2^-24 of its row's largest value
@@ -282,13 +268,18 @@ struct PageCodes {
 // whose values it loads. Page scales multiply the scores, and the weights relative to the largest value scale so far, which the sums are kept in.
 // Weights are 2^(s - m + 6) with a maximum that is raised only by scores above m + 8, so at most 2^14, and what fp16 rounds away of a weight is under
 // 2^-30 of the largest one.
-template <int D, bool TREE>
-__global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
-                                                         const __grid_constant__ Fp8Tokens tk) {
-  constexpr int NW = 4, KS = D / 16, NB = D / 8, KP = D / 64, VW = D / 32;
+//
+// Bound by memory. A warp keeps three pages on their way through a ring of its own in shared memory (with one, in registers, 8 contexts of up to 65000
+// tokens, 8 key heads of 128, took 156 us), which takes no registers and no barrier of the CTA.
+template <int D, int NW, bool TREE>
+__global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
+                                                             const __grid_constant__ Fp8Tokens tk) {
+  using M = PageMap<D>;
+  constexpr int KS = D / 16, NB = D / 8, KP = M::KP, VW = M::VW, ST = FP8_STAGES;
   constexpr float LIFT = 6.f, SLACK = 8.f;
+  extern __shared__ __align__(128) uint8_t ring[];               // NW x ST pages; afterwards the warps' sums
   __shared__ float sm_m[NW][16], sm_l[NW][16];
-  __shared__ float sm_o[NW][16][D];
+  release_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   int x = blockIdx.x;
   const int tile = x % a.tiles;
@@ -329,15 +320,33 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
   const int pg_lo = lo / FP8_PAGE, pg_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
   const int p0 = pg_lo + split * a.per_split, p1 = split + 1 < a.splits ? min(pg_hi, p0 + a.per_split) : pg_hi;    // the last one takes the rest
   if (split > 0 && p0 >= p1) return;
-  // visible positions of this lane's two rows: [vlo, vhi)
-  int vlo[2], vhi[2];
+
+  // ---- the warp's pages: its i-th is p0 + warp + NW i ----
+  // A lane keeps the number of one of 32 pages: `nf` of those that are fetched, three pages ahead of `nc` with the scales of those that are worked on; the
+  // next 32 are looked up in between, so that neither look-up is waited for.
+  const int mine = p1 > p0 + warp ? (p1 - p0 - warp + NW - 1) / NW : 0;
+  auto number_of = [&](int i) { return i < mine ? pool_page(tk, pool.pages, row, p0 + warp + NW * i) : -1; };
+  auto scale_at = [&](const float* scales, int id) { return id >= 0 ? scales[(long)id * pool.Hkv + hk] : 0.f; };
+  const uint32_t slots = smem_u32(ring) + warp * ST * M::BYTES;
+  int nf = number_of(lane), nn = -1;
+  auto fetch = [&](int i) {                                       // page i into its slot
+    const int id = __shfl_sync(0xffffffffu, nf, i & 31);
+    if (i < mine && id >= 0) {
+      const long base = ((long)id * pool.Hkv + hk) * FP8_PAGE * D;
+      const uint32_t dst = slots + (i % ST) * M::BYTES;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int p = start + min(r0 + n + 8 * e, rows - 1) / a.G;
-    vhi[e] = TREE ? len : p + 1;
-    vlo[e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
-  }
-  const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;    // positions that every row sees
+      for (int q = 0; q < D / 32; ++q) {
+        const int at = (q * 32 + lane) * 16;
+        copy16_async(dst + M::at(at), pool.k + base + at);
+        copy16_async(dst + FP8_PAGE * D + M::at(at), pool.v + base + at);
+      }
+    }
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) fetch(i);
+  int nc = nf;
+  float ksc = scale_at(pool.k_scale, nc), vsc = scale_at(pool.v_scale, nc), ksn = 0.f, vsn = 0.f;
 
   // ---- queries ----
   uint32_t qa[KS][4];
@@ -372,6 +381,15 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
         qa[j * 4 + i][2 + e] = half2_of(__uint_as_float(w1 << 16) * down, __uint_as_float(w1 & 0xffff0000u) * down);
       }
   }
+  // visible positions of this lane's two rows: [vlo, vhi)
+  int vlo[2], vhi[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int p = start + min(r0 + n + 8 * e, rows - 1) / a.G;
+    vhi[e] = TREE ? len : p + 1;
+    vlo[e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
+  }
+  const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;    // positions that every row sees
 
   float o[NB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f, vinv = 0.f;
 #pragma unroll
@@ -379,37 +397,27 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
 
-  // A lane keeps number and scales of one of the warp's next 32 pages.
-  int ids = -1;
-  float kss = 0.f, vss = 0.f;
-  auto look_up = [&](int pg) {
-    ids = -1;
-    if (pg < p1) {
-      ids = pool_page(tk, pool.pages, row, pg);
-      if (ids >= 0) {
-        kss = pool.k_scale[(long)ids * pool.Hkv + hk];
-        vss = pool.v_scale[(long)ids * pool.Hkv + hk];
-      }
-    }
-  };
-  const int mine = p1 > p0 + warp ? (p1 - p0 - warp + NW - 1) / NW : 0;          // pages of this warp
-  PageCodes<D> next;
-  int id_n = -1;
-  float ks_n = 0.f, vs_n = 0.f;
-  auto fetch = [&](int i) {
-    if ((i & 31) == 0) look_up(p0 + warp + NW * (i + lane));
-    id_n = __shfl_sync(0xffffffffu, ids, i & 31);
-    ks_n = __shfl_sync(0xffffffffu, kss, i & 31);
-    vs_n = __shfl_sync(0xffffffffu, vss, i & 31);
-    if (id_n >= 0) next.load(pool, id_n, hk, lane);
-  };
-  if (mine > 0) fetch(0);
   for (int i = 0; i < mine; ++i) {
-    const PageCodes<D> now = next;
-    const int id = id_n, pos = (p0 + warp + NW * i) * FP8_PAGE;
-    const float ks = ks_n, vs = vs_n;
-    if (i + 1 < mine) fetch(i + 1);
+    if ((i & 31) == 0) {
+      if (i > 0) {
+        nc = nf;
+        ksc = ksn;
+        vsc = vsn;
+      }
+      nn = number_of(i + 32 + lane);
+    }
+    if ((i & 31) == 16) {
+      ksn = scale_at(pool.k_scale, nn);
+      vsn = scale_at(pool.v_scale, nn);
+    }
+    if (((i + ST - 1) & 31) == 0) nf = nn;
+    const int id = __shfl_sync(0xffffffffu, nc, i & 31), pos = (p0 + warp + NW * i) * FP8_PAGE;
+    const float ks = __shfl_sync(0xffffffffu, ksc, i & 31), vs = __shfl_sync(0xffffffffu, vsc, i & 31);
+    copies_wait<ST - 2>();
+    __syncwarp();
+    fetch(i + ST - 1);                               // into the slot of page i - 1, which every lane has read
     if (id < 0) continue;
+    const uint8_t* page = ring + (warp * ST + i % ST) * M::BYTES;
     // ---- scores ----
     float s[2][4];
 #pragma unroll
@@ -418,7 +426,8 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
       for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
 #pragma unroll
       for (int q = 0; q < KP; ++q) {
-        const uint32_t w[4] = {now.k[j][q].x, now.k[j][q].y, now.k[j][q].z, now.k[j][q].w};
+        const uint4 k4 = *reinterpret_cast<const uint4*>(page + M::at(M::slot(j, n) * D + q * 64 + c * 16));
+        const uint32_t w[4] = {k4.x, k4.y, k4.z, k4.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t(&f)[4] = qa[q * 4 + k];
@@ -435,7 +444,7 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
       for (int e = 0; e < 4; ++e) {
         s[j][e] *= e < 2 ? f0 : f1;
         if (!whole) {
-          const int at = pos + 4 * c + 2 * j + (e & 1);
+          const int at = pos + M::slot(j, 2 * c + (e & 1));
           bool seen = at >= vlo[e >> 1] && at < vhi[e >> 1];
           if (TREE) seen = seen && (at < tail || (at - tail < 64 && ((bits >> ((at - tail) & 63)) & 1ull)));
           if (!seen) s[j][e] = -INFINITY;
@@ -483,14 +492,27 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
         pa[2 * j + e] = half2_of(x0, x1);
       }
     // ---- values ----
-    const int keep = hi - pos - 4 * c;                // slots past the end hold whatever was there
+    uint32_t v[4][VW];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int slot = M::slot(r >> 1, 2 * c + (r & 1));
+      const uint8_t* src = page + FP8_PAGE * D + M::at(slot * D + M::col(n));
+      if (D == 128) {
+        const uint4 w = *reinterpret_cast<const uint4*>(src);
+        v[r][0] = w.x; v[r][1] = w.y; v[r][VW - 2] = w.z; v[r][VW - 1] = w.w;
+      } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(src);
+        v[r][0] = w.x; v[r][1] = w.y;
+      }
+      if (!whole && pos + slot >= hi) {               // slots past the end hold whatever was there
+#pragma unroll
+        for (int q = 0; q < VW; ++q) v[r][q] = 0;
+      }
+    }
 #pragma unroll
     for (int q = 0; q < VW; ++q) {
-      uint32_t v[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = whole || r < keep ? now.v[r][q] : 0u;
-      const uint32_t a01 = __byte_perm(v[0], v[1], 0x5140), b01 = __byte_perm(v[0], v[1], 0x7362);
-      const uint32_t a23 = __byte_perm(v[2], v[3], 0x5140), b23 = __byte_perm(v[2], v[3], 0x7362);
+      const uint32_t a01 = __byte_perm(v[0][q], v[1][q], 0x5140), b01 = __byte_perm(v[0][q], v[1][q], 0x7362);
+      const uint32_t a23 = __byte_perm(v[2][q], v[3][q], 0x5140), b23 = __byte_perm(v[2][q], v[3][q], 0x7362);
       mma_f16(o[4 * q], pa[0], pa[1], pa[2], pa[3], half2_of_e4m3x2(a01), half2_of_e4m3x2(a23));
       mma_f16(o[4 * q + 1], pa[0], pa[1], pa[2], pa[3], half2_of_e4m3x2(a01 >> 16), half2_of_e4m3x2(a23 >> 16));
       mma_f16(o[4 * q + 2], pa[0], pa[1], pa[2], pa[3], half2_of_e4m3x2(b01), half2_of_e4m3x2(b23));
@@ -498,7 +520,11 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
     }
   }
 
-  // ---- the warps' shares ----
+  // ---- the warps' shares, each in its own part of the ring ----
+  copies_wait<0>();
+  __syncwarp();
+  constexpr int SHARE = ST * M::BYTES / 4;           // floats of a warp's part; 16 x D are used
+  float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
@@ -507,67 +533,76 @@ __global__ void __launch_bounds__(128) fp8_attend_kernel(const __grid_constant__
       sm_m[warp][n + 8 * e] = m[e];
       sm_l[warp][n + 8 * e] = l[e];
     }
+    if (n + 8 * e < nr) {
+      float* to = sums + warp * SHARE + (n + 8 * e) * D;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      sm_o[warp][n + 8 * e][2 * c * (D / 8) + b] = o[b][2 * e] * vref;
-      sm_o[warp][n + 8 * e][(2 * c + 1) * (D / 8) + b] = o[b][2 * e + 1] * vref;
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int b = 0; b < NB; b += 4)
+          *reinterpret_cast<float4*>(to + M::col(2 * c + h) + b) =
+              make_float4(o[b][2 * e + h] * vref, o[b + 1][2 * e + h] * vref, o[b + 2][2 * e + h] * vref, o[b + 3][2 * e + h] * vref);
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < nr * D; i += 128) {
-    const int r = i / D, d = i % D;
+  for (int i = threadIdx.x; i < nr * (D / 4); i += NW * 32) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
     float mm = sm_m[0][r];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm_m[w][r]);
-    float acc = 0.f, ll = 0.f;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float f = mm == -INFINITY ? 1.f : exp2_fast(sm_m[w][r] - mm);
-      acc += sm_o[w][r][d] * f;
+      const float4 v = *reinterpret_cast<const float4*>(sums + w * SHARE + r * D + d);
+      acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f;
       ll += sm_l[w][r] * f;
     }
     const int t = t0 + (r0 + r) / a.G, hd = hk * a.G + (r0 + r) % a.G;
     if (a.splits == 1) {
-      a.out[t * a.ld_o + hd * D + d] = __float2bfloat16_rn(ll == 0.f ? 0.f : acc / ll);
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      *reinterpret_cast<uint2*>(a.out + t * a.ld_o + hd * D + d) = make_uint2(cvt_bf16x2(acc[0] * inv, acc[1] * inv), cvt_bf16x2(acc[2] * inv, acc[3] * inv));
       continue;
     }
-    float* part = a.part + (((long)t * a.H + hd) * a.splits + split) * (D + 2);
-    part[2 + d] = acc;
+    const long at = ((long)t * a.H + hd) * a.splits + split;
+    *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     if (d == 0) {
-      part[0] = mm;
-      part[1] = ll;
+      a.part_ml[2 * at] = mm;
+      a.part_ml[2 * at + 1] = ll;
       if (split == 0) a.used[(long)t * a.H + hd] = max(1, min(a.splits, (pg_hi - pg_lo + a.per_split - 1) / a.per_split));
     }
   }
 }
 
-// Joins the splits of a row: a warp a row and head.
+// Joins the splits of a row: a warp a row and head, D / 32 values a lane.
 template <int D>
-__global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__ part, const int* __restrict__ used, __nv_bfloat16* __restrict__ out,
-                                                       long ld_o, int T, int H, int splits) {
+__global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__ part, const float* __restrict__ part_ml, const int* __restrict__ used,
+                                                       __nv_bfloat16* __restrict__ out, long ld_o, int T, int H, int splits) {
+  constexpr int E = D / 32;
   wait_previous();
   const long item = blockIdx.x * 8l + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (item >= (long)T * H) return;
-  const float* base = part + item * splits * (D + 2);
+  const float* base = part + item * splits * D + lane * E;
+  const float* ml = part_ml + item * splits * 2;
   const int ns = used[item];
   float mm = -INFINITY;
-  for (int s = lane; s < ns; s += 32) mm = fmaxf(mm, base[(long)s * (D + 2)]);
+  for (int s = lane; s < ns; s += 32) mm = fmaxf(mm, ml[2 * s]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-  float acc[D / 32], ll = 0.f;
+  float acc[E], ll = 0.f;
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int i = 0; i < E; ++i) acc[i] = 0.f;
+#pragma unroll 4
   for (int s = 0; s < ns; ++s) {
-    const float* p = base + (long)s * (D + 2);
-    const float f = mm == -INFINITY ? 1.f : exp2_fast(p[0] - mm);
-    ll += p[1] * f;
+    const float f = mm == -INFINITY ? 1.f : exp2_fast(ml[2 * s] - mm);
+    ll += ml[2 * s + 1] * f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] += p[2 + lane + 32 * i] * f;
+    for (int i = 0; i < E; ++i) acc[i] += base[(long)s * D + i] * f;
   }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  uint32_t* to = reinterpret_cast<uint32_t*>(out + item / H * ld_o + item % H * D + lane * E);
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-    out[item / H * ld_o + item % H * D + lane + 32 * i] = __float2bfloat16_rn(ll == 0.f ? 0.f : acc[i] / ll);
+  for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv, acc[i + 1] * inv);
 }
 
 }  // namespace inv
@@ -603,76 +638,95 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
-// Pages of a CTA, and from it CTAs along a sequence of `pages` pages.
-static int pages_per_split(long units, int pages) {
-  const long target = 148 * 12;
-  long per = (units * pages + target - 1) / target;
-  if (per < 32) per = 32;
-  return (int)(per < pages ? per : pages);
-}
-// Splits that inv_fp8_attend will use, for its caller's workspace: [T, H, splits, D + 2] floats and [T, H] ints where there are several.
-extern "C" int inv_fp8_attend_splits(int n, int Hkv, int G, int max_new, int max_len, int window) {
-  if (n < 1 || Hkv < 1 || G < 1 || max_new < 1 || max_len < 1) return 1;
-  const int tiles = (int)(((long)max_new * G + 15) / 16);
-  const long span = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
-  const int pages = (int)((span + 2 * FP8_PAGE - 2) / FP8_PAGE);
-  return (pages + pages_per_split((long)n * Hkv * tiles, pages) - 1) / pages_per_split((long)n * Hkv * tiles, pages);
+// How an attention is cut: row tiles of a sequence, pages of a CTA, CTAs along a sequence.
+struct Fp8Cut {
+  int tiles, per, splits;
+  Fp8Cut(int n, int Hkv, int G, int max_new, int max_len, int window) {
+    tiles = (int)(((long)max_new * G + 15) / 16);
+    const long span = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
+    const int pages = (int)((span + 2 * FP8_PAGE - 2) / FP8_PAGE);
+    const long units = (long)n * Hkv * tiles, target = 148 * 12;
+    per = (int)((units * pages + target - 1) / target);
+    if (per < 32) per = 32;
+    if (per > pages) per = pages;
+    splits = (pages + per - 1) / per;
+  }
+};
+// Floats of workspace that an attention wants (0: none). A call's own: it holds partial results from one launch to the next.
+extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int max_new, int max_len, int window) {
+  if (n < 1 || T < 1 || Hkv < 1 || H < Hkv || max_new < 1 || max_len < 1) return 0;
+  const Fp8Cut cut(n, Hkv, H / Hkv, max_new, max_len, window);
+  return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
 }
 
-static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, bool tree, cudaStream_t st) {
-  const int G = a.H / pool.Hkv;
-  a.G = G;
-  a.tiles = (int)(((long)max_new * G + 15) / 16);
-  a.splits = inv_fp8_attend_splits(tk.n, pool.Hkv, G, max_new, max_len, a.window);
-  const long span = a.window > 0 && (long)a.window + max_new < max_len ? (long)a.window + max_new : max_len;
-  const int pages = (int)((span + 2 * FP8_PAGE - 2) / FP8_PAGE);
-  a.per_split = pages_per_split((long)tk.n * pool.Hkv * a.tiles, pages);
-  if (a.splits > 1 && (!a.part || !a.used)) return -ERR_BAD_ARG;
+template <int D, bool TREE>
+static void fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
+  constexpr int NW = 4, SMEM = NW * FP8_STAGES * PageMap<D>::BYTES;
+  static std::atomic<uint64_t> ready{0};                           // devices whose limit has been raised
+  int device = 0;
+  cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (!(ready.load() & bit)) {
+    cudaFuncSetAttribute(fp8_attend_kernel<D, NW, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    ready.fetch_or(bit);
+  }
+  fp8_attend_kernel<D, NW, TREE><<<ctas, NW * 32, SMEM, st>>>(a, pool, tk);
+  if (a.splits > 1)
+    launch_early(fp8_join_kernel<D>, dim3((unsigned)(((long)tk.T * a.H + 7) / 8)), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, tk.T, a.H,
+                 a.splits);
+}
+
+static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, float* work, cudaStream_t st) {
+  a.G = a.H / pool.Hkv;
+  const Fp8Cut cut(tk.n, pool.Hkv, a.G, max_new, max_len, a.window);
+  a.tiles = cut.tiles;
+  a.per_split = cut.per;
+  a.splits = cut.splits;
+  if (cut.splits > 1) {
+    if (!work || off16(work)) return -ERR_BAD_ARG;
+    const long rows = (long)tk.T * a.H * cut.splits;
+    a.part = work;
+    a.part_ml = work + rows * D;
+    a.used = (int*)(work + rows * (D + 2));
+  }
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;
-#define INV_FP8(DD, TR) fp8_attend_kernel<DD, TR><<<(unsigned)ctas, 128, 0, st>>>(a, pool, tk)
-  if (D == 64) { if (tree) INV_FP8(64, true); else INV_FP8(64, false); }
-  else { if (tree) INV_FP8(128, true); else INV_FP8(128, false); }
-#undef INV_FP8
-  if (a.splits > 1) {
-    const dim3 grid((unsigned)(((long)tk.T * a.H + 7) / 8));
-    if (D == 64) launch_early(fp8_join_kernel<64>, grid, 256, 0, st, a.part, a.used, a.out, a.ld_o, tk.T, a.H, a.splits);
-    else launch_early(fp8_join_kernel<128>, grid, 256, 0, st, a.part, a.used, a.out, a.ld_o, tk.T, a.H, a.splits);
-  }
+  const bool tree = a.row_seq != nullptr;
+  if (D == 64) { if (tree) fp8_attend_launch<64, true>(a, pool, tk, (unsigned)ctas, st); else fp8_attend_launch<64, false>(a, pool, tk, (unsigned)ctas, st); }
+  else { if (tree) fp8_attend_launch<128, true>(a, pool, tk, (unsigned)ctas, st); else fp8_attend_launch<128, false>(a, pool, tk, (unsigned)ctas, st); }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
 // q [T, H D] bf16, rows ld_q apart -> out [T, H D], rows ld_o apart: the token at position p of its sequence sees the cached positions up to p, with a
-// window the latest `window` of them. No sequence has more than max_new new tokens or, with them, max_len tokens.
+// window the latest `window` of them. No sequence has more than max_new new tokens or, with them, max_len tokens. work: inv_fp8_attend_floats of them.
 extern "C" int inv_fp8_attend(const void* q, long ld_q, void* out, long ld_o, int H, int Hkv, int D, float scale, int window, const void* k_pool,
                               const void* v_pool, const float* k_scale, const float* v_scale, int pages, const int* page_table, int table_rows,
-                              int max_pages, const int* rows, const int* cu, const int* start, int n, int T, int max_new, int max_len, float* part,
-                              int* used, int* status, void* stream) {
+                              int max_pages, const int* rows, const int* cu, const int* start, int n, int T, int max_new, int max_len, float* work,
+                              int* status, void* stream) {
   if (fp8_bad_shape(H, Hkv, D, pages, n, T, table_rows, max_pages) || window < 0 || max_new < 1 || max_len < 1) return -ERR_BAD_ARG;
-  if (ld_q % 8 || off16(q, k_pool, v_pool)) return -ERR_BAD_ARG;
+  if (ld_q % 8 || ld_o % 8 || off16(q, k_pool, v_pool, out)) return -ERR_BAD_ARG;
   if (n == 0 || T == 0) return 0;
   Fp8Attend a{};
   a.q = (const __nv_bfloat16*)q; a.out = (__nv_bfloat16*)out; a.ld_q = ld_q; a.ld_o = ld_o; a.H = H; a.window = window; a.scale = scale;
-  a.part = part; a.used = used;
   const Fp8Pool pool{(uint8_t*)k_pool, (uint8_t*)v_pool, (float*)k_scale, (float*)v_scale, pages, Hkv};
   const Fp8Tokens tk{rows, cu, start, page_table, n, T, table_rows, max_pages, status};
-  return fp8_attend(a, pool, tk, D, max_new, max_len, false, (cudaStream_t)stream);
+  return fp8_attend(a, pool, tk, D, max_new, max_len, work, (cudaStream_t)stream);
 }
 
 // One query token a row over shared sequences: row t belongs to table row row_seq[t], which holds seq_lens[row_seq[t]] tokens, and sees those below
-// tail_start[t] and token tail_start[t] + i iff bit i of tail_mask[t] is set (both null: all).
+// tail_start[t] and token tail_start[t] + i iff bit i of tail_mask[t] is set (both null: all). work: as for T sequences of one new token.
 extern "C" int inv_fp8_attend_tree(const void* q, long ld_q, void* out, long ld_o, int H, int Hkv, int D, float scale, const void* k_pool,
                                    const void* v_pool, const float* k_scale, const float* v_scale, int pages, const int* page_table, int table_rows,
                                    int max_pages, const int* row_seq, const int* seq_lens, const int* tail_start, const unsigned long long* tail_mask,
-                                   int T, int max_len, float* part, int* used, int* status, void* stream) {
+                                   int T, int max_len, float* work, int* status, void* stream) {
   if (fp8_bad_shape(H, Hkv, D, pages, T, T, table_rows, max_pages) || max_len < 1 || !row_seq || !seq_lens || !tail_start != !tail_mask) return -ERR_BAD_ARG;
-  if (ld_q % 8 || off16(q, k_pool, v_pool)) return -ERR_BAD_ARG;
+  if (ld_q % 8 || ld_o % 8 || off16(q, k_pool, v_pool, out)) return -ERR_BAD_ARG;
   if (T == 0) return 0;
   Fp8Attend a{};
-  a.q = (const __nv_bfloat16*)q; a.out = (__nv_bfloat16*)out; a.ld_q = ld_q; a.ld_o = ld_o; a.H = H; a.scale = scale; a.part = part; a.used = used;
+  a.q = (const __nv_bfloat16*)q; a.out = (__nv_bfloat16*)out; a.ld_q = ld_q; a.ld_o = ld_o; a.H = H; a.scale = scale;
   a.row_seq = row_seq; a.seq_lens = seq_lens; a.tail_start = tail_start; a.tail_mask = tail_mask;
   const Fp8Pool pool{(uint8_t*)k_pool, (uint8_t*)v_pool, (float*)k_scale, (float*)v_scale, pages, Hkv};
   const Fp8Tokens tk{nullptr, nullptr, nullptr, page_table, T, T, table_rows, max_pages, status};
-  return fp8_attend(a, pool, tk, D, 1, max_len, true, (cudaStream_t)stream);
+  return fp8_attend(a, pool, tk, D, 1, max_len, work, (cudaStream_t)stream);
 }

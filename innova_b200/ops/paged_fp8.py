@@ -20,9 +20,9 @@ from .functional import _head_norm_rope, _weights16, check_rope
 _vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
 _native.register_cuda_sigs({
     "inv_fp8_append": [_vp, _vp, _l, _vp, _l, _vp, _l, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _i, _i, _vp] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i, _i, _vp, _vp],
-    "inv_fp8_attend_splits": [_i] * 6,
-    "inv_fp8_attend": [_vp, _l, _vp, _l, _i, _i, _i, _f, _i] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i] * 4 + [_vp] * 4,
-    "inv_fp8_attend_tree": [_vp, _l, _vp, _l, _i, _i, _i, _f] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 4 + [_i, _i] + [_vp] * 4,
+    "inv_fp8_attend_floats": [_i] * 8,
+    "inv_fp8_attend": [_vp, _l, _vp, _l, _i, _i, _i, _f, _i] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i] * 4 + [_vp] * 3,
+    "inv_fp8_attend_tree": [_vp, _l, _vp, _l, _i, _i, _i, _f] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 4 + [_i, _i] + [_vp] * 3,
 })
 
 PAGE, TOP, MIN_EXP = 16, 448.0, -64
@@ -93,11 +93,13 @@ def _check_new(new: NewTokens, dev):
     return n
 
 
+def _on16(x):
+    """Whether the rows of x start on 16-byte boundaries."""
+    return x.data_ptr() % 16 == 0 and (x.shape[0] <= 1 or x.stride(0) % 8 == 0)
+
+
 def _aligned(x):
-    """x with rows on 16-byte boundaries."""
-    if x.data_ptr() % 16 or (x.shape[0] > 1 and x.stride(0) % 8):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    return x if _on16(x) else x.clone(memory_format=torch.contiguous_format)
 
 
 def _ld(x):
@@ -195,7 +197,7 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
         return q_out
     if rot % 16:
         raise ValueError(f"{rot} rotated values: a multiple of 16 on a GPU")
-    if _ld(q_out) % 8 or q_out.data_ptr() % 16:
+    if not _on16(q_out):
         raise ValueError("q_out starts and steps on 16-byte boundaries")
     if T == 0 or n == 0:
         return q_out
@@ -260,11 +262,12 @@ def _check_out(out, q, width):
     return out
 
 
-def _workspace(T, heads, splits, dim, dev):
+def _workspace(n, T, heads, kv_heads, dim, max_new, max_len, window, dev):
     """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
-    if splits == 1:
-        return None, None
-    return (torch.empty(T * heads * splits * (dim + 2), dtype=torch.float32, device=dev), torch.empty(T * heads, dtype=torch.int32, device=dev))
+    fn = rt.lib().inv_fp8_attend_floats
+    fn.restype = _l
+    floats = fn(n, T, heads, kv_heads, dim, max_new, max_len, window)
+    return torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
 
 
 def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale: Optional[float] = None, window: int = 0,
@@ -289,15 +292,14 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
         return out
     if T == 0 or n == 0:
         return out
-    q = _aligned(q)
+    q, to = _aligned(q), out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
     with rt.device_of(q):
-        splits = rt.lib().inv_fp8_attend_splits(n, G, heads // G, new.max_new, new.max_len, window)
-        part, used = _workspace(T, heads, splits, D, q.device)
-        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, window,
+        work = _workspace(n, T, heads, G, D, new.max_new, new.max_len, window, q.device)
+        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, window,
                                          *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
-                                         new.max_new, new.max_len, rt.ptr(part), rt.ptr(used), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
+                                         new.max_new, new.max_len, rt.ptr(work), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
                  "inv_fp8_attend")
-    return out
+    return out if to is out else out.copy_(to)
 
 
 def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, max_len: int, scale: Optional[float] = None, tail_start=None,
@@ -327,12 +329,10 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
         return out
     if T == 0:
         return out
-    q = _aligned(q)
+    q, to = _aligned(q), out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
     with rt.device_of(q):
-        splits = rt.lib().inv_fp8_attend_splits(T, G, heads // G, 1, max_len, 0)
-        part, used = _workspace(T, heads, splits, D, q.device)
-        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), out.data_ptr(), _ld(out), heads, G, D, scale, *_pool_args(pages, page_table),
+        work = _workspace(T, T, heads, G, D, 1, max_len, 0, q.device)
+        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, *_pool_args(pages, page_table),
                                               row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
-                                              max_len, rt.ptr(part), rt.ptr(used), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
-                 "inv_fp8_attend_tree")
-    return out
+                                              max_len, rt.ptr(work), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()), "inv_fp8_attend_tree")
+    return out if to is out else out.copy_(to)
