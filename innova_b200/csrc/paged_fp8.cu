@@ -220,12 +220,6 @@ struct Fp8Attend {
   const unsigned long long* tail_mask;
 };
 
-__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -242,10 +236,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Where the codes of a page lie in a warp's ring, and which of them a lane takes. In shared memory a page's keys (and values) are lines of 128 bytes whose
-// 16-byte pieces are exchanged by the line's number, so that the eight lanes of a read meet all banks. n = lane / 4, c = lane % 4. Column n of block j of
-// a score product is token slot(j, n); a lane's scores are those of columns 2 c and 2 c + 1 of both blocks, and its values those four tokens'. Column n of
-// block b of the value product is dimension col(n) + b.
+// The transpose of an 8 x 8 matrix of 16-bit values over the warp: a lane's pair of row lane / 4 becomes one of column lane / 4.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+
+// Where the codes of a page lie in a warp's ring, and which of them a lane takes. A page's keys (and values) are lines of 128 bytes whose 16-byte pieces
+// are exchanged by the line's number (the copies' 128-byte swizzle), so that the eight lanes of a read meet all banks. n = lane / 4, c = lane % 4. Row n
+// and n + 8 of a score product are the tokens slot(0, n) and slot(1, n); a lane's values are those of the tokens of rows 2 c, 2 c + 1 and those + 8, from
+// dimension col(n) on.
 template <int D>
 struct PageMap {
   static constexpr int KP = D / 64, VW = D / 32, BYTES = 2 * FP8_PAGE * D;
@@ -257,30 +258,45 @@ struct PageMap {
   static __device__ __forceinline__ int col(int n) { return D == 128 ? ((n >> 1) + 4 * (n & 1)) * 16 : n * 8; }
 };
 
-constexpr int FP8_STAGES = 4;
+constexpr int FP8_STAGES = 4, FP8_WARPS = 4;
+template <int D>
+constexpr int fp8_attend_smem() { return FP8_WARPS * FP8_STAGES * PageMap<D>::BYTES + 1024; }
 
-// Sixteen rows (query tokens times the heads that share a key head) against a run of pages: grid = sequences x key heads x splits x row tiles, NW warps
+// 8 NR rows (query tokens times the heads that share a key head) against a run of pages: grid = sequences x key heads x splits x row tiles, four warps
 // that take a page in turn, each with a softmax of its own; they join at the end.
 //
-// Scores and values are products on m16n8k16 tensor instructions in fp16: a code is exact there, and so is a query up to 2^-24 of its row's largest value
-// once the row is scaled by a power of two. Which dimension or token an index of a product means is free as long as both operands agree, so a lane's
-// 16-byte pieces of a key row are its operands as they lie, and the tokens of a page are numbered such that a lane's four scores a row are the four tokens
-// whose values it loads. Page scales multiply the scores, and the weights relative to the largest value scale so far, which the sums are kept in.
-// Weights are 2^(s - m + 6) with a maximum that is raised only by scores above m + 8, so at most 2^14, and what fp16 rounds away of a weight is under
-// 2^-30 of the largest one.
+// Scores (keys times queries) and outputs (values times weights) are products on m16n8k16 tensor instructions in fp16, with the codes as the operand of 16
+// rows, so that eight query rows fill the other one. A code is exact in fp16, and so is a query up to 2^-24 of its row's largest value once the row is
+// scaled by a power of two. Which dimension or token an index of a product means is free as long as both operands agree, so a lane's 16-byte pieces of a
+// key are its operands as they lie; the weights turn into the other product's operand by an 8 x 8 transpose. Page scales multiply the scores, and the
+// weights relative to the largest value scale so far, which the sums are kept in. Weights are 2^(s - m + 6) with a maximum that is raised only by scores
+// above m + 8, so at most 2^14, and what fp16 rounds away of a weight is under 2^-30 of the largest one.
 //
-// Bound by memory. A warp keeps three pages on their way through a ring of its own in shared memory (with one, in registers, 8 contexts of up to 65000
-// tokens, 8 key heads of 128, took 156 us), which takes no registers and no barrier of the CTA.
-template <int D, int NW, bool TREE>
-__global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
-                                                             const __grid_constant__ Fp8Tokens tk) {
+// Bound by memory, with the conversion of codes (64 instructions a page and warp on the integer pipe) close behind. A warp keeps its next pages on their
+// way through a ring of its own in shared memory, filled by its first lane with one bulk copy each for keys and values, which takes no registers, hardly
+// an instruction and no barrier of the CTA.
+template <int D, int NR, bool TREE>
+__global__ void __launch_bounds__(FP8_WARPS * 32) fp8_attend_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
+                                                                    const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
+                                                                    const __grid_constant__ Fp8Tokens tk) {
   using M = PageMap<D>;
-  constexpr int KS = D / 16, NB = D / 8, KP = M::KP, VW = M::VW, ST = FP8_STAGES;
+  constexpr int NW = FP8_WARPS, ST = FP8_STAGES, KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR;
   constexpr float LIFT = 6.f, SLACK = 8.f;
-  extern __shared__ __align__(128) uint8_t ring[];               // NW x ST pages; afterwards the warps' sums
-  __shared__ float sm_m[NW][16], sm_l[NW][16];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));   // NW x ST pages; then the sums
+  __shared__ float sm_m[NW][ROWS], sm_l[NW][ROWS];
+  __shared__ __align__(8) uint64_t full[NW][ST];
+  __shared__ int abort_word;
   release_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < ST; ++i) mbar_init(&full[warp][i], 1);
+    fence_barrier_init();
+    if (warp == 0) abort_word = 0;
+  }
+  __syncthreads();
+  volatile int* abort_flag = &abort_word;
   int x = blockIdx.x;
   const int tile = x % a.tiles;
   x /= a.tiles;
@@ -311,9 +327,9 @@ __global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_consta
       return;
     }
     rows = count * a.G;
-    if (rows > 16 * a.tiles && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);         // more new tokens than the caller said
+    if (rows > ROWS * a.tiles && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);       // more new tokens than the caller said
   }
-  const int r0 = tile * 16, nr = min(16, rows - r0);
+  const int r0 = tile * ROWS, nr = min(ROWS, rows - r0);
   if (nr <= 0) return;
   const int first = start + r0 / a.G, last = start + (r0 + nr - 1) / a.G;       // positions of the tile's tokens
   const int hi = TREE ? len : last + 1, lo = !TREE && a.window > 0 ? max(0, first - a.window + 1) : 0;
@@ -322,38 +338,36 @@ __global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_consta
   if (split > 0 && p0 >= p1) return;
 
   // ---- the warp's pages: its i-th is p0 + warp + NW i ----
-  // A lane keeps the number of one of 32 pages: `nf` of those that are fetched, three pages ahead of `nc` with the scales of those that are worked on; the
+  // A lane keeps the number of one of 32 pages: `nf` of those that are fetched, ST - 1 pages ahead of `nc` with the scales of those that are worked on; the
   // next 32 are looked up in between, so that neither look-up is waited for.
   const int mine = p1 > p0 + warp ? (p1 - p0 - warp + NW - 1) / NW : 0;
   auto number_of = [&](int i) { return i < mine ? pool_page(tk, pool.pages, row, p0 + warp + NW * i) : -1; };
   auto scale_at = [&](const float* scales, int id) { return id >= 0 ? scales[(long)id * pool.Hkv + hk] : 0.f; };
-  const uint32_t slots = smem_u32(ring) + warp * ST * M::BYTES;
+  uint8_t* const slots = ring + warp * ST * M::BYTES;
   int nf = number_of(lane), nn = -1;
   auto fetch = [&](int i) {                                       // page i into its slot
     const int id = __shfl_sync(0xffffffffu, nf, i & 31);
-    if (i < mine && id >= 0) {
-      const long base = ((long)id * pool.Hkv + hk) * FP8_PAGE * D;
-      const uint32_t dst = slots + (i % ST) * M::BYTES;
-#pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
-        const int at = (q * 32 + lane) * 16;
-        copy16_async(dst + M::at(at), pool.k + base + at);
-        copy16_async(dst + FP8_PAGE * D + M::at(at), pool.v + base + at);
-      }
+    if (lane == 0 && i < mine && id >= 0) {
+      uint64_t* bar = &full[warp][i % ST];
+      uint8_t* dst = slots + (i % ST) * M::BYTES;
+      const int line = (id * pool.Hkv + hk) * (FP8_PAGE * D / 128);
+      mbar_expect_tx(bar, M::BYTES);
+      tma_load_2d(dst, &tmap_k, bar, 0, line);
+      tma_load_2d(dst + FP8_PAGE * D, &tmap_v, bar, 0, line);
     }
-    copies_commit();
   };
 #pragma unroll
   for (int i = 0; i < ST - 1; ++i) fetch(i);
   int nc = nf;
   float ksc = scale_at(pool.k_scale, nc), vsc = scale_at(pool.v_scale, nc), ksn = 0.f, vsn = 0.f;
 
-  // ---- queries ----
-  uint32_t qa[KS][4];
-  float qm[2];
+  // ---- queries: row n of a block of eight, as the second operand ----
+  uint32_t qb[NR][KS][2];
+  float qm[NR][2];                                                              // of this lane's columns: rows 2 c and 2 c + 1
+  int vlo[NR][2], vhi[NR][2];                                                   // positions that they see: [vlo, vhi)
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int r = r0 + n + 8 * e;
+  for (int b = 0; b < NR; ++b) {
+    const int r = r0 + b * 8 + n;
     uint4 raw[KP][2];
     uint32_t top = 0;
 #pragma unroll
@@ -361,7 +375,7 @@ __global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_consta
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         raw[j][i] = make_uint4(0, 0, 0, 0);
-        if (n + 8 * e < nr) raw[j][i] = *reinterpret_cast<const uint4*>(a.q + (t0 + r / a.G) * a.ld_q + (hk * a.G + r % a.G) * D + j * 64 + c * 16 + i * 8);
+        if (b * 8 + n < nr) raw[j][i] = *reinterpret_cast<const uint4*>(a.q + (t0 + r / a.G) * a.ld_q + (hk * a.G + r % a.G) * D + j * 64 + c * 16 + i * 8);
         const uint32_t w[4] = {raw[j][i].x, raw[j][i].y, raw[j][i].z, raw[j][i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
@@ -369,34 +383,38 @@ __global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_consta
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int ex = min(max((int)(top >> 7), 1), 253);                           // 2^(ex - 127): the row's largest value, but for its fraction
-    const float down = __uint_as_float((uint32_t)(254 - ex) << 23);
-    qm[e] = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);
+    const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);
 #pragma unroll
     for (int j = 0; j < KP; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint4 v = raw[j][i >> 1];
         const uint32_t w0 = i & 1 ? v.z : v.x, w1 = i & 1 ? v.w : v.y;
-        qa[j * 4 + i][e] = half2_of(__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down);
-        qa[j * 4 + i][2 + e] = half2_of(__uint_as_float(w1 << 16) * down, __uint_as_float(w1 & 0xffff0000u) * down);
+        qb[b][j * 4 + i][0] = half2_of(__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down);
+        qb[b][j * 4 + i][1] = half2_of(__uint_as_float(w1 << 16) * down, __uint_as_float(w1 & 0xffff0000u) * down);
       }
-  }
-  // visible positions of this lane's two rows: [vlo, vhi)
-  int vlo[2], vhi[2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int p = start + min(r0 + n + 8 * e, rows - 1) / a.G;
-    vhi[e] = TREE ? len : p + 1;
-    vlo[e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
+    for (int e = 0; e < 2; ++e) {
+      qm[b][e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4);
+      const int p = start + min(r0 + b * 8 + 2 * c + e, rows - 1) / a.G;
+      vhi[b][e] = TREE ? len : p + 1;
+      vlo[b][e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
+    }
   }
   const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;    // positions that every row sees
 
-  float o[NB][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, vref = 0.f, vinv = 0.f;
+  float o[NR][NI][4], m[NR][2], l[NR][2], vref = 0.f, vinv = 0.f;
 #pragma unroll
-  for (int i = 0; i < NB; ++i)
+  for (int b = 0; b < NR; ++b) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
+    m[b][0] = m[b][1] = -INFINITY;
+    l[b][0] = l[b][1] = 0.f;
+  }
 
+  bool ok = true;
   for (int i = 0; i < mine; ++i) {
     if ((i & 31) == 0) {
       if (i > 0) {
@@ -413,43 +431,45 @@ __global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_consta
     if (((i + ST - 1) & 31) == 0) nf = nn;
     const int id = __shfl_sync(0xffffffffu, nc, i & 31), pos = (p0 + warp + NW * i) * FP8_PAGE;
     const float ks = __shfl_sync(0xffffffffu, ksc, i & 31), vs = __shfl_sync(0xffffffffu, vsc, i & 31);
-    copies_wait<ST - 2>();
-    __syncwarp();
     fetch(i + ST - 1);                               // into the slot of page i - 1, which every lane has read
     if (id < 0) continue;
-    const uint8_t* page = ring + (warp * ST + i % ST) * M::BYTES;
-    // ---- scores ----
-    float s[2][4];
+    if (!mbar_wait_warp(&full[warp][i % ST], (i / ST) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) {
+      ok = false;
+      break;
+    }
+    const uint8_t* page = slots + (i % ST) * M::BYTES;
+    // ---- scores: 16 tokens x 8 rows ----
+    float s[NR][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int b = 0; b < NR; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[b][e] = 0.f;
 #pragma unroll
-      for (int q = 0; q < KP; ++q) {
-        const uint4 k4 = *reinterpret_cast<const uint4*>(page + M::at(M::slot(j, n) * D + q * 64 + c * 16));
-        const uint32_t w[4] = {k4.x, k4.y, k4.z, k4.w};
+    for (int q = 0; q < KP; ++q) {
+      const uint4 x4 = *reinterpret_cast<const uint4*>(page + M::at(M::slot(0, n) * D + q * 64 + c * 16));
+      const uint4 y4 = *reinterpret_cast<const uint4*>(page + M::at(M::slot(1, n) * D + q * 64 + c * 16));
+      const uint32_t xs[4] = {x4.x, x4.y, x4.z, x4.w}, ys[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t(&f)[4] = qa[q * 4 + k];
-          mma_f16(s[j], f[0], f[1], f[2], f[3], half2_of_e4m3x2(w[k]), half2_of_e4m3x2(w[k] >> 16));
-        }
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t k0 = half2_of_e4m3x2(xs[k]), k1 = half2_of_e4m3x2(ys[k]), k2 = half2_of_e4m3x2(xs[k] >> 16), k3 = half2_of_e4m3x2(ys[k] >> 16);
+#pragma unroll
+        for (int b = 0; b < NR; ++b) mma_f16(s[b], k0, k1, k2, k3, qb[b][q * 4 + k][0], qb[b][q * 4 + k][1]);
       }
     }
-    const float f0 = qm[0] * ks, f1 = qm[1] * ks;
     const bool whole = pos >= all_lo && pos + FP8_PAGE <= all_hi;
     bool over = vs > vref;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int b = 0; b < NR; ++b)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[j][e] *= e < 2 ? f0 : f1;
+        s[b][e] *= qm[b][e & 1] * ks;
         if (!whole) {
-          const int at = pos + M::slot(j, 2 * c + (e & 1));
-          bool seen = at >= vlo[e >> 1] && at < vhi[e >> 1];
+          const int at = pos + M::slot(e >> 1, n);
+          bool seen = at >= vlo[b][e & 1] && at < vhi[b][e & 1];
           if (TREE) seen = seen && (at < tail || (at - tail < 64 && ((bits >> ((at - tail) & 63)) & 1ull)));
-          if (!seen) s[j][e] = -INFINITY;
+          if (!seen) s[b][e] = -INFINITY;
         }
-        over |= s[j][e] > m[e >> 1] + SLACK;
+        over |= s[b][e] > m[b][e & 1] + SLACK;
       }
     if (__any_sync(0xffffffffu, over)) {
       const float beta = vs > vref ? vref / vs : 1.f;
@@ -457,41 +477,42 @@ __global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_consta
         vref = vs;
         vinv = 1.f / vs;
       }
-      float alpha[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float mx = fmaxf(fmaxf(s[0][2 * e], s[0][2 * e + 1]), fmaxf(s[1][2 * e], s[1][2 * e + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float up = fmaxf(m[e], mx);
-        alpha[e] = up == m[e] ? 1.f : exp2_fast(m[e] - up);
-        m[e] = up;
-        l[e] *= alpha[e];
-        alpha[e] *= beta;
-      }
+      for (int b = 0; b < NR; ++b) {
+        float alpha[2];
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        o[b][0] *= alpha[0];
-        o[b][1] *= alpha[0];
-        o[b][2] *= alpha[1];
-        o[b][3] *= alpha[1];
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(s[b][e], s[b][2 + e]);
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float up = fmaxf(m[b][e], mx);
+          alpha[e] = up == m[b][e] ? 1.f : exp2_fast(m[b][e] - up);
+          m[b][e] = up;
+          l[b][e] *= alpha[e];
+          alpha[e] *= beta;
+        }
+#pragma unroll
+        for (int k = 0; k < NI; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[e & 1];
       }
     }
     const float rel = vs * vinv;
-    uint32_t pa[4];
+    uint32_t pb[NR][2];                              // weights of rows n: tokens of rows 2 c, 2 c + 1 (and + 8) of the score product
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int b = 0; b < NR; ++b)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float w0 = exp2_fast(s[j][2 * e] - m[e] + LIFT), w1 = exp2_fast(s[j][2 * e + 1] - m[e] + LIFT), x0 = w0 * rel, x1 = w1 * rel;
+      for (int h = 0; h < 2; ++h) {
+        float w0 = exp2_fast(s[b][2 * h] - m[b][0] + LIFT), w1 = exp2_fast(s[b][2 * h + 1] - m[b][1] + LIFT), x0 = w0 * rel, x1 = w1 * rel;
         if (!whole) {                                 // nothing of a hidden place, whatever its scale and however little the row has seen
-          if (s[j][2 * e] == -INFINITY) w0 = x0 = 0.f;
-          if (s[j][2 * e + 1] == -INFINITY) w1 = x1 = 0.f;
+          if (s[b][2 * h] == -INFINITY) w0 = x0 = 0.f;
+          if (s[b][2 * h + 1] == -INFINITY) w1 = x1 = 0.f;
         }
-        l[e] += w0 + w1;
-        pa[2 * j + e] = half2_of(x0, x1);
+        l[b][0] += w0;
+        l[b][1] += w1;
+        pb[b][h] = transpose8(half2_of(x0, x1));
       }
-    // ---- values ----
+    // ---- values: dimensions x 8 rows ----
     uint32_t v[4][VW];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -510,39 +531,46 @@ __global__ void __launch_bounds__(NW * 32) fp8_attend_kernel(const __grid_consta
       }
     }
 #pragma unroll
-    for (int q = 0; q < VW; ++q) {
+    for (int q = 0; q < VW; ++q) {                    // four dimensions of the lane: two products, rows n and n + 8 one dimension each
       const uint32_t a01 = __byte_perm(v[0][q], v[1][q], 0x5140), b01 = __byte_perm(v[0][q], v[1][q], 0x7362);
       const uint32_t a23 = __byte_perm(v[2][q], v[3][q], 0x5140), b23 = __byte_perm(v[2][q], v[3][q], 0x7362);
-      mma_f16(o[4 * q], pa[0], pa[1], pa[2], pa[3], half2_of_e4m3x2(a01), half2_of_e4m3x2(a23));
-      mma_f16(o[4 * q + 1], pa[0], pa[1], pa[2], pa[3], half2_of_e4m3x2(a01 >> 16), half2_of_e4m3x2(a23 >> 16));
-      mma_f16(o[4 * q + 2], pa[0], pa[1], pa[2], pa[3], half2_of_e4m3x2(b01), half2_of_e4m3x2(b23));
-      mma_f16(o[4 * q + 3], pa[0], pa[1], pa[2], pa[3], half2_of_e4m3x2(b01 >> 16), half2_of_e4m3x2(b23 >> 16));
+      const uint32_t va[4] = {half2_of_e4m3x2(a01), half2_of_e4m3x2(a01 >> 16), half2_of_e4m3x2(a23), half2_of_e4m3x2(a23 >> 16)};
+      const uint32_t vb[4] = {half2_of_e4m3x2(b01), half2_of_e4m3x2(b01 >> 16), half2_of_e4m3x2(b23), half2_of_e4m3x2(b23 >> 16)};
+#pragma unroll
+      for (int b = 0; b < NR; ++b) {
+        mma_f16(o[b][2 * q], va[0], va[1], va[2], va[3], pb[b][0], pb[b][1]);
+        mma_f16(o[b][2 * q + 1], vb[0], vb[1], vb[2], vb[3], pb[b][0], pb[b][1]);
+      }
     }
+    __syncwarp();                                    // the slot may be filled again
+  }
+  if (!ok) {                                         // a copy did not arrive in time: the status word says so; what is on its way lands first
+    const uint64_t since = globaltimer_ns();
+    while (globaltimer_ns() - since < 2000000ull) __nanosleep(1000);
   }
 
   // ---- the warps' shares, each in its own part of the ring ----
-  copies_wait<0>();
-  __syncwarp();
-  constexpr int SHARE = ST * M::BYTES / 4;           // floats of a warp's part; 16 x D are used
+  constexpr int SHARE = ST * M::BYTES / 4;           // floats of a warp's part; ROWS x D are used
+  static_assert(ROWS * D <= SHARE, "sums fit the ring");
   float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    if (c == 0) {
-      sm_m[warp][n + 8 * e] = m[e];
-      sm_l[warp][n + 8 * e] = l[e];
-    }
-    if (n + 8 * e < nr) {
-      float* to = sums + warp * SHARE + (n + 8 * e) * D;
+  for (int b = 0; b < NR; ++b)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-        for (int b = 0; b < NB; b += 4)
-          *reinterpret_cast<float4*>(to + M::col(2 * c + h) + b) =
-              make_float4(o[b][2 * e + h] * vref, o[b + 1][2 * e + h] * vref, o[b + 2][2 * e + h] * vref, o[b + 3][2 * e + h] * vref);
+      for (int d = 4; d < 32; d *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
+      const int r = b * 8 + 2 * c + e;
+      if (n == 0) {
+        sm_m[warp][r] = m[b][e];
+        sm_l[warp][r] = l[b][e];
+      }
+      if (r < nr) {
+        float* to = sums + warp * SHARE + r * D + M::col(n);
+#pragma unroll
+        for (int k = 0; k < NI; k += 2)
+          *reinterpret_cast<float4*>(to + 2 * k) = make_float4(o[b][k][e] * vref, o[b][k][2 + e] * vref, o[b][k + 1][e] * vref, o[b][k + 1][2 + e] * vref);
+      }
     }
-  }
   __syncthreads();
   for (int i = threadIdx.x; i < nr * (D / 4); i += NW * 32) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
@@ -610,7 +638,8 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__
 using namespace inv;
 
 static bool fp8_bad_shape(int H, int Hkv, int D, int pages, int n, int T, int table_rows, int max_pages) {
-  return (D != 64 && D != 128) || Hkv < 1 || H < Hkv || H % Hkv || pages < 1 || n < 0 || T < 0 || table_rows < 1 || max_pages < 1;
+  // the lines of a pool are numbered in 31 bits
+  return (D != 64 && D != 128) || (long)pages * Hkv * (FP8_PAGE * D / 128) > 0x7fffffffl || Hkv < 1 || H < Hkv || H % Hkv || pages < 1 || n < 0 || T < 0 || table_rows < 1 || max_pages < 1;
 }
 static bool off16(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
   return ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16 != 0;
@@ -640,9 +669,10 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
 
 // How an attention is cut: row tiles of a sequence, pages of a CTA, CTAs along a sequence.
 struct Fp8Cut {
-  int tiles, per, splits;
+  int blocks, tiles, per, splits;      // blocks: of eight rows in a tile
   Fp8Cut(int n, int Hkv, int G, int max_new, int max_len, int window) {
-    tiles = (int)(((long)max_new * G + 15) / 16);
+    blocks = (long)max_new * G <= 8 ? 1 : 2;
+    tiles = (int)(((long)max_new * G + 8 * blocks - 1) / (8 * blocks));
     const long span = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
     const int pages = (int)((span + 2 * FP8_PAGE - 2) / FP8_PAGE);
     const long units = (long)n * Hkv * tiles, target = 148 * 12;
@@ -659,21 +689,48 @@ extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int m
   return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
 }
 
-template <int D, bool TREE>
-static void fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
-  constexpr int NW = 4, SMEM = NW * FP8_STAGES * PageMap<D>::BYTES;
+// The codes of a pool as lines of 128 bytes, read a page of a head at a time with the pieces of a line exchanged.
+static int fp8_tensor_map(CUtensorMap* out, const uint8_t* codes, long pages_heads, int D) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> known{nullptr};
+  bind_context();
+  Encode encode = known.load();
+  if (!encode) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return -1;
+    encode = reinterpret_cast<Encode>(f);
+    known.store(encode);
+  }
+  const cuuint32_t lines = FP8_PAGE * D / 128;
+  const cuuint64_t dims[2] = {128, (cuuint64_t)pages_heads * lines}, strides[1] = {128};
+  const cuuint32_t box[2] = {128, lines}, steps[2] = {1, 1};
+  const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -(int)r - 1000;
+}
+
+template <int D, int NR, bool TREE>
+static int fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
+  constexpr int SMEM = fp8_attend_smem<D>();
   static std::atomic<uint64_t> ready{0};                           // devices whose limit has been raised
   int device = 0;
   cudaGetDevice(&device);
   const uint64_t bit = 1ull << (device & 63);
   if (!(ready.load() & bit)) {
-    cudaFuncSetAttribute(fp8_attend_kernel<D, NW, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    cudaFuncSetAttribute(fp8_attend_kernel<D, NR, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     ready.fetch_or(bit);
   }
-  fp8_attend_kernel<D, NW, TREE><<<ctas, NW * 32, SMEM, st>>>(a, pool, tk);
+  CUtensorMap mk, mv;
+  if (int rc = fp8_tensor_map(&mk, pool.k, (long)pool.pages * pool.Hkv, D)) return rc;
+  if (int rc = fp8_tensor_map(&mv, pool.v, (long)pool.pages * pool.Hkv, D)) return rc;
+  fp8_attend_kernel<D, NR, TREE><<<ctas, FP8_WARPS * 32, SMEM, st>>>(mk, mv, a, pool, tk);
   if (a.splits > 1)
     launch_early(fp8_join_kernel<D>, dim3((unsigned)(((long)tk.T * a.H + 7) / 8)), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, tk.T, a.H,
                  a.splits);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : -(int)e;
 }
 
 static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, float* work, cudaStream_t st) {
@@ -691,11 +748,13 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
   }
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;
-  const bool tree = a.row_seq != nullptr;
-  if (D == 64) { if (tree) fp8_attend_launch<64, true>(a, pool, tk, (unsigned)ctas, st); else fp8_attend_launch<64, false>(a, pool, tk, (unsigned)ctas, st); }
-  else { if (tree) fp8_attend_launch<128, true>(a, pool, tk, (unsigned)ctas, st); else fp8_attend_launch<128, false>(a, pool, tk, (unsigned)ctas, st); }
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? 0 : -(int)e;
+  const unsigned grid = (unsigned)ctas;
+#define INV_FP8(DD)                                                                                                                        \
+  if (a.row_seq) return cut.blocks == 1 ? fp8_attend_launch<DD, 1, true>(a, pool, tk, grid, st) : fp8_attend_launch<DD, 2, true>(a, pool, tk, grid, st); \
+  return cut.blocks == 1 ? fp8_attend_launch<DD, 1, false>(a, pool, tk, grid, st) : fp8_attend_launch<DD, 2, false>(a, pool, tk, grid, st)
+  if (D == 64) { INV_FP8(64); }
+  INV_FP8(128);
+#undef INV_FP8
 }
 
 // q [T, H D] bf16, rows ld_q apart -> out [T, H D], rows ld_o apart: the token at position p of its sequence sees the cached positions up to p, with a
