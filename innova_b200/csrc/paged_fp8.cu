@@ -83,6 +83,8 @@ __global__ void __launch_bounds__(256) fp8_append_kernel(const __grid_constant__
   __shared__ int found[2];
   if (threadIdx.x == 0) found[0] = -1;
   __syncthreads();
+  wait_previous();
+  release_next();
   for (int i = threadIdx.x; i < tk.n; i += 256) {
     const int base = tk.cu[i] / FP8_PAGE + 2 * i, next = tk.cu[i + 1] / FP8_PAGE + 2 * (i + 1);
     if (base <= (int)blockIdx.x && (int)blockIdx.x < next) {
@@ -212,6 +214,7 @@ struct Fp8Attend {
   float scale;
   int per_split;        // pages of a CTA
   int splits, tiles;
+  uint32_t inv_tiles, inv_splits, inv_hkv, inv_g;     // div_reciprocal
   float *part, *part_ml;  // splits > 1: [T, H, splits, D] values, [T, H, splits, 2] maximum and sum
   int* used;            // splits > 1: [T, H] splits that a row has
   // Rows of a token tree (or null): row t is of table row row_seq[t], which holds seq_lens[.] tokens, and sees those below tail_start[t] and of the 64
@@ -236,6 +239,25 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint2 shared8(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// In front of code that is to stay behind its branch: selects in its place would be paid for by every page.
+__device__ __forceinline__ void rarely() { asm volatile(""); }
+
 // The transpose of an 8 x 8 matrix of 16-bit values over the warp: a lane's pair of row lane / 4 becomes one of column lane / 4.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t d;
@@ -244,7 +266,7 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
 }
 
 // Where the codes of a page lie in a warp's ring, and which of them a lane takes. A page's keys (and values) are lines of 128 bytes whose 16-byte pieces
-// are exchanged by the line's number (the copies' 128-byte swizzle), so that the eight lanes of a read meet all banks. n = lane / 4, c = lane % 4. Row n
+// are exchanged by the line's number, so that the eight lanes of a read meet all banks. n = lane / 4, c = lane % 4. Row n
 // and n + 8 of a score product are the tokens slot(0, n) and slot(1, n); a lane's values are those of the tokens of rows 2 c, 2 c + 1 and those + 8, from
 // dimension col(n) on.
 template <int D>
@@ -258,12 +280,12 @@ struct PageMap {
   static __device__ __forceinline__ int col(int n) { return D == 128 ? ((n >> 1) + 4 * (n & 1)) * 16 : n * 8; }
 };
 
-constexpr int FP8_STAGES = 4, FP8_WARPS = 4;
-template <int D>
-constexpr int fp8_attend_smem() { return FP8_WARPS * FP8_STAGES * PageMap<D>::BYTES + 1024; }
+constexpr int FP8_STAGES = 2;     // slots of two pages a warp
+template <int D, int NW>
+constexpr int fp8_attend_smem() { return NW * FP8_STAGES * 2 * PageMap<D>::BYTES; }
 
-// 8 NR rows (query tokens times the heads that share a key head) against a run of pages: grid = sequences x key heads x splits x row tiles, four warps
-// that take a page in turn, each with a softmax of its own; they join at the end.
+// 8 NR rows (query tokens times the heads that share a key head) against a run of pages: grid = sequences x key heads x splits x row tiles. Four warps take
+// two pages at a time in turn, each with a softmax of its own, and join at the end.
 //
 // Scores (keys times queries) and outputs (values times weights) are products on m16n8k16 tensor instructions in fp16, with the codes as the operand of 16
 // rows, so that eight query rows fill the other one. A code is exact in fp16, and so is a query up to 2^-24 of its row's largest value once the row is
@@ -272,47 +294,34 @@ constexpr int fp8_attend_smem() { return FP8_WARPS * FP8_STAGES * PageMap<D>::BY
 // weights relative to the largest value scale so far, which the sums are kept in. Weights are 2^(s - m + 6) with a maximum that is raised only by scores
 // above m + 8, so at most 2^14, and what fp16 rounds away of a weight is under 2^-30 of the largest one.
 //
-// Bound by memory, with the conversion of codes (64 instructions a page and warp on the integer pipe) close behind. A warp keeps its next pages on their
-// way through a ring of its own in shared memory, filled by its first lane with one bulk copy each for keys and values, which takes no registers, hardly
-// an instruction and no barrier of the CTA.
-template <int D, int NR, bool TREE>
-__global__ void __launch_bounds__(FP8_WARPS * 32) fp8_attend_kernel(const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v,
-                                                                    const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
-                                                                    const __grid_constant__ Fp8Tokens tk) {
+// Bound by memory where there are enough pages, by a warp's own chain of instructions where there are few. A warp keeps its next pages on their way through
+// a ring of its own in shared memory, without registers and without a barrier of the CTA. Bulk copies in their place cost their issuing thread over a
+// hundred cycles each: 8 contexts of up to 65000 tokens, 8 key heads of 128, took 99.7 us with each warp's first lane issuing them, 111 with a fifth warp.
+template <int D, int NR, int NW, bool TREE>
+__global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_kernel(const __grid_constant__ Fp8Attend a,
+                                                                                      const __grid_constant__ Fp8Pool pool,
+                                                                                      const __grid_constant__ Fp8Tokens tk) {
   using M = PageMap<D>;
-  constexpr int NW = FP8_WARPS, ST = FP8_STAGES, KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR;
+  constexpr int ST = FP8_STAGES, KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR, SLOT = 2 * M::BYTES;
   constexpr float LIFT = 6.f, SLACK = 8.f;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));   // NW x ST pages; then the sums
+  extern __shared__ __align__(128) uint8_t ring[];    // NW x ST slots; then the sums
   __shared__ float sm_m[NW][ROWS], sm_l[NW][ROWS];
-  __shared__ __align__(8) uint64_t full[NW][ST];
-  __shared__ int abort_word;
-  release_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < ST; ++i) mbar_init(&full[warp][i], 1);
-    fence_barrier_init();
-    if (warp == 0) abort_word = 0;
-  }
-  __syncthreads();
-  volatile int* abort_flag = &abort_word;
-  int x = blockIdx.x;
-  const int tile = x % a.tiles;
-  x /= a.tiles;
-  const int split = x % a.splits;
-  x /= a.splits;
-  const int hk = x % pool.Hkv, seq = x / pool.Hkv;
+  int x = div_by(blockIdx.x, a.tiles, a.inv_tiles);
+  const int tile = blockIdx.x - x * a.tiles, y = div_by(x, a.splits, a.inv_splits), split = x - y * a.splits;
+  const int seq = div_by(y, pool.Hkv, a.inv_hkv), hk = y - seq * pool.Hkv;
+  wait_previous();
+  release_next();
   // rows r of the tile: token r / G, head r % G of the key head's
   int t0, row, rows, start = 0, len = 0, tail = 0;
   unsigned long long bits = 0;
+  bool fine = true;
   if (TREE) {
     t0 = seq;
     row = a.row_seq[seq];
     rows = a.G;
-    if ((unsigned)row >= (unsigned)tk.table_rows) {
-      if (threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
-    } else {
+    fine = (unsigned)row < (unsigned)tk.table_rows;
+    if (fine) {
       len = a.seq_lens[row];
       tail = a.tail_start ? a.tail_start[seq] : len;
       bits = a.tail_mask ? a.tail_mask[seq] : 0;
@@ -322,255 +331,323 @@ __global__ void __launch_bounds__(FP8_WARPS * 32) fp8_attend_kernel(const __grid
     const int count = tk.cu[seq + 1] - t0;
     start = tk.start[seq];
     row = tk.rows[seq];
-    if (t0 < 0 || count < 0 || count > tk.T - t0 || start < 0) {
-      if (threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
-      return;
-    }
     rows = count * a.G;
-    if (rows > ROWS * a.tiles && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);       // more new tokens than the caller said
+    fine = t0 >= 0 && count >= 0 && count <= tk.T - t0 && start >= 0;
+    if (!fine) rows = 0;
+    if (rows > ROWS * a.tiles) fine = false;         // more new tokens than the caller said
   }
+  if (!fine && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
   const int r0 = tile * ROWS, nr = min(ROWS, rows - r0);
   if (nr <= 0) return;
-  const int first = start + r0 / a.G, last = start + (r0 + nr - 1) / a.G;       // positions of the tile's tokens
+  const int first = start + div_by(r0, a.G, a.inv_g), last = start + div_by(r0 + nr - 1, a.G, a.inv_g);       // positions of the tile's tokens
   const int hi = TREE ? len : last + 1, lo = !TREE && a.window > 0 ? max(0, first - a.window + 1) : 0;
   const int pg_lo = lo / FP8_PAGE, pg_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
   const int p0 = pg_lo + split * a.per_split, p1 = split + 1 < a.splits ? min(pg_hi, p0 + a.per_split) : pg_hi;    // the last one takes the rest
   if (split > 0 && p0 >= p1) return;
 
-  // ---- the warp's pages: its i-th is p0 + warp + NW i ----
-  // A lane keeps the number of one of 32 pages: `nf` of those that are fetched, ST - 1 pages ahead of `nc` with the scales of those that are worked on; the
-  // next 32 are looked up in between, so that neither look-up is waited for.
-  const int mine = p1 > p0 + warp ? (p1 - p0 - warp + NW - 1) / NW : 0;
-  auto number_of = [&](int i) { return i < mine ? pool_page(tk, pool.pages, row, p0 + warp + NW * i) : -1; };
+  // ---- the warp's pages: its step s takes p0 + 2 (warp + NW s) and the next ----
+  // A lane keeps the number of a page of sixteen steps: `nf` of those that are fetched, ST - 1 steps ahead of `nc` with the scales of those that are worked
+  // on; the next sixteen steps' are looked up in between, so that neither look-up is waited for.
+  const int steps = max(0, ((p1 - p0 + 1) / 2 - warp + NW - 1) / NW);
+  auto number_of = [&](int s) {                       // of step s + lane / 2
+    const int pg = p0 + 2 * (warp + NW * (s + (lane >> 1))) + (lane & 1);
+    return pg < p1 ? pool_page(tk, pool.pages, row, pg) : -1;
+  };
   auto scale_at = [&](const float* scales, int id) { return id >= 0 ? scales[(long)id * pool.Hkv + hk] : 0.f; };
-  uint8_t* const slots = ring + warp * ST * M::BYTES;
-  int nf = number_of(lane), nn = -1;
-  auto fetch = [&](int i) {                                       // page i into its slot
-    const int id = __shfl_sync(0xffffffffu, nf, i & 31);
-    if (lane == 0 && i < mine && id >= 0) {
-      uint64_t* bar = &full[warp][i % ST];
-      uint8_t* dst = slots + (i % ST) * M::BYTES;
-      const int line = (id * pool.Hkv + hk) * (FP8_PAGE * D / 128);
-      mbar_expect_tx(bar, M::BYTES);
-      tma_load_2d(dst, &tmap_k, bar, 0, line);
-      tma_load_2d(dst + FP8_PAGE * D, &tmap_v, bar, 0, line);
+  const uint32_t slots = smem_u32(ring) + warp * ST * SLOT;
+  const uint32_t even = M::at(lane * 16), odd = M::at((32 + lane) * 16) - 512;        // where a lane's piece of 512 bytes goes
+  int nf = number_of(0), nn = -1;
+  uint4 qraw[NR][KP][2];                              // the queries arrive with the pages' numbers
+#pragma unroll
+  for (int b = 0; b < NR; ++b) {
+    const int r = r0 + b * 8 + n, tok = div_by(r, a.G, a.inv_g);
+    const __nv_bfloat16* src = a.q + (t0 + tok) * a.ld_q + (hk * a.G + r - tok * a.G) * D + c * 16;
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) qraw[b][j][i] = b * 8 + n < nr ? *reinterpret_cast<const uint4*>(src + j * 64 + i * 8) : make_uint4(0, 0, 0, 0);
+  }
+  auto fetch = [&](int s) {                           // the pages of step s into their slot
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int id = __shfl_sync(0xffffffffu, nf, (2 * s + g) & 31);
+      if (s < steps && id >= 0) {
+        const long base = ((long)id * pool.Hkv + hk) * (FP8_PAGE * D) + lane * 16;
+        const uint8_t *ksrc = pool.k + base, *vsrc = pool.v + base;
+        const uint32_t dst = slots + (s % ST) * SLOT + g * M::BYTES;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          copy16_async(dst + q * 512 + (q & 1 ? odd : even), ksrc + q * 512);
+          copy16_async(dst + FP8_PAGE * D + q * 512 + (q & 1 ? odd : even), vsrc + q * 512);
+        }
+      }
     }
+    copies_commit();
   };
 #pragma unroll
-  for (int i = 0; i < ST - 1; ++i) fetch(i);
+  for (int s = 0; s < ST - 1; ++s) fetch(s);
   int nc = nf;
   float ksc = scale_at(pool.k_scale, nc), vsc = scale_at(pool.v_scale, nc), ksn = 0.f, vsn = 0.f;
 
-  // ---- queries: row n of a block of eight, as the second operand ----
-  uint32_t qb[NR][KS][2];
-  float qm[NR][2];                                                              // of this lane's columns: rows 2 c and 2 c + 1
-  int vlo[NR][2], vhi[NR][2];                                                   // positions that they see: [vlo, vhi)
+    // ---- queries: row n of a block of eight, as the second operand ----
+    uint32_t qb[NR][KS][2];
+    float qm[NR][2];                                                            // of this lane's columns: rows 2 c and 2 c + 1
+    int vlo[NR][2], vhi[NR][2];                                                 // positions that they see: [vlo, vhi)
 #pragma unroll
-  for (int b = 0; b < NR; ++b) {
-    const int r = r0 + b * 8 + n;
-    uint4 raw[KP][2];
-    uint32_t top = 0;
+    for (int b = 0; b < NR; ++b) {
+      uint4(&raw)[KP][2] = qraw[b];
+      uint32_t top = 0;
 #pragma unroll
-    for (int j = 0; j < KP; ++j)
+      for (int j = 0; j < KP; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        raw[j][i] = make_uint4(0, 0, 0, 0);
-        if (b * 8 + n < nr) raw[j][i] = *reinterpret_cast<const uint4*>(a.q + (t0 + r / a.G) * a.ld_q + (hk * a.G + r % a.G) * D + j * 64 + c * 16 + i * 8);
-        const uint32_t w[4] = {raw[j][i].x, raw[j][i].y, raw[j][i].z, raw[j][i].w};
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t w[4] = {raw[j][i].x, raw[j][i].y, raw[j][i].z, raw[j][i].w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-      }
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    const int ex = min(max((int)(top >> 7), 1), 253);                           // 2^(ex - 127): the row's largest value, but for its fraction
-    const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);
-#pragma unroll
-    for (int j = 0; j < KP; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 v = raw[j][i >> 1];
-        const uint32_t w0 = i & 1 ? v.z : v.x, w1 = i & 1 ? v.w : v.y;
-        qb[b][j * 4 + i][0] = half2_of(__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down);
-        qb[b][j * 4 + i][1] = half2_of(__uint_as_float(w1 << 16) * down, __uint_as_float(w1 & 0xffff0000u) * down);
-      }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      qm[b][e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4);
-      const int p = start + min(r0 + b * 8 + 2 * c + e, rows - 1) / a.G;
-      vhi[b][e] = TREE ? len : p + 1;
-      vlo[b][e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
-    }
-  }
-  const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;    // positions that every row sees
-
-  float o[NR][NI][4], m[NR][2], l[NR][2], vref = 0.f, vinv = 0.f;
-#pragma unroll
-  for (int b = 0; b < NR; ++b) {
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
-    m[b][0] = m[b][1] = -INFINITY;
-    l[b][0] = l[b][1] = 0.f;
-  }
-
-  bool ok = true;
-  for (int i = 0; i < mine; ++i) {
-    if ((i & 31) == 0) {
-      if (i > 0) {
-        nc = nf;
-        ksc = ksn;
-        vsc = vsn;
-      }
-      nn = number_of(i + 32 + lane);
-    }
-    if ((i & 31) == 16) {
-      ksn = scale_at(pool.k_scale, nn);
-      vsn = scale_at(pool.v_scale, nn);
-    }
-    if (((i + ST - 1) & 31) == 0) nf = nn;
-    const int id = __shfl_sync(0xffffffffu, nc, i & 31), pos = (p0 + warp + NW * i) * FP8_PAGE;
-    const float ks = __shfl_sync(0xffffffffu, ksc, i & 31), vs = __shfl_sync(0xffffffffu, vsc, i & 31);
-    fetch(i + ST - 1);                               // into the slot of page i - 1, which every lane has read
-    if (id < 0) continue;
-    if (!mbar_wait_warp(&full[warp][i % ST], (i / ST) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) {
-      ok = false;
-      break;
-    }
-    const uint8_t* page = slots + (i % ST) * M::BYTES;
-    // ---- scores: 16 tokens x 8 rows ----
-    float s[NR][4];
-#pragma unroll
-    for (int b = 0; b < NR; ++b)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) s[b][e] = 0.f;
-#pragma unroll
-    for (int q = 0; q < KP; ++q) {
-      const uint4 x4 = *reinterpret_cast<const uint4*>(page + M::at(M::slot(0, n) * D + q * 64 + c * 16));
-      const uint4 y4 = *reinterpret_cast<const uint4*>(page + M::at(M::slot(1, n) * D + q * 64 + c * 16));
-      const uint32_t xs[4] = {x4.x, x4.y, x4.z, x4.w}, ys[4] = {y4.x, y4.y, y4.z, y4.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t k0 = half2_of_e4m3x2(xs[k]), k1 = half2_of_e4m3x2(ys[k]), k2 = half2_of_e4m3x2(xs[k] >> 16), k3 = half2_of_e4m3x2(ys[k] >> 16);
-#pragma unroll
-        for (int b = 0; b < NR; ++b) mma_f16(s[b], k0, k1, k2, k3, qb[b][q * 4 + k][0], qb[b][q * 4 + k][1]);
-      }
-    }
-    const bool whole = pos >= all_lo && pos + FP8_PAGE <= all_hi;
-    bool over = vs > vref;
-#pragma unroll
-    for (int b = 0; b < NR; ++b)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        s[b][e] *= qm[b][e & 1] * ks;
-        if (!whole) {
-          const int at = pos + M::slot(e >> 1, n);
-          bool seen = at >= vlo[b][e & 1] && at < vhi[b][e & 1];
-          if (TREE) seen = seen && (at < tail || (at - tail < 64 && ((bits >> ((at - tail) & 63)) & 1ull)));
-          if (!seen) s[b][e] = -INFINITY;
+          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
         }
-        over |= s[b][e] > m[b][e & 1] + SLACK;
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int ex = min(max((int)(top >> 7), 1), 253);                         // 2^(ex - 127): the row's largest value, but for its fraction
+      const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+      for (int j = 0; j < KP; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 v = raw[j][i >> 1];
+          const uint32_t w0 = i & 1 ? v.z : v.x, w1 = i & 1 ? v.w : v.y;
+          qb[b][j * 4 + i][0] = half2_of(__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down);
+          qb[b][j * 4 + i][1] = half2_of(__uint_as_float(w1 << 16) * down, __uint_as_float(w1 & 0xffff0000u) * down);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qm[b][e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4);
+        const int p = start + div_by(min(r0 + b * 8 + 2 * c + e, rows - 1), a.G, a.inv_g);
+        vhi[b][e] = TREE ? len : p + 1;
+        vlo[b][e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
       }
-    if (__any_sync(0xffffffffu, over)) {
-      const float beta = vs > vref ? vref / vs : 1.f;
-      if (vs > vref) {
-        vref = vs;
-        vinv = 1.f / vs;
+    }
+    const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;  // positions that every row sees
+
+    float o[NR][NI][4], m[NR][2], l[NR][2], vref = 0.f, vinv = 0.f;
+#pragma unroll
+    for (int b = 0; b < NR; ++b) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
+      m[b][0] = m[b][1] = -INFINITY;
+      l[b][0] = l[b][1] = 0.f;
+    }
+
+    for (int st = 0; st < steps; ++st) {
+      if ((st & 15) == 0) {
+        if (st > 0) {
+          nc = nf;
+          ksc = ksn;
+          vsc = vsn;
+        }
+        nn = number_of(st + 16);
+      }
+      if ((st & 15) == 8) {
+        ksn = scale_at(pool.k_scale, nn);
+        vsn = scale_at(pool.v_scale, nn);
+      }
+      if (((st + ST - 1) & 15) == 0) nf = nn;
+      const int at0 = (2 * st) & 31, there = (__ballot_sync(0xffffffffu, nc >= 0) >> at0) & 3, pos = (p0 + 2 * (warp + NW * st)) * FP8_PAGE;
+      const float ks[2] = {__shfl_sync(0xffffffffu, ksc, at0), __shfl_sync(0xffffffffu, ksc, at0 + 1)};
+      const float vs[2] = {__shfl_sync(0xffffffffu, vsc, at0), __shfl_sync(0xffffffffu, vsc, at0 + 1)};
+      fetch(st + ST - 1);                              // into the slot of step st - 1, which every lane has read
+      copies_wait<ST - 1>();
+      __syncwarp();
+      const uint32_t pages = slots + (st % ST) * SLOT;
+      // ---- scores: 2 x 16 tokens x 8 rows ----
+      float s[NR][2][4];
+#pragma unroll
+      for (int b = 0; b < NR; ++b)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[b][g][e] = 0.f;
+#pragma unroll
+      for (int q = 0; q < KP; ++q) {
+        uint32_t xs[2][4], ys[2][4];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const uint4 x4 = shared16(pages + g * M::BYTES + M::at(M::slot(0, n) * D + q * 64 + c * 16));
+          const uint4 y4 = shared16(pages + g * M::BYTES + M::at(M::slot(1, n) * D + q * 64 + c * 16));
+          xs[g][0] = x4.x; xs[g][1] = x4.y; xs[g][2] = x4.z; xs[g][3] = x4.w;
+          ys[g][0] = y4.x; ys[g][1] = y4.y; ys[g][2] = y4.z; ys[g][3] = y4.w;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const uint32_t k0 = half2_of_e4m3x2(xs[g][k]), k1 = half2_of_e4m3x2(ys[g][k]), k2 = half2_of_e4m3x2(xs[g][k] >> 16),
+                           k3 = half2_of_e4m3x2(ys[g][k] >> 16);
+#pragma unroll
+            for (int b = 0; b < NR; ++b) mma_f16(s[b][g], k0, k1, k2, k3, qb[b][q * 4 + k][0], qb[b][q * 4 + k][1]);
+          }
+      }
+      const bool whole = pos >= all_lo && pos + 2 * FP8_PAGE <= all_hi && there == 3;
+      bool over = fmaxf(vs[0], vs[1]) > vref;
+#pragma unroll
+      for (int b = 0; b < NR; ++b)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const float f0 = qm[b][0] * ks[g], f1 = qm[b][1] * ks[g];
+          s[b][g][0] *= f0;
+          s[b][g][1] *= f1;
+          s[b][g][2] *= f0;
+          s[b][g][3] *= f1;
+        }
+      uint32_t hidden = 0;
+      if (!whole) {
+        rarely();
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int at = pos + g * FP8_PAGE + M::slot(e >> 1, n);
+              bool seen = at >= vlo[b][e & 1] && at < vhi[b][e & 1] && ((there >> g) & 1);
+              if (TREE) seen = seen && (at < tail || (at - tail < 64 && ((bits >> ((at - tail) & 63)) & 1ull)));
+              if (!seen) {
+                s[b][g][e] = -INFINITY;
+                hidden |= 1u << (b * 8 + g * 4 + e);
+              }
+            }
       }
 #pragma unroll
-      for (int b = 0; b < NR; ++b) {
-        float alpha[2];
+      for (int b = 0; b < NR; ++b)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(s[b][e], s[b][2 + e]);
-#pragma unroll
-          for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float up = fmaxf(m[b][e], mx);
-          alpha[e] = up == m[b][e] ? 1.f : exp2_fast(m[b][e] - up);
-          m[b][e] = up;
-          l[b][e] *= alpha[e];
-          alpha[e] *= beta;
+          const float top = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
+          over |= top > m[b][e] + SLACK;
+        }
+      if (__any_sync(0xffffffffu, over)) {
+        const float v_up = fmaxf(vs[0], vs[1]), beta = v_up > vref ? vref / v_up : 1.f;
+        if (v_up > vref) {
+          vref = v_up;
+          vinv = 1.f / v_up;
         }
 #pragma unroll
-        for (int k = 0; k < NI; ++k)
+        for (int b = 0; b < NR; ++b) {
+          float alpha[2];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[e & 1];
+          for (int e = 0; e < 2; ++e) {
+            float mx = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+            const float up = fmaxf(m[b][e], mx);
+            alpha[e] = up == m[b][e] ? 1.f : exp2_fast(m[b][e] - up);
+            m[b][e] = up;
+            l[b][e] *= alpha[e];
+            alpha[e] *= beta;
+          }
+#pragma unroll
+          for (int k = 0; k < NI; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[e & 1];
+        }
       }
+      const float rel[2] = {vs[0] * vinv, vs[1] * vinv};
+      float xw[NR][2][4];                              // weights times their page's scale
+#pragma unroll
+      for (int b = 0; b < NR; ++b) {
+        const float m0 = m[b][0] - LIFT, m1 = m[b][1] - LIFT;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[b][g][e] = exp2_fast(s[b][g][e] - (e & 1 ? m1 : m0));
+            xw[b][g][e] = s[b][g][e] * rel[g];
+          }
+      }
+      if (!whole) {                                    // nothing of a hidden place, whatever its scale and however little the row has seen
+        rarely();
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if ((hidden >> (b * 8 + g * 4 + e)) & 1) s[b][g][e] = xw[b][g][e] = 0.f;
+      }
+      uint32_t pb[NR][2][2];                           // weights of row n: tokens of rows 2 c, 2 c + 1 (and + 8) of the score product
+#pragma unroll
+      for (int b = 0; b < NR; ++b) {
+        l[b][0] += (s[b][0][0] + s[b][0][2]) + (s[b][1][0] + s[b][1][2]);
+        l[b][1] += (s[b][0][1] + s[b][0][3]) + (s[b][1][1] + s[b][1][3]);
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) pb[b][g][h] = transpose8(half2_of(xw[b][g][2 * h], xw[b][g][2 * h + 1]));
+      }
+      // ---- values: dimensions x 8 rows ----
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint32_t v[4][VW];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int tok = M::slot(r >> 1, 2 * c + (r & 1));
+          const uint32_t src = pages + g * M::BYTES + FP8_PAGE * D + M::at(tok * D + M::col(n));
+          if (D == 128) {
+            const uint4 w = shared16(src);
+            v[r][0] = w.x; v[r][1] = w.y; v[r][VW - 2] = w.z; v[r][VW - 1] = w.w;
+          } else {
+            const uint2 w = shared8(src);
+            v[r][0] = w.x; v[r][1] = w.y;
+          }
+        }
+        if (!whole) {                                   // slots past the end hold whatever was there
+          rarely();
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (pos + g * FP8_PAGE + M::slot(r >> 1, 2 * c + (r & 1)) >= hi || !((there >> g) & 1)) {
+#pragma unroll
+              for (int q = 0; q < VW; ++q) v[r][q] = 0;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < VW; ++q) {                  // four dimensions of the lane: two products, rows n and n + 8 one dimension each
+          const uint32_t a01 = __byte_perm(v[0][q], v[1][q], 0x5140), b01 = __byte_perm(v[0][q], v[1][q], 0x7362);
+          const uint32_t a23 = __byte_perm(v[2][q], v[3][q], 0x5140), b23 = __byte_perm(v[2][q], v[3][q], 0x7362);
+          const uint32_t va[4] = {half2_of_e4m3x2(a01), half2_of_e4m3x2(a01 >> 16), half2_of_e4m3x2(a23), half2_of_e4m3x2(a23 >> 16)};
+          const uint32_t vb[4] = {half2_of_e4m3x2(b01), half2_of_e4m3x2(b01 >> 16), half2_of_e4m3x2(b23), half2_of_e4m3x2(b23 >> 16)};
+#pragma unroll
+          for (int b = 0; b < NR; ++b) {
+            mma_f16(o[b][2 * q], va[0], va[1], va[2], va[3], pb[b][g][0], pb[b][g][1]);
+            mma_f16(o[b][2 * q + 1], vb[0], vb[1], vb[2], vb[3], pb[b][g][0], pb[b][g][1]);
+          }
+        }
+      }
+      __syncwarp();
     }
-    const float rel = vs * vinv;
-    uint32_t pb[NR][2];                              // weights of rows n: tokens of rows 2 c, 2 c + 1 (and + 8) of the score product
+
+    // ---- the warps' shares, each in its own part of the ring ----
+    constexpr int SHARE = ST * SLOT / 4;               // floats of a warp's part; ROWS x D are used
+    static_assert(ROWS * D <= SHARE, "sums fit the ring");
+    float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float w0 = exp2_fast(s[b][2 * h] - m[b][0] + LIFT), w1 = exp2_fast(s[b][2 * h + 1] - m[b][1] + LIFT), x0 = w0 * rel, x1 = w1 * rel;
-        if (!whole) {                                 // nothing of a hidden place, whatever its scale and however little the row has seen
-          if (s[b][2 * h] == -INFINITY) w0 = x0 = 0.f;
-          if (s[b][2 * h + 1] == -INFINITY) w1 = x1 = 0.f;
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int d = 4; d < 32; d *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
+        const int r = b * 8 + 2 * c + e;
+        if (n == 0) {
+          sm_m[warp][r] = m[b][e];
+          sm_l[warp][r] = l[b][e];
         }
-        l[b][0] += w0;
-        l[b][1] += w1;
-        pb[b][h] = transpose8(half2_of(x0, x1));
+        if (r < nr) {
+          float* to = sums + warp * SHARE + r * D + M::col(n);
+#pragma unroll
+          for (int k = 0; k < NI; k += 2)
+            *reinterpret_cast<float4*>(to + 2 * k) =
+                make_float4(o[b][k][e] * vref, o[b][k][2 + e] * vref, o[b][k + 1][e] * vref, o[b][k + 1][2 + e] * vref);
+        }
       }
-    // ---- values: dimensions x 8 rows ----
-    uint32_t v[4][VW];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int slot = M::slot(r >> 1, 2 * c + (r & 1));
-      const uint8_t* src = page + FP8_PAGE * D + M::at(slot * D + M::col(n));
-      if (D == 128) {
-        const uint4 w = *reinterpret_cast<const uint4*>(src);
-        v[r][0] = w.x; v[r][1] = w.y; v[r][VW - 2] = w.z; v[r][VW - 1] = w.w;
-      } else {
-        const uint2 w = *reinterpret_cast<const uint2*>(src);
-        v[r][0] = w.x; v[r][1] = w.y;
-      }
-      if (!whole && pos + slot >= hi) {               // slots past the end hold whatever was there
-#pragma unroll
-        for (int q = 0; q < VW; ++q) v[r][q] = 0;
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < VW; ++q) {                    // four dimensions of the lane: two products, rows n and n + 8 one dimension each
-      const uint32_t a01 = __byte_perm(v[0][q], v[1][q], 0x5140), b01 = __byte_perm(v[0][q], v[1][q], 0x7362);
-      const uint32_t a23 = __byte_perm(v[2][q], v[3][q], 0x5140), b23 = __byte_perm(v[2][q], v[3][q], 0x7362);
-      const uint32_t va[4] = {half2_of_e4m3x2(a01), half2_of_e4m3x2(a01 >> 16), half2_of_e4m3x2(a23), half2_of_e4m3x2(a23 >> 16)};
-      const uint32_t vb[4] = {half2_of_e4m3x2(b01), half2_of_e4m3x2(b01 >> 16), half2_of_e4m3x2(b23), half2_of_e4m3x2(b23 >> 16)};
-#pragma unroll
-      for (int b = 0; b < NR; ++b) {
-        mma_f16(o[b][2 * q], va[0], va[1], va[2], va[3], pb[b][0], pb[b][1]);
-        mma_f16(o[b][2 * q + 1], vb[0], vb[1], vb[2], vb[3], pb[b][0], pb[b][1]);
-      }
-    }
-    __syncwarp();                                    // the slot may be filled again
-  }
-  if (!ok) {                                         // a copy did not arrive in time: the status word says so; what is on its way lands first
-    const uint64_t since = globaltimer_ns();
-    while (globaltimer_ns() - since < 2000000ull) __nanosleep(1000);
-  }
-
-  // ---- the warps' shares, each in its own part of the ring ----
-  constexpr int SHARE = ST * M::BYTES / 4;           // floats of a warp's part; ROWS x D are used
-  static_assert(ROWS * D <= SHARE, "sums fit the ring");
-  float* sums = reinterpret_cast<float*>(ring);
-#pragma unroll
-  for (int b = 0; b < NR; ++b)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-#pragma unroll
-      for (int d = 4; d < 32; d *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
-      const int r = b * 8 + 2 * c + e;
-      if (n == 0) {
-        sm_m[warp][r] = m[b][e];
-        sm_l[warp][r] = l[b][e];
-      }
-      if (r < nr) {
-        float* to = sums + warp * SHARE + r * D + M::col(n);
-#pragma unroll
-        for (int k = 0; k < NI; k += 2)
-          *reinterpret_cast<float4*>(to + 2 * k) = make_float4(o[b][k][e] * vref, o[b][k][2 + e] * vref, o[b][k + 1][e] * vref, o[b][k + 1][2 + e] * vref);
-      }
-    }
   __syncthreads();
   for (int i = threadIdx.x; i < nr * (D / 4); i += NW * 32) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
@@ -585,7 +662,7 @@ __global__ void __launch_bounds__(FP8_WARPS * 32) fp8_attend_kernel(const __grid
       acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f;
       ll += sm_l[w][r] * f;
     }
-    const int t = t0 + (r0 + r) / a.G, hd = hk * a.G + (r0 + r) % a.G;
+    const int tok = div_by(r0 + r, a.G, a.inv_g), t = t0 + tok, hd = hk * a.G + r0 + r - tok * a.G;
     if (a.splits == 1) {
       const float inv = ll == 0.f ? 0.f : 1.f / ll;
       *reinterpret_cast<uint2*>(a.out + t * a.ld_o + hd * D + d) = make_uint2(cvt_bf16x2(acc[0] * inv, acc[1] * inv), cvt_bf16x2(acc[2] * inv, acc[3] * inv));
@@ -601,14 +678,17 @@ __global__ void __launch_bounds__(FP8_WARPS * 32) fp8_attend_kernel(const __grid
   }
 }
 
-// Joins the splits of a row: a warp a row and head, D / 32 values a lane.
-template <int D>
+// Joins the splits of a row (a query token's head), D / 32 values a lane. WIDE: a CTA a row, whose warps share the splits; else a warp a row. With 63
+// splits of 32 rows a warp a row took most of 24 us.
+template <int D, bool WIDE>
 __global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__ part, const float* __restrict__ part_ml, const int* __restrict__ used,
                                                        __nv_bfloat16* __restrict__ out, long ld_o, int T, int H, int splits) {
-  constexpr int E = D / 32;
+  constexpr int E = D / 32, NW = WIDE ? 8 : 1;
+  __shared__ float sm_l[8], sm_o[8][D];
   wait_previous();
-  const long item = blockIdx.x * 8l + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+  release_next();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long item = WIDE ? blockIdx.x : blockIdx.x * 8l + warp;
   if (item >= (long)T * H) return;
   const float* base = part + item * splits * D + lane * E;
   const float* ml = part_ml + item * splits * 2;
@@ -621,11 +701,27 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < ns; ++s) {
+  for (int s = WIDE ? warp : 0; s < ns; s += NW) {
     const float f = mm == -INFINITY ? 1.f : exp2_fast(ml[2 * s] - mm);
     ll += ml[2 * s + 1] * f;
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] += base[(long)s * D + i] * f;
+  }
+  if (WIDE) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) sm_o[warp][lane * E + i] = acc[i];
+    if (lane == 0) sm_l[warp] = ll;
+    __syncthreads();
+    if (warp) return;
+    ll = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      ll += sm_l[w];
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[i] += sm_o[w][lane * E + i];
+    }
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
   uint32_t* to = reinterpret_cast<uint32_t*>(out + item / H * ld_o + item % H * D + lane * E);
@@ -638,8 +734,7 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__
 using namespace inv;
 
 static bool fp8_bad_shape(int H, int Hkv, int D, int pages, int n, int T, int table_rows, int max_pages) {
-  // the lines of a pool are numbered in 31 bits
-  return (D != 64 && D != 128) || (long)pages * Hkv * (FP8_PAGE * D / 128) > 0x7fffffffl || Hkv < 1 || H < Hkv || H % Hkv || pages < 1 || n < 0 || T < 0 || table_rows < 1 || max_pages < 1;
+  return (D != 64 && D != 128) || Hkv < 1 || H < Hkv || H % Hkv || pages < 1 || n < 0 || T < 0 || table_rows < 1 || max_pages < 1;
 }
 static bool off16(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
   return ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16 != 0;
@@ -661,24 +756,34 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   const Fp8Tokens tk{rows, cu, start, page_table, n, T, table_rows, max_pages, status};
   const unsigned ctas = (unsigned)(T / FP8_PAGE + 2 * n);
   const dim3 grid(ctas, 1);
-  if (D == 64) fp8_append_kernel<64><<<grid, 256, 0, (cudaStream_t)stream>>>(a, pool, tk);
-  else fp8_append_kernel<128><<<grid, 256, 0, (cudaStream_t)stream>>>(a, pool, tk);
+  if (D == 64) launch_early(fp8_append_kernel<64>, grid, 256, 0, (cudaStream_t)stream, a, pool, tk);
+  else launch_early(fp8_append_kernel<128>, grid, 256, 0, (cudaStream_t)stream, a, pool, tk);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
-// How an attention is cut: row tiles of a sequence, pages of a CTA, CTAs along a sequence.
+// How an attention is cut: rows of a tile (8 `blocks`), warps and pages of a CTA, CTAs along a sequence.
 struct Fp8Cut {
-  int blocks, tiles, per, splits;      // blocks: of eight rows in a tile
+  int blocks, tiles, warps, per, splits;
   Fp8Cut(int n, int Hkv, int G, int max_new, int max_len, int window) {
     blocks = (long)max_new * G <= 8 ? 1 : 2;
     tiles = (int)(((long)max_new * G + 8 * blocks - 1) / (8 * blocks));
     const long span = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
-    const int pages = (int)((span + 2 * FP8_PAGE - 2) / FP8_PAGE);
-    const long units = (long)n * Hkv * tiles, target = 148 * 12;
-    per = (int)((units * pages + target - 1) / target);
-    if (per < 32) per = 32;
-    if (per > pages) per = pages;
+    const int pages = (int)((span + (window > 0 ? 2 * FP8_PAGE - 2 : FP8_PAGE - 1)) / FP8_PAGE);       // a window may begin inside a page
+    const long units = (long)n * Hkv * tiles;
+    // Joining the splits costs about three microseconds, and a CTA as much before its first and behind its last page, so up to 64 pages stay together (64 x
+    // 640 tokens, 512 units: 22.3 us, in two parts 25.9; 16 x 4 on 1000: 14.4 and 17.1). Longer ones are cut for two CTAs an SM, in parts of 16 pages or more
+    // (2000 tokens, 16 units: 16 / 32 / 64 / 126 pages 7.5, 9.6, 12.1, 15.3 us; 32000, 8 units: 24 / 64 / 128 pages 23.5, 17.8, 19.9) and of about 128 where
+    // there are many, which evens unequal lengths out (8 of up to 65000: 128 pages 71.7 us, 512 91.1). Where units alone fill the GPU several times, CTAs of
+    // two warps, which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251 90.1 and 106.6).
+    const bool many = blocks == 1 && units > 444 && pages <= 256;
+    warps = many ? 2 : 4;
+    const long total = units * pages;
+    long want = (total + 295) / 296;
+    if (want > 128) want = total / 1184 > 128 ? total / 1184 : 128;
+    if (want < 16) want = 16;
+    if (many || pages <= 64 || want > pages) want = pages;
+    per = want < pages ? (int)((want + 1) & ~1l) : pages;          // warps take two
     splits = (pages + per - 1) / per;
   }
 };
@@ -689,46 +794,23 @@ extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int m
   return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
 }
 
-// The codes of a pool as lines of 128 bytes, read a page of a head at a time with the pieces of a line exchanged.
-static int fp8_tensor_map(CUtensorMap* out, const uint8_t* codes, long pages_heads, int D) {
-  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static std::atomic<Encode> known{nullptr};
-  bind_context();
-  Encode encode = known.load();
-  if (!encode) {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) return -1;
-    encode = reinterpret_cast<Encode>(f);
-    known.store(encode);
-  }
-  const cuuint32_t lines = FP8_PAGE * D / 128;
-  const cuuint64_t dims[2] = {128, (cuuint64_t)pages_heads * lines}, strides[1] = {128};
-  const cuuint32_t box[2] = {128, lines}, steps[2] = {1, 1};
-  const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : -(int)r - 1000;
-}
-
-template <int D, int NR, bool TREE>
+template <int D, int NR, int NW, bool TREE>
 static int fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
-  constexpr int SMEM = fp8_attend_smem<D>();
+  constexpr int SMEM = fp8_attend_smem<D, NW>();
   static std::atomic<uint64_t> ready{0};                           // devices whose limit has been raised
   int device = 0;
   cudaGetDevice(&device);
   const uint64_t bit = 1ull << (device & 63);
   if (!(ready.load() & bit)) {
-    cudaFuncSetAttribute(fp8_attend_kernel<D, NR, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    cudaFuncSetAttribute(fp8_attend_kernel<D, NR, NW, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     ready.fetch_or(bit);
   }
-  CUtensorMap mk, mv;
-  if (int rc = fp8_tensor_map(&mk, pool.k, (long)pool.pages * pool.Hkv, D)) return rc;
-  if (int rc = fp8_tensor_map(&mv, pool.v, (long)pool.pages * pool.Hkv, D)) return rc;
-  fp8_attend_kernel<D, NR, TREE><<<ctas, FP8_WARPS * 32, SMEM, st>>>(mk, mv, a, pool, tk);
-  if (a.splits > 1)
-    launch_early(fp8_join_kernel<D>, dim3((unsigned)(((long)tk.T * a.H + 7) / 8)), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, tk.T, a.H,
-                 a.splits);
+  launch_early(fp8_attend_kernel<D, NR, NW, TREE>, dim3(ctas), NW * 32, SMEM, st, a, pool, tk);
+  const long items = (long)tk.T * a.H;
+  if (a.splits > 4)
+    launch_early(fp8_join_kernel<D, true>, dim3((unsigned)items), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, tk.T, a.H, a.splits);
+  else if (a.splits > 1)
+    launch_early(fp8_join_kernel<D, false>, dim3((unsigned)((items + 7) / 8)), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, tk.T, a.H, a.splits);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
@@ -739,6 +821,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
   a.tiles = cut.tiles;
   a.per_split = cut.per;
   a.splits = cut.splits;
+  a.inv_tiles = div_reciprocal(a.tiles); a.inv_splits = div_reciprocal(a.splits); a.inv_hkv = div_reciprocal(pool.Hkv); a.inv_g = div_reciprocal(a.G);
   if (cut.splits > 1) {
     if (!work || off16(work)) return -ERR_BAD_ARG;
     const long rows = (long)tk.T * a.H * cut.splits;
@@ -749,11 +832,14 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;
   const unsigned grid = (unsigned)ctas;
-#define INV_FP8(DD)                                                                                                                        \
-  if (a.row_seq) return cut.blocks == 1 ? fp8_attend_launch<DD, 1, true>(a, pool, tk, grid, st) : fp8_attend_launch<DD, 2, true>(a, pool, tk, grid, st); \
-  return cut.blocks == 1 ? fp8_attend_launch<DD, 1, false>(a, pool, tk, grid, st) : fp8_attend_launch<DD, 2, false>(a, pool, tk, grid, st)
-  if (D == 64) { INV_FP8(64); }
-  INV_FP8(128);
+#define INV_FP8(DD, TREE)                                                        \
+  return cut.blocks == 2  ? fp8_attend_launch<DD, 2, 4, TREE>(a, pool, tk, grid, st) \
+         : cut.warps == 4 ? fp8_attend_launch<DD, 1, 4, TREE>(a, pool, tk, grid, st) \
+                          : fp8_attend_launch<DD, 1, 2, TREE>(a, pool, tk, grid, st)
+  if (D == 64 && a.row_seq) INV_FP8(64, true);
+  if (D == 64) INV_FP8(64, false);
+  if (a.row_seq) INV_FP8(128, true);
+  INV_FP8(128, false);
 #undef INV_FP8
 }
 
