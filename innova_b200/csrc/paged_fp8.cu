@@ -678,6 +678,363 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   }
 }
 
+// ---------------------------------------------------------------------------------------------- attention of many rows
+__host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t M, uint32_t N, uint32_t b_mn_major) {
+  return (1u << 4) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);        // fp32 sums of fp16 operands
+}
+
+constexpr int FT_M = 128, FT_N = 128, FT_PAGES = FT_N / FP8_PAGE;
+constexpr int FT_THREADS = 288;        // four warps of softmax, one that issues the products, four that convert
+template <int D>
+struct FtSmem {
+  static constexpr int TILE = FT_M * D * 2;          // fp16 rows in pieces of 64 columns with the 128-byte swizzle: queries, keys, values
+  static constexpr int TOTAL = 3 * TILE + 1024;
+};
+
+// 128 rows (query tokens times the heads that share a key head) against blocks of 128 keys on the tcgen05 tensor cores: prompts behind a cache, and drafts of
+// more than a few tokens. grid = row tiles (the longest first) x splits x key heads x sequences, two CTAs an SM.
+//   warps 0-3  softmax, a row a thread: scores from tensor memory, weights in fp16 back in their place, in two passes of 32 columns at a time
+//   warp 4     one thread issues S = Q K^T and O += P V (P from tensor memory)
+//   warps 5-8  codes of the next block from the pages to registers, as fp16 to shared memory
+// Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are powers of two added to it (relative to the
+// largest one so far, which O is kept in) and taken out of the row sum again a page at a time, so neither costs anything a score. For the rest the sums are
+// those of the small kernel. One CTA's softmax runs under the other's products.
+template <int D>
+__global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
+                                                                        const __grid_constant__ Fp8Tokens tk) {
+  using L = FtSmem<D>;
+  constexpr int CH = D / 16;             // 16-byte pieces of a token's codes
+  constexpr float LIFT = 6.f, SLACK = 8.f;
+  constexpr uint32_t O_COL = 128, COLS = 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sQ = smem, *sK = smem + L::TILE, *sV = smem + 2 * L::TILE;
+  __shared__ __align__(8) uint64_t bars[10];
+  __shared__ float2 scales[2][FT_PAGES];             // of a block's pages: keys, values
+  __shared__ uint32_t present[2];                    // bit p: page p of the block is there
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 2, *v_full = bars + 3, *v_empty = bars + 4, *s_full = bars + 5, *p_full = bars + 6,
+           *o_full = bars + 7, *scales_full = bars + 8;          // two: scales of even and odd blocks
+  volatile int* abort_flag = &abort_word;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = div_by(blockIdx.x, a.tiles, a.inv_tiles);
+  const int tile = a.tiles - 1 - (blockIdx.x - x * a.tiles), y = div_by(x, a.splits, a.inv_splits), split = x - y * a.splits;
+  const int seq = div_by(y, pool.Hkv, a.inv_hkv), hk = y - seq * pool.Hkv;
+  wait_previous();
+  release_next();
+  const int t0 = tk.cu[seq], count = tk.cu[seq + 1] - t0, start = tk.start[seq], row = tk.rows[seq];
+  const bool fine = t0 >= 0 && count >= 0 && count <= tk.T - t0 && start >= 0;
+  const int rows = fine ? count * a.G : 0;
+  if ((!fine || rows > FT_M * a.tiles) && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
+  const int r0 = tile * FT_M, nr = min(FT_M, rows - r0);
+  if (nr <= 0) return;
+  const int first = start + div_by(r0, a.G, a.inv_g), last = start + div_by(r0 + nr - 1, a.G, a.inv_g);
+  const int hi = last + 1, lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
+  // key blocks start at whole blocks of the sequence; per_split is a multiple of a block's pages
+  const int b_lo = lo / FT_N, b_hi = (hi + FT_N - 1) / FT_N, per = a.per_split / FT_PAGES;
+  const int b0 = b_lo + split * per, b1 = split + 1 < a.splits ? min(b_hi, b0 + per) : b_hi;
+  if (split > 0 && b0 >= b1) return;
+  const int nb = b1 - b0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 4);
+    mbar_init(k_full, 4);
+    mbar_init(k_empty, 1);
+    mbar_init(v_full, 4);
+    mbar_init(v_empty, 1);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, 4);
+    mbar_init(o_full, 1);
+    mbar_init(scales_full, 1);
+    mbar_init(scales_full + 1, 1);
+    abort_word = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(&tmem_slot, COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp >= 5) {
+    // ---------------- conversion: a thread takes the same piece of every eighth (D = 64: every second) token ----------------
+    const int tid = threadIdx.x - 160;
+    constexpr int PER = FT_N * CH / 128;             // pieces of a thread in a block: 8 or 4
+    const int piece = tid % CH, tok0 = tid / CH;     // its tokens: tok0 + i * (128 / CH)
+    constexpr int STEP = 128 / CH;
+    uint4 kr[PER], vr[PER];
+    int id = -1;                                     // lanes 0 to 7: page of the block in hand
+    auto look_up = [&](int j) { id = lane < FT_PAGES && j < nb && (b0 + j) * FT_PAGES + lane < (hi + FP8_PAGE - 1) / FP8_PAGE
+                                         ? pool_page(tk, pool.pages, row, (b0 + j) * FT_PAGES + lane) : -1; };
+    auto load = [&](const uint8_t* codes, uint4 (&r)[PER], int ids, int j, bool values) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int tok = tok0 + i * STEP, pid = __shfl_sync(0xffffffffu, ids, tok / FP8_PAGE);
+        const bool live = pid >= 0 && j < nb && !(values && (b0 + j) * FT_N + tok >= hi);       // values past the end are nothing, whatever is there
+        r[i] = live ? *reinterpret_cast<const uint4*>(codes + (((long)pid * pool.Hkv + hk) * FP8_PAGE + tok % FP8_PAGE) * D + piece * 16)
+                    : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto store = [&](uint8_t* dst, const uint4 (&r)[PER]) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int tok = tok0 + i * STEP, at = 2 * piece;                          // 16-byte pieces `at` and `at` + 1 of the token's fp16 row
+        uint8_t* line = dst + (at >> 3) * (FT_N * 128) + tok * 128;
+        const uint4 h0 = make_uint4(half2_of_e4m3x2(r[i].x), half2_of_e4m3x2(r[i].x >> 16), half2_of_e4m3x2(r[i].y), half2_of_e4m3x2(r[i].y >> 16));
+        const uint4 h1 = make_uint4(half2_of_e4m3x2(r[i].z), half2_of_e4m3x2(r[i].z >> 16), half2_of_e4m3x2(r[i].w), half2_of_e4m3x2(r[i].w >> 16));
+        const bool odd = piece >= CH / 2;                                        // lanes of the second half store in the other order: no bank twice
+        *reinterpret_cast<uint4*>(line + ((((at & 7) + (odd ? 1 : 0)) ^ (tok & 7)) << 4)) = odd ? h1 : h0;
+        *reinterpret_cast<uint4*>(line + ((((at & 7) + (odd ? 0 : 1)) ^ (tok & 7)) << 4)) = odd ? h0 : h1;
+      }
+    };
+    auto publish = [&](uint64_t* bar) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    look_up(0);
+    int ids = id;
+    load(pool.k, kr, ids, 0, false);
+    load(pool.v, vr, ids, 0, true);
+    for (int j = 0; j < nb; ++j) {
+      float2 sc = make_float2(0.f, 0.f);
+      const uint32_t there = __ballot_sync(0xffffffffu, ids >= 0);
+      if (warp == 5 && ids >= 0) {
+        sc.x = pool.k_scale[(long)ids * pool.Hkv + hk];
+        sc.y = pool.v_scale[(long)ids * pool.Hkv + hk];
+      }
+      look_up(j + 1);
+      if (!mbar_wait_warp(k_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
+      store(sK, kr);
+      if (warp == 5) {
+        if (lane < FT_PAGES) scales[j & 1][lane] = sc;
+        if (lane == 0) present[j & 1] = there;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(scales_full + (j & 1));
+      }
+      publish(k_full);
+      load(pool.k, kr, id, j + 1, false);
+      if (!mbar_wait_warp(v_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
+      store(sV, vr);
+      publish(v_full);
+      load(pool.v, vr, id, j + 1, true);
+      ids = id;
+    }
+  } else if (warp == 4) {
+    if (elect_one_sync()) {
+      const uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
+      const uint32_t qb = smem_u32(sQ), kb = smem_u32(sK), vb = smem_u32(sV);
+      bool ok = mbar_wait(q_full, 0, abort_flag, tk.status, ERR_WAIT_FULL);
+      for (int j = 0; ok && j < nb; ++j) {
+        // the scores take the place of the last block's weights, which its product has read
+        if (!mbar_wait(k_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) break;
+        if (j > 0 && !mbar_wait(o_full, (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint32_t off = (s / 4) * (FT_M * 128) + (s % 4) * 32;
+          umma_bf16(tmem, make_smem_desc(qb + off, 16, 1024, 2), make_smem_desc(kb + off, 16, 1024, 2), idesc_qk, s > 0);
+        }
+        umma_commit(s_full);
+        umma_commit(k_empty);
+        if (!mbar_wait(p_full, j & 1, abort_flag, tk.status, ERR_WAIT_MISC)) break;
+        if (!mbar_wait(v_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < FT_N / 16; ++s)          // 16 keys: eight packed columns of weights
+          umma_bf16_tmem_a(tmem + O_COL, tmem + s * 8, make_smem_desc(vb + s * 2048, FT_N * 128, 1024, 2), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
+        umma_commit(o_full);
+        umma_commit(v_empty);
+      }
+    }
+  } else {
+    // ---------------- softmax: thread <-> row ----------------
+    const int r = warp * 32 + lane, rr = r0 + min(r, nr - 1), tok = div_by(rr, a.G, a.inv_g), hd = hk * a.G + rr - tok * a.G;
+    const int kmax = start + tok, kmin = a.window > 0 ? kmax - a.window + 1 : 0;
+    const uint32_t t_lane = tmem + (uint32_t(warp * 32) << 16);
+    float qm;
+    {                                                // the row's queries, scaled by a power of two, as fp16 rows for the products
+      const __nv_bfloat16* src = a.q + (t0 + tok) * a.ld_q + hd * D;
+      uint4 w[D / 8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * 8);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, max(v[k] & 0x7fffu, (v[k] >> 16) & 0x7fffu));
+      }
+      const int ex = min(max((int)(top >> 7), 1), 253);
+      const float sign = a.scale < 0.f ? -1.f : 1.f, down = sign * __uint_as_float((uint32_t)(254 - ex) << 23);
+      qm = sign * a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);      // not negative: largest scores stay largest
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) h[k] = half2_of(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
+        *reinterpret_cast<uint4*>(sQ + (i >> 3) * (FT_M * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+    }
+    const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
+    float m = -INFINITY, l = 0.f, vref = 0.f;
+    int vexp = 0;                                    // vref = 2^(vexp - 127)
+    bool ok = true;
+    for (int j = 0; j < nb; ++j) {
+      if (!mbar_wait_warp(s_full, j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
+      if (!mbar_wait_warp(scales_full + (j & 1), (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) { ok = false; break; }
+      tc_fence_after();
+      const float2* sc = scales[j & 1];
+      const int k0 = (b0 + j) * FT_N;
+      const uint32_t there = present[j & 1];
+      const bool whole = k0 >= all_lo && k0 + FT_N <= all_hi && there == (1u << FT_PAGES) - 1;
+      auto seen = [&](int i) { const int k = k0 + i; return k <= kmax && k >= kmin && ((there >> (i / FP8_PAGE)) & 1); };
+      // ---- the largest score and the largest value scale ----
+      float mx = -INFINITY, v_up = 0.f;
+#pragma unroll
+      for (int cc = 0; cc < FT_N / 32; ++cc) {
+        uint32_t s[32];
+        tmem_ld_32x32(t_lane + cc * 32, s);
+        tmem_ld_wait();
+        if (!whole) {
+          rarely();
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!seen(cc * 32 + i)) s[i] = 0xff800000u;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            x0 = fmax3(x0, __uint_as_float(s[h * 16 + i]), __uint_as_float(s[h * 16 + i + 1]));
+            x1 = fmax3(x1, __uint_as_float(s[h * 16 + i + 2]), __uint_as_float(s[h * 16 + i + 3]));
+          }
+          const float2 k = sc[cc * 2 + h];
+          mx = fmaxf(mx, fmaxf(x0, x1) * (qm * k.x));
+          v_up = fmaxf(v_up, k.y);
+        }
+      }
+      const bool raise = j == 0 || mx > m + SLACK;
+      const float up = raise ? fmaxf(m, mx) : m;
+      float alpha = j == 0 || up == m ? 1.f : exp2_fast(m - up);
+      m = up;
+      l *= alpha;
+      if (v_up > vref) {
+        if (j > 0) alpha *= vref / v_up;
+        vref = v_up;
+        vexp = (int)(__float_as_uint(v_up) >> 23);
+      }
+      if (__any_sync(0xffffffffu, j > 0 && alpha != 1.f)) {
+        // the last block's product is complete before these scores were computed
+#pragma unroll 1
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_lane + O_COL + cc * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st_32x32(t_lane + O_COL + cc * 32, o);
+        }
+      }
+      // ---- weights ----
+      const float base = LIFT - (m == -INFINITY ? 0.f : m);
+#pragma unroll
+      for (int cc = 0; cc < FT_N / 32; ++cc) {
+        uint32_t s[32];
+        tmem_ld_32x32(t_lane + cc * 32, s);
+        tmem_ld_wait();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float2 k = sc[cc * 2 + h];
+          // the value scale's exponent over vref's; 2^-60 and less weigh nothing. No number stays none.
+          const int d = k.y == k.y ? max((int)(__float_as_uint(k.y) >> 23) - vexp, -60) : 0;
+          const float f = qm * k.x, off = k.y == k.y ? base + (float)d : k.y, back = __uint_as_float((uint32_t)(127 - d) << 23);
+          float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float e0 = exp2_fast(fmaf(__uint_as_float(s[h * 16 + i]), f, off)), e1 = exp2_fast(fmaf(__uint_as_float(s[h * 16 + i + 1]), f, off));
+            s[h * 16 + i] = __float_as_uint(e0);
+            s[h * 16 + i + 1] = __float_as_uint(e1);
+          }
+          if (!whole) {
+            rarely();
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!seen(cc * 32 + h * 16 + i)) s[h * 16 + i] = 0u;
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            sum0 += __uint_as_float(s[h * 16 + i]);
+            sum1 += __uint_as_float(s[h * 16 + i + 1]);
+            s[h * 8 + i / 2] = half2_of(__uint_as_float(s[h * 16 + i]), __uint_as_float(s[h * 16 + i + 1]));
+          }
+          l = fmaf(sum0 + sum1, back, l);
+        }
+        tmem_st_32x16(t_lane + cc * 16, s);          // over scores that have been read
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    if (ok) ok = mbar_wait_warp(o_full, (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
+    if (ok) {
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : vref / l;
+      const long at = ((long)(t0 + tok) * a.H + hd) * a.splits + split;
+#pragma unroll 1
+      for (int cc = 0; cc < D / 32; ++cc) {
+        uint32_t o[32];
+        tmem_ld_32x32(t_lane + O_COL + cc * 32, o);
+        tmem_ld_wait();
+        if (r < nr && a.splits == 1) {
+          uint4* to = reinterpret_cast<uint4*>(a.out + (t0 + tok) * a.ld_o + hd * D + cc * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
+            to[i] = make_uint4(h[0], h[1], h[2], h[3]);
+          }
+        } else if (r < nr) {
+          float4* to = reinterpret_cast<float4*>(a.part + at * D + cc * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            to[i] = make_float4(__uint_as_float(o[i * 4]) * vref, __uint_as_float(o[i * 4 + 1]) * vref, __uint_as_float(o[i * 4 + 2]) * vref,
+                                __uint_as_float(o[i * 4 + 3]) * vref);
+        }
+        __syncwarp();
+      }
+      if (a.splits > 1 && r < nr) {
+        a.part_ml[2 * at] = m;
+        a.part_ml[2 * at + 1] = l;
+        if (split == 0) a.used[(long)(t0 + tok) * a.H + hd] = max(1, min(a.splits, (b_hi - b_lo + per - 1) / per));
+      }
+      tc_fence_before();
+    }
+  }
+
+  __syncthreads();
+  if (*abort_flag) {                                 // a wait ran out: products on their way end before their memory goes
+    const uint64_t since = globaltimer_ns();
+    while (globaltimer_ns() - since < 2000000ull) __nanosleep(1000);
+    __syncthreads();
+  }
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, COLS);
+  }
+}
+
 // Joins the splits of a row (a query token's head), D / 32 values a lane. WIDE: a CTA a row, whose warps share the splits; else a warp a row. With 63
 // splits of 32 rows a warp a row took most of 24 us.
 template <int D, bool WIDE>
@@ -762,12 +1119,14 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
+constexpr int FP8_FEW_ROWS = 32;      // of a sequence and key head, for the kernel of 16-row tiles
 // How an attention is cut: rows of a tile (8 `blocks`), warps and pages of a CTA, CTAs along a sequence.
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
-  Fp8Cut(int n, int Hkv, int G, int max_new, int max_len, int window) {
-    blocks = (long)max_new * G <= 8 ? 1 : 2;
-    tiles = (int)(((long)max_new * G + 8 * blocks - 1) / (8 * blocks));
+  Fp8Cut(int n, int Hkv, int G, int max_new, int max_len, int window, bool tree) {
+    const long rows = (long)max_new * G;
+    blocks = rows <= 8 ? 1 : rows <= FP8_FEW_ROWS || tree ? 2 : FT_M / 8;
+    tiles = (int)((rows + 8 * blocks - 1) / (8 * blocks));
     const long span = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
     const int pages = (int)((span + (window > 0 ? 2 * FP8_PAGE - 2 : FP8_PAGE - 1)) / FP8_PAGE);       // a window may begin inside a page
     const long units = (long)n * Hkv * tiles;
@@ -781,6 +1140,13 @@ struct Fp8Cut {
     const long total = units * pages;
     long want = (total + 295) / 296;
     if (want > 128) want = total / 1184 > 128 ? total / 1184 : 128;
+    if (blocks == FT_M / 8) {                                      // whole blocks of keys
+      if (want < 4 * FT_PAGES) want = 4 * FT_PAGES;
+      per = want < pages ? (int)((want + FT_PAGES - 1) / FT_PAGES * FT_PAGES) : (pages + FT_PAGES - 1) / FT_PAGES * FT_PAGES;
+      splits = ((pages + FT_PAGES - 1) / FT_PAGES * FT_PAGES + (window > 0 ? FT_PAGES : 0) + per - 1) / per;
+      if (pages <= per) splits = 1;
+      return;
+    }
     if (want < 16) want = 16;
     if (many || pages <= 64 || want > pages) want = pages;
     per = want < pages ? (int)((want + 1) & ~1l) : pages;          // warps take two
@@ -788,36 +1154,51 @@ struct Fp8Cut {
   }
 };
 // Floats of workspace that an attention wants (0: none). A call's own: it holds partial results from one launch to the next.
-extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int max_new, int max_len, int window) {
+extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int max_new, int max_len, int window, int tree) {
   if (n < 1 || T < 1 || Hkv < 1 || H < Hkv || max_new < 1 || max_len < 1) return 0;
-  const Fp8Cut cut(n, Hkv, H / Hkv, max_new, max_len, window);
+  const Fp8Cut cut(n, Hkv, H / Hkv, max_new, max_len, window, tree);
   return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
 }
 
-template <int D, int NR, int NW, bool TREE>
-static int fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
-  constexpr int SMEM = fp8_attend_smem<D, NW>();
-  static std::atomic<uint64_t> ready{0};                           // devices whose limit has been raised
+// The kernel's shared memory on the current device, asked for once.
+template <typename K>
+static void raise_smem(K* kernel, int bytes, std::atomic<uint64_t>& ready) {
   int device = 0;
   cudaGetDevice(&device);
   const uint64_t bit = 1ull << (device & 63);
-  if (!(ready.load() & bit)) {
-    cudaFuncSetAttribute(fp8_attend_kernel<D, NR, NW, TREE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-    ready.fetch_or(bit);
-  }
-  launch_early(fp8_attend_kernel<D, NR, NW, TREE>, dim3(ctas), NW * 32, SMEM, st, a, pool, tk);
-  const long items = (long)tk.T * a.H;
+  if (ready.load() & bit) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  ready.fetch_or(bit);
+}
+template <int D>
+static int fp8_attend_join(const Fp8Attend& a, int T, cudaStream_t st) {
+  const long items = (long)T * a.H;
   if (a.splits > 4)
-    launch_early(fp8_join_kernel<D, true>, dim3((unsigned)items), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, tk.T, a.H, a.splits);
+    launch_early(fp8_join_kernel<D, true>, dim3((unsigned)items), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, T, a.H, a.splits);
   else if (a.splits > 1)
-    launch_early(fp8_join_kernel<D, false>, dim3((unsigned)((items + 7) / 8)), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, tk.T, a.H, a.splits);
+    launch_early(fp8_join_kernel<D, false>, dim3((unsigned)((items + 7) / 8)), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, T, a.H, a.splits);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
+}
+template <int D, int NR, int NW, bool TREE>
+static int fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
+  constexpr int SMEM = fp8_attend_smem<D, NW>();
+  static std::atomic<uint64_t> ready{0};
+  raise_smem(fp8_attend_kernel<D, NR, NW, TREE>, SMEM, ready);
+  launch_early(fp8_attend_kernel<D, NR, NW, TREE>, dim3(ctas), NW * 32, SMEM, st, a, pool, tk);
+  return fp8_attend_join<D>(a, tk.T, st);
+}
+template <int D>
+static int fp8_attend_tile_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  raise_smem(fp8_attend_tile_kernel<D>, FtSmem<D>::TOTAL, ready);
+  launch_early(fp8_attend_tile_kernel<D>, dim3(ctas), FT_THREADS, FtSmem<D>::TOTAL, st, a, pool, tk);
+  return fp8_attend_join<D>(a, tk.T, st);
 }
 
 static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, float* work, cudaStream_t st) {
   a.G = a.H / pool.Hkv;
-  const Fp8Cut cut(tk.n, pool.Hkv, a.G, max_new, max_len, a.window);
+  const Fp8Cut cut(tk.n, pool.Hkv, a.G, max_new, max_len, a.window, a.row_seq != nullptr);
   a.tiles = cut.tiles;
   a.per_split = cut.per;
   a.splits = cut.splits;
@@ -832,6 +1213,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;
   const unsigned grid = (unsigned)ctas;
+  if (cut.blocks == FT_M / 8) return D == 64 ? fp8_attend_tile_launch<64>(a, pool, tk, grid, st) : fp8_attend_tile_launch<128>(a, pool, tk, grid, st);
 #define INV_FP8(DD, TREE)                                                        \
   return cut.blocks == 2  ? fp8_attend_launch<DD, 2, 4, TREE>(a, pool, tk, grid, st) \
          : cut.warps == 4 ? fp8_attend_launch<DD, 1, 4, TREE>(a, pool, tk, grid, st) \

@@ -20,7 +20,7 @@ from .functional import _head_norm_rope, _weights16, check_rope
 _vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
 _native.register_cuda_sigs({
     "inv_fp8_append": [_vp, _vp, _l, _vp, _l, _vp, _l, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _i, _i, _vp] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i, _i, _vp, _vp],
-    "inv_fp8_attend_floats": [_i] * 8,
+    "inv_fp8_attend_floats": [_i] * 9,
     "inv_fp8_attend": [_vp, _l, _vp, _l, _i, _i, _i, _f, _i] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i] * 4 + [_vp] * 3,
     "inv_fp8_attend_tree": [_vp, _l, _vp, _l, _i, _i, _i, _f] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 4 + [_i, _i] + [_vp] * 3,
 })
@@ -262,11 +262,11 @@ def _check_out(out, q, width):
     return out
 
 
-def _workspace(n, T, heads, kv_heads, dim, max_new, max_len, window, dev):
+def _workspace(n, T, heads, kv_heads, dim, max_new, max_len, window, tree, dev):
     """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
     fn = rt.lib().inv_fp8_attend_floats
     fn.restype = _l
-    floats = fn(n, T, heads, kv_heads, dim, max_new, max_len, window)
+    floats = fn(n, T, heads, kv_heads, dim, max_new, max_len, window, tree)
     return torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
 
 
@@ -294,7 +294,7 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
         return out
     q, to = _aligned(q), out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
     with rt.device_of(q):
-        work = _workspace(n, T, heads, G, D, new.max_new, new.max_len, window, q.device)
+        work = _workspace(n, T, heads, G, D, new.max_new, new.max_len, window, 0, q.device)
         rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, window,
                                          *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
                                          new.max_new, new.max_len, rt.ptr(work), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
@@ -331,7 +331,7 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
         return out
     q, to = _aligned(q), out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
     with rt.device_of(q):
-        work = _workspace(T, T, heads, G, D, 1, max_len, 0, q.device)
+        work = _workspace(T, T, heads, G, D, 1, max_len, 0, 1, q.device)
         rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, *_pool_args(pages, page_table),
                                               row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
                                               max_len, rt.ptr(work), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()), "inv_fp8_attend_tree")
