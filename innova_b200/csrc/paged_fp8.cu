@@ -239,6 +239,27 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t x) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ uint4 shared16(uint32_t at) {
   uint4 r;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
@@ -684,7 +705,7 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t M, uint32_t N, ui
 }
 
 constexpr int FT_M = 128, FT_N = 128, FT_PAGES = FT_N / FP8_PAGE;
-constexpr int FT_THREADS = 288;        // four warps of softmax, one that issues the products, four that convert
+constexpr int FT_THREADS = 256;        // four warps of softmax, four that convert
 template <int D>
 struct FtSmem {
   static constexpr int TILE = FT_M * D * 2;          // fp16 rows in pieces of 64 columns with the 128-byte swizzle: queries, keys, values
@@ -693,9 +714,9 @@ struct FtSmem {
 
 // 128 rows (query tokens times the heads that share a key head) against blocks of 128 keys on the tcgen05 tensor cores: prompts behind a cache, and drafts of
 // more than a few tokens. grid = row tiles (the longest first) x splits x key heads x sequences, two CTAs an SM.
-//   warps 0-3  softmax, a row a thread: scores from tensor memory, weights in fp16 back in their place, in two passes of 32 columns at a time
-//   warp 4     one thread issues S = Q K^T and O += P V (P from tensor memory)
-//   warps 5-8  codes of the next block from the pages to registers, as fp16 to shared memory
+//   warps 0-3  softmax, a row a thread: scores from tensor memory, weights in fp16 back in their place; a thread of warp 0 issues S = Q K^T and
+//              O += P V (P from tensor memory), which the row's own chain waits for anyway
+//   warps 4-7  codes of the next block from the pages to registers, as fp16 to shared memory
 // Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are powers of two added to it (relative to the
 // largest one so far, which O is kept in) and taken out of the row sum again a page at a time, so neither costs anything a score. For the rest the sums are
 // those of the small kernel. One CTA's softmax runs under the other's products.
@@ -760,96 +781,74 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp >= 5) {
-    // ---------------- conversion: a thread takes the same piece of every eighth (D = 64: every second) token ----------------
-    const int tid = threadIdx.x - 160;
-    constexpr int PER = FT_N * CH / 128;             // pieces of a thread in a block: 8 or 4
-    const int piece = tid % CH, tok0 = tid / CH;     // its tokens: tok0 + i * (128 / CH)
-    constexpr int STEP = 128 / CH;
-    uint4 kr[PER], vr[PER];
-    int id = -1;                                     // lanes 0 to 7: page of the block in hand
-    auto look_up = [&](int j) { id = lane < FT_PAGES && j < nb && (b0 + j) * FT_PAGES + lane < (hi + FP8_PAGE - 1) / FP8_PAGE
-                                         ? pool_page(tk, pool.pages, row, (b0 + j) * FT_PAGES + lane) : -1; };
-    auto load = [&](const uint8_t* codes, uint4 (&r)[PER], int ids, int j, bool values) {
+  if (warp >= 4) {
+    // ---------------- conversion: a thread takes the same piece of every sixteenth (D = 64: thirty-second) token ----------------
+    const int tid = threadIdx.x - 128;
+    constexpr int PER = FT_N * CH / 128, STEP = 128 / CH;      // pieces of a thread in a block; tokens from one to the next
+    const int piece = tid % CH, tok0 = tid / CH, pages_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
+    uint4 raw[PER];
+    // Lanes 0 to 7 look a block's pages up: read two blocks ahead, checked one ahead, scales read then, so that nothing is waited for.
+    auto read_id = [&](int j) {
+      const int pg = (b0 + j) * FT_PAGES + lane;
+      return lane < FT_PAGES && j < nb && pg < pages_hi && (unsigned)row < (unsigned)tk.table_rows && pg < tk.max_pages
+                 ? tk.page_table[(long)row * tk.max_pages + pg] : -1;
+    };
+    auto check_id = [&](int id, int j) {
+      const bool wanted = lane < FT_PAGES && j < nb && (b0 + j) * FT_PAGES + lane < pages_hi;
+      if ((unsigned)id < (unsigned)pool.pages) return id;
+      if (wanted) atomicCAS(tk.status, 0, ERR_BAD_ARG);
+      return -1;
+    };
+    auto scale_at = [&](const float* of, int id) { return id >= 0 ? of[(long)id * pool.Hkv + hk] : 0.f; };
+    auto load = [&](const uint8_t* codes, int ids, int j, bool values) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int tok = tok0 + i * STEP, pid = __shfl_sync(0xffffffffu, ids, tok / FP8_PAGE);
-        const bool live = pid >= 0 && j < nb && !(values && (b0 + j) * FT_N + tok >= hi);       // values past the end are nothing, whatever is there
-        r[i] = live ? *reinterpret_cast<const uint4*>(codes + (((long)pid * pool.Hkv + hk) * FP8_PAGE + tok % FP8_PAGE) * D + piece * 16)
-                    : make_uint4(0, 0, 0, 0);
+        const bool live = pid >= 0 && !(values && (b0 + j) * FT_N + tok >= hi);       // values past the end are nothing, whatever is there
+        raw[i] = live ? *reinterpret_cast<const uint4*>(codes + (((long)pid * pool.Hkv + hk) * FP8_PAGE + tok % FP8_PAGE) * D + piece * 16)
+                      : make_uint4(0, 0, 0, 0);
       }
     };
-    auto store = [&](uint8_t* dst, const uint4 (&r)[PER]) {
+    auto store = [&](uint8_t* dst, uint64_t* bar) {
+      const int at = 2 * piece;                                                  // 16-byte pieces `at` and `at` + 1 of a token's fp16 row
+      const bool odd = piece >= CH / 2;                                          // lanes of the second half store in the other order: no bank twice
+      uint8_t* to = dst + (at >> 3) * (FT_N * 128) + tok0 * 128;
+      const int x0 = (((at & 7) + (odd ? 1 : 0)) ^ (tok0 & 7)) << 4, x1 = (((at & 7) + (odd ? 0 : 1)) ^ (tok0 & 7)) << 4;
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int tok = tok0 + i * STEP, at = 2 * piece;                          // 16-byte pieces `at` and `at` + 1 of the token's fp16 row
-        uint8_t* line = dst + (at >> 3) * (FT_N * 128) + tok * 128;
-        const uint4 h0 = make_uint4(half2_of_e4m3x2(r[i].x), half2_of_e4m3x2(r[i].x >> 16), half2_of_e4m3x2(r[i].y), half2_of_e4m3x2(r[i].y >> 16));
-        const uint4 h1 = make_uint4(half2_of_e4m3x2(r[i].z), half2_of_e4m3x2(r[i].z >> 16), half2_of_e4m3x2(r[i].w), half2_of_e4m3x2(r[i].w >> 16));
-        const bool odd = piece >= CH / 2;                                        // lanes of the second half store in the other order: no bank twice
-        *reinterpret_cast<uint4*>(line + ((((at & 7) + (odd ? 1 : 0)) ^ (tok & 7)) << 4)) = odd ? h1 : h0;
-        *reinterpret_cast<uint4*>(line + ((((at & 7) + (odd ? 0 : 1)) ^ (tok & 7)) << 4)) = odd ? h0 : h1;
+        const uint4 r = raw[i];
+        const uint4 h0 = make_uint4(half2_of_e4m3x2(r.x), half2_of_e4m3x2(r.x >> 16), half2_of_e4m3x2(r.y), half2_of_e4m3x2(r.y >> 16));
+        const uint4 h1 = make_uint4(half2_of_e4m3x2(r.z), half2_of_e4m3x2(r.z >> 16), half2_of_e4m3x2(r.w), half2_of_e4m3x2(r.w >> 16));
+        *reinterpret_cast<uint4*>(to + i * STEP * 128 + x0) = odd ? h1 : h0;     // STEP is a multiple of eight: the swizzle stays
+        *reinterpret_cast<uint4*>(to + i * STEP * 128 + x1) = odd ? h0 : h1;
       }
-    };
-    auto publish = [&](uint64_t* bar) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    look_up(0);
-    int ids = id;
-    load(pool.k, kr, ids, 0, false);
-    load(pool.v, vr, ids, 0, true);
+    static_assert(STEP % 8 == 0, "a thread's tokens share a swizzle");
+    int id = check_id(read_id(0), 0), read = read_id(1);
+    float ks = scale_at(pool.k_scale, id), vs = scale_at(pool.v_scale, id);
     for (int j = 0; j < nb; ++j) {
-      float2 sc = make_float2(0.f, 0.f);
-      const uint32_t there = __ballot_sync(0xffffffffu, ids >= 0);
-      if (warp == 5 && ids >= 0) {
-        sc.x = pool.k_scale[(long)ids * pool.Hkv + hk];
-        sc.y = pool.v_scale[(long)ids * pool.Hkv + hk];
-      }
-      look_up(j + 1);
+      load(pool.k, id, j, false);
+      const int id_n = check_id(read, j + 1);
+      read = read_id(j + 2);
+      const float ks_n = scale_at(pool.k_scale, id_n), vs_n = scale_at(pool.v_scale, id_n);
+      const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
       if (!mbar_wait_warp(k_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
-      store(sK, kr);
-      if (warp == 5) {
-        if (lane < FT_PAGES) scales[j & 1][lane] = sc;
+      if (warp == 4) {
+        if (lane < FT_PAGES) scales[j & 1][lane] = make_float2(ks, vs);
         if (lane == 0) present[j & 1] = there;
         __syncwarp();
         if (lane == 0) mbar_arrive(scales_full + (j & 1));
       }
-      publish(k_full);
-      load(pool.k, kr, id, j + 1, false);
+      store(sK, k_full);
+      load(pool.v, id, j, true);
       if (!mbar_wait_warp(v_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
-      store(sV, vr);
-      publish(v_full);
-      load(pool.v, vr, id, j + 1, true);
-      ids = id;
-    }
-  } else if (warp == 4) {
-    if (elect_one_sync()) {
-      const uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
-      const uint32_t qb = smem_u32(sQ), kb = smem_u32(sK), vb = smem_u32(sV);
-      bool ok = mbar_wait(q_full, 0, abort_flag, tk.status, ERR_WAIT_FULL);
-      for (int j = 0; ok && j < nb; ++j) {
-        // the scores take the place of the last block's weights, which its product has read
-        if (!mbar_wait(k_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) break;
-        if (j > 0 && !mbar_wait(o_full, (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint32_t off = (s / 4) * (FT_M * 128) + (s % 4) * 32;
-          umma_bf16(tmem, make_smem_desc(qb + off, 16, 1024, 2), make_smem_desc(kb + off, 16, 1024, 2), idesc_qk, s > 0);
-        }
-        umma_commit(s_full);
-        umma_commit(k_empty);
-        if (!mbar_wait(p_full, j & 1, abort_flag, tk.status, ERR_WAIT_MISC)) break;
-        if (!mbar_wait(v_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) break;
-        tc_fence_after();
-#pragma unroll
-        for (int s = 0; s < FT_N / 16; ++s)          // 16 keys: eight packed columns of weights
-          umma_bf16_tmem_a(tmem + O_COL, tmem + s * 8, make_smem_desc(vb + s * 2048, FT_N * 128, 1024, 2), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
-        umma_commit(o_full);
-        umma_commit(v_empty);
-      }
+      store(sV, v_full);
+      id = id_n;
+      ks = ks_n;
+      vs = vs_n;
     }
   } else {
     // ---------------- softmax: thread <-> row ----------------
@@ -884,11 +883,44 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
+    const uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
+    auto issue_scores = [&](int j) -> bool {         // warp 0; in the place of the last block's weights, whose product is complete
+      if (!mbar_wait_warp(k_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
+      if (j > 0 && !mbar_wait_warp(o_full, (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t qb = smem_u32(sQ), kb = smem_u32(sK);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint32_t off = (s / 4) * (FT_M * 128) + (s % 4) * 32;
+          umma_bf16(tmem, make_smem_desc(qb + off, 16, 1024, 2), make_smem_desc(kb + off, 16, 1024, 2), idesc_qk, s > 0);
+        }
+        umma_commit(s_full);
+        umma_commit(k_empty);
+      }
+      __syncwarp();
+      return true;
+    };
+    auto issue_values = [&](int j) -> bool {         // warp 0, once all four have published their weights
+      if (!mbar_wait_warp(p_full, j & 1, abort_flag, tk.status, ERR_WAIT_MISC)) return false;
+      if (!mbar_wait_warp(v_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t vb = smem_u32(sV);
+#pragma unroll
+        for (int s = 0; s < FT_N / 16; ++s)          // 16 keys: eight packed columns of weights
+          umma_bf16_tmem_a(tmem + O_COL, tmem + s * 8, make_smem_desc(vb + s * 2048, FT_N * 128, 1024, 2), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
+        umma_commit(o_full);
+        umma_commit(v_empty);
+      }
+      __syncwarp();
+      return true;
+    };
     const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
     float m = -INFINITY, l = 0.f, vref = 0.f;
     int vexp = 0;                                    // vref = 2^(vexp - 127)
-    bool ok = true;
-    for (int j = 0; j < nb; ++j) {
+    bool ok = warp > 0 || (mbar_wait_warp(q_full, 0, abort_flag, tk.status, ERR_WAIT_FULL) && issue_scores(0));
+    for (int j = 0; ok && j < nb; ++j) {
       if (!mbar_wait_warp(s_full, j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
       if (!mbar_wait_warp(scales_full + (j & 1), (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) { ok = false; break; }
       tc_fence_after();
@@ -897,28 +929,30 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       const uint32_t there = present[j & 1];
       const bool whole = k0 >= all_lo && k0 + FT_N <= all_hi && there == (1u << FT_PAGES) - 1;
       auto seen = [&](int i) { const int k = k0 + i; return k <= kmax && k >= kmin && ((there >> (i / FP8_PAGE)) & 1); };
-      // ---- the largest score and the largest value scale ----
+      // ---- the largest score and the largest value scale; the first half of the scores stays ----
       float mx = -INFINITY, v_up = 0.f;
+      uint32_t s[2][32];
 #pragma unroll
-      for (int cc = 0; cc < FT_N / 32; ++cc) {
-        uint32_t s[32];
-        tmem_ld_32x32(t_lane + cc * 32, s);
+      for (int half = 1; half >= 0; --half) {
+        tmem_ld_32x32(t_lane + half * 64, s[0]);
+        tmem_ld_32x32(t_lane + half * 64 + 32, s[1]);
         tmem_ld_wait();
         if (!whole) {
           rarely();
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!seen(cc * 32 + i)) s[i] = 0xff800000u;
+          for (int i = 0; i < 64; ++i)
+            if (!seen(half * 64 + i)) s[i / 32][i % 32] = 0xff800000u;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 4; ++h) {
+          const uint32_t* u = s[h / 2] + h % 2 * 16;
           float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            x0 = fmax3(x0, __uint_as_float(s[h * 16 + i]), __uint_as_float(s[h * 16 + i + 1]));
-            x1 = fmax3(x1, __uint_as_float(s[h * 16 + i + 2]), __uint_as_float(s[h * 16 + i + 3]));
+            x0 = fmax3(x0, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+            x1 = fmax3(x1, __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
           }
-          const float2 k = sc[cc * 2 + h];
+          const float2 k = sc[half * 4 + h];
           mx = fmaxf(mx, fmaxf(x0, x1) * (qm * k.x));
           v_up = fmaxf(v_up, k.y);
         }
@@ -945,46 +979,47 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
           tmem_st_32x32(t_lane + O_COL + cc * 32, o);
         }
       }
-      // ---- weights ----
+      // ---- weights: 32 columns from registers while the ones after next are read again ----
       const float base = LIFT - (m == -INFINITY ? 0.f : m);
 #pragma unroll
       for (int cc = 0; cc < FT_N / 32; ++cc) {
-        uint32_t s[32];
-        tmem_ld_32x32(t_lane + cc * 32, s);
-        tmem_ld_wait();
+        uint32_t(&u)[32] = s[cc & 1];
+        if (cc > 1) tmem_ld_wait();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float2 k = sc[cc * 2 + h];
           // the value scale's exponent over vref's; 2^-60 and less weigh nothing. No number stays none.
           const int d = k.y == k.y ? max((int)(__float_as_uint(k.y) >> 23) - vexp, -60) : 0;
           const float f = qm * k.x, off = k.y == k.y ? base + (float)d : k.y, back = __uint_as_float((uint32_t)(127 - d) << 23);
-          float sum0 = 0.f, sum1 = 0.f;
+          const uint64_t ff = pair_of(f, f), oo = pair_of(off, off);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            float e0 = exp2_fast(fmaf(__uint_as_float(s[h * 16 + i]), f, off)), e1 = exp2_fast(fmaf(__uint_as_float(s[h * 16 + i + 1]), f, off));
-            s[h * 16 + i] = __float_as_uint(e0);
-            s[h * 16 + i + 1] = __float_as_uint(e1);
+          for (int i = h * 16; i < h * 16 + 16; i += 2) {
+            const float2 e = of_pair(fma_pair(pair_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), ff, oo));
+            u[i] = __float_as_uint(exp2_fast(e.x));
+            u[i + 1] = __float_as_uint(exp2_fast(e.y));
           }
           if (!whole) {
             rarely();
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (!seen(cc * 32 + h * 16 + i)) s[h * 16 + i] = 0u;
+              if (!seen(cc * 32 + h * 16 + i)) u[h * 16 + i] = 0u;
           }
+          uint64_t sum = pair_of(__uint_as_float(u[h * 16]), __uint_as_float(u[h * 16 + 1]));
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            sum0 += __uint_as_float(s[h * 16 + i]);
-            sum1 += __uint_as_float(s[h * 16 + i + 1]);
-            s[h * 8 + i / 2] = half2_of(__uint_as_float(s[h * 16 + i]), __uint_as_float(s[h * 16 + i + 1]));
-          }
-          l = fmaf(sum0 + sum1, back, l);
+          for (int i = h * 16 + 2; i < h * 16 + 16; i += 2) sum = add_pair(sum, pair_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1])));
+#pragma unroll
+          for (int i = h * 16; i < h * 16 + 16; i += 2) u[i / 2] = half2_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+          const float2 both = of_pair(sum);
+          l = fmaf(both.x + both.y, back, l);
         }
-        tmem_st_32x16(t_lane + cc * 16, s);          // over scores that have been read
+        tmem_st_32x16(t_lane + cc * 16, u);          // over scores that have been read
+        if (cc < 2) tmem_ld_32x32(t_lane + (cc + 2) * 32, u);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
+      if (warp == 0) ok = issue_values(j) && (j + 1 == nb || issue_scores(j + 1));
     }
     if (ok) ok = mbar_wait_warp(o_full, (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
     if (ok) {
