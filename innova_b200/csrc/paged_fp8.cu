@@ -381,12 +381,12 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   uint4 qraw[NR][KP][2];                              // the queries arrive with the pages' numbers
 #pragma unroll
   for (int b = 0; b < NR; ++b) {
-    const int r = r0 + b * 8 + n, tok = div_by(r, a.G, a.inv_g);
+    const int r = r0 + min(b * 8 + n, nr - 1), tok = div_by(r, a.G, a.inv_g);             // rows past the tile's repeat its last
     const __nv_bfloat16* src = a.q + (t0 + tok) * a.ld_q + (hk * a.G + r - tok * a.G) * D + c * 16;
 #pragma unroll
     for (int j = 0; j < KP; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) qraw[b][j][i] = b * 8 + n < nr ? *reinterpret_cast<const uint4*>(src + j * 64 + i * 8) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 2; ++i) qraw[b][j][i] = *reinterpret_cast<const uint4*>(src + j * 64 + i * 8);
   }
   auto fetch = [&](int s) {                           // the pages of step s into their slot
 #pragma unroll
@@ -704,6 +704,14 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t M, uint32_t N, ui
   return (1u << 4) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);        // fp32 sums of fp16 operands
 }
 
+// log2 of a page's scale, a power of two (0, of a page never written, is -127); NaN stays.
+__device__ __forceinline__ float log2_scale(float s) { return s == s ? (float)((int)((__float_as_uint(s) >> 23) & 255) - 127) : s; }
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 constexpr int FT_M = 128, FT_N = 128, FT_PAGES = FT_N / FP8_PAGE;
 constexpr int FT_THREADS = 256;        // four warps of softmax, four that convert
 template <int D>
@@ -731,7 +739,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = smem + L::TILE, *sV = smem + 2 * L::TILE;
   __shared__ __align__(8) uint64_t bars[10];
-  __shared__ float2 scales[2][FT_PAGES];             // of a block's pages: keys, values
+  __shared__ float2 scales[2][FT_PAGES];             // of a block's pages: the keys' scale, log2 of the values'
   __shared__ uint32_t present[2];                    // bit p: page p of the block is there
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
@@ -787,26 +795,24 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
     constexpr int PER = FT_N * CH / 128, STEP = 128 / CH;      // pieces of a thread in a block; tokens from one to the next
     const int piece = tid % CH, tok0 = tid / CH, pages_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
     uint4 raw[PER];
-    // Lanes 0 to 7 look a block's pages up: read two blocks ahead, checked one ahead, scales read then, so that nothing is waited for.
-    auto read_id = [&](int j) {
-      const int pg = (b0 + j) * FT_PAGES + lane;
-      return lane < FT_PAGES && j < nb && pg < pages_hi && (unsigned)row < (unsigned)tk.table_rows && pg < tk.max_pages
-                 ? tk.page_table[(long)row * tk.max_pages + pg] : -1;
-    };
+    // Lanes 0 to 7 look a block's pages up: read two blocks ahead, checked one ahead, scales read then, so that nothing is waited for. Loads stand outside of
+    // branches, from a place that exists where there is none to read: behind a branch the compiler copies what was loaded, and so waits for each in turn.
+    const bool known = (unsigned)row < (unsigned)tk.table_rows;
+    const int* list = tk.page_table + (known ? (long)row * tk.max_pages : 0);
+    auto read_id = [&](int j) { return list[min((b0 + j) * FT_PAGES + lane, tk.max_pages - 1)]; };
     auto check_id = [&](int id, int j) {
-      const bool wanted = lane < FT_PAGES && j < nb && (b0 + j) * FT_PAGES + lane < pages_hi;
-      if ((unsigned)id < (unsigned)pool.pages) return id;
-      if (wanted) atomicCAS(tk.status, 0, ERR_BAD_ARG);
+      const int pg = (b0 + j) * FT_PAGES + lane;
+      if (lane >= FT_PAGES || j >= nb || pg >= pages_hi) return -1;
+      if (known && pg < tk.max_pages && (unsigned)id < (unsigned)pool.pages) return id;
+      atomicCAS(tk.status, 0, ERR_BAD_ARG);
       return -1;
     };
-    auto scale_at = [&](const float* of, int id) { return id >= 0 ? of[(long)id * pool.Hkv + hk] : 0.f; };
-    auto load = [&](const uint8_t* codes, int ids, int j, bool values) {
+    auto scale_at = [&](const float* of, int id) { return of[(long)max(id, 0) * pool.Hkv + hk]; };
+    auto load = [&](const uint8_t* codes, int ids) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int tok = tok0 + i * STEP, pid = __shfl_sync(0xffffffffu, ids, tok / FP8_PAGE);
-        const bool live = pid >= 0 && !(values && (b0 + j) * FT_N + tok >= hi);       // values past the end are nothing, whatever is there
-        raw[i] = live ? *reinterpret_cast<const uint4*>(codes + (((long)pid * pool.Hkv + hk) * FP8_PAGE + tok % FP8_PAGE) * D + piece * 16)
-                      : make_uint4(0, 0, 0, 0);
+        const int tok = tok0 + i * STEP, pid = max(__shfl_sync(0xffffffffu, ids, tok / FP8_PAGE), 0);
+        raw[i] = *reinterpret_cast<const uint4*>(codes + (((long)pid * pool.Hkv + hk) * FP8_PAGE + tok % FP8_PAGE) * D + piece * 16);
       }
     };
     auto store = [&](uint8_t* dst, uint64_t* bar) {
@@ -830,21 +836,29 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
     int id = check_id(read_id(0), 0), read = read_id(1);
     float ks = scale_at(pool.k_scale, id), vs = scale_at(pool.v_scale, id);
     for (int j = 0; j < nb; ++j) {
-      load(pool.k, id, j, false);
+      load(pool.k, id);
       const int id_n = check_id(read, j + 1);
       read = read_id(j + 2);
       const float ks_n = scale_at(pool.k_scale, id_n), vs_n = scale_at(pool.v_scale, id_n);
       const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
       if (!mbar_wait_warp(k_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
       if (warp == 4) {
-        if (lane < FT_PAGES) scales[j & 1][lane] = make_float2(ks, vs);
+        if (lane < FT_PAGES) scales[j & 1][lane] = id >= 0 ? make_float2(ks, log2_scale(vs)) : make_float2(0.f, -127.f);
         if (lane == 0) present[j & 1] = there;
         __syncwarp();
         if (lane == 0) mbar_arrive(scales_full + (j & 1));
       }
       store(sK, k_full);
-      load(pool.v, id, j, true);
+      load(pool.v, id);
       if (!mbar_wait_warp(v_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
+      if ((b0 + j + 1) * FT_N > hi || there != (1u << FT_PAGES) - 1) {           // values that are not there are nothing, whatever was read
+        rarely();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int tok = tok0 + i * STEP;
+          if ((b0 + j) * FT_N + tok >= hi || !((there >> (tok / FP8_PAGE)) & 1)) raw[i] = make_uint4(0, 0, 0, 0);
+        }
+      }
       store(sV, v_full);
       id = id_n;
       ks = ks_n;
@@ -883,17 +897,18 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
     }
-    const uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
+    constexpr uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
+    const uint64_t desc_q = make_smem_desc(smem_u32(sQ), 16, 1024, 2), desc_k = make_smem_desc(smem_u32(sK), 16, 1024, 2),
+                   desc_v = make_smem_desc(smem_u32(sV), FT_N * 128, 1024, 2);                 // steps of a product add to the address field
     auto issue_scores = [&](int j) -> bool {         // warp 0; in the place of the last block's weights, whose product is complete
       if (!mbar_wait_warp(k_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
       if (j > 0 && !mbar_wait_warp(o_full, (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
       if (lane == 0) {
-        const uint32_t qb = smem_u32(sQ), kb = smem_u32(sK);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s) {
-          const uint32_t off = (s / 4) * (FT_M * 128) + (s % 4) * 32;
-          umma_bf16(tmem, make_smem_desc(qb + off, 16, 1024, 2), make_smem_desc(kb + off, 16, 1024, 2), idesc_qk, s > 0);
+          const uint64_t off = ((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4;
+          umma_bf16(tmem, desc_q + off, desc_k + off, idesc_qk, s > 0);
         }
         umma_commit(s_full);
         umma_commit(k_empty);
@@ -906,10 +921,9 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       if (!mbar_wait_warp(v_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
       tc_fence_after();
       if (lane == 0) {
-        const uint32_t vb = smem_u32(sV);
 #pragma unroll
         for (int s = 0; s < FT_N / 16; ++s)          // 16 keys: eight packed columns of weights
-          umma_bf16_tmem_a(tmem + O_COL, tmem + s * 8, make_smem_desc(vb + s * 2048, FT_N * 128, 1024, 2), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
+          umma_bf16_tmem_a(tmem + O_COL, tmem + s * 8, desc_v + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
         umma_commit(o_full);
         umma_commit(v_empty);
       }
@@ -917,8 +931,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       return true;
     };
     const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
-    float m = -INFINITY, l = 0.f, vref = 0.f;
-    int vexp = 0;                                    // vref = 2^(vexp - 127)
+    float m = -INFINITY, l = 0.f, vref = -200.f;     // vref: log2 of the scale that O is kept in
     bool ok = warp > 0 || (mbar_wait_warp(q_full, 0, abort_flag, tk.status, ERR_WAIT_FULL) && issue_scores(0));
     for (int j = 0; ok && j < nb; ++j) {
       if (!mbar_wait_warp(s_full, j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
@@ -930,7 +943,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       const bool whole = k0 >= all_lo && k0 + FT_N <= all_hi && there == (1u << FT_PAGES) - 1;
       auto seen = [&](int i) { const int k = k0 + i; return k <= kmax && k >= kmin && ((there >> (i / FP8_PAGE)) & 1); };
       // ---- the largest score and the largest value scale; the first half of the scores stays ----
-      float mx = -INFINITY, v_up = 0.f;
+      float mx = -INFINITY, v_up = -200.f;
       uint32_t s[2][32];
 #pragma unroll
       for (int half = 1; half >= 0; --half) {
@@ -963,9 +976,8 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       m = up;
       l *= alpha;
       if (v_up > vref) {
-        if (j > 0) alpha *= vref / v_up;
+        if (j > 0) alpha *= exp2_fast(vref - v_up);
         vref = v_up;
-        vexp = (int)(__float_as_uint(v_up) >> 23);
       }
       if (__any_sync(0xffffffffu, j > 0 && alpha != 1.f)) {
         // the last block's product is complete before these scores were computed
@@ -988,9 +1000,8 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float2 k = sc[cc * 2 + h];
-          // the value scale's exponent over vref's; 2^-60 and less weigh nothing. No number stays none.
-          const int d = k.y == k.y ? max((int)(__float_as_uint(k.y) >> 23) - vexp, -60) : 0;
-          const float f = qm * k.x, off = k.y == k.y ? base + (float)d : k.y, back = __uint_as_float((uint32_t)(127 - d) << 23);
+          // the value scale over the largest one: 2^-60 and less weigh nothing. Out of the sum again it is taken, but for no number, which is in the weights.
+          const float d = max_or_nan(k.y - vref, -60.f), f = qm * k.x, off = base + d, back = exp2_fast(fminf(60.f, -d));
           const uint64_t ff = pair_of(f, f), oo = pair_of(off, off);
 #pragma unroll
           for (int i = h * 16; i < h * 16 + 16; i += 2) {
@@ -1024,7 +1035,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
     if (ok) ok = mbar_wait_warp(o_full, (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
     if (ok) {
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : vref / l;
+      const float vscale = exp2_fast(vref), inv = l == 0.f ? 0.f : vscale / l;
       const long at = ((long)(t0 + tok) * a.H + hd) * a.splits + split;
 #pragma unroll 1
       for (int cc = 0; cc < D / 32; ++cc) {
@@ -1044,8 +1055,8 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
           float4* to = reinterpret_cast<float4*>(a.part + at * D + cc * 32);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            to[i] = make_float4(__uint_as_float(o[i * 4]) * vref, __uint_as_float(o[i * 4 + 1]) * vref, __uint_as_float(o[i * 4 + 2]) * vref,
-                                __uint_as_float(o[i * 4 + 3]) * vref);
+            to[i] = make_float4(__uint_as_float(o[i * 4]) * vscale, __uint_as_float(o[i * 4 + 1]) * vscale, __uint_as_float(o[i * 4 + 2]) * vscale,
+                                __uint_as_float(o[i * 4 + 3]) * vscale);
         }
         __syncwarp();
       }
