@@ -712,6 +712,41 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   return d;
 }
 
+// One product step or commit of a converged warp: the thread is chosen inside, under a predicate, so that operands stay in uniform registers (a branch to
+// one lane around them made each step cost about ninety cycles of its warp).
+__device__ __forceinline__ void mma_of_warp(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred one, add;\n"
+      "elect.sync _|one, 0xffffffff;\n"
+      "setp.ne.u32 add, %4, 0;\n"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, add;\n"
+      "}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_of_warp_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred one, add;\n"
+      "elect.sync _|one, 0xffffffff;\n"
+      "setp.ne.u32 add, %4, 0;\n"
+      "@one tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, add;\n"
+      "}\n"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void commit_of_warp(uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred one;\n"
+      "elect.sync _|one, 0xffffffff;\n"
+      "@one tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n"
+      ::"r"(smem_u32(bar))
+      : "memory");
+}
+
 constexpr int FT_M = 128, FT_N = 128, FT_PAGES = FT_N / FP8_PAGE;
 constexpr int FT_THREADS = 256;        // four warps of softmax, four that convert
 template <int D>
@@ -904,30 +939,24 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
       if (!mbar_wait_warp(k_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
       if (j > 0 && !mbar_wait_warp(o_full, (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) return false;
       tc_fence_after();
-      if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint64_t off = ((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4;
-          umma_bf16(tmem, desc_q + off, desc_k + off, idesc_qk, s > 0);
-        }
-        umma_commit(s_full);
-        umma_commit(k_empty);
+      for (int s = 0; s < D / 16; ++s) {
+        const uint64_t off = ((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4;
+        mma_of_warp(tmem, desc_q + off, desc_k + off, idesc_qk, s > 0);
       }
-      __syncwarp();
+      commit_of_warp(s_full);
+      commit_of_warp(k_empty);
       return true;
     };
     auto issue_values = [&](int j) -> bool {         // warp 0, once all four have published their weights
       if (!mbar_wait_warp(p_full, j & 1, abort_flag, tk.status, ERR_WAIT_MISC)) return false;
       if (!mbar_wait_warp(v_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
       tc_fence_after();
-      if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < FT_N / 16; ++s)          // 16 keys: eight packed columns of weights
-          umma_bf16_tmem_a(tmem + O_COL, tmem + s * 8, desc_v + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
-        umma_commit(o_full);
-        umma_commit(v_empty);
-      }
-      __syncwarp();
+      for (int s = 0; s < FT_N / 16; ++s)            // 16 keys: eight packed columns of weights
+        mma_of_warp_tmem(tmem + O_COL, tmem + s * 8, desc_v + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
+      commit_of_warp(o_full);
+      commit_of_warp(v_empty);
       return true;
     };
     const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
