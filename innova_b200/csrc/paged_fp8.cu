@@ -747,39 +747,40 @@ __device__ __forceinline__ void commit_of_warp(uint64_t* bar) {
       : "memory");
 }
 
-constexpr int FT_M = 128, FT_N = 128, FT_PAGES = FT_N / FP8_PAGE;
-constexpr int FT_THREADS = 256;        // four warps of softmax, four that convert
+constexpr int FT_M = 128, FT_N = 128, FT_PAGES = FT_N / FP8_PAGE, FT_ROWS = 2 * FT_M;
+constexpr int FT_THREADS = 512;        // two groups of four warps for the softmax of a tile each, one that converts, one whose first warp issues the products
+constexpr int FT_SLOTS = 2;            // of keys and of values
 template <int D>
 struct FtSmem {
   static constexpr int TILE = FT_M * D * 2;          // fp16 rows in pieces of 64 columns with the 128-byte swizzle: queries, keys, values
-  static constexpr int TOTAL = 3 * TILE + 1024;
+  static constexpr int TOTAL = (2 + 2 * FT_SLOTS) * TILE + 1024;
 };
 
-// 128 rows (query tokens times the heads that share a key head) against blocks of 128 keys on the tcgen05 tensor cores: prompts behind a cache, and drafts of
-// more than a few tokens. grid = row tiles (the longest first) x splits x key heads x sequences, two CTAs an SM.
-//   warps 0-3  softmax, a row a thread: scores from tensor memory, weights in fp16 back in their place; a thread of warp 0 issues S = Q K^T and
-//              O += P V (P from tensor memory), which the row's own chain waits for anyway
-//   warps 4-7  codes of the next block from the pages to registers, as fp16 to shared memory
+// 256 rows (query tokens times the heads that share a key head) as two tiles against blocks of 128 keys on the tcgen05 tensor cores: prompts behind a cache,
+// and drafts of more than a few tokens. grid = row tiles (the longest first) x splits x key heads x sequences, one CTA an SM.
+//   warps 0-7    softmax, a row a thread: scores from tensor memory, weights in fp16 back in their place
+//   warps 8-11   codes of the next blocks from the pages to registers, as fp16 to shared memory, for both tiles
+//   warp 12      issues S = Q K^T and O += P V (P from tensor memory) of the tiles in turn: one's softmax runs under the other's products
 // Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are powers of two added to it (relative to the
 // largest one so far, which O is kept in) and taken out of the row sum again a page at a time, so neither costs anything a score. For the rest the sums are
-// those of the small kernel. One CTA's softmax runs under the other's products.
+// those of the small kernel. Tensor memory, of 512 columns: scores (then weights) 0 and 128, O 256 and 384.
 template <int D>
-__global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
+__global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
                                                                         const __grid_constant__ Fp8Tokens tk) {
   using L = FtSmem<D>;
-  constexpr int CH = D / 16;             // 16-byte pieces of a token's codes
+  constexpr int CH = D / 16, NS = FT_SLOTS;          // 16-byte pieces of a token's codes
   constexpr float LIFT = 6.f, SLACK = 8.f;
-  constexpr uint32_t O_COL = 128, COLS = 256;
+  constexpr uint32_t O_COL = 256, COLS = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = smem, *sK = smem + L::TILE, *sV = smem + 2 * L::TILE;
-  __shared__ __align__(8) uint64_t bars[10];
-  __shared__ float2 scales[2][FT_PAGES];             // of a block's pages: the keys' scale, log2 of the values'
-  __shared__ uint32_t present[2];                    // bit p: page p of the block is there
+  uint8_t *sQ = smem, *sK = smem + 2 * L::TILE, *sV = smem + (2 + NS) * L::TILE;
+  __shared__ __align__(8) uint64_t q_full[2], k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2], p_full[2], o_full[2], scales_full[4];
+  // Of a block's pages: the keys' scale, log2 of the values'; bit p of `present`: page p is there. Block j + 4 takes block j's place once the scores of
+  // block j + 2 are computed, which both tiles ask for behind their softmax of block j.
+  __shared__ float2 scales[4][FT_PAGES];
+  __shared__ uint32_t present[4];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
-  uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = bars + 2, *v_full = bars + 3, *v_empty = bars + 4, *s_full = bars + 5, *p_full = bars + 6,
-           *o_full = bars + 7, *scales_full = bars + 8;          // two: scales of even and odd blocks
   volatile int* abort_flag = &abort_word;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int x = div_by(blockIdx.x, a.tiles, a.inv_tiles);
@@ -790,8 +791,8 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
   const int t0 = tk.cu[seq], count = tk.cu[seq + 1] - t0, start = tk.start[seq], row = tk.rows[seq];
   const bool fine = t0 >= 0 && count >= 0 && count <= tk.T - t0 && start >= 0;
   const int rows = fine ? count * a.G : 0;
-  if ((!fine || rows > FT_M * a.tiles) && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
-  const int r0 = tile * FT_M, nr = min(FT_M, rows - r0);
+  if ((!fine || rows > FT_ROWS * a.tiles) && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
+  const int r0 = tile * FT_ROWS, nr = min(FT_ROWS, rows - r0);
   if (nr <= 0) return;
   const int first = start + div_by(r0, a.G, a.inv_g), last = start + div_by(r0 + nr - 1, a.G, a.inv_g);
   const int hi = last + 1, lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
@@ -799,23 +800,29 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
   const int b_lo = lo / FT_N, b_hi = (hi + FT_N - 1) / FT_N, per = a.per_split / FT_PAGES;
   const int b0 = b_lo + split * per, b1 = split + 1 < a.splits ? min(b_hi, b0 + per) : b_hi;
   if (split > 0 && b0 >= b1) return;
-  const int nb = b1 - b0;
+  const int nb = b1 - b0, tiles = nr > FT_M ? 2 : 1;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 4);
-    mbar_init(k_full, 4);
-    mbar_init(k_empty, 1);
-    mbar_init(v_full, 4);
-    mbar_init(v_empty, 1);
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 4);
-    mbar_init(o_full, 1);
-    mbar_init(scales_full, 1);
-    mbar_init(scales_full + 1, 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 4);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_full[i], 1);
+    }
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      mbar_init(&k_full[i], 4);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 4);
+      mbar_init(&v_empty[i], 1);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mbar_init(&scales_full[i], 1);
     abort_word = 0;
     fence_barrier_init();
   }
-  if (warp == 4) {
+  if (warp == 12) {
     tmem_alloc(&tmem_slot, COLS);
     tmem_relinquish();
   }
@@ -824,9 +831,54 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  if (warp >= 4) {
+  // 512 x 128 registers at launch; 128 x (184 + 184 + 96 + 40) behind these
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 12) {
+      constexpr uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
+      const uint64_t desc_q = make_smem_desc(smem_u32(sQ), 16, 1024, 2), desc_k = make_smem_desc(smem_u32(sK), 16, 1024, 2),
+                     desc_v = make_smem_desc(smem_u32(sV), FT_N * 128, 1024, 2);               // steps of a product add to the address field
+      auto scores = [&](int t, int j) {
+        const uint64_t dq = desc_q + (uint64_t)(t * L::TILE >> 4), dk = desc_k + (uint64_t)((j % NS) * L::TILE >> 4);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s) {
+          const uint64_t off = ((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4;
+          mma_of_warp(tmem + t * FT_N, dq + off, dk + off, idesc_qk, s > 0);
+        }
+        commit_of_warp(&s_full[t]);
+        if (t + 1 == tiles) commit_of_warp(&k_empty[j % NS]);
+      };
+      bool ok = mbar_wait_warp(&k_full[0], 0, abort_flag, tk.status, ERR_WAIT_FULL);
+      for (int t = 0; ok && t < tiles; ++t) {
+        ok = mbar_wait_warp(&q_full[t], 0, abort_flag, tk.status, ERR_WAIT_FULL);
+        tc_fence_after();
+        if (ok) scores(t, 0);
+      }
+      for (int j = 0; ok && j < nb; ++j) {
+        ok = mbar_wait_warp(&v_full[j % NS], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL) &&
+             (j + 1 == nb || mbar_wait_warp(&k_full[(j + 1) % NS], ((j + 1) / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL));
+        for (int t = 0; ok && t < tiles; ++t) {
+          ok = mbar_wait_warp(&p_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_MISC);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dv = desc_v + (uint64_t)((j % NS) * L::TILE >> 4);
+#pragma unroll
+          for (int s = 0; s < FT_N / 16; ++s)        // 16 keys: eight packed columns of weights
+            mma_of_warp_tmem(tmem + O_COL + t * 128, tmem + t * FT_N + s * 8, dv + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
+          commit_of_warp(&o_full[t]);
+          if (t + 1 == tiles) commit_of_warp(&v_empty[j % NS]);
+          if (j + 1 == nb) continue;
+          // the next scores take the place of the weights that this product reads
+          ok = mbar_wait_warp(&o_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
+          tc_fence_after();
+          if (ok) scores(t, j + 1);
+        }
+      }
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ---------------- conversion: a thread takes the same piece of every sixteenth (D = 64: thirty-second) token ----------------
-    const int tid = threadIdx.x - 128;
+    const int tid = threadIdx.x - 256;
     constexpr int PER = FT_N * CH / 128, STEP = 128 / CH;      // pieces of a thread in a block; tokens from one to the next
     const int piece = tid % CH, tok0 = tid / CH, pages_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
     uint4 raw[PER];
@@ -871,21 +923,22 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
     int id = check_id(read_id(0), 0), read = read_id(1);
     float ks = scale_at(pool.k_scale, id), vs = scale_at(pool.v_scale, id);
     for (int j = 0; j < nb; ++j) {
+      const int slot = j % NS, turn = ((j / NS) & 1) ^ 1;
       load(pool.k, id);
       const int id_n = check_id(read, j + 1);
       read = read_id(j + 2);
       const float ks_n = scale_at(pool.k_scale, id_n), vs_n = scale_at(pool.v_scale, id_n);
       const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
-      if (!mbar_wait_warp(k_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
-      if (warp == 4) {
-        if (lane < FT_PAGES) scales[j & 1][lane] = id >= 0 ? make_float2(ks, log2_scale(vs)) : make_float2(0.f, -127.f);
-        if (lane == 0) present[j & 1] = there;
+      if (!mbar_wait_warp(&k_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
+      if (warp == 8) {
+        if (lane < FT_PAGES) scales[j & 3][lane] = id >= 0 ? make_float2(ks, log2_scale(vs)) : make_float2(0.f, -127.f);
+        if (lane == 0) present[j & 3] = there;
         __syncwarp();
-        if (lane == 0) mbar_arrive(scales_full + (j & 1));
+        if (lane == 0) mbar_arrive(&scales_full[j & 3]);
       }
-      store(sK, k_full);
+      store(sK + slot * L::TILE, &k_full[slot]);
       load(pool.v, id);
-      if (!mbar_wait_warp(v_empty, (j & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
+      if (!mbar_wait_warp(&v_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
       if ((b0 + j + 1) * FT_N > hi || there != (1u << FT_PAGES) - 1) {           // values that are not there are nothing, whatever was read
         rarely();
 #pragma unroll
@@ -894,207 +947,189 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
           if ((b0 + j) * FT_N + tok >= hi || !((there >> (tok / FP8_PAGE)) & 1)) raw[i] = make_uint4(0, 0, 0, 0);
         }
       }
-      store(sV, v_full);
+      store(sV + slot * L::TILE, &v_full[slot]);
       id = id_n;
       ks = ks_n;
       vs = vs_n;
     }
   } else {
-    // ---------------- softmax: thread <-> row ----------------
-    const int r = warp * 32 + lane, rr = r0 + min(r, nr - 1), tok = div_by(rr, a.G, a.inv_g), hd = hk * a.G + rr - tok * a.G;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    // ---------------- softmax: thread <-> row r of tile t ----------------
+    const int t = warp >> 2, r = threadIdx.x & 127, rt = t * FT_M + r, rr = r0 + min(rt, nr - 1), tok = div_by(rr, a.G, a.inv_g);
+    const int hd = hk * a.G + rr - tok * a.G;
     const int kmax = start + tok, kmin = a.window > 0 ? kmax - a.window + 1 : 0;
-    const uint32_t t_lane = tmem + (uint32_t(warp * 32) << 16);
-    float qm;
-    {                                                // the row's queries, scaled by a power of two, as fp16 rows for the products
-      const __nv_bfloat16* src = a.q + (t0 + tok) * a.ld_q + hd * D;
-      uint4 w[D / 8];
-      uint32_t top = 0;
+    const uint32_t t_lane = tmem + (uint32_t((warp & 3) * 32) << 16), t_s = t_lane + t * FT_N, t_o = t_lane + O_COL + t * 128;
+    if (t < tiles) {
+      float qm;
+      {                                              // the row's queries, scaled by a power of two, as fp16 rows for the products
+        const __nv_bfloat16* src = a.q + (t0 + tok) * a.ld_q + hd * D;
+        uint4 w[D / 8];
+        uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * 8);
+        for (int i = 0; i < D / 8; ++i) w[i] = *reinterpret_cast<const uint4*>(src + i * 8);
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max(v[k] & 0x7fffu, (v[k] >> 16) & 0x7fffu));
+          for (int k = 0; k < 4; ++k) top = max(top, max(v[k] & 0x7fffu, (v[k] >> 16) & 0x7fffu));
+        }
+        const int ex = min(max((int)(top >> 7), 1), 253);
+        const float sign = a.scale < 0.f ? -1.f : 1.f, down = sign * __uint_as_float((uint32_t)(254 - ex) << 23);
+        qm = sign * a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);      // not negative: largest scores stay largest
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          uint32_t h[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) h[k] = half2_of(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
+          *reinterpret_cast<uint4*>(sQ + t * L::TILE + (i >> 3) * (FT_M * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[t]);
       }
-      const int ex = min(max((int)(top >> 7), 1), 253);
-      const float sign = a.scale < 0.f ? -1.f : 1.f, down = sign * __uint_as_float((uint32_t)(254 - ex) << 23);
-      qm = sign * a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);      // not negative: largest scores stay largest
+      const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
+      float m = -INFINITY, l = 0.f, vref = -200.f;     // vref: log2 of the scale that O is kept in
+      bool ok = true;
+      for (int j = 0; j < nb; ++j) {
+        if (!mbar_wait_warp(&scales_full[j & 3], (j >> 2) & 1, abort_flag, tk.status, ERR_WAIT_FULL) ||
+            !mbar_wait_warp(&s_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t s[FT_N];
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint32_t v[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-        uint32_t h[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) h[k] = half2_of(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
-        *reinterpret_cast<uint4*>(sQ + (i >> 3) * (FT_M * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-    }
-    constexpr uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
-    const uint64_t desc_q = make_smem_desc(smem_u32(sQ), 16, 1024, 2), desc_k = make_smem_desc(smem_u32(sK), 16, 1024, 2),
-                   desc_v = make_smem_desc(smem_u32(sV), FT_N * 128, 1024, 2);                 // steps of a product add to the address field
-    auto issue_scores = [&](int j) -> bool {         // warp 0; in the place of the last block's weights, whose product is complete
-      if (!mbar_wait_warp(k_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
-      if (j > 0 && !mbar_wait_warp(o_full, (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) return false;
-      tc_fence_after();
-#pragma unroll
-      for (int s = 0; s < D / 16; ++s) {
-        const uint64_t off = ((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4;
-        mma_of_warp(tmem, desc_q + off, desc_k + off, idesc_qk, s > 0);
-      }
-      commit_of_warp(s_full);
-      commit_of_warp(k_empty);
-      return true;
-    };
-    auto issue_values = [&](int j) -> bool {         // warp 0, once all four have published their weights
-      if (!mbar_wait_warp(p_full, j & 1, abort_flag, tk.status, ERR_WAIT_MISC)) return false;
-      if (!mbar_wait_warp(v_full, j & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
-      tc_fence_after();
-#pragma unroll
-      for (int s = 0; s < FT_N / 16; ++s)            // 16 keys: eight packed columns of weights
-        mma_of_warp_tmem(tmem + O_COL, tmem + s * 8, desc_v + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
-      commit_of_warp(o_full);
-      commit_of_warp(v_empty);
-      return true;
-    };
-    const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
-    float m = -INFINITY, l = 0.f, vref = -200.f;     // vref: log2 of the scale that O is kept in
-    bool ok = warp > 0 || (mbar_wait_warp(q_full, 0, abort_flag, tk.status, ERR_WAIT_FULL) && issue_scores(0));
-    for (int j = 0; ok && j < nb; ++j) {
-      if (!mbar_wait_warp(s_full, j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) { ok = false; break; }
-      if (!mbar_wait_warp(scales_full + (j & 1), (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) { ok = false; break; }
-      tc_fence_after();
-      const float2* sc = scales[j & 1];
-      const int k0 = (b0 + j) * FT_N;
-      const uint32_t there = present[j & 1];
-      const bool whole = k0 >= all_lo && k0 + FT_N <= all_hi && there == (1u << FT_PAGES) - 1;
-      auto seen = [&](int i) { const int k = k0 + i; return k <= kmax && k >= kmin && ((there >> (i / FP8_PAGE)) & 1); };
-      // ---- the largest score and the largest value scale; the first half of the scores stays ----
-      float mx = -INFINITY, v_up = -200.f;
-      uint32_t s[2][32];
-#pragma unroll
-      for (int half = 1; half >= 0; --half) {
-        tmem_ld_32x32(t_lane + half * 64, s[0]);
-        tmem_ld_32x32(t_lane + half * 64 + 32, s[1]);
+        for (int cc = 0; cc < FT_N / 32; ++cc) tmem_ld_32x32(t_s + cc * 32, s + cc * 32);
+        const float2* sc = scales[j & 3];
+        const int k0 = (b0 + j) * FT_N;
+        const uint32_t there = present[j & 3];
+        const bool whole = k0 >= all_lo && k0 + FT_N <= all_hi && there == (1u << FT_PAGES) - 1;
+        auto seen = [&](int i) { const int k = k0 + i; return k <= kmax && k >= kmin && ((there >> (i / FP8_PAGE)) & 1); };
         tmem_ld_wait();
         if (!whole) {
           rarely();
 #pragma unroll
-          for (int i = 0; i < 64; ++i)
-            if (!seen(half * 64 + i)) s[i / 32][i % 32] = 0xff800000u;
+          for (int i = 0; i < FT_N; ++i)
+            if (!seen(i)) s[i] = 0xff800000u;
         }
+        // ---- the largest score and the largest value scale ----
+        float mx = -INFINITY, v_up = -200.f;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const uint32_t* u = s[h / 2] + h % 2 * 16;
+        for (int h = 0; h < FT_PAGES; ++h) {
+          const uint32_t* u = s + h * 16;
           float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
             x0 = fmax3(x0, __uint_as_float(u[i]), __uint_as_float(u[i + 1]));
             x1 = fmax3(x1, __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
           }
-          const float2 k = sc[half * 4 + h];
+          const float2 k = sc[h];
           mx = fmaxf(mx, fmaxf(x0, x1) * (qm * k.x));
           v_up = fmaxf(v_up, k.y);
         }
-      }
-      const bool raise = j == 0 || mx > m + SLACK;
-      const float up = raise ? fmaxf(m, mx) : m;
-      float alpha = j == 0 || up == m ? 1.f : exp2_fast(m - up);
-      m = up;
-      l *= alpha;
-      if (v_up > vref) {
-        if (j > 0) alpha *= exp2_fast(vref - v_up);
-        vref = v_up;
-      }
-      if (__any_sync(0xffffffffu, j > 0 && alpha != 1.f)) {
-        // the last block's product is complete before these scores were computed
-#pragma unroll 1
-        for (int cc = 0; cc < D / 32; ++cc) {
-          uint32_t o[32];
-          tmem_ld_32x32(t_lane + O_COL + cc * 32, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st_32x32(t_lane + O_COL + cc * 32, o);
+        const bool raise = j == 0 || mx > m + SLACK;
+        const float up = raise ? fmaxf(m, mx) : m;
+        float alpha = j == 0 || up == m ? 1.f : exp2_fast(m - up);
+        m = up;
+        l *= alpha;
+        if (v_up > vref) {
+          if (j > 0) alpha *= exp2_fast(vref - v_up);
+          vref = v_up;
         }
-      }
-      // ---- weights: 32 columns from registers while the ones after next are read again ----
-      const float base = LIFT - (m == -INFINITY ? 0.f : m);
+        if (__any_sync(0xffffffffu, j > 0 && alpha != 1.f)) {
+          // the last block's product is complete before these scores were computed
+          rarely();
+#pragma unroll 1
+          for (int cc = 0; cc < D / 16; ++cc) {
+            uint32_t o[16];
+            tmem_ld_32x16(t_o + cc * 16, o);
+            tmem_ld_wait();
 #pragma unroll
-      for (int cc = 0; cc < FT_N / 32; ++cc) {
-        uint32_t(&u)[32] = s[cc & 1];
-        if (cc > 1) tmem_ld_wait();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float2 k = sc[cc * 2 + h];
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            tmem_st_32x16(t_o + cc * 16, o);
+          }
+        }
+        // ---- weights: a page at a time, without a branch between pages where nothing is hidden, so that their chains overlap ----
+        const float base = LIFT - (m == -INFINITY ? 0.f : m);
+        auto weigh = [&](int h, bool masked) {
+          uint32_t* u = s + h * 16;
+          const float2 k = sc[h];
           // the value scale over the largest one: 2^-60 and less weigh nothing. Out of the sum again it is taken, but for no number, which is in the weights.
           const float d = max_or_nan(k.y - vref, -60.f), f = qm * k.x, off = base + d, back = exp2_fast(fminf(60.f, -d));
           const uint64_t ff = pair_of(f, f), oo = pair_of(off, off);
 #pragma unroll
-          for (int i = h * 16; i < h * 16 + 16; i += 2) {
+          for (int i = 0; i < 16; i += 2) {
             const float2 e = of_pair(fma_pair(pair_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1])), ff, oo));
             u[i] = __float_as_uint(exp2_fast(e.x));
             u[i + 1] = __float_as_uint(exp2_fast(e.y));
           }
-          if (!whole) {
-            rarely();
+          if (masked) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if (!seen(cc * 32 + h * 16 + i)) u[h * 16 + i] = 0u;
+              if (!seen(h * 16 + i)) u[i] = 0u;
           }
-          uint64_t sum = pair_of(__uint_as_float(u[h * 16]), __uint_as_float(u[h * 16 + 1]));
+          uint64_t sum0 = pair_of(__uint_as_float(u[0]), __uint_as_float(u[1])), sum1 = pair_of(__uint_as_float(u[2]), __uint_as_float(u[3]));
 #pragma unroll
-          for (int i = h * 16 + 2; i < h * 16 + 16; i += 2) sum = add_pair(sum, pair_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1])));
-#pragma unroll
-          for (int i = h * 16; i < h * 16 + 16; i += 2) u[i / 2] = half2_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1]));
-          const float2 both = of_pair(sum);
+          for (int i = 4; i < 16; i += 4) {
+            sum0 = add_pair(sum0, pair_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1])));
+            sum1 = add_pair(sum1, pair_of(__uint_as_float(u[i + 2]), __uint_as_float(u[i + 3])));
+          }
+          const float2 both = of_pair(add_pair(sum0, sum1));
           l = fmaf(both.x + both.y, back, l);
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) s[h * 8 + i / 2] = half2_of(__uint_as_float(u[i]), __uint_as_float(u[i + 1]));
+        };
+        if (whole) {
+#pragma unroll
+          for (int h = 0; h < FT_PAGES; ++h) weigh(h, false);
+        } else {
+          rarely();
+#pragma unroll
+          for (int h = 0; h < FT_PAGES; ++h) weigh(h, true);
         }
-        tmem_st_32x16(t_lane + cc * 16, u);          // over scores that have been read
-        if (cc < 2) tmem_ld_32x32(t_lane + (cc + 2) * 32, u);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-      if (warp == 0) ok = issue_values(j) && (j + 1 == nb || issue_scores(j + 1));
-    }
-    if (ok) ok = mbar_wait_warp(o_full, (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
-    if (ok) {
-      tc_fence_after();
-      const float vscale = exp2_fast(vref), inv = l == 0.f ? 0.f : vscale / l;
-      const long at = ((long)(t0 + tok) * a.H + hd) * a.splits + split;
-#pragma unroll 1
-      for (int cc = 0; cc < D / 32; ++cc) {
-        uint32_t o[32];
-        tmem_ld_32x32(t_lane + O_COL + cc * 32, o);
-        tmem_ld_wait();
-        if (r < nr && a.splits == 1) {
-          uint4* to = reinterpret_cast<uint4*>(a.out + (t0 + tok) * a.ld_o + hd * D + cc * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t h[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
-            to[i] = make_uint4(h[0], h[1], h[2], h[3]);
-          }
-        } else if (r < nr) {
-          float4* to = reinterpret_cast<float4*>(a.part + at * D + cc * 32);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            to[i] = make_float4(__uint_as_float(o[i * 4]) * vscale, __uint_as_float(o[i * 4 + 1]) * vscale, __uint_as_float(o[i * 4 + 2]) * vscale,
-                                __uint_as_float(o[i * 4 + 3]) * vscale);
-        }
+        tmem_st_32x32(t_s, s);                         // over the scores, which are all in registers
+        tmem_st_32x32(t_s + 32, s + 32);
+        tmem_st_wait();
+        tc_fence_before();
         __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
       }
-      if (a.splits > 1 && r < nr) {
-        a.part_ml[2 * at] = m;
-        a.part_ml[2 * at + 1] = l;
-        if (split == 0) a.used[(long)(t0 + tok) * a.H + hd] = max(1, min(a.splits, (b_hi - b_lo + per - 1) / per));
+      if (ok) ok = mbar_wait_warp(&o_full[t], (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
+      if (ok) {
+        tc_fence_after();
+        const float vscale = exp2_fast(vref), inv = l == 0.f ? 0.f : vscale / l;
+        const long at = ((long)(t0 + tok) * a.H + hd) * a.splits + split;
+#pragma unroll 1
+        for (int cc = 0; cc < D / 32; ++cc) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_o + cc * 32, o);
+          tmem_ld_wait();
+          if (rt < nr && a.splits == 1) {
+            uint4* to = reinterpret_cast<uint4*>(a.out + (t0 + tok) * a.ld_o + hd * D + cc * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t h[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
+              to[i] = make_uint4(h[0], h[1], h[2], h[3]);
+            }
+          } else if (rt < nr) {
+            float4* to = reinterpret_cast<float4*>(a.part + at * D + cc * 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              to[i] = make_float4(__uint_as_float(o[i * 4]) * vscale, __uint_as_float(o[i * 4 + 1]) * vscale, __uint_as_float(o[i * 4 + 2]) * vscale,
+                                  __uint_as_float(o[i * 4 + 3]) * vscale);
+          }
+          __syncwarp();
+        }
+        if (a.splits > 1 && rt < nr) {
+          a.part_ml[2 * at] = m;
+          a.part_ml[2 * at + 1] = l;
+          if (split == 0) a.used[(long)(t0 + tok) * a.H + hd] = max(1, min(a.splits, (b_hi - b_lo + per - 1) / per));
+        }
+        tc_fence_before();
       }
-      tc_fence_before();
     }
   }
 
@@ -1104,7 +1139,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fp8_attend_tile_kernel(const __
     while (globaltimer_ns() - since < 2000000ull) __nanosleep(1000);
     __syncthreads();
   }
-  if (warp == 4) {
+  if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, COLS);
   }
@@ -1200,7 +1235,7 @@ struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
   Fp8Cut(int n, int Hkv, int G, int max_new, int max_len, int window, bool tree) {
     const long rows = (long)max_new * G;
-    blocks = rows <= 8 ? 1 : rows <= FP8_FEW_ROWS || tree ? 2 : FT_M / 8;
+    blocks = rows <= 8 ? 1 : rows <= FP8_FEW_ROWS || tree ? 2 : FT_ROWS / 8;
     tiles = (int)((rows + 8 * blocks - 1) / (8 * blocks));
     const long span = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
     const int pages = (int)((span + (window > 0 ? 2 * FP8_PAGE - 2 : FP8_PAGE - 1)) / FP8_PAGE);       // a window may begin inside a page
@@ -1215,7 +1250,7 @@ struct Fp8Cut {
     const long total = units * pages;
     long want = (total + 295) / 296;
     if (want > 128) want = total / 1184 > 128 ? total / 1184 : 128;
-    if (blocks == FT_M / 8) {                                      // whole blocks of keys
+    if (blocks == FT_ROWS / 8) {                                      // whole blocks of keys
       if (want < 4 * FT_PAGES) want = 4 * FT_PAGES;
       per = want < pages ? (int)((want + FT_PAGES - 1) / FT_PAGES * FT_PAGES) : (pages + FT_PAGES - 1) / FT_PAGES * FT_PAGES;
       splits = ((pages + FT_PAGES - 1) / FT_PAGES * FT_PAGES + (window > 0 ? FT_PAGES : 0) + per - 1) / per;
@@ -1288,7 +1323,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;
   const unsigned grid = (unsigned)ctas;
-  if (cut.blocks == FT_M / 8) return D == 64 ? fp8_attend_tile_launch<64>(a, pool, tk, grid, st) : fp8_attend_tile_launch<128>(a, pool, tk, grid, st);
+  if (cut.blocks == FT_ROWS / 8) return D == 64 ? fp8_attend_tile_launch<64>(a, pool, tk, grid, st) : fp8_attend_tile_launch<128>(a, pool, tk, grid, st);
 #define INV_FP8(DD, TREE)                                                        \
   return cut.blocks == 2  ? fp8_attend_launch<DD, 2, 4, TREE>(a, pool, tk, grid, st) \
          : cut.warps == 4 ? fp8_attend_launch<DD, 1, 4, TREE>(a, pool, tk, grid, st) \
