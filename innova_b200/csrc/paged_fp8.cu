@@ -747,38 +747,41 @@ __device__ __forceinline__ void commit_of_warp(uint64_t* bar) {
       : "memory");
 }
 
-constexpr int FT_M = 128, FT_N = 128, FT_PAGES = FT_N / FP8_PAGE, FT_ROWS = 2 * FT_M;
+constexpr int FT_M = 128, FT_N = 64, FT_PAGES = FT_N / FP8_PAGE, FT_ROWS = 2 * FT_M;
 constexpr int FT_THREADS = 512;        // two groups of four warps for the softmax of a tile each, one that converts, one whose first warp issues the products
-constexpr int FT_SLOTS = 2;            // of keys and of values
+constexpr int FT_SLOTS = 4;            // of keys and of values
 template <int D>
 struct FtSmem {
-  static constexpr int TILE = FT_M * D * 2;          // fp16 rows in pieces of 64 columns with the 128-byte swizzle: queries, keys, values
-  static constexpr int TOTAL = (2 + 2 * FT_SLOTS) * TILE + 1024;
+  static constexpr int QUERIES = FT_M * D * 2, KEYS = FT_N * D * 2;        // fp16 rows in pieces of 64 columns with the 128-byte swizzle
+  static constexpr int TOTAL = 2 * QUERIES + 2 * FT_SLOTS * KEYS + 1024;
 };
 
-// 256 rows (query tokens times the heads that share a key head) as two tiles against blocks of 128 keys on the tcgen05 tensor cores: prompts behind a cache,
+// 256 rows (query tokens times the heads that share a key head) as two tiles against blocks of 64 keys on the tcgen05 tensor cores: prompts behind a cache,
 // and drafts of more than a few tokens. grid = row tiles (the longest first) x splits x key heads x sequences, one CTA an SM.
 //   warps 0-7    softmax, a row a thread: scores from tensor memory, weights in fp16 back in their place
 //   warps 8-11   codes of the next blocks from the pages to registers, as fp16 to shared memory, for both tiles
-//   warp 12      issues S = Q K^T and O += P V (P from tensor memory) of the tiles in turn: one's softmax runs under the other's products
+//   warps 12-13  issue a tile's S = Q K^T and O += P V (P from tensor memory)
+// A tile has two places for scores: the next block's are computed under this one's softmax, so that a row's chain does not wait for products (with one, and
+// blocks of 128 keys, a tile's softmax and products took turns: 548 us for 2 x 1500 tokens on 5500, 32 heads of 128 on 8).
 // Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are powers of two added to it (relative to the
 // largest one so far, which O is kept in) and taken out of the row sum again a page at a time, so neither costs anything a score. For the rest the sums are
-// those of the small kernel. Tensor memory, of 512 columns: scores (then weights) 0 and 128, O 256 and 384.
+// those of the small kernel. Tensor memory, a tile 256 columns: scores (then weights) at 0 and 64, O at 128.
 template <int D>
 __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
                                                                         const __grid_constant__ Fp8Tokens tk) {
   using L = FtSmem<D>;
   constexpr int CH = D / 16, NS = FT_SLOTS;          // 16-byte pieces of a token's codes
   constexpr float LIFT = 6.f, SLACK = 8.f;
-  constexpr uint32_t O_COL = 256, COLS = 512;
+  constexpr uint32_t T_COLS = 256, O_COL = 128, COLS = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = smem, *sK = smem + 2 * L::TILE, *sV = smem + (2 + NS) * L::TILE;
-  __shared__ __align__(8) uint64_t q_full[2], k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2], p_full[2], o_full[2], scales_full[4];
-  // Of a block's pages: the keys' scale, log2 of the values'; bit p of `present`: page p is there. Block j + 4 takes block j's place once the scores of
-  // block j + 2 are computed, which both tiles ask for behind their softmax of block j.
-  __shared__ float2 scales[4][FT_PAGES];
-  __shared__ uint32_t present[4];
+  uint8_t *sQ = smem, *sK = smem + 2 * L::QUERIES, *sV = sK + NS * L::KEYS;
+  // s_full and p_full: [tile][even or odd block]
+  __shared__ __align__(8) uint64_t q_full[2], k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_full[2], scales_full[8];
+  // Of a block's pages: the keys' scale, log2 of the values'; bit p of `present`: page p is there. Block j + 8 takes block j's place once the scores of
+  // block j + 4 are computed, which both tiles ask for behind their softmax of block j + 2.
+  __shared__ float2 scales[8][FT_PAGES];
+  __shared__ uint32_t present[8];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
@@ -806,19 +809,22 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 4);
-      mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
       mbar_init(&o_full[i], 1);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[i][b], 1);
+        mbar_init(&p_full[i][b], 4);
+      }
     }
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       mbar_init(&k_full[i], 4);
-      mbar_init(&k_empty[i], 1);
+      mbar_init(&k_empty[i], tiles);
       mbar_init(&v_full[i], 4);
-      mbar_init(&v_empty[i], 1);
+      mbar_init(&v_empty[i], tiles);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mbar_init(&scales_full[i], 1);
+    for (int i = 0; i < 8; ++i) mbar_init(&scales_full[i], 1);
     abort_word = 0;
     fence_barrier_init();
   }
@@ -831,59 +837,52 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  // 512 x 128 registers at launch; 128 x (184 + 184 + 96 + 40) behind these
   if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 12) {
+    // ---------------- products of tile t. A wait that is over costs its warp some 150 cycles all the same, so each tile has a warp to itself ----------------
+    const int t = warp - 12;
+    if (t < tiles) {
       constexpr uint32_t idesc_qk = make_idesc_f16(FT_M, FT_N, 0), idesc_pv = make_idesc_f16(FT_M, D, 1);
-      const uint64_t desc_q = make_smem_desc(smem_u32(sQ), 16, 1024, 2), desc_k = make_smem_desc(smem_u32(sK), 16, 1024, 2),
+      const uint64_t desc_q = make_smem_desc(smem_u32(sQ) + t * L::QUERIES, 16, 1024, 2), desc_k = make_smem_desc(smem_u32(sK), 16, 1024, 2),
                      desc_v = make_smem_desc(smem_u32(sV), FT_N * 128, 1024, 2);               // steps of a product add to the address field
-      auto scores = [&](int t, int j) {
-        const uint64_t dq = desc_q + (uint64_t)(t * L::TILE >> 4), dk = desc_k + (uint64_t)((j % NS) * L::TILE >> 4);
-#pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint64_t off = ((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4;
-          mma_of_warp(tmem + t * FT_N, dq + off, dk + off, idesc_qk, s > 0);
-        }
-        commit_of_warp(&s_full[t]);
-        if (t + 1 == tiles) commit_of_warp(&k_empty[j % NS]);
-      };
-      bool ok = mbar_wait_warp(&k_full[0], 0, abort_flag, tk.status, ERR_WAIT_FULL);
-      for (int t = 0; ok && t < tiles; ++t) {
-        ok = mbar_wait_warp(&q_full[t], 0, abort_flag, tk.status, ERR_WAIT_FULL);
+      const uint32_t t_s = tmem + t * T_COLS, t_o = t_s + O_COL;
+      // scores of block j in the place of the weights of block j - 2, whose product is complete
+      auto scores = [&](int j) -> bool {
+        const int slot = j % NS;
+        if (!mbar_wait_warp(&k_full[slot], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
+        if (j > 1 && !mbar_wait_warp(&o_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) return false;
         tc_fence_after();
-        if (ok) scores(t, 0);
-      }
-      for (int j = 0; ok && j < nb; ++j) {
-        ok = mbar_wait_warp(&v_full[j % NS], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL) &&
-             (j + 1 == nb || mbar_wait_warp(&k_full[(j + 1) % NS], ((j + 1) / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL));
-        for (int t = 0; ok && t < tiles; ++t) {
-          ok = mbar_wait_warp(&p_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_MISC);
-          if (!ok) break;
-          tc_fence_after();
-          const uint64_t dv = desc_v + (uint64_t)((j % NS) * L::TILE >> 4);
+        const uint64_t dk = desc_k + (uint64_t)(slot * L::KEYS >> 4);
 #pragma unroll
-          for (int s = 0; s < FT_N / 16; ++s)        // 16 keys: eight packed columns of weights
-            mma_of_warp_tmem(tmem + O_COL + t * 128, tmem + t * FT_N + s * 8, dv + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
-          commit_of_warp(&o_full[t]);
-          if (t + 1 == tiles) commit_of_warp(&v_empty[j % NS]);
-          if (j + 1 == nb) continue;
-          // the next scores take the place of the weights that this product reads
-          ok = mbar_wait_warp(&o_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
-          tc_fence_after();
-          if (ok) scores(t, j + 1);
-        }
-      }
+        for (int s = 0; s < D / 16; ++s)
+          mma_of_warp(t_s + (j & 1) * FT_N, desc_q + (((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4), dk + (((s / 4) * (FT_N * 128) + (s % 4) * 32) >> 4),
+                      idesc_qk, s > 0);
+        commit_of_warp(&s_full[t][j & 1]);
+        commit_of_warp(&k_empty[slot]);
+        return true;
+      };
+      auto values = [&](int j) -> bool {
+        const int slot = j % NS;
+        if (!mbar_wait_warp(&v_full[slot], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
+        if (!mbar_wait_warp(&p_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_MISC)) return false;
+        tc_fence_after();
+        const uint64_t dv = desc_v + (uint64_t)(slot * L::KEYS >> 4);
+#pragma unroll
+        for (int s = 0; s < FT_N / 16; ++s)          // 16 keys: eight packed columns of weights
+          mma_of_warp_tmem(t_o, t_s + (j & 1) * FT_N + s * 8, dv + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
+        commit_of_warp(&o_full[t]);
+        commit_of_warp(&v_empty[slot]);
+        return true;
+      };
+      bool ok = mbar_wait_warp(&q_full[t], 0, abort_flag, tk.status, ERR_WAIT_FULL) && scores(0) && (nb == 1 || scores(1));
+      for (int j = 0; ok && j < nb; ++j) ok = values(j) && (j + 2 >= nb || scores(j + 2));
     }
   } else if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
     // ---------------- conversion: a thread takes the same piece of every sixteenth (D = 64: thirty-second) token ----------------
     const int tid = threadIdx.x - 256;
     constexpr int PER = FT_N * CH / 128, STEP = 128 / CH;      // pieces of a thread in a block; tokens from one to the next
     const int piece = tid % CH, tok0 = tid / CH, pages_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
-    uint4 raw[PER];
-    // Lanes 0 to 7 look a block's pages up: read two blocks ahead, checked one ahead, scales read then, so that nothing is waited for. Loads stand outside of
-    // branches, from a place that exists where there is none to read: behind a branch the compiler copies what was loaded, and so waits for each in turn.
+    uint4 rk[2][PER], rv[2][PER];                    // of even and odd blocks, two ahead
+    // Lanes 0 to 3 look a block's pages up: read three blocks ahead, checked two ahead and codes and scales read then, so that nothing is waited for. Loads stand outside of branches, from a place that exists where there is none to read: behind a branch the compiler copies what was loaded, and so waits for each in turn.
     const bool known = (unsigned)row < (unsigned)tk.table_rows;
     const int* list = tk.page_table + (known ? (long)row * tk.max_pages : 0);
     auto read_id = [&](int j) { return list[min((b0 + j) * FT_PAGES + lane, tk.max_pages - 1)]; };
@@ -895,14 +894,14 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       return -1;
     };
     auto scale_at = [&](const float* of, int id) { return of[(long)max(id, 0) * pool.Hkv + hk]; };
-    auto load = [&](const uint8_t* codes, int ids) {
+    auto load = [&](uint4 (&raw)[PER], const uint8_t* codes, int ids) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int tok = tok0 + i * STEP, pid = max(__shfl_sync(0xffffffffu, ids, tok / FP8_PAGE), 0);
         raw[i] = *reinterpret_cast<const uint4*>(codes + (((long)pid * pool.Hkv + hk) * FP8_PAGE + tok % FP8_PAGE) * D + piece * 16);
       }
     };
-    auto store = [&](uint8_t* dst, uint64_t* bar) {
+    auto store = [&](const uint4 (&raw)[PER], uint8_t* dst, uint64_t* bar) {
       const int at = 2 * piece;                                                  // 16-byte pieces `at` and `at` + 1 of a token's fp16 row
       const bool odd = piece >= CH / 2;                                          // lanes of the second half store in the other order: no bank twice
       uint8_t* to = dst + (at >> 3) * (FT_N * 128) + tok0 * 128;
@@ -920,45 +919,50 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       if (lane == 0) mbar_arrive(bar);
     };
     static_assert(STEP % 8 == 0, "a thread's tokens share a swizzle");
-    int id = check_id(read_id(0), 0), read = read_id(1);
-    float ks = scale_at(pool.k_scale, id), vs = scale_at(pool.v_scale, id);
-    for (int j = 0; j < nb; ++j) {
+    int id[2] = {check_id(read_id(0), 0), check_id(read_id(1), 1)}, read = read_id(2);
+    float ks[2] = {scale_at(pool.k_scale, id[0]), scale_at(pool.k_scale, id[1])}, vs[2] = {scale_at(pool.v_scale, id[0]), scale_at(pool.v_scale, id[1])};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      load(rk[e], pool.k, id[e]);
+      load(rv[e], pool.v, id[e]);
+    }
+    auto block = [&](int j, int e) -> bool {
       const int slot = j % NS, turn = ((j / NS) & 1) ^ 1;
-      load(pool.k, id);
-      const int id_n = check_id(read, j + 1);
-      read = read_id(j + 2);
-      const float ks_n = scale_at(pool.k_scale, id_n), vs_n = scale_at(pool.v_scale, id_n);
-      const uint32_t there = __ballot_sync(0xffffffffu, id >= 0);
-      if (!mbar_wait_warp(&k_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
+      const uint32_t there = __ballot_sync(0xffffffffu, id[e] >= 0);
+      if (!mbar_wait_warp(&k_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) return false;
       if (warp == 8) {
-        if (lane < FT_PAGES) scales[j & 3][lane] = id >= 0 ? make_float2(ks, log2_scale(vs)) : make_float2(0.f, -127.f);
-        if (lane == 0) present[j & 3] = there;
+        if (lane < FT_PAGES) scales[j & 7][lane] = id[e] >= 0 ? make_float2(ks[e], log2_scale(vs[e])) : make_float2(0.f, -127.f);
+        if (lane == 0) present[j & 7] = there;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&scales_full[j & 3]);
+        if (lane == 0) mbar_arrive(&scales_full[j & 7]);
       }
-      store(sK + slot * L::TILE, &k_full[slot]);
-      load(pool.v, id);
-      if (!mbar_wait_warp(&v_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) break;
+      store(rk[e], sK + slot * L::KEYS, &k_full[slot]);
+      id[e] = check_id(read, j + 2);
+      read = read_id(j + 3);
+      load(rk[e], pool.k, id[e]);
+      ks[e] = scale_at(pool.k_scale, id[e]);
+      vs[e] = scale_at(pool.v_scale, id[e]);
+      if (!mbar_wait_warp(&v_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) return false;
       if ((b0 + j + 1) * FT_N > hi || there != (1u << FT_PAGES) - 1) {           // values that are not there are nothing, whatever was read
         rarely();
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const int tok = tok0 + i * STEP;
-          if ((b0 + j) * FT_N + tok >= hi || !((there >> (tok / FP8_PAGE)) & 1)) raw[i] = make_uint4(0, 0, 0, 0);
+          if ((b0 + j) * FT_N + tok >= hi || !((there >> (tok / FP8_PAGE)) & 1)) rv[e][i] = make_uint4(0, 0, 0, 0);
         }
       }
-      store(sV + slot * L::TILE, &v_full[slot]);
-      id = id_n;
-      ks = ks_n;
-      vs = vs_n;
-    }
+      store(rv[e], sV + slot * L::KEYS, &v_full[slot]);
+      load(rv[e], pool.v, id[e]);
+      return true;
+    };
+    for (int j = 0; j < nb; j += 2)
+      if (!block(j, 0) || (j + 1 < nb && !block(j + 1, 1))) break;
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ---------------- softmax: thread <-> row r of tile t ----------------
     const int t = warp >> 2, r = threadIdx.x & 127, rt = t * FT_M + r, rr = r0 + min(rt, nr - 1), tok = div_by(rr, a.G, a.inv_g);
     const int hd = hk * a.G + rr - tok * a.G;
     const int kmax = start + tok, kmin = a.window > 0 ? kmax - a.window + 1 : 0;
-    const uint32_t t_lane = tmem + (uint32_t((warp & 3) * 32) << 16), t_s = t_lane + t * FT_N, t_o = t_lane + O_COL + t * 128;
+    const uint32_t t_lane = tmem + (uint32_t((warp & 3) * 32) << 16), t_o = t_lane + t * T_COLS + O_COL;
     if (t < tiles) {
       float qm;
       {                                              // the row's queries, scaled by a power of two, as fp16 rows for the products
@@ -982,7 +986,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           uint32_t h[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) h[k] = half2_of(__uint_as_float(v[k] << 16) * down, __uint_as_float(v[k] & 0xffff0000u) * down);
-          *reinterpret_cast<uint4*>(sQ + t * L::TILE + (i >> 3) * (FT_M * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(sQ + t * L::QUERIES + (i >> 3) * (FT_M * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -992,18 +996,19 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       float m = -INFINITY, l = 0.f, vref = -200.f;     // vref: log2 of the scale that O is kept in
       bool ok = true;
       for (int j = 0; j < nb; ++j) {
-        if (!mbar_wait_warp(&scales_full[j & 3], (j >> 2) & 1, abort_flag, tk.status, ERR_WAIT_FULL) ||
-            !mbar_wait_warp(&s_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
+        if (!mbar_wait_warp(&scales_full[j & 7], (j >> 3) & 1, abort_flag, tk.status, ERR_WAIT_FULL) ||
+            !mbar_wait_warp(&s_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
           ok = false;
           break;
         }
         tc_fence_after();
         uint32_t s[FT_N];
+        const uint32_t t_s = t_lane + t * T_COLS + (j & 1) * FT_N;
 #pragma unroll
         for (int cc = 0; cc < FT_N / 32; ++cc) tmem_ld_32x32(t_s + cc * 32, s + cc * 32);
-        const float2* sc = scales[j & 3];
+        const float2* sc = scales[j & 7];
         const int k0 = (b0 + j) * FT_N;
-        const uint32_t there = present[j & 3];
+        const uint32_t there = present[j & 7];
         const bool whole = k0 >= all_lo && k0 + FT_N <= all_hi && there == (1u << FT_PAGES) - 1;
         auto seen = [&](int i) { const int k = k0 + i; return k <= kmax && k >= kmin && ((there >> (i / FP8_PAGE)) & 1); };
         tmem_ld_wait();
@@ -1028,26 +1033,31 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           mx = fmaxf(mx, fmaxf(x0, x1) * (qm * k.x));
           v_up = fmaxf(v_up, k.y);
         }
-        const bool raise = j == 0 || mx > m + SLACK;
-        const float up = raise ? fmaxf(m, mx) : m;
-        float alpha = j == 0 || up == m ? 1.f : exp2_fast(m - up);
-        m = up;
-        l *= alpha;
-        if (v_up > vref) {
-          if (j > 0) alpha *= exp2_fast(vref - v_up);
-          vref = v_up;
-        }
-        if (__any_sync(0xffffffffu, j > 0 && alpha != 1.f)) {
-          // the last block's product is complete before these scores were computed
+        if (__any_sync(0xffffffffu, mx > m + SLACK || v_up > vref)) {
           rarely();
+          const float up = j == 0 || mx > m + SLACK ? fmaxf(m, mx) : m;
+          float alpha = up == m ? 1.f : exp2_fast(m - up);
+          m = up;
+          l *= alpha;
+          if (v_up > vref) {
+            alpha *= exp2_fast(vref - v_up);
+            vref = v_up;
+          }
+          if (j > 0) {                                 // O is that of the blocks before, once the last one's product is complete
+            if (!mbar_wait_warp(&o_full[t], (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
 #pragma unroll 1
-          for (int cc = 0; cc < D / 16; ++cc) {
-            uint32_t o[16];
-            tmem_ld_32x16(t_o + cc * 16, o);
-            tmem_ld_wait();
+            for (int cc = 0; cc < D / 16; ++cc) {
+              uint32_t o[16];
+              tmem_ld_32x16(t_o + cc * 16, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-            tmem_st_32x16(t_o + cc * 16, o);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x16(t_o + cc * 16, o);
+            }
           }
         }
         // ---- weights: a page at a time, without a branch between pages where nothing is hidden, so that their chains overlap ----
@@ -1089,12 +1099,13 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           for (int h = 0; h < FT_PAGES; ++h) weigh(h, true);
         }
         tmem_st_32x32(t_s, s);                         // over the scores, which are all in registers
-        tmem_st_32x32(t_s + 32, s + 32);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        if (lane == 0) mbar_arrive(&p_full[t][j & 1]);
       }
+      // the last two products, in turn: a barrier's parity tells a phase from the next one only
+      if (ok && nb > 1) ok = mbar_wait_warp(&o_full[t], nb & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
       if (ok) ok = mbar_wait_warp(&o_full[t], (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
       if (ok) {
         tc_fence_after();
