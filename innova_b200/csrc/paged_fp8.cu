@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = smem + 2 * L::QUERIES, *sV = sK + NS * L::KEYS;
   // s_full and p_full: [tile][even or odd block]
-  __shared__ __align__(8) uint64_t q_full[2], k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_full[2], scales_full[8];
+  __shared__ __align__(8) uint64_t q_full[2], k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_full[2];
   // Of a block's pages: the keys' scale, log2 of the values'; bit p of `present`: page p is there. Block j + 8 takes block j's place once the scores of
   // block j + 4 are computed, which both tiles ask for behind their softmax of block j + 2.
   __shared__ float2 scales[8][FT_PAGES];
@@ -812,7 +812,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       mbar_init(&o_full[i], 1);
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        mbar_init(&s_full[i][b], 1);
+        mbar_init(&s_full[i][b], 2);
         mbar_init(&p_full[i][b], 4);
       }
     }
@@ -823,8 +823,6 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       mbar_init(&v_full[i], 4);
       mbar_init(&v_empty[i], tiles);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mbar_init(&scales_full[i], 1);
     abort_word = 0;
     fence_barrier_init();
   }
@@ -848,7 +846,6 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       // scores of block j in the place of the weights of block j - 2, whose product is complete
       auto scores = [&](int j) -> bool {
         const int slot = j % NS;
-        if (!mbar_wait_warp(&k_full[slot], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
         if (j > 1 && !mbar_wait_warp(&o_full[t], j & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) return false;
         tc_fence_after();
         const uint64_t dk = desc_k + (uint64_t)(slot * L::KEYS >> 4);
@@ -858,11 +855,15 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
                       idesc_qk, s > 0);
         commit_of_warp(&s_full[t][j & 1]);
         commit_of_warp(&k_empty[slot]);
+        if (lane == 0) mbar_arrive(&s_full[t][j & 1]);         // with it goes on what came with the keys: the block's scales
+        __syncwarp();
         return true;
       };
+      auto keys = [&](int j) { return mbar_wait_warp(&k_full[j % NS], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL); };
       auto values = [&](int j) -> bool {
         const int slot = j % NS;
         if (!mbar_wait_warp(&v_full[slot], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
+        if (j + 2 < nb && !keys(j + 2)) return false;                            // while the weights are not there yet
         if (!mbar_wait_warp(&p_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_MISC)) return false;
         tc_fence_after();
         const uint64_t dv = desc_v + (uint64_t)(slot * L::KEYS >> 4);
@@ -873,7 +874,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
         commit_of_warp(&v_empty[slot]);
         return true;
       };
-      bool ok = mbar_wait_warp(&q_full[t], 0, abort_flag, tk.status, ERR_WAIT_FULL) && scores(0) && (nb == 1 || scores(1));
+      bool ok = mbar_wait_warp(&q_full[t], 0, abort_flag, tk.status, ERR_WAIT_FULL) && keys(0) && scores(0) && (nb == 1 || (keys(1) && scores(1)));
       for (int j = 0; ok && j < nb; ++j) ok = values(j) && (j + 2 >= nb || scores(j + 2));
     }
   } else if (warp >= 8) {
@@ -933,8 +934,6 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       if (warp == 8) {
         if (lane < FT_PAGES) scales[j & 7][lane] = id[e] >= 0 ? make_float2(ks[e], log2_scale(vs[e])) : make_float2(0.f, -127.f);
         if (lane == 0) present[j & 7] = there;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&scales_full[j & 7]);
       }
       store(rk[e], sK + slot * L::KEYS, &k_full[slot]);
       id[e] = check_id(read, j + 2);
@@ -996,8 +995,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       float m = -INFINITY, l = 0.f, vref = -200.f;     // vref: log2 of the scale that O is kept in
       bool ok = true;
       for (int j = 0; j < nb; ++j) {
-        if (!mbar_wait_warp(&scales_full[j & 7], (j >> 3) & 1, abort_flag, tk.status, ERR_WAIT_FULL) ||
-            !mbar_wait_warp(&s_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
+        if (!mbar_wait_warp(&s_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
           ok = false;
           break;
         }
