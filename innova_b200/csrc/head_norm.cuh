@@ -21,48 +21,67 @@ struct HeadUnit {
   __device__ __forceinline__ HeadUnit(int u, int D, int rot) {
     has = u * 16 < D;
     turns = u * 16 < rot;
-    e0 = turns ? u * 8 : u * 16;
-    e1 = turns ? rot / 2 + u * 8 : u * 16 + 8;
+    e0 = turns ? u * 8 : has ? u * 16 : 0;              // a lane without a unit reads the head's first values
+    e1 = turns ? rot / 2 + u * 8 : e0 + 8;
   }
 };
 
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float* f) {
-  const uint4 r = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-  }
-}
 __device__ __forceinline__ void load8(const float* p, float* f) {
   const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
   f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
   f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float* f) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(cvt_bf16x2(f[0], f[1]), cvt_bf16x2(f[2], f[3]), cvt_bf16x2(f[4], f[5]), cvt_bf16x2(f[6], f[7]));
-}
-__device__ __forceinline__ void store8(float* p, const float* f) {
-  *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
-}
+
+// A unit as it lies in memory: fetched without a branch, so that several are on their way at once, and widened when they are there.
+template <typename T>
+struct RawUnit {
+  static constexpr int N = sizeof(T) / 2;               // 16-byte pieces of a run
+  uint4 r[2 * N];
+  __device__ __forceinline__ void fetch(const T* head, const HeadUnit& u) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      r[i] = reinterpret_cast<const uint4*>(head + u.e0)[i];
+      r[N + i] = reinterpret_cast<const uint4*>(head + u.e1)[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* head, const HeadUnit& u) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      reinterpret_cast<uint4*>(head + u.e0)[i] = r[i];
+      reinterpret_cast<uint4*>(head + u.e1)[i] = r[N + i];
+    }
+  }
+  __device__ __forceinline__ void get(const HeadUnit& u, float (&x)[16]) const {
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+      const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (N == 1) {
+          x[i * 8 + 2 * k] = u.has ? __uint_as_float(w[k] << 16) : 0.f;
+          x[i * 8 + 2 * k + 1] = u.has ? __uint_as_float(w[k] & 0xffff0000u) : 0.f;
+        } else {
+          x[i * 4 + k] = u.has ? __uint_as_float(w[k]) : 0.f;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+      if constexpr (N == 1)
+        r[i] = make_uint4(cvt_bf16x2(x[i * 8], x[i * 8 + 1]), cvt_bf16x2(x[i * 8 + 2], x[i * 8 + 3]), cvt_bf16x2(x[i * 8 + 4], x[i * 8 + 5]),
+                          cvt_bf16x2(x[i * 8 + 6], x[i * 8 + 7]));
+      else
+        r[i] = make_uint4(__float_as_uint(x[i * 4]), __float_as_uint(x[i * 4 + 1]), __float_as_uint(x[i * 4 + 2]), __float_as_uint(x[i * 4 + 3]));
+    }
+  }
+};
 template <typename T>
 __device__ __forceinline__ void load_unit(const T* head, const HeadUnit& u, float (&x)[16]) {
-  if (u.has) {
-    load8(head + u.e0, x);
-    load8(head + u.e1, x + 8);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = 0.f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store_unit(T* head, const HeadUnit& u, const float (&x)[16]) {
-  if (u.has) {
-    store8(head + u.e0, x);
-    store8(head + u.e1, x + 8);
-  }
+  RawUnit<T> raw;
+  raw.fetch(head, u);
+  raw.get(u, x);
 }
 
 // Sum over the L lanes of a head.
@@ -85,8 +104,7 @@ __device__ __forceinline__ float head_rstd(const float (&x)[16], float inv_d, fl
 struct Turn {
   float c[8], s[8];
   __device__ __forceinline__ void load(const float* cos_t, const float* sin_t, int rot, int pos, int u, const HeadUnit& h) {
-    if (!h.turns) return;
-    const size_t at = (size_t)pos * (rot / 2) + u * 8;
+    const size_t at = (size_t)pos * (rot / 2) + (h.turns ? u * 8 : 0);
     load8(cos_t + at, c);
     load8(sin_t + at, s);
   }

@@ -70,111 +70,132 @@ struct Fp8Append {
   __nv_bfloat16* q;
   long ld_in, ld_v, ld_q;
   int H, rot, table_rows;
+  uint32_t inv_h;                       // div_reciprocal
   float eps;
 };
 
-// A CTA takes the new tokens of one page, and of the heads its share blockIdx.y. Sequence i owns the CTAs from cu[i] / 16 + 2 i on, which is enough for
-// the pages that its tokens touch wherever it starts. A warp stores the keys or values of one head: all of the page's new tokens in its registers, so
-// that their largest value is known before any is rounded; queries it takes by groups of tokens, whose angles are loaded once.
+// A CTA takes the new tokens of one page, or with blockIdx.y a share of what they bring: items for its warps. Sequence i owns the CTAs from cu[i] / 16 + 2 i
+// on, which is enough for the pages that its tokens touch wherever it starts. An item is the keys or the values of one head, all of the page's new tokens
+// in a warp's registers, so that their largest value is known before any is rounded; or a run of query heads. Rows stay in registers as they were read
+// (keys are normed and turned twice, for their largest value and for the codes), so that three CTAs an SM keep four units a lane on their way.
 template <int D>
-__global__ void __launch_bounds__(256) fp8_append_kernel(const __grid_constant__ Fp8Append a, const __grid_constant__ Fp8Pool pool,
-                                                         const __grid_constant__ Fp8Tokens tk) {
-  constexpr int L = D / 16, HPW = 32 / L, NIT = FP8_PAGE / HPW;
-  __shared__ int found[2];
+__global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constant__ Fp8Append a, const __grid_constant__ Fp8Pool pool,
+                                                            const __grid_constant__ Fp8Tokens tk) {
+  constexpr int L = D / 16, HPW = 32 / L, NIT = FP8_PAGE / HPW, NQ = 4;
+  using Raw = RawUnit<__nv_bfloat16>;
+  __shared__ int found[5];
   if (threadIdx.x == 0) found[0] = -1;
   __syncthreads();
   wait_previous();
   release_next();
   for (int i = threadIdx.x; i < tk.n; i += 256) {
-    const int base = tk.cu[i] / FP8_PAGE + 2 * i, next = tk.cu[i + 1] / FP8_PAGE + 2 * (i + 1);
+    const int c0 = tk.cu[i], c1 = tk.cu[i + 1], start = tk.start[i], row = tk.rows[i];
+    const int base = c0 / FP8_PAGE + 2 * i, next = c1 / FP8_PAGE + 2 * (i + 1);
     if (base <= (int)blockIdx.x && (int)blockIdx.x < next) {
-      found[0] = i;
-      found[1] = base;
+      found[0] = base;
+      found[1] = c0;
+      found[2] = c1;
+      found[3] = start;
+      found[4] = row;
     }
   }
   __syncthreads();
-  const int seq = found[0];
-  if (seq < 0) return;
-  const int t0 = tk.cu[seq], count = tk.cu[seq + 1] - t0, start = tk.start[seq];
+  if (found[0] < 0) return;
+  const int t0 = found[1], count = found[2] - t0, start = found[3], row = found[4];
   if (t0 < 0 || count < 0 || count > tk.T - t0 || start < 0) {
     if (threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
     return;
   }
-  const int pg = start / FP8_PAGE + ((int)blockIdx.x - found[1]);
+  const int pg = start / FP8_PAGE + ((int)blockIdx.x - found[0]);
   const int lo = max(start, pg * FP8_PAGE), m = min(start + count, (pg + 1) * FP8_PAGE) - lo;      // positions [lo, lo + m)
   if (m <= 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, u = lane % L, sub = lane / L;
-  const int groups = (m + HPW - 1) / HPW;
-  const int zs = gridDim.y, z = blockIdx.y;
-  const int h0 = (int)((long)a.H * z / zs), h1 = (int)((long)a.H * (z + 1) / zs);
-  const int g0 = (int)((long)pool.Hkv * 2 * z / zs), g1 = (int)((long)pool.Hkv * 2 * (z + 1) / zs);
-  const int page = pool_page(tk, pool.pages, tk.rows[seq], pg);
+  const bool listed = (unsigned)row < (unsigned)tk.table_rows && (unsigned)pg < (unsigned)tk.max_pages;
+  const int id = tk.page_table[listed ? (long)row * tk.max_pages + pg : 0];
   const HeadUnit h(u, D, a.rot);
-  // queries: (group of tokens, a run of heads)
-  const int run = max(1, (h1 - h0) * groups / 16), runs = (h1 - h0 + run - 1) / run;      // none without query heads
-  const int n_kv = page < 0 ? 0 : g1 - g0;
-  for (int item = warp; item < n_kv + groups * runs; item += 8) {
+  const int first = t0 + lo - start;                             // row of the page's first new token
+  auto angles = [&](Turn& turn, int i) {
+    turn.load(a.cos_t, a.sin_t, a.rot, table_row(a.pos ? a.pos[first + i] : lo + i, a.table_rows, tk.status), u, h);
+  };
+  const int n_kv = 2 * pool.Hkv, n_q = (m * a.H + NQ * HPW - 1) / (NQ * HPW);
+  for (int item = blockIdx.y * 8 + warp; item < n_kv + n_q; item += gridDim.y * 8) {
     if (item >= n_kv) {
-      const int grp = (item - n_kv) % groups, hq = h0 + (item - n_kv) / groups * run;
-      const int i = grp * HPW + sub;
-      const bool ok = i < m;
-      const int at = lo + min(i, m - 1), t = t0 + at - start;
+      // ---- heads of tokens, one behind the other ----
+      const int s0 = (item - n_kv) * (NQ * HPW) + sub;
+      Raw raw[NQ];
+      int tok[NQ], hd[NQ];
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        const int s = min(s0 + j * HPW, m * a.H - 1);
+        tok[j] = div_by(s, a.H, a.inv_h);
+        hd[j] = s - tok[j] * a.H;
+        raw[j].fetch(a.q_in + (first + tok[j]) * a.ld_in + hd[j] * D, h);
+      }
       Turn turn;
-      if (a.rot) turn.load(a.cos_t, a.sin_t, a.rot, table_row(a.pos ? a.pos[t] : at, a.table_rows, tk.status), u, h);
-      float w[16];
-      if (a.wq) load_unit(a.wq, h, w);
-      const __nv_bfloat16* src = a.q_in + t * a.ld_in;
-      __nv_bfloat16* dst = a.q + t * a.ld_q;
-#pragma unroll 2
-      for (int hd = hq; hd < min(h1, hq + run); ++hd) {
+      if (a.rot) angles(turn, tok[0]);
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        if (j && a.rot && tok[j] != tok[j - 1]) angles(turn, tok[j]);
         float v[16];
-        load_unit(src + hd * D, h, v);
+        raw[j].get(h, v);
         if (a.wq) {
           const float r = head_rstd<L>(v, 1.f / D, a.eps);
+          float w[16];
+          load_unit(a.wq, h, w);
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
         }
-        turn.apply<false>(h, v);
-        if (ok) store_unit(dst + hd * D, h, v);
+        if (a.rot) turn.apply<false>(h, v);
+        raw[j].set(v);
+        if (s0 + j * HPW < m * a.H) raw[j].store(a.q + (first + tok[j]) * a.ld_q + hd[j] * D, h);
       }
       continue;
     }
-    const int g = g0 + item, hk = g >> 1, which = g & 1;         // 0 keys, 1 values
+    // ---- keys or values of a head ----
+    const int hk = item >> 1, which = item & 1;                  // 0 keys, 1 values
     const __nv_bfloat16* src = (which ? a.v_in : a.k_in) + hk * D;
     const long ld = which ? a.ld_v : a.ld_in;
-    float x[NIT][16];
+    Raw raw[NIT];
+#pragma unroll
+    for (int it = 0; it < NIT; ++it) raw[it].fetch(src + (first + min(it * HPW + sub, m - 1)) * ld, h);      // lanes past the last token repeat it
+    if (!listed || (unsigned)id >= (unsigned)pool.pages) {
+      if (lane == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
+      continue;
+    }
+    const long block = (long)id * pool.Hkv + hk;
+    uint8_t* codes = (which ? pool.v : pool.k) + block * FP8_PAGE * D;
+    float* scales = (which ? pool.v_scale : pool.k_scale) + block;
+    const float old = *scales;
+    auto values = [&](int it, float (&x)[16]) {
+      raw[it].get(h, x);
+      if (which) return;
+      if (a.wk) {
+        float w[16];
+        load_unit(a.wk, h, w);
+        const float r = head_rstd<L>(x, 1.f / D, a.eps);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = x[e] * r * w[e];
+      }
+      if (a.rot) {
+        Turn turn;
+        angles(turn, min(it * HPW + sub, m - 1));
+        turn.apply<false>(h, x);
+      }
+    };
     uint32_t amax = 0;
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      if (it >= groups) break;
-      const int at = lo + min(it * HPW + sub, m - 1), t = t0 + at - start;      // lanes past the last token repeat it
-      load_unit(src + t * ld, h, x[it]);
-      if (!which) {
-        if (a.wk) {
-          float w[16];
-          load_unit(a.wk, h, w);
-          const float r = head_rstd<L>(x[it], 1.f / D, a.eps);
+      if (it * HPW >= m) break;
+      float x[16];
+      values(it, x);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[it][e] = x[it][e] * r * w[e];
-        }
-        if (a.rot) {
-          Turn turn;
-          turn.load(a.cos_t, a.sin_t, a.rot, table_row(a.pos ? a.pos[t] : at, a.table_rows, tk.status), u, h);
-          turn.apply<false>(h, x[it]);
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(x[it][e]) & 0x7fffffffu);
+      for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7fffffffu);
     }
     amax = __reduce_max_sync(0xffffffffu, amax);
     float scale = scale_of_bits(amax);
-    const long block = (long)page * pool.Hkv + hk;
-    uint8_t* codes = (which ? pool.v : pool.k) + block * FP8_PAGE * D;
-    float* scales = (which ? pool.v_scale : pool.k_scale) + block;
     const int slot0 = lo % FP8_PAGE;
+    __syncwarp();
     if (slot0 > 0) {                                             // earlier tokens of the sequence are in the page
-      const float old = *scales;
-      __syncwarp();
       if (scale > old) {
         const float f = old / scale;
         uint4* p = reinterpret_cast<uint4*>(codes);
@@ -192,14 +213,18 @@ __global__ void __launch_bounds__(256) fp8_append_kernel(const __grid_constant__
     if (lane == 0) *scales = scale;
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
-      if (it * HPW + sub >= m) break;
+      if (it * HPW >= m) break;
+      float x[16];
+      values(it, x);
       uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        w[e] = number ? e4m3x2(x[it][4 * e] * inv, x[it][4 * e + 1] * inv) | (e4m3x2(x[it][4 * e + 2] * inv, x[it][4 * e + 3] * inv) << 16) : 0u;
-      uint8_t* dst = codes + (slot0 + it * HPW + sub) * D;
-      *reinterpret_cast<uint2*>(dst + h.e0) = make_uint2(w[0], w[1]);
-      *reinterpret_cast<uint2*>(dst + h.e1) = make_uint2(w[2], w[3]);
+        w[e] = number ? e4m3x2(x[4 * e] * inv, x[4 * e + 1] * inv) | (e4m3x2(x[4 * e + 2] * inv, x[4 * e + 3] * inv) << 16) : 0u;
+      if (it * HPW + sub < m) {
+        uint8_t* dst = codes + (slot0 + it * HPW + sub) * D;
+        *reinterpret_cast<uint2*>(dst + h.e0) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(dst + h.e1) = make_uint2(w[2], w[3]);
+      }
     }
   }
 }
@@ -1227,11 +1252,14 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   if (ld_in % 8 || ld_v % 8 || ld_q % 8 || off16(q_in, k_in, v_in, q) || off16(wq, wk) || off16(cos_t, sin_t, k_pool, v_pool)) return -ERR_BAD_ARG;
   if (n == 0 || T == 0) return 0;
   const Fp8Append a{(const __nv_bfloat16*)q_in, (const __nv_bfloat16*)k_in, (const __nv_bfloat16*)v_in, (const __nv_bfloat16*)wq,
-                    (const __nv_bfloat16*)wk, cos_t, sin_t, pos, (__nv_bfloat16*)q, ld_in, ld_v, ld_q, H, rot, rope_rows, eps};
+                    (const __nv_bfloat16*)wk, cos_t, sin_t, pos, (__nv_bfloat16*)q, ld_in, ld_v, ld_q, H, rot, rope_rows, div_reciprocal(H ? H : 1), eps};
   const Fp8Pool pool{(uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, pages, Hkv};
   const Fp8Tokens tk{rows, cu, start, page_table, n, T, table_rows, max_pages, status};
   const unsigned ctas = (unsigned)(T / FP8_PAGE + 2 * n);
-  const dim3 grid(ctas, 1);
+  const int hpw = 512 / D, tokens = T / n < FP8_PAGE ? (T + n - 1) / n : FP8_PAGE;      // of an average page
+  const int items = 2 * Hkv + (tokens * H + 4 * hpw - 1) / (4 * hpw);
+  const int most = (items + 7) / 8, shares = ctas <= 296 ? most : (items + 15) / 16;      // an item a warp where there are few pages, else two
+  const dim3 grid(ctas, shares < 65535 ? shares : 65535);
   if (D == 64) launch_early(fp8_append_kernel<64>, grid, 256, 0, (cudaStream_t)stream, a, pool, tk);
   else launch_early(fp8_append_kernel<128>, grid, 256, 0, (cudaStream_t)stream, a, pool, tk);
   const cudaError_t e = cudaGetLastError();

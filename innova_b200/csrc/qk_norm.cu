@@ -6,7 +6,8 @@
 //
 // Both are bound by memory: forward reads and writes the buffer once, backward reads dy, reads x of the normed heads and writes dx. Heads live in the
 // lanes of a warp as units that hold both halves of their rotation pairs (head_norm.cuh), with two 16-byte loads a lane and no shuffles but the sum
-// over a head. A warp takes one token and walks over its heads, so that the token's cosines and sines are loaded once.
+// over a head. A warp takes one token and walks over its heads, so that the token's cosines and sines are loaded once, and has the loads of several
+// heads on their way at once.
 #include "head_norm.cuh"
 #include "inv_api.h"
 
@@ -17,145 +18,159 @@ struct QkNorm {
   void* y;                     // forward: the result; backward: dx
   const float *cos_t, *sin_t;
   const int* pos;              // position of every token; null: t % S
-  float* part;                 // backward: [grid, 2, D] sums of dw
+  float* part;                 // backward: sums of dw, [ctas_q, D] of the queries' norm and [the others, D] of the keys'
   int* status;
-  int T, S, H, Hkv, D, rot, table_rows, chunk;
+  int T, S, H, Hkv, D, rot, table_rows, chunk, ctas_q, chunk_q;      // backward: chunk of the key and value heads, chunk_q of the query heads
   long ld_x, ld_y, ld_dy;
   float eps, inv_d;
 };
 
+// Units that a lane has on its way at once.
+template <typename T>
+constexpr int UNITS = sizeof(T) == 2 ? 4 : 2;
+
+template <typename T, int L>
+__device__ __forceinline__ void load_turn(const QkNorm& p, int t, int u, const HeadUnit& h, Turn& turn) {
+  if (p.rot) turn.load(p.cos_t, p.sin_t, p.rot, table_row(p.pos ? p.pos[t] : t % p.S, p.table_rows, p.status), u, h);
+}
+
 // A warp's share: token `t`, head slots [s0, s0 + chunk) of H + 2 Hkv. chunk: all of them where tokens alone fill the GPU.
 template <typename T, int L>
-__global__ void __launch_bounds__(256) qk_norm_fwd_kernel(const __grid_constant__ QkNorm p) {
-  constexpr int HPW = 32 / L;
+__global__ void __launch_bounds__(256, 2) qk_norm_fwd_kernel(const __grid_constant__ QkNorm p) {
+  constexpr int HPW = 32 / L, N = UNITS<T>;
   const int lane = threadIdx.x & 31, u = lane % L, sub = lane / L;
   const int slots = p.H + 2 * p.Hkv, per = (slots + p.chunk - 1) / p.chunk;
   const long item = blockIdx.x * 8l + (threadIdx.x >> 5);
+  wait_previous();
+  release_next();
   if (item >= (long)p.T * per) return;
   const int t = (int)(item / per), s0 = (int)(item % per) * p.chunk, s1 = min(slots, s0 + p.chunk);
   const HeadUnit h(u, p.D, p.rot);
-  Turn turn;
-  if (p.rot && s0 < p.H + p.Hkv) turn.load(p.cos_t, p.sin_t, p.rot, table_row(p.pos ? p.pos[t] : t % p.S, p.table_rows, p.status), u, h);
   const T* x = (const T*)p.x + t * p.ld_x;
   T* y = (T*)p.y + t * p.ld_y;
+  Turn turn;
+  load_turn<T, L>(p, t, u, h, turn);
+  for (int s = s0; s < s1; s += N * HPW) {
+    RawUnit<T> raw[N];
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const int lo = max(s0, part ? p.H : 0), hi = min(s1, part ? p.H + p.Hkv : p.H);
-    if (lo >= hi) continue;
-    float w[16];
-    load_unit((const T*)(part ? p.wk : p.wq), h, w);
-#pragma unroll 2
-    for (int s = lo; s < hi; s += HPW) {
-      const bool ok = s + sub < hi;                 // lanes past the last head repeat it and store nothing
-      const long at = (long)min(s + sub, hi - 1) * p.D;
-      float v[16];
-      load_unit(x + at, h, v);
+    for (int j = 0; j < N; ++j) raw[j].fetch(x + (long)min(s + j * HPW + sub, s1 - 1) * p.D, h);      // lanes past the last head repeat it
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int slot = s + j * HPW + sub;
+      if (s + j * HPW >= s1) break;
+      const bool normed = slot < p.H + p.Hkv;
+      float v[16], w[16];
+      load_unit((const T*)(slot < p.H ? p.wq : p.wk), h, w);
+      raw[j].get(h, v);
       const float r = head_rstd<L>(v, p.inv_d, p.eps);
+      if (normed) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = v[i] * r * w[i];
-      turn.apply<false>(h, v);
-      if (ok) store_unit(y + at, h, v);
+        for (int i = 0; i < 16; ++i) v[i] = v[i] * r * w[i];
+        turn.apply<false>(h, v);
+        raw[j].set(v);
+      }
+      if (slot < s1 && h.has) raw[j].store(y + (long)slot * p.D, h);
     }
   }
-  for (int s = max(s0, p.H + p.Hkv); s < s1; s += HPW)
-    if (s + sub < s1) {
-      const long at = (long)(s + sub) * p.D;
-      float v[16];
-      load_unit(x + at, h, v);
-      store_unit(y + at, h, v);
-    }
 }
 
-// Warps walk over the tokens and keep their sums of dw in registers; a CTA adds its warps' in order and leaves one row.
+// The first ctas_q CTAs take the query heads, the others the key and value heads: a lane then keeps the sums of one dw in registers. Warps walk over the
+// tokens; a CTA adds its warps' sums in order and leaves one row.
 template <typename T, int L>
-__global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const __grid_constant__ QkNorm p) {
-  constexpr int HPW = 32 / L;
-  __shared__ float sums[8][2][L * 16];
+__global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_constant__ QkNorm p) {
+  constexpr int HPW = 32 / L, N = UNITS<T> / 2;
+  __shared__ float sums[8][L * 16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, u = lane % L, sub = lane / L;
-  const int slots = p.H + 2 * p.Hkv, per = (slots + p.chunk - 1) / p.chunk;
+  const bool keys = (int)blockIdx.x >= p.ctas_q;
+  const int first = keys ? p.H : 0, normed = keys ? p.H + p.Hkv : p.H, slots = keys ? 2 * p.Hkv : p.H, chunk = keys ? p.chunk : p.chunk_q;
+  const int per = (slots + chunk - 1) / chunk, cta = keys ? blockIdx.x - p.ctas_q : blockIdx.x, ctas = keys ? gridDim.x - p.ctas_q : p.ctas_q;
   const HeadUnit h(u, p.D, p.rot);
-  float dw[2][16];
+  wait_previous();
+  release_next();
+  float dw[16], w[16];
+  load_unit((const T*)(keys ? p.wk : p.wq), h, w);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0.f;
-  for (long item = blockIdx.x * 8l + warp; item < (long)p.T * per; item += gridDim.x * 8l) {
-    const int t = (int)(item / per), s0 = (int)(item % per) * p.chunk, s1 = min(slots, s0 + p.chunk);
-    Turn turn;
-    if (p.rot && s0 < p.H + p.Hkv) turn.load(p.cos_t, p.sin_t, p.rot, table_row(p.pos ? p.pos[t] : t % p.S, p.table_rows, p.status), u, h);
+  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
+  for (long item = cta * 8l + warp; item < (long)p.T * per; item += ctas * 8l) {
+    const int t = (int)(item / per), s0 = first + (int)(item - (long)t * per) * chunk, s1 = min(first + slots, s0 + chunk);
     const T *x = (const T*)p.x + t * p.ld_x, *dy = (const T*)p.dy + t * p.ld_dy;
     T* dx = (T*)p.y + t * p.ld_y;
+    Turn turn;
+    load_turn<T, L>(p, t, u, h, turn);
+    for (int s = s0; s < s1; s += N * HPW) {
+      RawUnit<T> rx[N], rg[N];
 #pragma unroll
-    for (int part = 0; part < 2; ++part) {
-      const int lo = max(s0, part ? p.H : 0), hi = min(s1, part ? p.H + p.Hkv : p.H);
-      if (lo >= hi) continue;
-      float w[16];
-      load_unit((const T*)(part ? p.wk : p.wq), h, w);
-      for (int s = lo; s < hi; s += HPW) {
-        const bool ok = s + sub < hi;
-        const long at = (long)min(s + sub, hi - 1) * p.D;
+      for (int j = 0; j < N; ++j) {
+        const int slot = min(s + j * HPW + sub, s1 - 1);                        // lanes past the last head repeat it
+        rg[j].fetch(dy + (long)slot * p.D, h);
+        rx[j].fetch((slot < normed ? x : dy) + (long)slot * p.D, h);            // of values only the gradient
+      }
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        if (s + j * HPW >= s1) break;
+        const int slot = s + j * HPW + sub;
         float v[16], g[16];
-        load_unit(x + at, h, v);
-        load_unit(dy + at, h, g);
+        rx[j].get(h, v);
+        rg[j].get(h, g);
         const float r = head_rstd<L>(v, p.inv_d, p.eps);
         turn.apply<true>(h, g);
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           v[i] *= r;                                // xh
-          if (ok) dw[part][i] = fmaf(g[i], v[i], dw[part][i]);
+          if (slot < min(normed, s1)) dw[i] = fmaf(g[i], v[i], dw[i]);
           g[i] *= w[i];
           dot = fmaf(g[i], v[i], dot);
         }
         const float mean = head_sum<L>(dot) * p.inv_d;
 #pragma unroll
         for (int i = 0; i < 16; ++i) g[i] = r * (g[i] - v[i] * mean);
-        if (ok) store_unit(dx + at, h, g);
+        if (slot < normed) rg[j].set(g);
+        if (slot < s1 && h.has) rg[j].store(dx + (long)slot * p.D, h);
       }
     }
-    for (int s = max(s0, p.H + p.Hkv); s < s1; s += HPW)
-      if (s + sub < s1) {
-        const long at = (long)(s + sub) * p.D;
-        float v[16];
-        load_unit(dy + at, h, v);
-        store_unit(dx + at, h, v);
-      }
   }
 #pragma unroll
-  for (int part = 0; part < 2; ++part)
+  for (int i = 0; i < 16; ++i) {
+    float v = dw[i];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float v = dw[part][i];
-#pragma unroll
-      for (int o = 16; o >= L; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (sub == 0 && h.has) sums[warp][part][(i < 8 ? h.e0 : h.e1 - 8) + i] = v;
-    }
+    for (int o = 16; o >= L; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (sub == 0 && h.has) sums[warp][(i < 8 ? h.e0 : h.e1 - 8) + i] = v;
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < 2 * p.D; e += 256) {
-    const int part = e / p.D, d = e % p.D;
+  for (int d = threadIdx.x; d < p.D; d += 256) {
     float v = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) v += sums[w][part][d];
-    p.part[(long)blockIdx.x * 2 * p.D + e] = v;
+    for (int k = 0; k < 8; ++k) v += sums[k][d];
+    p.part[(long)blockIdx.x * p.D + d] = v;
   }
 }
 
-// dw[part][d] = (what is there, with `add`) + the sum of `rows` rows, in an order that only their number decides. A CTA: 32 columns.
-__global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict__ part, int rows, int D, void* dwq, void* dwk, int mode_q, int mode_k) {
-  __shared__ float sums[8][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.x * 32 + lane;
+// dw[d] = (what is there, with `add`) + the sum of its rows, in an order that only their number decides. A CTA: 32 columns of the queries' or the keys'.
+__global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restrict__ part, int rows_q, int rows, int D, void* dwq, void* dwk, int mode_q,
+                                                          int mode_k) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
+  wait_previous();
+  release_next();
+  const int r0 = blockIdx.y ? rows_q : 0, r1 = blockIdx.y ? rows : rows_q;
   float v = 0.f;
-  if (e < 2 * D)
-    for (int r = warp; r < rows; r += 8) v += part[(long)r * 2 * D + e];
+  if (d < D) {
+#pragma unroll 8
+    for (int r = r0 + warp; r < r1; r += 32) v += part[(long)r * D + d];
+  }
   sums[warp][lane] = v;
   __syncthreads();
-  if (warp || e >= 2 * D) return;
-  v = 0.f;
+  v = sums[lane][warp];                              // warp <-> column, lane <-> the sum of a warp
 #pragma unroll
-  for (int w = 0; w < 8; ++w) v += sums[w][lane];
-  const int mode = e < D ? mode_q : mode_k, d = e % D;
-  void* out = e < D ? dwq : dwk;
-  if (mode == 2) ((float*)out)[d] += v;
-  else if (mode == 1) ((float*)out)[d] = v;
-  else ((__nv_bfloat16*)out)[d] = __float2bfloat16_rn(v);
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int col = blockIdx.x * 32 + warp;
+  if (lane || col >= D) return;
+  const int mode = blockIdx.y ? mode_k : mode_q;
+  void* out = blockIdx.y ? dwk : dwq;
+  if (mode == 2) ((float*)out)[col] += v;
+  else if (mode == 1) ((float*)out)[col] = v;
+  else ((__nv_bfloat16*)out)[col] = __float2bfloat16_rn(v);
 }
 
 // Slots a warp takes of a token: all, or as few as fill the GPU with warps (four to eight an SM hide the loads of a short call).
@@ -167,6 +182,20 @@ static int slot_chunk(int T, int slots, int hpw) {
   chunk = (chunk + hpw - 1) / hpw * hpw;
   return chunk < most ? chunk : most;
 }
+// CTAs of the backward kernel, in proportion to the bytes of either side: dy, x and dx of a normed head, dy and dx of a value head. At most two an SM.
+struct QkBwdCut {
+  int chunk_q, chunk, ctas_q, ctas;
+  QkBwdCut(int T, int H, int Hkv, int D) {
+    const int hpw = 32 / head_lanes(D);
+    const long want_q = H ? 148l * 2 * 3 * H / (3 * H + 5 * Hkv) : 0;
+    chunk_q = slot_chunk(T, H, hpw);
+    chunk = slot_chunk(T, 2 * Hkv, hpw);
+    const long most_q = H ? ((long)T * ((H + chunk_q - 1) / chunk_q) + 7) / 8 : 0, most = Hkv ? ((long)T * ((2 * Hkv + chunk - 1) / chunk) + 7) / 8 : 0;
+    const long lo_q = want_q > 0 || !H ? want_q : 1, lo = 148l * 2 - lo_q;
+    ctas_q = (int)(most_q < lo_q ? most_q : lo_q);
+    ctas = ctas_q + (int)(most < lo ? most : lo);
+  }
+};
 
 }  // namespace inv
 
@@ -182,18 +211,18 @@ static int qk_norm_args(const QkNorm& p, int f32) {
 }
 #define INV_QK_L(T, KERNEL)                                                                                                   \
   switch (head_lanes(p.D)) {                                                                                                  \
-    case 1: KERNEL<T, 1><<<grid, 256, 0, st>>>(p); break;                                                                     \
-    case 2: KERNEL<T, 2><<<grid, 256, 0, st>>>(p); break;                                                                     \
-    case 4: KERNEL<T, 4><<<grid, 256, 0, st>>>(p); break;                                                                     \
-    case 8: KERNEL<T, 8><<<grid, 256, 0, st>>>(p); break;                                                                     \
-    default: KERNEL<T, 16><<<grid, 256, 0, st>>>(p);                                                                          \
+    case 1: launch_early(KERNEL<T, 1>, grid, 256, 0, st, p); break;                                                                     \
+    case 2: launch_early(KERNEL<T, 2>, grid, 256, 0, st, p); break;                                                                     \
+    case 4: launch_early(KERNEL<T, 4>, grid, 256, 0, st, p); break;                                                                     \
+    case 8: launch_early(KERNEL<T, 8>, grid, 256, 0, st, p); break;                                                                     \
+    default: launch_early(KERNEL<T, 16>, grid, 256, 0, st, p);                                                                          \
   }
 
 // x, y: [T, (H + 2 Hkv) D], bf16 or fp32 (then the weights are too), rows ld_x and ld_y apart. cos_t, sin_t: [table_rows, rot / 2] fp32.
 extern "C" int inv_qk_norm_fwd(const void* x, long ld_x, void* y, long ld_y, const void* wq, const void* wk, const float* cos_t, const float* sin_t,
                                int table_rows, const int* pos, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status,
                                void* stream) {
-  QkNorm p{x, wq, wk, nullptr, y, cos_t, sin_t, pos, nullptr, status, T, S, H, Hkv, D, rot, table_rows, 0, ld_x, ld_y, 0, eps, 1.f / (float)D};
+  QkNorm p{x, wq, wk, nullptr, y, cos_t, sin_t, pos, nullptr, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, ld_x, ld_y, 0, eps, 1.f / (float)D};
   if (int rc = qk_norm_args(p, f32)) return rc;
   if (T <= 0) return 0;
   const int slots = H + 2 * Hkv;
@@ -206,27 +235,29 @@ extern "C" int inv_qk_norm_fwd(const void* x, long ld_x, void* y, long ld_y, con
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
-// CTAs of the backward kernel, and so rows of [2, D] floats that its caller provides.
+// CTAs of the backward kernel, and so rows of [D] floats that its caller provides.
 extern "C" int inv_qk_norm_bwd_grid(int T, int H, int Hkv, int D) {
-  if (T <= 0 || D < 16 || D > 256) return 0;
-  const int slots = H + 2 * Hkv, chunk = slot_chunk(T, slots, 32 / head_lanes(D));
-  const long ctas = ((long)T * ((slots + chunk - 1) / chunk) + 7) / 8;
-  return (int)(ctas < 148 * 4 ? ctas : 148 * 4);
+  if (T <= 0 || D < 16 || D > 256 || H < 0 || Hkv < 0) return 0;
+  return QkBwdCut(T, H, Hkv, D).ctas;
 }
 
 // dx, dy as y and x above. dwq, dwk: [D]; mode 0: bf16, written; 1: fp32, written; 2: fp32, added to.
 extern "C" int inv_qk_norm_bwd(const void* x, long ld_x, const void* dy, long ld_dy, void* dx, long ld_dx, const void* wq, const void* wk,
                                const float* cos_t, const float* sin_t, int table_rows, const int* pos, void* dwq, int mode_q, void* dwk, int mode_k,
                                float* part, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status, void* stream) {
-  QkNorm p{x, wq, wk, dy, dx, cos_t, sin_t, pos, part, status, T, S, H, Hkv, D, rot, table_rows, 0, ld_x, ld_dx, ld_dy, eps, 1.f / (float)D};
+  QkNorm p{x, wq, wk, dy, dx, cos_t, sin_t, pos, part, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, ld_x, ld_dx, ld_dy, eps, 1.f / (float)D};
   if (int rc = qk_norm_args(p, f32)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)inv_qk_norm_bwd_grid(T, H, Hkv, D);
-  if (grid) {
-    p.chunk = slot_chunk(T, H + 2 * Hkv, 32 / head_lanes(D));
+  unsigned grid = 0;
+  if (T > 0) {
+    const QkBwdCut cut(T, H, Hkv, D);
+    p.chunk = cut.chunk;
+    p.chunk_q = cut.chunk_q;
+    p.ctas_q = cut.ctas_q;
+    grid = (unsigned)cut.ctas;
     if (f32) { INV_QK_L(float, qk_norm_bwd_kernel) } else { INV_QK_L(__nv_bfloat16, qk_norm_bwd_kernel) }
   }
-  qk_norm_dw_kernel<<<(2 * D + 31) / 32, 256, 0, st>>>(part, (int)grid, D, dwq, dwk, mode_q, mode_k);
+  launch_early(qk_norm_dw_kernel, dim3((D + 31) / 32, 2), 1024, 0, st, (const float*)part, p.ctas_q, (int)grid, D, dwq, dwk, mode_q, mode_k);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }

@@ -365,7 +365,7 @@ class _QkNormRopeFn(torch.autograd.Function):
         for g, mg in zip(grads, (mg_q, mg_k)):
             outs += [mg.data_ptr(), 2] if mg is not None else [g.data_ptr(), int(g.dtype == torch.float32)]
         grid = rt.lib().inv_qk_norm_bwd_grid(T, H, G, D)
-        part = torch.empty(max(grid, 1) * 2 * D, dtype=torch.float32, device=x.device)
+        part = torch.empty(max(grid, 1) * D, dtype=torch.float32, device=x.device)
         rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), _ld(x), d.data_ptr(), _ld(d), dx.data_ptr(), x.shape[1], a.data_ptr(), b.data_ptr(),
                                           rt.ptr(cos), rt.ptr(sin), ctx.rows, rt.ptr(positions), *outs, part.data_ptr(), *ctx.sizes,
                                           rt.stream_ptr()), "inv_qk_norm_bwd")
