@@ -26,10 +26,31 @@ struct HeadUnit {
   }
 };
 
-__device__ __forceinline__ void load8(const float* p, float* f) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-  f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+// Two 32-bit values as one operand of the packed instructions.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 of_pair(uint64_t x) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 // A unit as it lies in memory: fetched without a branch, so that several are on their way at once, and widened when they are there.
@@ -51,72 +72,94 @@ struct RawUnit {
       reinterpret_cast<uint4*>(head + u.e1)[i] = r[N + i];
     }
   }
-  __device__ __forceinline__ void get(const HeadUnit& u, float (&x)[16]) const {
+  __device__ __forceinline__ void get(uint64_t (&x)[8]) const {
 #pragma unroll
     for (int i = 0; i < 2 * N; ++i) {
       const uint32_t w[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+      if constexpr (N == 1) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (N == 1) {
-          x[i * 8 + 2 * k] = u.has ? __uint_as_float(w[k] << 16) : 0.f;
-          x[i * 8 + 2 * k + 1] = u.has ? __uint_as_float(w[k] & 0xffff0000u) : 0.f;
-        } else {
-          x[i * 4 + k] = u.has ? __uint_as_float(w[k]) : 0.f;
-        }
+        for (int k = 0; k < 4; ++k) x[i * 4 + k] = pair_of(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+      } else {
+        x[i * 2] = pair_of(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        x[i * 2 + 1] = pair_of(__uint_as_float(w[2]), __uint_as_float(w[3]));
       }
     }
   }
-  __device__ __forceinline__ void set(const float (&x)[16]) {
+  __device__ __forceinline__ void set(const uint64_t (&x)[8]) {
+    uint32_t w[8 * N];
 #pragma unroll
-    for (int i = 0; i < 2 * N; ++i) {
-      if constexpr (N == 1)
-        r[i] = make_uint4(cvt_bf16x2(x[i * 8], x[i * 8 + 1]), cvt_bf16x2(x[i * 8 + 2], x[i * 8 + 3]), cvt_bf16x2(x[i * 8 + 4], x[i * 8 + 5]),
-                          cvt_bf16x2(x[i * 8 + 6], x[i * 8 + 7]));
-      else
-        r[i] = make_uint4(__float_as_uint(x[i * 4]), __float_as_uint(x[i * 4 + 1]), __float_as_uint(x[i * 4 + 2]), __float_as_uint(x[i * 4 + 3]));
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = of_pair(x[i]);
+      if constexpr (N == 1) {
+        w[i] = cvt_bf16x2(v.x, v.y);
+      } else {
+        w[2 * i] = __float_as_uint(v.x);
+        w[2 * i + 1] = __float_as_uint(v.y);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) r[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
   }
 };
 template <typename T>
-__device__ __forceinline__ void load_unit(const T* head, const HeadUnit& u, float (&x)[16]) {
+__device__ __forceinline__ void load_unit(const T* head, const HeadUnit& u, uint64_t (&x)[8]) {
   RawUnit<T> raw;
   raw.fetch(head, u);
-  raw.get(u, x);
+  raw.get(x);
 }
 
-// Sum over the L lanes of a head.
+// Sum over the L lanes of a head; what a lane without a unit brings counts for nothing.
 template <int L>
-__device__ __forceinline__ float head_sum(float v) {
+__device__ __forceinline__ float head_sum(uint64_t two, const HeadUnit& u) {
+  const float2 e = of_pair(two);
+  float v = u.has ? e.x + e.y : 0.f;
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 // 1 / sqrt(mean of squares + eps)
 template <int L>
-__device__ __forceinline__ float head_rstd(const float (&x)[16], float inv_d, float eps) {
-  float s = 0.f;
+__device__ __forceinline__ float head_rstd(const uint64_t (&x)[8], const HeadUnit& u, float inv_d, float eps) {
+  uint64_t s0 = mul_pair(x[0], x[0]), s1 = mul_pair(x[1], x[1]);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) s = fmaf(x[i], x[i], s);
-  return 1.f / sqrtf(head_sum<L>(s) * inv_d + eps);
+  for (int i = 2; i < 8; i += 2) {
+    s0 = fma_pair(x[i], x[i], s0);
+    s1 = fma_pair(x[i + 1], x[i + 1], s1);
+  }
+  return rsqrtf(head_sum<L>(add_pair(s0, s1), u) * inv_d + eps);
+}
+template <int L, typename T>
+__device__ __forceinline__ void head_norm(uint64_t (&x)[8], const T* weight, const HeadUnit& u, float inv_d, float eps) {
+  uint64_t w[8];
+  load_unit(weight, u, w);
+  const float r = head_rstd<L>(x, u, inv_d, eps);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = mul_pair(mul_pair(x[i], pair_of(r, r)), w[i]);
 }
 
 // Cosines and sines of a unit's eight pairs at one position.
 struct Turn {
-  float c[8], s[8];
+  uint64_t c[4], s[4];
   __device__ __forceinline__ void load(const float* cos_t, const float* sin_t, int rot, int pos, int u, const HeadUnit& h) {
     const size_t at = (size_t)pos * (rot / 2) + (h.turns ? u * 8 : 0);
-    load8(cos_t + at, c);
-    load8(sin_t + at, s);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 a = reinterpret_cast<const float4*>(cos_t + at)[i], b = reinterpret_cast<const float4*>(sin_t + at)[i];
+      c[2 * i] = pair_of(a.x, a.y);
+      c[2 * i + 1] = pair_of(a.z, a.w);
+      s[2 * i] = pair_of(b.x, b.y);
+      s[2 * i + 1] = pair_of(b.z, b.w);
+    }
   }
   // (x1, x2) -> (x1 c - x2 s, x1 s + x2 c); INV: by the transpose. Products are rounded by themselves, as written.
   template <bool INV>
-  __device__ __forceinline__ void apply(const HeadUnit& h, float (&x)[16]) const {
+  __device__ __forceinline__ void apply(const HeadUnit& h, uint64_t (&x)[8]) const {
     if (!h.turns) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = x[i], b = x[i + 8], sn = INV ? -s[i] : s[i];
-      x[i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, sn));
-      x[i + 8] = __fadd_rn(__fmul_rn(a, sn), __fmul_rn(b, c[i]));
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t a = x[i], b = x[i + 4], minus = 0x8000000080000000ull;
+      x[i] = add_pair(mul_pair(a, c[i]), mul_pair(INV ? b : b ^ minus, s[i]));
+      x[i + 4] = add_pair(mul_pair(INV ? a ^ minus : a, s[i]), mul_pair(b, c[i]));
     }
   }
 };

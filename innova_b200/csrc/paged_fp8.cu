@@ -79,7 +79,7 @@ struct Fp8Append {
 // in a warp's registers, so that their largest value is known before any is rounded; or a run of query heads. Rows stay in registers as they were read
 // (keys are normed and turned twice, for their largest value and for the codes), so that three CTAs an SM keep four units a lane on their way.
 template <int D>
-__global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constant__ Fp8Append a, const __grid_constant__ Fp8Pool pool,
+__global__ void __launch_bounds__(128, 4) fp8_append_kernel(const __grid_constant__ Fp8Append a, const __grid_constant__ Fp8Pool pool,
                                                             const __grid_constant__ Fp8Tokens tk) {
   constexpr int L = D / 16, HPW = 32 / L, NIT = FP8_PAGE / HPW, NQ = 4;
   using Raw = RawUnit<__nv_bfloat16>;
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constan
   __syncthreads();
   wait_previous();
   release_next();
-  for (int i = threadIdx.x; i < tk.n; i += 256) {
+  for (int i = threadIdx.x; i < tk.n; i += 128) {
     const int c0 = tk.cu[i], c1 = tk.cu[i + 1], start = tk.start[i], row = tk.rows[i];
     const int base = c0 / FP8_PAGE + 2 * i, next = c1 / FP8_PAGE + 2 * (i + 1);
     if (base <= (int)blockIdx.x && (int)blockIdx.x < next) {
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constan
     turn.load(a.cos_t, a.sin_t, a.rot, table_row(a.pos ? a.pos[first + i] : lo + i, a.table_rows, tk.status), u, h);
   };
   const int n_kv = 2 * pool.Hkv, n_q = (m * a.H + NQ * HPW - 1) / (NQ * HPW);
-  for (int item = blockIdx.y * 8 + warp; item < n_kv + n_q; item += gridDim.y * 8) {
+  for (int item = blockIdx.y * 4 + warp; item < n_kv + n_q; item += gridDim.y * 4) {
     if (item >= n_kv) {
       // ---- heads of tokens, one behind the other ----
       const int s0 = (item - n_kv) * (NQ * HPW) + sub;
@@ -136,15 +136,9 @@ __global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constan
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
         if (j && a.rot && tok[j] != tok[j - 1]) angles(turn, tok[j]);
-        float v[16];
-        raw[j].get(h, v);
-        if (a.wq) {
-          const float r = head_rstd<L>(v, 1.f / D, a.eps);
-          float w[16];
-          load_unit(a.wq, h, w);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
-        }
+        uint64_t v[8];
+        raw[j].get(v);
+        if (a.wq) head_norm<L>(v, a.wq, h, 1.f / D, a.eps);
         if (a.rot) turn.apply<false>(h, v);
         raw[j].set(v);
         if (s0 + j * HPW < m * a.H) raw[j].store(a.q + (first + tok[j]) * a.ld_q + hd[j] * D, h);
@@ -166,16 +160,10 @@ __global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constan
     uint8_t* codes = (which ? pool.v : pool.k) + block * FP8_PAGE * D;
     float* scales = (which ? pool.v_scale : pool.k_scale) + block;
     const float old = *scales;
-    auto values = [&](int it, float (&x)[16]) {
-      raw[it].get(h, x);
+    auto values = [&](int it, uint64_t (&x)[8]) {
+      raw[it].get(x);
       if (which) return;
-      if (a.wk) {
-        float w[16];
-        load_unit(a.wk, h, w);
-        const float r = head_rstd<L>(x, 1.f / D, a.eps);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = x[e] * r * w[e];
-      }
+      if (a.wk) head_norm<L>(x, a.wk, h, 1.f / D, a.eps);
       if (a.rot) {
         Turn turn;
         angles(turn, min(it * HPW + sub, m - 1));
@@ -186,10 +174,10 @@ __global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constan
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
       if (it * HPW >= m) break;
-      float x[16];
+      uint64_t x[8];
       values(it, x);
 #pragma unroll
-      for (int e = 0; e < 16; ++e) amax = max(amax, __float_as_uint(x[e]) & 0x7fffffffu);
+      for (int e = 0; e < 8; ++e) amax = max(amax, max((uint32_t)x[e] & 0x7fffffffu, (uint32_t)(x[e] >> 32) & 0x7fffffffu));
     }
     amax = __reduce_max_sync(0xffffffffu, amax);
     float scale = scale_of_bits(amax);
@@ -214,12 +202,14 @@ __global__ void __launch_bounds__(256, 3) fp8_append_kernel(const __grid_constan
 #pragma unroll
     for (int it = 0; it < NIT; ++it) {
       if (it * HPW >= m) break;
-      float x[16];
+      uint64_t x[8];
       values(it, x);
       uint32_t w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = number ? e4m3x2(x[4 * e] * inv, x[4 * e + 1] * inv) | (e4m3x2(x[4 * e + 2] * inv, x[4 * e + 3] * inv) << 16) : 0u;
+      for (int e = 0; e < 4; ++e) {
+        const float2 lo2 = of_pair(mul_pair(x[2 * e], pair_of(inv, inv))), hi2 = of_pair(mul_pair(x[2 * e + 1], pair_of(inv, inv)));
+        w[e] = number ? e4m3x2(lo2.x, lo2.y) | (e4m3x2(hi2.x, hi2.y) << 16) : 0u;
+      }
       if (it * HPW + sub < m) {
         uint8_t* dst = codes + (slot0 + it * HPW + sub) * D;
         *reinterpret_cast<uint2*>(dst + h.e0) = make_uint2(w[0], w[1]);
@@ -265,26 +255,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 }
 
 // Two fp32 operations in one instruction.
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ float2 of_pair(uint64_t x) {
-  float2 d;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 __device__ __forceinline__ uint4 shared16(uint32_t at) {
   uint4 r;
   asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
@@ -1258,10 +1228,10 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   const unsigned ctas = (unsigned)(T / FP8_PAGE + 2 * n);
   const int hpw = 512 / D, tokens = T / n < FP8_PAGE ? (T + n - 1) / n : FP8_PAGE;      // of an average page
   const int items = 2 * Hkv + (tokens * H + 4 * hpw - 1) / (4 * hpw);
-  const int most = (items + 7) / 8, shares = ctas <= 296 ? most : (items + 15) / 16;      // an item a warp where there are few pages, else two
+  const int most = (items + 3) / 4, shares = ctas <= 296 ? most : (items + 7) / 8;      // an item a warp where there are few pages, else two
   const dim3 grid(ctas, shares < 65535 ? shares : 65535);
-  if (D == 64) launch_early(fp8_append_kernel<64>, grid, 256, 0, (cudaStream_t)stream, a, pool, tk);
-  else launch_early(fp8_append_kernel<128>, grid, 256, 0, (cudaStream_t)stream, a, pool, tk);
+  if (D == 64) launch_early(fp8_append_kernel<64>, grid, 128, 0, (cudaStream_t)stream, a, pool, tk);
+  else launch_early(fp8_append_kernel<128>, grid, 128, 0, (cudaStream_t)stream, a, pool, tk);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }

@@ -59,13 +59,10 @@ __global__ void __launch_bounds__(256, 2) qk_norm_fwd_kernel(const __grid_consta
       const int slot = s + j * HPW + sub;
       if (s + j * HPW >= s1) break;
       const bool normed = slot < p.H + p.Hkv;
-      float v[16], w[16];
-      load_unit((const T*)(slot < p.H ? p.wq : p.wk), h, w);
-      raw[j].get(h, v);
-      const float r = head_rstd<L>(v, p.inv_d, p.eps);
+      uint64_t v[8];
+      raw[j].get(v);
+      head_norm<L>(v, (const T*)(slot < p.H ? p.wq : p.wk), h, p.inv_d, p.eps);
       if (normed) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = v[i] * r * w[i];
         turn.apply<false>(h, v);
         raw[j].set(v);
       }
@@ -87,10 +84,10 @@ __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_consta
   const HeadUnit h(u, p.D, p.rot);
   wait_previous();
   release_next();
-  float dw[16], w[16];
+  uint64_t dw[8], w[8];
   load_unit((const T*)(keys ? p.wk : p.wq), h, w);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) dw[i] = 0.f;
+  for (int i = 0; i < 8; ++i) dw[i] = 0;
   for (long item = cta * 8l + warp; item < (long)p.T * per; item += ctas * 8l) {
     const int t = (int)(item / per), s0 = first + (int)(item - (long)t * per) * chunk, s1 = min(first + slots, s0 + chunk);
     const T *x = (const T*)p.x + t * p.ld_x, *dy = (const T*)p.dy + t * p.ld_dy;
@@ -109,22 +106,28 @@ __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_consta
       for (int j = 0; j < N; ++j) {
         if (s + j * HPW >= s1) break;
         const int slot = s + j * HPW + sub;
-        float v[16], g[16];
-        rx[j].get(h, v);
-        rg[j].get(h, g);
-        const float r = head_rstd<L>(v, p.inv_d, p.eps);
+        uint64_t v[8], g[8];
+        rx[j].get(v);
+        rg[j].get(g);
+        const float r = head_rstd<L>(v, h, p.inv_d, p.eps);
         turn.apply<true>(h, g);
-        float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          v[i] *= r;                                // xh
-          if (slot < min(normed, s1)) dw[i] = fmaf(g[i], v[i], dw[i]);
-          g[i] *= w[i];
-          dot = fmaf(g[i], v[i], dot);
+        for (int i = 0; i < 8; ++i) v[i] = mul_pair(v[i], pair_of(r, r));       // xh
+        if (slot < min(normed, s1)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dw[i] = fma_pair(g[i], v[i], dw[i]);
         }
-        const float mean = head_sum<L>(dot) * p.inv_d;
+        uint64_t d0 = 0, d1 = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) g[i] = r * (g[i] - v[i] * mean);
+        for (int i = 0; i < 8; i += 2) {
+          g[i] = mul_pair(g[i], w[i]);
+          g[i + 1] = mul_pair(g[i + 1], w[i + 1]);
+          d0 = fma_pair(g[i], v[i], d0);
+          d1 = fma_pair(g[i + 1], v[i + 1], d1);
+        }
+        const float mean = head_sum<L>(add_pair(d0, d1), h) * -p.inv_d;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = mul_pair(pair_of(r, r), fma_pair(v[i], pair_of(mean, mean), g[i]));
         if (slot < normed) rg[j].set(g);
         if (slot < s1 && h.has) rg[j].store(dx + (long)slot * p.D, h);
       }
@@ -132,7 +135,8 @@ __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_consta
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
-    float v = dw[i];
+    const float2 two = of_pair(dw[i / 2]);
+    float v = i % 2 ? two.y : two.x;
 #pragma unroll
     for (int o = 16; o >= L; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (sub == 0 && h.has) sums[warp][(i < 8 ? h.e0 : h.e1 - 8) + i] = v;
