@@ -7,6 +7,8 @@
 #pragma once
 #include "sm100_common.cuh"
 
+#include <atomic>
+
 namespace inv {
 
 __host__ __device__ constexpr int head_lanes(int D) {
@@ -52,6 +54,23 @@ __device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+
+__device__ __forceinline__ uint4 shared16(uint32_t at) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ uint2 shared8(uint32_t at) {
+  uint2 r;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
+  return r;
+}
+__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // A unit as it lies in memory: fetched without a branch, so that several are on their way at once, and widened when they are there.
 template <typename T>
@@ -169,6 +188,17 @@ __device__ __forceinline__ int table_row(int pos, int rows, int* status) {
   if ((unsigned)pos < (unsigned)rows) return pos;
   atomicCAS(status, 0, ERR_BAD_ARG);
   return pos < 0 ? 0 : rows - 1;
+}
+
+// The kernel's shared memory on the current device, asked for once.
+template <typename K>
+static void raise_smem(K* kernel, int bytes, std::atomic<uint64_t>& ready) {
+  int device = 0;
+  cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (ready.load() & bit) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  ready.fetch_or(bit);
 }
 
 }  // namespace inv

@@ -12,7 +12,6 @@
 
 #include <cuda_fp16.h>
 
-#include <atomic>
 
 namespace inv {
 
@@ -254,23 +253,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Two fp32 operations in one instruction.
-__device__ __forceinline__ uint4 shared16(uint32_t at) {
-  uint4 r;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(at));
-  return r;
-}
-__device__ __forceinline__ uint2 shared8(uint32_t at) {
-  uint2 r;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(at));
-  return r;
-}
-__device__ __forceinline__ void copy16_async(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // In front of code that is to stay behind its branch: selects in its place would be paid for by every page.
 __device__ __forceinline__ void rarely() { asm volatile(""); }
 
@@ -1275,17 +1257,6 @@ extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int m
   if (n < 1 || T < 1 || Hkv < 1 || H < Hkv || max_new < 1 || max_len < 1) return 0;
   const Fp8Cut cut(n, Hkv, H / Hkv, max_new, max_len, window, tree);
   return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
-}
-
-// The kernel's shared memory on the current device, asked for once.
-template <typename K>
-static void raise_smem(K* kernel, int bytes, std::atomic<uint64_t>& ready) {
-  int device = 0;
-  cudaGetDevice(&device);
-  const uint64_t bit = 1ull << (device & 63);
-  if (ready.load() & bit) return;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  ready.fetch_or(bit);
 }
 template <int D>
 static int fp8_attend_join(const Fp8Attend& a, int T, cudaStream_t st) {

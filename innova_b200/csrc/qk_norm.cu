@@ -6,13 +6,18 @@
 //
 // Both are bound by memory: forward reads and writes the buffer once, backward reads dy, reads x of the normed heads and writes dx. Heads live in the
 // lanes of a warp as units that hold both halves of their rotation pairs (head_norm.cuh), with two 16-byte loads a lane and no shuffles but the sum
-// over a head. A warp takes one token and walks over its heads, so that the token's cosines and sines are loaded once, and has the loads of several
-// heads on their way at once.
+// over a head. A lane has several units on their way at once, of heads that lie one behind the other.
 #include "head_norm.cuh"
 #include "inv_api.h"
 
 namespace inv {
 
+// How head slots, a token's behind the other's, are dealt to warps: a lane has `units` of them on their way at once, and a warp goes on for `rounds`, all in
+// the same token, whose angles it then loads once.
+struct QkRun {
+  int units, rounds;
+  bool same;                   // what a warp has on its way at once is of one token
+};
 struct QkNorm {
   const void *x, *wq, *wk, *dy;
   void* y;                     // forward: the result; backward: dx
@@ -20,7 +25,9 @@ struct QkNorm {
   const int* pos;              // position of every token; null: t % S
   float* part;                 // backward: sums of dw, [ctas_q, D] of the queries' norm and [the others, D] of the keys'
   int* status;
-  int T, S, H, Hkv, D, rot, table_rows, chunk, ctas_q, chunk_q;      // backward: chunk of the key and value heads, chunk_q of the query heads
+  int T, S, H, Hkv, D, rot, table_rows, ctas_q;
+  QkRun run, run_q;            // backward: of the key and value heads, of the query heads
+  uint32_t inv_s, inv_slots, inv_slots_q;      // div_reciprocal of S and of the head slots of a token (backward: key and value heads, query heads)
   long ld_x, ld_y, ld_dy;
   float eps, inv_d;
 };
@@ -29,109 +36,155 @@ struct QkNorm {
 template <typename T>
 constexpr int UNITS = sizeof(T) == 2 ? 4 : 2;
 
-template <typename T, int L>
+// Head slots s, s + HPW, ... `units` of them; those past the end repeat the last.
+template <int N, int HPW>
+struct Slots {
+  int tok[N], hd[N];
+  bool in[N];
+  __device__ __forceinline__ Slots(int s, int all, int units, int slots, uint32_t inv) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int at = min(s + min(j, units - 1) * HPW, all - 1);
+      in[j] = j < units && s + j * HPW < all;
+      tok[j] = div_by(at, slots, inv);
+      hd[j] = at - tok[j] * slots;
+    }
+  }
+};
 __device__ __forceinline__ void load_turn(const QkNorm& p, int t, int u, const HeadUnit& h, Turn& turn) {
-  if (p.rot) turn.load(p.cos_t, p.sin_t, p.rot, table_row(p.pos ? p.pos[t] : t % p.S, p.table_rows, p.status), u, h);
+  turn.load(p.cos_t, p.sin_t, p.rot, table_row(p.pos ? p.pos[t] : t - div_by(t, p.S, p.inv_s) * p.S, p.table_rows, p.status), u, h);
 }
 
-// A warp's share: token `t`, head slots [s0, s0 + chunk) of H + 2 Hkv. chunk: all of them where tokens alone fill the GPU.
 template <typename T, int L>
 __global__ void __launch_bounds__(256, 2) qk_norm_fwd_kernel(const __grid_constant__ QkNorm p) {
   constexpr int HPW = 32 / L, N = UNITS<T>;
   const int lane = threadIdx.x & 31, u = lane % L, sub = lane / L;
-  const int slots = p.H + 2 * p.Hkv, per = (slots + p.chunk - 1) / p.chunk;
-  const long item = blockIdx.x * 8l + (threadIdx.x >> 5);
+  const int slots = p.H + 2 * p.Hkv, all = p.T * slots;
+  const int step = p.run.units * HPW, stride = step * p.run.rounds;
+  const HeadUnit h(u, p.D, p.rot);
   wait_previous();
   release_next();
-  if (item >= (long)p.T * per) return;
-  const int t = (int)(item / per), s0 = (int)(item % per) * p.chunk, s1 = min(slots, s0 + p.chunk);
-  const HeadUnit h(u, p.D, p.rot);
-  const T* x = (const T*)p.x + t * p.ld_x;
-  T* y = (T*)p.y + t * p.ld_y;
   Turn turn;
-  load_turn<T, L>(p, t, u, h, turn);
-  for (int s = s0; s < s1; s += N * HPW) {
+  for (long from = (blockIdx.x * 8l + (threadIdx.x >> 5)) * stride; from < all; from += gridDim.x * 8l * stride)
+  for (int base = (int)from; base < min(from + stride, (long)all); base += step) {
+    const Slots<N, HPW> s(base + sub, all, p.run.units, slots, p.inv_slots);
     RawUnit<T> raw[N];
 #pragma unroll
-    for (int j = 0; j < N; ++j) raw[j].fetch(x + (long)min(s + j * HPW + sub, s1 - 1) * p.D, h);      // lanes past the last head repeat it
+    for (int j = 0; j < N; ++j) raw[j].fetch((const T*)p.x + s.tok[j] * p.ld_x + s.hd[j] * p.D, h);
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int slot = s + j * HPW + sub;
-      if (s + j * HPW >= s1) break;
-      const bool normed = slot < p.H + p.Hkv;
+      if (j >= p.run.units) break;
+      if (p.rot && (!p.run.same || (j == 0 && base == from))) load_turn(p, s.tok[j], u, h, turn);
       uint64_t v[8];
       raw[j].get(v);
-      head_norm<L>(v, (const T*)(slot < p.H ? p.wq : p.wk), h, p.inv_d, p.eps);
-      if (normed) {
+      head_norm<L>(v, (const T*)(s.hd[j] < p.H ? p.wq : p.wk), h, p.inv_d, p.eps);
+      if (s.hd[j] < p.H + p.Hkv) {
         turn.apply<false>(h, v);
         raw[j].set(v);
       }
-      if (slot < s1 && h.has) raw[j].store(y + (long)slot * p.D, h);
+      if (s.in[j] && h.has) raw[j].store((T*)p.y + s.tok[j] * p.ld_y + s.hd[j] * p.D, h);
     }
   }
 }
 
-// The first ctas_q CTAs take the query heads, the others the key and value heads: a lane then keeps the sums of one dw in registers. Warps walk over the
-// tokens; a CTA adds its warps' sums in order and leaves one row.
+// Backward: what a lane reads of its next steps comes by asynchronous copies into its own places of shared memory, which needs no registers and no barrier.
+template <typename T>
+struct QkRing {
+  static constexpr int PIECES = 4 * RawUnit<T>::N, STAGES = sizeof(T) == 2 ? 4 : 3, BYTES = 8 * STAGES * PIECES * 32 * 16;
+};
+
+// The first ctas_q CTAs take the query heads, the others the key and value heads: a lane then keeps the sums of one dw in registers. A CTA adds its warps'
+// sums in order and leaves one row.
 template <typename T, int L>
 __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_constant__ QkNorm p) {
-  constexpr int HPW = 32 / L, N = UNITS<T> / 2;
+  using Ring = QkRing<T>;
+  constexpr int HPW = 32 / L, NP = RawUnit<T>::N, ST = Ring::STAGES;
+  extern __shared__ uint4 ring[];
   __shared__ float sums[8][L * 16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, u = lane % L, sub = lane / L;
   const bool keys = (int)blockIdx.x >= p.ctas_q;
-  const int first = keys ? p.H : 0, normed = keys ? p.H + p.Hkv : p.H, slots = keys ? 2 * p.Hkv : p.H, chunk = keys ? p.chunk : p.chunk_q;
-  const int per = (slots + chunk - 1) / chunk, cta = keys ? blockIdx.x - p.ctas_q : blockIdx.x, ctas = keys ? gridDim.x - p.ctas_q : p.ctas_q;
+  const int first = keys ? p.H : 0, normed = keys ? p.Hkv : p.H, slots = keys ? 2 * p.Hkv : p.H, all = p.T * slots;
+  const uint32_t inv = keys ? p.inv_slots : p.inv_slots_q;
+  const int cta = keys ? blockIdx.x - p.ctas_q : blockIdx.x, ctas = keys ? gridDim.x - p.ctas_q : p.ctas_q;
+  const QkRun run = keys ? p.run : p.run_q;
+  const long stride = HPW * run.rounds, jump = ctas * 8l * stride;
   const HeadUnit h(u, p.D, p.rot);
+  struct Walk {                                      // steps of a warp: HPW slots at `base`, in runs of `stride` from `from` on
+    long from;
+    int base;
+  };
+  auto on = [&](Walk& k) {
+    k.base += HPW;
+    if (k.base >= min(k.from + stride, (long)all)) {
+      k.from += jump;
+      k.base = (int)k.from;
+    }
+  };
   wait_previous();
   release_next();
+  uint4* mine = ring + warp * (ST * Ring::PIECES * 32) + lane;
+  auto copy = [&](Walk& k, int stage) {
+    if (k.from < all) {
+      const Slots<1, HPW> s(k.base + sub, all, 1, slots, inv);
+      const int at = (first + s.hd[0]) * p.D;
+      const T *dy = (const T*)p.dy + s.tok[0] * p.ld_dy + at, *x = s.hd[0] < normed ? (const T*)p.x + s.tok[0] * p.ld_x + at : dy;      // of values only dy
+      const uint32_t to = smem_u32(mine + stage * (Ring::PIECES * 32));
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        copy16_async(to + i * 512, x + h.e0 + i * (16 / sizeof(T)));
+        copy16_async(to + (NP + i) * 512, x + h.e1 + i * (16 / sizeof(T)));
+        copy16_async(to + (2 * NP + i) * 512, dy + h.e0 + i * (16 / sizeof(T)));
+        copy16_async(to + (3 * NP + i) * 512, dy + h.e1 + i * (16 / sizeof(T)));
+      }
+      on(k);
+    }
+    copies_commit();
+  };
+  const long mine0 = (cta * 8l + warp) * stride;
+  Walk ahead{mine0, (int)mine0}, now = ahead;
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) copy(ahead, i);
   uint64_t dw[8], w[8];
   load_unit((const T*)(keys ? p.wk : p.wq), h, w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[i] = 0;
-  for (long item = cta * 8l + warp; item < (long)p.T * per; item += ctas * 8l) {
-    const int t = (int)(item / per), s0 = first + (int)(item - (long)t * per) * chunk, s1 = min(first + slots, s0 + chunk);
-    const T *x = (const T*)p.x + t * p.ld_x, *dy = (const T*)p.dy + t * p.ld_dy;
-    T* dx = (T*)p.y + t * p.ld_y;
-    Turn turn;
-    load_turn<T, L>(p, t, u, h, turn);
-    for (int s = s0; s < s1; s += N * HPW) {
-      RawUnit<T> rx[N], rg[N];
+  Turn turn;
+  for (int stage = 0; now.from < all; on(now)) {
+    const Slots<1, HPW> s(now.base + sub, all, 1, slots, inv);
+    if (p.rot && (!run.same || now.base == now.from)) load_turn(p, s.tok[0], u, h, turn);
+    copies_wait<ST - 2>();
+    RawUnit<T> rx, rg;
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const int slot = min(s + j * HPW + sub, s1 - 1);                        // lanes past the last head repeat it
-        rg[j].fetch(dy + (long)slot * p.D, h);
-        rx[j].fetch((slot < normed ? x : dy) + (long)slot * p.D, h);            // of values only the gradient
-      }
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        if (s + j * HPW >= s1) break;
-        const int slot = s + j * HPW + sub;
-        uint64_t v[8], g[8];
-        rx[j].get(v);
-        rg[j].get(g);
-        const float r = head_rstd<L>(v, h, p.inv_d, p.eps);
-        turn.apply<true>(h, g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = mul_pair(v[i], pair_of(r, r));       // xh
-        if (slot < min(normed, s1)) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) dw[i] = fma_pair(g[i], v[i], dw[i]);
-        }
-        uint64_t d0 = 0, d1 = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          g[i] = mul_pair(g[i], w[i]);
-          g[i + 1] = mul_pair(g[i + 1], w[i + 1]);
-          d0 = fma_pair(g[i], v[i], d0);
-          d1 = fma_pair(g[i + 1], v[i + 1], d1);
-        }
-        const float mean = head_sum<L>(add_pair(d0, d1), h) * -p.inv_d;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = mul_pair(pair_of(r, r), fma_pair(v[i], pair_of(mean, mean), g[i]));
-        if (slot < normed) rg[j].set(g);
-        if (slot < s1 && h.has) rg[j].store(dx + (long)slot * p.D, h);
-      }
+    for (int i = 0; i < 2 * NP; ++i) {
+      rx.r[i] = mine[(stage * Ring::PIECES + i) * 32];
+      rg.r[i] = mine[(stage * Ring::PIECES + 2 * NP + i) * 32];
     }
+    uint64_t v[8], g[8];
+    rx.get(v);
+    rg.get(g);
+    const float r = head_rstd<L>(v, h, p.inv_d, p.eps);
+    copy(ahead, stage ? stage - 1 : ST - 1);         // where the step before this one was
+    if (++stage == ST) stage = 0;
+    turn.apply<true>(h, g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = mul_pair(v[i], pair_of(r, r));           // xh
+    if (s.in[0] && s.hd[0] < normed) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dw[i] = fma_pair(g[i], v[i], dw[i]);
+    }
+    uint64_t d0 = 0, d1 = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      g[i] = mul_pair(g[i], w[i]);
+      g[i + 1] = mul_pair(g[i + 1], w[i + 1]);
+      d0 = fma_pair(g[i], v[i], d0);
+      d1 = fma_pair(g[i + 1], v[i + 1], d1);
+    }
+    const float mean = head_sum<L>(add_pair(d0, d1), h) * -p.inv_d;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) g[i] = mul_pair(pair_of(r, r), fma_pair(v[i], pair_of(mean, mean), g[i]));
+    if (s.hd[0] < normed) rg.set(g);
+    if (s.in[0] && h.has) rg.store((T*)p.y + s.tok[0] * p.ld_y + (first + s.hd[0]) * p.D, h);
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -177,27 +230,30 @@ __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restric
   else ((__nv_bfloat16*)out)[col] = __float2bfloat16_rn(v);
 }
 
-// Slots a warp takes of a token: all, or as few as fill the GPU with warps (four to eight an SM hide the loads of a short call).
-static int slot_chunk(int T, int slots, int hpw) {
-  const int most = (slots + hpw - 1) / hpw * hpw;
-  const long want = 148l * 32 / (T < 1 ? 1 : T);            // warps a token may have
-  if (want <= 1) return most;
-  int chunk = (int)((slots + want - 1) / want);
-  chunk = (chunk + hpw - 1) / hpw * hpw;
-  return chunk < most ? chunk : most;
+// Two CTAs an SM stay. As many units a lane as leave the warps of all of them one, then as many rounds as leave each of them two runs.
+static QkRun qk_run(long T, int slots, int hpw, int most, long ctas) {
+  QkRun r{1, 1, false};
+  if (slots < 1 || ctas < 1) return r;
+  const long lanes = (T * slots + hpw - 1) / hpw, warps = 8 * ctas;
+  while (r.units < most && lanes > warps * r.units) r.units *= 2;
+  r.same = slots % (r.units * hpw) == 0;
+  const int whole = slots / (r.units * hpw);
+  if (r.same && T >= 2 * warps) r.rounds = whole;
+  return r;
 }
-// CTAs of the backward kernel, in proportion to the bytes of either side: dy, x and dx of a normed head, dy and dx of a value head. At most two an SM.
+static int qk_ctas(long T, int slots, int hpw, long share) {
+  const long ctas = (T * slots + 8 * hpw - 1) / (8 * hpw);
+  return (int)(ctas < share ? ctas : share);
+}
+// CTAs of the backward kernel, in proportion to the bytes of either side: dy, x and dx of a normed head, dy and dx of a value head.
 struct QkBwdCut {
-  int chunk_q, chunk, ctas_q, ctas;
+  int ctas_q, ctas;
   QkBwdCut(int T, int H, int Hkv, int D) {
     const int hpw = 32 / head_lanes(D);
-    const long want_q = H ? 148l * 2 * 3 * H / (3 * H + 5 * Hkv) : 0;
-    chunk_q = slot_chunk(T, H, hpw);
-    chunk = slot_chunk(T, 2 * Hkv, hpw);
-    const long most_q = H ? ((long)T * ((H + chunk_q - 1) / chunk_q) + 7) / 8 : 0, most = Hkv ? ((long)T * ((2 * Hkv + chunk - 1) / chunk) + 7) / 8 : 0;
-    const long lo_q = want_q > 0 || !H ? want_q : 1, lo = 148l * 2 - lo_q;
-    ctas_q = (int)(most_q < lo_q ? most_q : lo_q);
-    ctas = ctas_q + (int)(most < lo ? most : lo);
+    long share = H ? 296l * 3 * H / (3 * H + 5 * Hkv) : 0;
+    if (H && share < 1) share = 1;
+    ctas_q = qk_ctas(T, H, hpw, share);
+    ctas = ctas_q + qk_ctas(T, 2 * Hkv, hpw, 296 - share);
   }
 };
 
@@ -209,32 +265,44 @@ static int qk_norm_args(const QkNorm& p, int f32) {
   const int vec = f32 ? 4 : 8;
   if (p.D < 16 || p.D > 256 || p.D % 16 || p.rot < 0 || p.rot > p.D || p.rot % 16 || p.H < 0 || p.Hkv < 0 || p.H + p.Hkv < 1 || p.S < 1) return -ERR_BAD_ARG;
   if (p.rot && (!p.cos_t || !p.sin_t || p.table_rows < 1)) return -ERR_BAD_ARG;
+  if ((long)p.T * (p.H + 2l * p.Hkv) > 0x7fff0000l) return -ERR_BAD_ARG;
   if (p.ld_x % vec || p.ld_y % vec || p.ld_dy % vec) return -ERR_BAD_ARG;
   if (((uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.dy | (uintptr_t)p.wq | (uintptr_t)p.wk | (uintptr_t)p.cos_t | (uintptr_t)p.sin_t) % 16) return -ERR_BAD_ARG;
   return 0;
 }
-#define INV_QK_L(T, KERNEL)                                                                                                   \
-  switch (head_lanes(p.D)) {                                                                                                  \
-    case 1: launch_early(KERNEL<T, 1>, grid, 256, 0, st, p); break;                                                                     \
-    case 2: launch_early(KERNEL<T, 2>, grid, 256, 0, st, p); break;                                                                     \
-    case 4: launch_early(KERNEL<T, 4>, grid, 256, 0, st, p); break;                                                                     \
-    case 8: launch_early(KERNEL<T, 8>, grid, 256, 0, st, p); break;                                                                     \
-    default: launch_early(KERNEL<T, 16>, grid, 256, 0, st, p);                                                                          \
+template <typename T, int L>
+static void qk_fwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
+  launch_early(qk_norm_fwd_kernel<T, L>, grid, 256, 0, st, p);
+}
+template <typename T, int L>
+static void qk_bwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
+  static std::atomic<uint64_t> ready{0};
+  raise_smem(qk_norm_bwd_kernel<T, L>, QkRing<T>::BYTES, ready);
+  launch_early(qk_norm_bwd_kernel<T, L>, grid, 256, QkRing<T>::BYTES, st, p);
+}
+#define INV_QK_L(T, LAUNCH)                       \
+  switch (head_lanes(p.D)) {                      \
+    case 1: LAUNCH<T, 1>(p, grid, st); break;     \
+    case 2: LAUNCH<T, 2>(p, grid, st); break;     \
+    case 4: LAUNCH<T, 4>(p, grid, st); break;     \
+    case 8: LAUNCH<T, 8>(p, grid, st); break;     \
+    default: LAUNCH<T, 16>(p, grid, st);          \
   }
 
 // x, y: [T, (H + 2 Hkv) D], bf16 or fp32 (then the weights are too), rows ld_x and ld_y apart. cos_t, sin_t: [table_rows, rot / 2] fp32.
 extern "C" int inv_qk_norm_fwd(const void* x, long ld_x, void* y, long ld_y, const void* wq, const void* wk, const float* cos_t, const float* sin_t,
                                int table_rows, const int* pos, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status,
                                void* stream) {
-  QkNorm p{x, wq, wk, nullptr, y, cos_t, sin_t, pos, nullptr, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, ld_x, ld_y, 0, eps, 1.f / (float)D};
+  QkNorm p{x, wq, wk, nullptr, y, cos_t, sin_t, pos, nullptr, status, T, S, H, Hkv, D, rot, table_rows, 0, {}, {}, 0, 0, 0, ld_x, ld_y, 0, eps, 1.f / (float)D};
   if (int rc = qk_norm_args(p, f32)) return rc;
   if (T <= 0) return 0;
-  const int slots = H + 2 * Hkv;
-  p.chunk = slot_chunk(T, slots, 32 / head_lanes(D));
-  const long items = (long)T * ((slots + p.chunk - 1) / p.chunk);
-  const unsigned grid = (unsigned)((items + 7) / 8);
+  const int slots = H + 2 * Hkv, hpw = 32 / head_lanes(D);
+  p.inv_s = div_reciprocal(S);
+  p.inv_slots = div_reciprocal(slots);
+  const unsigned grid = (unsigned)qk_ctas(T, slots, hpw, 296);
+  p.run = qk_run(T, slots, hpw, f32 ? UNITS<float> : UNITS<__nv_bfloat16>, grid);
   cudaStream_t st = (cudaStream_t)stream;
-  if (f32) { INV_QK_L(float, qk_norm_fwd_kernel) } else { INV_QK_L(__nv_bfloat16, qk_norm_fwd_kernel) }
+  if (f32) { INV_QK_L(float, qk_fwd) } else { INV_QK_L(__nv_bfloat16, qk_fwd) }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
@@ -249,17 +317,21 @@ extern "C" int inv_qk_norm_bwd_grid(int T, int H, int Hkv, int D) {
 extern "C" int inv_qk_norm_bwd(const void* x, long ld_x, const void* dy, long ld_dy, void* dx, long ld_dx, const void* wq, const void* wk,
                                const float* cos_t, const float* sin_t, int table_rows, const int* pos, void* dwq, int mode_q, void* dwk, int mode_k,
                                float* part, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status, void* stream) {
-  QkNorm p{x, wq, wk, dy, dx, cos_t, sin_t, pos, part, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, ld_x, ld_dx, ld_dy, eps, 1.f / (float)D};
+  QkNorm p{x, wq, wk, dy, dx, cos_t, sin_t, pos, part, status, T, S, H, Hkv, D, rot, table_rows, 0, {}, {}, 0, 0, 0, ld_x, ld_dx, ld_dy, eps, 1.f / (float)D};
   if (int rc = qk_norm_args(p, f32)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   unsigned grid = 0;
   if (T > 0) {
     const QkBwdCut cut(T, H, Hkv, D);
-    p.chunk = cut.chunk;
-    p.chunk_q = cut.chunk_q;
+    const int hpw = 32 / head_lanes(D);
+    p.run_q = qk_run(T, H, hpw, 1, cut.ctas_q);
+    p.run = qk_run(T, 2 * Hkv, hpw, 1, cut.ctas - cut.ctas_q);
+    p.inv_s = div_reciprocal(S);
+    p.inv_slots = div_reciprocal(Hkv ? 2 * Hkv : 1);
+    p.inv_slots_q = div_reciprocal(H ? H : 1);
     p.ctas_q = cut.ctas_q;
     grid = (unsigned)cut.ctas;
-    if (f32) { INV_QK_L(float, qk_norm_bwd_kernel) } else { INV_QK_L(__nv_bfloat16, qk_norm_bwd_kernel) }
+    if (f32) { INV_QK_L(float, qk_bwd) } else { INV_QK_L(__nv_bfloat16, qk_bwd) }
   }
   launch_early(qk_norm_dw_kernel, dim3((D + 31) / 32, 2), 1024, 0, st, (const float*)part, p.ctas_q, (int)grid, D, dwq, dwk, mode_q, mode_k);
   const cudaError_t e = cudaGetLastError();
