@@ -318,8 +318,10 @@ def _head_norm_rope(x, weight, eps, cos, sin):
 
 def _rows16(x, width):
     """x as rows [T, width] that start on 16-byte boundaries: a view where it is one, else a copy."""
-    x = x.reshape(-1, width)
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) * x.element_size() % 16) or x.data_ptr() % 16:
+    if x.dim() != 2:
+        x = x.reshape(-1, width)
+    row, step = x.stride()
+    if step != 1 or (x.shape[0] > 1 and row * x.element_size() % 16) or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
@@ -333,20 +335,26 @@ def _ld(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]          # the stride of a single row says nothing
 
 
+def _qk_norm_forward(qkv, wq, wk, spec):
+    """-> the result, the rows that were read, and what the backward pass's entry is given too."""
+    cos, sin, positions, seq_len, heads, kv_heads, dim, eps = spec
+    width = qkv.shape[-1]
+    x = _rows16(qkv, width)
+    a, b = _weights16(wq, wk)
+    y = torch.empty_like(qkv, memory_format=torch.contiguous_format)
+    rot, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
+    sizes = (x.shape[0], seq_len, heads, kv_heads, dim, rot, eps, int(x.dtype == torch.float32), rt.status_tensor(x.device).data_ptr())
+    rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), _ld(x), y.data_ptr(), width, a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
+                                      rt.ptr(positions), *sizes, rt.stream_ptr()), "inv_qk_norm_fwd")
+    return y, x, rows, sizes
+
+
 class _QkNormRopeFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, wq, wk, cos, sin, positions, seq_len, heads, kv_heads, dim, eps):
-        x = _rows16(qkv, qkv.shape[-1])
-        T, W = x.shape
-        y = torch.empty(qkv.shape, dtype=x.dtype, device=x.device)
-        rot, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
-        a, b = _weights16(wq, wk)
-        ctx.rows, ctx.sizes = rows, (T, seq_len, heads, kv_heads, dim, rot, float(eps), int(x.dtype == torch.float32),
-                                     rt.status_tensor(x.device).data_ptr())
-        rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), _ld(x), y.data_ptr(), W, a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
-                                          rt.ptr(positions), *ctx.sizes, rt.stream_ptr()), "inv_qk_norm_fwd")
+    def forward(ctx, qkv, wq, wk, spec):
+        y, x, ctx.rows, ctx.sizes = _qk_norm_forward(qkv, wq, wk, spec)
         ctx.main_grads = main_grads(wq, wk)
-        ctx.save_for_backward(x, wq, wk, cos, sin, positions)
+        ctx.save_for_backward(x, wq, wk, *spec[:3])
         return y
 
     @staticmethod
@@ -354,25 +362,26 @@ class _QkNormRopeFn(torch.autograd.Function):
     def backward(ctx, dy):
         x, wq, wk, cos, sin, positions = ctx.saved_tensors
         T, _, H, G, D = ctx.sizes[:5]
-        d, (a, b) = _rows16(dy, x.shape[1]), _weights16(wq, wk)
-        dx = torch.empty(dy.shape, dtype=x.dtype, device=x.device)
+        width = x.shape[1]
+        d, (a, b) = _rows16(dy, width), _weights16(wq, wk)
+        dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
         mg_q, mg_k = (main_grad_of(w, kept) for w, kept in zip((wq, wk), ctx.main_grads))
         shared = None
         if mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr():     # one weight for both norms: added one after the other
             shared = mg_k = torch.zeros_like(mg_q)
-        grads = [None if mg is not None else torch.empty(w.shape, dtype=w.dtype, device=w.device) for w, mg in ((wq, mg_q), (wk, mg_k))]
+        grads = [None if mg is not None else torch.empty_like(w, memory_format=torch.contiguous_format) for w, mg in ((wq, mg_q), (wk, mg_k))]
         outs = []
         for g, mg in zip(grads, (mg_q, mg_k)):
             outs += [mg.data_ptr(), 2] if mg is not None else [g.data_ptr(), int(g.dtype == torch.float32)]
         grid = rt.lib().inv_qk_norm_bwd_grid(T, H, G, D)
         part = torch.empty(max(grid, 1) * D, dtype=torch.float32, device=x.device)
-        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), _ld(x), d.data_ptr(), _ld(d), dx.data_ptr(), x.shape[1], a.data_ptr(), b.data_ptr(),
+        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), _ld(x), d.data_ptr(), _ld(d), dx.data_ptr(), width, a.data_ptr(), b.data_ptr(),
                                           rt.ptr(cos), rt.ptr(sin), ctx.rows, rt.ptr(positions), *outs, part.data_ptr(), *ctx.sizes,
                                           rt.stream_ptr()), "inv_qk_norm_bwd")
         rt.count_launches(1)
         if shared is not None:
             mg_q.add_(shared)
-        return (dx, *grads, None, None, None, None, None, None, None, None)
+        return dx, *grads, None
 
 
 def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_dim, positions=None, eps=1e-6):
@@ -386,7 +395,7 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
     if qkv.dim() < 2 or qkv.shape[-1] != width or n_q_heads < 1 or n_kv_heads < 1:
         raise ValueError(f"qkv of {tuple(qkv.shape)} for {n_q_heads} query and {n_kv_heads} key heads of {head_dim}")
     for w in (q_weight, k_weight):
-        if w.shape != (head_dim,) or w.dtype != qkv.dtype or w.device != qkv.device:
+        if w.shape != (head_dim,) or w.dtype is not qkv.dtype or w.get_device() != qkv.get_device():
             raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {qkv.dtype} heads of {head_dim} on {qkv.device}")
     rot = check_rope(cos, sin, head_dim, qkv.device)
     tokens = qkv.numel() // width
@@ -414,8 +423,11 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
         positions = positions.reshape(-1).to(torch.int32).contiguous()
     if rot:
         cos, sin = cos.contiguous(), sin.contiguous()
+    spec = (cos, sin, positions, max(S, 1), n_q_heads, n_kv_heads, head_dim, float(eps))
     with rt.device_of(qkv):
-        return _QkNormRopeFn.apply(qkv, q_weight, k_weight, cos, sin, positions, max(S, 1), n_q_heads, n_kv_heads, head_dim, eps)
+        if torch.is_grad_enabled() and (qkv.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+            return _QkNormRopeFn.apply(qkv, q_weight, k_weight, spec)
+        return _qk_norm_forward(qkv, q_weight, k_weight, spec)[0]
 
 
 # --------------------------------------------------------------------------------------------

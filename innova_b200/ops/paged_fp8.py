@@ -26,6 +26,7 @@ _native.register_cuda_sigs({
 })
 
 PAGE, TOP, MIN_EXP = 16, 448.0, -64
+_e4m3, _fp32, _bf16, _int32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
 
 
 class Fp8Pages(NamedTuple):
@@ -57,37 +58,50 @@ def new_pages(num_pages: int, kv_heads: int, dim: int, device) -> Fp8Pages:
 
 
 def _check(x, what, heads, pages: Fp8Pages, page_table, kv_heads=None):
+    """-> pages, key heads, size of a head. Asked in one expression, a few microseconds; what is wrong with arguments that fail is found by ``_refuse``."""
+    k, v, ks, vs = pages
+    shape, dev = k.shape, x.get_device()
+    if (len(shape) == 4 and shape[2] == PAGE and shape[1] > 0 and v.shape == shape and k.dtype is _e4m3 and v.dtype is _e4m3
+            and ks.shape == shape[:2] and vs.shape == shape[:2] and ks.dtype is _fp32 and vs.dtype is _fp32
+            and k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()
+            and heads > 0 and heads % shape[1] == 0 and (kv_heads is None or kv_heads == shape[1])
+            and page_table.dim() == 2 and page_table.dtype is _int32 and page_table.is_contiguous() and page_table.numel() > 0
+            and x.dim() == 2 and x.stride(1) == 1
+            and dev == k.get_device() == v.get_device() == ks.get_device() == vs.get_device() == page_table.get_device()
+            and (dev < 0 or (x.dtype is _bf16 and shape[3] in (64, 128)))):
+        return shape[0], shape[1], shape[3]
+    _refuse(x, what, heads, pages, page_table, kv_heads)
+
+
+def _refuse(x, what, heads, pages, page_table, kv_heads):
     k = pages.k
     N, G, P, D = k.shape if k.dim() == 4 else (0, 0, 0, 0)
-    if P != PAGE or pages.v.shape != k.shape or k.dtype != torch.float8_e4m3fn or pages.v.dtype != k.dtype:
+    if P != PAGE or pages.v.shape != k.shape or k.dtype != _e4m3 or pages.v.dtype != k.dtype:
         raise ValueError(f"pages of {k.dtype} {tuple(k.shape)} and {pages.v.dtype} {tuple(pages.v.shape)}: [pages, heads, {PAGE}, dim] of float8_e4m3fn")
     for s in (pages.k_scale, pages.v_scale):
-        if s.shape != (N, G) or s.dtype != torch.float32:
+        if s.shape != (N, G) or s.dtype != _fp32:
             raise ValueError(f"page scales of {s.dtype} {tuple(s.shape)}: fp32 {(N, G)}")
     if not all(t.is_contiguous() for t in pages):
         raise ValueError("pages and their scales are contiguous")
     if heads < 1 or G < 1 or heads % G or (kv_heads is not None and kv_heads != G):
         raise ValueError(f"{heads} query heads on pages of {G}")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.is_contiguous() or page_table.numel() == 0:
+    if page_table.dim() != 2 or page_table.dtype != _int32 or not page_table.is_contiguous() or page_table.numel() == 0:
         raise ValueError(f"page table of {page_table.dtype} {tuple(page_table.shape)}: contiguous int32 [rows, pages]")
     if x.dim() != 2 or x.stride(1) != 1:
         raise ValueError(f"{what} of {tuple(x.shape)}: rows of tokens with unit stride")
-    dev = x.device
-    if any(t.device != dev for t in (*pages, page_table)):
-        raise ValueError(f"{what} on {dev}, pages on {k.device}, page table on {page_table.device}")
-    if x.is_cuda:
-        if x.dtype != torch.bfloat16:
-            raise TypeError(f"{what} in bf16 on a GPU, not {x.dtype}")
-        if D not in (64, 128):
-            raise ValueError(f"heads of {D}: 64 or 128 on a GPU")
-    return N, G, D
+    if any(t.device != x.device for t in (*pages, page_table)):
+        raise ValueError(f"{what} on {x.device}, pages on {k.device}, page table on {page_table.device}")
+    if x.dtype != _bf16:
+        raise TypeError(f"{what} in bf16 on a GPU, not {x.dtype}")
+    raise ValueError(f"heads of {D}: 64 or 128 on a GPU")
 
 
-def _check_new(new: NewTokens, dev):
-    n = new.rows.numel()
-    for t, size in ((new.rows, n), (new.cu, n + 1), (new.start, n)):
-        if t.dtype != torch.int32 or t.numel() != size or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"rows, cu and start of {n} sequences: contiguous int32 on {dev}")
+def _check_new(new: NewTokens, x):
+    rows, cu, start = new.rows, new.cu, new.start
+    n, dev = rows.numel(), x.get_device()
+    if not (cu.numel() == n + 1 and start.numel() == n and rows.dtype is _int32 and cu.dtype is _int32 and start.dtype is _int32
+            and rows.is_contiguous() and cu.is_contiguous() and start.is_contiguous() and dev == rows.get_device() == cu.get_device() == start.get_device()):
+        raise ValueError(f"rows, cu and start of {n} sequences: contiguous int32 on {x.device}")
     if n and (new.max_new < 1 or new.max_len < new.max_new):
         raise ValueError(f"max_new {new.max_new}, max_len {new.max_len}")
     return n
@@ -172,7 +186,7 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
         if w is not None and (w.shape != (D,) or w.dtype != qkv.dtype or w.device != qkv.device):
             raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {qkv.dtype} heads of {D} on {qkv.device}")
     rot = check_rope(cos, sin, D, qkv.device)
-    n = _check_new(new, qkv.device)
+    n = _check_new(new, qkv)
     if positions is not None and (positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous() or positions.device != qkv.device):
         raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)}: contiguous int32, one for each of {T} tokens")
     if q_out is None:
@@ -220,7 +234,7 @@ def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens):
     T = k.shape[0]
     if k.shape[1] != G * D or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or v.stride(1) != 1:
         raise ValueError(f"k of {k.dtype} {tuple(k.shape)}, v of {v.dtype} {tuple(v.shape)} for {G} heads of {D}")
-    n = _check_new(new, k.device)
+    n = _check_new(new, k)
     if not k.is_cuda:
         for t0, m, start, ids in _places(new, page_table, N, T):
             _write_tokens(k[t0:t0 + m].float().view(m, G, D), v[t0:t0 + m].float().view(m, G, D), pages, ids, start)
@@ -256,7 +270,7 @@ def _softmax_rows(q, k, v, scale, seen):
 
 def _check_out(out, q, width):
     if out is None:
-        return torch.empty(q.shape[0], width, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != (q.shape[0], width) or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1:
         raise ValueError(f"out of {out.dtype} {tuple(out.shape)} for {q.shape[0]} rows of {width}")
     return out
@@ -265,7 +279,8 @@ def _check_out(out, q, width):
 def _workspace(n, T, heads, kv_heads, dim, max_new, max_len, window, tree, dev):
     """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
     fn = rt.lib().inv_fp8_attend_floats
-    fn.restype = _l
+    if fn.restype is not _l:
+        fn.restype = _l
     floats = fn(n, T, heads, kv_heads, dim, max_new, max_len, window, tree)
     return torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
 
@@ -279,7 +294,7 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
     T = q.shape[0]
     if q.shape[1] != heads * D or window < 0:
         raise ValueError(f"q of {tuple(q.shape)} for {heads} heads of {D}, window {window}")
-    n = _check_new(new, q.device)
+    n = _check_new(new, q)
     scale = D ** -0.5 if scale is None else float(scale)
     out = _check_out(out, q, heads * D)
     if not q.is_cuda:
