@@ -343,7 +343,7 @@ def _qk_norm_forward(qkv, wq, wk, spec):
     a, b = _weights16(wq, wk)
     y = torch.empty_like(qkv, memory_format=torch.contiguous_format)
     rot, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
-    sizes = (x.shape[0], seq_len, heads, kv_heads, dim, rot, eps, int(x.dtype == torch.float32), rt.status_tensor(x.device).data_ptr())
+    sizes = (x.shape[0], seq_len, heads, kv_heads, dim, rot, eps, int(x.dtype == torch.float32), rt.status_ptr(x))
     rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), _ld(x), y.data_ptr(), width, a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
                                       rt.ptr(positions), *sizes, rt.stream_ptr()), "inv_qk_norm_fwd")
     return y, x, rows, sizes

@@ -109,11 +109,16 @@ def _check_new(new: NewTokens, x):
 
 def _on16(x):
     """Whether the rows of x start on 16-byte boundaries."""
-    return x.data_ptr() % 16 == 0 and (x.shape[0] <= 1 or x.stride(0) % 8 == 0)
+    return x.data_ptr() % 16 == 0 and (x.stride(0) % 8 == 0 or x.shape[0] <= 1)
 
 
 def _aligned(x):
     return x if _on16(x) else x.clone(memory_format=torch.contiguous_format)
+
+
+def _rows_for(out):
+    """`out`, or rows to be copied to it where its own are not aligned."""
+    return out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
 
 
 def _ld(x):
@@ -224,7 +229,7 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
         rt.check(rt.lib().inv_fp8_append(at, at + heads * size, ld, at + (heads + G) * size, ld, q_out.data_ptr(), _ld(q_out), heads, G, D,
                                          rt.ptr(q_weight), rt.ptr(k_weight), float(eps), rt.ptr(cos), rt.ptr(sin), cos.shape[0] if rot else 0, rot,
                                          rt.ptr(positions), *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(),
-                                         new.start.data_ptr(), n, T, rt.status_tensor(qkv.device).data_ptr(), rt.stream_ptr()), "inv_fp8_append")
+                                         new.start.data_ptr(), n, T, rt.status_ptr(qkv), rt.stream_ptr()), "inv_fp8_append")
     return q_out
 
 
@@ -245,7 +250,7 @@ def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens):
     with rt.device_of(k):
         rt.check(rt.lib().inv_fp8_append(0, k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), 0, 0, 0, G, D, 0, 0, 0.0, 0, 0, 0, 0, 0,
                                          *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
-                                         rt.status_tensor(k.device).data_ptr(), rt.stream_ptr()), "inv_fp8_append")
+                                         rt.status_ptr(k), rt.stream_ptr()), "inv_fp8_append")
 
 
 def read(pages: Fp8Pages, ids: torch.Tensor, length: int):
@@ -307,12 +312,12 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
         return out
     if T == 0 or n == 0:
         return out
-    q, to = _aligned(q), out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
+    q, to = _aligned(q), _rows_for(out)
     with rt.device_of(q):
         work = _workspace(n, T, heads, G, D, new.max_new, new.max_len, window, 0, q.device)
         rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, window,
                                          *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
-                                         new.max_new, new.max_len, rt.ptr(work), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()),
+                                         new.max_new, new.max_len, rt.ptr(work), rt.status_ptr(q), rt.stream_ptr()),
                  "inv_fp8_attend")
     return out if to is out else out.copy_(to)
 
@@ -344,10 +349,10 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
         return out
     if T == 0:
         return out
-    q, to = _aligned(q), out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
+    q, to = _aligned(q), _rows_for(out)
     with rt.device_of(q):
         work = _workspace(T, T, heads, G, D, 1, max_len, 0, 1, q.device)
         rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, *_pool_args(pages, page_table),
                                               row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
-                                              max_len, rt.ptr(work), rt.status_tensor(q.device).data_ptr(), rt.stream_ptr()), "inv_fp8_attend_tree")
+                                              max_len, rt.ptr(work), rt.status_ptr(q), rt.stream_ptr()), "inv_fp8_attend_tree")
     return out if to is out else out.copy_(to)

@@ -21,12 +21,14 @@ class device_of:
     """``with device_of(t)``: launches go to the device of ``t`` and its current stream. Costs nothing where that device is current."""
 
     def __init__(self, t: torch.Tensor):
-        self.index, self.back = t.device.index, None
+        self.index, self.back = t.get_device(), None
 
     def __enter__(self):
-        if self.index is not None and self.index != torch.cuda.current_device():
-            self.back = torch.cuda.current_device()
-            torch.cuda.set_device(self.index)
+        if self.index >= 0:
+            now = torch.cuda.current_device()
+            if self.index != now:
+                self.back = now
+                torch.cuda.set_device(self.index)
 
     def __exit__(self, *exc):
         if self.back is not None:
@@ -48,6 +50,12 @@ def status_tensor(device=None) -> torch.Tensor:
         t = torch.zeros(1, dtype=torch.int32, device=dev)
         _status[key] = t
     return t
+
+
+def status_ptr(t: torch.Tensor) -> int:
+    """Where kernels that work on ``t``, on a GPU, write that code."""
+    word = _status.get(t.get_device())
+    return (status_tensor(t.device) if word is None else word).data_ptr()
 
 
 _on_error = []
