@@ -1218,7 +1218,10 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
-constexpr int FP8_FEW_ROWS = 32;      // of a sequence and key head, for the kernel of 16-row tiles
+// Rows of a sequence and key head up to which the kernel of 16-row tiles takes them, each tile reading the pages again, and not the one of 256. Of 32 heads
+// on 8, the small kernel and the large one: 16 sequences of 4000 with 8 / 12 / 16 new tokens each 58, 83, 108 and 85 us; 64 of 1000 66, 95, 116 and 102;
+// one of 4000 13.6, 14.2, 15.3 and 15.4, 16.0, 16.4.
+constexpr int FP8_FEW_ROWS = 48;
 // How an attention is cut: rows of a tile (8 `blocks`), warps and pages of a CTA, CTAs along a sequence.
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
@@ -1226,24 +1229,36 @@ struct Fp8Cut {
     const long rows = (long)max_new * G;
     blocks = rows <= 8 ? 1 : rows <= FP8_FEW_ROWS || tree ? 2 : FT_ROWS / 8;
     tiles = (int)((rows + 8 * blocks - 1) / (8 * blocks));
-    const long span = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
+    const int tokens = max_new < 8 * blocks / G + 2 ? max_new : 8 * blocks / G + 2;       // of a tile
+    const long span = window > 0 && (long)window + tokens < max_len ? (long)window + tokens : max_len;
     const int pages = (int)((span + (window > 0 ? 2 * FP8_PAGE - 2 : FP8_PAGE - 1)) / FP8_PAGE);       // a window may begin inside a page
     const long units = (long)n * Hkv * tiles;
     // Joining the splits costs about three microseconds, and a CTA as much before its first and behind its last page, so up to 64 pages stay together (64 x
     // 640 tokens, 512 units: 22.3 us, in two parts 25.9; 16 x 4 on 1000: 14.4 and 17.1). Longer ones are cut for two CTAs an SM, in parts of 16 pages or more
-    // (2000 tokens, 16 units: 16 / 32 / 64 / 126 pages 7.5, 9.6, 12.1, 15.3 us; 32000, 8 units: 24 / 64 / 128 pages 23.5, 17.8, 19.9) and of about 128 where
-    // there are many, which evens unequal lengths out (8 of up to 65000: 128 pages 71.7 us, 512 91.1). Where units alone fill the GPU several times, CTAs of
+    // (2000 tokens, 16 units: 16 / 32 / 64 / 126 pages 7.5, 9.6, 12.1, 15.3 us; 32000, 8 units: 24 / 64 / 128 pages 23.5, 17.8, 19.9) and of 128 at most,
+    // which evens unequal lengths out (8 of up to 65000: 128 / 192 / 512 pages 71.5, 84.6, 91.2 us; of 64999 each 165, 171, 209; 64 of 8000 164, 167). Where units alone fill the GPU several times, CTAs of
     // two warps, which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251 90.1 and 106.6).
     const bool many = blocks == 1 && units > 444 && pages <= 256;
     warps = many ? 2 : 4;
     const long total = units * pages;
     long want = (total + 295) / 296;
-    if (want > 128) want = total / 1184 > 128 ? total / 1184 : 128;
+    if (want > 128) want = 128;
     if (blocks == FT_ROWS / 8) {                                      // whole blocks of keys
-      if (want < 4 * FT_PAGES) want = 4 * FT_PAGES;
-      per = want < pages ? (int)((want + FT_PAGES - 1) / FT_PAGES * FT_PAGES) : (pages + FT_PAGES - 1) / FT_PAGES * FT_PAGES;
-      splits = ((pages + FT_PAGES - 1) / FT_PAGES * FT_PAGES + (window > 0 ? FT_PAGES : 0) + per - 1) / per;
-      if (pages <= per) splits = 1;
+      // One CTA an SM. A page takes a CTA about 0.3 us, all else as much as 24 pages; a join costs 10 of them and the partial results their bytes. Cut where
+      // that comes out ahead (4 x 128 on 20000, 64 units: in 5 314 us, whole 424; 16 x 32 on 4000, 128 units: in 2 103, whole 87; 64 on 8000, 8 units: in 16
+      // 31, in 4 55).
+      const int most = pages / (2 * FT_PAGES) < 64 ? pages / (2 * FT_PAGES) : 64;
+      const double bytes = (double)n * max_new * Hkv * G * 8 * 130 / 1.2e6;
+      double best = 0;
+      for (int s = 1; s == 1 || s <= most; ++s) {
+        const int p = ((pages + s - 1) / s + FT_PAGES - 1) / FT_PAGES * FT_PAGES, parts = (pages + p - 1) / p;
+        const double cost = (double)((units * parts + 147) / 148) * (p + 24) + (s > 1 ? 10 + parts * bytes : 0);
+        if (s == 1 || cost < best) {
+          best = cost;
+          per = p;
+          splits = parts;
+        }
+      }
       return;
     }
     if (want < 16) want = 16;
