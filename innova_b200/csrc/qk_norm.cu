@@ -6,18 +6,14 @@
 //
 // Both are bound by memory: forward reads and writes the buffer once, backward reads dy, reads x of the normed heads and writes dx. Heads live in the
 // lanes of a warp as units that hold both halves of their rotation pairs (head_norm.cuh), with two 16-byte loads a lane and no shuffles but the sum
-// over a head. A lane has several units on their way at once, of heads that lie one behind the other.
+// over a head. The warps stay and take heads that lie one behind the other; what they read next is on its way meanwhile. 16384 tokens, 32 heads of 128 on
+// 8, bf16: forward 72 us (5.6 TB/s), backward 114 (5.0), sums of dw 8 at most, all three in a graph 178; instructions, at two thirds of what the SMs can
+// issue, come next to memory, so the arithmetic is in pairs.
 #include "head_norm.cuh"
 #include "inv_api.h"
 
 namespace inv {
 
-// How head slots, a token's behind the other's, are dealt to warps: a lane has `units` of them on their way at once, and a warp goes on for `rounds`, all in
-// the same token, whose angles it then loads once.
-struct QkRun {
-  int units, rounds;
-  bool same;                   // what a warp has on its way at once is of one token
-};
 struct QkNorm {
   const void *x, *wq, *wk, *dy;
   void* y;                     // forward: the result; backward: dx
@@ -26,79 +22,117 @@ struct QkNorm {
   float* part;                 // backward: sums of dw, [ctas_q, D] of the queries' norm and [the others, D] of the keys'
   int* status;
   int T, S, H, Hkv, D, rot, table_rows, ctas_q;
-  QkRun run, run_q;            // backward: of the key and value heads, of the query heads
+  int rounds, rounds_q;        // steps of a run (Walk); backward: of the key and value heads, of the query heads
   uint32_t inv_s, inv_slots, inv_slots_q;      // div_reciprocal of S and of the head slots of a token (backward: key and value heads, query heads)
   long ld_x, ld_y, ld_dy;
   float eps, inv_d;
 };
 
-// Units that a lane has on its way at once.
-template <typename T>
-constexpr int UNITS = sizeof(T) == 2 ? 4 : 2;
-
-// Head slots s, s + HPW, ... `units` of them; those past the end repeat the last.
-template <int N, int HPW>
-struct Slots {
-  int tok[N], hd[N];
-  bool in[N];
-  __device__ __forceinline__ Slots(int s, int all, int units, int slots, uint32_t inv) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int at = min(s + min(j, units - 1) * HPW, all - 1);
-      in[j] = j < units && s + j * HPW < all;
-      tok[j] = div_by(at, slots, inv);
-      hd[j] = at - tok[j] * slots;
+// The head slots of a call, a token's behind the other's, dealt to warps: 32 / L at a time, in runs of `stride` from `from` on. A run is one step, or the
+// head slots of a token where those are whole steps: its angles are then loaded once.
+struct Walk {
+  long from, stride, jump;
+  int base, step, all;
+  __device__ __forceinline__ Walk(int step, int rounds, int warp, int warps, int all)
+      : from((long)warp * step * rounds), stride((long)step * rounds), jump((long)warps * step * rounds), base((int)from), step(step), all(all) {}
+  __device__ __forceinline__ bool more() const { return from < all; }
+  __device__ __forceinline__ bool first() const { return base == from; }
+  __device__ __forceinline__ void next() {
+    base += step;
+    if (base >= min(from + stride, (long)all)) {
+      from += jump;
+      base = (int)from;
     }
+  }
+};
+// Token and head of a slot; one past the end repeats the last.
+struct Slot {
+  int tok, hd;
+  bool in;
+  __device__ __forceinline__ Slot(int s, int all, int slots, uint32_t inv) {
+    const int at = min(s, all - 1);
+    in = s < all;
+    tok = div_by(at, slots, inv);
+    hd = at - tok * slots;
   }
 };
 __device__ __forceinline__ void load_turn(const QkNorm& p, int t, int u, const HeadUnit& h, Turn& turn) {
   turn.load(p.cos_t, p.sin_t, p.rot, table_row(p.pos ? p.pos[t] : t - div_by(t, p.S, p.inv_s) * p.S, p.table_rows, p.status), u, h);
 }
 
+// What a lane reads of its next steps comes by asynchronous copies into its own places of shared memory, which takes no registers and no barrier. With loads
+// to registers, four units a lane, forward 75 us, and backward, two units, 140. Two CTAs an SM: forward with three 5 us more, with four 35.
+template <typename T, int UNITS, int STAGES_>
+struct QkRing {
+  static constexpr int NP = RawUnit<T>::N, PIECES = UNITS * 2 * NP, STAGES = STAGES_, BYTES = 8 * STAGES * PIECES * 32 * 16;
+  __device__ __forceinline__ static uint4* of_lane(uint4* ring) { return ring + (threadIdx.x >> 5) * (STAGES * PIECES * 32) + (threadIdx.x & 31); }
+  __device__ __forceinline__ static void copy(uint4* mine, int stage, int unit, const T* head, const HeadUnit& h) {
+    const uint32_t to = smem_u32(mine + (stage * PIECES + unit * 2 * NP) * 32);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      copy16_async(to + i * 512, head + h.e0 + i * (16 / sizeof(T)));
+      copy16_async(to + (NP + i) * 512, head + h.e1 + i * (16 / sizeof(T)));
+    }
+  }
+  __device__ __forceinline__ static void get(const uint4* mine, int stage, int unit, RawUnit<T>& raw) {
+#pragma unroll
+    for (int i = 0; i < 2 * NP; ++i) raw.r[i] = mine[(stage * PIECES + unit * 2 * NP + i) * 32];
+  }
+};
+template <typename T>
+using QkFwdRing = QkRing<T, 1, 6>;
+template <typename T>
+using QkBwdRing = QkRing<T, 2, sizeof(T) == 2 ? 3 : 2>;
+
+constexpr int QK_FWD_CTAS = 2;
 template <typename T, int L>
-__global__ void __launch_bounds__(256, 2) qk_norm_fwd_kernel(const __grid_constant__ QkNorm p) {
-  constexpr int HPW = 32 / L, N = UNITS<T>;
-  const int lane = threadIdx.x & 31, u = lane % L, sub = lane / L;
+__global__ void __launch_bounds__(256, QK_FWD_CTAS) qk_norm_fwd_kernel(const __grid_constant__ QkNorm p) {
+  using Ring = QkFwdRing<T>;
+  constexpr int HPW = 32 / L, ST = Ring::STAGES;
+  extern __shared__ uint4 ring[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, u = lane % L, sub = lane / L;
   const int slots = p.H + 2 * p.Hkv, all = p.T * slots;
-  const int step = p.run.units * HPW, stride = step * p.run.rounds;
   const HeadUnit h(u, p.D, p.rot);
   wait_previous();
   release_next();
-  Turn turn;
-  for (long from = (blockIdx.x * 8l + (threadIdx.x >> 5)) * stride; from < all; from += gridDim.x * 8l * stride)
-  for (int base = (int)from; base < min(from + stride, (long)all); base += step) {
-    const Slots<N, HPW> s(base + sub, all, p.run.units, slots, p.inv_slots);
-    RawUnit<T> raw[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) raw[j].fetch((const T*)p.x + s.tok[j] * p.ld_x + s.hd[j] * p.D, h);
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      if (j >= p.run.units) break;
-      if (p.rot && (!p.run.same || (j == 0 && base == from))) load_turn(p, s.tok[j], u, h, turn);
-      uint64_t v[8];
-      raw[j].get(v);
-      head_norm<L>(v, (const T*)(s.hd[j] < p.H ? p.wq : p.wk), h, p.inv_d, p.eps);
-      if (s.hd[j] < p.H + p.Hkv) {
-        turn.apply<false>(h, v);
-        raw[j].set(v);
-      }
-      if (s.in[j] && h.has) raw[j].store((T*)p.y + s.tok[j] * p.ld_y + s.hd[j] * p.D, h);
+  uint4* mine = Ring::of_lane(ring);
+  Walk now(HPW, p.rounds, blockIdx.x * 8 + warp, gridDim.x * 8, all), ahead = now;
+  auto copy = [&](int stage) {
+    if (ahead.more()) {
+      const Slot s(ahead.base + sub, all, slots, p.inv_slots);
+      Ring::copy(mine, stage, 0, (const T*)p.x + s.tok * p.ld_x + s.hd * p.D, h);
+      ahead.next();
     }
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) copy(i);
+  Turn turn;
+  for (int stage = 0; now.more(); now.next()) {
+    const Slot s(now.base + sub, all, slots, p.inv_slots);
+    if (p.rot && now.first()) load_turn(p, s.tok, u, h, turn);
+    copies_wait<ST - 2>();
+    RawUnit<T> raw;
+    Ring::get(mine, stage, 0, raw);
+    uint64_t v[8];
+    raw.get(v);
+    head_norm<L>(v, (const T*)(s.hd < p.H ? p.wq : p.wk), h, p.inv_d, p.eps);
+    copy(stage ? stage - 1 : ST - 1);                // where the step before this one was
+    if (++stage == ST) stage = 0;
+    if (s.hd < p.H + p.Hkv) {
+      turn.apply<false>(h, v);
+      raw.set(v);
+    }
+    if (s.in && h.has) raw.store((T*)p.y + s.tok * p.ld_y + s.hd * p.D, h);
   }
 }
-
-// Backward: what a lane reads of its next steps comes by asynchronous copies into its own places of shared memory, which needs no registers and no barrier.
-template <typename T>
-struct QkRing {
-  static constexpr int PIECES = 4 * RawUnit<T>::N, STAGES = sizeof(T) == 2 ? 4 : 3, BYTES = 8 * STAGES * PIECES * 32 * 16;
-};
 
 // The first ctas_q CTAs take the query heads, the others the key and value heads: a lane then keeps the sums of one dw in registers. A CTA adds its warps'
 // sums in order and leaves one row.
 template <typename T, int L>
 __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_constant__ QkNorm p) {
-  using Ring = QkRing<T>;
-  constexpr int HPW = 32 / L, NP = RawUnit<T>::N, ST = Ring::STAGES;
+  using Ring = QkBwdRing<T>;
+  constexpr int HPW = 32 / L, ST = Ring::STAGES;
   extern __shared__ uint4 ring[];
   __shared__ float sums[8][L * 16];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, u = lane % L, sub = lane / L;
@@ -106,69 +140,46 @@ __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_consta
   const int first = keys ? p.H : 0, normed = keys ? p.Hkv : p.H, slots = keys ? 2 * p.Hkv : p.H, all = p.T * slots;
   const uint32_t inv = keys ? p.inv_slots : p.inv_slots_q;
   const int cta = keys ? blockIdx.x - p.ctas_q : blockIdx.x, ctas = keys ? gridDim.x - p.ctas_q : p.ctas_q;
-  const QkRun run = keys ? p.run : p.run_q;
-  const long stride = HPW * run.rounds, jump = ctas * 8l * stride;
   const HeadUnit h(u, p.D, p.rot);
-  struct Walk {                                      // steps of a warp: HPW slots at `base`, in runs of `stride` from `from` on
-    long from;
-    int base;
-  };
-  auto on = [&](Walk& k) {
-    k.base += HPW;
-    if (k.base >= min(k.from + stride, (long)all)) {
-      k.from += jump;
-      k.base = (int)k.from;
-    }
-  };
   wait_previous();
   release_next();
-  uint4* mine = ring + warp * (ST * Ring::PIECES * 32) + lane;
-  auto copy = [&](Walk& k, int stage) {
-    if (k.from < all) {
-      const Slots<1, HPW> s(k.base + sub, all, 1, slots, inv);
-      const int at = (first + s.hd[0]) * p.D;
-      const T *dy = (const T*)p.dy + s.tok[0] * p.ld_dy + at, *x = s.hd[0] < normed ? (const T*)p.x + s.tok[0] * p.ld_x + at : dy;      // of values only dy
-      const uint32_t to = smem_u32(mine + stage * (Ring::PIECES * 32));
-#pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        copy16_async(to + i * 512, x + h.e0 + i * (16 / sizeof(T)));
-        copy16_async(to + (NP + i) * 512, x + h.e1 + i * (16 / sizeof(T)));
-        copy16_async(to + (2 * NP + i) * 512, dy + h.e0 + i * (16 / sizeof(T)));
-        copy16_async(to + (3 * NP + i) * 512, dy + h.e1 + i * (16 / sizeof(T)));
-      }
-      on(k);
+  uint4* mine = Ring::of_lane(ring);
+  Walk now(HPW, keys ? p.rounds : p.rounds_q, cta * 8 + warp, ctas * 8, all), ahead = now;
+  auto copy = [&](int stage) {
+    if (ahead.more()) {
+      const Slot s(ahead.base + sub, all, slots, inv);
+      const int at = (first + s.hd) * p.D;
+      const T* dy = (const T*)p.dy + s.tok * p.ld_dy + at;
+      Ring::copy(mine, stage, 0, s.hd < normed ? (const T*)p.x + s.tok * p.ld_x + at : dy, h);      // of values only dy
+      Ring::copy(mine, stage, 1, dy, h);
+      ahead.next();
     }
     copies_commit();
   };
-  const long mine0 = (cta * 8l + warp) * stride;
-  Walk ahead{mine0, (int)mine0}, now = ahead;
 #pragma unroll
-  for (int i = 0; i < ST - 1; ++i) copy(ahead, i);
+  for (int i = 0; i < ST - 1; ++i) copy(i);
   uint64_t dw[8], w[8];
   load_unit((const T*)(keys ? p.wk : p.wq), h, w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) dw[i] = 0;
   Turn turn;
-  for (int stage = 0; now.from < all; on(now)) {
-    const Slots<1, HPW> s(now.base + sub, all, 1, slots, inv);
-    if (p.rot && (!run.same || now.base == now.from)) load_turn(p, s.tok[0], u, h, turn);
+  for (int stage = 0; now.more(); now.next()) {
+    const Slot s(now.base + sub, all, slots, inv);
+    if (p.rot && now.first()) load_turn(p, s.tok, u, h, turn);
     copies_wait<ST - 2>();
     RawUnit<T> rx, rg;
-#pragma unroll
-    for (int i = 0; i < 2 * NP; ++i) {
-      rx.r[i] = mine[(stage * Ring::PIECES + i) * 32];
-      rg.r[i] = mine[(stage * Ring::PIECES + 2 * NP + i) * 32];
-    }
+    Ring::get(mine, stage, 0, rx);
+    Ring::get(mine, stage, 1, rg);
     uint64_t v[8], g[8];
     rx.get(v);
     rg.get(g);
     const float r = head_rstd<L>(v, h, p.inv_d, p.eps);
-    copy(ahead, stage ? stage - 1 : ST - 1);         // where the step before this one was
+    copy(stage ? stage - 1 : ST - 1);                // where the step before this one was
     if (++stage == ST) stage = 0;
     turn.apply<true>(h, g);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = mul_pair(v[i], pair_of(r, r));           // xh
-    if (s.in[0] && s.hd[0] < normed) {
+    if (s.in && s.hd < normed) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) dw[i] = fma_pair(g[i], v[i], dw[i]);
     }
@@ -183,8 +194,8 @@ __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_consta
     const float mean = head_sum<L>(add_pair(d0, d1), h) * -p.inv_d;
 #pragma unroll
     for (int i = 0; i < 8; ++i) g[i] = mul_pair(pair_of(r, r), fma_pair(v[i], pair_of(mean, mean), g[i]));
-    if (s.hd[0] < normed) rg.set(g);
-    if (s.in[0] && h.has) rg.store((T*)p.y + s.tok[0] * p.ld_y + (first + s.hd[0]) * p.D, h);
+    if (s.hd < normed) rg.set(g);
+    if (s.in && h.has) rg.store((T*)p.y + s.tok * p.ld_y + (first + s.hd) * p.D, h);
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
@@ -230,17 +241,8 @@ __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restric
   else ((__nv_bfloat16*)out)[col] = __float2bfloat16_rn(v);
 }
 
-// Two CTAs an SM stay. As many units a lane as leave the warps of all of them one, then as many rounds as leave each of them two runs.
-static QkRun qk_run(long T, int slots, int hpw, int most, long ctas) {
-  QkRun r{1, 1, false};
-  if (slots < 1 || ctas < 1) return r;
-  const long lanes = (T * slots + hpw - 1) / hpw, warps = 8 * ctas;
-  while (r.units < most && lanes > warps * r.units) r.units *= 2;
-  r.same = slots % (r.units * hpw) == 0;
-  const int whole = slots / (r.units * hpw);
-  if (r.same && T >= 2 * warps) r.rounds = whole;
-  return r;
-}
+// A token's head slots where they are whole steps and that leaves each of the warps, which stay, two tokens or more; else a step, which deals them evenly.
+static int qk_rounds(long T, int slots, int hpw, long ctas) { return slots > hpw && slots % hpw == 0 && T >= 16 * ctas ? slots / hpw : 1; }
 static int qk_ctas(long T, int slots, int hpw, long share) {
   const long ctas = (T * slots + 8 * hpw - 1) / (8 * hpw);
   return (int)(ctas < share ? ctas : share);
@@ -272,13 +274,15 @@ static int qk_norm_args(const QkNorm& p, int f32) {
 }
 template <typename T, int L>
 static void qk_fwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
-  launch_early(qk_norm_fwd_kernel<T, L>, grid, 256, 0, st, p);
+  static std::atomic<uint64_t> ready{0};
+  raise_smem(qk_norm_fwd_kernel<T, L>, QkFwdRing<T>::BYTES, ready);
+  launch_early(qk_norm_fwd_kernel<T, L>, grid, 256, QkFwdRing<T>::BYTES, st, p);
 }
 template <typename T, int L>
 static void qk_bwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
-  raise_smem(qk_norm_bwd_kernel<T, L>, QkRing<T>::BYTES, ready);
-  launch_early(qk_norm_bwd_kernel<T, L>, grid, 256, QkRing<T>::BYTES, st, p);
+  raise_smem(qk_norm_bwd_kernel<T, L>, QkBwdRing<T>::BYTES, ready);
+  launch_early(qk_norm_bwd_kernel<T, L>, grid, 256, QkBwdRing<T>::BYTES, st, p);
 }
 #define INV_QK_L(T, LAUNCH)                       \
   switch (head_lanes(p.D)) {                      \
@@ -293,14 +297,14 @@ static void qk_bwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
 extern "C" int inv_qk_norm_fwd(const void* x, long ld_x, void* y, long ld_y, const void* wq, const void* wk, const float* cos_t, const float* sin_t,
                                int table_rows, const int* pos, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status,
                                void* stream) {
-  QkNorm p{x, wq, wk, nullptr, y, cos_t, sin_t, pos, nullptr, status, T, S, H, Hkv, D, rot, table_rows, 0, {}, {}, 0, 0, 0, ld_x, ld_y, 0, eps, 1.f / (float)D};
+  QkNorm p{x, wq, wk, nullptr, y, cos_t, sin_t, pos, nullptr, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, 0, 0, 0, ld_x, ld_y, 0, eps, 1.f / (float)D};
   if (int rc = qk_norm_args(p, f32)) return rc;
   if (T <= 0) return 0;
   const int slots = H + 2 * Hkv, hpw = 32 / head_lanes(D);
   p.inv_s = div_reciprocal(S);
   p.inv_slots = div_reciprocal(slots);
-  const unsigned grid = (unsigned)qk_ctas(T, slots, hpw, 296);
-  p.run = qk_run(T, slots, hpw, f32 ? UNITS<float> : UNITS<__nv_bfloat16>, grid);
+  const unsigned grid = (unsigned)qk_ctas(T, slots, hpw, 148 * QK_FWD_CTAS);
+  p.rounds = qk_rounds(T, slots, hpw, grid);
   cudaStream_t st = (cudaStream_t)stream;
   if (f32) { INV_QK_L(float, qk_fwd) } else { INV_QK_L(__nv_bfloat16, qk_fwd) }
   const cudaError_t e = cudaGetLastError();
@@ -317,15 +321,15 @@ extern "C" int inv_qk_norm_bwd_grid(int T, int H, int Hkv, int D) {
 extern "C" int inv_qk_norm_bwd(const void* x, long ld_x, const void* dy, long ld_dy, void* dx, long ld_dx, const void* wq, const void* wk,
                                const float* cos_t, const float* sin_t, int table_rows, const int* pos, void* dwq, int mode_q, void* dwk, int mode_k,
                                float* part, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status, void* stream) {
-  QkNorm p{x, wq, wk, dy, dx, cos_t, sin_t, pos, part, status, T, S, H, Hkv, D, rot, table_rows, 0, {}, {}, 0, 0, 0, ld_x, ld_dx, ld_dy, eps, 1.f / (float)D};
+  QkNorm p{x, wq, wk, dy, dx, cos_t, sin_t, pos, part, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, 0, 0, 0, ld_x, ld_dx, ld_dy, eps, 1.f / (float)D};
   if (int rc = qk_norm_args(p, f32)) return rc;
   cudaStream_t st = (cudaStream_t)stream;
   unsigned grid = 0;
   if (T > 0) {
     const QkBwdCut cut(T, H, Hkv, D);
     const int hpw = 32 / head_lanes(D);
-    p.run_q = qk_run(T, H, hpw, 1, cut.ctas_q);
-    p.run = qk_run(T, 2 * Hkv, hpw, 1, cut.ctas - cut.ctas_q);
+    p.rounds_q = qk_rounds(T, H, hpw, cut.ctas_q);
+    p.rounds = qk_rounds(T, 2 * Hkv, hpw, cut.ctas - cut.ctas_q);
     p.inv_s = div_reciprocal(S);
     p.inv_slots = div_reciprocal(Hkv ? 2 * Hkv : 1);
     p.inv_slots_q = div_reciprocal(H ? H : 1);
