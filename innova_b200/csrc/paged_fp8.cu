@@ -1008,7 +1008,9 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           mx = fmaxf(mx, fmaxf(x0, x1) * (qm * k.x));
           v_up = fmaxf(v_up, k.y);
         }
-        if (__any_sync(0xffffffffu, mx > m + SLACK || v_up > vref)) {
+        // The last block passes here too, for the wait: the product after this one is waited for behind the loop, a barrier's parity tells a phase from its
+        // neighbours only, and here it is sure that the phase before has ended and the one after has not.
+        if (__any_sync(0xffffffffu, mx > m + SLACK || v_up > vref) || j == nb - 1) {
           rarely();
           const float up = j == 0 || mx > m + SLACK ? fmaxf(m, mx) : m;
           float alpha = up == m ? 1.f : exp2_fast(m - up);
@@ -1024,8 +1026,9 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
               break;
             }
             tc_fence_after();
+            const int steps = __any_sync(0xffffffffu, alpha != 1.f) ? D / 16 : 0;
 #pragma unroll 1
-            for (int cc = 0; cc < D / 16; ++cc) {
+            for (int cc = 0; cc < steps; ++cc) {
               uint32_t o[16];
               tmem_ld_32x16(t_o + cc * 16, o);
               tmem_ld_wait();
@@ -1079,8 +1082,6 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[t][j & 1]);
       }
-      // the last two products, in turn: a barrier's parity tells a phase from the next one only
-      if (ok && nb > 1) ok = mbar_wait_warp(&o_full[t], nb & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
       if (ok) ok = mbar_wait_warp(&o_full[t], (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
       if (ok) {
         tc_fence_after();

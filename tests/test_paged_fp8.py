@@ -181,6 +181,22 @@ def test_attend_extreme_values(dev):
     check_attend(s, q=q)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("ctx, new", [([300, 41], [600, 35]), ([0], [130]), ([1000], [64])])
+def test_many_rows_again_and_again(ctx, new):
+    """The roles of a CTA hand blocks to one another hundreds of times in each of these calls: no wait may run out, and no result may change."""
+    s = Setup(ctx, new, 32, 8, 128, "cuda")
+    q = s.q()
+    outs = [torch.empty(s.T, 32 * 128, dtype=q.dtype, device="cuda") for _ in range(8)]
+    first = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 32)
+    for i in range(4000):
+        pf.kv_attend(q, s.pool, s.page_table, s.tokens, 32, out=outs[i % 8])
+        if i % 250 == 0:
+            assert torch.equal(outs[i % 8], first)
+    assert all(torch.equal(o, first) for o in outs)
+    rt.check_status()
+
+
 TREE = [([30, 5, 0], 4, 2, 64, [0, 0, 1, 2, 1, 0]), ([3000, 17], 8, 1, 128, [1, 0, 0])]
 
 
