@@ -739,7 +739,10 @@ struct FtSmem {
 //   warps 8-11   codes of the next blocks from the pages to registers, as fp16 to shared memory, for both tiles
 //   warps 12-13  issue a tile's S = Q K^T and O += P V (P from tensor memory)
 // A tile has two places for scores: the next block's are computed under this one's softmax, so that a row's chain does not wait for products (with one, and
-// blocks of 128 keys, a tile's softmax and products took turns: 548 us for 2 x 1500 tokens on 5500, 32 heads of 128 on 8).
+// blocks of 128 keys, a tile's softmax and products took turns: 548 us in two parts against 514).
+// 2 x 1500 tokens on 5500, 32 heads of 128 on 8: 411 us, 748 TFLOP/s. A block takes both tiles some 2400 cycles, of which the tensor cores are busy with
+// 1260 (the queries are read from shared memory again for 64 keys each) and the exponentials' unit 1024: what bounds it is a row's chain of reading scores,
+// maximum, exponentials and writing weights. Four warps for each half of a block's keys shorten the chain, but the exponentials of all then fall together: 443.
 // Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are powers of two added to it (relative to the
 // largest one so far, which O is kept in) and taken out of the row sum again a page at a time, so neither costs anything a score. For the rest the sums are
 // those of the small kernel. Tensor memory, a tile 256 columns: scores (then weights) at 0 and 64, O at 128.
@@ -860,7 +863,8 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
     constexpr int PER = FT_N * CH / 128, STEP = 128 / CH;      // pieces of a thread in a block; tokens from one to the next
     const int piece = tid % CH, tok0 = tid / CH, pages_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
     uint4 rk[2][PER], rv[2][PER];                    // of even and odd blocks, two ahead
-    // Lanes 0 to 3 look a block's pages up: read three blocks ahead, checked two ahead and codes and scales read then, so that nothing is waited for. Loads stand outside of branches, from a place that exists where there is none to read: behind a branch the compiler copies what was loaded, and so waits for each in turn.
+    // Lanes 0 to 3 look a block's pages up: read three blocks ahead, checked two ahead and codes and scales read then, so that nothing is waited for. Loads
+    // stand outside of branches, from a place that exists where there is none to read: behind a branch the compiler copies what was loaded, and so waits.
     const bool known = (unsigned)row < (unsigned)tk.table_rows;
     const int* list = tk.page_table + (known ? (long)row * tk.max_pages : 0);
     auto read_id = [&](int j) { return list[min((b0 + j) * FT_PAGES + lane, tk.max_pages - 1)]; };
@@ -980,7 +984,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
         uint32_t s[FT_N];
         const uint32_t t_s = t_lane + t * T_COLS + (j & 1) * FT_N;
 #pragma unroll
-        for (int cc = 0; cc < FT_N / 32; ++cc) tmem_ld_32x32(t_s + cc * 32, s + cc * 32);
+        for (int cc = 0; cc < FT_N / 16; ++cc) tmem_ld_32x16(t_s + cc * 16, s + cc * 16);
         const float2* sc = scales[j & 7];
         const int k0 = (b0 + j) * FT_N;
         const uint32_t there = present[j & 7];
