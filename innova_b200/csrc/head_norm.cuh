@@ -127,6 +127,26 @@ __device__ __forceinline__ void load_unit(const T* head, const HeadUnit& u, uint
   raw.get(x);
 }
 
+// Units that a lane will read come by asynchronous copies into its own places of shared memory, which takes no registers and no barrier: a ring of STAGES
+// steps of UNITS units for each of WARPS warps.
+template <typename T, int UNITS, int STAGES_, int WARPS>
+struct UnitRing {
+  static constexpr int NP = RawUnit<T>::N, PIECES = UNITS * 2 * NP, STAGES = STAGES_, BYTES = WARPS * STAGES * PIECES * 32 * 16;
+  __device__ __forceinline__ static uint4* of_lane(uint4* ring) { return ring + (threadIdx.x >> 5) * (STAGES * PIECES * 32) + (threadIdx.x & 31); }
+  __device__ __forceinline__ static void copy(uint4* mine, int stage, int unit, const T* head, const HeadUnit& h) {
+    const uint32_t to = smem_u32(mine + (stage * PIECES + unit * 2 * NP) * 32);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      copy16_async(to + i * 512, head + h.e0 + i * (16 / sizeof(T)));
+      copy16_async(to + (NP + i) * 512, head + h.e1 + i * (16 / sizeof(T)));
+    }
+  }
+  __device__ __forceinline__ static void get(const uint4* mine, int stage, int unit, RawUnit<T>& raw) {
+#pragma unroll
+    for (int i = 0; i < 2 * NP; ++i) raw.r[i] = mine[(stage * PIECES + unit * 2 * NP + i) * 32];
+  }
+};
+
 // Sum over the L lanes of a head; what a lane without a unit brings counts for nothing.
 template <int L>
 __device__ __forceinline__ float head_sum(uint64_t two, const HeadUnit& u) {
@@ -161,9 +181,12 @@ struct Turn {
   uint64_t c[4], s[4];
   __device__ __forceinline__ void load(const float* cos_t, const float* sin_t, int rot, int pos, int u, const HeadUnit& h) {
     const size_t at = (size_t)pos * (rot / 2) + (h.turns ? u * 8 : 0);
+    take(reinterpret_cast<const float4*>(cos_t + at), reinterpret_cast<const float4*>(sin_t + at));
+  }
+  __device__ __forceinline__ void take(const float4* cosines, const float4* sines) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float4 a = reinterpret_cast<const float4*>(cos_t + at)[i], b = reinterpret_cast<const float4*>(sin_t + at)[i];
+      const float4 a = cosines[i], b = sines[i];
       c[2 * i] = pair_of(a.x, a.y);
       c[2 * i + 1] = pair_of(a.z, a.w);
       s[2 * i] = pair_of(b.x, b.y);

@@ -73,16 +73,25 @@ struct Fp8Append {
   float eps;
 };
 
+// Memory bounds it where there are many tokens: 2 x 8000 of 32 heads of 128 on 8, 369 MB in 65.5 us (5.6 TB/s). With rows in registers and angles read from
+// the tables by each head, whose latency nothing hid, 82 us; with 32-bit rows in registers at one CTA an SM 193. A call of 64 x 1 takes 4.0 us, its chain of
+// sequence, page, scale and store. Five CTAs an SM; four 5 us more, six 1.
+constexpr int FP8_APPEND_CTAS = 5;
+using Fp8AppendRing = UnitRing<__nv_bfloat16, 4, 2, 4>;
 // A CTA takes the new tokens of one page, or with blockIdx.y a share of what they bring: items for its warps. Sequence i owns the CTAs from cu[i] / 16 + 2 i
 // on, which is enough for the pages that its tokens touch wherever it starts. An item is the keys or the values of one head, all of the page's new tokens
-// in a warp's registers, so that their largest value is known before any is rounded; or a run of query heads. Rows stay in registers as they were read
-// (keys are normed and turned twice, for their largest value and for the codes), so that three CTAs an SM keep four units a lane on their way.
+// before a warp, so that their largest value is known before any is rounded; or a run of query heads. A warp's next item is on its way while it works on
+// one, whose rows it reads again where it needs them (keys are normed and turned twice, for their largest value and for the codes).
 template <int D>
-__global__ void __launch_bounds__(128, 4) fp8_append_kernel(const __grid_constant__ Fp8Append a, const __grid_constant__ Fp8Pool pool,
+__global__ void __launch_bounds__(128, FP8_APPEND_CTAS) fp8_append_kernel(const __grid_constant__ Fp8Append a, const __grid_constant__ Fp8Pool pool,
                                                             const __grid_constant__ Fp8Tokens tk) {
   constexpr int L = D / 16, HPW = 32 / L, NIT = FP8_PAGE / HPW, NQ = 4;
   using Raw = RawUnit<__nv_bfloat16>;
+  using Ring = Fp8AppendRing;
+  constexpr int ST = Ring::STAGES;
+  extern __shared__ uint4 units[];
   __shared__ int found[5];
+  __shared__ float4 cosines[FP8_PAGE][D / 8], sines[FP8_PAGE][D / 8];        // of the page's new tokens
   if (threadIdx.x == 0) found[0] = -1;
   __syncthreads();
   wait_previous();
@@ -114,43 +123,74 @@ __global__ void __launch_bounds__(128, 4) fp8_append_kernel(const __grid_constan
   const HeadUnit h(u, D, a.rot);
   const int first = t0 + lo - start;                             // row of the page's first new token
   auto angles = [&](Turn& turn, int i) {
-    turn.load(a.cos_t, a.sin_t, a.rot, table_row(a.pos ? a.pos[first + i] : lo + i, a.table_rows, tk.status), u, h);
+    const int at = h.turns ? u * 2 : 0;
+    turn.take(cosines[i] + at, sines[i] + at);
   };
   const int n_kv = 2 * pool.Hkv, n_q = (m * a.H + NQ * HPW - 1) / (NQ * HPW);
-  for (int item = blockIdx.y * 4 + warp; item < n_kv + n_q; item += gridDim.y * 4) {
+  uint4* mine = Ring::of_lane(units);
+  auto slot = [&](int item, int j, int& tok, int& hd) {          // the j-th head of a run in this lane
+    const int s = (item - n_kv) * (NQ * HPW) + j * HPW + sub, at = min(s, m * a.H - 1);
+    tok = div_by(at, a.H, a.inv_h);
+    hd = at - tok * a.H;
+    return s < m * a.H;
+  };
+  auto fetch = [&](int item, int stage) {
+    if (item < n_kv) {
+      const __nv_bfloat16* src = (item & 1 ? a.v_in : a.k_in) + (item >> 1) * D;
+      const long ld = item & 1 ? a.ld_v : a.ld_in;
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) Ring::copy(mine, stage, it, src + (first + min(it * HPW + sub, m - 1)) * ld, h);      // past the last token: the last
+    } else if (item < n_kv + n_q) {
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        int tok, hd;
+        slot(item, j, tok, hd);
+        Ring::copy(mine, stage, j, a.q_in + (first + tok) * a.ld_in + hd * D, h);
+      }
+    }
+    copies_commit();
+  };
+  const int item0 = blockIdx.y * 4 + warp, step = gridDim.y * 4;
+#pragma unroll
+  for (int i = 0; i < ST - 1; ++i) fetch(item0 + i * step, i);
+  if (a.rot) {                                                   // every head of the page's tokens turns by them
+    const int pieces = a.rot / 8;                                // of 16 bytes, of a token's cosines
+    for (int i = threadIdx.x; i < m * pieces; i += 128) {
+      const int tok = i / pieces, e = i - tok * pieces;
+      const size_t at = (size_t)table_row(a.pos ? a.pos[first + tok] : lo + tok, a.table_rows, tk.status) * pieces + e;
+      cosines[tok][e] = reinterpret_cast<const float4*>(a.cos_t)[at];
+      sines[tok][e] = reinterpret_cast<const float4*>(a.sin_t)[at];
+    }
+    __syncthreads();
+  }
+  int stage = ST - 1;                                            // of the item that is fetched next
+  for (int item = item0; item < n_kv + n_q; item += step) {
+    fetch(item + (ST - 1) * step, stage);                        // where the item before this one was
+    stage = stage + 1 == ST ? 0 : stage + 1;
+    copies_wait<ST - 1>();
     if (item >= n_kv) {
       // ---- heads of tokens, one behind the other ----
-      const int s0 = (item - n_kv) * (NQ * HPW) + sub;
-      Raw raw[NQ];
-      int tok[NQ], hd[NQ];
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
-        const int s = min(s0 + j * HPW, m * a.H - 1);
-        tok[j] = div_by(s, a.H, a.inv_h);
-        hd[j] = s - tok[j] * a.H;
-        raw[j].fetch(a.q_in + (first + tok[j]) * a.ld_in + hd[j] * D, h);
-      }
-      Turn turn;
-      if (a.rot) angles(turn, tok[0]);
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-        if (j && a.rot && tok[j] != tok[j - 1]) angles(turn, tok[j]);
+        int tok, hd;
+        const bool in = slot(item, j, tok, hd);
+        Raw raw;
+        Ring::get(mine, stage, j, raw);
         uint64_t v[8];
-        raw[j].get(v);
+        raw.get(v);
         if (a.wq) head_norm<L>(v, a.wq, h, 1.f / D, a.eps);
-        if (a.rot) turn.apply<false>(h, v);
-        raw[j].set(v);
-        if (s0 + j * HPW < m * a.H) raw[j].store(a.q + (first + tok[j]) * a.ld_q + hd[j] * D, h);
+        if (a.rot) {
+          Turn turn;
+          angles(turn, tok);
+          turn.apply<false>(h, v);
+        }
+        raw.set(v);
+        if (in) raw.store(a.q + (first + tok) * a.ld_q + hd * D, h);
       }
       continue;
     }
     // ---- keys or values of a head ----
     const int hk = item >> 1, which = item & 1;                  // 0 keys, 1 values
-    const __nv_bfloat16* src = (which ? a.v_in : a.k_in) + hk * D;
-    const long ld = which ? a.ld_v : a.ld_in;
-    Raw raw[NIT];
-#pragma unroll
-    for (int it = 0; it < NIT; ++it) raw[it].fetch(src + (first + min(it * HPW + sub, m - 1)) * ld, h);      // lanes past the last token repeat it
     if (!listed || (unsigned)id >= (unsigned)pool.pages) {
       if (lane == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
       continue;
@@ -160,7 +200,9 @@ __global__ void __launch_bounds__(128, 4) fp8_append_kernel(const __grid_constan
     float* scales = (which ? pool.v_scale : pool.k_scale) + block;
     const float old = *scales;
     auto values = [&](int it, uint64_t (&x)[8]) {
-      raw[it].get(x);
+      Raw raw;
+      Ring::get(mine, stage, it, raw);
+      raw.get(x);
       if (which) return;
       if (a.wk) head_norm<L>(x, a.wk, h, 1.f / D, a.eps);
       if (a.rot) {
@@ -1215,10 +1257,12 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   const unsigned ctas = (unsigned)(T / FP8_PAGE + 2 * n);
   const int hpw = 512 / D, tokens = T / n < FP8_PAGE ? (T + n - 1) / n : FP8_PAGE;      // of an average page
   const int items = 2 * Hkv + (tokens * H + 4 * hpw - 1) / (4 * hpw);
-  const int most = (items + 3) / 4, shares = ctas <= 296 ? most : (items + 7) / 8;      // an item a warp where there are few pages, else two
+  // An item a warp where there are few pages (128 sequences with a token each 6.1 us, six items 9.8), else six, behind one another (2 x 8000 tokens 65.5 us; two
+  // items 74.6, twelve 73.1. 16 x 500 with norms 52.8, 49.8, 56.2).
+  const int most = (items + 3) / 4, shares = ctas <= 296 ? most : (items + 23) / 24;
   const dim3 grid(ctas, shares < 65535 ? shares : 65535);
-  if (D == 64) launch_early(fp8_append_kernel<64>, grid, 128, 0, (cudaStream_t)stream, a, pool, tk);
-  else launch_early(fp8_append_kernel<128>, grid, 128, 0, (cudaStream_t)stream, a, pool, tk);
+  if (D == 64) launch_early(fp8_append_kernel<64>, grid, 128, Fp8AppendRing::BYTES, (cudaStream_t)stream, a, pool, tk);
+  else launch_early(fp8_append_kernel<128>, grid, 128, Fp8AppendRing::BYTES, (cudaStream_t)stream, a, pool, tk);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }

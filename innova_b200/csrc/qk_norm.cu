@@ -60,29 +60,11 @@ __device__ __forceinline__ void load_turn(const QkNorm& p, int t, int u, const H
   turn.load(p.cos_t, p.sin_t, p.rot, table_row(p.pos ? p.pos[t] : t - div_by(t, p.S, p.inv_s) * p.S, p.table_rows, p.status), u, h);
 }
 
-// What a lane reads of its next steps comes by asynchronous copies into its own places of shared memory, which takes no registers and no barrier. With loads
-// to registers, four units a lane, forward 75 us, and backward, two units, 140. Two CTAs an SM: forward with three 5 us more, with four 35.
-template <typename T, int UNITS, int STAGES_>
-struct QkRing {
-  static constexpr int NP = RawUnit<T>::N, PIECES = UNITS * 2 * NP, STAGES = STAGES_, BYTES = 8 * STAGES * PIECES * 32 * 16;
-  __device__ __forceinline__ static uint4* of_lane(uint4* ring) { return ring + (threadIdx.x >> 5) * (STAGES * PIECES * 32) + (threadIdx.x & 31); }
-  __device__ __forceinline__ static void copy(uint4* mine, int stage, int unit, const T* head, const HeadUnit& h) {
-    const uint32_t to = smem_u32(mine + (stage * PIECES + unit * 2 * NP) * 32);
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      copy16_async(to + i * 512, head + h.e0 + i * (16 / sizeof(T)));
-      copy16_async(to + (NP + i) * 512, head + h.e1 + i * (16 / sizeof(T)));
-    }
-  }
-  __device__ __forceinline__ static void get(const uint4* mine, int stage, int unit, RawUnit<T>& raw) {
-#pragma unroll
-    for (int i = 0; i < 2 * NP; ++i) raw.r[i] = mine[(stage * PIECES + unit * 2 * NP + i) * 32];
-  }
-};
+// With loads to registers, four units a lane, forward 75 us, and backward, two units, 140. Two CTAs an SM: forward with three 5 us more, with four 35.
 template <typename T>
-using QkFwdRing = QkRing<T, 1, 6>;
+using QkFwdRing = UnitRing<T, 1, 6, 8>;
 template <typename T>
-using QkBwdRing = QkRing<T, 2, sizeof(T) == 2 ? 3 : 2>;
+using QkBwdRing = UnitRing<T, 2, sizeof(T) == 2 ? 3 : 2, 8>;
 
 constexpr int QK_FWD_CTAS = 2;
 template <typename T, int L>
