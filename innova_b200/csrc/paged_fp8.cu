@@ -61,6 +61,17 @@ __device__ __forceinline__ int pool_page(const Fp8Tokens& t, int pages, int row,
   return -1;
 }
 
+// The new tokens of a sequence, rows [t0, t0 + count) at positions [start, start + count). None where what the caller wrote cannot be: rows outside the
+// tensor, positions behind the page table.
+struct Fp8Span {
+  int t0, count, start;
+  bool fine;
+  __device__ __forceinline__ Fp8Span(const Fp8Tokens& t, int cu0, int cu1, int start) : t0(cu0), count(cu1 - cu0), start(start) {
+    fine = t0 >= 0 && count >= 0 && count <= t.T - t0 && start >= 0 && (long)start + count <= (long)t.max_pages * FP8_PAGE;
+  }
+  __device__ __forceinline__ Fp8Span(const Fp8Tokens& t, int seq) : Fp8Span(t, t.cu[seq], t.cu[seq + 1], t.start[seq]) {}
+};
+
 // ---------------------------------------------------------------------------------------------- append
 struct Fp8Append {
   const __nv_bfloat16 *q_in, *k_in, *v_in, *wq, *wk;   // rows ld_in apart, H, Hkv and Hkv heads side by side; weights null: no norm
@@ -109,8 +120,9 @@ __global__ void __launch_bounds__(128, FP8_APPEND_CTAS) fp8_append_kernel(const 
   }
   __syncthreads();
   if (found[0] < 0) return;
-  const int t0 = found[1], count = found[2] - t0, start = found[3], row = found[4];
-  if (t0 < 0 || count < 0 || count > tk.T - t0 || start < 0) {
+  const Fp8Span span(tk, found[1], found[2], found[3]);
+  const int t0 = span.t0, count = span.count, start = span.start, row = found[4];
+  if (!span.fine) {
     if (threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
     return;
   }
@@ -363,17 +375,18 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
     fine = (unsigned)row < (unsigned)tk.table_rows;
     if (fine) {
       len = a.seq_lens[row];
+      fine = len <= tk.max_pages * (long)FP8_PAGE;
+      if (!fine) len = 0;
       tail = a.tail_start ? a.tail_start[seq] : len;
       bits = a.tail_mask ? a.tail_mask[seq] : 0;
     }
   } else {
-    t0 = tk.cu[seq];
-    const int count = tk.cu[seq + 1] - t0;
-    start = tk.start[seq];
+    const Fp8Span span(tk, seq);
+    t0 = span.t0;
+    start = span.start;
     row = tk.rows[seq];
-    rows = count * a.G;
-    fine = t0 >= 0 && count >= 0 && count <= tk.T - t0 && start >= 0;
-    if (!fine) rows = 0;
+    fine = span.fine;
+    rows = fine ? span.count * a.G : 0;
     if (rows > ROWS * a.tiles) fine = false;         // more new tokens than the caller said
   }
   if (!fine && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
@@ -551,7 +564,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
             for (int e = 0; e < 4; ++e) {
               const int at = pos + g * FP8_PAGE + M::slot(e >> 1, n);
               bool seen = at >= vlo[b][e & 1] && at < vhi[b][e & 1] && ((there >> g) & 1);
-              if (TREE) seen = seen && (at < tail || (at - tail < 64 && ((bits >> ((at - tail) & 63)) & 1ull)));
+              if (TREE) seen = seen && (at < tail || ((unsigned)(at - tail) < 64u && ((bits >> ((at - tail) & 63)) & 1ull)));
               if (!seen) {
                 s[b][g][e] = -INFINITY;
                 hidden |= 1u << (b * 8 + g * 4 + e);
@@ -813,10 +826,9 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
   const int seq = div_by(y, pool.Hkv, a.inv_hkv), hk = y - seq * pool.Hkv;
   wait_previous();
   release_next();
-  const int t0 = tk.cu[seq], count = tk.cu[seq + 1] - t0, start = tk.start[seq], row = tk.rows[seq];
-  const bool fine = t0 >= 0 && count >= 0 && count <= tk.T - t0 && start >= 0;
-  const int rows = fine ? count * a.G : 0;
-  if ((!fine || rows > FT_ROWS * a.tiles) && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
+  const Fp8Span span(tk, seq);
+  const int t0 = span.t0, start = span.start, row = tk.rows[seq], rows = span.fine ? span.count * a.G : 0;
+  if ((!span.fine || rows > FT_ROWS * a.tiles) && threadIdx.x == 0) atomicCAS(tk.status, 0, ERR_BAD_ARG);
   const int r0 = tile * FT_ROWS, nr = min(FT_ROWS, rows - r0);
   if (nr <= 0) return;
   const int first = start + div_by(r0, a.G, a.inv_g), last = start + div_by(r0 + nr - 1, a.G, a.inv_g);
@@ -1178,21 +1190,38 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
   }
 }
 
-// Joins the splits of a row (a query token's head), D / 32 values a lane. WIDE: a CTA a row, whose warps share the splits; else a warp a row. With 63
-// splits of 32 rows a warp a row took most of 24 us.
+// The sequence of a row, by a warp: the last one that starts at or before it.
+__device__ __forceinline__ int sequence_of(const Fp8Tokens& tk, int t, int lane) {
+  int lo = 0;
+  for (int len = tk.n; len > 1;) {
+    const int step = (len + 31) / 32;
+    const uint32_t below = __ballot_sync(0xffffffffu, lane * step < len && tk.cu[lo + lane * step] <= t);
+    const int k = below ? 31 - __clz(below) : 0;
+    lo += k * step;
+    len = min(step, len - k * step);
+  }
+  return lo;
+}
+
+// Joins the splits of a row (a query token's head), D / 32 values a lane; rows that belong to no sequence stay as they are. WIDE: a CTA a row, whose warps
+// share the splits; else a warp a row. With 63 splits of 32 rows a warp a row took most of 24 us.
 template <int D, bool WIDE>
-__global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__ part, const float* __restrict__ part_ml, const int* __restrict__ used,
-                                                       __nv_bfloat16* __restrict__ out, long ld_o, int T, int H, int splits) {
+__global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Tokens tk, int tile_rows) {
   constexpr int E = D / 32, NW = WIDE ? 8 : 1;
   __shared__ float sm_l[8], sm_o[8][D];
   wait_previous();
   release_next();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, splits = a.splits;
   const long item = WIDE ? blockIdx.x : blockIdx.x * 8l + warp;
-  if (item >= (long)T * H) return;
-  const float* base = part + item * splits * D + lane * E;
-  const float* ml = part_ml + item * splits * 2;
-  const int ns = used[item];
+  if (item >= (long)tk.T * a.H) return;
+  const int t = (int)(item / a.H), head = (int)(item - (long)t * a.H);
+  if (!a.row_seq) {                                  // what the other kernel left out, of this row too
+    const Fp8Span span(tk, sequence_of(tk, t, lane));
+    if (!span.fine || t < span.t0 || t - span.t0 >= span.count || (long)(t - span.t0) * a.G + head % a.G >= (long)tile_rows * a.tiles) return;
+  }
+  const float* base = a.part + item * splits * D + lane * E;
+  const float* ml = a.part_ml + item * splits * 2;
+  const int ns = min(max(a.used[item], 0), splits);  // where a wait ran out there may be anything
   float mm = -INFINITY;
   for (int s = lane; s < ns; s += 32) mm = fmaxf(mm, ml[2 * s]);
 #pragma unroll
@@ -1224,7 +1253,7 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const float* __restrict__
     }
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  uint32_t* to = reinterpret_cast<uint32_t*>(out + item / H * ld_o + item % H * D + lane * E);
+  uint32_t* to = reinterpret_cast<uint32_t*>(a.out + t * a.ld_o + head * D + lane * E);
 #pragma unroll
   for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv, acc[i + 1] * inv);
 }
@@ -1323,12 +1352,10 @@ extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int m
   return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
 }
 template <int D>
-static int fp8_attend_join(const Fp8Attend& a, int T, cudaStream_t st) {
-  const long items = (long)T * a.H;
-  if (a.splits > 4)
-    launch_early(fp8_join_kernel<D, true>, dim3((unsigned)items), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, T, a.H, a.splits);
-  else if (a.splits > 1)
-    launch_early(fp8_join_kernel<D, false>, dim3((unsigned)((items + 7) / 8)), 256, 0, st, a.part, a.part_ml, a.used, a.out, a.ld_o, T, a.H, a.splits);
+static int fp8_attend_join(const Fp8Attend& a, const Fp8Tokens& tk, int tile_rows, cudaStream_t st) {
+  const long items = (long)tk.T * a.H;
+  if (a.splits > 4) launch_early(fp8_join_kernel<D, true>, dim3((unsigned)items), 256, 0, st, a, tk, tile_rows);
+  else if (a.splits > 1) launch_early(fp8_join_kernel<D, false>, dim3((unsigned)((items + 7) / 8)), 256, 0, st, a, tk, tile_rows);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
@@ -1338,14 +1365,14 @@ static int fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8T
   static std::atomic<uint64_t> ready{0};
   raise_smem(fp8_attend_kernel<D, NR, NW, TREE>, SMEM, ready);
   launch_early(fp8_attend_kernel<D, NR, NW, TREE>, dim3(ctas), NW * 32, SMEM, st, a, pool, tk);
-  return fp8_attend_join<D>(a, tk.T, st);
+  return fp8_attend_join<D>(a, tk, 8 * NR, st);
 }
 template <int D>
 static int fp8_attend_tile_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
   static std::atomic<uint64_t> ready{0};
   raise_smem(fp8_attend_tile_kernel<D>, FtSmem<D>::TOTAL, ready);
   launch_early(fp8_attend_tile_kernel<D>, dim3(ctas), FT_THREADS, FtSmem<D>::TOTAL, st, a, pool, tk);
-  return fp8_attend_join<D>(a, tk.T, st);
+  return fp8_attend_join<D>(a, tk, FT_ROWS, st);
 }
 
 static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, float* work, cudaStream_t st) {

@@ -148,6 +148,20 @@ def test_attend_strides(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 1e-30])
+def test_attend_scales(scale, dev):
+    """Scores turned round, and none: the mean of the values seen. One token and many, in one part and in several."""
+    for ctx, new in (([37], [1]), ([2500], [2]), ([70], [90])):
+        s = Setup(ctx, new, 4, 2, 64, dev)
+        q = s.q()
+        got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 4, scale).cpu()
+        k, v = s.values(0, ctx[0] + new[0])
+        for t in range(0, new[0], 11):
+            o, size = attention(q[t].cpu().double().view(4, 64), k, v, torch.arange(len(k)) <= ctx[0] + t, scale)
+            close_attention(got[t].view(4, 64), o, size, q.dtype)
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_attend_values_that_are_no_numbers(dev):
     """A page of NaN poisons the rows that see it, and no others; so does a query of its row."""
     s = Setup([100, 40], [30, 2], 4, 2, 64, dev)
@@ -465,6 +479,51 @@ def test_entries_outside_the_pool(dev):
             codes = x.element_size() == 1
             x, y = (z.cpu().view(torch.uint8 if codes else torch.int32) for z in (x, y))
             assert torch.equal(x[~own], y[~own]) and not (codes and torch.equal(x[own], y[own]))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("ctx, new", [([5, 40], [1, 3]), ([2000, 3], [1, 1]), ([9000], [1]), ([3000, 0], [20, 0]), ([5000, 100], [70, 9]), ([0, 0], [0, 0])])
+def test_rows_of_no_sequence_stay_as_they_are(ctx, new, dev):
+    """A padded batch: rows in front of the first sequence and behind the last, of calls in one part and in several."""
+    s = Setup(ctx, new, 8, 2, 64, dev)
+    q = torch.randn(s.T + 5, 8 * 64, device=dev).to(dtype_of(dev))
+    out = torch.full_like(q, 7.0)
+    padded = s.tokens._replace(cu=s.tokens.cu + 2)
+    pf.kv_attend(q, s.pool, s.page_table, padded, 8, out=out)
+    assert bool((out[:2] == 7).all()) and bool((out[2 + s.T:] == 7).all())
+    want = pf.kv_attend(q[2:2 + s.T], s.pool, s.page_table, s.tokens, 8)
+    assert torch.equal(out[2:2 + s.T], want)
+    if dev == "cuda":
+        rt.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[1, 1], [30, 30]])
+def test_gpu_positions_behind_the_page_table(new):
+    """Nothing is looked for behind the table, however far: the sequence is left out and reported, the other one is served."""
+    s = Setup([5000, 333], new, 8, 2, 64, "cuda")
+    q = s.q()
+    for far in (s.page_table.shape[1] * 16 - new[0] + 1, 2 ** 31 - 3):
+        want = pf.kv_attend(q, s.pool, s.page_table, s.tokens, 8)                     # the append below is another one's keys
+        out = torch.full_like(q, 7.0)
+        pf.kv_attend(q, s.pool, s.page_table, s.tokens._replace(start=i32([far, 333], "cuda")), 8, out=out)
+        with pytest.raises(RuntimeError):
+            rt.check_status()
+        assert bool((out[:new[0]] == 7).all()) and torch.equal(out[new[0]:], want[new[0]:])
+        before = [x.clone() for x in s.pool]
+        pf.kv_append(q[:, :128], q[:, 128:256], s.pool, s.page_table, s.tokens._replace(start=i32([far, 333], "cuda")))
+        with pytest.raises(RuntimeError):
+            rt.check_status()
+        own = torch.zeros(s.pages, dtype=torch.bool, device="cuda")
+        own[s.ids[1]] = True
+        for x, y in zip(s.pool, before):
+            x, y = (z.view(torch.uint8 if z.element_size() == 1 else torch.int32) for z in (x, y))
+            assert torch.equal(x[~own], y[~own])
+    lens = i32([2 ** 31 - 1] * s.page_table.shape[0], "cuda")
+    got = pf.tree_attend(q[:2], s.pool, s.page_table, lens, i32([s.owner[0]] * 2, "cuda"), 8, 6000)
+    with pytest.raises(RuntimeError):
+        rt.check_status()
+    assert not bool(got.any())
 
 
 @pytest.mark.gpu
