@@ -812,9 +812,9 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem, *sK = smem + 2 * L::QUERIES, *sV = sK + NS * L::KEYS;
   // s_full and p_full: [tile][even or odd block]
-  __shared__ __align__(8) uint64_t q_full[2], k_full[NS], k_empty[NS], v_full[NS], v_empty[NS], s_full[2][2], p_full[2][2], o_full[2];
-  // Of a block's pages: the keys' scale, log2 of the values'; bit p of `present`: page p is there. Block j + 8 takes block j's place once the scores of
-  // block j + 4 are computed, which both tiles ask for behind their softmax of block j + 2.
+  __shared__ __align__(8) uint64_t q_full[2], full[NS], empty[NS], s_full[2][2], p_full[2][2], o_full[2];
+  // Of a block's pages: the keys' scale, log2 of the values'; bit p of `present`: page p is there. Block j + 8 takes block j's place once the products of
+  // block j + 4 are complete.
   __shared__ float2 scales[8][FT_PAGES];
   __shared__ uint32_t present[8];
   __shared__ uint32_t tmem_slot;
@@ -852,10 +852,8 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
     }
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      mbar_init(&k_full[i], 4);
-      mbar_init(&k_empty[i], tiles);
-      mbar_init(&v_full[i], 4);
-      mbar_init(&v_empty[i], tiles);
+      mbar_init(&full[i], 4);
+      mbar_init(&empty[i], tiles);
     }
     abort_word = 0;
     fence_barrier_init();
@@ -888,16 +886,14 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           mma_of_warp(t_s + (j & 1) * FT_N, desc_q + (((s / 4) * (FT_M * 128) + (s % 4) * 32) >> 4), dk + (((s / 4) * (FT_N * 128) + (s % 4) * 32) >> 4),
                       idesc_qk, s > 0);
         commit_of_warp(&s_full[t][j & 1]);
-        commit_of_warp(&k_empty[slot]);
         if (lane == 0) mbar_arrive(&s_full[t][j & 1]);         // with it goes on what came with the keys: the block's scales
         __syncwarp();
         return true;
       };
-      auto keys = [&](int j) { return mbar_wait_warp(&k_full[j % NS], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL); };
+      auto loaded = [&](int j) { return mbar_wait_warp(&full[j % NS], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL); };
       auto values = [&](int j) -> bool {
         const int slot = j % NS;
-        if (!mbar_wait_warp(&v_full[slot], (j / NS) & 1, abort_flag, tk.status, ERR_WAIT_FULL)) return false;
-        if (j + 2 < nb && !keys(j + 2)) return false;                            // while the weights are not there yet
+        if (j + 2 < nb && !loaded(j + 2)) return false;                          // while the weights are not there yet
         if (!mbar_wait_warp(&p_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_MISC)) return false;
         tc_fence_after();
         const uint64_t dv = desc_v + (uint64_t)(slot * L::KEYS >> 4);
@@ -905,10 +901,10 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
         for (int s = 0; s < FT_N / 16; ++s)          // 16 keys: eight packed columns of weights
           mma_of_warp_tmem(t_o, t_s + (j & 1) * FT_N + s * 8, dv + (s * 2048 >> 4), idesc_pv, (j > 0 || s > 0) ? 1u : 0u);
         commit_of_warp(&o_full[t]);
-        commit_of_warp(&v_empty[slot]);
+        commit_of_warp(&empty[slot]);
         return true;
       };
-      bool ok = mbar_wait_warp(&q_full[t], 0, abort_flag, tk.status, ERR_WAIT_FULL) && keys(0) && scores(0) && (nb == 1 || (keys(1) && scores(1)));
+      bool ok = mbar_wait_warp(&q_full[t], 0, abort_flag, tk.status, ERR_WAIT_FULL) && loaded(0) && scores(0) && (nb == 1 || (loaded(1) && scores(1)));
       for (int j = 0; ok && j < nb; ++j) ok = values(j) && (j + 2 >= nb || scores(j + 2));
     }
   } else if (warp >= 8) {
@@ -930,53 +926,44 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       return -1;
     };
     auto scale_at = [&](const float* of, int id) { return of[(long)max(id, 0) * pool.Hkv + hk]; };
-    auto load = [&](uint4 (&raw)[PER], const uint8_t* codes, int ids) {
+    // A thread's place in a page is always the same; `at`: what it reads of page 0, key head 0.
+    const uint8_t *k_at = pool.k + (tok0 % FP8_PAGE) * D + piece * 16, *v_at = pool.v + (tok0 % FP8_PAGE) * D + piece * 16;
+    auto load = [&](uint4 (&k)[PER], uint4 (&v)[PER], int id) {
+      const int head = max(id, 0) * pool.Hkv + hk;                               // under 2^31: there are as many scales
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const int tok = tok0 + i * STEP, pid = max(__shfl_sync(0xffffffffu, ids, tok / FP8_PAGE), 0);
-        raw[i] = *reinterpret_cast<const uint4*>(codes + (((long)pid * pool.Hkv + hk) * FP8_PAGE + tok % FP8_PAGE) * D + piece * 16);
+        const size_t off = (size_t)(unsigned)__shfl_sync(0xffffffffu, head, (tok0 + i * STEP) / FP8_PAGE) * (FP8_PAGE * D);
+        k[i] = *reinterpret_cast<const uint4*>(k_at + off);
+        v[i] = *reinterpret_cast<const uint4*>(v_at + off);
       }
     };
-    auto store = [&](const uint4 (&raw)[PER], uint8_t* dst, uint64_t* bar) {
-      const int at = 2 * piece;                                                  // 16-byte pieces `at` and `at` + 1 of a token's fp16 row
-      const bool odd = piece >= CH / 2;                                          // lanes of the second half store in the other order: no bank twice
-      uint8_t* to = dst + (at >> 3) * (FT_N * 128) + tok0 * 128;
-      const int x0 = (((at & 7) + (odd ? 1 : 0)) ^ (tok0 & 7)) << 4, x1 = (((at & 7) + (odd ? 0 : 1)) ^ (tok0 & 7)) << 4;
+    const int at = 2 * piece;                                                    // 16-byte pieces `at` and `at` + 1 of a token's fp16 row
+    const bool odd = piece >= CH / 2;                                            // lanes of the second half store in the other order: no bank twice
+    const int to = (at >> 3) * (FT_N * 128) + tok0 * 128;
+    const int x0 = (((at & 7) + (odd ? 1 : 0)) ^ (tok0 & 7)) << 4, x1 = (((at & 7) + (odd ? 0 : 1)) ^ (tok0 & 7)) << 4;
+    auto store = [&](const uint4 (&raw)[PER], uint8_t* dst) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const uint4 r = raw[i];
-        const uint4 h0 = make_uint4(half2_of_e4m3x2(r.x), half2_of_e4m3x2(r.x >> 16), half2_of_e4m3x2(r.y), half2_of_e4m3x2(r.y >> 16));
-        const uint4 h1 = make_uint4(half2_of_e4m3x2(r.z), half2_of_e4m3x2(r.z >> 16), half2_of_e4m3x2(r.w), half2_of_e4m3x2(r.w >> 16));
-        *reinterpret_cast<uint4*>(to + i * STEP * 128 + x0) = odd ? h1 : h0;     // STEP is a multiple of eight: the swizzle stays
-        *reinterpret_cast<uint4*>(to + i * STEP * 128 + x1) = odd ? h0 : h1;
+        const uint32_t a0 = odd ? r.z : r.x, a1 = odd ? r.w : r.y, b0 = odd ? r.x : r.z, b1 = odd ? r.y : r.w;
+        uint8_t* row = dst + to + i * STEP * 128;                                // STEP is a multiple of eight: the swizzle stays
+        *reinterpret_cast<uint4*>(row + x0) = make_uint4(half2_of_e4m3x2(a0), half2_of_e4m3x2(a0 >> 16), half2_of_e4m3x2(a1), half2_of_e4m3x2(a1 >> 16));
+        *reinterpret_cast<uint4*>(row + x1) = make_uint4(half2_of_e4m3x2(b0), half2_of_e4m3x2(b0 >> 16), half2_of_e4m3x2(b1), half2_of_e4m3x2(b1 >> 16));
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
     };
-    static_assert(STEP % 8 == 0, "a thread's tokens share a swizzle");
+    static_assert(STEP % FP8_PAGE == 0, "a thread's tokens share their place in a page, and a swizzle");
     int id[2] = {check_id(read_id(0), 0), check_id(read_id(1), 1)}, read = read_id(2);
     float ks[2] = {scale_at(pool.k_scale, id[0]), scale_at(pool.k_scale, id[1])}, vs[2] = {scale_at(pool.v_scale, id[0]), scale_at(pool.v_scale, id[1])};
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      load(rk[e], pool.k, id[e]);
-      load(rv[e], pool.v, id[e]);
-    }
+    for (int e = 0; e < 2; ++e) load(rk[e], rv[e], id[e]);
     auto block = [&](int j, int e) -> bool {
-      const int slot = j % NS, turn = ((j / NS) & 1) ^ 1;
+      const int slot = j % NS;
       const uint32_t there = __ballot_sync(0xffffffffu, id[e] >= 0);
-      if (!mbar_wait_warp(&k_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) return false;
+      if (!mbar_wait_warp(&empty[slot], ((j / NS) & 1) ^ 1, abort_flag, tk.status, ERR_WAIT_EMPTY)) return false;
       if (warp == 8) {
         if (lane < FT_PAGES) scales[j & 7][lane] = id[e] >= 0 ? make_float2(ks[e], log2_scale(vs[e])) : make_float2(0.f, -127.f);
         if (lane == 0) present[j & 7] = there;
       }
-      store(rk[e], sK + slot * L::KEYS, &k_full[slot]);
-      id[e] = check_id(read, j + 2);
-      read = read_id(j + 3);
-      load(rk[e], pool.k, id[e]);
-      ks[e] = scale_at(pool.k_scale, id[e]);
-      vs[e] = scale_at(pool.v_scale, id[e]);
-      if (!mbar_wait_warp(&v_empty[slot], turn, abort_flag, tk.status, ERR_WAIT_EMPTY)) return false;
       if ((b0 + j + 1) * FT_N > hi || there != (1u << FT_PAGES) - 1) {           // values that are not there are nothing, whatever was read
         rarely();
 #pragma unroll
@@ -985,8 +972,16 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           if ((b0 + j) * FT_N + tok >= hi || !((there >> (tok / FP8_PAGE)) & 1)) rv[e][i] = make_uint4(0, 0, 0, 0);
         }
       }
-      store(rv[e], sV + slot * L::KEYS, &v_full[slot]);
-      load(rv[e], pool.v, id[e]);
+      store(rk[e], sK + slot * L::KEYS);
+      store(rv[e], sV + slot * L::KEYS);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[slot]);
+      id[e] = check_id(read, j + 2);
+      read = read_id(j + 3);
+      load(rk[e], rv[e], id[e]);
+      ks[e] = scale_at(pool.k_scale, id[e]);
+      vs[e] = scale_at(pool.v_scale, id[e]);
       return true;
     };
     for (int j = 0; j < nb; j += 2)
