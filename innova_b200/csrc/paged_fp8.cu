@@ -795,9 +795,10 @@ struct FtSmem {
 //   warps 12-13  issue a tile's S = Q K^T and O += P V (P from tensor memory)
 // A tile has two places for scores: the next block's are computed under this one's softmax, so that a row's chain does not wait for products (with one, and
 // blocks of 128 keys, a tile's softmax and products took turns: 548 us in two parts against 514).
-// 2 x 1500 tokens on 5500, 32 heads of 128 on 8: 411 us, 748 TFLOP/s. A block takes both tiles some 2400 cycles, of which the tensor cores are busy with
+// 2 x 1500 tokens on 5500, 32 heads of 128 on 8: 363 us, 847 TFLOP/s. A block takes both tiles some 2100 cycles, of which the tensor cores are busy with
 // 1260 (the queries are read from shared memory again for 64 keys each) and the exponentials' unit 1024: what bounds it is a row's chain of reading scores,
-// maximum, exponentials and writing weights. Four warps for each half of a block's keys shorten the chain, but the exponentials of all then fall together: 443.
+// maximum, exponentials and writing weights. Two threads a row, half of a block's keys each, shorten the chain but leave the conversion half the registers:
+// 412. With barriers for keys and values apart the conversion was what every block waited for: 418.
 // Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are powers of two added to it (relative to the
 // largest one so far, which O is kept in) and taken out of the row sum again a page at a time, so neither costs anything a score. For the rest the sums are
 // those of the small kernel. Tensor memory, a tile 256 columns: scores (then weights) at 0 and 64, O at 128.
@@ -1291,16 +1292,21 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
-// Rows of a sequence and key head up to which the kernel of 16-row tiles takes them, each tile reading the pages again, and not the one of 256. Of 32 heads
-// on 8, the small kernel and the large one: 16 sequences of 4000 with 8 / 12 / 16 new tokens each 58, 83, 108 and 85 us; 64 of 1000 66, 95, 116 and 102;
-// one of 4000 13.6, 14.2, 15.3 and 15.4, 16.0, 16.4.
-constexpr int FP8_FEW_ROWS = 48;
+// Whether the kernel of 16-row tiles takes the rows of a sequence and key head, each tile reading the pages again, and not the one of 256: up to 32 rows of
+// heads of 128 and 64 of 64, whose pages are half as large, and twice that while no SM has more than 64 pages to read. Small kernel and large one: 32 heads of
+// 128 on 8, 16 sequences of 4000 with 8 / 12 / 16 new tokens each 59.7, 84.3, 109.7 and 69.8, 70.3, 70.5 us, 64 of 1000 66.5, 95.6, 116.2 and 86.7, 87.7, 88.2,
+// four of 1000 13.3, 13.2, 13.5 and 16.4, 17.9, 18.3; 8 heads of 64 on 8, 16 of 4000 with 48 61.0 and 82.4.
+static bool fp8_few_rows(long rows, int D, long units, int pages) {
+  const int few = 4096 / D;
+  return rows <= few || (rows <= 2 * few && (rows + 15) / 16 * units * pages <= 148 * 64);
+}
 // How an attention is cut: rows of a tile (8 `blocks`), warps and pages of a CTA, CTAs along a sequence.
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
-  Fp8Cut(int n, int Hkv, int G, int max_new, int max_len, int window, bool tree) {
+  Fp8Cut(int n, int Hkv, int G, int D, int max_new, int max_len, int window, bool tree) {
     const long rows = (long)max_new * G;
-    blocks = rows <= 8 ? 1 : rows <= FP8_FEW_ROWS || tree ? 2 : FT_ROWS / 8;
+    const long reach = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
+    blocks = rows <= 8 ? 1 : tree || fp8_few_rows(rows, D, (long)n * Hkv, (int)(reach / FP8_PAGE) + 1) ? 2 : FT_ROWS / 8;
     tiles = (int)((rows + 8 * blocks - 1) / (8 * blocks));
     const int tokens = max_new < 8 * blocks / G + 2 ? max_new : 8 * blocks / G + 2;       // of a tile
     const long span = window > 0 && (long)window + tokens < max_len ? (long)window + tokens : max_len;
@@ -1309,17 +1315,18 @@ struct Fp8Cut {
     // Joining the splits costs about three microseconds, and a CTA as much before its first and behind its last page, so up to 64 pages stay together (64 x
     // 640 tokens, 512 units: 22.3 us, in two parts 25.9; 16 x 4 on 1000: 14.4 and 17.1). Longer ones are cut for two CTAs an SM, in parts of 16 pages or more
     // (2000 tokens, 16 units: 16 / 32 / 64 / 126 pages 7.5, 9.6, 12.1, 15.3 us; 32000, 8 units: 24 / 64 / 128 pages 23.5, 17.8, 19.9) and of 128 at most,
-    // which evens unequal lengths out (8 of up to 65000: 128 / 192 / 512 pages 71.5, 84.6, 91.2 us; of 64999 each 165, 171, 209; 64 of 8000 164, 167). Where units alone fill the GPU several times, CTAs of
-    // two warps, which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251 90.1 and 106.6).
+    // which evens unequal lengths out (8 of up to 65000: 128 / 192 / 512 pages 71.5, 84.6, 91.2 us; of 64999 each 165, 171, 209; 64 of 8000 164, 167). Where
+    // units alone fill the GPU several times, CTAs of two warps, which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251
+    // 90.1 and 106.6).
     const bool many = blocks == 1 && units > 444 && pages <= 256;
     warps = many ? 2 : 4;
     const long total = units * pages;
     long want = (total + 295) / 296;
     if (want > 128) want = 128;
     if (blocks == FT_ROWS / 8) {                                      // whole blocks of keys
-      // One CTA an SM. A page takes a CTA about 0.3 us, all else as much as 24 pages; a join costs 10 of them and the partial results their bytes. Cut where
-      // that comes out ahead (4 x 128 on 20000, 64 units: in 5 314 us, whole 424; 16 x 32 on 4000, 128 units: in 2 103, whole 87; 64 on 8000, 8 units: in 16
-      // 31, in 4 55).
+      // One CTA an SM. A page takes a CTA about 0.25 us, all else as much as 24 pages; a join costs 10 of them and the partial results their bytes. Cut where
+      // that comes out ahead (4 x 128 on 20000, 64 units: in 2 226 us, in 5 314, whole 424; 16 x 32 on 4000, 128 units: in 2 103, whole 87; 64 on 8000, 8
+      // units: in 16 31, in 4 55).
       const int most = pages / (2 * FT_PAGES) < 64 ? pages / (2 * FT_PAGES) : 64;
       const double bytes = (double)n * max_new * Hkv * G * 8 * 130 / 1.2e6;
       double best = 0;
@@ -1342,8 +1349,8 @@ struct Fp8Cut {
 };
 // Floats of workspace that an attention wants (0: none). A call's own: it holds partial results from one launch to the next.
 extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int max_new, int max_len, int window, int tree) {
-  if (n < 1 || T < 1 || Hkv < 1 || H < Hkv || max_new < 1 || max_len < 1) return 0;
-  const Fp8Cut cut(n, Hkv, H / Hkv, max_new, max_len, window, tree);
+  if (n < 1 || T < 1 || Hkv < 1 || H < Hkv || D < 1 || max_new < 1 || max_len < 1) return 0;
+  const Fp8Cut cut(n, Hkv, H / Hkv, D, max_new, max_len, window, tree);
   return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
 }
 template <int D>
@@ -1372,7 +1379,7 @@ static int fp8_attend_tile_launch(const Fp8Attend& a, const Fp8Pool& pool, const
 
 static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, float* work, cudaStream_t st) {
   a.G = a.H / pool.Hkv;
-  const Fp8Cut cut(tk.n, pool.Hkv, a.G, max_new, max_len, a.window, a.row_seq != nullptr);
+  const Fp8Cut cut(tk.n, pool.Hkv, a.G, D, max_new, max_len, a.window, a.row_seq != nullptr);
   a.tiles = cut.tiles;
   a.per_split = cut.per;
   a.splits = cut.splits;
