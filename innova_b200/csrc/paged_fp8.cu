@@ -442,265 +442,265 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   int nc = nf;
   float ksc = scale_at(pool.k_scale, nc), vsc = scale_at(pool.v_scale, nc), ksn = 0.f, vsn = 0.f;
 
-    // ---- queries: row n of a block of eight, as the second operand ----
-    uint32_t qb[NR][KS][2];
-    float qm[NR][2];                                                            // of this lane's columns: rows 2 c and 2 c + 1
-    int vlo[NR][2], vhi[NR][2];                                                 // positions that they see: [vlo, vhi)
+  // ---- queries: row n of a block of eight, as the second operand ----
+  uint32_t qb[NR][KS][2];
+  float qm[NR][2];                                                            // of this lane's columns: rows 2 c and 2 c + 1
+  int vlo[NR][2], vhi[NR][2];                                                 // positions that they see: [vlo, vhi)
 #pragma unroll
-    for (int b = 0; b < NR; ++b) {
-      uint4(&raw)[KP][2] = qraw[b];
-      uint32_t top = 0;
+  for (int b = 0; b < NR; ++b) {
+    uint4(&raw)[KP][2] = qraw[b];
+    uint32_t top = 0;
 #pragma unroll
-      for (int j = 0; j < KP; ++j)
+    for (int j = 0; j < KP; ++j)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t w[4] = {raw[j][i].x, raw[j][i].y, raw[j][i].z, raw[j][i].w};
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t w[4] = {raw[j][i].x, raw[j][i].y, raw[j][i].z, raw[j][i].w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
-        }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int ex = min(max((int)(top >> 7), 1), 253);                         // 2^(ex - 127): the row's largest value, but for its fraction
-      const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);
-#pragma unroll
-      for (int j = 0; j < KP; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 v = raw[j][i >> 1];
-          const uint32_t w0 = i & 1 ? v.z : v.x, w1 = i & 1 ? v.w : v.y;
-          qb[b][j * 4 + i][0] = half2_of(__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down);
-          qb[b][j * 4 + i][1] = half2_of(__uint_as_float(w1 << 16) * down, __uint_as_float(w1 & 0xffff0000u) * down);
-        }
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        qm[b][e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4);
-        const int p = start + div_by(min(r0 + b * 8 + 2 * c + e, rows - 1), a.G, a.inv_g);
-        vhi[b][e] = TREE ? len : p + 1;
-        vlo[b][e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
+        for (int k = 0; k < 4; ++k) top = max(top, max(w[k] & 0x7fffu, (w[k] >> 16) & 0x7fffu));
       }
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int ex = min(max((int)(top >> 7), 1), 253);                         // 2^(ex - 127): the row's largest value, but for its fraction
+    const float down = __uint_as_float((uint32_t)(254 - ex) << 23), up = a.scale * 1.4426950408889634f * __uint_as_float((uint32_t)ex << 23);
+#pragma unroll
+    for (int j = 0; j < KP; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 v = raw[j][i >> 1];
+        const uint32_t w0 = i & 1 ? v.z : v.x, w1 = i & 1 ? v.w : v.y;
+        qb[b][j * 4 + i][0] = half2_of(__uint_as_float(w0 << 16) * down, __uint_as_float(w0 & 0xffff0000u) * down);
+        qb[b][j * 4 + i][1] = half2_of(__uint_as_float(w1 << 16) * down, __uint_as_float(w1 & 0xffff0000u) * down);
+      }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      qm[b][e] = __shfl_sync(0xffffffffu, up, (2 * c + e) * 4);
+      const int p = start + div_by(min(r0 + b * 8 + 2 * c + e, rows - 1), a.G, a.inv_g);
+      vhi[b][e] = TREE ? len : p + 1;
+      vlo[b][e] = !TREE && a.window > 0 ? p - a.window + 1 : 0;
     }
-    const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;  // positions that every row sees
+  }
+  const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;  // positions that every row sees
 
-    float o[NR][NI][4], m[NR][2], l[NR][2], vref = 0.f, vinv = 0.f;
+  float o[NR][NI][4], m[NR][2], l[NR][2], vref = 0.f, vinv = 0.f;
 #pragma unroll
-    for (int b = 0; b < NR; ++b) {
+  for (int b = 0; b < NR; ++b) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
-      m[b][0] = m[b][1] = -INFINITY;
-      l[b][0] = l[b][1] = 0.f;
+      for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
+    m[b][0] = m[b][1] = -INFINITY;
+    l[b][0] = l[b][1] = 0.f;
+  }
+
+  for (int st = 0; st < steps; ++st) {
+    if ((st & 15) == 0) {
+      if (st > 0) {
+        nc = nf;
+        ksc = ksn;
+        vsc = vsn;
+      }
+      nn = number_of(st + 16);
     }
-
-    for (int st = 0; st < steps; ++st) {
-      if ((st & 15) == 0) {
-        if (st > 0) {
-          nc = nf;
-          ksc = ksn;
-          vsc = vsn;
-        }
-        nn = number_of(st + 16);
+    if ((st & 15) == 8) {
+      ksn = scale_at(pool.k_scale, nn);
+      vsn = scale_at(pool.v_scale, nn);
+    }
+    if (((st + ST - 1) & 15) == 0) nf = nn;
+    const int at0 = (2 * st) & 31, there = (__ballot_sync(0xffffffffu, nc >= 0) >> at0) & 3, pos = (p0 + 2 * (warp + NW * st)) * FP8_PAGE;
+    const float ks[2] = {__shfl_sync(0xffffffffu, ksc, at0), __shfl_sync(0xffffffffu, ksc, at0 + 1)};
+    const float vs[2] = {__shfl_sync(0xffffffffu, vsc, at0), __shfl_sync(0xffffffffu, vsc, at0 + 1)};
+    fetch(st + ST - 1);                              // into the slot of step st - 1, which every lane has read
+    copies_wait<ST - 1>();
+    __syncwarp();
+    const uint32_t pages = slots + (st % ST) * SLOT;
+    // ---- scores: 2 x 16 tokens x 8 rows ----
+    float s[NR][2][4];
+#pragma unroll
+    for (int b = 0; b < NR; ++b)
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[b][g][e] = 0.f;
+#pragma unroll
+    for (int q = 0; q < KP; ++q) {
+      uint32_t xs[2][4], ys[2][4];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const uint4 x4 = shared16(pages + g * M::BYTES + M::at(M::slot(0, n) * D + q * 64 + c * 16));
+        const uint4 y4 = shared16(pages + g * M::BYTES + M::at(M::slot(1, n) * D + q * 64 + c * 16));
+        xs[g][0] = x4.x; xs[g][1] = x4.y; xs[g][2] = x4.z; xs[g][3] = x4.w;
+        ys[g][0] = y4.x; ys[g][1] = y4.y; ys[g][2] = y4.z; ys[g][3] = y4.w;
       }
-      if ((st & 15) == 8) {
-        ksn = scale_at(pool.k_scale, nn);
-        vsn = scale_at(pool.v_scale, nn);
-      }
-      if (((st + ST - 1) & 15) == 0) nf = nn;
-      const int at0 = (2 * st) & 31, there = (__ballot_sync(0xffffffffu, nc >= 0) >> at0) & 3, pos = (p0 + 2 * (warp + NW * st)) * FP8_PAGE;
-      const float ks[2] = {__shfl_sync(0xffffffffu, ksc, at0), __shfl_sync(0xffffffffu, ksc, at0 + 1)};
-      const float vs[2] = {__shfl_sync(0xffffffffu, vsc, at0), __shfl_sync(0xffffffffu, vsc, at0 + 1)};
-      fetch(st + ST - 1);                              // into the slot of step st - 1, which every lane has read
-      copies_wait<ST - 1>();
-      __syncwarp();
-      const uint32_t pages = slots + (st % ST) * SLOT;
-      // ---- scores: 2 x 16 tokens x 8 rows ----
-      float s[NR][2][4];
 #pragma unroll
-      for (int b = 0; b < NR; ++b)
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[b][g][e] = 0.f;
-#pragma unroll
-      for (int q = 0; q < KP; ++q) {
-        uint32_t xs[2][4], ys[2][4];
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const uint4 x4 = shared16(pages + g * M::BYTES + M::at(M::slot(0, n) * D + q * 64 + c * 16));
-          const uint4 y4 = shared16(pages + g * M::BYTES + M::at(M::slot(1, n) * D + q * 64 + c * 16));
-          xs[g][0] = x4.x; xs[g][1] = x4.y; xs[g][2] = x4.z; xs[g][3] = x4.w;
-          ys[g][0] = y4.x; ys[g][1] = y4.y; ys[g][2] = y4.z; ys[g][3] = y4.w;
+          const uint32_t k0 = half2_of_e4m3x2(xs[g][k]), k1 = half2_of_e4m3x2(ys[g][k]), k2 = half2_of_e4m3x2(xs[g][k] >> 16),
+                         k3 = half2_of_e4m3x2(ys[g][k] >> 16);
+#pragma unroll
+          for (int b = 0; b < NR; ++b) mma_f16(s[b][g], k0, k1, k2, k3, qb[b][q * 4 + k][0], qb[b][q * 4 + k][1]);
         }
+    }
+    const bool whole = pos >= all_lo && pos + 2 * FP8_PAGE <= all_hi && there == 3;
+    bool over = fmaxf(vs[0], vs[1]) > vref;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+    for (int b = 0; b < NR; ++b)
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const uint32_t k0 = half2_of_e4m3x2(xs[g][k]), k1 = half2_of_e4m3x2(ys[g][k]), k2 = half2_of_e4m3x2(xs[g][k] >> 16),
-                           k3 = half2_of_e4m3x2(ys[g][k] >> 16);
-#pragma unroll
-            for (int b = 0; b < NR; ++b) mma_f16(s[b][g], k0, k1, k2, k3, qb[b][q * 4 + k][0], qb[b][q * 4 + k][1]);
-          }
+      for (int g = 0; g < 2; ++g) {
+        const float f0 = qm[b][0] * ks[g], f1 = qm[b][1] * ks[g];
+        s[b][g][0] *= f0;
+        s[b][g][1] *= f1;
+        s[b][g][2] *= f0;
+        s[b][g][3] *= f1;
       }
-      const bool whole = pos >= all_lo && pos + 2 * FP8_PAGE <= all_hi && there == 3;
-      bool over = fmaxf(vs[0], vs[1]) > vref;
+    uint32_t hidden = 0;
+    if (!whole) {
+      rarely();
 #pragma unroll
       for (int b = 0; b < NR; ++b)
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const float f0 = qm[b][0] * ks[g], f1 = qm[b][1] * ks[g];
-          s[b][g][0] *= f0;
-          s[b][g][1] *= f1;
-          s[b][g][2] *= f0;
-          s[b][g][3] *= f1;
-        }
-      uint32_t hidden = 0;
-      if (!whole) {
-        rarely();
-#pragma unroll
-        for (int b = 0; b < NR; ++b)
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int at = pos + g * FP8_PAGE + M::slot(e >> 1, n);
-              bool seen = at >= vlo[b][e & 1] && at < vhi[b][e & 1] && ((there >> g) & 1);
-              if (TREE) seen = seen && (at < tail || ((unsigned)(at - tail) < 64u && ((bits >> ((at - tail) & 63)) & 1ull)));
-              if (!seen) {
-                s[b][g][e] = -INFINITY;
-                hidden |= 1u << (b * 8 + g * 4 + e);
-              }
-            }
-      }
-#pragma unroll
-      for (int b = 0; b < NR; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float top = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
-          over |= top > m[b][e] + SLACK;
-        }
-      if (__any_sync(0xffffffffu, over)) {
-        const float v_up = fmaxf(vs[0], vs[1]), beta = v_up > vref ? vref / v_up : 1.f;
-        if (v_up > vref) {
-          vref = v_up;
-          vinv = 1.f / v_up;
-        }
-#pragma unroll
-        for (int b = 0; b < NR; ++b) {
-          float alpha[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
-#pragma unroll
-            for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            const float up = fmaxf(m[b][e], mx);
-            alpha[e] = up == m[b][e] ? 1.f : exp2_fast(m[b][e] - up);
-            m[b][e] = up;
-            l[b][e] *= alpha[e];
-            alpha[e] *= beta;
-          }
-#pragma unroll
-          for (int k = 0; k < NI; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[e & 1];
-        }
-      }
-      const float rel[2] = {vs[0] * vinv, vs[1] * vinv};
-      float xw[NR][2][4];                              // weights times their page's scale
-#pragma unroll
-      for (int b = 0; b < NR; ++b) {
-        const float m0 = m[b][0] - LIFT, m1 = m[b][1] - LIFT;
 #pragma unroll
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            s[b][g][e] = exp2_fast(s[b][g][e] - (e & 1 ? m1 : m0));
-            xw[b][g][e] = s[b][g][e] * rel[g];
-          }
-      }
-      if (!whole) {                                    // nothing of a hidden place, whatever its scale and however little the row has seen
-        rarely();
-#pragma unroll
-        for (int b = 0; b < NR; ++b)
-#pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if ((hidden >> (b * 8 + g * 4 + e)) & 1) s[b][g][e] = xw[b][g][e] = 0.f;
-      }
-      uint32_t pb[NR][2][2];                           // weights of row n: tokens of rows 2 c, 2 c + 1 (and + 8) of the score product
-#pragma unroll
-      for (int b = 0; b < NR; ++b) {
-        l[b][0] += (s[b][0][0] + s[b][0][2]) + (s[b][1][0] + s[b][1][2]);
-        l[b][1] += (s[b][0][1] + s[b][0][3]) + (s[b][1][1] + s[b][1][3]);
-#pragma unroll
-        for (int g = 0; g < 2; ++g)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) pb[b][g][h] = transpose8(half2_of(xw[b][g][2 * h], xw[b][g][2 * h + 1]));
-      }
-      // ---- values: dimensions x 8 rows ----
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        uint32_t v[4][VW];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int tok = M::slot(r >> 1, 2 * c + (r & 1));
-          const uint32_t src = pages + g * M::BYTES + FP8_PAGE * D + M::at(tok * D + M::col(n));
-          if (D == 128) {
-            const uint4 w = shared16(src);
-            v[r][0] = w.x; v[r][1] = w.y; v[r][VW - 2] = w.z; v[r][VW - 1] = w.w;
-          } else {
-            const uint2 w = shared8(src);
-            v[r][0] = w.x; v[r][1] = w.y;
-          }
-        }
-        if (!whole) {                                   // slots past the end hold whatever was there
-          rarely();
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (pos + g * FP8_PAGE + M::slot(r >> 1, 2 * c + (r & 1)) >= hi || !((there >> g) & 1)) {
-#pragma unroll
-              for (int q = 0; q < VW; ++q) v[r][q] = 0;
+            const int at = pos + g * FP8_PAGE + M::slot(e >> 1, n);
+            bool seen = at >= vlo[b][e & 1] && at < vhi[b][e & 1] && ((there >> g) & 1);
+            if (TREE) seen = seen && (at < tail || ((unsigned)(at - tail) < 64u && ((bits >> ((at - tail) & 63)) & 1ull)));
+            if (!seen) {
+              s[b][g][e] = -INFINITY;
+              hidden |= 1u << (b * 8 + g * 4 + e);
             }
-        }
-#pragma unroll
-        for (int q = 0; q < VW; ++q) {                  // four dimensions of the lane: two products, rows n and n + 8 one dimension each
-          const uint32_t a01 = __byte_perm(v[0][q], v[1][q], 0x5140), b01 = __byte_perm(v[0][q], v[1][q], 0x7362);
-          const uint32_t a23 = __byte_perm(v[2][q], v[3][q], 0x5140), b23 = __byte_perm(v[2][q], v[3][q], 0x7362);
-          const uint32_t va[4] = {half2_of_e4m3x2(a01), half2_of_e4m3x2(a01 >> 16), half2_of_e4m3x2(a23), half2_of_e4m3x2(a23 >> 16)};
-          const uint32_t vb[4] = {half2_of_e4m3x2(b01), half2_of_e4m3x2(b01 >> 16), half2_of_e4m3x2(b23), half2_of_e4m3x2(b23 >> 16)};
-#pragma unroll
-          for (int b = 0; b < NR; ++b) {
-            mma_f16(o[b][2 * q], va[0], va[1], va[2], va[3], pb[b][g][0], pb[b][g][1]);
-            mma_f16(o[b][2 * q + 1], vb[0], vb[1], vb[2], vb[3], pb[b][g][0], pb[b][g][1]);
           }
-        }
-      }
-      __syncwarp();
     }
-
-    // ---- the warps' shares, each in its own part of the ring ----
-    constexpr int SHARE = ST * SLOT / 4;               // floats of a warp's part; ROWS x D are used
-    static_assert(ROWS * D <= SHARE, "sums fit the ring");
-    float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        const float top = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
+        over |= top > m[b][e] + SLACK;
+      }
+    if (__any_sync(0xffffffffu, over)) {
+      const float v_up = fmaxf(vs[0], vs[1]), beta = v_up > vref ? vref / v_up : 1.f;
+      if (v_up > vref) {
+        vref = v_up;
+        vinv = 1.f / v_up;
+      }
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
-        const int r = b * 8 + 2 * c + e;
-        if (n == 0) {
-          sm_m[warp][r] = m[b][e];
-          sm_l[warp][r] = l[b][e];
+      for (int b = 0; b < NR; ++b) {
+        float alpha[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mx = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+          const float up = fmaxf(m[b][e], mx);
+          alpha[e] = up == m[b][e] ? 1.f : exp2_fast(m[b][e] - up);
+          m[b][e] = up;
+          l[b][e] *= alpha[e];
+          alpha[e] *= beta;
         }
-        if (r < nr) {
-          float* to = sums + warp * SHARE + r * D + M::col(n);
 #pragma unroll
-          for (int k = 0; k < NI; k += 2)
-            *reinterpret_cast<float4*>(to + 2 * k) =
-                make_float4(o[b][k][e] * vref, o[b][k][2 + e] * vref, o[b][k + 1][e] * vref, o[b][k + 1][2 + e] * vref);
+        for (int k = 0; k < NI; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[e & 1];
+      }
+    }
+    const float rel[2] = {vs[0] * vinv, vs[1] * vinv};
+    float xw[NR][2][4];                              // weights times their page's scale
+#pragma unroll
+    for (int b = 0; b < NR; ++b) {
+      const float m0 = m[b][0] - LIFT, m1 = m[b][1] - LIFT;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[b][g][e] = exp2_fast(s[b][g][e] - (e & 1 ? m1 : m0));
+          xw[b][g][e] = s[b][g][e] * rel[g];
+        }
+    }
+    if (!whole) {                                    // nothing of a hidden place, whatever its scale and however little the row has seen
+      rarely();
+#pragma unroll
+      for (int b = 0; b < NR; ++b)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if ((hidden >> (b * 8 + g * 4 + e)) & 1) s[b][g][e] = xw[b][g][e] = 0.f;
+    }
+    uint32_t pb[NR][2][2];                           // weights of row n: tokens of rows 2 c, 2 c + 1 (and + 8) of the score product
+#pragma unroll
+    for (int b = 0; b < NR; ++b) {
+      l[b][0] += (s[b][0][0] + s[b][0][2]) + (s[b][1][0] + s[b][1][2]);
+      l[b][1] += (s[b][0][1] + s[b][0][3]) + (s[b][1][1] + s[b][1][3]);
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) pb[b][g][h] = transpose8(half2_of(xw[b][g][2 * h], xw[b][g][2 * h + 1]));
+    }
+    // ---- values: dimensions x 8 rows ----
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t v[4][VW];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tok = M::slot(r >> 1, 2 * c + (r & 1));
+        const uint32_t src = pages + g * M::BYTES + FP8_PAGE * D + M::at(tok * D + M::col(n));
+        if (D == 128) {
+          const uint4 w = shared16(src);
+          v[r][0] = w.x; v[r][1] = w.y; v[r][VW - 2] = w.z; v[r][VW - 1] = w.w;
+        } else {
+          const uint2 w = shared8(src);
+          v[r][0] = w.x; v[r][1] = w.y;
         }
       }
+      if (!whole) {                                   // slots past the end hold whatever was there
+        rarely();
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (pos + g * FP8_PAGE + M::slot(r >> 1, 2 * c + (r & 1)) >= hi || !((there >> g) & 1)) {
+#pragma unroll
+            for (int q = 0; q < VW; ++q) v[r][q] = 0;
+          }
+      }
+#pragma unroll
+      for (int q = 0; q < VW; ++q) {                  // four dimensions of the lane: two products, rows n and n + 8 one dimension each
+        const uint32_t a01 = __byte_perm(v[0][q], v[1][q], 0x5140), b01 = __byte_perm(v[0][q], v[1][q], 0x7362);
+        const uint32_t a23 = __byte_perm(v[2][q], v[3][q], 0x5140), b23 = __byte_perm(v[2][q], v[3][q], 0x7362);
+        const uint32_t va[4] = {half2_of_e4m3x2(a01), half2_of_e4m3x2(a01 >> 16), half2_of_e4m3x2(a23), half2_of_e4m3x2(a23 >> 16)};
+        const uint32_t vb[4] = {half2_of_e4m3x2(b01), half2_of_e4m3x2(b01 >> 16), half2_of_e4m3x2(b23), half2_of_e4m3x2(b23 >> 16)};
+#pragma unroll
+        for (int b = 0; b < NR; ++b) {
+          mma_f16(o[b][2 * q], va[0], va[1], va[2], va[3], pb[b][g][0], pb[b][g][1]);
+          mma_f16(o[b][2 * q + 1], vb[0], vb[1], vb[2], vb[3], pb[b][g][0], pb[b][g][1]);
+        }
+      }
+    }
+    __syncwarp();
+  }
+
+  // ---- the warps' shares, each in its own part of the ring ----
+  constexpr int SHARE = ST * SLOT / 4;               // floats of a warp's part; ROWS x D are used
+  static_assert(ROWS * D <= SHARE, "sums fit the ring");
+  float* sums = reinterpret_cast<float*>(ring);
+#pragma unroll
+  for (int b = 0; b < NR; ++b)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int d = 4; d < 32; d *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
+      const int r = b * 8 + 2 * c + e;
+      if (n == 0) {
+        sm_m[warp][r] = m[b][e];
+        sm_l[warp][r] = l[b][e];
+      }
+      if (r < nr) {
+        float* to = sums + warp * SHARE + r * D + M::col(n);
+#pragma unroll
+        for (int k = 0; k < NI; k += 2)
+          *reinterpret_cast<float4*>(to + 2 * k) =
+              make_float4(o[b][k][e] * vref, o[b][k][2 + e] * vref, o[b][k + 1][e] * vref, o[b][k + 1][2 + e] * vref);
+      }
+    }
   __syncthreads();
   for (int i = threadIdx.x; i < nr * (D / 4); i += NW * 32) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
