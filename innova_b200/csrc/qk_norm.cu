@@ -293,13 +293,7 @@ extern "C" int inv_qk_norm_fwd(const void* x, long ld_x, void* y, long ld_y, con
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
-// CTAs of the backward kernel, and so rows of [D] floats that its caller provides.
-extern "C" int inv_qk_norm_bwd_grid(int T, int H, int Hkv, int D) {
-  if (T <= 0 || D < 16 || D > 256 || H < 0 || Hkv < 0) return 0;
-  return QkBwdCut(T, H, Hkv, D).ctas;
-}
-
-// dx, dy as y and x above. dwq, dwk: [D]; mode 0: bf16, written; 1: fp32, written; 2: fp32, added to.
+// part: 296 rows of [D] floats. dx, dy as y and x above. dwq, dwk: [D]; mode 0: bf16, written; 1: fp32, written; 2: fp32, added to.
 extern "C" int inv_qk_norm_bwd(const void* x, long ld_x, const void* dy, long ld_dy, void* dx, long ld_dx, const void* wq, const void* wk,
                                const float* cos_t, const float* sin_t, int table_rows, const int* pos, void* dwq, int mode_q, void* dwk, int mode_k,
                                float* part, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status, void* stream) {

@@ -17,7 +17,6 @@ from .gemm import EPI_ATOMIC, gemm, main_grad_of, main_grads
 _vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
 _native.register_cuda_sigs({
     "inv_qk_norm_fwd": [_vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _i, _vp] + [_i] * 6 + [_f, _i, _vp, _vp],
-    "inv_qk_norm_bwd_grid": [_i] * 4,
     "inv_qk_norm_bwd": [_vp, _l, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp] + [_i] * 6 + [_f, _i, _vp, _vp],
 })
 
@@ -295,10 +294,11 @@ def check_rope(cos, sin, head_dim, device):
     """The tables of a rotation, fp32 [positions, pairs], of at most ``head_dim`` values, or None twice -> rotated values of a head."""
     if cos is None and sin is None:
         return 0
-    if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError("cos and sin are fp32 tables [positions, pairs], both or neither")
-    rot = 2 * cos.shape[1]
-    if not 0 < rot <= head_dim or cos.shape[0] < 1:
+    rows, pairs = cos.shape
+    rot = 2 * pairs
+    if not 0 < rot <= head_dim or rows < 1:
         raise ValueError(f"tables {tuple(cos.shape)} for heads of {head_dim}")
     if cos.device != device or sin.device != device:
         raise ValueError(f"rotation tables on {cos.device}, heads on {device}")
@@ -335,25 +335,34 @@ def _ld(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]          # the stride of a single row says nothing
 
 
+def _dense_rows(x, width):
+    """x itself where its rows of ``width`` lie one behind the other on 16-byte boundaries, else as ``_rows16``; and how far apart they are."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0 and width * x.element_size() % 16 == 0:
+        return x, width
+    x = _rows16(x, width)
+    return x, _ld(x)
+
+
+_QK_ROWS = 296          # rows of [head_dim] sums that the backward kernel leaves at most: two CTAs an SM
+
+
 def _qk_norm_forward(qkv, wq, wk, spec):
-    """-> the result, the rows that were read, and what the backward pass's entry is given too."""
-    cos, sin, positions, seq_len, heads, kv_heads, dim, eps = spec
-    width = qkv.shape[-1]
-    x = _rows16(qkv, width)
+    """-> the result, the rows that were read and their stride, and what the backward pass's entry is given too."""
+    cos, sin, positions, rot, rows, tokens, width, seq_len, heads, kv_heads, dim, eps = spec
+    x, ld = _dense_rows(qkv, width)
     a, b = _weights16(wq, wk)
     y = torch.empty_like(qkv, memory_format=torch.contiguous_format)
-    rot, rows = (0, 0) if cos is None else (2 * cos.shape[1], cos.shape[0])
-    sizes = (x.shape[0], seq_len, heads, kv_heads, dim, rot, eps, int(x.dtype == torch.float32), rt.status_ptr(x))
-    rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), _ld(x), y.data_ptr(), width, a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
+    sizes = (tokens, seq_len, heads, kv_heads, dim, rot, eps, qkv.dtype is torch.float32, rt.status_ptr(x))
+    rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), ld, y.data_ptr(), width, a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
                                       rt.ptr(positions), *sizes, rt.stream_ptr()), "inv_qk_norm_fwd")
-    return y, x, rows, sizes
+    return y, x, ld, sizes
 
 
 class _QkNormRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, wq, wk, spec):
-        y, x, ctx.rows, ctx.sizes = _qk_norm_forward(qkv, wq, wk, spec)
-        ctx.main_grads = main_grads(wq, wk)
+        y, x, ctx.ld, ctx.sizes = _qk_norm_forward(qkv, wq, wk, spec)
+        ctx.rows, ctx.width, ctx.main_grads = spec[4], spec[6], main_grads(wq, wk)
         ctx.save_for_backward(x, wq, wk, *spec[:3])
         return y
 
@@ -361,27 +370,24 @@ class _QkNormRopeFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, wq, wk, cos, sin, positions = ctx.saved_tensors
-        T, _, H, G, D = ctx.sizes[:5]
-        width = x.shape[1]
-        d, (a, b) = _rows16(dy, width), _weights16(wq, wk)
+        d, ld = _dense_rows(dy, ctx.width)
+        a, b = _weights16(wq, wk)
         dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
-        mg_q, mg_k = (main_grad_of(w, kept) for w, kept in zip((wq, wk), ctx.main_grads))
+        part = torch.empty(_QK_ROWS * ctx.sizes[4], dtype=torch.float32, device=x.device)
+        mg_q, mg_k = main_grad_of(wq, ctx.main_grads[0]), main_grad_of(wk, ctx.main_grads[1])
         shared = None
         if mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr():     # one weight for both norms: added one after the other
             shared = mg_k = torch.zeros_like(mg_q)
-        grads = [None if mg is not None else torch.empty_like(w, memory_format=torch.contiguous_format) for w, mg in ((wq, mg_q), (wk, mg_k))]
-        outs = []
-        for g, mg in zip(grads, (mg_q, mg_k)):
-            outs += [mg.data_ptr(), 2] if mg is not None else [g.data_ptr(), int(g.dtype == torch.float32)]
-        grid = rt.lib().inv_qk_norm_bwd_grid(T, H, G, D)
-        part = torch.empty(max(grid, 1) * D, dtype=torch.float32, device=x.device)
-        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), _ld(x), d.data_ptr(), _ld(d), dx.data_ptr(), width, a.data_ptr(), b.data_ptr(),
-                                          rt.ptr(cos), rt.ptr(sin), ctx.rows, rt.ptr(positions), *outs, part.data_ptr(), *ctx.sizes,
-                                          rt.stream_ptr()), "inv_qk_norm_bwd")
+        gq, gk = (None if mg is not None else torch.empty_like(w, memory_format=torch.contiguous_format) for w, mg in ((wq, mg_q), (wk, mg_k)))
+        to_q, mode_q = (gq.data_ptr(), int(gq.dtype is torch.float32)) if mg_q is None else (mg_q.data_ptr(), 2)
+        to_k, mode_k = (gk.data_ptr(), int(gk.dtype is torch.float32)) if mg_k is None else (mg_k.data_ptr(), 2)
+        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), ctx.ld, d.data_ptr(), ld, dx.data_ptr(), ctx.width, a.data_ptr(), b.data_ptr(),
+                                          rt.ptr(cos), rt.ptr(sin), ctx.rows, rt.ptr(positions), to_q, mode_q, to_k, mode_k, part.data_ptr(),
+                                          *ctx.sizes, rt.stream_ptr()), "inv_qk_norm_bwd")
         rt.count_launches(1)
         if shared is not None:
             mg_q.add_(shared)
-        return dx, *grads, None
+        return dx, gq, gk, None
 
 
 def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_dim, positions=None, eps=1e-6):
@@ -391,18 +397,20 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
     the nearest row and ``check_status`` raises); None: 0 to S - 1. bf16 or fp32, weights in the same type; differentiable in qkv and the weights,
     whose gradients are summed in an order that the sizes alone decide. On a GPU head_dim and the rotated values are multiples of 16, head_dim at
     most 256."""
-    S, width = qkv.shape[-2] if qkv.dim() > 1 else 1, (n_q_heads + 2 * n_kv_heads) * head_dim
-    if qkv.dim() < 2 or qkv.shape[-1] != width or n_q_heads < 1 or n_kv_heads < 1:
-        raise ValueError(f"qkv of {tuple(qkv.shape)} for {n_q_heads} query and {n_kv_heads} key heads of {head_dim}")
+    shape, dtype, width = qkv.shape, qkv.dtype, (n_q_heads + 2 * n_kv_heads) * head_dim
+    if len(shape) < 2 or shape[-1] != width or n_q_heads < 1 or n_kv_heads < 1 or head_dim < 1:
+        raise ValueError(f"qkv of {tuple(shape)} for {n_q_heads} query and {n_kv_heads} key heads of {head_dim}")
+    S, dev = shape[-2], qkv.get_device()
     for w in (q_weight, k_weight):
-        if w.shape != (head_dim,) or w.dtype is not qkv.dtype or w.get_device() != qkv.get_device():
-            raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {qkv.dtype} heads of {head_dim} on {qkv.device}")
+        if w.shape != (head_dim,) or w.dtype is not dtype or w.get_device() != dev:
+            raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {dtype} heads of {head_dim} on {qkv.device}")
     rot = check_rope(cos, sin, head_dim, qkv.device)
+    rows = cos.shape[0] if rot else 0
     tokens = qkv.numel() // width
     if positions is not None and (positions.numel() != tokens or positions.dtype.is_floating_point or positions.device != qkv.device):
         raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)} on {positions.device} for {tokens} tokens on {qkv.device}")
-    if rot and positions is None and S > cos.shape[0]:
-        raise ValueError(f"{S} positions, tables of {cos.shape[0]}")
+    if rot and positions is None and S > rows:
+        raise ValueError(f"{S} positions, tables of {rows}")
     if not qkv.is_cuda:
         c = s = None
         if rot:
@@ -421,9 +429,9 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
         raise ValueError(f"heads of {head_dim} with {rot} rotated values: multiples of 16 up to 256 on a GPU")
     if positions is not None:
         positions = positions.reshape(-1).to(torch.int32).contiguous()
-    if rot:
+    if rot and not (cos.is_contiguous() and sin.is_contiguous()):
         cos, sin = cos.contiguous(), sin.contiguous()
-    spec = (cos, sin, positions, max(S, 1), n_q_heads, n_kv_heads, head_dim, float(eps))
+    spec = (cos, sin, positions, rot, rows, tokens, width, max(S, 1), n_q_heads, n_kv_heads, head_dim, float(eps))
     with rt.device_of(qkv):
         if torch.is_grad_enabled() and (qkv.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
             return _QkNormRopeFn.apply(qkv, q_weight, k_weight, spec)

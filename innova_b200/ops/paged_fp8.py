@@ -113,16 +113,27 @@ def _on16(x):
 
 
 def _aligned(x):
-    return x if _on16(x) else x.clone(memory_format=torch.contiguous_format)
-
-
-def _rows_for(out):
-    """`out`, or rows to be copied to it where its own are not aligned."""
-    return out if _on16(out) else torch.empty(out.shape, dtype=out.dtype, device=out.device)
+    """Rows of x on 16-byte boundaries, a copy where they are not, and how far apart they are."""
+    if not _on16(x):
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, _ld(x)
 
 
 def _ld(x):
-    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+    rows, width = x.shape
+    return x.stride(0) if rows > 1 else width
+
+
+def _result(out, x, rows, width):
+    """Where a call's result goes: new rows, or ``out``; with what the kernel writes, another tensor where ``out`` is not on 16-byte boundaries."""
+    if out is None:
+        out = torch.empty(rows, width, dtype=x.dtype, device=x.device)
+        return out, out, width
+    if out.shape != (rows, width) or out.dtype != x.dtype or out.device != x.device or out.stride(1) != 1:
+        raise ValueError(f"out of {out.dtype} {tuple(out.shape)} for {rows} rows of {width}")
+    if not x.is_cuda or _on16(out):
+        return out, out, _ld(out)
+    return out, out.clone(memory_format=torch.contiguous_format), width          # with its rows that the call leaves alone
 
 
 def scale_of(amax: torch.Tensor) -> torch.Tensor:
@@ -182,22 +193,19 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
     tokens' places in their sequences. Returns the queries [T, heads * dim]. On a GPU an entry that points outside the tables or the pool is reported
     (``check_status`` raises) and its keys and values are not written."""
     N, G, D = _check(qkv, "qkv", heads, pages, page_table, kv_heads)
-    T = qkv.shape[0]
-    if D != dim or qkv.shape[1] != (heads + 2 * G) * D:
+    T, width = qkv.shape
+    if D != dim or width != (heads + 2 * G) * D:
         raise ValueError(f"qkv of {tuple(qkv.shape)} for {heads} query and {kv_heads} key heads of {dim} on pages of {D}")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("norm weights of queries and keys, both or neither")
     for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (D,) or w.dtype != qkv.dtype or w.device != qkv.device):
+        if w is not None and (w.shape != (D,) or w.dtype is not qkv.dtype or w.get_device() != qkv.get_device()):
             raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {qkv.dtype} heads of {D} on {qkv.device}")
     rot = check_rope(cos, sin, D, qkv.device)
     n = _check_new(new, qkv)
     if positions is not None and (positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous() or positions.device != qkv.device):
         raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)}: contiguous int32, one for each of {T} tokens")
-    if q_out is None:
-        q_out = torch.empty(T, heads * D, dtype=qkv.dtype, device=qkv.device)
-    elif q_out.shape != (T, heads * D) or q_out.dtype != qkv.dtype or q_out.device != qkv.device or q_out.stride(1) != 1:
-        raise ValueError(f"q_out of {q_out.dtype} {tuple(q_out.shape)} for {T} tokens of {heads} heads of {D}")
+    q_out, to, ld_q = _result(q_out, qkv, T, heads * D)
     if not qkv.is_cuda:
         x = qkv.float().view(T, heads + 2 * G, D)
         for t0, m, start, ids in _places(new, page_table, N, T):
@@ -216,21 +224,19 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
         return q_out
     if rot % 16:
         raise ValueError(f"{rot} rotated values: a multiple of 16 on a GPU")
-    if not _on16(q_out):
-        raise ValueError("q_out starts and steps on 16-byte boundaries")
     if T == 0 or n == 0:
         return q_out
-    qkv = _aligned(qkv)
+    qkv, ld = _aligned(qkv)
     q_weight, k_weight = _weights16(q_weight, k_weight)
-    if rot:
+    if rot and not (cos.is_contiguous() and sin.is_contiguous()):
         cos, sin = cos.contiguous(), sin.contiguous()
-    at, size, ld = qkv.data_ptr(), D * qkv.element_size(), _ld(qkv)
+    at, size = qkv.data_ptr(), D * qkv.element_size()
     with rt.device_of(qkv):
-        rt.check(rt.lib().inv_fp8_append(at, at + heads * size, ld, at + (heads + G) * size, ld, q_out.data_ptr(), _ld(q_out), heads, G, D,
+        rt.check(rt.lib().inv_fp8_append(at, at + heads * size, ld, at + (heads + G) * size, ld, to.data_ptr(), ld_q, heads, G, D,
                                          rt.ptr(q_weight), rt.ptr(k_weight), float(eps), rt.ptr(cos), rt.ptr(sin), cos.shape[0] if rot else 0, rot,
                                          rt.ptr(positions), *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(),
                                          new.start.data_ptr(), n, T, rt.status_ptr(qkv), rt.stream_ptr()), "inv_fp8_append")
-    return q_out
+    return q_out if to is q_out else q_out.copy_(to)
 
 
 def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens):
@@ -246,9 +252,9 @@ def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens):
         return
     if T == 0 or n == 0:
         return
-    k, v = _aligned(k), _aligned(v)
+    (k, ld), (v, ld_v) = _aligned(k), _aligned(v)
     with rt.device_of(k):
-        rt.check(rt.lib().inv_fp8_append(0, k.data_ptr(), _ld(k), v.data_ptr(), _ld(v), 0, 0, 0, G, D, 0, 0, 0.0, 0, 0, 0, 0, 0,
+        rt.check(rt.lib().inv_fp8_append(0, k.data_ptr(), ld, v.data_ptr(), ld_v, 0, 0, 0, G, D, 0, 0, 0.0, 0, 0, 0, 0, 0,
                                          *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
                                          rt.status_ptr(k), rt.stream_ptr()), "inv_fp8_append")
 
@@ -273,14 +279,6 @@ def _softmax_rows(q, k, v, scale, seen):
     return o.masked_fill(lost.unsqueeze(2), float("nan")).reshape(q.shape[0], -1)
 
 
-def _check_out(out, q, width):
-    if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format)
-    if out.shape != (q.shape[0], width) or out.dtype != q.dtype or out.device != q.device or out.stride(1) != 1:
-        raise ValueError(f"out of {out.dtype} {tuple(out.shape)} for {q.shape[0]} rows of {width}")
-    return out
-
-
 def _workspace(n, T, heads, kv_heads, dim, max_new, max_len, window, tree, dev):
     """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
     fn = rt.lib().inv_fp8_attend_floats
@@ -296,12 +294,12 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
     sees the positions up to p, or with ``window`` > 0 the latest ``window`` of them, its own included; query head h uses key head
     h // (heads / kv_heads). Returns [T, heads * dim]."""
     N, G, D = _check(q, "q", heads, pages, page_table)
-    T = q.shape[0]
-    if q.shape[1] != heads * D or window < 0:
+    T, width = q.shape
+    if width != heads * D or window < 0:
         raise ValueError(f"q of {tuple(q.shape)} for {heads} heads of {D}, window {window}")
     n = _check_new(new, q)
     scale = D ** -0.5 if scale is None else float(scale)
-    out = _check_out(out, q, heads * D)
+    out, to, ld_o = _result(out, q, T, width)
     if not q.is_cuda:
         for t0, m, start, ids in _places(new, page_table, N, T):
             if m:
@@ -312,10 +310,10 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
         return out
     if T == 0 or n == 0:
         return out
-    q, to = _aligned(q), _rows_for(out)
+    q, ld = _aligned(q)
     with rt.device_of(q):
         work = _workspace(n, T, heads, G, D, new.max_new, new.max_len, window, 0, q.device)
-        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, window,
+        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), ld, to.data_ptr(), ld_o, heads, G, D, scale, window,
                                          *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
                                          new.max_new, new.max_len, rt.ptr(work), rt.status_ptr(q), rt.stream_ptr()),
                  "inv_fp8_attend")
@@ -328,14 +326,14 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
     and sees those below ``tail_start[t]`` and token ``tail_start[t] + i``, i < 64, iff bit i of ``tail_mask[t]`` (int64) is set; all of them without a
     tail. A row that sees nothing gives zeros. No row of the page table holds more than ``max_len`` tokens."""
     N, G, D = _check(q, "q", heads, pages, page_table)
-    T = q.shape[0]
-    if q.shape[1] != heads * D or max_len < 1 or (tail_start is None) != (tail_mask is None):
+    T, width = q.shape
+    if width != heads * D or max_len < 1 or (tail_start is None) != (tail_mask is None):
         raise ValueError(f"q of {tuple(q.shape)} for {heads} heads of {D}, max_len {max_len}, tail_start and tail_mask both or neither")
     for t, size, dt in ((seq_lens, page_table.shape[0], torch.int32), (row_seq, T, torch.int32), (tail_start, T, torch.int32), (tail_mask, T, torch.int64)):
         if t is not None and (t.dtype != dt or t.numel() != size or not t.is_contiguous() or t.device != q.device):
             raise ValueError(f"{tuple(t.shape)} {t.dtype} on {t.device}: contiguous {dt} [{size}] on {q.device}")
     scale = D ** -0.5 if scale is None else float(scale)
-    out = _check_out(out, q, heads * D)
+    out, to, ld_o = _result(out, q, T, width)
     if not q.is_cuda:
         lens, starts, masks = seq_lens.tolist(), tail_start.tolist() if tail_start is not None else None, tail_mask.tolist() if tail_mask is not None else None
         for t, row in enumerate(row_seq.tolist()):
@@ -349,10 +347,10 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
         return out
     if T == 0:
         return out
-    q, to = _aligned(q), _rows_for(out)
+    q, ld = _aligned(q)
     with rt.device_of(q):
         work = _workspace(T, T, heads, G, D, 1, max_len, 0, 1, q.device)
-        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), _ld(q), to.data_ptr(), _ld(to), heads, G, D, scale, *_pool_args(pages, page_table),
+        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), ld, to.data_ptr(), ld_o, heads, G, D, scale, *_pool_args(pages, page_table),
                                               row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
                                               max_len, rt.ptr(work), rt.status_ptr(q), rt.stream_ptr()), "inv_fp8_attend_tree")
     return out if to is out else out.copy_(to)

@@ -487,12 +487,17 @@ def test_rows_of_no_sequence_stay_as_they_are(ctx, new, dev):
     """A padded batch: rows in front of the first sequence and behind the last, of calls in one part and in several."""
     s = Setup(ctx, new, 8, 2, 64, dev)
     q = torch.randn(s.T + 5, 8 * 64, device=dev).to(dtype_of(dev))
-    out = torch.full_like(q, 7.0)
     padded = s.tokens._replace(cu=s.tokens.cu + 2)
-    pf.kv_attend(q, s.pool, s.page_table, padded, 8, out=out)
-    assert bool((out[:2] == 7).all()) and bool((out[2 + s.T:] == 7).all())
     want = pf.kv_attend(q[2:2 + s.T], s.pool, s.page_table, s.tokens, 8)
-    assert torch.equal(out[2:2 + s.T], want)
+    for off in (0, 3):                                   # off 16 bytes too
+        out = torch.full((s.T + 5, 8 * 64 + 5), 7.0, dtype=q.dtype, device=dev)[:, off:off + 8 * 64]
+        pf.kv_attend(q, s.pool, s.page_table, padded, 8, out=out)
+        assert bool((out[:2] == 7).all()) and bool((out[2 + s.T:] == 7).all()) and torch.equal(out[2:2 + s.T], want)
+    qkv = torch.randn(s.T + 5, 12 * 64, device=dev).to(q.dtype)
+    for off in (0, 3):
+        out = torch.full((s.T + 5, 8 * 64 + 5), 7.0, dtype=q.dtype, device=dev)[:, off:off + 8 * 64]
+        pf.qkv_append(qkv, 8, 2, 64, s.pool, s.page_table, padded, q_out=out)
+        assert bool((out[:2] == 7).all()) and bool((out[2 + s.T:] == 7).all()) and torch.equal(out[2:2 + s.T], qkv[2:2 + s.T, :8 * 64])
     if dev == "cuda":
         rt.check_status()
 
