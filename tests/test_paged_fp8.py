@@ -532,6 +532,33 @@ def test_gpu_positions_behind_the_page_table(new):
 
 
 @pytest.mark.gpu
+def test_gpu_pages_behind_four_gigabytes():
+    """Pages whose bytes lie behind 2^32 of each pool: the results and the pages of a small pool."""
+    far = 2 ** 18 + 5                                                                 # pages of 8 heads of 128: 16 KB
+    s = Setup([700, 40], [1, 90], 16, 8, 128, "cuda")
+    s.pool.k_scale.nan_to_num_(1.0)
+    s.pool.v_scale.nan_to_num_(1.0)
+    big = pf.Fp8Pages(*(torch.empty(far + s.pages, *x.shape[1:], dtype=torch.uint8 if x.element_size() == 1 else x.dtype, device="cuda") for x in s.pool))
+    big = pf.Fp8Pages(*(x.view(y.dtype) for x, y in zip(big, s.pool)))
+    for x, y in zip(big, s.pool):
+        x[far:].view(torch.uint8).copy_(y.view(torch.uint8))
+    table = torch.where(s.page_table >= 0, s.page_table + far, s.page_table)
+    qkv = torch.randn(s.T, 32 * 128, device="cuda").bfloat16()
+    cos, sin = ops.rope_tables(1000, 128, device="cuda")
+    outs = []
+    for pool, tab in ((s.pool, s.page_table), (big, table)):
+        for new in (s.tokens, s.tokens._replace(max_new=1, cu=i32([0, 1, 1], "cuda"))):
+            q = pf.qkv_append(qkv, 16, 8, 128, pool, tab, s.tokens, cos, sin)
+            out = torch.zeros_like(q)
+            pf.kv_attend(q, pool, tab, new, 16, out=out)
+            outs.append((q, out))
+    assert all(torch.equal(x, y) for a, b in ((0, 2), (1, 3)) for x, y in zip(outs[a], outs[b]))
+    for x, y in zip(big, s.pool):
+        assert torch.equal(x[far:].view(torch.uint8), y.view(torch.uint8))
+    rt.check_status()
+
+
+@pytest.mark.gpu
 def test_gpu_more_tokens_than_the_bounds_say():
     """Sequences longer than max_len are still read whole; more new tokens than max_new are reported."""
     s = Setup([5000], [1], 8, 1, 64, "cuda")
@@ -551,6 +578,26 @@ def test_gpu_more_tokens_than_the_bounds_say():
 def decode_step(s, qkv, cos, sin):
     q = pf.qkv_append(qkv, s.H, s.G, s.D, s.pool, s.page_table, s.tokens, cos, sin)
     return pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H)
+
+
+@pytest.mark.gpu
+def test_gpu_calls_of_two_streams_at_once():
+    """Prompts on one stream, single tokens split over many CTAs on another: what each gives alone."""
+    work = []
+    for ctx, new, seed in (([900, 30], [300, 400], 1), ([9000, 100], [1, 1], 2)):
+        s = Setup(ctx, new, 16, 4, 128, "cuda", seed)
+        q = s.q()
+        work.append((s, q, pf.kv_attend(q, s.pool, s.page_table, s.tokens, 16), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        outs = []
+        for s, q, _, st in work:
+            with torch.cuda.stream(st):
+                outs.append([pf.kv_attend(q, s.pool, s.page_table, s.tokens, 16) for _ in range(5)])
+        torch.cuda.synchronize()
+        for got, (_, _, want, _) in zip(outs, work):
+            assert all(torch.equal(x, want) for x in got)
+    rt.check_status()
 
 
 @pytest.mark.gpu
