@@ -39,8 +39,9 @@ class Fp8Pages(NamedTuple):
 
 class NewTokens(NamedTuple):
     """Where a step's packed tokens belong: tokens [cu[i], cu[i + 1]) are the next ones of page table row ``rows[i]``, whose first ``start[i]`` positions
-    are cached already. int32 on the pools' device; ``rows`` are distinct. The bounds size the launches, so a captured step is given the largest that it
-    will be replayed with: no sequence has more than ``max_new`` tokens here, or ``max_len`` positions with them."""
+    are cached already. int32 on the pools' device; ``rows`` are distinct. Tokens in front of ``cu[0]`` and behind ``cu[n]`` are padding: what they would
+    give stays as it is. The bounds size the launches, so a captured step is given the largest that it will be replayed with: no sequence has more than
+    ``max_new`` tokens here, or ``max_len`` positions with them."""
     rows: torch.Tensor       # [n]
     cu: torch.Tensor         # [n + 1]
     start: torch.Tensor      # [n]
