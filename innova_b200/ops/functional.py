@@ -327,7 +327,7 @@ def _rows16(x, width):
 
 
 def _weights16(*weights):
-    """Norm weights as the kernels read them: dense, on 16-byte boundaries."""
+    """Norm weights, and tables, as the kernels read them: dense, on 16-byte boundaries."""
     return [w if w is None or (w.is_contiguous() and w.data_ptr() % 16 == 0) else w.detach().clone(memory_format=torch.contiguous_format) for w in weights]
 
 
@@ -429,8 +429,7 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
         raise ValueError(f"heads of {head_dim} with {rot} rotated values: multiples of 16 up to 256 on a GPU")
     if positions is not None:
         positions = positions.reshape(-1).to(torch.int32).contiguous()
-    if rot and not (cos.is_contiguous() and sin.is_contiguous()):
-        cos, sin = cos.contiguous(), sin.contiguous()
+    cos, sin = _weights16(cos, sin)
     spec = (cos, sin, positions, rot, rows, tokens, width, max(S, 1), n_q_heads, n_kv_heads, head_dim, float(eps))
     with rt.device_of(qkv):
         if torch.is_grad_enabled() and (qkv.requires_grad or q_weight.requires_grad or k_weight.requires_grad):

@@ -228,9 +228,7 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
     if T == 0 or n == 0:
         return q_out
     qkv, ld = _aligned(qkv)
-    q_weight, k_weight = _weights16(q_weight, k_weight)
-    if rot and not (cos.is_contiguous() and sin.is_contiguous()):
-        cos, sin = cos.contiguous(), sin.contiguous()
+    q_weight, k_weight, cos, sin = _weights16(q_weight, k_weight, cos, sin)
     at, size = qkv.data_ptr(), D * qkv.element_size()
     with rt.device_of(qkv):
         rt.check(rt.lib().inv_fp8_append(at, at + heads * size, ld, at + (heads + G) * size, ld, to.data_ptr(), ld_q, heads, G, D,

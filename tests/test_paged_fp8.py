@@ -559,6 +559,18 @@ def test_gpu_pages_behind_four_gigabytes():
 
 
 @pytest.mark.gpu
+def test_gpu_append_with_tables_off_16_bytes():
+    cos, sin = ops.rope_tables(60, 64, device="cuda")
+    off = [torch.zeros(t.numel() + 1, device="cuda")[1:].view_as(t).copy_(t) for t in (cos, sin)]
+    got = []
+    for tables in ((cos, sin), off):
+        s = Setup([20, 3], [2, 5], 4, 2, 64, "cuda")
+        qkv = torch.arange(s.T * 8 * 64, device="cuda").sin().bfloat16().view(s.T, -1)
+        got.append([pf.qkv_append(qkv, 4, 2, 64, s.pool, s.page_table, s.tokens, *tables), *s.pool])
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(*got))
+
+
+@pytest.mark.gpu
 def test_gpu_more_tokens_than_the_bounds_say():
     """Sequences longer than max_len are still read whole; more new tokens than max_new are reported."""
     s = Setup([5000], [1], 8, 1, 64, "cuda")

@@ -270,3 +270,13 @@ def test_gpu_model_trains_as_on_the_cpu():
         # a value passes about forty roundings of half a bf16 step on its way through two layers and back: at most 40 * 2^-8, of random signs near 2.5 %
         assert float((b.grad.float().cpu() - a.grad).norm() / a.grad.norm()) < 0.08, n
     rt.check_status()
+
+
+@pytest.mark.gpu
+def test_gpu_tables_off_16_bytes():
+    x, wq, wk, dy, cos, sin = inputs(2, 9, 4, 2, 64, 32, torch.bfloat16, DEV)
+    off = [torch.zeros(t.numel() + 1, device=DEV)[1:].view_as(t).copy_(t) for t in (cos, sin)]
+    assert all(t.data_ptr() % 16 for t in off)
+    assert torch.equal(ops.qk_norm_rope(x, wq, wk, *off, 4, 2, 64), ops.qk_norm_rope(x, wq, wk, cos, sin, 4, 2, 64))
+    wide = [torch.zeros(t.shape[0], t.shape[1] + 3, device=DEV)[:, 1:-2].copy_(t) for t in (cos, sin)]
+    assert torch.equal(ops.qk_norm_rope(x, wq, wk, *wide, 4, 2, 64), ops.qk_norm_rope(x, wq, wk, cos, sin, 4, 2, 64))
