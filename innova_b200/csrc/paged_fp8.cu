@@ -1258,27 +1258,61 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ F
 
 using namespace inv;
 
-static bool fp8_bad_shape(int H, int Hkv, int D, int pages, int n, int T, int table_rows, int max_pages) {
-  return (D != 64 && D != 128) || Hkv < 1 || H < Hkv || H % Hkv || pages < 1 || n < 0 || T < 0 || table_rows < 1 || max_pages < 1;
-}
 static bool off16(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
   return ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) % 16 != 0;
 }
 
+// What a call's entry is given (the Python side packs the same fields in the same order): pointers, sizes in 64 bits, numbers.
+struct Fp8Where {                       // the pools, where a step's tokens belong, and where the work goes
+  void *k, *v;
+  float *k_scale, *v_scale;
+  const int *page_table, *rows, *cu, *start;
+  int* status;
+  void* stream;
+};
+struct Fp8Sizes {
+  long H, Hkv, D, pages, table_rows, max_pages, n, T;
+  bool bad() const {
+    constexpr long TOP = 0x7fffffff;
+    return (D != 64 && D != 128) || Hkv < 1 || H < Hkv || H % Hkv || pages < 1 || n < 0 || T < 0 || table_rows < 1 || max_pages < 1 || H * D > TOP ||
+           pages > TOP || table_rows > TOP || max_pages > TOP || n > TOP / 4 || T > TOP / 2;
+  }
+};
+
+static Fp8Pool pool_of(const Fp8Where& w, const Fp8Sizes& s) { return {(uint8_t*)w.k, (uint8_t*)w.v, w.k_scale, w.v_scale, (int)s.pages, (int)s.Hkv}; }
+static Fp8Tokens tokens_of(const Fp8Where& w, const Fp8Sizes& s) {
+  return {w.rows, w.cu, w.start, w.page_table, (int)s.n, (int)s.T, (int)s.table_rows, (int)s.max_pages, w.status};
+}
+
 // q_in [T, H D], k_in, v_in [T, Hkv D] bf16 -> q [T, H D] normed and rotated, and the pools. Queries and keys have rows ld_in apart, values ld_v, q
 // ld_q; H may be 0. wq, wk [D] bf16 or null; cos_t, sin_t [rope_rows, rot / 2] fp32 or null with rot 0; pos [T] or null.
-extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, const void* v_in, long ld_v, void* q, long ld_q, int H, int Hkv, int D,
-                              const void* wq, const void* wk, float eps, const float* cos_t, const float* sin_t, int rope_rows, int rot, const int* pos,
-                              void* k_pool, void* v_pool, float* k_scale, float* v_scale, int pages, const int* page_table, int table_rows,
-                              int max_pages, const int* rows, const int* cu, const int* start, int n, int T, int* status, void* stream) {
-  if (fp8_bad_shape(H ? H : Hkv, Hkv, D, pages, n, T, table_rows, max_pages) || rot < 0 || rot > D || rot % 16) return -ERR_BAD_ARG;
-  if (rot && (!cos_t || !sin_t || rope_rows < 1)) return -ERR_BAD_ARG;
-  if (ld_in % 8 || ld_v % 8 || ld_q % 8 || off16(q_in, k_in, v_in, q) || off16(wq, wk) || off16(cos_t, sin_t, k_pool, v_pool)) return -ERR_BAD_ARG;
+struct Fp8AppendDesc {
+  const void *q_in, *k_in, *v_in;
+  void* q;
+  const void *wq, *wk;
+  const float *cos_t, *sin_t;
+  const int* pos;
+  Fp8Where at;
+  Fp8Sizes size;
+  long ld_in, ld_v, ld_q, rope_rows, rot;
+  double eps;
+};
+extern "C" int inv_fp8_append(const Fp8AppendDesc* d) {
+  const int H = (int)d->size.H, Hkv = (int)d->size.Hkv, D = (int)d->size.D, n = (int)d->size.n, T = (int)d->size.T, rot = (int)d->rot;
+  Fp8Sizes s = d->size;
+  if (s.H == 0) s.H = s.Hkv;
+  if (s.bad() || d->rot < 0 || d->rot > D || rot % 16) return -ERR_BAD_ARG;
+  if (rot && (!d->cos_t || !d->sin_t || d->rope_rows < 1 || d->rope_rows > 0x7fffffffl)) return -ERR_BAD_ARG;
+  if (d->ld_in % 8 || d->ld_v % 8 || d->ld_q % 8 || off16(d->q_in, d->k_in, d->v_in, d->q) || off16(d->wq, d->wk) ||
+      off16(d->cos_t, d->sin_t, d->at.k, d->at.v))
+    return -ERR_BAD_ARG;
   if (n == 0 || T == 0) return 0;
-  const Fp8Append a{(const __nv_bfloat16*)q_in, (const __nv_bfloat16*)k_in, (const __nv_bfloat16*)v_in, (const __nv_bfloat16*)wq,
-                    (const __nv_bfloat16*)wk, cos_t, sin_t, pos, (__nv_bfloat16*)q, ld_in, ld_v, ld_q, H, rot, rope_rows, div_reciprocal(H ? H : 1), eps};
-  const Fp8Pool pool{(uint8_t*)k_pool, (uint8_t*)v_pool, k_scale, v_scale, pages, Hkv};
-  const Fp8Tokens tk{rows, cu, start, page_table, n, T, table_rows, max_pages, status};
+  const Fp8Append a{(const __nv_bfloat16*)d->q_in, (const __nv_bfloat16*)d->k_in, (const __nv_bfloat16*)d->v_in, (const __nv_bfloat16*)d->wq,
+                    (const __nv_bfloat16*)d->wk, d->cos_t, d->sin_t, d->pos, (__nv_bfloat16*)d->q, d->ld_in, d->ld_v, d->ld_q, H, rot, (int)d->rope_rows,
+                    div_reciprocal(H ? H : 1), (float)d->eps};
+  const Fp8Pool pool = pool_of(d->at, d->size);
+  const Fp8Tokens tk = tokens_of(d->at, d->size);
+  cudaStream_t st = (cudaStream_t)d->at.stream;
   const unsigned ctas = (unsigned)(T / FP8_PAGE + 2 * n);
   const int hpw = 512 / D, tokens = T / n < FP8_PAGE ? (T + n - 1) / n : FP8_PAGE;      // of an average page
   const int items = 2 * Hkv + (tokens * H + 4 * hpw - 1) / (4 * hpw);
@@ -1286,8 +1320,8 @@ extern "C" int inv_fp8_append(const void* q_in, const void* k_in, long ld_in, co
   // items 74.6, twelve 73.1. 16 x 500 with norms 52.8, 49.8, 56.2).
   const int most = (items + 3) / 4, shares = ctas <= 296 ? most : (items + 23) / 24;
   const dim3 grid(ctas, shares < 65535 ? shares : 65535);
-  if (D == 64) launch_early(fp8_append_kernel<64>, grid, 128, Fp8AppendRing::BYTES, (cudaStream_t)stream, a, pool, tk);
-  else launch_early(fp8_append_kernel<128>, grid, 128, Fp8AppendRing::BYTES, (cudaStream_t)stream, a, pool, tk);
+  if (D == 64) launch_early(fp8_append_kernel<64>, grid, 128, Fp8AppendRing::BYTES, st, a, pool, tk);
+  else launch_early(fp8_append_kernel<128>, grid, 128, Fp8AppendRing::BYTES, st, a, pool, tk);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
@@ -1385,7 +1419,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
   a.splits = cut.splits;
   a.inv_tiles = div_reciprocal(a.tiles); a.inv_splits = div_reciprocal(a.splits); a.inv_hkv = div_reciprocal(pool.Hkv); a.inv_g = div_reciprocal(a.G);
   if (cut.splits > 1) {
-    if (!work || off16(work)) return -ERR_BAD_ARG;
+    if (!work || off16(work) || (long)tk.T * a.H > 0x7fffffffl) return -ERR_BAD_ARG;
     const long rows = (long)tk.T * a.H * cut.splits;
     a.part = work;
     a.part_ml = work + rows * D;
@@ -1408,33 +1442,37 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
 
 // q [T, H D] bf16, rows ld_q apart -> out [T, H D], rows ld_o apart: the token at position p of its sequence sees the cached positions up to p, with a
 // window the latest `window` of them. No sequence has more than max_new new tokens or, with them, max_len tokens. work: inv_fp8_attend_floats of them.
-extern "C" int inv_fp8_attend(const void* q, long ld_q, void* out, long ld_o, int H, int Hkv, int D, float scale, int window, const void* k_pool,
-                              const void* v_pool, const float* k_scale, const float* v_scale, int pages, const int* page_table, int table_rows,
-                              int max_pages, const int* rows, const int* cu, const int* start, int n, int T, int max_new, int max_len, float* work,
-                              int* status, void* stream) {
-  if (fp8_bad_shape(H, Hkv, D, pages, n, T, table_rows, max_pages) || window < 0 || max_new < 1 || max_len < 1) return -ERR_BAD_ARG;
-  if (ld_q % 8 || ld_o % 8 || off16(q, k_pool, v_pool, out)) return -ERR_BAD_ARG;
-  if (n == 0 || T == 0) return 0;
-  Fp8Attend a{};
-  a.q = (const __nv_bfloat16*)q; a.out = (__nv_bfloat16*)out; a.ld_q = ld_q; a.ld_o = ld_o; a.H = H; a.window = window; a.scale = scale;
-  const Fp8Pool pool{(uint8_t*)k_pool, (uint8_t*)v_pool, (float*)k_scale, (float*)v_scale, pages, Hkv};
-  const Fp8Tokens tk{rows, cu, start, page_table, n, T, table_rows, max_pages, status};
-  return fp8_attend(a, pool, tk, D, max_new, max_len, work, (cudaStream_t)stream);
-}
-
-// One query token a row over shared sequences: row t belongs to table row row_seq[t], which holds seq_lens[row_seq[t]] tokens, and sees those below
+// Rows of a token tree, where row_seq is given: row t belongs to table row row_seq[t], which holds seq_lens[row_seq[t]] tokens, and sees those below
 // tail_start[t] and token tail_start[t] + i iff bit i of tail_mask[t] is set (both null: all). work: as for T sequences of one new token.
-extern "C" int inv_fp8_attend_tree(const void* q, long ld_q, void* out, long ld_o, int H, int Hkv, int D, float scale, const void* k_pool,
-                                   const void* v_pool, const float* k_scale, const float* v_scale, int pages, const int* page_table, int table_rows,
-                                   int max_pages, const int* row_seq, const int* seq_lens, const int* tail_start, const unsigned long long* tail_mask,
-                                   int T, int max_len, float* work, int* status, void* stream) {
-  if (fp8_bad_shape(H, Hkv, D, pages, T, T, table_rows, max_pages) || max_len < 1 || !row_seq || !seq_lens || !tail_start != !tail_mask) return -ERR_BAD_ARG;
-  if (ld_q % 8 || ld_o % 8 || off16(q, k_pool, v_pool, out)) return -ERR_BAD_ARG;
-  if (T == 0) return 0;
+struct Fp8AttendDesc {
+  const void* q;
+  void* out;
+  float* work;
+  const int *row_seq, *seq_lens, *tail_start;
+  const unsigned long long* tail_mask;
+  Fp8Where at;
+  Fp8Sizes size;
+  long ld_q, ld_o, window, max_new, max_len;
+  double scale;
+};
+extern "C" int inv_fp8_attend(const Fp8AttendDesc* d) {
+  constexpr long TOP = 0x7fffffff;
+  if (d->size.bad() || d->window < 0 || d->max_new < 1 || d->max_len < 1 || d->max_new > TOP / 4 || d->max_len > TOP / 4) return -ERR_BAD_ARG;
+  if (d->row_seq && (!d->seq_lens || !d->tail_start != !d->tail_mask || d->window || d->max_new != 1 || d->size.n != d->size.T)) return -ERR_BAD_ARG;
+  if (d->ld_q % 8 || d->ld_o % 8 || off16(d->q, d->at.k, d->at.v, d->out)) return -ERR_BAD_ARG;
+  if (d->size.n == 0 || d->size.T == 0) return 0;
   Fp8Attend a{};
-  a.q = (const __nv_bfloat16*)q; a.out = (__nv_bfloat16*)out; a.ld_q = ld_q; a.ld_o = ld_o; a.H = H; a.scale = scale;
-  a.row_seq = row_seq; a.seq_lens = seq_lens; a.tail_start = tail_start; a.tail_mask = tail_mask;
-  const Fp8Pool pool{(uint8_t*)k_pool, (uint8_t*)v_pool, (float*)k_scale, (float*)v_scale, pages, Hkv};
-  const Fp8Tokens tk{nullptr, nullptr, nullptr, page_table, T, T, table_rows, max_pages, status};
-  return fp8_attend(a, pool, tk, D, 1, max_len, work, (cudaStream_t)stream);
+  a.q = (const __nv_bfloat16*)d->q;
+  a.out = (__nv_bfloat16*)d->out;
+  a.ld_q = d->ld_q;
+  a.ld_o = d->ld_o;
+  a.H = (int)d->size.H;
+  a.window = (int)(d->window < TOP ? d->window : TOP);
+  a.scale = (float)d->scale;
+  a.row_seq = d->row_seq;
+  a.seq_lens = d->seq_lens;
+  a.tail_start = d->tail_start;
+  a.tail_mask = d->tail_mask;
+  return fp8_attend(a, pool_of(d->at, d->size), tokens_of(d->at, d->size), (int)d->size.D, (int)d->max_new, (int)d->max_len, d->work,
+                    (cudaStream_t)d->at.stream);
 }

@@ -245,13 +245,32 @@ struct QkBwdCut {
 
 using namespace inv;
 
-static int qk_norm_args(const QkNorm& p, int f32) {
-  const int vec = f32 ? 4 : 8;
-  if (p.D < 16 || p.D > 256 || p.D % 16 || p.rot < 0 || p.rot > p.D || p.rot % 16 || p.H < 0 || p.Hkv < 0 || p.H + p.Hkv < 1 || p.S < 1) return -ERR_BAD_ARG;
-  if (p.rot && (!p.cos_t || !p.sin_t || p.table_rows < 1)) return -ERR_BAD_ARG;
-  if ((long)p.T * (p.H + 2l * p.Hkv) > 0x7fff0000l) return -ERR_BAD_ARG;
-  if (p.ld_x % vec || p.ld_y % vec || p.ld_dy % vec) return -ERR_BAD_ARG;
-  if (((uintptr_t)p.x | (uintptr_t)p.y | (uintptr_t)p.dy | (uintptr_t)p.wq | (uintptr_t)p.wk | (uintptr_t)p.cos_t | (uintptr_t)p.sin_t) % 16) return -ERR_BAD_ARG;
+// What a call's entry is given (the Python side packs the same fields in the same order).
+struct QkNormDesc {
+  const void* x;                   // [T, (H + 2 Hkv) D], bf16 or fp32 (then the weights are too), rows ld_x apart
+  void* y;                         // forward: as x; backward: dx
+  const void *wq, *wk;             // [D]
+  const float *cos_t, *sin_t;      // [table_rows, rot / 2], or null with rot 0
+  const int* pos;                  // [T], or null
+  int* status;
+  void* stream;
+  // backward
+  const void* dy;
+  void *dwq, *dwk;                 // [D]; mode 0: bf16, written; 1: fp32, written; 2: fp32, added to
+  float* part;                     // 296 rows of [D]
+  long ld_x, ld_y, ld_dy, table_rows, T, S, H, Hkv, D, rot, f32, mode_q, mode_k;
+  double eps;
+};
+static int qk_norm_args(const QkNormDesc& d, QkNorm& p) {
+  const long vec = d.f32 ? 4 : 8, top = 0x7fff0000l;
+  if (d.D < 16 || d.D > 256 || d.D % 16 || d.rot < 0 || d.rot > d.D || d.rot % 16 || d.H < 0 || d.Hkv < 0 || d.H + d.Hkv < 1 || d.S < 1 || d.S > top ||
+      d.T < 0 || d.T > top || d.H + 2 * d.Hkv > top || d.T * (d.H + 2 * d.Hkv) > top)
+    return -ERR_BAD_ARG;
+  if (d.rot && (!d.cos_t || !d.sin_t || d.table_rows < 1 || d.table_rows > top)) return -ERR_BAD_ARG;
+  if (d.ld_x % vec || d.ld_y % vec || d.ld_dy % vec) return -ERR_BAD_ARG;
+  if (((uintptr_t)d.x | (uintptr_t)d.y | (uintptr_t)d.dy | (uintptr_t)d.wq | (uintptr_t)d.wk | (uintptr_t)d.cos_t | (uintptr_t)d.sin_t) % 16) return -ERR_BAD_ARG;
+  p = QkNorm{d.x, d.wq, d.wk, d.dy, d.y, d.cos_t, d.sin_t, d.pos, d.part, d.status, (int)d.T, (int)d.S, (int)d.H, (int)d.Hkv, (int)d.D, (int)d.rot,
+             (int)d.table_rows, 0, 0, 0, div_reciprocal((int)d.S), 0, 0, d.ld_x, d.ld_y, d.ld_dy, (float)d.eps, 1.f / (float)d.D};
   return 0;
 }
 template <typename T, int L>
@@ -275,45 +294,38 @@ static void qk_bwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
     default: LAUNCH<T, 16>(p, grid, st);          \
   }
 
-// x, y: [T, (H + 2 Hkv) D], bf16 or fp32 (then the weights are too), rows ld_x and ld_y apart. cos_t, sin_t: [table_rows, rot / 2] fp32.
-extern "C" int inv_qk_norm_fwd(const void* x, long ld_x, void* y, long ld_y, const void* wq, const void* wk, const float* cos_t, const float* sin_t,
-                               int table_rows, const int* pos, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status,
-                               void* stream) {
-  QkNorm p{x, wq, wk, nullptr, y, cos_t, sin_t, pos, nullptr, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, 0, 0, 0, ld_x, ld_y, 0, eps, 1.f / (float)D};
-  if (int rc = qk_norm_args(p, f32)) return rc;
-  if (T <= 0) return 0;
-  const int slots = H + 2 * Hkv, hpw = 32 / head_lanes(D);
-  p.inv_s = div_reciprocal(S);
+extern "C" int inv_qk_norm_fwd(const QkNormDesc* d) {
+  QkNorm p;
+  if (int rc = qk_norm_args(*d, p)) return rc;
+  if (p.T == 0) return 0;
+  const int slots = p.H + 2 * p.Hkv, hpw = 32 / head_lanes(p.D);
   p.inv_slots = div_reciprocal(slots);
-  const unsigned grid = (unsigned)qk_ctas(T, slots, hpw, 148 * QK_FWD_CTAS);
-  p.rounds = qk_rounds(T, slots, hpw, grid);
-  cudaStream_t st = (cudaStream_t)stream;
-  if (f32) { INV_QK_L(float, qk_fwd) } else { INV_QK_L(__nv_bfloat16, qk_fwd) }
+  const unsigned grid = (unsigned)qk_ctas(p.T, slots, hpw, 148 * QK_FWD_CTAS);
+  p.rounds = qk_rounds(p.T, slots, hpw, grid);
+  cudaStream_t st = (cudaStream_t)d->stream;
+  if (d->f32) { INV_QK_L(float, qk_fwd) } else { INV_QK_L(__nv_bfloat16, qk_fwd) }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
 
-// part: 296 rows of [D] floats. dx, dy as y and x above. dwq, dwk: [D]; mode 0: bf16, written; 1: fp32, written; 2: fp32, added to.
-extern "C" int inv_qk_norm_bwd(const void* x, long ld_x, const void* dy, long ld_dy, void* dx, long ld_dx, const void* wq, const void* wk,
-                               const float* cos_t, const float* sin_t, int table_rows, const int* pos, void* dwq, int mode_q, void* dwk, int mode_k,
-                               float* part, int T, int S, int H, int Hkv, int D, int rot, float eps, int f32, int* status, void* stream) {
-  QkNorm p{x, wq, wk, dy, dx, cos_t, sin_t, pos, part, status, T, S, H, Hkv, D, rot, table_rows, 0, 0, 0, 0, 0, 0, ld_x, ld_dx, ld_dy, eps, 1.f / (float)D};
-  if (int rc = qk_norm_args(p, f32)) return rc;
-  cudaStream_t st = (cudaStream_t)stream;
+extern "C" int inv_qk_norm_bwd(const QkNormDesc* d) {
+  QkNorm p;
+  if (int rc = qk_norm_args(*d, p)) return rc;
+  cudaStream_t st = (cudaStream_t)d->stream;
   unsigned grid = 0;
-  if (T > 0) {
-    const QkBwdCut cut(T, H, Hkv, D);
-    const int hpw = 32 / head_lanes(D);
-    p.rounds_q = qk_rounds(T, H, hpw, cut.ctas_q);
-    p.rounds = qk_rounds(T, 2 * Hkv, hpw, cut.ctas - cut.ctas_q);
-    p.inv_s = div_reciprocal(S);
-    p.inv_slots = div_reciprocal(Hkv ? 2 * Hkv : 1);
-    p.inv_slots_q = div_reciprocal(H ? H : 1);
+  if (p.T > 0) {
+    const QkBwdCut cut(p.T, p.H, p.Hkv, p.D);
+    p.inv_slots = div_reciprocal(p.Hkv ? 2 * p.Hkv : 1);
+    p.inv_slots_q = div_reciprocal(p.H ? p.H : 1);
+    const int hpw = 32 / head_lanes(p.D);
+    p.rounds_q = qk_rounds(p.T, p.H, hpw, cut.ctas_q);
+    p.rounds = qk_rounds(p.T, 2 * p.Hkv, hpw, cut.ctas - cut.ctas_q);
     p.ctas_q = cut.ctas_q;
     grid = (unsigned)cut.ctas;
-    if (f32) { INV_QK_L(float, qk_bwd) } else { INV_QK_L(__nv_bfloat16, qk_bwd) }
+    if (d->f32) { INV_QK_L(float, qk_bwd) } else { INV_QK_L(__nv_bfloat16, qk_bwd) }
   }
-  launch_early(qk_norm_dw_kernel, dim3((D + 31) / 32, 2), 1024, 0, st, (const float*)part, p.ctas_q, (int)grid, D, dwq, dwk, mode_q, mode_k);
+  launch_early(qk_norm_dw_kernel, dim3((p.D + 31) / 32, 2), 1024, 0, st, (const float*)p.part, p.ctas_q, (int)grid, p.D, d->dwq, d->dwk, (int)d->mode_q,
+               (int)d->mode_k);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }

@@ -7,6 +7,8 @@ the GPU tests). Parameters that carry an fp32 ``main_grad`` receive their gradie
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 import torch.nn.functional as F
 
@@ -14,11 +16,7 @@ from .. import _native
 from . import runtime as rt
 from .gemm import EPI_ATOMIC, gemm, main_grad_of, main_grads
 
-_vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
-_native.register_cuda_sigs({
-    "inv_qk_norm_fwd": [_vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _i, _vp] + [_i] * 6 + [_f, _i, _vp, _vp],
-    "inv_qk_norm_bwd": [_vp, _l, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _vp, _i, _vp] + [_i] * 6 + [_f, _i, _vp, _vp],
-})
+_native.register_cuda_sigs({"inv_qk_norm_fwd": [_native.vp], "inv_qk_norm_bwd": [_native.vp]})
 
 
 def _acc_grad(param, g32):
@@ -344,6 +342,9 @@ def _dense_rows(x, width):
 
 
 _QK_ROWS = 296          # rows of [head_dim] sums that the backward kernel leaves at most: two CTAs an SM
+# What the entries are given: x, y, the weights, tables, positions, status and stream; dy, the weights' gradients, sums; strides of x, y and dy, rows of the
+# tables, tokens, S, heads, key heads, dim, rot, fp32, how the gradients are left; eps.
+_QK_PACK = struct.Struct("=13Q 13q d").pack
 
 
 def _qk_norm_forward(qkv, wq, wk, spec):
@@ -352,9 +353,9 @@ def _qk_norm_forward(qkv, wq, wk, spec):
     x, ld = _dense_rows(qkv, width)
     a, b = _weights16(wq, wk)
     y = torch.empty_like(qkv, memory_format=torch.contiguous_format)
-    sizes = (tokens, seq_len, heads, kv_heads, dim, rot, eps, qkv.dtype is torch.float32, rt.status_ptr(x))
-    rt.check(rt.lib().inv_qk_norm_fwd(x.data_ptr(), ld, y.data_ptr(), width, a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rows,
-                                      rt.ptr(positions), *sizes, rt.stream_ptr()), "inv_qk_norm_fwd")
+    sizes = (rows, tokens, seq_len, heads, kv_heads, dim, rot, qkv.dtype is torch.float32)
+    rt.check(rt.lib().inv_qk_norm_fwd(_QK_PACK(x.data_ptr(), y.data_ptr(), a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rt.ptr(positions),
+                                               rt.status_ptr(x), rt.stream_ptr(), 0, 0, 0, 0, ld, width, 0, *sizes, 0, 0, eps)), "inv_qk_norm_fwd")
     return y, x, ld, sizes
 
 
@@ -362,7 +363,7 @@ class _QkNormRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, wq, wk, spec):
         y, x, ctx.ld, ctx.sizes = _qk_norm_forward(qkv, wq, wk, spec)
-        ctx.rows, ctx.width, ctx.main_grads = spec[4], spec[6], main_grads(wq, wk)
+        ctx.width, ctx.eps, ctx.main_grads = spec[6], spec[11], main_grads(wq, wk)
         ctx.save_for_backward(x, wq, wk, *spec[:3])
         return y
 
@@ -373,7 +374,7 @@ class _QkNormRopeFn(torch.autograd.Function):
         d, ld = _dense_rows(dy, ctx.width)
         a, b = _weights16(wq, wk)
         dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
-        part = torch.empty(_QK_ROWS * ctx.sizes[4], dtype=torch.float32, device=x.device)
+        part = torch.empty(_QK_ROWS * ctx.sizes[5], dtype=torch.float32, device=x.device)
         mg_q, mg_k = main_grad_of(wq, ctx.main_grads[0]), main_grad_of(wk, ctx.main_grads[1])
         shared = None
         if mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr():     # one weight for both norms: added one after the other
@@ -381,9 +382,9 @@ class _QkNormRopeFn(torch.autograd.Function):
         gq, gk = (None if mg is not None else torch.empty_like(w, memory_format=torch.contiguous_format) for w, mg in ((wq, mg_q), (wk, mg_k)))
         to_q, mode_q = (gq.data_ptr(), int(gq.dtype is torch.float32)) if mg_q is None else (mg_q.data_ptr(), 2)
         to_k, mode_k = (gk.data_ptr(), int(gk.dtype is torch.float32)) if mg_k is None else (mg_k.data_ptr(), 2)
-        rt.check(rt.lib().inv_qk_norm_bwd(x.data_ptr(), ctx.ld, d.data_ptr(), ld, dx.data_ptr(), ctx.width, a.data_ptr(), b.data_ptr(),
-                                          rt.ptr(cos), rt.ptr(sin), ctx.rows, rt.ptr(positions), to_q, mode_q, to_k, mode_k, part.data_ptr(),
-                                          *ctx.sizes, rt.stream_ptr()), "inv_qk_norm_bwd")
+        rt.check(rt.lib().inv_qk_norm_bwd(_QK_PACK(x.data_ptr(), dx.data_ptr(), a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rt.ptr(positions),
+                                                   rt.status_ptr(x), rt.stream_ptr(), d.data_ptr(), to_q, to_k, part.data_ptr(), ctx.ld, ctx.width, ld,
+                                                   *ctx.sizes, mode_q, mode_k, ctx.eps)), "inv_qk_norm_bwd")
         rt.count_launches(1)
         if shared is not None:
             mg_q.add_(shared)

@@ -9,6 +9,8 @@ the codes that are there are then rounded to the new scale, which changes nothin
 finite makes a page of its head read as NaN until its first slot is written again."""
 from __future__ import annotations
 
+import functools
+import struct
 from typing import NamedTuple, Optional
 
 import torch
@@ -17,13 +19,12 @@ from .. import _native
 from . import runtime as rt
 from .functional import _head_norm_rope, _weights16, check_rope
 
-_vp, _i, _l, _f = _native.vp, _native.i32, _native.i64, _native.f32
-_native.register_cuda_sigs({
-    "inv_fp8_append": [_vp, _vp, _l, _vp, _l, _vp, _l, _i, _i, _i, _vp, _vp, _f, _vp, _vp, _i, _i, _vp] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i, _i, _vp, _vp],
-    "inv_fp8_attend_floats": [_i] * 9,
-    "inv_fp8_attend": [_vp, _l, _vp, _l, _i, _i, _i, _f, _i] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 3 + [_i] * 4 + [_vp] * 3,
-    "inv_fp8_attend_tree": [_vp, _l, _vp, _l, _i, _i, _i, _f] + [_vp] * 4 + [_i, _vp, _i, _i] + [_vp] * 4 + [_i, _i] + [_vp] * 3,
-})
+_native.register_cuda_sigs({"inv_fp8_append": [_native.vp], "inv_fp8_attend": [_native.vp], "inv_fp8_attend_floats": [_native.i32] * 9})
+
+# What the entries are given: their own pointers; the pools, page table, rows, cu, start, status and stream; heads, key heads, dim, pages, rows and width of
+# the table, sequences, tokens; their own sizes; a number.
+_APPEND = struct.Struct("=9Q 10Q 8q 5q d").pack
+_ATTEND = struct.Struct("=7Q 10Q 8q 5q d").pack
 
 PAGE, TOP, MIN_EXP = 16, 448.0, -64
 _e4m3, _fp32, _bf16, _int32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
@@ -167,9 +168,9 @@ def _write_tokens(k, v, pages: Fp8Pages, ids, start: int):
         at = end
 
 
-def _pool_args(pages: Fp8Pages, page_table):
-    return (pages.k.data_ptr(), pages.v.data_ptr(), pages.k_scale.data_ptr(), pages.v_scale.data_ptr(), pages.k.shape[0], page_table.data_ptr(),
-            *page_table.shape)
+def _where(pages: Fp8Pages, page_table, rows, cu, start):
+    k, v, ks, vs = pages
+    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), page_table.data_ptr(), rows, cu, start, rt.status_ptr(k), rt.stream_ptr())
 
 
 def _places(new: NewTokens, page_table, pages: int, T: int):
@@ -231,10 +232,11 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
     q_weight, k_weight, cos, sin = _weights16(q_weight, k_weight, cos, sin)
     at, size = qkv.data_ptr(), D * qkv.element_size()
     with rt.device_of(qkv):
-        rt.check(rt.lib().inv_fp8_append(at, at + heads * size, ld, at + (heads + G) * size, ld, to.data_ptr(), ld_q, heads, G, D,
-                                         rt.ptr(q_weight), rt.ptr(k_weight), float(eps), rt.ptr(cos), rt.ptr(sin), cos.shape[0] if rot else 0, rot,
-                                         rt.ptr(positions), *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(),
-                                         new.start.data_ptr(), n, T, rt.status_ptr(qkv), rt.stream_ptr()), "inv_fp8_append")
+        rt.check(rt.lib().inv_fp8_append(_APPEND(at, at + heads * size, at + (heads + G) * size, to.data_ptr(), rt.ptr(q_weight), rt.ptr(k_weight),
+                                                 rt.ptr(cos), rt.ptr(sin), rt.ptr(positions),
+                                                 *_where(pages, page_table, new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr()),
+                                                 heads, G, D, N, *page_table.shape, n, T, ld, ld, ld_q, cos.shape[0] if rot else 0, rot, eps)),
+                 "inv_fp8_append")
     return q_out if to is q_out else q_out.copy_(to)
 
 
@@ -253,9 +255,9 @@ def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens):
         return
     (k, ld), (v, ld_v) = _aligned(k), _aligned(v)
     with rt.device_of(k):
-        rt.check(rt.lib().inv_fp8_append(0, k.data_ptr(), ld, v.data_ptr(), ld_v, 0, 0, 0, G, D, 0, 0, 0.0, 0, 0, 0, 0, 0,
-                                         *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
-                                         rt.status_ptr(k), rt.stream_ptr()), "inv_fp8_append")
+        rt.check(rt.lib().inv_fp8_append(_APPEND(0, k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 0, 0,
+                                                 *_where(pages, page_table, new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr()),
+                                                 0, G, D, N, *page_table.shape, n, T, ld, ld_v, 0, 0, 0, 0.0)), "inv_fp8_append")
 
 
 def read(pages: Fp8Pages, ids: torch.Tensor, length: int):
@@ -278,12 +280,16 @@ def _softmax_rows(q, k, v, scale, seen):
     return o.masked_fill(lost.unsqueeze(2), float("nan")).reshape(q.shape[0], -1)
 
 
-def _workspace(n, T, heads, kv_heads, dim, max_new, max_len, window, tree, dev):
-    """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
+@functools.lru_cache(maxsize=1024)
+def _floats(n, T, heads, kv_heads, dim, max_new, max_len, window, tree):
     fn = rt.lib().inv_fp8_attend_floats
-    if fn.restype is not _l:
-        fn.restype = _l
-    floats = fn(n, T, heads, kv_heads, dim, max_new, max_len, window, tree)
+    fn.restype = _native.i64
+    return fn(n, T, heads, kv_heads, dim, max_new, max_len, window, tree)
+
+
+def _workspace(dev, *sizes):
+    """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
+    floats = _floats(*sizes)
     return torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
 
 
@@ -310,11 +316,12 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
     if T == 0 or n == 0:
         return out
     q, ld = _aligned(q)
+    window = min(window, 2 ** 31 - 1)
     with rt.device_of(q):
-        work = _workspace(n, T, heads, G, D, new.max_new, new.max_len, window, 0, q.device)
-        rt.check(rt.lib().inv_fp8_attend(q.data_ptr(), ld, to.data_ptr(), ld_o, heads, G, D, scale, window,
-                                         *_pool_args(pages, page_table), new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr(), n, T,
-                                         new.max_new, new.max_len, rt.ptr(work), rt.status_ptr(q), rt.stream_ptr()),
+        work = _workspace(q.device, n, T, heads, G, D, new.max_new, new.max_len, window, 0)
+        rt.check(rt.lib().inv_fp8_attend(_ATTEND(q.data_ptr(), to.data_ptr(), rt.ptr(work), 0, 0, 0, 0,
+                                                 *_where(pages, page_table, new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr()),
+                                                 heads, G, D, N, *page_table.shape, n, T, ld, ld_o, window, new.max_new, new.max_len, scale)),
                  "inv_fp8_attend")
     return out if to is out else out.copy_(to)
 
@@ -348,8 +355,8 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
         return out
     q, ld = _aligned(q)
     with rt.device_of(q):
-        work = _workspace(T, T, heads, G, D, 1, max_len, 0, 1, q.device)
-        rt.check(rt.lib().inv_fp8_attend_tree(q.data_ptr(), ld, to.data_ptr(), ld_o, heads, G, D, scale, *_pool_args(pages, page_table),
-                                              row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start), rt.ptr(tail_mask), T,
-                                              max_len, rt.ptr(work), rt.status_ptr(q), rt.stream_ptr()), "inv_fp8_attend_tree")
+        work = _workspace(q.device, T, T, heads, G, D, 1, max_len, 0, 1)
+        rt.check(rt.lib().inv_fp8_attend(_ATTEND(q.data_ptr(), to.data_ptr(), rt.ptr(work), row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start),
+                                                 rt.ptr(tail_mask), *_where(pages, page_table, 0, 0, 0),
+                                                 heads, G, D, N, *page_table.shape, T, T, ld, ld_o, 0, 1, max_len, scale)), "inv_fp8_attend")
     return out if to is out else out.copy_(to)
