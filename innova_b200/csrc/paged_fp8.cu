@@ -1337,6 +1337,7 @@ static bool fp8_few_rows(long rows, int D, long units, int pages) {
 // How an attention is cut: rows of a tile (8 `blocks`), warps and pages of a CTA, CTAs along a sequence.
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
+  long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 2l) + 1); }      // of partial results
   Fp8Cut(int n, int Hkv, int G, int D, int max_new, int max_len, int window, bool tree) {
     const long rows = (long)max_new * G;
     const long reach = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
@@ -1349,14 +1350,18 @@ struct Fp8Cut {
     // Joining the splits costs about three microseconds, and a CTA as much before its first and behind its last page, so up to 64 pages stay together (64 x
     // 640 tokens, 512 units: 22.3 us, in two parts 25.9; 16 x 4 on 1000: 14.4 and 17.1). Longer ones are cut for two CTAs an SM, in parts of 16 pages or more
     // (2000 tokens, 16 units: 16 / 32 / 64 / 126 pages 7.5, 9.6, 12.1, 15.3 us; 32000, 8 units: 24 / 64 / 128 pages 23.5, 17.8, 19.9) and of 128 at most,
-    // which evens unequal lengths out (8 of up to 65000: 128 / 192 / 512 pages 71.5, 84.6, 91.2 us; of 64999 each 165, 171, 209; 64 of 8000 164, 167). Where
-    // units alone fill the GPU several times, CTAs of two warps, which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251
+    // which evens unequal lengths out (8 of up to 65000: 128 / 192 / 512 pages 71.5, 84.6, 91.2 us; of 64999 each 165, 171, 209; 64 of 8000 164, 167). A
+    // sequence alone has none to even out: its parts fill the GPU once (128000 tokens 53.3 us, in parts of 128 pages 63.3; 250000 95.1 and 101.9; with four
+    // new tokens 100000 46.2 and 61.0, 200000 74.0 and 94.9; not so 300000 113.6 and 109.2). Where units alone fill the GPU several times, CTAs of two warps, which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251
     // 90.1 and 106.6).
     const bool many = blocks == 1 && units > 444 && pages <= 256;
     warps = many ? 2 : 4;
     const long total = units * pages;
     long want = (total + 295) / 296;
-    if (want > 128) want = 128;
+    if (want > 128) {
+      const long alone = n == 1 ? (total + (blocks == 1 ? 443 : 295)) / (blocks == 1 ? 444 : 296) : 0;
+      want = alone > 128 ? alone : 128;
+    }
     if (blocks == FT_ROWS / 8) {                                      // whole blocks of keys
       // One CTA an SM. A page takes a CTA about 0.25 us, all else as much as 24 pages; a join costs 10 of them and the partial results their bytes. Cut where
       // that comes out ahead (4 x 128 on 20000, 64 units: in 2 226 us, in 5 314, whole 424; 16 x 32 on 4000, 128 units: in 2 103, whole 87; 64 on 8000, 8
@@ -1385,7 +1390,7 @@ struct Fp8Cut {
 extern "C" long inv_fp8_attend_floats(int n, int T, int H, int Hkv, int D, int max_new, int max_len, int window, int tree) {
   if (n < 1 || T < 1 || Hkv < 1 || H < Hkv || D < 1 || max_new < 1 || max_len < 1) return 0;
   const Fp8Cut cut(n, Hkv, H / Hkv, D, max_new, max_len, window, tree);
-  return cut.splits == 1 ? 0 : (long)T * H * (cut.splits * (D + 2l) + 1);
+  return cut.floats(T, H, D);
 }
 template <int D>
 static int fp8_attend_join(const Fp8Attend& a, const Fp8Tokens& tk, int tile_rows, cudaStream_t st) {
@@ -1411,7 +1416,7 @@ static int fp8_attend_tile_launch(const Fp8Attend& a, const Fp8Pool& pool, const
   return fp8_attend_join<D>(a, tk, FT_ROWS, st);
 }
 
-static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, float* work, cudaStream_t st) {
+static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int D, int max_new, int max_len, float* work, long floats, cudaStream_t st) {
   a.G = a.H / pool.Hkv;
   const Fp8Cut cut(tk.n, pool.Hkv, a.G, D, max_new, max_len, a.window, a.row_seq != nullptr);
   a.tiles = cut.tiles;
@@ -1419,7 +1424,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
   a.splits = cut.splits;
   a.inv_tiles = div_reciprocal(a.tiles); a.inv_splits = div_reciprocal(a.splits); a.inv_hkv = div_reciprocal(pool.Hkv); a.inv_g = div_reciprocal(a.G);
   if (cut.splits > 1) {
-    if (!work || off16(work) || (long)tk.T * a.H > 0x7fffffffl) return -ERR_BAD_ARG;
+    if (!work || off16(work) || floats < cut.floats(tk.T, a.H, D) || (long)tk.T * a.H > 0x7fffffffl) return -ERR_BAD_ARG;
     const long rows = (long)tk.T * a.H * cut.splits;
     a.part = work;
     a.part_ml = work + rows * D;
@@ -1452,7 +1457,7 @@ struct Fp8AttendDesc {
   const unsigned long long* tail_mask;
   Fp8Where at;
   Fp8Sizes size;
-  long ld_q, ld_o, window, max_new, max_len;
+  long ld_q, ld_o, window, max_new, max_len, work_floats;
   double scale;
 };
 extern "C" int inv_fp8_attend(const Fp8AttendDesc* d) {
@@ -1474,5 +1479,5 @@ extern "C" int inv_fp8_attend(const Fp8AttendDesc* d) {
   a.tail_start = d->tail_start;
   a.tail_mask = d->tail_mask;
   return fp8_attend(a, pool_of(d->at, d->size), tokens_of(d->at, d->size), (int)d->size.D, (int)d->max_new, (int)d->max_len, d->work,
-                    (cudaStream_t)d->at.stream);
+                    d->work_floats, (cudaStream_t)d->at.stream);
 }

@@ -24,7 +24,7 @@ _native.register_cuda_sigs({"inv_fp8_append": [_native.vp], "inv_fp8_attend": [_
 # What the entries are given: their own pointers; the pools, page table, rows, cu, start, status and stream; heads, key heads, dim, pages, rows and width of
 # the table, sequences, tokens; their own sizes; a number.
 _APPEND = struct.Struct("=9Q 10Q 8q 5q d").pack
-_ATTEND = struct.Struct("=7Q 10Q 8q 5q d").pack
+_ATTEND = struct.Struct("=7Q 10Q 8q 6q d").pack
 
 PAGE, TOP, MIN_EXP = 16, 448.0, -64
 _e4m3, _fp32, _bf16, _int32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
@@ -288,9 +288,9 @@ def _floats(n, T, heads, kv_heads, dim, max_new, max_len, window, tree):
 
 
 def _workspace(dev, *sizes):
-    """Partial results of a split attention. A call's own, so that calls on two streams and captured graphs share none."""
+    """Partial results of a split attention, and how many values. A call's own, so that calls on two streams and captured graphs share none."""
     floats = _floats(*sizes)
-    return torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+    return torch.empty(floats, dtype=torch.float32, device=dev) if floats else None, floats
 
 
 def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale: Optional[float] = None, window: int = 0,
@@ -318,10 +318,10 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
     q, ld = _aligned(q)
     window = min(window, 2 ** 31 - 1)
     with rt.device_of(q):
-        work = _workspace(q.device, n, T, heads, G, D, new.max_new, new.max_len, window, 0)
+        work, floats = _workspace(q.device, n, T, heads, G, D, new.max_new, new.max_len, window, 0)
         rt.check(rt.lib().inv_fp8_attend(_ATTEND(q.data_ptr(), to.data_ptr(), rt.ptr(work), 0, 0, 0, 0,
                                                  *_where(pages, page_table, new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr()),
-                                                 heads, G, D, N, *page_table.shape, n, T, ld, ld_o, window, new.max_new, new.max_len, scale)),
+                                                 heads, G, D, N, *page_table.shape, n, T, ld, ld_o, window, new.max_new, new.max_len, floats, scale)),
                  "inv_fp8_attend")
     return out if to is out else out.copy_(to)
 
@@ -355,8 +355,8 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
         return out
     q, ld = _aligned(q)
     with rt.device_of(q):
-        work = _workspace(q.device, T, T, heads, G, D, 1, max_len, 0, 1)
+        work, floats = _workspace(q.device, T, T, heads, G, D, 1, max_len, 0, 1)
         rt.check(rt.lib().inv_fp8_attend(_ATTEND(q.data_ptr(), to.data_ptr(), rt.ptr(work), row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start),
                                                  rt.ptr(tail_mask), *_where(pages, page_table, 0, 0, 0),
-                                                 heads, G, D, N, *page_table.shape, T, T, ld, ld_o, 0, 1, max_len, scale)), "inv_fp8_attend")
+                                                 heads, G, D, N, *page_table.shape, T, T, ld, ld_o, 0, 1, max_len, floats, scale)), "inv_fp8_attend")
     return out if to is out else out.copy_(to)
