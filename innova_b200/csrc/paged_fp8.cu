@@ -1352,8 +1352,8 @@ struct Fp8Cut {
     // (2000 tokens, 16 units: 16 / 32 / 64 / 126 pages 7.5, 9.6, 12.1, 15.3 us; 32000, 8 units: 24 / 64 / 128 pages 23.5, 17.8, 19.9) and of 128 at most,
     // which evens unequal lengths out (8 of up to 65000: 128 / 192 / 512 pages 71.5, 84.6, 91.2 us; of 64999 each 165, 171, 209; 64 of 8000 164, 167). A
     // sequence alone has none to even out: its parts fill the GPU once (128000 tokens 53.3 us, in parts of 128 pages 63.3; 250000 95.1 and 101.9; with four
-    // new tokens 100000 46.2 and 61.0, 200000 74.0 and 94.9; not so 300000 113.6 and 109.2). Where units alone fill the GPU several times, CTAs of two warps, which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251
-    // 90.1 and 106.6).
+    // new tokens 100000 46.2 and 61.0, 200000 74.0 and 94.9; not so 300000 113.6 and 109.2). Where units alone fill the GPU several times, CTAs of two warps,
+    // which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251 90.1 and 106.6).
     const bool many = blocks == 1 && units > 444 && pages <= 256;
     warps = many ? 2 : 4;
     const long total = units * pages;
