@@ -332,9 +332,9 @@ struct PageMap {
   static __device__ __forceinline__ int col(int n) { return D == 128 ? ((n >> 1) + 4 * (n & 1)) * 16 : n * 8; }
 };
 
-constexpr int FP8_STAGES = 2;     // slots of two pages a warp
-template <int D, int NW>
-constexpr int fp8_attend_smem() { return NW * FP8_STAGES * 2 * PageMap<D>::BYTES; }
+// ST slots of two pages a warp.
+template <int D, int NW, int ST>
+constexpr int fp8_attend_smem() { return NW * ST * 2 * PageMap<D>::BYTES; }
 
 // 8 NR rows (query tokens times the heads that share a key head) against a run of pages: grid = sequences x key heads x splits x row tiles. Four warps take
 // two pages at a time in turn, each with a softmax of its own, and join at the end.
@@ -349,12 +349,12 @@ constexpr int fp8_attend_smem() { return NW * FP8_STAGES * 2 * PageMap<D>::BYTES
 // Bound by memory where there are enough pages, by a warp's own chain of instructions where there are few. A warp keeps its next pages on their way through
 // a ring of its own in shared memory, without registers and without a barrier of the CTA. Bulk copies in their place cost their issuing thread over a
 // hundred cycles each: 8 contexts of up to 65000 tokens, 8 key heads of 128, took 99.7 us with each warp's first lane issuing them, 111 with a fifth warp.
-template <int D, int NR, int NW, bool TREE>
+template <int D, int NR, int NW, bool TREE, int ST>
 __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_kernel(const __grid_constant__ Fp8Attend a,
                                                                                       const __grid_constant__ Fp8Pool pool,
                                                                                       const __grid_constant__ Fp8Tokens tk) {
   using M = PageMap<D>;
-  constexpr int ST = FP8_STAGES, KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR, SLOT = 2 * M::BYTES;
+  constexpr int KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR, SLOT = 2 * M::BYTES;
   constexpr float LIFT = 6.f, SLACK = 8.f;
   extern __shared__ __align__(128) uint8_t ring[];    // NW x ST slots; then the sums
   __shared__ float sm_m[NW][ROWS], sm_l[NW][ROWS];
@@ -1337,6 +1337,7 @@ static bool fp8_few_rows(long rows, int D, long units, int pages) {
 // How an attention is cut: rows of a tile (8 `blocks`), warps and pages of a CTA, CTAs along a sequence.
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
+  bool deep;             // one slot more a warp
   long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 2l) + 1); }      // of partial results
   Fp8Cut(int n, int Hkv, int G, int D, int max_new, int max_len, int window, bool tree) {
     const long rows = (long)max_new * G;
@@ -1356,6 +1357,9 @@ struct Fp8Cut {
     // which are dealt out more evenly (1536 units of 63 pages: 38.3 us, four warps 43.0; 512 of 251 90.1 and 106.6).
     const bool many = blocks == 1 && units > 444 && pages <= 256;
     warps = many ? 2 : 4;
+    // Four of them an SM have room for a third slot a warp (64 x 640 tokens, 512 units: 19.3 us, with three 18.2; 64 x 4000 90.3 and 86.2); more need six an
+    // SM (96 x 640, 768 units: 26.6 and 33.5; 128 x 1000, 12 heads of 64, 1536 units: 38.5 and 44.6).
+    deep = many && units <= 592;
     const long total = units * pages;
     long want = (total + 295) / 296;
     if (want > 128) {
@@ -1400,12 +1404,12 @@ static int fp8_attend_join(const Fp8Attend& a, const Fp8Tokens& tk, int tile_row
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
-template <int D, int NR, int NW, bool TREE>
+template <int D, int NR, int NW, bool TREE, int ST = 2>
 static int fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
-  constexpr int SMEM = fp8_attend_smem<D, NW>();
+  constexpr int SMEM = fp8_attend_smem<D, NW, ST>();
   static std::atomic<uint64_t> ready{0};
-  raise_smem(fp8_attend_kernel<D, NR, NW, TREE>, SMEM, ready);
-  launch_early(fp8_attend_kernel<D, NR, NW, TREE>, dim3(ctas), NW * 32, SMEM, st, a, pool, tk);
+  raise_smem(fp8_attend_kernel<D, NR, NW, TREE, ST>, SMEM, ready);
+  launch_early(fp8_attend_kernel<D, NR, NW, TREE, ST>, dim3(ctas), NW * 32, SMEM, st, a, pool, tk);
   return fp8_attend_join<D>(a, tk, 8 * NR, st);
 }
 template <int D>
@@ -1437,6 +1441,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
 #define INV_FP8(DD, TREE)                                                        \
   return cut.blocks == 2  ? fp8_attend_launch<DD, 2, 4, TREE>(a, pool, tk, grid, st) \
          : cut.warps == 4 ? fp8_attend_launch<DD, 1, 4, TREE>(a, pool, tk, grid, st) \
+         : cut.deep       ? fp8_attend_launch<DD, 1, 2, TREE, 3>(a, pool, tk, grid, st) \
                           : fp8_attend_launch<DD, 1, 2, TREE>(a, pool, tk, grid, st)
   if (D == 64 && a.row_seq) INV_FP8(64, true);
   if (D == 64) INV_FP8(64, false);

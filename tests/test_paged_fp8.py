@@ -196,6 +196,24 @@ def test_attend_extreme_values(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n, G, D", [(60, 8, 64), (57, 8, 128), (80, 8, 128), (150, 4, 64)])
+def test_gpu_many_sequences(n, G, D):
+    """So many that each is left to a CTA of two warps: single tokens by place, and as rows of a tree that see all of their sequence."""
+    g = torch.Generator().manual_seed(n)
+    ctx = torch.randint(0, 400, (n,), generator=g).tolist()
+    ctx[3], ctx[4], ctx[5] = 0, 15, 16
+    s = Setup(ctx, [1] * n, 2 * G, G, D, "cuda")
+    q = s.q()
+    got = check_attend(s, q=q)
+    lens = torch.zeros(s.page_table.shape[0], dtype=torch.int32)
+    for row, c in zip(s.owner, ctx):
+        lens[row] = c + 1
+    assert torch.equal(pf.tree_attend(q, s.pool, s.page_table, lens.cuda(), i32(s.owner, "cuda"), 2 * G, 401).cpu(), got)
+    check_attend(s, window=37, q=q)
+    rt.check_status()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("ctx, new", [([300, 41], [600, 35]), ([0], [130]), ([1000], [64])])
 def test_many_rows_again_and_again(ctx, new):
     """The roles of a CTA hand blocks to one another hundreds of times in each of these calls: no wait may run out, and no result may change."""
