@@ -5,8 +5,9 @@ the pages. ``kv_attend`` is the attention of the same new tokens over all that t
 sliding window; ``tree_attend`` that of single rows with masks of their own. ``inference.kv_cache.PagedKVCache`` with ``fmt="fp8"`` calls them.
 
 The scale of a page and head is the smallest power of two 2^e, at least 2^-64, with |x| <= 448 * 2^e for every token in it. Later tokens can raise it;
-the codes that are there are then rounded to the new scale, which changes nothing but their exponent unless they fall under 2^-6. A value that is not
-finite makes a page of its head read as NaN until its first slot is written again."""
+the codes that are there are then rounded to the new scale, which changes nothing but their exponent unless they fall under 2^-6. Tokens that are taken
+back (a draft that was not accepted) leave the scale that they raised. A value that is not finite makes a page of its head read as NaN until its first slot
+is written again."""
 from __future__ import annotations
 
 import functools
