@@ -283,7 +283,7 @@ struct Fp8Attend {
   int per_split;        // pages of a CTA
   int splits, tiles;
   uint32_t inv_tiles, inv_splits, inv_hkv, inv_g;     // div_reciprocal
-  float *part, *part_ml;  // splits > 1: [T, H, splits, D] values, [T, H, splits, 2] maximum and sum
+  float *part, *part_ref;  // splits > 1: [T, H, splits, D] values; [T, H, splits, 3] log2 of the reference of the row sum, that of the values, the sum
   int* used;            // splits > 1: [T, H] splits that a row has
   // Rows of a token tree (or null): row t is of table row row_seq[t], which holds seq_lens[.] tokens, and sees those below tail_start[t] and of the 64
   // from there on the ones whose bit is set.
@@ -296,6 +296,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// log2 of a page's scale, a power of two (0, of a page never written, is -127); NaN stays.
+__device__ __forceinline__ float log2_scale(float s) { return s == s ? (float)((int)((__float_as_uint(s) >> 23) & 255) - 127) : s; }
+// How partial sums of a row meet: the factor to a common reference, which all have where none has seen a key.
+__device__ __forceinline__ float to_reference(float from, float to) { return to == -INFINITY ? 1.f : exp2_fast(from - to); }
+// The root of 2^(values' reference - sum's). Values over the sum are multiplied by it twice: neither factor leaves the range where the result is in it.
+__device__ __forceinline__ float root_of_step(float values, float sum) { return values == -INFINITY ? 1.f : exp2_fast(0.5f * (values - sum)); }
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   constexpr int KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR, SLOT = 2 * M::BYTES;
   constexpr float LIFT = 6.f, SLACK = 8.f;
   extern __shared__ __align__(128) uint8_t ring[];    // NW x ST slots; then the sums
-  __shared__ float sm_m[NW][ROWS], sm_l[NW][ROWS];
+  __shared__ float sm_m[NW][ROWS], sm_r[NW][ROWS], sm_l[NW][ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   int x = div_by(blockIdx.x, a.tiles, a.inv_tiles);
   const int tile = blockIdx.x - x * a.tiles, y = div_by(x, a.splits, a.inv_splits), split = x - y * a.splits;
@@ -691,6 +697,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
       const int r = b * 8 + 2 * c + e;
       if (n == 0) {
         sm_m[warp][r] = m[b][e];
+        sm_r[warp][r] = m[b][e] + log2_scale(vref);
         sm_l[warp][r] = l[b][e];
       }
       if (r < nr) {
@@ -698,34 +705,40 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
 #pragma unroll
         for (int k = 0; k < NI; k += 2)
           *reinterpret_cast<float4*>(to + 2 * k) =
-              make_float4(o[b][k][e] * vref, o[b][k][2 + e] * vref, o[b][k + 1][e] * vref, o[b][k + 1][2 + e] * vref);
+              make_float4(o[b][k][e], o[b][k][2 + e], o[b][k + 1][e], o[b][k + 1][2 + e]);
       }
     }
   __syncthreads();
   for (int i = threadIdx.x; i < nr * (D / 4); i += NW * 32) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float mm = sm_m[0][r];
+    float mm = sm_m[0][r], rr = sm_r[0][r];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm_m[w][r]);
+    for (int w = 1; w < NW; ++w) {
+      mm = fmaxf(mm, sm_m[w][r]);
+      rr = fmaxf(rr, sm_r[w][r]);
+    }
     float acc[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
-      const float f = mm == -INFINITY ? 1.f : exp2_fast(sm_m[w][r] - mm);
+      const float f = to_reference(sm_r[w][r], rr);
       const float4 v = *reinterpret_cast<const float4*>(sums + w * SHARE + r * D + d);
       acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f;
-      ll += sm_l[w][r] * f;
+      ll += sm_l[w][r] * to_reference(sm_m[w][r], mm);
     }
     const int tok = div_by(r0 + r, a.G, a.inv_g), t = t0 + tok, hd = hk * a.G + r0 + r - tok * a.G;
     if (a.splits == 1) {
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;
-      *reinterpret_cast<uint2*>(a.out + t * a.ld_o + hd * D + d) = make_uint2(cvt_bf16x2(acc[0] * inv, acc[1] * inv), cvt_bf16x2(acc[2] * inv, acc[3] * inv));
+      const float inv = ll == 0.f ? 0.f : 1.f / ll, root = root_of_step(rr, mm);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * inv * root * root;
+      *reinterpret_cast<uint2*>(a.out + t * a.ld_o + hd * D + d) = make_uint2(cvt_bf16x2(acc[0], acc[1]), cvt_bf16x2(acc[2], acc[3]));
       continue;
     }
     const long at = ((long)t * a.H + hd) * a.splits + split;
     *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     if (d == 0) {
-      a.part_ml[2 * at] = mm;
-      a.part_ml[2 * at + 1] = ll;
+      a.part_ref[3 * at] = mm;
+      a.part_ref[3 * at + 1] = rr;
+      a.part_ref[3 * at + 2] = ll;
       if (split == 0) a.used[(long)t * a.H + hd] = max(1, min(a.splits, (pg_hi - pg_lo + a.per_split - 1) / a.per_split));
     }
   }
@@ -736,8 +749,6 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t M, uint32_t N, ui
   return (1u << 4) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);        // fp32 sums of fp16 operands
 }
 
-// log2 of a page's scale, a power of two (0, of a page never written, is -127); NaN stays.
-__device__ __forceinline__ float log2_scale(float s) { return s == s ? (float)((int)((__float_as_uint(s) >> 23) & 255) - 127) : s; }
 __device__ __forceinline__ float max_or_nan(float a, float b) {
   float d;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
@@ -1139,7 +1150,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       if (ok) ok = mbar_wait_warp(&o_full[t], (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
       if (ok) {
         tc_fence_after();
-        const float vscale = exp2_fast(vref), inv = l == 0.f ? 0.f : vscale / l;
+        const float inv = l == 0.f ? 0.f : 1.f / l, values = m + vref, root = root_of_step(values, m);
         const long at = ((long)(t0 + tok) * a.H + hd) * a.splits + split;
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
@@ -1152,21 +1163,22 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
             for (int i = 0; i < 4; ++i) {
               uint32_t h[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
+              for (int k = 0; k < 4; ++k)
+                h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv * root * root, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv * root * root);
               to[i] = make_uint4(h[0], h[1], h[2], h[3]);
             }
           } else if (rt < nr) {
             float4* to = reinterpret_cast<float4*>(a.part + at * D + cc * 32);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              to[i] = make_float4(__uint_as_float(o[i * 4]) * vscale, __uint_as_float(o[i * 4 + 1]) * vscale, __uint_as_float(o[i * 4 + 2]) * vscale,
-                                  __uint_as_float(o[i * 4 + 3]) * vscale);
+              to[i] = make_float4(__uint_as_float(o[i * 4]), __uint_as_float(o[i * 4 + 1]), __uint_as_float(o[i * 4 + 2]), __uint_as_float(o[i * 4 + 3]));
           }
           __syncwarp();
         }
         if (a.splits > 1 && rt < nr) {
-          a.part_ml[2 * at] = m;
-          a.part_ml[2 * at + 1] = l;
+          a.part_ref[3 * at] = m;
+          a.part_ref[3 * at + 1] = values;
+          a.part_ref[3 * at + 2] = l;
           if (split == 0) a.used[(long)(t0 + tok) * a.H + hd] = max(1, min(a.splits, (b_hi - b_lo + per - 1) / per));
         }
         tc_fence_before();
@@ -1216,19 +1228,25 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ F
     if (!span.fine || t < span.t0 || t - span.t0 >= span.count || (long)(t - span.t0) * a.G + head % a.G >= (long)tile_rows * a.tiles) return;
   }
   const float* base = a.part + item * splits * D + lane * E;
-  const float* ml = a.part_ml + item * splits * 2;
+  const float* ref = a.part_ref + item * splits * 3;
   const int ns = min(max(a.used[item], 0), splits);  // where a wait ran out there may be anything
-  float mm = -INFINITY;
-  for (int s = lane; s < ns; s += 32) mm = fmaxf(mm, ml[2 * s]);
+  float mm = -INFINITY, rr = -INFINITY;
+  for (int s = lane; s < ns; s += 32) {
+    mm = fmaxf(mm, ref[3 * s]);
+    rr = fmaxf(rr, ref[3 * s + 1]);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  for (int o = 16; o > 0; o >>= 1) {
+    mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    rr = fmaxf(rr, __shfl_xor_sync(0xffffffffu, rr, o));
+  }
   float acc[E], ll = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int s = WIDE ? warp : 0; s < ns; s += NW) {
-    const float f = mm == -INFINITY ? 1.f : exp2_fast(ml[2 * s] - mm);
-    ll += ml[2 * s + 1] * f;
+    const float f = to_reference(ref[3 * s + 1], rr);
+    ll += ref[3 * s + 2] * to_reference(ref[3 * s], mm);
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] += base[(long)s * D + i] * f;
   }
@@ -1248,10 +1266,10 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ F
       for (int i = 0; i < E; ++i) acc[i] += sm_o[w][lane * E + i];
     }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  const float inv = ll == 0.f ? 0.f : 1.f / ll, root = root_of_step(rr, mm);
   uint32_t* to = reinterpret_cast<uint32_t*>(a.out + t * a.ld_o + head * D + lane * E);
 #pragma unroll
-  for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+  for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv * root * root, acc[i + 1] * inv * root * root);
 }
 
 }  // namespace inv
@@ -1338,7 +1356,7 @@ static bool fp8_few_rows(long rows, int D, long units, int pages) {
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
   bool deep;             // one slot more a warp
-  long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 2l) + 1); }      // of partial results
+  long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 3l) + 1); }      // of partial results
   Fp8Cut(int n, int Hkv, int G, int D, int max_new, int max_len, int window, bool tree) {
     const long rows = (long)max_new * G;
     const long reach = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
@@ -1431,8 +1449,8 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
     if (!work || off16(work) || floats < cut.floats(tk.T, a.H, D) || (long)tk.T * a.H > 0x7fffffffl) return -ERR_BAD_ARG;
     const long rows = (long)tk.T * a.H * cut.splits;
     a.part = work;
-    a.part_ml = work + rows * D;
-    a.used = (int*)(work + rows * (D + 2));
+    a.part_ref = work + rows * D;
+    a.used = (int*)(work + rows * (D + 3));
   }
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;

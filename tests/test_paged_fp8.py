@@ -195,6 +195,37 @@ def test_attend_extreme_values(dev):
     check_attend(s, q=q)
 
 
+def close_rows(got, q, s, i, t, seen):
+    """Row t of sequence i against the formula; beside ``close_attention``'s bound, what fp16 drops of a weight times its page's scale: 2^-31 of the row's
+    largest such product (half a step of 2^-24, the largest at 2^6 or more), for each key, times its code."""
+    k, v = s.values(i, s.ctx[i] + s.new[i])
+    row = q[s.cu[i] + t].cpu().double().view(s.H, s.D)
+    o, size = attention(row, k, v, seen, s.D ** -0.5)
+    scale = torch.cat([s.pool.v_scale[p].cpu().double().expand(16, s.G) for p in s.ids[i]])[:len(k)][seen]          # [keys, G]
+    w = torch.softmax(torch.einsum("ghd,jgd->ghj", row.view(s.G, -1, s.D), k[seen]) * s.D ** -0.5, -1)
+    top = (w * scale.t().unsqueeze(1)).amax(-1).view(s.H, 1)
+    codes = (v[seen].abs() / scale.unsqueeze(-1)).sum(0).repeat_interleave(s.H // s.G, 0)                          # [H, D]
+    bound = torch.finfo(q.dtype).eps / 2 * o.abs() + 2.0 ** -9 * size + 2.0 ** -31 * top * codes
+    err = (got[s.cu[i] + t].double().view(s.H, s.D) - o).abs()
+    assert bool((err <= bound).all()), (i, t, float((err / bound).nan_to_num(posinf=1e30).max()))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("case", [([200], [1], 2, 1, 64), ([90], [3], 8, 2, 128), ([100], [64], 4, 2, 64), ([3000], [1], 4, 2, 128), ([4000], [40], 8, 2, 64),
+                                  ([150] * 60, [1] * 60, 16, 8, 64)])
+def test_attend_values_near_the_largest(case, dev):
+    """Pages of scale 2^112 and codes up to 448: the mean is finite, and so is the result. One row, sixteen, tiles; in one part and in several."""
+    s = Setup(*case, dev)
+    for ids in s.ids:
+        for p in ids:
+            s.pool.v_scale[p] = 2.0 ** 112
+    q = s.q()
+    got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H).cpu()
+    for i, (a, b) in enumerate(zip(s.ctx, s.new)):
+        for t in range(0, b, max(1, b // 6)):
+            close_rows(got, q, s, i, t, torch.arange(a + b) <= a + t)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n, G, D", [(60, 8, 64), (57, 8, 128), (80, 8, 128), (150, 4, 64)])
 def test_gpu_many_sequences(n, G, D):
