@@ -283,7 +283,7 @@ struct Fp8Attend {
   int per_split;        // pages of a CTA
   int splits, tiles;
   uint32_t inv_tiles, inv_splits, inv_hkv, inv_g;     // div_reciprocal
-  float *part, *part_ref;  // splits > 1: [T, H, splits, D] values; [T, H, splits, 3] log2 of the reference of the row sum, that of the values, the sum
+  float *part, *part_ref;  // splits > 1: [T, H, splits, D] values; [T, H, splits, 2] their reference and the row sum
   int* used;            // splits > 1: [T, H] splits that a row has
   // Rows of a token tree (or null): row t is of table row row_seq[t], which holds seq_lens[.] tokens, and sees those below tail_start[t] and of the 64
   // from there on the ones whose bit is set.
@@ -296,12 +296,21 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// log2 of a page's scale, a power of two (0, of a page never written, is -127); NaN stays.
-__device__ __forceinline__ float log2_scale(float s) { return s == s ? (float)((int)((__float_as_uint(s) >> 23) & 255) - 127) : s; }
-// How partial sums of a row meet: the factor to a common reference, which all have where none has seen a key.
+// log2 of a page's scale, a power of two from 2^-64 on (0, of a page never written, counts as that: its codes are 0); NaN stays.
+__device__ __forceinline__ float log2_scale(float s) { return s == s ? (float)max((int)((__float_as_uint(s) >> 23) & 255) - 127, -64) : s; }
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+// A row's sums have one reference r, the largest s + log2 of the value scale that it has seen (s: its scores, in powers of two; within SLACK, so that it is
+// seldom raised). Values are summed with weights 2^(s + log2 scale - r + LIFT), which are the product's fp16 operand: at most 2^14, and what is rounded away
+// of one is under 2^-30 of the row's largest weight times scale, whatever pages of large values weigh little or are not seen at all. The sum of the row's
+// weights, 2^(s - r + SUM_LIFT), fits fp32 for all scales: its largest term is between 2^(-120 - SLACK + SUM_LIFT) and 2^(64 + SLACK + SUM_LIFT).
+constexpr float LIFT = 6.f, SLACK = 8.f, SUM_LIFT = 30.f;
+constexpr float SUM_OVER_VALUES = 1 << 24;                    // 2^(SUM_LIFT - LIFT)
+// The factor that takes partial sums to a common reference, which all have where none has seen a key.
 __device__ __forceinline__ float to_reference(float from, float to) { return to == -INFINITY ? 1.f : exp2_fast(from - to); }
-// The root of 2^(values' reference - sum's). Values over the sum are multiplied by it twice: neither factor leaves the range where the result is in it.
-__device__ __forceinline__ float root_of_step(float values, float sum) { return values == -INFINITY ? 1.f : exp2_fast(0.5f * (values - sum)); }
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -348,9 +357,9 @@ constexpr int fp8_attend_smem() { return NW * ST * 2 * PageMap<D>::BYTES; }
 // Scores (keys times queries) and outputs (values times weights) are products on m16n8k16 tensor instructions in fp16, with the codes as the operand of 16
 // rows, so that eight query rows fill the other one. A code is exact in fp16, and so is a query up to 2^-24 of its row's largest value once the row is
 // scaled by a power of two. Which dimension or token an index of a product means is free as long as both operands agree, so a lane's 16-byte pieces of a
-// key are its operands as they lie; the weights turn into the other product's operand by an 8 x 8 transpose. Page scales multiply the scores, and the
-// weights relative to the largest value scale so far, which the sums are kept in. Weights are 2^(s - m + 6) with a maximum that is raised only by scores
-// above m + 8, so at most 2^14, and what fp16 rounds away of a weight is under 2^-30 of the largest one.
+// key are its operands as they lie; the weights turn into the other product's operand by an 8 x 8 transpose. Scales of keys multiply the scores, scales of
+// values are added to the exponent of the weights. Every score has two exponentials, one for the sum: with one, and a factor for each page that takes the
+// value scale out again, 8 contexts of up to 65000 tokens took 76.5 us, with two 73.9.
 //
 // Bound by memory where there are enough pages, by a warp's own chain of instructions where there are few. A warp keeps its next pages on their way through
 // a ring of its own in shared memory, without registers and without a barrier of the CTA. Bulk copies in their place cost their issuing thread over a
@@ -361,9 +370,8 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
                                                                                       const __grid_constant__ Fp8Tokens tk) {
   using M = PageMap<D>;
   constexpr int KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR, SLOT = 2 * M::BYTES;
-  constexpr float LIFT = 6.f, SLACK = 8.f;
   extern __shared__ __align__(128) uint8_t ring[];    // NW x ST slots; then the sums
-  __shared__ float sm_m[NW][ROWS], sm_r[NW][ROWS], sm_l[NW][ROWS];
+  __shared__ float sm_r[NW][ROWS], sm_l[NW][ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   int x = div_by(blockIdx.x, a.tiles, a.inv_tiles);
   const int tile = blockIdx.x - x * a.tiles, y = div_by(x, a.splits, a.inv_splits), split = x - y * a.splits;
@@ -446,7 +454,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
 #pragma unroll
   for (int s = 0; s < ST - 1; ++s) fetch(s);
   int nc = nf;
-  float ksc = scale_at(pool.k_scale, nc), vsc = scale_at(pool.v_scale, nc), ksn = 0.f, vsn = 0.f;
+  float ksc = scale_at(pool.k_scale, nc), vsc = log2_scale(scale_at(pool.v_scale, nc)), ksn = 0.f, vsn = 0.f;
 
   // ---- queries: row n of a block of eight, as the second operand ----
   uint32_t qb[NR][KS][2];
@@ -487,14 +495,14 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   }
   const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;  // positions that every row sees
 
-  float o[NR][NI][4], m[NR][2], l[NR][2], vref = 0.f, vinv = 0.f;
+  float o[NR][NI][4], l[NR][2], ref[NR][2];                                   // ref: the reference, SLACK included
 #pragma unroll
   for (int b = 0; b < NR; ++b) {
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
-    m[b][0] = m[b][1] = -INFINITY;
+    ref[b][0] = ref[b][1] = -INFINITY;
     l[b][0] = l[b][1] = 0.f;
   }
 
@@ -503,7 +511,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
       if (st > 0) {
         nc = nf;
         ksc = ksn;
-        vsc = vsn;
+        vsc = log2_scale(vsn);
       }
       nn = number_of(st + 16);
     }
@@ -514,7 +522,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
     if (((st + ST - 1) & 15) == 0) nf = nn;
     const int at0 = (2 * st) & 31, there = (__ballot_sync(0xffffffffu, nc >= 0) >> at0) & 3, pos = (p0 + 2 * (warp + NW * st)) * FP8_PAGE;
     const float ks[2] = {__shfl_sync(0xffffffffu, ksc, at0), __shfl_sync(0xffffffffu, ksc, at0 + 1)};
-    const float vs[2] = {__shfl_sync(0xffffffffu, vsc, at0), __shfl_sync(0xffffffffu, vsc, at0 + 1)};
+    const float vs[2] = {__shfl_sync(0xffffffffu, vsc, at0), __shfl_sync(0xffffffffu, vsc, at0 + 1)};      // log2
     fetch(st + ST - 1);                              // into the slot of step st - 1, which every lane has read
     copies_wait<ST - 1>();
     __syncwarp();
@@ -548,7 +556,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
         }
     }
     const bool whole = pos >= all_lo && pos + 2 * FP8_PAGE <= all_hi && there == 3;
-    bool over = fmaxf(vs[0], vs[1]) > vref;
+    bool over = false;
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
@@ -577,32 +585,24 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
             }
           }
     }
+    auto highest = [&](int b, int e) { return fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]) + vs[0], fmaxf(s[b][1][e], s[b][1][2 + e]) + vs[1]); };
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float top = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
-        over |= top > m[b][e] + SLACK;
-      }
+      for (int e = 0; e < 2; ++e) over |= highest(b, e) > ref[b][e];
     if (__any_sync(0xffffffffu, over)) {
-      const float v_up = fmaxf(vs[0], vs[1]), beta = v_up > vref ? vref / v_up : 1.f;
-      if (v_up > vref) {
-        vref = v_up;
-        vinv = 1.f / v_up;
-      }
 #pragma unroll
       for (int b = 0; b < NR; ++b) {
         float alpha[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float mx = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
+          float up = highest(b, e);
 #pragma unroll
-          for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-          const float up = fmaxf(m[b][e], mx);
-          alpha[e] = up == m[b][e] ? 1.f : exp2_fast(m[b][e] - up);
-          m[b][e] = up;
+          for (int d = 4; d < 32; d *= 2) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, d));
+          up = fmaxf(ref[b][e], up + SLACK);
+          alpha[e] = up == ref[b][e] ? 1.f : exp2_fast(ref[b][e] - up);
+          ref[b][e] = up;
           l[b][e] *= alpha[e];
-          alpha[e] *= beta;
         }
 #pragma unroll
         for (int k = 0; k < NI; ++k)
@@ -610,19 +610,18 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
           for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[e & 1];
       }
     }
-    const float rel[2] = {vs[0] * vinv, vs[1] * vinv};
-    float xw[NR][2][4];                              // weights times their page's scale
+    float w[NR][2][4];                               // what the values are weighed with; s: what is summed
 #pragma unroll
-    for (int b = 0; b < NR; ++b) {
-      const float m0 = m[b][0] - LIFT, m1 = m[b][1] - LIFT;
+    for (int b = 0; b < NR; ++b)
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
+      for (int e = 0; e < 4; ++e) {
+        const float sum_off = (SUM_LIFT + SLACK) - ref[b][e & 1], off = (LIFT + SLACK) - ref[b][e & 1];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[b][g][e] = exp2_fast(s[b][g][e] - (e & 1 ? m1 : m0));
-          xw[b][g][e] = s[b][g][e] * rel[g];
+        for (int g = 0; g < 2; ++g) {
+          w[b][g][e] = exp2_fast(s[b][g][e] + (off + vs[g]));
+          s[b][g][e] = exp2_fast(s[b][g][e] + sum_off);
         }
-    }
+      }
     if (!whole) {                                    // nothing of a hidden place, whatever its scale and however little the row has seen
       rarely();
 #pragma unroll
@@ -631,7 +630,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if ((hidden >> (b * 8 + g * 4 + e)) & 1) s[b][g][e] = xw[b][g][e] = 0.f;
+            if ((hidden >> (b * 8 + g * 4 + e)) & 1) s[b][g][e] = w[b][g][e] = 0.f;
     }
     uint32_t pb[NR][2][2];                           // weights of row n: tokens of rows 2 c, 2 c + 1 (and + 8) of the score product
 #pragma unroll
@@ -641,7 +640,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
 #pragma unroll
       for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) pb[b][g][h] = transpose8(half2_of(xw[b][g][2 * h], xw[b][g][2 * h + 1]));
+        for (int h = 0; h < 2; ++h) pb[b][g][h] = transpose8(half2_of(w[b][g][2 * h], w[b][g][2 * h + 1]));
     }
     // ---- values: dimensions x 8 rows ----
 #pragma unroll
@@ -696,8 +695,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
       for (int d = 4; d < 32; d *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
       const int r = b * 8 + 2 * c + e;
       if (n == 0) {
-        sm_m[warp][r] = m[b][e];
-        sm_r[warp][r] = m[b][e] + log2_scale(vref);
+        sm_r[warp][r] = ref[b][e];
         sm_l[warp][r] = l[b][e];
       }
       if (r < nr) {
@@ -711,34 +709,30 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   __syncthreads();
   for (int i = threadIdx.x; i < nr * (D / 4); i += NW * 32) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float mm = sm_m[0][r], rr = sm_r[0][r];
+    float rr = sm_r[0][r];
 #pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      mm = fmaxf(mm, sm_m[w][r]);
-      rr = fmaxf(rr, sm_r[w][r]);
-    }
+    for (int w = 1; w < NW; ++w) rr = fmaxf(rr, sm_r[w][r]);
     float acc[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float f = to_reference(sm_r[w][r], rr);
       const float4 v = *reinterpret_cast<const float4*>(sums + w * SHARE + r * D + d);
       acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f;
-      ll += sm_l[w][r] * to_reference(sm_m[w][r], mm);
+      ll += sm_l[w][r] * f;
     }
     const int tok = div_by(r0 + r, a.G, a.inv_g), t = t0 + tok, hd = hk * a.G + r0 + r - tok * a.G;
     if (a.splits == 1) {
-      const float inv = ll == 0.f ? 0.f : 1.f / ll, root = root_of_step(rr, mm);
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * inv * root * root;
+      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * inv * SUM_OVER_VALUES;           // inv first: the values' own scale is in it
       *reinterpret_cast<uint2*>(a.out + t * a.ld_o + hd * D + d) = make_uint2(cvt_bf16x2(acc[0], acc[1]), cvt_bf16x2(acc[2], acc[3]));
       continue;
     }
     const long at = ((long)t * a.H + hd) * a.splits + split;
     *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     if (d == 0) {
-      a.part_ref[3 * at] = mm;
-      a.part_ref[3 * at + 1] = rr;
-      a.part_ref[3 * at + 2] = ll;
+      a.part_ref[2 * at] = rr;
+      a.part_ref[2 * at + 1] = ll;
       if (split == 0) a.used[(long)t * a.H + hd] = max(1, min(a.splits, (pg_hi - pg_lo + a.per_split - 1) / a.per_split));
     }
   }
@@ -749,11 +743,6 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t M, uint32_t N, ui
   return (1u << 4) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);        // fp32 sums of fp16 operands
 }
 
-__device__ __forceinline__ float max_or_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 
 // One product step or commit of a converged warp: the thread is chosen inside, under a predicate, so that operands stay in uniform registers (a branch to
 // one lane around them made each step cost about ninety cycles of its warp).
@@ -810,15 +799,14 @@ struct FtSmem {
 // 1260 (the queries are read from shared memory again for 64 keys each) and the exponentials' unit 1024: what bounds it is a row's chain of reading scores,
 // maximum, exponentials and writing weights. Two threads a row, half of a block's keys each, shorten the chain but leave the conversion half the registers:
 // 412. With barriers for keys and values apart the conversion was what every block waited for: 418.
-// Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are powers of two added to it (relative to the
-// largest one so far, which O is kept in) and taken out of the row sum again a page at a time, so neither costs anything a score. For the rest the sums are
-// those of the small kernel. Tensor memory, a tile 256 columns: scores (then weights) at 0 and 64, O at 128.
+// Scales of keys multiply the scores of their 16 columns in the exponential's argument, scales of values are added to it and taken out of the row sum again
+// a page at a time, so neither costs anything a score. The sums and their references are those of the small kernel. Tensor memory, a tile 256 columns:
+// scores (then weights) at 0 and 64, O at 128.
 template <int D>
 __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __grid_constant__ Fp8Attend a, const __grid_constant__ Fp8Pool pool,
                                                                         const __grid_constant__ Fp8Tokens tk) {
   using L = FtSmem<D>;
   constexpr int CH = D / 16, NS = FT_SLOTS;          // 16-byte pieces of a token's codes
-  constexpr float LIFT = 6.f, SLACK = 8.f;
   constexpr uint32_t T_COLS = 256, O_COL = 128, COLS = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1034,7 +1022,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
         if (lane == 0) mbar_arrive(&q_full[t]);
       }
       const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
-      float m = -INFINITY, l = 0.f, vref = -200.f;     // vref: log2 of the scale that O is kept in
+      float m = -INFINITY, l = 0.f, ref = -INFINITY;   // the sum has a reference of its own, the largest score
       bool ok = true;
       for (int j = 0; j < nb; ++j) {
         if (!mbar_wait_warp(&s_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
@@ -1058,8 +1046,8 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           for (int i = 0; i < FT_N; ++i)
             if (!seen(i)) s[i] = 0xff800000u;
         }
-        // ---- the largest score and the largest value scale ----
-        float mx = -INFINITY, v_up = -200.f;
+        // ---- the largest score, and the largest score and log2 of the value scale ----
+        float mx = -INFINITY, rx = -INFINITY;
 #pragma unroll
         for (int h = 0; h < FT_PAGES; ++h) {
           const uint32_t* u = s + h * 16;
@@ -1070,21 +1058,20 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
             x1 = fmax3(x1, __uint_as_float(u[i + 2]), __uint_as_float(u[i + 3]));
           }
           const float2 k = sc[h];
-          mx = fmaxf(mx, fmaxf(x0, x1) * (qm * k.x));
-          v_up = fmaxf(v_up, k.y);
+          const float top = fmaxf(x0, x1) * (qm * k.x);
+          mx = fmaxf(mx, top);
+          rx = fmaxf(rx, top + k.y);
         }
         // The last block passes here too, for the wait: the product after this one is waited for behind the loop, a barrier's parity tells a phase from its
         // neighbours only, and here it is sure that the phase before has ended and the one after has not.
-        if (__any_sync(0xffffffffu, mx > m + SLACK || v_up > vref) || j == nb - 1) {
+        if (__any_sync(0xffffffffu, mx > m + SLACK || rx > ref + SLACK) || j == nb - 1) {
           rarely();
           const float up = j == 0 || mx > m + SLACK ? fmaxf(m, mx) : m;
-          float alpha = up == m ? 1.f : exp2_fast(m - up);
+          const float r_up = j == 0 || rx > ref + SLACK ? fmaxf(ref, rx) : ref;
+          const float alpha = r_up == ref ? 1.f : exp2_fast(ref - r_up);
+          l *= up == m ? 1.f : exp2_fast(m - up);
           m = up;
-          l *= alpha;
-          if (v_up > vref) {
-            alpha *= exp2_fast(vref - v_up);
-            vref = v_up;
-          }
+          ref = r_up;
           if (j > 0) {                                 // O is that of the blocks before, once the last one's product is complete
             if (!mbar_wait_warp(&o_full[t], (j - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
               ok = false;
@@ -1104,12 +1091,13 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           }
         }
         // ---- weights: a page at a time, without a branch between pages where nothing is hidden, so that their chains overlap ----
-        const float base = LIFT - (m == -INFINITY ? 0.f : m);
+        const float base = LIFT - (m == -INFINITY ? 0.f : m), shift = ref == -INFINITY ? 0.f : m - ref;
         auto weigh = [&](int h, bool masked) {
           uint32_t* u = s + h * 16;
           const float2 k = sc[h];
-          // the value scale over the largest one: 2^-60 and less weigh nothing. Out of the sum again it is taken, but for no number, which is in the weights.
-          const float d = max_or_nan(k.y - vref, -60.f), f = qm * k.x, off = base + d, back = exp2_fast(fminf(60.f, -d));
+          // The page's value scale against the reference: 2^-60 and less leave nothing of a weight in fp16, so no less is said. Out of the sum again it is
+          // taken, but for no number, which is in the weights.
+          const float d = max_or_nan(k.y + shift, -60.f), f = qm * k.x, off = base + d, back = exp2_fast(fminf(60.f, -d));
           const uint64_t ff = pair_of(f, f), oo = pair_of(off, off);
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
@@ -1150,7 +1138,8 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       if (ok) ok = mbar_wait_warp(&o_full[t], (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
       if (ok) {
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l, values = m + vref, root = root_of_step(values, m);
+        l = l == 0.f ? 0.f : l * exp2_fast(m - ref + (SUM_LIFT - LIFT));          // to the values' reference
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         const long at = ((long)(t0 + tok) * a.H + hd) * a.splits + split;
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
@@ -1164,7 +1153,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
               uint32_t h[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv * root * root, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv * root * root);
+                h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv * SUM_OVER_VALUES, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv * SUM_OVER_VALUES);
               to[i] = make_uint4(h[0], h[1], h[2], h[3]);
             }
           } else if (rt < nr) {
@@ -1176,9 +1165,8 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           __syncwarp();
         }
         if (a.splits > 1 && rt < nr) {
-          a.part_ref[3 * at] = m;
-          a.part_ref[3 * at + 1] = values;
-          a.part_ref[3 * at + 2] = l;
+          a.part_ref[2 * at] = ref;
+          a.part_ref[2 * at + 1] = l;
           if (split == 0) a.used[(long)(t0 + tok) * a.H + hd] = max(1, min(a.splits, (b_hi - b_lo + per - 1) / per));
         }
         tc_fence_before();
@@ -1228,25 +1216,19 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ F
     if (!span.fine || t < span.t0 || t - span.t0 >= span.count || (long)(t - span.t0) * a.G + head % a.G >= (long)tile_rows * a.tiles) return;
   }
   const float* base = a.part + item * splits * D + lane * E;
-  const float* ref = a.part_ref + item * splits * 3;
+  const float* ref = a.part_ref + item * splits * 2;
   const int ns = min(max(a.used[item], 0), splits);  // where a wait ran out there may be anything
-  float mm = -INFINITY, rr = -INFINITY;
-  for (int s = lane; s < ns; s += 32) {
-    mm = fmaxf(mm, ref[3 * s]);
-    rr = fmaxf(rr, ref[3 * s + 1]);
-  }
+  float rr = -INFINITY;
+  for (int s = lane; s < ns; s += 32) rr = fmaxf(rr, ref[2 * s]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
-    rr = fmaxf(rr, __shfl_xor_sync(0xffffffffu, rr, o));
-  }
+  for (int o = 16; o > 0; o >>= 1) rr = fmaxf(rr, __shfl_xor_sync(0xffffffffu, rr, o));
   float acc[E], ll = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int s = WIDE ? warp : 0; s < ns; s += NW) {
-    const float f = to_reference(ref[3 * s + 1], rr);
-    ll += ref[3 * s + 2] * to_reference(ref[3 * s], mm);
+    const float f = to_reference(ref[2 * s], rr);
+    ll += ref[2 * s + 1] * f;
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] += base[(long)s * D + i] * f;
   }
@@ -1266,10 +1248,10 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ F
       for (int i = 0; i < E; ++i) acc[i] += sm_o[w][lane * E + i];
     }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll, root = root_of_step(rr, mm);
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
   uint32_t* to = reinterpret_cast<uint32_t*>(a.out + t * a.ld_o + head * D + lane * E);
 #pragma unroll
-  for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv * root * root, acc[i + 1] * inv * root * root);
+  for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv * SUM_OVER_VALUES, acc[i + 1] * inv * SUM_OVER_VALUES);
 }
 
 }  // namespace inv
@@ -1356,7 +1338,7 @@ static bool fp8_few_rows(long rows, int D, long units, int pages) {
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
   bool deep;             // one slot more a warp
-  long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 3l) + 1); }      // of partial results
+  long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 2l) + 1); }      // of partial results
   Fp8Cut(int n, int Hkv, int G, int D, int max_new, int max_len, int window, bool tree) {
     const long rows = (long)max_new * G;
     const long reach = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
@@ -1450,7 +1432,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
     const long rows = (long)tk.T * a.H * cut.splits;
     a.part = work;
     a.part_ref = work + rows * D;
-    a.used = (int*)(work + rows * (D + 3));
+    a.used = (int*)(work + rows * (D + 2));
   }
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;

@@ -226,6 +226,85 @@ def test_attend_values_near_the_largest(case, dev):
             close_rows(got, q, s, i, t, torch.arange(a + b) <= a + t)
 
 
+def along(s, apart):
+    """Scores that a test decides: all keys are +1 or, on the pages ``apart`` (sequence, page), -1 along one direction of signs; a query is that direction
+    times a size from 0 to 3 of its row and head, so that weights apart are e^-(2 size sqrt(D)) of the others. -> queries."""
+    g = torch.Generator().manual_seed(11)
+    u = torch.where(torch.rand(s.D, generator=g) < 0.5, -1.0, 1.0)
+    one = u.to(torch.float8_e4m3fn).view(torch.uint8)
+    raw = s.pool.k.view(torch.uint8)
+    for i, ids in enumerate(s.ids):
+        for j, p in enumerate(ids):
+            raw[p, :, s.filled[p].to(s.dev)] = (one ^ 128 if (i, j) in apart else one).to(s.dev)
+            s.pool.k_scale[p] = 1.0
+    size = 3 * torch.rand(s.T, s.H, 1, generator=g)
+    size[::5] = 0                                                                     # rows that weigh all pages alike
+    return (size * u).view(s.T, -1).to(dtype_of(s.dev)).to(s.dev)
+
+
+UNEVEN = [
+    # cached, new, query heads, key heads, dim: one row, sixteen, tiles; in one part and in several; many sequences
+    ([200], [1], 1, 1, 64), ([90, 37], [2, 3], 8, 2, 128), ([300, 5], [33, 40], 4, 2, 64), ([129], [150], 4, 1, 128), ([3000], [1], 8, 2, 64),
+    ([2500], [4], 8, 2, 128), ([4000, 100], [40, 3], 8, 2, 128), ([150 + i for i in range(60)], [1] * 60, 16, 8, 64),
+    ([150 + i for i in range(80)], [1] * 80, 16, 8, 128)]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("ratio", [-60, -40, 25, 30, 40, 60])
+@pytest.mark.parametrize("case", UNEVEN)
+def test_attend_pages_of_unequal_scales(case, ratio, dev):
+    """Every third page holds values 2^ratio times as large, under weights down to e^-48 and less of the others': a row is right by its own sum."""
+    s = Setup(*case, dev)
+    apart = {(i, j) for i, ids in enumerate(s.ids) for j in range(1, len(ids), 3)}
+    q = along(s, apart)
+    for i, j in apart:
+        s.pool.v_scale[s.ids[i][j]] *= 2.0 ** ratio
+    got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H).cpu()
+    for i, (a, b) in enumerate(zip(s.ctx, s.new)):
+        if i % 7 == 0 or s.n < 10:
+            for t in range(0, b, max(1, b // 6)):
+                close_rows(got, q, s, i, t, torch.arange(a + b) <= a + t)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("ratio", [30, 60, 100])
+@pytest.mark.parametrize("case", [([31], [33], 1, 1, 64, 17), ([31], [5], 2, 1, 128, 17), ([20], [200], 4, 2, 64, 40), ([2000], [300], 4, 1, 128, 700),
+                                  ([2000], [3], 4, 1, 128, 700), ([64, 70], [40, 150], 8, 2, 128, 16)])
+def test_attend_hidden_pages_of_large_values(case, ratio, dev):
+    """Pages that a row does not see leave no mark on it, however large their values: behind its window, and ahead of it."""
+    *sizes, window = case
+    for front in (True, False):
+        s = Setup(*sizes, dev)
+        q = s.q()
+        for i, (a, b) in enumerate(zip(s.ctx, s.new)):
+            far = max(0, a + 1 - window) // 16 if front else (a + b - 1) // 16         # the first page that the first token sees; the last token's
+            s.pool.v_scale[s.ids[i][far]] *= 2.0 ** ratio
+        got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H, window=window).cpu()
+        for i, (a, b) in enumerate(zip(s.ctx, s.new)):
+            j = torch.arange(a + b)
+            for t in sorted({*range(0, b, max(1, b // 9)), *range(max(0, b - 3), b)}):
+                close_rows(got, q, s, i, t, (j <= a + t) & (j > a + t - window))
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("ratio", [30, 60, 100])
+@pytest.mark.parametrize("n, H, G, D", [(70, 4, 2, 64), (2500, 8, 1, 128)])
+def test_tree_rows_hidden_pages_of_large_values(n, H, G, D, ratio, dev):
+    """The last page's values are large, and most rows' masks leave it out."""
+    s = Setup([n], [0], H, G, D, dev)
+    s.T, s.cu = 4, [0]
+    q = s.q()
+    s.pool.v_scale[s.ids[0][-1]] *= 2.0 ** ratio
+    tail = n // 16 * 16 - 16                                                          # the page before the last one, and the last
+    mask = [0xffff, -1, 0x5555, (1 << 16) - 1]
+    lens = torch.zeros(s.page_table.shape[0], dtype=torch.int32)
+    lens[s.owner[0]] = n
+    got = pf.tree_attend(q, s.pool, s.page_table, lens.to(dev), i32([s.owner[0]] * 4, dev), H, n, tail_start=i32([tail] * 4, dev),
+                         tail_mask=torch.tensor(mask, dtype=torch.int64, device=dev)).cpu()
+    for t in range(4):
+        close_rows(got, q, s, 0, t, torch.tensor([i < tail or bool(mask[t] >> (i - tail) & 1) for i in range(n)]))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n, G, D", [(60, 8, 64), (57, 8, 128), (80, 8, 128), (150, 4, 64)])
 def test_gpu_many_sequences(n, G, D):
