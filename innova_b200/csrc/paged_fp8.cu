@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
     // ---------------- conversion: a thread takes the same piece of every sixteenth (D = 64: thirty-second) token ----------------
     const int tid = threadIdx.x - 256;
     constexpr int PER = FT_N * CH / 128, STEP = 128 / CH;      // pieces of a thread in a block; tokens from one to the next
-    const int piece = tid % CH, tok0 = tid / CH, pages_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
+    const int piece = tid % CH, tok0 = tid / CH, pages_lo = lo / FP8_PAGE, pages_hi = (hi + FP8_PAGE - 1) / FP8_PAGE;
     uint4 rk[2][PER], rv[2][PER];                    // of even and odd blocks, two ahead
     // Lanes 0 to 3 look a block's pages up: read three blocks ahead, checked two ahead and codes and scales read then, so that nothing is waited for. Loads
     // stand outside of branches, from a place that exists where there is none to read: behind a branch the compiler copies what was loaded, and so waits.
@@ -920,7 +920,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
     auto read_id = [&](int j) { return list[min((b0 + j) * FT_PAGES + lane, tk.max_pages - 1)]; };
     auto check_id = [&](int id, int j) {
       const int pg = (b0 + j) * FT_PAGES + lane;
-      if (lane >= FT_PAGES || j >= nb || pg >= pages_hi) return -1;
+      if (lane >= FT_PAGES || j >= nb || pg < pages_lo || pg >= pages_hi) return -1;       // a block may begin in front of the window: such pages are absent
       if (known && pg < tk.max_pages && (unsigned)id < (unsigned)pool.pages) return id;
       atomicCAS(tk.status, 0, ERR_BAD_ARG);
       return -1;

@@ -174,8 +174,8 @@ def _where(pages: Fp8Pages, page_table, rows, cu, start):
     return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), page_table.data_ptr(), rows, cu, start, rt.status_ptr(k), rt.stream_ptr())
 
 
-def _places(new: NewTokens, page_table, pages: int, T: int):
-    """(first token, tokens, first position, page ids) of every sequence, on the CPU."""
+def _places(new: NewTokens, page_table, pages: int, T: int, window: int = 0):
+    """(first token, tokens, first position, page ids) of every sequence, on the CPU. What the table says of pages behind the window is not asked."""
     cu = new.cu.tolist()
     for i, (row, start) in enumerate(zip(new.rows.tolist(), new.start.tolist())):
         n = cu[i + 1] - cu[i]
@@ -183,6 +183,9 @@ def _places(new: NewTokens, page_table, pages: int, T: int):
         if not (0 <= cu[i] <= cu[i + 1] <= T and start >= 0 and 0 <= row < page_table.shape[0] and need <= page_table.shape[1] and n <= new.max_new):
             raise ValueError(f"sequence {i}: tokens [{cu[i]}, {cu[i + 1]}) of {T} at position {start} of row {row}")
         ids = page_table[row, :need].tolist()
+        if window:
+            behind = min(max(0, start - window + 1) // PAGE, need)
+            ids[:behind] = [0] * behind
         if n and not all(0 <= p < pages for p in ids):
             raise ValueError(f"row {row} lists a page outside the pool of {pages}")
         yield cu[i], n, start, ids
@@ -297,8 +300,8 @@ def _workspace(dev, *sizes):
 def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale: Optional[float] = None, window: int = 0,
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, heads * dim]: the queries of ``new``'s tokens, whose keys and values are in the pages already. The token at position p of its sequence
-    sees the positions up to p, or with ``window`` > 0 the latest ``window`` of them, its own included; query head h uses key head
-    h // (heads / kv_heads). Returns [T, heads * dim]."""
+    sees the positions up to p, or with ``window`` > 0 the latest ``window`` of them, its own included; pages that all of a sequence's new tokens have
+    left behind are not looked up. Query head h uses key head h // (heads / kv_heads). Returns [T, heads * dim]."""
     N, G, D = _check(q, "q", heads, pages, page_table)
     T, width = q.shape
     if width != heads * D or window < 0:
@@ -307,7 +310,7 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
     scale = D ** -0.5 if scale is None else float(scale)
     out, to, ld_o = _result(out, q, T, width)
     if not q.is_cuda:
-        for t0, m, start, ids in _places(new, page_table, N, T):
+        for t0, m, start, ids in _places(new, page_table, N, T, window):
             if m:
                 k, v = read(pages, torch.tensor(ids), start + m)
                 p, j = torch.arange(start, start + m).view(-1, 1), torch.arange(start + m)

@@ -659,6 +659,25 @@ def test_gpu_positions_behind_the_page_table(new):
     assert not bool(got.any())
 
 
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("case", [([3000], [200], 4, 2, 64), ([3001], [3], 4, 2, 64), ([3007, 333], [64, 90], 8, 2, 128), ([20000], [40], 8, 2, 128)])
+def test_pages_behind_the_window_are_not_looked_up(case, dev):
+    """Their entries may point nowhere; that of the first page that is seen may not."""
+    window = 100
+    s = Setup(*case, dev)
+    q = s.q()
+    want = pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H, window=window)
+    for r, a in zip(s.owner, s.ctx):
+        s.page_table[r, :(a - window + 1) // 16] = -1
+    assert torch.equal(pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H, window=window), want)
+    if dev == "cuda":
+        rt.check_status()
+    s.page_table[s.owner[0], (s.ctx[0] - window + 1) // 16] = -1
+    with pytest.raises(ValueError if dev == "cpu" else RuntimeError):
+        pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H, window=window)
+        rt.check_status()
+
+
 @pytest.mark.gpu
 def test_gpu_pages_behind_four_gigabytes():
     """Pages whose bytes lie behind 2^32 of each pool: the results and the pages of a small pool."""
