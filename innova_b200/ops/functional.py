@@ -11,6 +11,7 @@ import struct
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from .. import _native
 from . import runtime as rt
@@ -396,7 +397,7 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
     pass over qkv [..., S, (n_q + 2 n_kv) * head_dim]; the value heads are carried over. Returns a new tensor. The tables [positions, pairs] may turn
     the first 2 * pairs values of a head only, or be None for norms alone. ``positions``: one per token, inside the tables (on a GPU one outside takes
     the nearest row and ``check_status`` raises); None: 0 to S - 1. bf16 or fp32, weights in the same type; differentiable in qkv and the weights,
-    whose gradients are summed in an order that the sizes alone decide. On a GPU head_dim and the rotated values are multiples of 16, head_dim at
+    whose gradients are summed in an order that the sizes alone decide (in forward mode on the CPU alone: a GPU refuses tangents). On a GPU head_dim and the rotated values are multiples of 16, head_dim at
     most 256."""
     shape, dtype, width = qkv.shape, qkv.dtype, (n_q_heads + 2 * n_kv_heads) * head_dim
     if len(shape) < 2 or shape[-1] != width or n_q_heads < 1 or n_kv_heads < 1 or head_dim < 1:
@@ -433,7 +434,8 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
     cos, sin = _weights16(cos, sin)
     spec = (cos, sin, positions, rot, rows, tokens, width, max(S, 1), n_q_heads, n_kv_heads, head_dim, float(eps))
     with rt.device_of(qkv):
-        if torch.is_grad_enabled() and (qkv.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
+        # inside a forward-mode level too: the function refuses tangents, which the entry alone would drop
+        if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (qkv.requires_grad or q_weight.requires_grad or k_weight.requires_grad):
             return _QkNormRopeFn.apply(qkv, q_weight, k_weight, spec)
         return _qk_norm_forward(qkv, q_weight, k_weight, spec)[0]
 

@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from innova_b200 import ops
 from innova_b200.models import DenseModel, MoEModel, TransformerConfig
@@ -112,6 +113,32 @@ def test_refusals(dev):
             call(x=x.half(), wq=wq.half(), wk=wk.half())
         with pytest.raises(ValueError):
             ops.qk_norm_rope(x[..., :8 * 8], wq[:8], wk[:8], cos[:, :4], sin[:, :4], 4, 2, 8)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_forward_mode_is_not_dropped(dev):
+    """A tangent of any input comes back right (the directional derivative that the gradients give) or is refused; without one nothing changes."""
+    x, wq, wk, dy, cos, sin = inputs(1, 5, 2, 1, 32, 16, torch.float32, dev)
+    call = lambda x, wq, wk: ops.qk_norm_rope(x, wq, wk, cos, sin, 2, 1, 32)  # noqa: E731
+    want = call(x, wq, wk)
+    assert not want.requires_grad
+    for which in range(3):
+        args = [x, wq, wk]
+        tangent = torch.randn(args[which].shape, generator=torch.Generator().manual_seed(which)).to(dev)
+        alone = lambda t: call(*[t if i == which else a for i, a in enumerate(args)])  # noqa: E731
+        if dev == "cpu":
+            got = torch.func.jvp(alone, (args[which],), (tangent,))[1]
+            leaf = args[which].clone().requires_grad_()
+            g = torch.autograd.grad(alone(leaf), leaf, dy)[0]
+            a, b = (got * dy).double().sum(), (g * tangent).double().sum()          # the same sum in two orders, of terms that lose under FLOAT
+            assert abs(a - b) <= 4 * FLOAT * float((got * dy).abs().sum() + (g * tangent).abs().sum())
+            continue
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(alone, (args[which],), (tangent,))
+        with fwd.dual_level():
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                alone(fwd.make_dual(args[which], tangent))
+            assert torch.equal(call(x, wq, wk), want)
 
 
 def tiny(cls=DenseModel, **kw):
