@@ -19,7 +19,7 @@ struct QkNorm {
   void* y;                     // forward: the result; backward: dx
   const float *cos_t, *sin_t;
   const int* pos;              // position of every token; null: t % S
-  float* part;                 // backward: sums of dw, [ctas_q, D] of the queries' norm and [the others, D] of the keys'
+  float* part;                 // backward: sums of dw, [ctas_q, D] of the queries' norm and [the others, D] of the keys'; null: not asked for
   int* status;
   int T, S, H, Hkv, D, rot, table_rows, ctas_q;
   int rounds, rounds_q;        // steps of a run (Walk); backward: of the key and value heads, of the query heads
@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(256, 2) qk_norm_bwd_kernel(const __grid_consta
     if (s.hd < normed) rg.set(g);
     if (s.in && h.has) rg.store((T*)p.y + s.tok * p.ld_y + (first + s.hd) * p.D, h);
   }
+  if (!p.part) return;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const float2 two = of_pair(dw[i / 2]);
@@ -203,7 +204,8 @@ __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restric
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, d = blockIdx.x * 32 + lane;
   wait_previous();
   release_next();
-  const int r0 = blockIdx.y ? rows_q : 0, r1 = blockIdx.y ? rows : rows_q;
+  const int r0 = blockIdx.y ? rows_q : 0, r1 = blockIdx.y ? rows : rows_q, mode = blockIdx.y ? mode_k : mode_q;
+  if (mode == 3) return;
   float v = 0.f;
   if (d < D) {
 #pragma unroll 8
@@ -216,7 +218,6 @@ __global__ void __launch_bounds__(1024) qk_norm_dw_kernel(const float* __restric
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   const int col = blockIdx.x * 32 + warp;
   if (lane || col >= D) return;
-  const int mode = blockIdx.y ? mode_k : mode_q;
   void* out = blockIdx.y ? dwk : dwq;
   if (mode == 2) ((float*)out)[col] += v;
   else if (mode == 1) ((float*)out)[col] = v;
@@ -256,8 +257,8 @@ struct QkNormDesc {
   void* stream;
   // backward
   const void* dy;
-  void *dwq, *dwk;                 // [D]; mode 0: bf16, written; 1: fp32, written; 2: fp32, added to
-  float* part;                     // 296 rows of [D]
+  void *dwq, *dwk;                 // [D]; mode 0: bf16, written; 1: fp32, written; 2: fp32, added to; 3: not asked for
+  float* part;                     // 296 rows of [D], or null with both modes 3
   long ld_x, ld_y, ld_dy, table_rows, T, S, H, Hkv, D, rot, f32, mode_q, mode_k;
   double eps;
 };
@@ -311,6 +312,8 @@ extern "C" int inv_qk_norm_fwd(const QkNormDesc* d) {
 extern "C" int inv_qk_norm_bwd(const QkNormDesc* d) {
   QkNorm p;
   if (int rc = qk_norm_args(*d, p)) return rc;
+  const bool sums = d->mode_q != 3 || d->mode_k != 3;
+  if (sums != (p.part != nullptr)) return -ERR_BAD_ARG;
   cudaStream_t st = (cudaStream_t)d->stream;
   unsigned grid = 0;
   if (p.T > 0) {
@@ -324,8 +327,9 @@ extern "C" int inv_qk_norm_bwd(const QkNormDesc* d) {
     grid = (unsigned)cut.ctas;
     if (d->f32) { INV_QK_L(float, qk_bwd) } else { INV_QK_L(__nv_bfloat16, qk_bwd) }
   }
-  launch_early(qk_norm_dw_kernel, dim3((p.D + 31) / 32, 2), 1024, 0, st, (const float*)p.part, p.ctas_q, (int)grid, p.D, d->dwq, d->dwk, (int)d->mode_q,
-               (int)d->mode_k);
+  if (sums)
+    launch_early(qk_norm_dw_kernel, dim3((p.D + 31) / 32, 2), 1024, 0, st, (const float*)p.part, p.ctas_q, (int)grid, p.D, d->dwq, d->dwk, (int)d->mode_q,
+                 (int)d->mode_k);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }

@@ -360,6 +360,16 @@ def _qk_norm_forward(qkv, wq, wk, spec):
     return y, x, ld, sizes
 
 
+def _qk_weight_grad(w, mg, wanted):
+    """(what autograd gets, where the entry leaves the gradient and how: 0 bf16 and 1 fp32 written, 2 added to the fp32 ``mg``, 3 not asked for)."""
+    if not wanted:
+        return None, 0, 3
+    if mg is not None:
+        return None, mg.data_ptr(), 2
+    g = torch.empty_like(w, memory_format=torch.contiguous_format)
+    return g, g.data_ptr(), int(g.dtype is torch.float32)
+
+
 class _QkNormRopeFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, wq, wk, spec):
@@ -372,24 +382,26 @@ class _QkNormRopeFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, wq, wk, cos, sin, positions = ctx.saved_tensors
+        want_x, want_q, want_k = ctx.needs_input_grad[:3]
         d, ld = _dense_rows(dy, ctx.width)
         a, b = _weights16(wq, wk)
         dx = torch.empty_like(dy, memory_format=torch.contiguous_format)
-        part = torch.empty(_QK_ROWS * ctx.sizes[5], dtype=torch.float32, device=x.device)
-        mg_q, mg_k = main_grad_of(wq, ctx.main_grads[0]), main_grad_of(wk, ctx.main_grads[1])
+        part = torch.empty(_QK_ROWS * ctx.sizes[5], dtype=torch.float32, device=x.device) if want_q or want_k else None
+        mg_q = main_grad_of(wq, ctx.main_grads[0]) if want_q else None
+        mg_k = main_grad_of(wk, ctx.main_grads[1]) if want_k else None
         shared = None
         if mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr():     # one weight for both norms: added one after the other
             shared = mg_k = torch.zeros_like(mg_q)
-        gq, gk = (None if mg is not None else torch.empty_like(w, memory_format=torch.contiguous_format) for w, mg in ((wq, mg_q), (wk, mg_k)))
-        to_q, mode_q = (gq.data_ptr(), int(gq.dtype is torch.float32)) if mg_q is None else (mg_q.data_ptr(), 2)
-        to_k, mode_k = (gk.data_ptr(), int(gk.dtype is torch.float32)) if mg_k is None else (mg_k.data_ptr(), 2)
+        gq, to_q, mode_q = _qk_weight_grad(wq, mg_q, want_q)
+        gk, to_k, mode_k = _qk_weight_grad(wk, mg_k, want_k)
         rt.check(rt.lib().inv_qk_norm_bwd(_QK_PACK(x.data_ptr(), dx.data_ptr(), a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rt.ptr(positions),
-                                                   rt.status_ptr(x), rt.stream_ptr(), d.data_ptr(), to_q, to_k, part.data_ptr(), ctx.ld, ctx.width, ld,
+                                                   rt.status_ptr(x), rt.stream_ptr(), d.data_ptr(), to_q, to_k, rt.ptr(part), ctx.ld, ctx.width, ld,
                                                    *ctx.sizes, mode_q, mode_k, ctx.eps)), "inv_qk_norm_bwd")
-        rt.count_launches(1)
+        if part is not None:
+            rt.count_launches(1)
         if shared is not None:
             mg_q.add_(shared)
-        return dx, gq, gk, None
+        return dx if want_x else None, gq, gk, None
 
 
 def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_dim, positions=None, eps=1e-6):

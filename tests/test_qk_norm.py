@@ -255,6 +255,29 @@ def test_gpu_gradients_repeat_and_go_to_main_grads():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("wants", [(1, 0, 0), (1, 1, 0), (1, 0, 1), (0, 1, 1), (0, 1, 0), (0, 0, 1)])
+def test_gpu_gradients_that_nobody_asked_for(wants):
+    """A frozen input gets none and a frozen weight's main_grad is left alone; the others' are the same to the bit, and frozen norms save their launch."""
+    x, wq, wk, dy, cos, sin = inputs(3, 50, 8, 4, 64, 64, torch.bfloat16, DEV)
+    full = [t.clone().requires_grad_() for t in (x, wq, wk)]
+    ops.qk_norm_rope(*full, cos, sin, 8, 4, 64).backward(dy)
+    for with_main in (False, True):
+        some = [t.clone().requires_grad_(bool(w)) for t, w in zip((x, wq, wk), wants)]
+        if with_main:
+            for w in some[1:]:
+                w.main_grad = torch.ones(64, device=DEV)
+        before = rt.launch_count()
+        ops.qk_norm_rope(*some, cos, sin, 8, 4, 64).backward(dy)
+        assert rt.launch_count() - before == (3 if wants[1] or wants[2] else 2)
+        for i, (t, f, w) in enumerate(zip(some, full, wants)):
+            if with_main and i:
+                assert t.grad is None
+                assert torch.allclose(t.main_grad - 1, f.grad.float(), rtol=2.0 ** -7, atol=1e-3) if w else bool((t.main_grad == 1).all())
+            else:
+                assert torch.equal(t.grad, f.grad) if w else t.grad is None
+
+
+@pytest.mark.gpu
 def test_gpu_captured_forward_and_backward():
     x, wq, wk, dy, cos, sin = inputs(2, 50, 4, 2, 128, 128, torch.bfloat16, DEV)
     leaves = [t.clone().requires_grad_() for t in (x, wq, wk)]
