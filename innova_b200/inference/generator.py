@@ -89,10 +89,12 @@ class Generator:
                     cache.commit(batch_ids, [s + S for s in start])
                 x = self._after_attention(blk, x, cache.attend(li, q, packed, H, scale).view(B, S, -1))
                 continue
+            if packed is not None:                         # before the rotation, which rounds: a prompt and a portion store the same
+                flat, (_, k_weight, eps) = qkv.reshape(B * S, -1), blk.attention.head_norms()
+                cache.append_keys(li, flat[:, H * D:(H + Hkv) * D], flat[:, (H + Hkv) * D:], packed, rope, None, k_weight, eps)
             qkv = blk.attention.turn(qkv, rope, pos32)
-            k = qkv[..., H * D:(H + Hkv) * D]
-            v = qkv[..., (H + Hkv) * D:]
-            cache.append(li, k, v, batch_ids, start, packed)
+            if packed is None:
+                cache.append(li, qkv[..., H * D:(H + Hkv) * D], qkv[..., (H + Hkv) * D:], batch_ids, start)
             if prefill:
                 a = ops.flash_attention(qkv.contiguous(), H, Hkv, D, causal=True)
             else:

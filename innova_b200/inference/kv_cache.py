@@ -201,6 +201,12 @@ class PagedKVCache(PagedRows):
         cos, sin = rope if rope is not None else (None, None)
         return paged_fp8.qkv_append(qkv, num_heads, self.Hkv, self.D, self.pages[layer], self.page_table, new, cos, sin, positions, q_weight, k_weight, eps)
 
+    def append_keys(self, layer: int, k: torch.Tensor, v: torch.Tensor, new: paged_fp8.NewTokens, rope=None, positions=None, k_weight=None,
+                    eps: float = 1e-6):
+        """``append_rope`` of keys and values [T, kv_heads * D] alone: the pages get the same, to the bit."""
+        cos, sin = rope if rope is not None else (None, None)
+        paged_fp8.kv_append(k, v, self.pages[layer], self.page_table, new, cos, sin, positions, k_weight, eps)
+
     def attend(self, layer: int, q: torch.Tensor, new: paged_fp8.NewTokens, num_heads: int, scale: float, window: int = 0,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of the step's tokens, which are in the pages, over their sequences. q [T, num_heads * D] -> the same shape."""
@@ -210,7 +216,7 @@ class PagedKVCache(PagedRows):
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor, batch_ids: List[int], start: List[int],
                new: Optional[paged_fp8.NewTokens] = None):
         """k, v: [B, S_new, Hkv*D] views (token-major, unit inner stride) for the listed sequences. ``new``: the step's, where the cache is fp8 and it
-        is made already."""
+        is made already. An fp8 cache that is given keys rounded after their rotation rounds them again: ``append_keys`` rotates them itself."""
         B, S_new = k.shape[0], k.shape[1]
         if self.fmt == "fp8":
             k, v = (x.reshape(B * S_new, x.shape[-1]) for x in (k, v))

@@ -191,6 +191,28 @@ def _places(new: NewTokens, page_table, pages: int, T: int, window: int = 0):
         yield cu[i], n, start, ids
 
 
+def _check_weights(x, dim, *weights):
+    for w in weights:
+        if w is not None and (w.shape != (dim,) or w.dtype is not x.dtype or w.get_device() != x.get_device()):
+            raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {x.dtype} heads of {dim} on {x.device}")
+
+
+def _check_positions(positions, x):
+    if positions is not None and (positions.dtype != _int32 or positions.numel() != x.shape[0] or not positions.is_contiguous()
+                                  or positions.device != x.device):
+        raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)}: contiguous int32, one for each of {x.shape[0]} tokens")
+
+
+def _angles(cos, sin, positions, t0: int, m: int, start: int):
+    """Cosines and sines [m, 1, pairs] of tokens [t0, t0 + m), on the CPU."""
+    if cos is None:
+        return None, None
+    pos = torch.arange(start, start + m) if positions is None else positions[t0:t0 + m].long()
+    if not (0 <= int(pos.min()) and int(pos.max()) < cos.shape[0]):
+        raise ValueError(f"a position outside the tables of {cos.shape[0]}")
+    return cos[pos].unsqueeze(1), sin[pos].unsqueeze(1)
+
+
 def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_table, new: NewTokens, cos=None, sin=None, positions=None, q_weight=None,
                k_weight=None, eps: float = 1e-6, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """qkv [T, (heads + 2 kv_heads) * dim]: packed tokens from the fused projection, bias included. Query and key heads are normed (``q_weight`` and
@@ -204,25 +226,17 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
         raise ValueError(f"qkv of {tuple(qkv.shape)} for {heads} query and {kv_heads} key heads of {dim} on pages of {D}")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("norm weights of queries and keys, both or neither")
-    for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (D,) or w.dtype is not qkv.dtype or w.get_device() != qkv.get_device()):
-            raise ValueError(f"head norm weight {w.dtype} {tuple(w.shape)} on {w.device} for {qkv.dtype} heads of {D} on {qkv.device}")
+    _check_weights(qkv, D, q_weight, k_weight)
     rot = check_rope(cos, sin, D, qkv.device)
     n = _check_new(new, qkv)
-    if positions is not None and (positions.dtype != torch.int32 or positions.numel() != T or not positions.is_contiguous() or positions.device != qkv.device):
-        raise ValueError(f"positions {positions.dtype} {tuple(positions.shape)}: contiguous int32, one for each of {T} tokens")
+    _check_positions(positions, qkv)
     q_out, to, ld_q = _result(q_out, qkv, T, heads * D)
     if not qkv.is_cuda:
         x = qkv.float().view(T, heads + 2 * G, D)
         for t0, m, start, ids in _places(new, page_table, N, T):
             if not m:
                 continue
-            pos = torch.arange(start, start + m) if positions is None else positions[t0:t0 + m].long()
-            c = s = None
-            if rot:
-                if not (0 <= int(pos.min()) and int(pos.max()) < cos.shape[0]):
-                    raise ValueError(f"a position outside the tables of {cos.shape[0]}")
-                c, s = cos[pos].unsqueeze(1), sin[pos].unsqueeze(1)
+            c, s = _angles(cos, sin, positions, t0, m, start)
             part = x[t0:t0 + m]
             q_out[t0:t0 + m] = _head_norm_rope(part[:, :heads], q_weight, eps, c, s).reshape(m, -1).to(qkv.dtype)
             k, v = _head_norm_rope(part[:, heads:heads + G], k_weight, eps, c, s), part[:, heads + G:]
@@ -244,24 +258,35 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
     return q_out if to is q_out else q_out.copy_(to)
 
 
-def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens):
-    """Keys and values [T, kv_heads * dim] of packed tokens, as they are, into the pages: ``qkv_append`` for heads that were normed and rotated before."""
+def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens, cos=None, sin=None, positions=None, k_weight=None, eps: float = 1e-6):
+    """Keys and values [T, kv_heads * dim] of packed tokens into the pages: ``qkv_append`` without queries, for those who norm and rotate them elsewhere.
+    Key heads are normed with ``k_weight`` and rotated by the tables as there, and what is stored is the same to the bit; with neither they are stored as
+    they are."""
     N, G, D = _check(k, "k", 1 if pages.k.dim() != 4 else pages.k.shape[1], pages, page_table)
     T = k.shape[0]
     if k.shape[1] != G * D or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device or v.stride(1) != 1:
         raise ValueError(f"k of {k.dtype} {tuple(k.shape)}, v of {v.dtype} {tuple(v.shape)} for {G} heads of {D}")
+    _check_weights(k, D, k_weight)
+    rot = check_rope(cos, sin, D, k.device)
     n = _check_new(new, k)
+    _check_positions(positions, k)
     if not k.is_cuda:
         for t0, m, start, ids in _places(new, page_table, N, T):
-            _write_tokens(k[t0:t0 + m].float().view(m, G, D), v[t0:t0 + m].float().view(m, G, D), pages, ids, start)
+            if m:
+                c, s = _angles(cos, sin, positions, t0, m, start)
+                keys = _head_norm_rope(k[t0:t0 + m].float().view(m, G, D), k_weight, eps, c, s)
+                _write_tokens(keys, v[t0:t0 + m].float().view(m, G, D), pages, ids, start)
         return
+    if rot % 16:
+        raise ValueError(f"{rot} rotated values: a multiple of 16 on a GPU")
     if T == 0 or n == 0:
         return
     (k, ld), (v, ld_v) = _aligned(k), _aligned(v)
+    k_weight, cos, sin = _weights16(k_weight, cos, sin)
     with rt.device_of(k):
-        rt.check(rt.lib().inv_fp8_append(_APPEND(0, k.data_ptr(), v.data_ptr(), 0, 0, 0, 0, 0, 0,
+        rt.check(rt.lib().inv_fp8_append(_APPEND(0, k.data_ptr(), v.data_ptr(), 0, 0, rt.ptr(k_weight), rt.ptr(cos), rt.ptr(sin), rt.ptr(positions),
                                                  *_where(pages, page_table, new.rows.data_ptr(), new.cu.data_ptr(), new.start.data_ptr()),
-                                                 0, G, D, N, *page_table.shape, n, T, ld, ld_v, 0, 0, 0, 0.0)), "inv_fp8_append")
+                                                 0, G, D, N, *page_table.shape, n, T, ld, ld_v, 0, cos.shape[0] if rot else 0, rot, eps)), "inv_fp8_append")
 
 
 def read(pages: Fp8Pages, ids: torch.Tensor, length: int):

@@ -489,6 +489,51 @@ def test_append_in_portions_reads_the_same(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("H, G, D, rot, norm, given", [(4, 2, 64, 64, True, False), (8, 1, 128, 32, False, False), (3, 3, 64, 0, True, False),
+                                                       (6, 2, 128, 128, True, True)])
+def test_keys_alone_are_stored_as_with_their_queries(H, G, D, rot, norm, given, dev):
+    """``kv_append`` norms and rotates as ``qkv_append`` does; ragged portions behind cached tokens."""
+    ctx, new = [0, 21, 500, 16], [40, 1, 19, 0]
+    s = Setup([a + b for a, b in zip(ctx, new)], [0] * 4, H, G, D, dev)
+    tokens = pf.NewTokens(i32(s.owner, dev), i32([0, 40, 41, 60, 60], dev), i32(ctx, dev), 40, 520)
+    g = torch.Generator().manual_seed(2)
+    qkv = torch.randn(60, (H + 2 * G) * D, generator=g).to(dtype_of(dev)).to(dev)
+    cos, sin = ops.rope_tables(600, rot, device=dev) if rot else (None, None)
+    w = (1 + 0.3 * torch.randn(D, generator=g)).to(qkv.dtype).to(dev) if norm else None
+    pos = torch.randint(0, 600, (60,), generator=g).int().to(dev) if given else None
+    other = pf.Fp8Pages(*(x.clone() for x in s.pool))
+    pf.qkv_append(qkv, H, G, D, s.pool, s.page_table, tokens, cos, sin, pos, w, w)
+    pf.kv_append(qkv[:, H * D:(H + G) * D], qkv[:, (H + G) * D:], other, s.page_table, tokens, cos, sin, pos, w)
+    for a, b in zip(s.pool, other):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    k = qkv[:, :G * D]
+    for bad in (dict(cos=torch.ones(9, 8, device=dev)), dict(k_weight=torch.ones(D - 1, device=dev)), dict(k_weight=torch.ones(D, device=dev).double()),
+                dict(positions=i32([0], dev)), dict(positions=torch.zeros(60, device=dev, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            pf.kv_append(k, k, other, s.page_table, tokens, **bad)
+    if dev == "cuda":
+        rt.check_status()
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("kw", [{}, dict(qk_norm=False)])
+def test_prompt_and_portions_store_the_same(kw, dev):
+    """In bf16, keys with norms and rotation: what a first prompt leaves in the pages is what portions leave. A projection that takes the tokens one at a
+    time gives each the same row in both."""
+    torch.manual_seed(0)
+    m = DenseModel(tiny(num_layers=1, **kw), dtype=torch.bfloat16, device=dev).eval()
+    rows = lambda x, lin: torch.stack([lin.weight @ r for r in x.reshape(-1, x.shape[-1])]).view(*x.shape[:-1], -1)  # noqa: E731
+    ids = torch.randint(0, 300, (2, 37), device=dev)
+    pools = []
+    for cuts in ([0, 37], [0, 1, 5, 30, 37]):
+        gen = Generator(m, kv_format="fp8", max_batch=2, max_seq=64, linear_fn=rows)
+        for a, b in zip(cuts, cuts[1:]):
+            gen._forward(ids[:, a:b], [a, a])
+        pools.append([x for b in range(2) for x in gen.cache.gather(0, b)])
+    assert all(torch.equal(x, y) for x, y in zip(*pools))
+
+
+@pytest.mark.parametrize("dev", DEVS)
 def test_append_values_at_the_edges(dev):
     """Zeros, values below the smallest scale, the largest ones, infinities and NaN; a page starts over with its first slot."""
     D, table = 64, torch.zeros(1, 1, dtype=torch.int32, device=dev)
