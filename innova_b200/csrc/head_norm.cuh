@@ -5,9 +5,8 @@
 // u * 8 and its partner rot / 2 + u * 8, so that every pair of the rotation sits in one thread; behind it units are simply sixteen values in a row. A
 // head takes the next power of two of lanes, of which D / 16 have a unit.
 #pragma once
+#include "once_per_device.h"
 #include "sm100_common.cuh"
-
-#include <atomic>
 
 namespace inv {
 
@@ -213,15 +212,15 @@ __device__ __forceinline__ int table_row(int pos, int rows, int* status) {
   return pos < 0 ? 0 : rows - 1;
 }
 
-// The kernel's shared memory on the current device, asked for once.
+// The kernel's shared memory on the current device. 0, or the entry's error code.
 template <typename K>
-static void raise_smem(K* kernel, int bytes, std::atomic<uint64_t>& ready) {
+static int raise_smem(K* kernel, int bytes, OncePerDevice& ready) {
   int device = 0;
-  cudaGetDevice(&device);
-  const uint64_t bit = 1ull << (device & 63);
-  if (ready.load() & bit) return;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  ready.fetch_or(bit);
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess)
+    e = (cudaError_t)ready.ask(device, [&] { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+  if (e != cudaSuccess) cudaGetLastError();          // returned here, not by the next entry that asks
+  return -(int)e;
 }
 
 }  // namespace inv

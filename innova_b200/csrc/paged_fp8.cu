@@ -1407,15 +1407,15 @@ static int fp8_attend_join(const Fp8Attend& a, const Fp8Tokens& tk, int tile_row
 template <int D, int NR, int NW, bool TREE, int ST = 2>
 static int fp8_attend_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
   constexpr int SMEM = fp8_attend_smem<D, NW, ST>();
-  static std::atomic<uint64_t> ready{0};
-  raise_smem(fp8_attend_kernel<D, NR, NW, TREE, ST>, SMEM, ready);
+  static OncePerDevice ready;
+  if (int rc = raise_smem(fp8_attend_kernel<D, NR, NW, TREE, ST>, SMEM, ready)) return rc;
   launch_early(fp8_attend_kernel<D, NR, NW, TREE, ST>, dim3(ctas), NW * 32, SMEM, st, a, pool, tk);
   return fp8_attend_join<D>(a, tk, 8 * NR, st);
 }
 template <int D>
 static int fp8_attend_tile_launch(const Fp8Attend& a, const Fp8Pool& pool, const Fp8Tokens& tk, unsigned ctas, cudaStream_t st) {
-  static std::atomic<uint64_t> ready{0};
-  raise_smem(fp8_attend_tile_kernel<D>, FtSmem<D>::TOTAL, ready);
+  static OncePerDevice ready;
+  if (int rc = raise_smem(fp8_attend_tile_kernel<D>, FtSmem<D>::TOTAL, ready)) return rc;
   launch_early(fp8_attend_tile_kernel<D>, dim3(ctas), FT_THREADS, FtSmem<D>::TOTAL, st, a, pool, tk);
   return fp8_attend_join<D>(a, tk, FT_ROWS, st);
 }

@@ -275,25 +275,36 @@ static int qk_norm_args(const QkNormDesc& d, QkNorm& p) {
   return 0;
 }
 template <typename T, int L>
-static void qk_fwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
-  static std::atomic<uint64_t> ready{0};
-  raise_smem(qk_norm_fwd_kernel<T, L>, QkFwdRing<T>::BYTES, ready);
+static int qk_fwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
+  static OncePerDevice ready;
+  if (int rc = raise_smem(qk_norm_fwd_kernel<T, L>, QkFwdRing<T>::BYTES, ready)) return rc;
   launch_early(qk_norm_fwd_kernel<T, L>, grid, 256, QkFwdRing<T>::BYTES, st, p);
+  return 0;
 }
 template <typename T, int L>
-static void qk_bwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
-  static std::atomic<uint64_t> ready{0};
-  raise_smem(qk_norm_bwd_kernel<T, L>, QkBwdRing<T>::BYTES, ready);
+static int qk_bwd(const QkNorm& p, unsigned grid, cudaStream_t st) {
+  static OncePerDevice ready;
+  if (int rc = raise_smem(qk_norm_bwd_kernel<T, L>, QkBwdRing<T>::BYTES, ready)) return rc;
   launch_early(qk_norm_bwd_kernel<T, L>, grid, 256, QkBwdRing<T>::BYTES, st, p);
+  return 0;
 }
-#define INV_QK_L(T, LAUNCH)                       \
-  switch (head_lanes(p.D)) {                      \
-    case 1: LAUNCH<T, 1>(p, grid, st); break;     \
-    case 2: LAUNCH<T, 2>(p, grid, st); break;     \
-    case 4: LAUNCH<T, 4>(p, grid, st); break;     \
-    case 8: LAUNCH<T, 8>(p, grid, st); break;     \
-    default: LAUNCH<T, 16>(p, grid, st);          \
+#define INV_QK_L(T, LAUNCH)                    \
+  switch (head_lanes(p.D)) {                   \
+    case 1: return LAUNCH<T, 1>(p, grid, st);  \
+    case 2: return LAUNCH<T, 2>(p, grid, st);  \
+    case 4: return LAUNCH<T, 4>(p, grid, st);  \
+    case 8: return LAUNCH<T, 8>(p, grid, st);  \
+    default: return LAUNCH<T, 16>(p, grid, st); \
   }
+static int qk_fwd(const QkNorm& p, bool f32, unsigned grid, cudaStream_t st) {
+  if (f32) INV_QK_L(float, qk_fwd)
+  INV_QK_L(__nv_bfloat16, qk_fwd)
+}
+static int qk_bwd(const QkNorm& p, bool f32, unsigned grid, cudaStream_t st) {
+  if (f32) INV_QK_L(float, qk_bwd)
+  INV_QK_L(__nv_bfloat16, qk_bwd)
+}
+#undef INV_QK_L
 
 extern "C" int inv_qk_norm_fwd(const QkNormDesc* d) {
   QkNorm p;
@@ -304,7 +315,7 @@ extern "C" int inv_qk_norm_fwd(const QkNormDesc* d) {
   const unsigned grid = (unsigned)qk_ctas(p.T, slots, hpw, 148 * QK_FWD_CTAS);
   p.rounds = qk_rounds(p.T, slots, hpw, grid);
   cudaStream_t st = (cudaStream_t)d->stream;
-  if (d->f32) { INV_QK_L(float, qk_fwd) } else { INV_QK_L(__nv_bfloat16, qk_fwd) }
+  if (int rc = qk_fwd(p, d->f32 != 0, grid, st)) return rc;
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : -(int)e;
 }
@@ -325,7 +336,7 @@ extern "C" int inv_qk_norm_bwd(const QkNormDesc* d) {
     p.rounds = qk_rounds(p.T, 2 * p.Hkv, hpw, cut.ctas - cut.ctas_q);
     p.ctas_q = cut.ctas_q;
     grid = (unsigned)cut.ctas;
-    if (d->f32) { INV_QK_L(float, qk_bwd) } else { INV_QK_L(__nv_bfloat16, qk_bwd) }
+    if (int rc = qk_bwd(p, d->f32 != 0, grid, st)) return rc;
   }
   if (sums)
     launch_early(qk_norm_dw_kernel, dim3((p.D + 31) / 32, 2), 1024, 0, st, (const float*)p.part, p.ctas_q, (int)grid, p.D, d->dwq, d->dwk, (int)d->mode_q,

@@ -27,7 +27,7 @@ _native.register_cuda_sigs({"inv_fp8_append": [_native.vp], "inv_fp8_attend": [_
 _APPEND = struct.Struct("=9Q 10Q 8q 5q d").pack
 _ATTEND = struct.Struct("=7Q 10Q 8q 6q d").pack
 
-PAGE, TOP, MIN_EXP = 16, 448.0, -64
+PAGE, MIN_EXP = 16, -64
 _e4m3, _fp32, _bf16, _int32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int32
 
 
@@ -141,7 +141,7 @@ def _result(out, x, rows, width):
 
 def scale_of(amax: torch.Tensor) -> torch.Tensor:
     """The scale of pages with these largest values."""
-    m, e = torch.frexp(amax.float())                           # amax = m 2^e, m in [1/2, 1); 448 = 7/8 2^9
+    m, e = torch.frexp(amax.float())                           # amax = m 2^e, m in [1/2, 1); the largest code is 448 = 7/8 2^9
     e = torch.where(m == 0, MIN_EXP, torch.where(m > 0.875, e - 8, e - 9)).clamp(MIN_EXP, 120)
     return torch.where(torch.isfinite(amax), torch.ldexp(torch.ones_like(m), e), torch.nan)
 
