@@ -432,7 +432,7 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
             if tokens and not (0 <= int(pos.min()) and int(pos.max()) < cos.shape[0]):
                 raise ValueError(f"a position outside the tables of {cos.shape[0]}")
             c, s = cos[pos].unsqueeze(1), sin[pos].unsqueeze(1)
-        x = qkv.reshape(tokens, -1, head_dim)
+        x = qkv.reshape(tokens, n_q_heads + 2 * n_kv_heads, head_dim)
         x = x if x.dtype == torch.float64 else x.float()
         q, k, v = x.split([n_q_heads, n_kv_heads, n_kv_heads], dim=1)
         y = torch.cat([_head_norm_rope(q, q_weight, eps, c, s), _head_norm_rope(k, k_weight, eps, c, s), v], dim=1)

@@ -93,6 +93,14 @@ def test_cpu_gradients_against_differences():
     assert torch.autograd.gradcheck(lambda *a: ops.qk_norm_rope(*a, cos, sin, 3, 1, 16), leaves)
 
 
+@pytest.mark.parametrize("shape", [(2, 0, 512), (0, 3, 512), (0, 512)])
+def test_cpu_no_tokens(shape):
+    cos, sin = ops.rope_tables(9, 64)
+    x, w = torch.zeros(shape), torch.ones(64, requires_grad=True)
+    y = ops.qk_norm_rope(x, w, torch.ones(64), cos, sin, 4, 2, 64)
+    assert y.shape == shape and float(torch.autograd.grad(y.sum(), w)[0].abs().sum()) == 0
+
+
 @pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
 def test_refusals(dev):
     x, wq, wk, _, cos, sin = inputs(2, 5, 4, 2, 64, 64, torch.float32 if dev == "cpu" else torch.bfloat16, dev)
