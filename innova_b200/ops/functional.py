@@ -442,6 +442,8 @@ def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_
     if head_dim % 16 or head_dim > 256 or rot % 16:
         raise ValueError(f"heads of {head_dim} with {rot} rotated values: multiples of 16 up to 256 on a GPU")
     if positions is not None:
+        if positions.dtype is torch.int64:               # what 32 bits cannot say is outside every table all the same
+            positions = positions.clamp(-1, 2 ** 31 - 1)
         positions = positions.reshape(-1).to(torch.int32).contiguous()
     cos, sin = _weights16(cos, sin)
     spec = (cos, sin, positions, rot, rows, tokens, width, max(S, 1), n_q_heads, n_kv_heads, head_dim, float(eps))

@@ -241,6 +241,17 @@ def test_gpu_position_outside_the_table_is_reported():
 
 
 @pytest.mark.gpu
+def test_gpu_positions_of_64_bits_are_not_cut():
+    x, wq, wk, _, cos, sin = inputs(1, 4, 2, 1, 64, 64, torch.bfloat16, DEV)
+    pos = torch.tensor([0, 3, 2 ** 32 + 2, -2 ** 32 + 1], device=DEV)
+    y = ops.qk_norm_rope(x, wq, wk, cos, sin, 2, 1, 64, pos)
+    with pytest.raises(RuntimeError):
+        rt.check_status()
+    assert torch.equal(y, ops.qk_norm_rope(x, wq, wk, cos, sin, 2, 1, 64, pos.clamp(0, cos.shape[0] - 1)))
+    rt.check_status()
+
+
+@pytest.mark.gpu
 def test_gpu_gradients_repeat_and_go_to_main_grads():
     x, wq, wk, dy, cos, sin = inputs(3, 500, 8, 4, 64, 64, torch.bfloat16, DEV)
     leaves = [t.clone().requires_grad_() for t in (x, wq, wk)]
