@@ -192,15 +192,16 @@ struct Turn {
       s[2 * i + 1] = pair_of(b.z, b.w);
     }
   }
-  // (x1, x2) -> (x1 c - x2 s, x1 s + x2 c); INV: by the transpose. Products are rounded by themselves, as written.
+  // (x1, x2) -> (x1 c - x2 s, x1 s + x2 c); INV: by the transpose. The products with x2 are rounded, those with x1 enter the sum as they are. Said here,
+  // since a packed product and a sum behind it are made one instruction by the assembler in any case, whatever rounding they name.
   template <bool INV>
   __device__ __forceinline__ void apply(const HeadUnit& h, uint64_t (&x)[8]) const {
     if (!h.turns) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint64_t a = x[i], b = x[i + 4], minus = 0x8000000080000000ull;
-      x[i] = add_pair(mul_pair(a, c[i]), mul_pair(INV ? b : b ^ minus, s[i]));
-      x[i + 4] = add_pair(mul_pair(INV ? a ^ minus : a, s[i]), mul_pair(b, c[i]));
+      x[i] = fma_pair(a, c[i], mul_pair(INV ? b : b ^ minus, s[i]));
+      x[i + 4] = fma_pair(INV ? a ^ minus : a, s[i], mul_pair(b, c[i]));
     }
   }
 };

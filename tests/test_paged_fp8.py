@@ -566,6 +566,20 @@ def test_append_values_at_the_edges(dev):
     assert put(0, 3.0) == (2.0 ** -7, [3.0])                                          # ... until it starts over
 
 
+@pytest.mark.gpu
+def test_gpu_rotation_rounds_one_product_of_two():
+    """(a c - b s, a s + b c) with both products of the size p = 1 + 2^-7 + 2^-23: (1 + 2^-7) (1 + 2^-23) is p + 2^-30, which fp32 rounds to p. The product with
+    a keeps the rest, that with b loses it."""
+    D, p, near, step = 64, 1 + 2.0 ** -7 + 2.0 ** -23, 1 + 2.0 ** -7, 1 + 2.0 ** -23
+    pool, table = pf.new_pages(1, 1, D, "cuda"), i32([[0]], "cuda")
+    new = pf.NewTokens(i32([0], "cuda"), i32([0, 1], "cuda"), i32([0], "cuda"), 1, 1)
+    for a, c, b, s, half, want in ((near, step, 1, p, 0, 2.0 ** -30), (1, p, near, step, 0, 0.0), (near, p, -1, step, 1, 2.0 ** -30), (1, step, -near, p, 1, 0.0)):
+        qkv = torch.tensor([[a] * 32 + [b] * 32] * 3, device="cuda").view(1, -1).bfloat16()
+        cos, sin = (torch.full((1, D // 2), x, device="cuda") for x in (c, s))
+        q = pf.qkv_append(qkv, 1, 1, D, pool, table, new, cos, sin)
+        assert bool((q[0, 32 * half:32 * half + 32] == want).all())
+
+
 # ---------------------------------------------------------------------------------------------- refusals and bad tables
 @pytest.mark.parametrize("dev", DEVS)
 def test_refusals(dev):
