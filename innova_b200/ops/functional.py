@@ -315,14 +315,16 @@ def _head_norm_rope(x, weight, eps, cos, sin):
     return torch.cat([a * cos - b * sin, a * sin + b * cos, x[..., 2 * half:]], dim=-1)
 
 
+def _on16(x):
+    """Whether the rows of x [T, width] start on 16-byte boundaries."""
+    return x.data_ptr() % 16 == 0 and (x.shape[0] <= 1 or x.stride(0) * x.element_size() % 16 == 0)
+
+
 def _rows16(x, width):
-    """x as rows [T, width] that start on 16-byte boundaries: a view where it is one, else a copy."""
+    """x as rows [T, width] with unit stride that start on 16-byte boundaries: a view where it is one, else a copy."""
     if x.dim() != 2:
         x = x.reshape(-1, width)
-    row, step = x.stride()
-    if step != 1 or (x.shape[0] > 1 and row * x.element_size() % 16) or x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x
+    return x if x.stride(1) == 1 and _on16(x) else x.clone(memory_format=torch.contiguous_format)
 
 
 def _weights16(*weights):

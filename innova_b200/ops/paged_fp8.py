@@ -18,7 +18,7 @@ import torch
 
 from .. import _native
 from . import runtime as rt
-from .functional import _head_norm_rope, _weights16, check_rope
+from .functional import _dense_rows, _head_norm_rope, _ld, _on16, _weights16, check_rope
 
 _native.register_cuda_sigs({"inv_fp8_append": [_native.vp], "inv_fp8_attend": [_native.vp], "inv_fp8_attend_floats": [_native.i32] * 9})
 
@@ -108,23 +108,6 @@ def _check_new(new: NewTokens, x):
     if n and (new.max_new < 1 or new.max_len < new.max_new):
         raise ValueError(f"max_new {new.max_new}, max_len {new.max_len}")
     return n
-
-
-def _on16(x):
-    """Whether the rows of x start on 16-byte boundaries."""
-    return x.data_ptr() % 16 == 0 and (x.stride(0) % 8 == 0 or x.shape[0] <= 1)
-
-
-def _aligned(x):
-    """Rows of x on 16-byte boundaries, a copy where they are not, and how far apart they are."""
-    if not _on16(x):
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x, _ld(x)
-
-
-def _ld(x):
-    rows, width = x.shape
-    return x.stride(0) if rows > 1 else width
 
 
 def _result(out, x, rows, width):
@@ -246,7 +229,7 @@ def qkv_append(qkv, heads: int, kv_heads: int, dim: int, pages: Fp8Pages, page_t
         raise ValueError(f"{rot} rotated values: a multiple of 16 on a GPU")
     if T == 0 or n == 0:
         return q_out
-    qkv, ld = _aligned(qkv)
+    qkv, ld = _dense_rows(qkv, width)
     q_weight, k_weight, cos, sin = _weights16(q_weight, k_weight, cos, sin)
     at, size = qkv.data_ptr(), D * qkv.element_size()
     with rt.device_of(qkv):
@@ -281,7 +264,7 @@ def kv_append(k, v, pages: Fp8Pages, page_table, new: NewTokens, cos=None, sin=N
         raise ValueError(f"{rot} rotated values: a multiple of 16 on a GPU")
     if T == 0 or n == 0:
         return
-    (k, ld), (v, ld_v) = _aligned(k), _aligned(v)
+    (k, ld), (v, ld_v) = _dense_rows(k, G * D), _dense_rows(v, G * D)
     k_weight, cos, sin = _weights16(k_weight, cos, sin)
     with rt.device_of(k):
         rt.check(rt.lib().inv_fp8_append(_APPEND(0, k.data_ptr(), v.data_ptr(), 0, 0, rt.ptr(k_weight), rt.ptr(cos), rt.ptr(sin), rt.ptr(positions),
@@ -344,7 +327,7 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
         return out
     if T == 0 or n == 0:
         return out
-    q, ld = _aligned(q)
+    q, ld = _dense_rows(q, width)
     window = min(window, 2 ** 31 - 1)
     with rt.device_of(q):
         work, floats = _workspace(q.device, n, T, heads, G, D, new.max_new, new.max_len, window, 0)
@@ -382,7 +365,7 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
         return out
     if T == 0:
         return out
-    q, ld = _aligned(q)
+    q, ld = _dense_rows(q, width)
     with rt.device_of(q):
         work, floats = _workspace(q.device, T, T, heads, G, D, 1, max_len, 0, 1)
         rt.check(rt.lib().inv_fp8_attend(_ATTEND(q.data_ptr(), to.data_ptr(), rt.ptr(work), row_seq.data_ptr(), seq_lens.data_ptr(), rt.ptr(tail_start),
