@@ -342,7 +342,8 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
                 tail_mask=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rows with masks of their own: row t of q [T, heads * dim] belongs to page table row ``row_seq[t]``, which holds ``seq_lens[row_seq[t]]`` tokens,
     and sees those below ``tail_start[t]`` and token ``tail_start[t] + i``, i < 64, iff bit i of ``tail_mask[t]`` (int64) is set; all of them without a
-    tail. A row that sees nothing gives zeros. No row of the page table holds more than ``max_len`` tokens."""
+    tail. A row that sees nothing gives zeros. No row of the page table holds more than ``max_len`` tokens. On a GPU a row outside the table, or one that
+    would hold more than the table lists, gives zeros, a page outside the pool is skipped, and ``check_status`` raises."""
     N, G, D = _check(q, "q", heads, pages, page_table)
     T, width = q.shape
     if width != heads * D or max_len < 1 or (tail_start is None) != (tail_mask is None):
@@ -355,7 +356,12 @@ def tree_attend(q, pages: Fp8Pages, page_table, seq_lens, row_seq, heads: int, m
     if not q.is_cuda:
         lens, starts, masks = seq_lens.tolist(), tail_start.tolist() if tail_start is not None else None, tail_mask.tolist() if tail_mask is not None else None
         for t, row in enumerate(row_seq.tolist()):
-            k, v = read(pages, page_table[row, : -(-lens[row] // PAGE)], lens[row])
+            if not (0 <= row < page_table.shape[0] and 0 <= lens[row] <= PAGE * page_table.shape[1]):
+                raise ValueError(f"row {t} of table row {row}" + (f", which holds {lens[row]} tokens" if 0 <= row < len(lens) else f" of {len(lens)}"))
+            ids = page_table[row, : -(-lens[row] // PAGE)]
+            if lens[row] and not (0 <= int(ids.min()) and int(ids.max()) < N):
+                raise ValueError(f"row {row} lists a page outside the pool of {N}")
+            k, v = read(pages, ids, lens[row])
             j = torch.arange(lens[row])
             seen = torch.ones(lens[row], dtype=torch.bool)
             if starts is not None:

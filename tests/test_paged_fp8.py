@@ -669,6 +669,33 @@ def test_entries_outside_the_pool(dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("what", ["row behind", "row before", "length", "page", "page before"])
+def test_tree_rows_outside_the_pool(what, dev):
+    """An error on the CPU; on the GPU zeros (a skipped page: what the others give), the status word, and the other rows as they are."""
+    s = Setup([40, 33], [0, 0], 4, 2, 64, dev)
+    q = torch.randn(3, 4 * 64, device=dev).to(dtype_of(dev))
+    lens = torch.zeros(s.page_table.shape[0], dtype=torch.int32)
+    lens[s.owner[0]], lens[s.owner[1]] = 40, 33
+    rows, table = [s.owner[1], s.owner[0], s.owner[1]], s.page_table.clone()
+    want = pf.tree_attend(q, s.pool, table, lens.to(dev), i32(rows, dev), 4, 40)
+    if what.startswith("row"):
+        rows[1] = len(lens) if what == "row behind" else -1
+    elif what == "length":
+        lens[s.owner[0]] = 16 * table.shape[1] + 1
+    else:
+        table[s.owner[0], 1] = s.pages if what == "page" else -1
+    call = lambda: pf.tree_attend(q, s.pool, table, lens.to(dev), i32(rows, dev), 4, 40)  # noqa: E731
+    if dev == "cpu":
+        with pytest.raises(ValueError):
+            call()
+        return
+    got = call()
+    with pytest.raises(RuntimeError):
+        rt.check_status()
+    assert torch.equal(got[[0, 2]], want[[0, 2]]) and bool(got[1].isfinite().all()) and bool(got[1].any()) == what.startswith("page")
+
+
+@pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("ctx, new", [([5, 40], [1, 3]), ([2000, 3], [1, 1]), ([9000], [1]), ([3000, 0], [20, 0]), ([5000, 100], [70, 9]), ([0, 0], [0, 0])])
 def test_rows_of_no_sequence_stay_as_they_are(ctx, new, dev):
     """A padded batch: rows in front of the first sequence and behind the last, of calls in one part and in several."""
