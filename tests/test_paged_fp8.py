@@ -250,7 +250,7 @@ UNEVEN = [
 
 
 @pytest.mark.parametrize("dev", DEVS)
-@pytest.mark.parametrize("ratio", [-60, -40, 25, 30, 40, 60])
+@pytest.mark.parametrize("ratio", [-50, -40, 25, 30, 40, 60])
 @pytest.mark.parametrize("case", UNEVEN)
 def test_attend_pages_of_unequal_scales(case, ratio, dev):
     """Every third page holds values 2^ratio times as large, under weights down to e^-48 and less of the others': a row is right by its own sum."""
