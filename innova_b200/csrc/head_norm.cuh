@@ -204,6 +204,16 @@ struct Turn {
       x[i + 4] = fma_pair(INV ? a ^ minus : a, s[i], mul_pair(b, c[i]));
     }
   }
+  // The same with every product rounded by itself: what elementary operations give, to the bit, for values that are to be rounded to a few bits.
+  __device__ __forceinline__ void apply_apart(const HeadUnit& h, uint64_t (&x)[8]) const {
+    if (!h.turns) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = of_pair(x[i]), b = of_pair(x[i + 4]), k = of_pair(c[i]), n = of_pair(s[i]);
+      x[i] = pair_of(__fsub_rn(__fmul_rn(a.x, k.x), __fmul_rn(b.x, n.x)), __fsub_rn(__fmul_rn(a.y, k.y), __fmul_rn(b.y, n.y)));
+      x[i + 4] = pair_of(__fadd_rn(__fmul_rn(a.x, n.x), __fmul_rn(b.x, k.x)), __fadd_rn(__fmul_rn(a.y, n.y), __fmul_rn(b.y, k.y)));
+    }
+  }
 };
 
 // The table's row of a position; one outside the table is reported and takes the nearest row.

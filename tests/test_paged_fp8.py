@@ -567,6 +567,32 @@ def test_append_values_at_the_edges(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H, G, D, rot", [(8, 4, 64, 64), (4, 2, 128, 128), (6, 3, 128, 32)])
+def test_gpu_pages_are_those_of_elementary_operations(H, G, D, rot):
+    """Rotated keys, and values, of portions and scales that rise: the pages that the CPU's elementary operations leave, to the bit."""
+    g = torch.Generator().manual_seed(rot)
+    cos, sin = ops.rope_tables(3000, rot)
+    ctx, new = [0, 5, 700, 0], [1500, 60, 800, 1]
+    need = [-(-(a + b) // 16) for a, b in zip(ctx, new)]
+    table = torch.full((4, max(need)), -1, dtype=torch.int32)
+    order = torch.randperm(sum(need), generator=g).int()
+    for i, m in enumerate(need):
+        table[i, :m] = order[sum(need[:i]):sum(need[:i]) + m]
+    pools = []
+    for dev in ("cpu", "cuda"):
+        pool = pf.new_pages(sum(need), G, D, dev)
+        for seed, starts, counts in ((1, [0] * 4, ctx), (2, ctx, new)):
+            x = torch.randn(sum(counts), (H + 2 * G) * D, generator=torch.Generator().manual_seed(seed)).bfloat16().to(dev)
+            cu = [sum(counts[:i]) for i in range(5)]
+            tokens = pf.NewTokens(i32(range(4), dev), i32(cu, dev), i32(starts, dev), max(counts), 1600)
+            pf.qkv_append(x, H, G, D, pool, table.to(dev), tokens, cos.to(dev), sin.to(dev))
+        pools.append(pool)
+    for a, b in zip(*pools):
+        assert int((a.view(torch.uint8) != b.cpu().view(torch.uint8)).sum()) == 0
+    rt.check_status()
+
+
+@pytest.mark.gpu
 def test_gpu_rotation_rounds_one_product_of_two():
     """(a c - b s, a s + b c) with both products of the size p = 1 + 2^-7 + 2^-23: (1 + 2^-7) (1 + 2^-23) is p + 2^-30, which fp32 rounds to p. The product with
     a keeps the rest, that with b loses it."""
