@@ -2,9 +2,11 @@
 
 ``qkv_append`` is everything between a fused projection and the attention: norms of the query and key heads, rotation, append of keys and values to
 the pages. ``kv_attend`` is the attention of the same new tokens over all that the pages hold, one token a sequence or many, causal, with or without a
-sliding window; ``tree_attend`` that of single rows with masks of their own. ``inference.kv_cache.PagedKVCache`` with ``fmt="fp8"`` calls them.
+sliding window; ``tree_attend`` that of single rows with masks of their own. ``inference.kv_cache.PagedKVCache`` with ``fmt="fp8"`` calls them. They serve:
+on a GPU no gradient and no tangent passes through them.
 
-The scale of a page and head is the smallest power of two 2^e, at least 2^-64, with |x| <= 448 * 2^e for every token in it. Later tokens can raise it;
+The scale of a page and head is the smallest power of two 2^e, at least 2^-64, with |x| <= 448 * 2^e for every token in it, keys as they are in fp32 behind
+their norm and rotation (a first prompt and a later portion store the same; keys that were rounded before, to bf16, are rounded twice). Later tokens can raise it;
 the codes that are there are then rounded to the new scale, which changes nothing but their exponent unless they fall under 2^-6. Tokens that are taken
 back (a draft that was not accepted) leave the scale that they raised. A value that is not finite makes a page of its head read as NaN until its first slot
 is written again."""
@@ -32,7 +34,7 @@ _e4m3, _fp32, _bf16, _int32 = torch.float8_e4m3fn, torch.float32, torch.bfloat16
 
 
 class Fp8Pages(NamedTuple):
-    """The pools of one layer, contiguous."""
+    """The pools of one layer, contiguous. Scales are powers of two from 2^-64 to 2^120, NaN in a page that holds no number, 0 in one never written."""
     k: torch.Tensor          # [pages, kv_heads, 16, dim] float8_e4m3fn
     v: torch.Tensor
     k_scale: torch.Tensor    # [pages, kv_heads] fp32
