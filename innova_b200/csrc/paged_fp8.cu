@@ -283,7 +283,7 @@ struct Fp8Attend {
   int per_split;        // pages of a CTA
   int splits, tiles;
   uint32_t inv_tiles, inv_splits, inv_hkv, inv_g;     // div_reciprocal
-  float *part, *part_ref;  // splits > 1: [T, H, splits, D] values; [T, H, splits, 2] their reference and the row sum
+  float *part, *part_ref;  // splits > 1: [T, H, splits, D] values; [T, H, splits, 3] ref, lift and the row sum
   int* used;            // splits > 1: [T, H] splits that a row has
   // Rows of a token tree (or null): row t is of table row row_seq[t], which holds seq_lens[.] tokens, and sees those below tail_start[t] and of the 64
   // from there on the ones whose bit is set.
@@ -303,14 +303,22 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// A row's sums have one reference r, the largest s + log2 of the value scale that it has seen (s: its scores, in powers of two; within SLACK, so that it is
-// seldom raised). Values are summed with weights 2^(s + log2 scale - r + LIFT), which are the product's fp16 operand: at most 2^14, and what is rounded away
-// of one is under 2^-30 of the row's largest weight times scale, whatever pages of large values weigh little or are not seen at all. The sum of the row's
-// weights, 2^(s - r + SUM_LIFT), fits fp32 for all scales: its largest term is between 2^(-120 - SLACK + SUM_LIFT) and 2^(64 + SLACK + SUM_LIFT).
-constexpr float LIFT = 6.f, SLACK = 8.f, SUM_LIFT = 30.f;
-constexpr float SUM_OVER_VALUES = 1 << 24;                    // 2^(SUM_LIFT - LIFT)
-// The factor that takes partial sums to a common reference, which all have where none has seen a key.
-__device__ __forceinline__ float to_reference(float from, float to) { return to == -INFINITY ? 1.f : exp2_fast(from - to); }
+// What a row sums, s being its scores in powers of two: 2^(s - ref), and values weighed with 2^(s - ref + log2 of their page's scale + lift), which is the
+// product's fp16 operand. ref is such that the largest of these that the row has seen lies between 2^TOP and, SLACK lower, 2^6 (and is raised only when they
+// leave that): what is rounded away of a weight is under 2^-30 of the row's largest weight times scale, whatever pages of large values weigh little or are
+// not seen at all. With LIFT a term of the row sum is then between 2^-106 and 2^102 where it is the largest, so that fp32 holds it for scales of 2^-64 to 2^120.
+// Differences of scores come first and are added to afterwards, so that both exponents are off by the same where scores are large.
+constexpr float TOP = 14.f, SLACK = 8.f, LIFT = -24.f;
+// A score of FAR and more leaves a float no room for the scale beside it. Such rows (far) have the largest score for ref, raised at every step, and a lift of
+// their own for the scale. The tiles have no such rows: they report scores of twice that, where a weight may leave fp16.
+constexpr float FAR = 4194304.f;
+__device__ __forceinline__ bool is_far(float score) { return fabsf(score) > FAR && score > -INFINITY; }
+// Partial sums meet at the largest ref and at the lift that the one with the largest weights has there. Their factors; 1 where none has seen a key.
+__device__ __forceinline__ float lift_there(float ref, float lift, float to_ref) { return lift - (ref - to_ref); }
+__device__ __forceinline__ float sum_factor(float ref, float to_ref) { return to_ref == -INFINITY ? 1.f : exp2_fast(ref - to_ref); }
+__device__ __forceinline__ float values_factor(float ref, float lift, float to_ref, float to_lift) {
+  return to_ref == -INFINITY ? 1.f : exp2_fast((ref - to_ref) + (to_lift - lift));
+}
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   uint32_t d;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
@@ -358,12 +366,13 @@ constexpr int fp8_attend_smem() { return NW * ST * 2 * PageMap<D>::BYTES; }
 // rows, so that eight query rows fill the other one. A code is exact in fp16, and so is a query up to 2^-24 of its row's largest value once the row is
 // scaled by a power of two. Which dimension or token an index of a product means is free as long as both operands agree, so a lane's 16-byte pieces of a
 // key are its operands as they lie; the weights turn into the other product's operand by an 8 x 8 transpose. Scales of keys multiply the scores, scales of
-// values are added to the exponent of the weights. Every score has two exponentials, one for the sum: with one, and a factor for each page that takes the
-// value scale out again, 8 contexts of up to 65000 tokens took 76.5 us, with two 73.9.
+// values are added to the exponent of the weights. Every score has two exponentials, one for the sum.
 //
 // Bound by memory where there are enough pages, by a warp's own chain of instructions where there are few. A warp keeps its next pages on their way through
 // a ring of its own in shared memory, without registers and without a barrier of the CTA. Bulk copies in their place cost their issuing thread over a
 // hundred cycles each: 8 contexts of up to 65000 tokens, 8 key heads of 128, took 99.7 us with each warp's first lane issuing them, 111 with a fifth warp.
+// All shared memory is in the ring: three CTAs then fit the setting of 196 KB, and with 128 bytes more each take the next one from the first-level cache
+// (the same 8 contexts 74 and 76.5 us).
 template <int D, int NR, int NW, bool TREE, int ST>
 __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_kernel(const __grid_constant__ Fp8Attend a,
                                                                                       const __grid_constant__ Fp8Pool pool,
@@ -371,7 +380,6 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   using M = PageMap<D>;
   constexpr int KS = D / 16, NI = D / 16, KP = M::KP, VW = M::VW, ROWS = 8 * NR, SLOT = 2 * M::BYTES;
   extern __shared__ __align__(128) uint8_t ring[];    // NW x ST slots; then the sums
-  __shared__ float sm_r[NW][ROWS], sm_l[NW][ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c = lane & 3;
   int x = div_by(blockIdx.x, a.tiles, a.inv_tiles);
   const int tile = blockIdx.x - x * a.tiles, y = div_by(x, a.splits, a.inv_splits), split = x - y * a.splits;
@@ -495,7 +503,8 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   }
   const int all_lo = !TREE && a.window > 0 ? last - a.window + 1 : 0, all_hi = TREE ? min(tail, len) : first + 1;  // positions that every row sees
 
-  float o[NR][NI][4], l[NR][2], ref[NR][2];                                   // ref: the reference, SLACK included
+  float o[NR][NI][4], l[NR][2], ref[NR][2], lift[NR][2];
+  bool far = false;                                   // any of the warp's rows
 #pragma unroll
   for (int b = 0; b < NR; ++b) {
 #pragma unroll
@@ -504,6 +513,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
       for (int e = 0; e < 4; ++e) o[b][i][e] = 0.f;
     ref[b][0] = ref[b][1] = -INFINITY;
     l[b][0] = l[b][1] = 0.f;
+    lift[b][0] = lift[b][1] = LIFT;
   }
 
   for (int st = 0; st < steps; ++st) {
@@ -556,7 +566,7 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
         }
     }
     const bool whole = pos >= all_lo && pos + 2 * FP8_PAGE <= all_hi && there == 3;
-    bool over = false;
+    bool over = far;
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
@@ -585,43 +595,88 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
             }
           }
     }
-    auto highest = [&](int b, int e) { return fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]) + vs[0], fmaxf(s[b][1][e], s[b][1][2 + e]) + vs[1]); };
+    float w[NR][2][4], up[NR][2][2];                 // scores over ref, then what the values are weighed with; a page's share in its exponent
+    auto relate = [&](int b) {
 #pragma unroll
-    for (int b = 0; b < NR; ++b)
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) over |= highest(b, e) > ref[b][e];
+        for (int e = 0; e < 4; ++e) w[b][g][e] = s[b][g][e] - ref[b][e & 1];
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) up[b][g][e] = vs[g] + lift[b][e];
+    };
+#pragma unroll
+    for (int b = 0; b < NR; ++b) {
+      relate(b);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        over |= fmaxf(fmaxf(w[b][0][e], w[b][0][2 + e]) + up[b][0][e], fmaxf(w[b][1][e], w[b][1][2 + e]) + up[b][1][e]) > TOP;
+    }
     if (__any_sync(0xffffffffu, over)) {
+      auto highest = [&](int b, int e, float from) {             // of the row's scores over `from` with their page's scale
+        float x = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]) - from + vs[0], fmaxf(s[b][1][e], s[b][1][2 + e]) - from + vs[1]);
 #pragma unroll
-      for (int b = 0; b < NR; ++b) {
-        float alpha[2];
+        for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+        return x;
+      };
+      float now[NR][2], alpha[NR][2];
+#pragma unroll
+      for (int b = 0; b < NR; ++b)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float up = highest(b, e);
-#pragma unroll
-          for (int d = 4; d < 32; d *= 2) up = fmaxf(up, __shfl_xor_sync(0xffffffffu, up, d));
-          up = fmaxf(ref[b][e], up + SLACK);
-          alpha[e] = up == ref[b][e] ? 1.f : exp2_fast(ref[b][e] - up);
-          ref[b][e] = up;
-          l[b][e] *= alpha[e];
+          now[b][e] = fmaxf(ref[b][e], highest(b, e, 0.f) + (SLACK - TOP + LIFT));
+          alpha[b][e] = now[b][e] == ref[b][e] ? 1.f : exp2_fast(ref[b][e] - now[b][e]);
+          far |= is_far(now[b][e]);
         }
+      if (__any_sync(0xffffffffu, far)) {
+        rarely();
+        far = false;
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(fmaxf(s[b][0][e], s[b][0][2 + e]), fmaxf(s[b][1][e], s[b][1][2 + e]));
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            top = fmaxf(ref[b][e], top);
+            const float most = highest(b, e, is_far(top) ? top : 0.f), was = ref[b][e], raised = is_far(top) ? top : now[b][e];
+            const float lifted = is_far(top) ? fminf(TOP - SLACK - most, lift_there(was, lift[b][e], raised)) : LIFT;
+            const float step = was == raised ? 0.f : was - raised;
+            l[b][e] *= exp2_fast(step);
+            alpha[b][e] = exp2_fast(step + (lifted - lift[b][e]));
+            ref[b][e] = raised;
+            lift[b][e] = lifted;
+            far |= is_far(top);
+          }
+        far = __any_sync(0xffffffffu, far);
+      } else {
+#pragma unroll
+        for (int b = 0; b < NR; ++b)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            l[b][e] *= alpha[b][e];
+            ref[b][e] = now[b][e];
+          }
+      }
+#pragma unroll
+      for (int b = 0; b < NR; ++b) {
 #pragma unroll
         for (int k = 0; k < NI; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[e & 1];
+          for (int e = 0; e < 4; ++e) o[b][k][e] *= alpha[b][e & 1];
+        relate(b);
       }
     }
-    float w[NR][2][4];                               // what the values are weighed with; s: what is summed
 #pragma unroll
     for (int b = 0; b < NR; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float sum_off = (SUM_LIFT + SLACK) - ref[b][e & 1], off = (LIFT + SLACK) - ref[b][e & 1];
+      for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          w[b][g][e] = exp2_fast(s[b][g][e] + (off + vs[g]));
-          s[b][g][e] = exp2_fast(s[b][g][e] + sum_off);
+        for (int e = 0; e < 4; ++e) {
+          s[b][g][e] = exp2_fast(w[b][g][e]);
+          w[b][g][e] = exp2_fast(w[b][g][e] + up[b][g][e & 1]);
         }
-      }
     if (!whole) {                                    // nothing of a hidden place, whatever its scale and however little the row has seen
       rarely();
 #pragma unroll
@@ -684,9 +739,10 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
   }
 
   // ---- the warps' shares, each in its own part of the ring ----
-  constexpr int SHARE = ST * SLOT / 4;               // floats of a warp's part; ROWS x D are used
-  static_assert(ROWS * D <= SHARE, "sums fit the ring");
+  constexpr int SHARE = ST * SLOT / 4;               // floats of a warp's part: ROWS x D sums, behind them a row's ref, sum and lift
+  static_assert(ROWS * (D + 3) <= SHARE, "sums fit the ring");
   float* sums = reinterpret_cast<float*>(ring);
+  auto of_row = [&](int w, int what, int r) -> float& { return sums[w * SHARE + ROWS * (D + what) + r]; };
 #pragma unroll
   for (int b = 0; b < NR; ++b)
 #pragma unroll
@@ -695,44 +751,57 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
       for (int d = 4; d < 32; d *= 2) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], d);
       const int r = b * 8 + 2 * c + e;
       if (n == 0) {
-        sm_r[warp][r] = ref[b][e];
-        sm_l[warp][r] = l[b][e];
+        of_row(warp, 0, r) = ref[b][e];
+        of_row(warp, 2, r) = lift[b][e];
+        of_row(warp, 1, r) = l[b][e];
       }
       if (r < nr) {
         float* to = sums + warp * SHARE + r * D + M::col(n);
 #pragma unroll
         for (int k = 0; k < NI; k += 2)
-          *reinterpret_cast<float4*>(to + 2 * k) =
-              make_float4(o[b][k][e], o[b][k][2 + e], o[b][k + 1][e], o[b][k + 1][2 + e]);
+          *reinterpret_cast<float4*>(to + 2 * k) = make_float4(o[b][k][e], o[b][k][2 + e], o[b][k + 1][e], o[b][k + 1][2 + e]);
       }
     }
-  __syncthreads();
+  const bool cta_far = __syncthreads_or(far);
   for (int i = threadIdx.x; i < nr * (D / 4); i += NW * 32) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float rr = sm_r[0][r];
+    float rr = of_row(0, 0, r);
 #pragma unroll
-    for (int w = 1; w < NW; ++w) rr = fmaxf(rr, sm_r[w][r]);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float f = to_reference(sm_r[w][r], rr);
+    for (int w = 1; w < NW; ++w) rr = fmaxf(rr, of_row(w, 0, r));
+    float to_lift = LIFT, acc[4] = {0.f, 0.f, 0.f, 0.f}, ll = 0.f;
+    auto add = [&](int w, float f, float fv) {
       const float4 v = *reinterpret_cast<const float4*>(sums + w * SHARE + r * D + d);
-      acc[0] += v.x * f; acc[1] += v.y * f; acc[2] += v.z * f; acc[3] += v.w * f;
-      ll += sm_l[w][r] * f;
+      acc[0] += v.x * fv; acc[1] += v.y * fv; acc[2] += v.z * fv; acc[3] += v.w * fv;
+      ll += of_row(w, 1, r) * f;
+    };
+    if (cta_far) {
+      rarely();
+      to_lift = INFINITY;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) to_lift = fminf(to_lift, lift_there(of_row(w, 0, r), of_row(w, 2, r), rr));
+#pragma unroll
+      for (int w = 0; w < NW; ++w) add(w, sum_factor(of_row(w, 0, r), rr), values_factor(of_row(w, 0, r), of_row(w, 2, r), rr, to_lift));
+    } else {
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = sum_factor(of_row(w, 0, r), rr);
+        add(w, f, f);
+      }
     }
     const int tok = div_by(r0 + r, a.G, a.inv_g), t = t0 + tok, hd = hk * a.G + r0 + r - tok * a.G;
     if (a.splits == 1) {
-      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      const float inv = ll == 0.f ? 0.f : 1.f / ll, drop = cta_far ? exp2_fast(-to_lift) : exp2_fast(-LIFT);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * inv * SUM_OVER_VALUES;           // inv first: the values' own scale is in it
+      for (int i = 0; i < 4; ++i) acc[i] = acc[i] * inv * drop;                      // inv first: the values' own scale is in the other one
       *reinterpret_cast<uint2*>(a.out + t * a.ld_o + hd * D + d) = make_uint2(cvt_bf16x2(acc[0], acc[1]), cvt_bf16x2(acc[2], acc[3]));
       continue;
     }
     const long at = ((long)t * a.H + hd) * a.splits + split;
     *reinterpret_cast<float4*>(a.part + at * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     if (d == 0) {
-      a.part_ref[2 * at] = rr;
-      a.part_ref[2 * at + 1] = ll;
+      a.part_ref[3 * at] = rr;
+      a.part_ref[3 * at + 1] = to_lift;
+      a.part_ref[3 * at + 2] = ll;
       if (split == 0) a.used[(long)t * a.H + hd] = max(1, min(a.splits, (pg_hi - pg_lo + a.per_split - 1) / a.per_split));
     }
   }
@@ -742,7 +811,6 @@ __global__ void __launch_bounds__(NW * 32, (NR == 1 ? 12 : 8) / NW) fp8_attend_k
 __host__ __device__ constexpr uint32_t make_idesc_f16(uint32_t M, uint32_t N, uint32_t b_mn_major) {
   return (1u << 4) | (b_mn_major << 16) | ((N >> 3) << 17) | ((M >> 4) << 24);        // fp32 sums of fp16 operands
 }
-
 
 // One product step or commit of a converged warp: the thread is chosen inside, under a predicate, so that operands stay in uniform registers (a branch to
 // one lane around them made each step cost about ninety cycles of its warp).
@@ -1022,7 +1090,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
         if (lane == 0) mbar_arrive(&q_full[t]);
       }
       const int all_lo = a.window > 0 ? last - a.window + 1 : 0, all_hi = first + 1;      // positions that every row sees
-      float m = -INFINITY, l = 0.f, ref = -INFINITY;   // the sum has a reference of its own, the largest score
+      float m = -INFINITY, l = 0.f, ref = -INFINITY;   // l: sum of 2^(s - m + TOP - SLACK); ref: the largest s + log2 of the value scale
       bool ok = true;
       for (int j = 0; j < nb; ++j) {
         if (!mbar_wait_warp(&s_full[t][j & 1], (j >> 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL)) {
@@ -1091,7 +1159,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           }
         }
         // ---- weights: a page at a time, without a branch between pages where nothing is hidden, so that their chains overlap ----
-        const float base = LIFT - (m == -INFINITY ? 0.f : m), shift = ref == -INFINITY ? 0.f : m - ref;
+        const float base = (TOP - SLACK) - (m == -INFINITY ? 0.f : m), shift = ref == -INFINITY ? 0.f : m - ref;
         auto weigh = [&](int h, bool masked) {
           uint32_t* u = s + h * 16;
           const float2 k = sc[h];
@@ -1138,8 +1206,9 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
       if (ok) ok = mbar_wait_warp(&o_full[t], (nb - 1) & 1, abort_flag, tk.status, ERR_WAIT_TMEM_FULL);
       if (ok) {
         tc_fence_after();
-        l = l == 0.f ? 0.f : l * exp2_fast(m - ref + (SUM_LIFT - LIFT));          // to the values' reference
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (rt < nr && is_far(0.5f * m) && m < INFINITY) atomicCAS(tk.status, 0, ERR_BAD_ARG);
+        l = l == 0.f ? 0.f : l * exp2_fast(m - ref - LIFT);                       // to the values' reference and lift
+        const float inv = l == 0.f ? 0.f : 1.f / l, drop = exp2_fast(-LIFT);
         const long at = ((long)(t0 + tok) * a.H + hd) * a.splits + split;
 #pragma unroll 1
         for (int cc = 0; cc < D / 32; ++cc) {
@@ -1153,7 +1222,7 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
               uint32_t h[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv * SUM_OVER_VALUES, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv * SUM_OVER_VALUES);
+                h[k] = cvt_bf16x2(__uint_as_float(o[i * 8 + 2 * k]) * inv * drop, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv * drop);
               to[i] = make_uint4(h[0], h[1], h[2], h[3]);
             }
           } else if (rt < nr) {
@@ -1165,8 +1234,9 @@ __global__ void __launch_bounds__(FT_THREADS, 1) fp8_attend_tile_kernel(const __
           __syncwarp();
         }
         if (a.splits > 1 && rt < nr) {
-          a.part_ref[2 * at] = ref;
-          a.part_ref[2 * at + 1] = l;
+          a.part_ref[3 * at] = ref;
+          a.part_ref[3 * at + 1] = LIFT;
+          a.part_ref[3 * at + 2] = l;
           if (split == 0) a.used[(long)(t0 + tok) * a.H + hd] = max(1, min(a.splits, (b_hi - b_lo + per - 1) / per));
         }
         tc_fence_before();
@@ -1216,19 +1286,28 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ F
     if (!span.fine || t < span.t0 || t - span.t0 >= span.count || (long)(t - span.t0) * a.G + head % a.G >= (long)tile_rows * a.tiles) return;
   }
   const float* base = a.part + item * splits * D + lane * E;
-  const float* ref = a.part_ref + item * splits * 2;
+  const float* ref = a.part_ref + item * splits * 3;
   const int ns = min(max(a.used[item], 0), splits);  // where a wait ran out there may be anything
   float rr = -INFINITY;
-  for (int s = lane; s < ns; s += 32) rr = fmaxf(rr, ref[2 * s]);
+  bool far = false;
+  for (int s = lane; s < ns; s += 32) {
+    rr = fmaxf(rr, ref[3 * s]);
+    far |= ref[3 * s + 1] != LIFT;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) rr = fmaxf(rr, __shfl_xor_sync(0xffffffffu, rr, o));
+  float to_lift = LIFT;
+  if (__any_sync(0xffffffffu, far)) {
+    to_lift = INFINITY;
+    for (int s = 0; s < ns; ++s) to_lift = fminf(to_lift, lift_there(ref[3 * s], ref[3 * s + 1], rr));
+  }
   float acc[E], ll = 0.f;
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.f;
 #pragma unroll 4
   for (int s = WIDE ? warp : 0; s < ns; s += NW) {
-    const float f = to_reference(ref[2 * s], rr);
-    ll += ref[2 * s + 1] * f;
+    const float f = values_factor(ref[3 * s], ref[3 * s + 1], rr, to_lift);
+    ll += ref[3 * s + 2] * sum_factor(ref[3 * s], rr);
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] += base[(long)s * D + i] * f;
   }
@@ -1248,10 +1327,10 @@ __global__ void __launch_bounds__(256) fp8_join_kernel(const __grid_constant__ F
       for (int i = 0; i < E; ++i) acc[i] += sm_o[w][lane * E + i];
     }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  const float inv = ll == 0.f ? 0.f : 1.f / ll, drop = ll == 0.f ? 0.f : exp2_fast(-to_lift);
   uint32_t* to = reinterpret_cast<uint32_t*>(a.out + t * a.ld_o + head * D + lane * E);
 #pragma unroll
-  for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv * SUM_OVER_VALUES, acc[i + 1] * inv * SUM_OVER_VALUES);
+  for (int i = 0; i < E; i += 2) to[i / 2] = cvt_bf16x2(acc[i] * inv * drop, acc[i + 1] * inv * drop);
 }
 
 }  // namespace inv
@@ -1338,7 +1417,7 @@ static bool fp8_few_rows(long rows, int D, long units, int pages) {
 struct Fp8Cut {
   int blocks, tiles, warps, per, splits;
   bool deep;             // one slot more a warp
-  long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 2l) + 1); }      // of partial results
+  long floats(int T, int H, int D) const { return splits == 1 ? 0 : (long)T * H * (splits * (D + 3l) + 1); }      // of partial results
   Fp8Cut(int n, int Hkv, int G, int D, int max_new, int max_len, int window, bool tree) {
     const long rows = (long)max_new * G;
     const long reach = window > 0 && (long)window + max_new < max_len ? (long)window + max_new : max_len;
@@ -1432,7 +1511,7 @@ static int fp8_attend(Fp8Attend a, const Fp8Pool& pool, const Fp8Tokens& tk, int
     const long rows = (long)tk.T * a.H * cut.splits;
     a.part = work;
     a.part_ref = work + rows * D;
-    a.used = (int*)(work + rows * (D + 2));
+    a.used = (int*)(work + rows * (D + 3));
   }
   const long ctas = (long)tk.n * pool.Hkv * a.splits * a.tiles;
   if (ctas > 0x7fffffffl) return -ERR_BAD_ARG;

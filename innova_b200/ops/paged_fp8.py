@@ -311,7 +311,8 @@ def kv_attend(q, pages: Fp8Pages, page_table, new: NewTokens, heads: int, scale:
               out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """q [T, heads * dim]: the queries of ``new``'s tokens, whose keys and values are in the pages already. The token at position p of its sequence
     sees the positions up to p, or with ``window`` > 0 the latest ``window`` of them, its own included; pages that all of a sequence's new tokens have
-    left behind are not looked up. Query head h uses key head h // (heads / kv_heads). Returns [T, heads * dim]."""
+    left behind are not looked up. Query head h uses key head h // (heads / kv_heads). Returns [T, heads * dim]. On a GPU calls of many rows take scores
+    (scale q.k) up to 5.8 million; where a row's largest is beyond that ``check_status`` raises."""
     N, G, D = _check(q, "q", heads, pages, page_table)
     T, width = q.shape
     if width != heads * D or window < 0:

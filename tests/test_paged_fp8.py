@@ -267,6 +267,42 @@ def test_attend_pages_of_unequal_scales(case, ratio, dev):
 
 
 @pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("ratio", [0, -30, 20])
+@pytest.mark.parametrize("case, sizes", [(c, (10, 14, 18, 21, 22, 23, 24, 30, 60, -24)) for c in (
+    ([200], [1], 2, 1, 64), ([90, 37], [2, 3], 8, 2, 128), ([3000], [1], 8, 2, 64), ([150] * 60, [1] * 60, 16, 8, 64))] + [
+    (c, (10, 14, 16)) for c in (([129], [80], 4, 1, 128), ([2000], [40], 8, 2, 64))])
+def test_attend_scores_of_any_size(case, sizes, ratio, dev):
+    """Scores so large that a float holds no fraction of them, and more (in tiles up to a million): the keys that share the largest one share the weight,
+    whatever their pages' scales."""
+    for size in sizes:
+        s = Setup(*case, dev)
+        apart = {(i, j) for i, ids in enumerate(s.ids) for j in range(1, len(ids), 3)}
+        q = (along(s, apart).float() * (2.0 ** size if size > 0 else -(2.0 ** -size))).to(dtype_of(dev))
+        for i, j in apart:
+            s.pool.v_scale[s.ids[i][j - 1]] *= 2.0 ** ratio
+        got = pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H).cpu()
+        for i, (a, b) in enumerate(zip(s.ctx, s.new)):
+            if i % 7 == 0 or s.n < 10:
+                for t in range(0, b, max(1, b // 6)):
+                    close_rows(got, q, s, i, t, torch.arange(a + b) <= a + t)
+    if dev == "cuda":
+        rt.check_status()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [([129], [80], 4, 1, 128), ([2000], [40], 8, 2, 64)])
+def test_gpu_scores_beyond_the_tiles_are_reported(case):
+    s = Setup(*case, "cuda")
+    q = (along(s, ()).float() * 2.0 ** 22).bfloat16()
+    pf.kv_attend(q, s.pool, s.page_table, s.tokens, s.H)
+    with pytest.raises(RuntimeError):
+        rt.check_status()
+    q[3] = float("inf")                                                               # no number, but not that
+    pf.kv_attend((q.float() * 2.0 ** -22).bfloat16(), s.pool, s.page_table, s.tokens, s.H)
+    rt.check_status()
+
+
+@pytest.mark.parametrize("dev", DEVS)
 @pytest.mark.parametrize("ratio", [30, 60, 100])
 @pytest.mark.parametrize("case", [([31], [33], 1, 1, 64, 17), ([31], [5], 2, 1, 128, 17), ([20], [200], 4, 2, 64, 40), ([2000], [300], 4, 1, 128, 700),
                                   ([2000], [3], 4, 1, 128, 700), ([64, 70], [40, 150], 8, 2, 128, 16)])
