@@ -863,7 +863,7 @@ struct FtSmem {
 //   warps 12-13  issue a tile's S = Q K^T and O += P V (P from tensor memory)
 // A tile has two places for scores: the next block's are computed under this one's softmax, so that a row's chain does not wait for products (with one, and
 // blocks of 128 keys, a tile's softmax and products took turns: 548 us in two parts against 514).
-// 2 x 1500 tokens on 5500, 32 heads of 128 on 8: 365 us, 842 TFLOP/s. A block takes both tiles some 2100 cycles, of which the tensor cores are busy with
+// 2 x 1500 tokens on 5500, 32 heads of 128 on 8: 363 us, 847 TFLOP/s. A block takes both tiles some 2100 cycles, of which the tensor cores are busy with
 // 1260 (the queries are read from shared memory again for 64 keys each) and the exponentials' unit 1024: what bounds it is a row's chain of reading scores,
 // maximum, exponentials and writing weights. Two threads a row, half of a block's keys each, shorten the chain but leave the conversion half the registers:
 // 412 against 363 then. With barriers for keys and values apart the conversion was what every block waited for: 418.
