@@ -362,14 +362,23 @@ def _qk_norm_forward(qkv, wq, wk, spec):
     return y, x, ld, sizes
 
 
-def _qk_weight_grad(w, mg, wanted):
-    """(what autograd gets, where the entry leaves the gradient and how: 0 bf16 and 1 fp32 written, 2 added to the fp32 ``mg``, 3 not asked for)."""
+def _qk_weight_grad(w, mg, wanted, apart=False):
+    """(a gradient of its own or None, where the entry leaves it and how: 0 bf16 and 1 fp32 written, 2 added to ``mg``, 3 not asked for). The entry adds to a
+    dense fp32 ``mg`` alone; others, and one that is to be kept ``apart``, are added to behind it."""
     if not wanted:
         return None, 0, 3
-    if mg is not None:
+    if mg is not None and mg.dtype is torch.float32 and mg.is_contiguous() and not apart:
         return None, mg.data_ptr(), 2
-    g = torch.empty_like(w, memory_format=torch.contiguous_format)
+    g = torch.empty_like(w, dtype=w.dtype if mg is None else torch.float32, memory_format=torch.contiguous_format)
     return g, g.data_ptr(), int(g.dtype is torch.float32)
+
+
+def _to_main_grad(g, mg):
+    """What autograd gets of ``g``: nothing where a ``main_grad`` takes it."""
+    if g is None or mg is None:
+        return g
+    mg.add_(g.view(mg.shape))
+    return None
 
 
 class _QkNormRopeFn(torch.autograd.Function):
@@ -391,19 +400,16 @@ class _QkNormRopeFn(torch.autograd.Function):
         part = torch.empty(_QK_ROWS * ctx.sizes[5], dtype=torch.float32, device=x.device) if want_q or want_k else None
         mg_q = main_grad_of(wq, ctx.main_grads[0]) if want_q else None
         mg_k = main_grad_of(wk, ctx.main_grads[1]) if want_k else None
-        shared = None
-        if mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr():     # one weight for both norms: added one after the other
-            shared = mg_k = torch.zeros_like(mg_q)
+        # one weight for both norms: the second gradient is added behind the kernel
+        same = mg_q is not None and mg_k is not None and mg_q.data_ptr() == mg_k.data_ptr()
         gq, to_q, mode_q = _qk_weight_grad(wq, mg_q, want_q)
-        gk, to_k, mode_k = _qk_weight_grad(wk, mg_k, want_k)
+        gk, to_k, mode_k = _qk_weight_grad(wk, mg_k, want_k, same)
         rt.check(rt.lib().inv_qk_norm_bwd(_QK_PACK(x.data_ptr(), dx.data_ptr(), a.data_ptr(), b.data_ptr(), rt.ptr(cos), rt.ptr(sin), rt.ptr(positions),
                                                    rt.status_ptr(x), rt.stream_ptr(), d.data_ptr(), to_q, to_k, rt.ptr(part), ctx.ld, ctx.width, ld,
                                                    *ctx.sizes, mode_q, mode_k, ctx.eps)), "inv_qk_norm_bwd")
         if part is not None:
             rt.count_launches(1)
-        if shared is not None:
-            mg_q.add_(shared)
-        return dx if want_x else None, gq, gk, None
+        return dx if want_x else None, _to_main_grad(gq, mg_q), _to_main_grad(gk, mg_k), None
 
 
 def qk_norm_rope(qkv, q_weight, k_weight, cos, sin, n_q_heads, n_kv_heads, head_dim, positions=None, eps=1e-6):

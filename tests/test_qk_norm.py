@@ -274,6 +274,28 @@ def test_gpu_gradients_repeat_and_go_to_main_grads():
 
 
 @pytest.mark.gpu
+def test_gpu_main_grads_of_other_forms():
+    """A main_grad that is not dense fp32 is added to, and nothing beside it."""
+    x, wq, wk, dy, cos, sin = inputs(2, 50, 8, 4, 64, 64, torch.bfloat16, DEV)
+    plain = [t.clone().requires_grad_() for t in (x, wq, wk)]
+    ops.qk_norm_rope(*plain, cos, sin, 8, 4, 64).backward(dy)
+    want = [w.grad.float() for w in plain[1:]]
+    for shape, dtype, part in (((128,), torch.bfloat16, lambda t: t[:64]), ((64, 2), torch.float32, lambda t: t[:, 0]), ((8, 8), torch.float32, lambda t: t),
+                               ((64,), torch.float64, lambda t: t)):
+        some = [t.clone().requires_grad_() for t in (x, wq, wk)]
+        whole = [torch.ones(shape, device=DEV, dtype=dtype) for _ in "qk"]
+        for w, t in zip(some[1:], whole):
+            w.main_grad = part(t)
+        ops.qk_norm_rope(*some, cos, sin, 8, 4, 64).backward(dy)
+        for w, t, g in zip(some[1:], whole, want):
+            assert w.grad is None
+            # the gradient's own rounding in `want`, the main_grad's here
+            assert bool(((w.main_grad.reshape(64).float() - 1 - g).abs() <= 2.0 ** -8 * g.abs() + 2.0 ** -8 * (g + 1).abs() + 2.0 ** -20).all())
+            part(t).fill_(1)
+            assert bool((t == 1).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("wants", [(1, 0, 0), (1, 1, 0), (1, 0, 1), (0, 1, 1), (0, 1, 0), (0, 0, 1)])
 def test_gpu_gradients_that_nobody_asked_for(wants):
     """A frozen input gets none and a frozen weight's main_grad is left alone; the others' are the same to the bit, and frozen norms save their launch."""
