@@ -51,7 +51,7 @@ class Int8Weight(NamedTuple):
         return self.q.float() * self.scale.unsqueeze(-1)
 
 
-def _check_grad(what, *tensors):
+def refuse_gradients(what, *tensors):
     if forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} serves: no gradient and no tangent passes through it (call it under torch.no_grad())")
 
@@ -73,7 +73,7 @@ def _rows_of(x):
 
 def quantize_rows(x: torch.Tensor) -> Int8Rows:
     """x [..., K] in bf16 or fp32 -> whole numbers and a scale for each row, to be given to several products."""
-    _check_grad("quantize_rows", x)
+    refuse_gradients("quantize_rows", x)
     if x.dim() < 1 or x.dtype not in (_bf16, _fp32):
         raise TypeError(f"rows of bf16 or fp32, not {x.dtype} {tuple(x.shape)}")
     K = x.shape[-1]
@@ -123,7 +123,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
             and (codes is None or dtype is _int8 and codes.scale.shape == x.shape[:-1] and codes.scale.dtype is _fp32 and codes.scale.get_device() == dev)
             and (dev < 0 or q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0)) or gated and q.shape[0] % 2:
         _refuse(x, codes, w, bias, out_dtype, gated)
-    _check_grad("int8_linear", x, bias)
+    refuse_gradients("int8_linear", x, bias)
     N, K = q.shape
     cols = N // 2 if gated else N
     if dev < 0:

@@ -13,12 +13,17 @@ shift the reported loss value (src/moe_trainer.cpp:88-169), both carry gradients
 """
 from __future__ import annotations
 
+import struct
+from typing import Optional, Tuple, Union
+
 import torch
 import torch.nn.functional as F
 
 from .. import _native
 from . import runtime as rt
+from .functional import _dense_rows
 from .gemm import EPI_ATOMIC, EPI_NONE, gemm
+from .int8 import Int8Weight, check_weight, refuse_gradients
 
 _native.register_cuda_sigs({
     "inv_moe_router": [_native.vp] * 6 + [_native.i32] * 3 + [_native.vp],
@@ -28,6 +33,7 @@ _native.register_cuda_sigs({
     "inv_gemm_grouped": [_native.vp] * 3 + [_native.i32] * 9 + [_native.vp, _native.vp, _native.i32, _native.vp, _native.i32, _native.i32,
                                                                _native.i32, _native.i32, _native.vp, _native.vp, _native.i32, _native.i32,
                                                                _native.i64, _native.vp, _native.vp],
+    "inv_moe_few": [_native.vp], "inv_moe_few_bytes": [_native.i64] * 5 + [_native.i32],
 })
 
 ALIGN = 128
@@ -216,3 +222,120 @@ def moe_ffn(x, router_w, w_gu, w_down, residual=None, top_k=2, lb_coef=0.01, z_c
     if not x.is_cuda:
         return moe_ffn_reference(x, router_w, w_gu, w_down, residual, top_k, lb_coef, z_coef, reference_lb)
     return _MoEFn.apply(x, router_w, w_gu, w_down, residual, top_k, lb_coef, z_coef, reference_lb)
+
+
+# ---------------------------------------------------------------------------------------------- a few tokens
+FEW_TOKENS, FEW_EXPERTS, FEW_TOP = 64, 256, 16
+# What the entry is given: x, router, residual; both stacks, their scales; the shared expert's, their scales; result, counts, workspace, status, stream;
+# T, D, F, E, top_k, strides of x and residual, weights in 8 bits, bytes of the workspace.
+_FEW = struct.Struct("=16Q 9q").pack
+Weight = Union[torch.Tensor, Int8Weight]
+
+
+def moe_few_supported(x, router_w, w_gu, w_down, top_k=2) -> bool:
+    """Whether ``moe_ffn_few`` takes these tokens on their device: of at most 64, and on a GPU bf16 with sizes of its kernel."""
+    T, D = x.numel() // max(1, x.shape[-1]), x.shape[-1]
+    i8 = isinstance(w_gu, Int8Weight)
+    grain, E, inner = 16 if i8 else 8, router_w.shape[0], (w_down.q if i8 else w_down).shape[-1]
+    return T <= FEW_TOKENS and top_k <= min(E, FEW_TOP) and E <= FEW_EXPERTS and (not x.is_cuda or (x.dtype == torch.bfloat16 and D % grain == 0 and inner % grain == 0))
+
+
+def _plain(w: Weight) -> torch.Tensor:
+    return w.q if isinstance(w, Int8Weight) else w
+
+
+def _few_stack(w: Weight, dims: int, x, what: str):
+    """-> its values and scales, checked."""
+    if isinstance(w, Int8Weight):
+        check_weight(w, dims)
+        q, s = w
+        if x.is_cuda and not q.is_contiguous():
+            raise ValueError(f"{what} of {tuple(q.shape)} in 8 bits: rows one behind the other on a GPU")
+    else:
+        q, s = w, None
+        if q.dim() != dims or q.dtype != x.dtype or (x.is_cuda and (not q.is_contiguous() or q.data_ptr() % 16)):
+            raise ValueError(f"{what} of {q.dtype} {tuple(q.shape)}: contiguous {x.dtype} on 16-byte boundaries with {dims} dimensions, or an Int8Weight")
+    if q.device != x.device:
+        raise ValueError(f"{what} on {q.device}, x on {x.device}")
+    return q, s
+
+
+def _few_check(x, router_w, w_gu, w_down, residual, top_k, shared):
+    """-> T, D, F, E and (values, scales) of the stacks and of the shared expert."""
+    if x.dim() < 1 or x.dtype not in (torch.bfloat16, torch.float32) or (x.is_cuda and x.dtype != torch.bfloat16):
+        raise TypeError(f"x of {x.dtype} {tuple(x.shape)}: bf16 (fp32 too on the CPU)")
+    D = x.shape[-1]
+    T = x.numel() // max(1, D)
+    i8 = [isinstance(w, Int8Weight) for w in (w_gu, w_down, *(shared or ()))]
+    if any(i8) != all(i8) or (shared is not None and len(shared) != 2):
+        raise ValueError("experts and a shared one (gate_up, down): all in 8 bits or none")
+    if router_w.dim() != 2 or router_w.shape[1] != D or router_w.dtype != x.dtype or router_w.device != x.device:
+        raise ValueError(f"router of {router_w.dtype} {tuple(router_w.shape)} on {router_w.device}: {x.dtype} [experts, {D}] on {x.device}")
+    E, inner = router_w.shape[0], _plain(w_down).shape[-1]
+    stacks = [_few_stack(w_gu, 3, x, "w_gate_up"), _few_stack(w_down, 3, x, "w_down")]
+    if shared is not None:
+        stacks += [_few_stack(shared[0], 2, x, "shared gate_up"), _few_stack(shared[1], 2, x, "shared down")]
+    for (q, _), shape in zip(stacks, ((E, 2 * inner, D), (E, D, inner), (2 * inner, D), (D, inner))):
+        if q.shape != shape:
+            raise ValueError(f"a weight of {tuple(q.shape)} where {shape} is needed for {E} experts of {inner} on {D}")
+    if not 1 <= top_k <= E:
+        raise ValueError(f"top_k {top_k} of {E} experts")
+    if T > FEW_TOKENS or top_k > FEW_TOP or E > FEW_EXPERTS:
+        raise ValueError(f"{T} tokens, {E} experts, top_k {top_k}: at most {FEW_TOKENS}, {FEW_EXPERTS} and {FEW_TOP} (moe_ffn takes more tokens)")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"residual of {residual.dtype} {tuple(residual.shape)} on {residual.device} for x of {x.dtype} {tuple(x.shape)}")
+    grain = 16 if i8[0] else 8
+    if x.is_cuda and (D % grain or inner % grain or not D or not inner):
+        raise ValueError(f"width {D} and expert width {inner}: multiples of {grain} on a GPU")
+    return T, D, inner, E, stacks
+
+
+def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Optional[torch.Tensor] = None, top_k: int = 2,
+                shared: Optional[Tuple[Weight, Weight]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``moe_ffn`` for serving up to 64 tokens, in two launches (``csrc/moe_few.cu``) -> (y, tokens_per_expert). x [..., D] in bf16; router_w [E, D];
+    w_gate_up [E, 2F, D] (gate | up) and w_down [E, D, F] in bf16, or both as ``ops.int8.Int8Weight``; ``shared`` (gate_up [2F, D], down [D, F]): an expert that
+    every token goes to with weight one. The routing weights are the raw probabilities; ties go to the lowest expert. Sums are kept in fp32, the activations
+    between the products rounded to bf16, the result once. A token's result depends on no other. No gradient and no tangent passes through it."""
+    T, D, inner, E, stacks = _few_check(x, router_w, w_gate_up, w_down, residual, top_k, shared)
+    refuse_gradients("moe_ffn_few", x, router_w, residual, *(q for q, _ in stacks))
+    if not x.is_cuda:
+        return _few_plain(x.reshape(T, D), router_w, stacks, residual, top_k, x.shape)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    counts = torch.empty(E, dtype=torch.int32, device=x.device)
+    if T == 0:
+        return out, counts.zero_()
+    with rt.device_of(x):
+        rows, ldx = _dense_rows(x, D)
+        res, ldr = (None, 0) if residual is None else _dense_rows(residual, D)
+        router_w = router_w if router_w.is_contiguous() and router_w.data_ptr() % 16 == 0 else router_w.clone(memory_format=torch.contiguous_format)
+        fn = rt.lib().inv_moe_few_bytes
+        fn.restype = _native.i64
+        size = fn(T, D, inner, E, top_k, shared is not None)
+        work = torch.empty(size, dtype=torch.uint8, device=x.device)
+        at = [(q.data_ptr(), rt.ptr(s)) for q, s in stacks] + [(0, 0)] * (4 - len(stacks))
+        rt.check(rt.lib().inv_moe_few(_FEW(rows.data_ptr(), router_w.data_ptr(), rt.ptr(res), at[0][0], at[1][0], at[0][1], at[1][1], at[2][0], at[3][0], at[2][1],
+                                           at[3][1], out.data_ptr(), counts.data_ptr(), work.data_ptr(), rt.status_ptr(x), rt.stream_ptr(),
+                                           T, D, inner, E, top_k, ldx, ldr, stacks[0][1] is not None, size)), "inv_moe_few")
+        rt.count_launches(1)
+    return out, counts
+
+
+def _few_plain(x, router_w, stacks, residual, top_k, shape):
+    T, E = x.shape[0], router_w.shape[0]
+
+    def expert(h, pair, e=None):
+        gate_up, down = ((q if e is None else q[e], s if s is None or e is None else s[e]) for q, s in pair)
+        gate_up, down = (q.float() if s is None else q.float() * s.unsqueeze(-1) for q, s in (gate_up, down))
+        g, u = (h @ gate_up.t()).chunk(2, -1)
+        return (F.silu(g) * u) @ down.t()
+
+    h = x.float()
+    probs = torch.softmax(h @ router_w.float().t(), -1)
+    order = torch.sort(probs, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    y = torch.zeros_like(h) if residual is None else residual.reshape(h.shape).float()
+    if len(stacks) == 4:
+        y = y + expert(h, stacks[2:])
+    for e in order.unique().tolist():
+        rows = (order == e).any(-1).nonzero().flatten()
+        y = y.index_add(0, rows, expert(h[rows], stacks[:2], e) * probs[rows, e].unsqueeze(-1))
+    return y.to(x.dtype).view(shape), torch.bincount(order.reshape(-1), minlength=E).int()
