@@ -3,6 +3,7 @@
 #include "sm100_common.cuh"
 #include "inv_api.h"
 #include "side_job.cuh"
+#include <initializer_list>
 
 namespace inv {
 
@@ -60,7 +61,8 @@ struct GemmParams {
 int make_tmap_2d_bf16(CUtensorMap* out, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner,
                       uint32_t box_outer);
 
-int make_tmap_2d_u8(CUtensorMap* out, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner, uint32_t box_outer);
+int make_tmap(CUtensorMap* out, CUtensorMapDataType type, int rank, const void* ptr, std::initializer_list<uint64_t> sizes, std::initializer_list<uint64_t> strides,
+              std::initializer_list<uint32_t> box);
 
 int make_tmap_2d_f32(CUtensorMap* out, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner, uint32_t box_outer);
 

@@ -18,6 +18,7 @@
 // All waits are bounded; a wait that runs out writes a code into *status and the CTA unwinds.
 #include "gemm_common.cuh"
 
+#include <algorithm>
 #include <mutex>
 
 namespace inv {
@@ -362,16 +363,19 @@ int make_tmap_2d_bf16(CUtensorMap* out, const void* ptr, uint64_t inner, uint64_
   return r == CUDA_SUCCESS ? 0 : -(int)r - 1000;
 }
 
-// The same over bytes.
-int make_tmap_2d_u8(CUtensorMap* out, const void* ptr, uint64_t inner, uint64_t outer, uint64_t ld, uint32_t box_inner, uint32_t box_outer) {
+// A map of any type and rank, 128B swizzle: sizes and box with the innermost first, strides in bytes from the second dimension on.
+int make_tmap(CUtensorMap* out, CUtensorMapDataType type, int rank, const void* ptr, std::initializer_list<uint64_t> sizes, std::initializer_list<uint64_t> strides,
+              std::initializer_list<uint32_t> box) {
   EncodeTiledFn enc = get_encode_fn();
   if (!enc) return -1;
-  cuuint64_t dims[2] = {inner, outer};
-  cuuint64_t strides[1] = {ld};
-  cuuint32_t box[2] = {box_inner, box_outer};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rank < 2 || rank > 5 || (int)sizes.size() != rank || (int)strides.size() != rank - 1 || (int)box.size() != rank) return -ERR_BAD_ARG;
+  cuuint64_t d[5], s[5];
+  cuuint32_t b[5], one[5] = {1, 1, 1, 1, 1};
+  std::copy(sizes.begin(), sizes.end(), d);
+  std::copy(strides.begin(), strides.end(), s);
+  std::copy(box.begin(), box.end(), b);
+  const CUresult r = enc(out, type, (cuuint32_t)rank, const_cast<void*>(ptr), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -(int)r - 1000;
 }
 

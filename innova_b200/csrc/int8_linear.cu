@@ -11,6 +11,7 @@
 #include "cta_pair.cuh"
 #include "gemm_common.cuh"
 #include "once_per_device.h"
+#include <cstdlib>
 
 namespace inv {
 
@@ -40,58 +41,104 @@ __device__ __forceinline__ int int8_code(float x, float s, float inv) {
   return d > 0.f || (d == 0.f && (i & 1)) ? i + 1 : i;
 }
 
-template <typename T>
-__device__ __forceinline__ float int8_as_float(T v);
-template <>
-__device__ __forceinline__ float int8_as_float(float v) { return v; }
-template <>
-__device__ __forceinline__ float int8_as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-// A CTA takes a row; VEC: rows on 16-byte boundaries. A row with a value that is not finite gets NaN for its scale.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ x, long ldx, int K, int8_t* __restrict__ codes, long ldc, float* __restrict__ sx) {
-  constexpr int PER = 16 / sizeof(T);
-  __shared__ uint32_t sh[8];
-  release_next();
-  const T* row = x + (long)blockIdx.x * ldx;
-  int8_t* to = codes + (long)blockIdx.x * ldc;
-  const int tid = threadIdx.x, vecs = VEC ? K / PER : 0;
-  uint32_t top = 0;                                       // bits of the largest |x|: not a number is above infinity is above the rest
-  for (int i = tid; i < vecs; i += 256) {
-    const uint4 v = reinterpret_cast<const uint4*>(row)[i];
-    const T* e = reinterpret_cast<const T*>(&v);
+// Eight values from `row`, of which n exist; VEC: all of them, on a 16-byte boundary.
+template <bool VEC>
+__device__ __forceinline__ void int8_eight(const __nv_bfloat16* row, int n, float* v) {
+  if constexpr (VEC) {
+    const uint4 w = *reinterpret_cast<const uint4*>(row);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int j = 0; j < PER; ++j) top = max(top, __float_as_uint(int8_as_float(e[j])) & 0x7fffffffu);
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = __uint_as_float(u[j] << 16);
+      v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? __bfloat162float(row[j]) : 0.f;
   }
-  for (int i = vecs * PER + tid; i < K; i += 256) top = max(top, __float_as_uint(int8_as_float(row[i])) & 0x7fffffffu);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((tid & 31) == 0) sh[tid >> 5] = top;
-  __syncthreads();
+}
+template <bool VEC>
+__device__ __forceinline__ void int8_eight(const float* row, int n, float* v) {
+  if constexpr (VEC) {
+    const float4 a = reinterpret_cast<const float4*>(row)[0], b = reinterpret_cast<const float4*>(row)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  } else {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, sh[i]);
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? row[j] : 0.f;
+  }
+}
+
+// A CTA takes a row, or (WARP) each of its warps one, a thread HOLD times eight of its values, which it keeps between the maximum and the rounding; what a long
+// row has beyond that is read twice. VEC: rows on 16-byte boundaries, whole eights. A row with a value that is not finite gets NaN for its scale. Codes are written in eights, zeros behind the row.
+template <typename T, bool VEC, bool WARP>
+__global__ void __launch_bounds__(512) int8_rows_kernel(const T* __restrict__ x, long ldx, int rows, int K, int8_t* __restrict__ codes, long ldc, float* __restrict__ sx) {
+  constexpr int HOLD = WARP ? 4 : 3;
+  __shared__ uint32_t sh[16];
+  release_next();
+  const long r = WARP ? (long)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && r >= rows) return;
+  const T* row = x + r * ldx;
+  int8_t* to = codes + r * ldc;
+  const int tid = WARP ? threadIdx.x & 31 : threadIdx.x, threads = WARP ? 32 : blockDim.x, eights = (K + 7) / 8;
+  float v[HOLD][8];
+#pragma unroll
+  for (int h = 0; h < HOLD; ++h) {
+    const int i = tid + h * threads;
+    if (i < eights) int8_eight<VEC>(row + i * 8, K - i * 8, v[h]);
+  }
+  uint32_t top = 0;                                       // bits of the largest |x|: not a number is above infinity is above the rest
+#pragma unroll
+  for (int h = 0; h < HOLD; ++h)
+    if (tid + h * threads < eights) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[h][j]) & 0x7fffffffu);
+    }
+  for (int i = tid + HOLD * threads; i < eights; i += threads) {
+    float w[8];
+    int8_eight<VEC>(row + i * 8, K - i * 8, w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(w[j]) & 0x7fffffffu);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (!WARP) {
+    if ((tid & 31) == 0) sh[tid >> 5] = top;
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, (tid & 31) < threads / 32 ? sh[tid & 31] : 0u);
+  }
   const bool finite = top < 0x7f800000u;
   const float s = finite ? __fdiv_rn(fmaxf(__uint_as_float(top), INT8_LEAST), 127.f) : __uint_as_float(0x7fc00000u);
   const float inv = finite ? __frcp_rn(s) : 0.f;
-  if (tid == 0) sx[blockIdx.x] = s;
-  for (int i = tid; i < vecs; i += 256) {
-    const uint4 v = reinterpret_cast<const uint4*>(row)[i];
-    const T* e = reinterpret_cast<const T*>(&v);
-    uint32_t w[PER / 4];
+  if (tid == 0) sx[r] = s;
+  auto store = [&](int i, const float* w) {
+    uint32_t u[2] = {0u, 0u};
+    if (finite) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint32_t c = finite ? (uint32_t)int8_code(int8_as_float(e[j]), s, inv) & 255u : 0u;
-      w[j / 4] = j % 4 ? w[j / 4] | c << (8 * (j % 4)) : c;
+      for (int j = 0; j < 8; ++j) u[j / 4] |= ((uint32_t)int8_code(w[j], s, inv) & 255u) << (8 * (j % 4));
     }
-    if constexpr (PER == 8) reinterpret_cast<uint2*>(to)[i] = make_uint2(w[0], w[1]);
-    else reinterpret_cast<uint32_t*>(to)[i] = w[0];
+    *reinterpret_cast<uint2*>(to + i * 8) = make_uint2(u[0], u[1]);
+  };
+#pragma unroll
+  for (int h = 0; h < HOLD; ++h)
+    if (tid + h * threads < eights) store(tid + h * threads, v[h]);
+  for (int i = tid + HOLD * threads; i < eights; i += threads) {
+    float w[8];
+    int8_eight<VEC>(row + i * 8, K - i * 8, w);
+    store(i, w);
   }
-  for (int i = vecs * PER + tid; i < K; i += 256) to[i] = finite ? (int8_t)int8_code(int8_as_float(row[i]), s, inv) : (int8_t)0;
 }
 
 static int launch_int8_rows(const Int8Call& c, cudaStream_t st) {
   const int size = c.x_f32 ? 4 : 2;
-  const bool vec = ((uintptr_t)c.x | (uintptr_t)(c.T > 1 ? c.ldx * size : 0)) % 16 == 0;
-#define INV_ROWS(E, V) int8_rows_kernel<E, V><<<(unsigned)c.T, 256, 0, st>>>((const E*)c.x, c.ldx, (int)c.K, c.codes, c.ldc, c.sx)
+  const bool vec = c.K % 8 == 0 && ((uintptr_t)c.x | (uintptr_t)(c.T > 1 ? c.ldx * size : 0)) % 16 == 0;
+  const bool warps = c.K <= 1024 && c.T > 296;
+  const int threads = warps ? 256 : c.K <= 512 ? 64 : c.K <= 1024 ? 128 : c.K <= 4096 ? 256 : 512;
+  const unsigned grid = (unsigned)(warps ? (c.T + 7) / 8 : c.T);
+#define INV_ROW(E, V, W) int8_rows_kernel<E, V, W><<<grid, threads, 0, st>>>((const E*)c.x, c.ldx, (int)c.T, (int)c.K, c.codes, c.ldc, c.sx)
+#define INV_ROWS(E, V)             \
+  do {                             \
+    if (warps) INV_ROW(E, V, true); \
+    else INV_ROW(E, V, false);     \
+  } while (0)
   if (c.x_f32) {
     if (vec) INV_ROWS(float, true);
     else INV_ROWS(float, false);
@@ -100,12 +147,13 @@ static int launch_int8_rows(const Int8Call& c, cudaStream_t st) {
     else INV_ROWS(__nv_bfloat16, false);
   }
 #undef INV_ROWS
+#undef INV_ROW
   return -(int)cudaGetLastError();
 }
 
 __device__ __forceinline__ float int8_silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
-// ---------------------------------------------------------------------------------------------- up to 64 rows
+// ---------------------------------------------------------------------------------------------- up to eight rows
 struct Int8Few {
   const int8_t *codes, *q;
   const float *sx, *sw;
@@ -140,19 +188,19 @@ __device__ __forceinline__ float int8_bias(const void* b, int f32, int i) {
   return b == nullptr ? 0.f : f32 ? static_cast<const float*>(b)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
 }
 
-// A CTA takes 32 weight rows at a time (gated: 16 of the gate and their 16 of the up product) as the 16-row operand, NT x 8 activations as the other. Its eight
-// warps take every eighth slice of K, 128 bytes of a row, and meet in shared memory. Both operands read a lane's 32 consecutive bytes in the same order, which
-// a sum over k does not notice.
-constexpr int FEW_WARPS = 8, FEW_SLICE = 128, FEW_PL = 36;
+// Weights go from memory straight into fragments, with none of a tile's set-up. A CTA takes 32 weight rows at a time (gated: 16 of the gate and their 16 of the up
+// product) as the 16-row operand, the activations as the other. Its eight warps take every eighth slice of K, 128 bytes of a row, and meet in shared memory. Both
+// operands read a lane's 32 consecutive bytes in the same order, which a sum over k does not notice. The warp-level product of 8-bit integers is slow on this GPU,
+// some 80 cycles an instruction and scheduler: sixteen rows took 27 us of 22016 x 4096, 64 rows 110, where the tiles below take 20 and 22.
+constexpr int FEW_WARPS = 8, FEW_SLICE = 128, FEW_PL = 36, FEW_ROWS = 8, FEW_RING = 2;
 
-template <int NT, bool GATED>
-__global__ void __launch_bounds__(FEW_WARPS * 32, NT <= 2 ? 2 : 1) int8_few_kernel(const Int8Few p) {
-  constexpr int UN = NT <= 2 ? 2 : 4;                      // slices of a warp on their way
-  extern __shared__ int few_part[];                        // [FEW_WARPS][8 NT][FEW_PL]
+template <bool GATED>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8Few p) {
+  __shared__ int part[FEW_WARPS * FEW_ROWS * FEW_PL];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
   const int slices = (p.K + FEW_SLICE - 1) / FEW_SLICE;
   release_next();
-  uint4 ring[UN][4][2];
+  uint4 ring[FEW_RING][4][2];
   auto fetch = [&](int tile, int s, uint4 (&r)[4][2]) {
     const int at = s * FEW_SLICE + tig * 32;
 #pragma unroll
@@ -165,66 +213,54 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, NT <= 2 ? 2 : 1) int8_few_kern
   };
   int tile = blockIdx.x;
 #pragma unroll
-  for (int u = 0; u < UN; ++u)
+  for (int u = 0; u < FEW_RING; ++u)
     if (warp + u * FEW_WARPS < slices) fetch(tile, warp + u * FEW_WARPS, ring[u]);
   wait_previous();                                         // codes and scales of the activations
-  const int8_t* xp[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n) xp[n] = p.codes + (long)min(n * 8 + g, p.T - 1) * p.ldc + tig * 32;
+  const int8_t* x = p.codes + (long)min(g, p.T - 1) * p.ldc + tig * 32;
   for (; tile < p.tiles; tile += gridDim.x) {
-    int acc[NT][2][4];
+    int acc[2][4] = {};
+    for (int s0 = warp; s0 < slices; s0 += FEW_RING * FEW_WARPS) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[n][i / 4][i % 4] = 0;
-    for (int s0 = warp; s0 < slices; s0 += UN * FEW_WARPS) {
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
+      for (int u = 0; u < FEW_RING; ++u) {
         const int s = s0 + u * FEW_WARPS;
         if (s >= slices) break;
         const int left = p.K - s * FEW_SLICE - tig * 32;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+          uint4 b = make_uint4(0, 0, 0, 0);
+          if (left > 16 * i) {
+            b = *reinterpret_cast<const uint4*>(x + s * FEW_SLICE + 16 * i);
+            if (left < 16 * i + 16) b = int8_mask(b, left - 16 * i);
+          }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (left > 16 * i) {
-              b = *reinterpret_cast<const uint4*>(xp[n] + s * FEW_SLICE + 16 * i);
-              if (left < 16 * i + 16) b = int8_mask(b, left - 16 * i);
-            }
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              const uint4 lo = ring[u][2 * m][i], hi = ring[u][2 * m + 1][i];
-              int8_mma(acc[n][m], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
-              int8_mma(acc[n][m], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
-            }
+          for (int m = 0; m < 2; ++m) {
+            const uint4 lo = ring[u][2 * m][i], hi = ring[u][2 * m + 1][i];
+            int8_mma(acc[m], lo.x, hi.x, lo.y, hi.y, b.x, b.y);
+            int8_mma(acc[m], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
           }
         }
-        const int next = s + UN * FEW_WARPS;
+        const int next = s + FEW_RING * FEW_WARPS;
         if (next < slices) fetch(tile, next, ring[u]);
         else if (tile + (int)gridDim.x < p.tiles && warp + u * FEW_WARPS < slices) fetch(tile + gridDim.x, warp + u * FEW_WARPS, ring[u]);
       }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        int* to = few_part + ((warp * NT + n) * 8 + 2 * tig) * FEW_PL + m * 16 + g;
-        to[0] = acc[n][m][0];
-        to[FEW_PL] = acc[n][m][1];
-        to[8] = acc[n][m][2];
-        to[FEW_PL + 8] = acc[n][m][3];
-      }
+    for (int m = 0; m < 2; ++m) {
+      int* to = part + (warp * FEW_ROWS + 2 * tig) * FEW_PL + m * 16 + g;
+      to[0] = acc[m][0];
+      to[FEW_PL] = acc[m][1];
+      to[8] = acc[m][2];
+      to[FEW_PL + 8] = acc[m][3];
+    }
     __syncthreads();
     constexpr int COLS = GATED ? 16 : 32;
-    for (int i = tid; i < p.T * COLS; i += FEW_WARPS * 32) {
-      const int t = i / COLS, c = i % COLS, col = tile * COLS + c;
-      if (col >= p.cols) continue;
+    const int t = tid / COLS, c = tid % COLS, col = tile * COLS + c;
+    if (t < p.T && col < p.cols) {
       int a = 0, b = 0;
 #pragma unroll
       for (int w = 0; w < FEW_WARPS; ++w) {
-        a += few_part[(w * NT * 8 + t) * FEW_PL + c];
-        if (GATED) b += few_part[(w * NT * 8 + t) * FEW_PL + 16 + c];
+        a += part[(w * FEW_ROWS + t) * FEW_PL + c];
+        if (GATED) b += part[(w * FEW_ROWS + t) * FEW_PL + 16 + c];
       }
       const float s = p.sx[t];
       float y = fmaf((float)a * s, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
@@ -236,14 +272,262 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, NT <= 2 ? 2 : 1) int8_few_kern
   }
 }
 
-template <int NT, bool GATED>
-static int launch_int8_few(const Int8Few& p, bool early, int device, cudaStream_t st) {
-  constexpr int bytes = FEW_WARPS * NT * 8 * FEW_PL * 4, ctas = 148 * (NT <= 2 ? 2 : 1);
-  static OncePerDevice once;
-  if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(int8_few_kernel<NT, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }))
-    return -e;
-  launch_step(early, int8_few_kernel<NT, GATED>, dim3(p.tiles < ctas ? p.tiles : ctas), FEW_WARPS * 32, bytes, st, p);
+template <bool GATED>
+static int launch_int8_few(const Int8Call& c, bool early, cudaStream_t st) {
+  const int cols = (int)(GATED ? c.N / 2 : c.N), per = GATED ? 16 : 32, tiles = (cols + per - 1) / per;
+  const Int8Few p = {c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, cols, tiles, (int)c.bias_f32, (int)c.out_f32};
+  launch_step(early, int8_few_kernel<GATED>, dim3(tiles < 296 ? tiles : 296), FEW_WARPS * 32, 0, st, p);
   return -(int)cudaGetLastError();
+}
+
+// ---------------------------------------------------------------------------------------------- few tiles
+// Weight rows are the 128-row operand and TB activations the other one (tcgen05 kind::i8 on one SM), so that few activations fill an instruction. A cluster of up
+// to eight CTAs shares a tile: each has a part of K, leaves its sums in its shared memory and adds up its share of the tile's results from all of them.
+namespace i8s {
+constexpr int THREADS = 192, BK = 128, A_STAGE = 128 * BK;  // warp 0 loads, warp 1 products, warps 2 to 5 sums
+constexpr int MAX_STAGES = 12, REST = 1024 + 256;
+constexpr int stages(int tb, int ctas) { return (227 * 1024 / ctas - 1024 * (ctas - 1) - REST - 4 * tb) / (A_STAGE + tb * BK); }    // with so many CTAs an SM
+constexpr int smem_bytes(int tb, int n) { return n * (A_STAGE + tb * BK) + REST + 4 * tb; }
+}  // namespace i8s
+
+struct Int8Split {
+  const float *sx, *sw;
+  const void* bias;
+  void* out;
+  int* status;
+  long ldo;
+  int T, cols, kb, t_tiles, parts, stages;     // kb: steps of 128 bytes of K; t_tiles: tiles of activations; parts: CTAs of a tile; stages: of the ring
+  uint32_t inv_t, inv_parts;           // div_reciprocal
+  int bias_f32, out_f32, fours;        // fours: four results of a row are stored at once
+};
+
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n"
+      "}\n"
+      ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ int4 ld_cluster_v4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
+// GATED: a tile's rows are 16 of the gate and the same 16 of the up product in turn (boxes of a map of three dimensions).
+template <int TB, bool GATED>
+__global__ void __launch_bounds__(i8s::THREADS, 2)
+    int8_split_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ Int8Split p) {
+  using namespace i8s;
+  constexpr int B_STAGE = TB * BK, COLS = GATED ? 64 : 128;
+  constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(TB >> 3) << 17) | ((128u >> 4) << 24);
+  constexpr int TMEM_COLS = TB < 32 ? 32 : TB;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  const int STAGES = p.stages;
+  uint8_t* sB = smem + STAGES * A_STAGE;
+  int* sums = reinterpret_cast<int*>(smem);                // [TB][128], once the stages have been used
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sB + STAGES * B_STAGE);
+  uint64_t* empty_bar = full_bar + MAX_STAGES;
+  uint64_t* tmem_full = empty_bar + MAX_STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_full + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* scales = reinterpret_cast<float*>(tmem_slot + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int tile = div_by(blockIdx.x, p.parts, p.inv_parts), rank = (int)blockIdx.x - tile * p.parts;
+  const int ct = div_by(tile, p.t_tiles, p.inv_t), t0 = (tile - ct * p.t_tiles) * TB, left = min(TB, p.T - t0), n0 = ct * COLS;
+  const int k0 = rank * p.kb / p.parts, steps = (rank + 1) * p.kb / p.parts - k0;
+
+  release_next();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    mbar_init(tmem_full, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    if (elect_one_sync()) {
+      auto load_w = [&](int i, int s) {
+        mbar_expect_tx(&full_bar[s], A_STAGE + B_STAGE);
+        if constexpr (GATED) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tma_load_3d(sA + s * A_STAGE + j * 4096, &tmap_w, &full_bar[s], (k0 + i) * BK, n0 + 16 * j, 0);
+        } else {
+          tma_load_2d(sA + s * A_STAGE, &tmap_w, &full_bar[s], (k0 + i) * BK, n0);
+        }
+      };
+      auto load_x = [&](int i, int s) { tma_load_2d(sB + s * B_STAGE, &tmap_x, &full_bar[s], (k0 + i) * BK, t0); };
+      const int head = min(steps, STAGES);                 // weights flow while the activations are still being made
+      for (int i = 0; i < head; ++i) load_w(i, i);
+      wait_previous();
+      for (int i = 0; i < head; ++i) load_x(i, i);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int i = head; i < steps; ++i) {
+        if (!mbar_wait(&empty_bar[s], ph, abort_flag, p.status, ERR_WAIT_EMPTY)) break;
+        load_w(i, s);
+        load_x(i, s);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    if (elect_one_sync()) {
+      const uint64_t da0 = make_smem_desc(smem_u32(sA), 16, 1024, 2), db0 = make_smem_desc(smem_u32(sB), 16, 1024, 2);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int i = 0; i < steps; ++i) {
+        if (!mbar_wait(&full_bar[s], ph, abort_flag, p.status, ERR_WAIT_FULL)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t da = da0 + (uint64_t)(s * (A_STAGE >> 4)), db = db0 + (uint64_t)(s * (B_STAGE >> 4));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) umma_i8(tmem_base, da + 2 * k, db + 2 * k, IDESC, i > 0 || k > 0 ? 1u : 0u);
+        umma_commit(&empty_bar[s]);
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+      }
+      if (ok) umma_commit(tmem_full);
+    }
+  } else {
+    const int q = warp & 3, row = q * 32 + lane;           // the lanes of tensor memory that this warp may read
+    if (mbar_wait_warp(tmem_full, 0, abort_flag, p.status, ERR_WAIT_TMEM_FULL)) {
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < TB; c += 16) {
+        if (c >= left) break;
+        uint32_t r[16];
+        tmem_ld_32x16(tmem_base + c + (uint32_t(q * 32) << 16), r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + row] = (int)r[j];
+      }
+      tc_fence_before();
+    }
+  }
+  wait_previous();
+  for (int t = threadIdx.x; t < left; t += THREADS) scales[t] = p.sx[t0 + t];
+  __syncwarp();
+  if (p.parts > 1) cluster_sync_all();
+  else __syncthreads();
+  if (*abort_flag) {                          // let the loads and products that are under way end before the memory they use is given up
+    const uint64_t since = globaltimer_ns();
+    while (globaltimer_ns() - since < 2000000ull) __nanosleep(1000);
+  } else {
+    // four columns a lane; a warp takes a token at a time, or two halves of the gated form one each
+    constexpr int SUB = GATED ? 2 : 1;
+    const int c = GATED ? (lane & 15) * 4 : lane * 4, col = n0 + c, in_row = GATED ? (c >> 4) * 32 + (c & 15) : c;
+    float sw[SUB][4], bias[SUB][4];
+#pragma unroll
+    for (int h = 0; h < SUB; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool fine = col + i < p.cols;
+        sw[h][i] = fine ? p.sw[h * p.cols + col + i] : 0.f;
+        bias[h][i] = fine ? int8_bias(p.bias, p.bias_f32, h * p.cols + col + i) : 0.f;
+      }
+    const uint32_t base = smem_u32(sums) + in_row * 4;
+#pragma unroll 2
+    for (int t = rank + p.parts * (warp * SUB + (GATED ? lane >> 4 : 0)); t < left; t += p.parts * (THREADS / 32) * SUB) {
+      int v[SUB][4] = {};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j >= p.parts) break;
+        const uint32_t there = mapa_shared(base + t * 512, j);
+#pragma unroll
+        for (int h = 0; h < SUB; ++h) {
+          const int4 w = ld_cluster_v4(there + h * 64);
+          v[h][0] += w.x; v[h][1] += w.y; v[h][2] += w.z; v[h][3] += w.w;
+        }
+      }
+      const float sx = scales[t];
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        y[i] = fmaf((float)v[0][i] * sx, sw[0][i], bias[0][i]);
+        if (GATED) y[i] = int8_silu(y[i]) * fmaf((float)v[SUB - 1][i] * sx, sw[SUB - 1][i], bias[SUB - 1][i]);
+      }
+      const long o = (long)(t0 + t) * p.ldo + col;
+      if (p.fours && col + 3 < p.cols) {
+        if (p.out_f32) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + o) = make_float4(y[0], y[1], y[2], y[3]);
+        else *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + o) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (col + i >= p.cols) break;
+          if (p.out_f32) static_cast<float*>(p.out)[o + i] = y[i];
+          else static_cast<__nv_bfloat16*>(p.out)[o + i] = __float2bfloat16_rn(y[i]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncwarp();
+  if (p.parts > 1) cluster_sync_all();                     // the others have read this CTA's sums
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+template <int TB, bool GATED>
+static int launch_int8_split(const Int8Call& c, bool early, int device, cudaStream_t st) {
+  using namespace i8s;
+  static OncePerDevice once;
+  if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(int8_split_kernel<TB, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(TB, stages(TB, 1))); }))
+    return -e;
+  const int cols = (int)(GATED ? c.N / 2 : c.N);
+  Int8Split p;
+  p.sx = c.sx; p.sw = c.sw; p.bias = c.bias; p.out = c.out; p.ldo = c.ldo; p.T = (int)c.T; p.cols = cols; p.status = c.status;
+  p.kb = (int)((c.K + BK - 1) / BK); p.t_tiles = (int)((c.T + TB - 1) / TB);
+  const int tiles = (cols + (GATED ? 63 : 127)) / (GATED ? 64 : 128) * p.t_tiles;
+  auto fit = [&](int ctas) { const int n = ctas / tiles; return n < 1 ? 1 : n > 4 ? 4 : n; };
+  int parts = fit(128);
+  if (parts * tiles < 112) parts = fit(256);
+  if (const char* e = getenv("I8S")) parts = atoi(e);
+  p.parts = parts > p.kb ? p.kb : parts;
+  const int per_sm = tiles * p.parts <= 128 ? 1 : 2, most = stages(TB, per_sm), steps = (p.kb + p.parts - 1) / p.parts;
+  p.stages = most < steps ? most : steps;
+  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
+  if (p.stages * (A_STAGE + TB * BK) < TB * 512) p.stages = (TB * 512 + A_STAGE + TB * BK - 1) / (A_STAGE + TB * BK);   // the sums take their place
+  p.inv_t = div_reciprocal(p.t_tiles); p.inv_parts = div_reciprocal(p.parts);
+  p.bias_f32 = (int)c.bias_f32; p.out_f32 = (int)c.out_f32;
+  p.fours = c.ldo % 4 == 0 && (uintptr_t)c.out % 16 == 0;
+  CUtensorMap tw, tx;
+  const uint64_t K = c.K, N = c.N, T = c.T, ld = c.ldw;
+  const CUtensorMapDataType u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  int rc = GATED ? make_tmap(&tw, u8, 3, c.q, {K, N / 2, 2}, {ld, ld * (N / 2)}, {BK, 16, 2}) : make_tmap(&tw, u8, 2, c.q, {K, N}, {ld}, {BK, 128});
+  if (rc == 0) rc = make_tmap(&tx, u8, 2, c.codes, {K, T}, {(uint64_t)c.ldc}, {BK, TB});
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(tiles * p.parts);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem_bytes(TB, p.stages);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = early ? 2 : 1;
+  return -(int)cudaLaunchKernelEx(&cfg, int8_split_kernel<TB, GATED>, tw, tx, p);
 }
 
 // ---------------------------------------------------------------------------------------------- tiles
@@ -500,8 +784,8 @@ static int launch_int8_tiles(const Int8Call& c, bool early, int device, cudaStre
   p.bias_f32 = (int)c.bias_f32; p.status = c.status;
   p.boxes = ((uintptr_t)c.out | (uintptr_t)(c.ldo * size)) % 16 == 0;
   CUtensorMap ta, tb, tc;
-  int rc = make_tmap_2d_u8(&ta, c.codes, (uint64_t)c.K, (uint64_t)c.T, (uint64_t)c.ldc, BK, 128);
-  if (rc == 0) rc = make_tmap_2d_u8(&tb, c.q, (uint64_t)c.K, (uint64_t)c.N, (uint64_t)c.ldw, BK, 128);
+  int rc = make_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.codes, {(uint64_t)c.K, (uint64_t)c.T}, {(uint64_t)c.ldc}, {BK, 128});
+  if (rc == 0) rc = make_tmap(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.q, {(uint64_t)c.K, (uint64_t)c.N}, {(uint64_t)c.ldw}, {BK, 128});
   tc = ta;
   if (rc == 0 && p.boxes) rc = F32 ? make_tmap_2d_f32(&tc, c.out, (uint64_t)cols, (uint64_t)c.T, (uint64_t)c.ldo, 32, 32)
                                    : make_tmap_2d_bf16(&tc, c.out, (uint64_t)cols, (uint64_t)c.T, (uint64_t)c.ldo, 64, 32);
@@ -510,6 +794,14 @@ static int launch_int8_tiles(const Int8Call& c, bool early, int device, cudaStre
   const int pairs = (int)(total < 74 ? total : 74);
   launch_step(early, int8_tile_kernel<GATED, F32>, dim3(2 * pairs), THREADS, SMEM_BYTES, st, ta, tb, tc, p);
   return -(int)cudaGetLastError();
+}
+
+enum Int8Route { INT8_FEW, INT8_SPLIT, INT8_TILES };
+static Int8Route int8_route(const Int8Call& c) {
+  if (const char* e = getenv("I8ROUTE")) return (Int8Route)atoi(e);
+  if (c.T <= FEW_ROWS && c.N * c.K <= (32l << 20)) return INT8_FEW;
+  const long tiles = (c.T + 127) / 128 * ((c.gated ? c.N / 2 + 63 : c.N + 127) / (c.gated ? 64 : 128));
+  return c.T <= 128 || tiles <= 148 ? INT8_SPLIT : INT8_TILES;
 }
 
 }  // namespace inv
@@ -527,20 +819,24 @@ extern "C" int inv_int8_rows(const void* call) {
 extern "C" int inv_int8_linear(const void* call) {
   const Int8Call& c = *static_cast<const Int8Call*>(call);
   if (c.T <= 0 || c.N <= 0 || c.K <= 0) return 0;
-  if (c.K > 133144 || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2)) return -ERR_BAD_ARG;
+  if (c.K > 133144 || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2) || (c.gated && c.N < 2)) return -ERR_BAD_ARG;
   cudaStream_t st = (cudaStream_t)c.stream;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;
   const bool early = c.x != nullptr;
+  const Int8Route route = int8_route(c);
   if (early)
     if (const int e = launch_int8_rows(c, st)) return e;
-  if (c.T <= 64) {
-    const int cols = (int)(c.gated ? c.N / 2 : c.N), per = c.gated ? 16 : 32;
-    const Int8Few p = {c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, cols, (cols + per - 1) / per, (int)c.bias_f32,
-                       (int)c.out_f32};
-#define INV_FEW(NT) (c.gated ? launch_int8_few<NT, true>(p, early, device, st) : launch_int8_few<NT, false>(p, early, device, st))
-    return c.T <= 8 ? INV_FEW(1) : c.T <= 16 ? INV_FEW(2) : c.T <= 32 ? INV_FEW(4) : INV_FEW(8);
-#undef INV_FEW
+  if (route == INT8_FEW) return c.gated ? launch_int8_few<true>(c, early, st) : launch_int8_few<false>(c, early, st);
+  if (route == INT8_SPLIT) {
+#define INV_SPLIT(TB) (c.gated ? launch_int8_split<TB, true>(c, early, device, st) : launch_int8_split<TB, false>(c, early, device, st))
+    const long col_tiles = (c.gated ? c.N / 2 + 63 : c.N + 127) / (c.gated ? 64 : 128);
+    int tb = c.T <= 16 ? 16 : c.T <= 32 ? 32 : c.T <= 64 ? 64 : 128;
+    if (c.T > 64)
+      while (tb > 32 && (c.T + tb - 1) / tb * col_tiles < 100) tb /= 2;
+    if (const char* e = getenv("I8TB")) tb = atoi(e);
+    return tb <= 16 ? INV_SPLIT(16) : tb <= 32 ? INV_SPLIT(32) : tb <= 64 ? INV_SPLIT(64) : INV_SPLIT(128);
+#undef INV_SPLIT
   }
   if (c.gated) return c.out_f32 ? launch_int8_tiles<true, true>(c, early, device, st) : launch_int8_tiles<true, false>(c, early, device, st);
   return c.out_f32 ? launch_int8_tiles<false, true>(c, early, device, st) : launch_int8_tiles<false, false>(c, early, device, st);

@@ -6,22 +6,27 @@
 // every expert to 128 rows and takes seven launches.
 //
 // moe_few_router_kernel   a CTA a token: logits, softmax, the largest entries; clears the counters of the next kernel
-// moe_few_kernel          gate and up products, then down products and their sum, without a launch between them
+// moe_few_kernel          gate and up products, down products and their sum, one CTA an SM, without a launch between them
 //
-// The second kernel's work is a list of items: 16 columns of one expert's gate and up product, then 32 columns of one expert's down product. CTAs draw items in order
-// from a counter. A down item waits until its expert's gate and up items are done; these were all drawn earlier, by CTAs that run and wait for nothing, so every
-// wait ends, whatever else runs on the GPU. Down products of an expert go to memory in fp32; the CTA that finishes the last expert's part of 32 output
-// columns adds them up in the order of the router's choices: no result depends on an order of arrival.
+// The second kernel's work is a list of items: 128 weight rows of one expert's gate and up product (eight and eight in turn) by all of K; then 128 rows of its down
+// product by a part of K; then sums of 128 output columns for four tokens. CTAs draw items in order from a counter. Down items and sums wait for what they
+// read; that comes from items drawn earlier, by CTAs that run, so every wait ends, whatever else runs on the GPU. How K is cut depends on the layer's sizes alone, and
+// the parts are added in one order: a token's result depends on no order of arrival and on no other token. (Gate and up products in parts, added by
+// the warp that finished the last one, made the SMs more even and were slower, 145 us against 114 for 64 tokens of the 24-layer mixture: fences and counters take
+// microseconds in a loaded memory system.)
 //
-// Weights go from memory straight into the fragments of warp-level products, as the 16-row operand; tokens are the other one, eight at a time. (A tcgen05 tile
-// has 128 rows of tokens or weights to fill, of which an item has 32.) Weights in 8 bits become bf16 in registers, exactly; their channel scales are applied to the sums.
+// Weight rows are the 128-row operand of tcgen05 products, all tokens the other one, whichever experts they chose: columns that are not an expert's are computed
+// and not looked at, which costs nothing that counts (128 x 64 x 64 takes 200 cycles, its 16 KB of weights 700 from memory). Down products take an
+// expert's own activations, which lie one behind the other. Weights in 8 bits become bf16 on their way from shared to tensor memory, exactly; their scales are
+// applied to the sums.
+#include "gemm_common.cuh"
 #include "once_per_device.h"
-#include "sm100_common.cuh"
 
 namespace inv {
 
 constexpr int MF_TOKENS = 64, MF_EXPERTS = 256, MF_TOP = 16;
-constexpr int MF_WARPS = 8, MF_SLICE = 128, MF_PL = 36, MF_F = 16, MF_D = 32;
+constexpr int MF_STEPS = 16;                       // of 128 bytes of K, of a down item at most
+constexpr int MF_F = 64, MF_D = 128, MF_GROUP = 4; // columns of a gate and up item, of a down item; tokens of a sum
 
 // What the entry is given; sizes in elements.
 struct MoeFewCall {
@@ -38,47 +43,60 @@ struct MoeFewCall {
   int64_t T, D, F, E, top_k, ldx, ldr, i8, work_bytes;
 };
 
-// Where things stand in the workspace, in bytes.
+// How the work is cut, and where things stand in the workspace, in bytes.
 struct MoeFewPlan {
-  long choice, weight, counters, act, part, bytes;
-  int ld_act, n_counters, slots;
-  __host__ __device__ MoeFewPlan(long T, long D, long F, long E, long top_k, bool shared) {
+  int slots, ld_act, f_tiles, d_tiles, experts, n_counters;
+  int gate_steps, down_steps, down_per, down_parts;    // of K: in all, of a part, parts
+  long choice, weight, counters, act, sums, bytes;
+  MoeFewPlan(long T, long D, long F, long E, long top_k, bool shared, bool i8) {
     auto up = [](long v) { return (v + 255) / 256 * 256; };
+    const int step = i8 ? 128 : 64;
+    gate_steps = (int)((D + step - 1) / step);
+    down_steps = (int)((F + step - 1) / step);
+    down_parts = (down_steps + MF_STEPS - 1) / MF_STEPS;
+    down_per = (down_steps + down_parts - 1) / down_parts;      // equal parts, but for the last
+    down_parts = (down_steps + down_per - 1) / down_per;
     slots = (int)(T * top_k + (shared ? T : 0));
+    experts = (int)((T * top_k < E ? T * top_k : E) + (shared ? 1 : 0));       // that are met, at most
     ld_act = (int)((F + 63) / 64 * 64);
-    n_counters = (int)(1 + E + 1 + (D + MF_D - 1) / MF_D);
+    f_tiles = (int)((F + MF_F - 1) / MF_F);
+    d_tiles = (int)((D + MF_D - 1) / MF_D);
+    n_counters = 1 + experts + d_tiles;
     choice = 0;
     weight = up(choice + T * top_k * 4);
     counters = up(weight + T * top_k * 4);
-    act = up(counters + n_counters * 4);
-    part = up(act + (long)slots * ld_act * 2);
-    bytes = up(part + (long)slots * D * 4);
+    act = up(counters + n_counters * 4L);
+    sums = up(act + (long)slots * ld_act * 2);
+    bytes = up(sums + (long)down_parts * slots * D * 4);
   }
 };
 
 // ---------------------------------------------------------------------------------------------- router
-__global__ void __launch_bounds__(256) moe_few_router_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const __nv_bfloat16* __restrict__ router, int D, int E,
-                                                             int top_k, int* __restrict__ choice, float* __restrict__ weight, int* __restrict__ counters,
-                                                             int n_counters) {
-  __shared__ float logit[MF_EXPERTS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x;
+// 32 warps: slices of D times groups of experts, so that every load of a usual router is on its way at once.
+__global__ void __launch_bounds__(1024) moe_few_router_kernel(const __nv_bfloat16* __restrict__ x, long ldx, const __nv_bfloat16* __restrict__ router, int D, int E,
+                                                              int top_k, int slices, int* __restrict__ choice, float* __restrict__ weight,
+                                                              int* __restrict__ counters, int n_counters) {
+  constexpr int SLICES = 8, AT_ONCE = 8;
+  __shared__ float part[SLICES][MF_EXPERTS], logit[MF_EXPERTS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x, slice = warp & (slices - 1), groups = 32 / slices;
   release_next();
-  if (t == 0)
-    for (int i = tid; i < n_counters; i += 256) counters[i] = 0;
-  const uint4* row = reinterpret_cast<const uint4*>(x + t * ldx);
+  for (int i = t * 1024 + tid; i < n_counters; i += gridDim.x * 1024) counters[i] = 0;
+  const uint4* row = reinterpret_cast<const uint4*>(x + (long)t * ldx);
   const int vecs = D / 8;
-  for (int e0 = warp * 4; e0 < E; e0 += 32) {
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    const uint4* r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = reinterpret_cast<const uint4*>(router + (long)min(e0 + j, E - 1) * D);
-    for (int i = lane; i < vecs; i += 32) {
+  // experts warp / slices, and every groups-th behind it
+  for (int e0 = warp / slices; e0 < E; e0 += groups * AT_ONCE) {
+    float s[AT_ONCE] = {};
+    for (int i = slice * 32 + lane; i < vecs; i += slices * 32) {
       const uint4 a = row[i];
       const uint32_t aw[4] = {a.x, a.y, a.z, a.w};
+      uint4 b[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint4 b = r[j][i];
-        const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+      for (int j = 0; j < AT_ONCE; ++j)
+        if (e0 + j * groups < E) b[j] = reinterpret_cast<const uint4*>(router + (long)(e0 + j * groups) * D)[i];
+#pragma unroll
+      for (int j = 0; j < AT_ONCE; ++j) {
+        if (e0 + j * groups >= E) break;
+        const uint32_t bw[4] = {b[j].x, b[j].y, b[j].z, b[j].w};
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           s[j] = fmaf(__uint_as_float(aw[q] << 16), __uint_as_float(bw[q] << 16), s[j]);
@@ -87,18 +105,27 @@ __global__ void __launch_bounds__(256) moe_few_router_kernel(const __nv_bfloat16
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < AT_ONCE; ++j) {
+      if (e0 + j * groups >= E) break;
 #pragma unroll
       for (int o = 16; o; o >>= 1) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
-      if (lane == 0 && e0 + j < E) logit[e0 + j] = s[j];
+      if (lane == 0) part[slice][e0 + j * groups] = s[j];
     }
+  }
+  __syncthreads();
+  if (tid < E) {
+    float s = 0.f;
+    for (int i = 0; i < slices; ++i) s += part[i][tid];
+    logit[tid] = s;
   }
   __syncthreads();
   if (warp) return;
   constexpr int PER = MF_EXPERTS / 32;
+  const int per = (E + 31) / 32;
   float p[PER], top = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
+    if (j >= per) break;
     p[j] = j * 32 + lane < E ? logit[j * 32 + lane] : -INFINITY;
     top = fmaxf(top, p[j]);
   }
@@ -106,62 +133,77 @@ __global__ void __launch_bounds__(256) moe_few_router_kernel(const __nv_bfloat16
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
+    if (j >= per) break;
     p[j] = j * 32 + lane < E ? expf(p[j] - top) : 0.f;
     sum += p[j];
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  // The largest first, ties to the lowest expert: the bits of numbers that are not negative are ordered as they are, with NaN above all. Every choice is another expert,
-  // whatever the probabilities hold.
-  uint32_t taken = 0;
+  // The largest first, ties to the lowest expert: the bits of numbers that are not negative are ordered as they are, with NaN above all, and one more than them is
+  // above the 0 of what was taken. Every choice is another expert, whatever the probabilities hold.
+  uint32_t key[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (j >= per) break;
+    key[j] = j * 32 + lane < E ? (__float_as_uint(p[j] / sum) & 0x7fffffffu) + 1u : 0u;
+  }
   for (int k = 0; k < top_k; ++k) {
-    unsigned long long best = 0;
+    uint32_t best = 0;
+    int e = MF_EXPERTS;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int e = j * 32 + lane;
-      const unsigned long long key = (unsigned long long)((__float_as_uint(p[j] / sum) & 0x7fffffffu) + 1u) << 32 | (uint32_t)(MF_EXPERTS - e);
-      if (e < E && !(taken >> j & 1) && key > best) best = key;
+      if (j >= per) break;
+      if (key[j] > best) { best = key[j]; e = j * 32 + lane; }
     }
+    const uint32_t most = __reduce_max_sync(0xffffffffu, best);
+    e = __reduce_min_sync(0xffffffffu, best == most ? e : MF_EXPERTS);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-      best = other > best ? other : best;
+    for (int j = 0; j < PER; ++j) {
+      if (j >= per) break;
+      if (e == j * 32 + lane) key[j] = 0u;
     }
-    const int e = MF_EXPERTS - (int)(uint32_t)best;
-    if ((e & 31) == lane) taken |= 1u << (e >> 5);
     if (lane == 0) {
       choice[t * top_k + k] = e;
-      weight[t * top_k + k] = __uint_as_float((uint32_t)(best >> 32) - 1u);
+      weight[t * top_k + k] = __uint_as_float(most - 1u);
     }
   }
 }
 
 // ---------------------------------------------------------------------------------------------- products
 struct MoeFew {
-  const __nv_bfloat16 *x, *residual;
-  const uint8_t *gate_up, *down, *shared_gate_up, *shared_down;
+  const __nv_bfloat16* residual;
   const float *gate_up_scale, *down_scale, *shared_gate_up_scale, *shared_down_scale;
   __nv_bfloat16* out;
   int *counts, *counters, *status;
   const int* choice;
   const float* weight;
   __nv_bfloat16* act;              // [slots, ld_act]
-  float* part;                     // [slots, D]
-  long ldx, ldr;
-  int T, D, F, E, top_k, ld_act, f_tiles, d_tiles;
-  uint32_t inv_f, inv_d;           // div_reciprocal
+  float* sums;                     // [down_parts, slots, D]
+  long ldr;
+  int T, D, F, E, top_k, shared, ld_act, slots, f_tiles, d_tiles, experts;
+  int gate_steps, down_steps, down_per, down_parts;
+  uint32_t inv_k, inv_f, inv_down, inv_down_parts, inv_d;   // div_reciprocal
 };
 
-__device__ __forceinline__ void mf_mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint4 mf_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
+namespace mf {
+constexpr int A_STAGE = 128 * 128, QUEUE = 8, ACC = 4, CONV = 4;
+// Bytes of a weight row's step are 128: 64 or 128 values of K.
+template <int TB, bool I8>
+struct Shape {
+  static constexpr int STEP = I8 ? 128 : 64, B_STAGE = (I8 ? 2 : 1) * TB * 128, ROOM = (220 * 1024 - 1024) / (A_STAGE + B_STAGE),
+                       SETS = I8 ? 2 : 3;   // of four warps of sums; conversions take the threads of the third
+  static constexpr int STAGES = ROOM < 12 ? ROOM : 12, SUMS = 3, CONVERT = SUMS + 4 * SETS,
+                       THREADS = 32 * (CONVERT + (I8 ? 4 * CONV : 0));    // warps of loads, of products, of items, of sums, of conversions
+  static constexpr int SMEM = STAGES * (A_STAGE + B_STAGE) + 1024;
+  static constexpr int COLS = ACC * TB + (I8 ? CONV * 64 : 0), TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+};
+enum Kind { GATE, DOWN, SUM, END };
+struct __align__(16) Item {
+  int kind, a, tile, part;         // a: which of the experts that are met; SUM: part: the group of tokens
+  int e, first, k0, steps;         // e: the expert, E for the shared one; its first slot; steps of K
+};
+}  // namespace mf
+
 // Four codes into bf16: 128 + (the lower seven bits), less 128, or 256 where the sign bit is set. Each is a number of eight bits, so nothing is rounded.
 __device__ __forceinline__ void mf_widen(uint32_t v, uint32_t& lo, uint32_t& hi) {
   const uint32_t m = v & 0x7f7f7f7fu, s = v & 0x80808080u, c = 0x43434343u;
@@ -176,33 +218,119 @@ __device__ __forceinline__ int mf_acquire(const int* p) {
   asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
+__device__ __forceinline__ void mf_release(int* p) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(p) : "memory");
+}
+__device__ __forceinline__ void mf_fence_proxy() { asm volatile("fence.proxy.async;" ::: "memory"); }
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m, uint64_t* bar, int c0, int c1, int c2, int c3, int c4) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+      : "memory");
+}
+// Asks without waiting, which mbarrier.try_wait does for tens of microseconds.
+__device__ __forceinline__ bool mf_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Until *p reaches n. False where the limit runs out.
+__device__ __forceinline__ bool mf_wait(const int* p, int n, volatile int* abort_flag, int* status) {
+  uint64_t t0 = 0;
+  for (uint32_t spins = 1; mf_acquire(p) < n; ++spins) {
+    if (spins & 0xff) continue;
+    if (*abort_flag) return false;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    else if (now - t0 > INV_WAIT_LIMIT_NS) {
+      *abort_flag = 1;
+      atomicCAS(status, 0, (int)ERR_WAIT_MISC);
+      return false;
+    }
+  }
+  return true;
+}
 
-// NT: tokens of an expert, in eights. I8: weights in 8 bits.
-template <int NT, bool I8>
-__global__ void __launch_bounds__(MF_WARPS * 32, 2) moe_few_kernel(const MoeFew p) {
-  constexpr int THREADS = MF_WARPS * 32, UN = NT <= 4 ? 2 : 1, SLOTS = MF_TOKENS * (MF_TOP + 1);
-  constexpr int ES = I8 ? 1 : 2;                           // bytes of a weight
-  extern __shared__ float mf_part[];                       // [MF_WARPS][8 NT][MF_PL]
-  __shared__ int s_first[MF_EXPERTS + 2];                  // first slot of an expert; E: the shared one's
-  __shared__ uint16_t s_active[MF_EXPERTS + 1], s_token[SLOTS], s_slot[MF_TOKENS * MF_TOP];
-  __shared__ int s_next, s_last, s_n;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
-  const int chosen = p.T * p.top_k;
+template <int TB, bool I8>
+__global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
+    moe_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_act, const __grid_constant__ CUtensorMap map_gate,
+                   const __grid_constant__ CUtensorMap map_down, const __grid_constant__ CUtensorMap map_shared_gate,
+                   const __grid_constant__ CUtensorMap map_shared_down, const __grid_constant__ MoeFew p) {
+  using namespace mf;
+  using S = Shape<TB, I8>;
+  constexpr int STAGES = S::STAGES, B_STAGE = S::B_STAGE, STEP = S::STEP;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], item_full[QUEUE], item_empty[QUEUE], acc_full[ACC], acc_empty[ACC], conv_full[CONV], conv_empty[CONV];
+  __shared__ uint32_t s_mask[MF_EXPERTS + 1][2];                 // tokens of an expert; E: of the shared one
+  __shared__ uint16_t s_index[MF_EXPERTS], s_expert[MF_EXPERTS + 1], s_first[MF_EXPERTS + 2], s_slot[MF_TOKENS * MF_TOP];
+  __shared__ Item s_item[QUEUE];
+  __shared__ int s_n;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int s_abort;
+  volatile int* abort_flag = &s_abort;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * A_STAGE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, chosen = p.T * p.top_k;
+
   release_next();
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&full_bar[i], 1);
+      mbar_init(&empty_bar[i], 1);
+    }
+    for (int i = 0; i < QUEUE; ++i) {
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 2 + 4 * S::SETS + (I8 ? 4 * CONV : 0));
+    }
+    for (int i = 0; i < ACC; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 4);
+    }
+    for (int i = 0; i < CONV; ++i) {
+      mbar_init(&conv_full[i], 4);
+      mbar_init(&conv_empty[i], 1);
+    }
+    s_abort = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&map_gate);
+    tma_prefetch_desc(&map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, S::TMEM);
+    tmem_relinquish();
+  }
+  for (int i = tid; i < 2 * (MF_EXPERTS + 1); i += S::THREADS) (&s_mask[0][0])[i] = 0;
+  tc_fence_before();
   wait_previous();
-  if (tid == 0) s_next = atomicAdd(p.counters, 2);
-  // Slots: the choices in the order of their experts, tokens in order within an expert.
-  int* s_count = reinterpret_cast<int*>(mf_part);          // before it holds sums
-  for (int e = warp; e < p.E; e += MF_WARPS) {
-    int n = 0;
-    for (int i = 0; i < chosen; i += 32) n += __popc(__ballot_sync(0xffffffffu, i + lane < chosen && p.choice[i + lane] == e));
-    if (lane == 0) s_count[e] = n;
+  int ticket = 0;
+  if (warp == 2 && lane == 0) ticket = atomicAdd(p.counters, 1);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = tmem_slot;
+
+  // Who goes where: the tokens of each expert, the experts that are met, and a slot for each choice, in the order of experts and of tokens within one.
+  for (int i = tid; i < chosen; i += S::THREADS) {
+    const int t = div_by(i, p.top_k, p.inv_k);
+    atomicOr(&s_mask[p.choice[i]][t >> 5], 1u << (t & 31));
+  }
+  if (p.shared && tid == 0) {
+    s_mask[p.E][0] = p.T >= 32 ? 0xffffffffu : (1u << p.T) - 1;
+    s_mask[p.E][1] = p.T >= 64 ? 0xffffffffu : p.T > 32 ? (1u << (p.T - 32)) - 1 : 0u;
   }
   __syncthreads();
   if (warp == 0) {
     int first = 0, active = 0;
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int n = e0 + lane < p.E ? s_count[e0 + lane] : 0;
+    for (int e0 = 0; e0 < p.E + p.shared; e0 += 32) {
+      const int e = e0 + lane, n = e < p.E + p.shared ? __popc(s_mask[e][0]) + __popc(s_mask[e][1]) : 0;
       int sum = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -210,237 +338,350 @@ __global__ void __launch_bounds__(MF_WARPS * 32, 2) moe_few_kernel(const MoeFew 
         if (lane >= o) sum += v;
       }
       const uint32_t has = __ballot_sync(0xffffffffu, n > 0);
-      if (e0 + lane < p.E) {
-        s_first[e0 + lane] = first + sum - n;
-        if (n > 0) s_active[active + __popc(has & ((1u << lane) - 1))] = (uint16_t)(e0 + lane);
-        if (blockIdx.x == 0) p.counts[e0 + lane] = n;
+      const int a = active + __popc(has & ((1u << lane) - 1));
+      if (n > 0) {
+        s_expert[a] = (uint16_t)e;
+        s_first[a] = (uint16_t)(first + sum - n);
+      }
+      if (e < p.E) {
+        s_index[e] = (uint16_t)a;
+        if (blockIdx.x == 0) p.counts[e] = n;
       }
       first += __shfl_sync(0xffffffffu, sum, 31);
       active += __popc(has);
     }
     if (lane == 0) {
-      s_first[p.E] = first;
-      if (p.shared_gate_up != nullptr) {
-        s_active[active++] = (uint16_t)p.E;
-        s_first[p.E + 1] = first + p.T;
-      }
+      s_first[active] = (uint16_t)first;
       s_n = active;
     }
   }
   __syncthreads();
-  for (int e = warp; e < p.E; e += MF_WARPS) {
-    int at = s_first[e];
-    if (s_first[e + 1] == at) continue;
-    for (int i = 0; i < chosen; i += 32) {
-      const bool mine = i + lane < chosen && p.choice[i + lane] == e;
-      const uint32_t has = __ballot_sync(0xffffffffu, mine);
-      if (mine) {
-        const int slot = at + __popc(has & ((1u << lane) - 1));
-        s_slot[i + lane] = (uint16_t)slot;
-        s_token[slot] = (uint16_t)((i + lane) / p.top_k);
-      }
-      at += __popc(has);
-    }
+  for (int i = tid; i < chosen; i += S::THREADS) {
+    const int t = div_by(i, p.top_k, p.inv_k), e = p.choice[i];
+    const int below = t < 32 ? __popc(s_mask[e][0] & ((1u << t) - 1)) : __popc(s_mask[e][0]) + __popc(s_mask[e][1] & ((1u << (t - 32)) - 1));
+    s_slot[i] = (uint16_t)(s_first[s_index[e]] + below);
   }
-  if (p.shared_gate_up != nullptr)
-    for (int t = tid; t < p.T; t += THREADS) s_token[chosen + t] = (uint16_t)t;
   __syncthreads();
 
-  const int n_active = s_n, n_gate = n_active * p.f_tiles, n_items = n_gate + n_active * p.d_tiles;
-  struct Item {
-    int a, tile;
-    bool down;
-  };
-  auto decode = [&](int i) {
-    Item it;
-    it.down = i >= n_gate;
-    const int j = it.down ? i - n_gate : i;
-    it.a = it.down ? div_by(j, p.d_tiles, p.inv_d) : div_by(j, p.f_tiles, p.inv_f);
-    it.tile = j - it.a * (it.down ? p.d_tiles : p.f_tiles);
-    return it;
-  };
-  auto slices_of = [&](bool down) { return ((down ? p.F : p.D) * ES + MF_SLICE - 1) / MF_SLICE; };
-  uint4 ring[UN][4][2];
-  auto fetch = [&](const Item& it, int s, uint4 (&r)[4][2]) {
-    const int e = s_active[it.a], width = (it.down ? p.F : p.D) * ES, rows = it.down ? p.D : 2 * p.F, at = s * MF_SLICE + tig * 32;
-    const uint8_t* from = it.down ? (e == p.E ? p.shared_down : p.down) : (e == p.E ? p.shared_gate_up : p.gate_up);
-    from += (long)(e == p.E ? 0 : e) * rows * width + at;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int row = it.down ? min(it.tile * MF_D + t * 8 + g, p.D - 1) : min(it.tile * MF_F + (t & 1) * 8 + g, p.F - 1) + (t >> 1) * p.F;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) r[t][i] = at + 16 * i < width ? mf_stream(from + (long)row * width + 16 * i) : make_uint4(0, 0, 0, 0);
+  const int n_active = s_n, per_down = p.d_tiles * p.down_parts, n_gate = n_active * p.f_tiles, n_down = n_gate + n_active * per_down, n_items = n_down + p.d_tiles * ((p.T + MF_GROUP - 1) / MF_GROUP);
+  int* done = p.counters + 1;                      // [experts] warps that have written activations
+  int* down_done = done + p.experts;               // [d_tiles] warps that have written sums
+
+  if (warp == 2) {
+    // ---------------- items: drawn and described for the others ----------------
+    if (lane == 0) {
+      int qi = 0;
+      uint32_t qph = 1;
+      while (true) {
+        const int next = ticket < n_items ? atomicAdd(p.counters, 1) : ticket;      // on its way while this one is described
+        Item it;
+        int i = ticket;
+        it.a = it.e = it.first = it.k0 = it.steps = 0;
+        if (i < n_gate) {
+          it.kind = GATE;
+          it.a = div_by(i, p.f_tiles, p.inv_f);
+          it.tile = i - it.a * p.f_tiles;
+          it.part = 0;
+          it.steps = p.gate_steps;
+        } else if (i < n_down) {
+          it.kind = DOWN;
+          i -= n_gate;
+          it.a = div_by(i, per_down, p.inv_down);
+          i -= it.a * per_down;
+          it.tile = div_by(i, p.down_parts, p.inv_down_parts);
+          it.part = i - it.tile * p.down_parts;
+          it.k0 = it.part * p.down_per;
+          it.steps = min(p.down_per, p.down_steps - it.k0);
+        } else {
+          it.kind = i < n_items ? SUM : END;
+          i -= n_down;
+          it.part = div_by(i, p.d_tiles, p.inv_d);
+          it.tile = i - it.part * p.d_tiles;
+        }
+        if (it.kind <= DOWN) {
+          it.e = s_expert[it.a];
+          it.first = s_first[it.a];
+        }
+        if (!mbar_wait(&item_empty[qi], qph, abort_flag, p.status, ERR_WAIT_MISC)) break;
+        s_item[qi] = it;
+        mbar_arrive(&item_full[qi]);
+        if (++qi == QUEUE) { qi = 0; qph ^= 1; }
+        if (it.kind == END) break;
+        ticket = next;
+      }
     }
-  };
-  int now = s_next, next = now + 1;
-  Item it = decode(now);
-  if (now < n_items) {
-    const int slices = slices_of(it.down);
+  } else if (warp == 0) {
+    // ---------------- loads ----------------
+    if (elect_one_sync()) {
+      int s = 0, qi = 0, ready = -1;               // experts up to `ready` have their activations
+      uint32_t ph = 1, qph = 0;
+      bool ok = true;
+      while (ok) {
+        if (!mbar_wait(&item_full[qi], qph, abort_flag, p.status, ERR_WAIT_MISC)) break;
+        const Item it = s_item[qi];
+        mbar_arrive(&item_empty[qi]);
+        if (++qi == QUEUE) { qi = 0; qph ^= 1; }
+        if (it.kind == END) break;
+        if (it.kind == SUM) continue;
+        const int e = it.e, k0 = it.k0, steps = it.steps;
+        const bool shared = e == p.E;
+        const CUtensorMap* map = it.kind == GATE ? (shared ? &map_shared_gate : &map_gate) : (shared ? &map_shared_down : &map_down);
+        auto weights = [&](int i, int at) {
+          mbar_expect_tx(&full_bar[at], A_STAGE + B_STAGE);
+          const int k = (k0 + i) * STEP, plane = shared ? 0 : e;
+          if (it.kind == GATE) tma_load_5d(sA + at * A_STAGE, map, &full_bar[at], k, 0, 0, it.tile * (MF_F / 8), plane);
+          else tma_load_3d(sA + at * A_STAGE, map, &full_bar[at], k, it.tile * MF_D, plane);
+        };
+        auto tokens = [&](int i, int at) {
 #pragma unroll
-    for (int u = 0; u < UN; ++u)
-      if (warp + u * MF_WARPS < slices) fetch(it, warp + u * MF_WARPS, ring[u]);
-  }
-  while (now < n_items) {
-    const Item nx = decode(next);
-    const int slices = slices_of(it.down), ahead = next < n_items ? slices_of(nx.down) : 0, width = it.down ? p.F : p.D;
-    const int e = s_active[it.a], first = s_first[e], n = s_first[e + 1] - first;
-    __syncthreads();                                       // s_next and the sums of the last item have been read
-    if (tid == 0) {
-      s_next = atomicAdd(p.counters, 1);
-      if (it.down) {                                       // the expert's activations: written by CTAs that drew their items before this one
-        const int* done = p.counters + 1 + it.a;
-        uint64_t t0 = 0;
-        for (uint32_t spins = 1; mf_acquire(done) < p.f_tiles; ++spins) {
-          if (spins & 0xff) continue;
-          const uint64_t clock = globaltimer_ns();
-          if (t0 == 0) t0 = clock;
-          else if (clock - t0 > INV_WAIT_LIMIT_NS) {
-            atomicCAS(p.status, 0, (int)ERR_WAIT_MISC);
-            break;
+          for (int h = 0; h < (I8 ? 2 : 1); ++h) {
+            if (it.kind == GATE) tma_load_2d(sB + at * B_STAGE + h * TB * 128, &map_x, &full_bar[at], (k0 + i) * STEP + 64 * h, 0);
+            else tma_load_2d(sB + at * B_STAGE + h * TB * 128, &map_act, &full_bar[at], (k0 + i) * STEP + 64 * h, it.first);
           }
+        };
+        int i = 0;
+        if (it.kind == DOWN && it.a > ready) {     // its weights may come before its activations are there
+          int at = s;
+          uint32_t aph = ph;
+          for (; i < steps && i < STAGES && mf_test(&empty_bar[at], aph); ++i) {
+            weights(i, at);
+            if (++at == STAGES) { at = 0; aph ^= 1; }
+          }
+          // a load whose other half never comes would be waited for in vain: it is sent in any case
+          ok = mf_wait(&done[it.a], p.f_tiles * 4, abort_flag, p.status);
+          mf_fence_proxy();
+          ready = it.a;
+          for (int j = 0; j < i; ++j) {
+            tokens(j, s);
+            if (++s == STAGES) { s = 0; ph ^= 1; }
+          }
+          if (!ok) break;
+        }
+        for (; i < steps; ++i) {
+          if (!mbar_wait(&empty_bar[s], ph, abort_flag, p.status, ERR_WAIT_EMPTY)) { ok = false; break; }
+          weights(i, s);
+          tokens(i, s);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
         }
       }
     }
-    if (it.down) __syncthreads();
-    const __nv_bfloat16* xp[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int slot = first + min(j * 8 + g, n - 1);
-      xp[j] = (it.down ? p.act + (long)slot * p.ld_act : p.x + (long)s_token[slot] * p.ldx) + tig * 32 / ES;
-    }
-#pragma unroll
-    for (int u = 0; u < UN; ++u)                           // a place that this item has no slice for
-      if (warp + u * MF_WARPS >= slices && warp + u * MF_WARPS < ahead) fetch(nx, warp + u * MF_WARPS, ring[u]);
-    float acc[NT][2][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[j][i / 4][i % 4] = 0.f;
-    for (int s0 = warp; s0 < slices; s0 += UN * MF_WARPS) {
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        const int s = s0 + u * MF_WARPS;
-        if (s >= slices) break;
-        const int k0 = s * (MF_SLICE / ES), left = width - k0 - tig * 32 / ES;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
+  } else if (warp == 1) {
+    // ---------------- products ----------------
+    if (elect_one_sync()) {
+      constexpr uint32_t idesc = make_idesc_bf16(128, TB, 0, 0);
+      const uint64_t da0 = make_smem_desc(smem_u32(sA), 16, 1024, 2), db0 = make_smem_desc(smem_u32(sB), 16, 1024, 2);
+      int s = 0, qi = 0, acc = 0, cv = 0;
+      uint32_t ph = 0, qph = 0, accph = 1, cvph = 0;
+      bool ok = true;
+      while (ok) {
+        if (!mbar_wait(&item_full[qi], qph, abort_flag, p.status, ERR_WAIT_MISC)) break;
+        const int kind = s_item[qi].kind, steps = s_item[qi].steps;
+        mbar_arrive(&item_empty[qi]);
+        if (++qi == QUEUE) { qi = 0; qph ^= 1; }
+        if (kind == END) break;
+        if (kind == SUM) continue;
+        if (!mbar_wait(&acc_empty[acc], accph, abort_flag, p.status, ERR_WAIT_TMEM_EMPTY)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + acc * TB;
+        for (int j = 0; j < steps; ++j) {
+          if (!mbar_wait(&full_bar[s], ph, abort_flag, p.status, ERR_WAIT_FULL)) { ok = false; break; }
+          if (I8 && !mbar_wait(&conv_full[cv], cvph, abort_flag, p.status, ERR_WAIT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t db = db0 + (uint64_t)(s * (B_STAGE >> 4));
           if constexpr (I8) {
+            const uint32_t a = tmem_base + ACC * TB + cv * 64;
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              uint32_t lo[8], hi[8];
-              const uint4 a = ring[u][2 * m][i], b = ring[u][2 * m + 1][i];
-              mf_widen(a.x, lo[0], lo[1]); mf_widen(a.y, lo[2], lo[3]); mf_widen(a.z, lo[4], lo[5]); mf_widen(a.w, lo[6], lo[7]);
-              mf_widen(b.x, hi[0], hi[1]); mf_widen(b.y, hi[2], hi[3]); mf_widen(b.z, hi[4], hi[5]); mf_widen(b.w, hi[6], hi[7]);
-#pragma unroll
-              for (int j = 0; j < NT; ++j) {
-                if (j && j * 8 >= n) break;
-                uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-                if (left > 16 * i) {
-                  v0 = *reinterpret_cast<const uint4*>(xp[j] + k0 + 16 * i);
-                  v1 = *reinterpret_cast<const uint4*>(xp[j] + k0 + 16 * i + 8);
-                }
-                mf_mma(acc[j][m], lo[0], hi[0], lo[1], hi[1], v0.x, v0.y);
-                mf_mma(acc[j][m], lo[2], hi[2], lo[3], hi[3], v0.z, v0.w);
-                mf_mma(acc[j][m], lo[4], hi[4], lo[5], hi[5], v1.x, v1.y);
-                mf_mma(acc[j][m], lo[6], hi[6], lo[7], hi[7], v1.z, v1.w);
-              }
-            }
+            for (int k = 0; k < 8; ++k) umma_bf16_tmem_a(d, a + k * 8, db + (k & 3) * 2 + (k >> 2) * (TB * 128 >> 4), idesc, j > 0 || k > 0 ? 1u : 0u);
+            umma_commit(&conv_empty[cv]);
+            if (++cv == CONV) { cv = 0; cvph ^= 1; }
           } else {
+            const uint64_t da = da0 + (uint64_t)(s * (A_STAGE >> 4));
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              if (j && j * 8 >= n) break;
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (left > 8 * i) v = *reinterpret_cast<const uint4*>(xp[j] + k0 + 8 * i);
+            for (int k = 0; k < 4; ++k) umma_bf16(d, da + k * 2, db + k * 2, idesc, j > 0 || k > 0 ? 1u : 0u);
+          }
+          umma_commit(&empty_bar[s]);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+        if (!ok) break;
+        umma_commit(&acc_full[acc]);
+        if (++acc == ACC) { acc = 0; accph ^= 1; }
+      }
+    }
+  } else if (warp < S::CONVERT) {
+    // ---------------- sums: sets of four warps take items in turn, since an item's fences and counters take longer than its products ----------------
+    const int q = warp & 3, row = q * 32 + lane;           // the lanes of tensor memory that this warp may read
+    const int set = (warp - S::SUMS) >> 2;
+    int qi = 0, turn = 0, next_acc = 0;
+    uint32_t qph = 0, next_accph = 0;
+    while (true) {
+      if (!mbar_wait_warp(&item_full[qi], qph, abort_flag, p.status, ERR_WAIT_MISC)) break;
+      const Item it = s_item[qi];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[qi]);
+      if (++qi == QUEUE) { qi = 0; qph ^= 1; }
+      if (it.kind == END) break;
+      const bool mine = turn == set;
+      if (++turn == S::SETS) turn = 0;
+      const int acc = next_acc;
+      const uint32_t accph = next_accph;
+      if (it.kind != SUM && ++next_acc == ACC) { next_acc = 0; next_accph ^= 1; }
+      if (!mine) continue;
+      if (it.kind == SUM) {
+        bool there = true;
+        if (lane == 0) there = mf_wait(&down_done[it.tile], n_active * p.down_parts * 4, abort_flag, p.status);
+        if (!__shfl_sync(0xffffffffu, there, 0)) break;
+        // eight lanes of a warp have 32 columns between them and add every fourth part; the four groups of lanes add up theirs
+        const int col = it.tile * MF_D + q * 32 + (lane & 7) * 4, t0 = it.part * MF_GROUP;
+        float y[MF_GROUP][4] = {};
+        if (col < p.D) {
+          for (int k = p.shared ? -1 : 0; k < p.top_k; ++k) {
+            float w[MF_GROUP];
+            const float* from[MF_GROUP];
 #pragma unroll
-              for (int m = 0; m < 2; ++m) {
-                const uint4 lo = ring[u][2 * m][i], hi = ring[u][2 * m + 1][i];
-                mf_mma(acc[j][m], lo.x, hi.x, lo.y, hi.y, v.x, v.y);
-                mf_mma(acc[j][m], lo.z, hi.z, lo.w, hi.w, v.z, v.w);
-              }
+            for (int j = 0; j < MF_GROUP; ++j) {
+              const int t = min(t0 + j, p.T - 1), c = t * p.top_k + max(k, 0);
+              w[j] = k < 0 ? 1.f : p.weight[c];
+              from[j] = p.sums + (long)(k < 0 ? chosen + t : s_slot[c]) * p.D + col;
             }
+#pragma unroll 2
+            for (int part = lane >> 3; part < p.down_parts; part += 4)
+#pragma unroll
+              for (int j = 0; j < MF_GROUP; ++j) {
+                const float4 u = __ldcg(reinterpret_cast<const float4*>(from[j] + (long)part * p.slots * p.D));
+                y[j][0] = fmaf(w[j], u.x, y[j][0]); y[j][1] = fmaf(w[j], u.y, y[j][1]); y[j][2] = fmaf(w[j], u.z, y[j][2]); y[j][3] = fmaf(w[j], u.w, y[j][3]);
+              }
           }
         }
-        const int then = s + UN * MF_WARPS;
-        if (then < slices) fetch(it, then, ring[u]);
-        else if (warp + u * MF_WARPS < ahead) fetch(nx, warp + u * MF_WARPS, ring[u]);
-      }
-    }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      if (j && j * 8 >= n) break;
+        for (int j = 0; j < MF_GROUP; ++j) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        float* to = mf_part + ((warp * NT + j) * 8 + 2 * tig) * MF_PL + m * 16 + g;
-        to[0] = acc[j][m][0];
-        to[MF_PL] = acc[j][m][1];
-        to[8] = acc[j][m][2];
-        to[MF_PL + 8] = acc[j][m][3];
-      }
-    }
-    __syncthreads();
-    if (!it.down) {
-      for (int i = tid; i < n * MF_F; i += THREADS) {
-        const int j = i / MF_F, c = i % MF_F, f = it.tile * MF_F + c;
-        if (f >= p.F) continue;
-        float a = 0.f, b = 0.f;
-#pragma unroll
-        for (int w = 0; w < MF_WARPS; ++w) {
-          a += mf_part[(w * NT * 8 + j) * MF_PL + c];
-          b += mf_part[(w * NT * 8 + j) * MF_PL + MF_F + c];
+          for (int x = 0; x < 4; ++x) {
+            y[j][x] += __shfl_xor_sync(0xffffffffu, y[j][x], 8);
+            y[j][x] += __shfl_xor_sync(0xffffffffu, y[j][x], 16);
+          }
+          const int t = t0 + j;
+          if (lane >> 3 == j && t < p.T && col < p.D) {
+            if (p.residual != nullptr) {
+              const uint2 r = *reinterpret_cast<const uint2*>(p.residual + t * p.ldr + col);
+              y[j][0] += __uint_as_float(r.x << 16); y[j][1] += __uint_as_float(r.x & 0xffff0000u);
+              y[j][2] += __uint_as_float(r.y << 16); y[j][3] += __uint_as_float(r.y & 0xffff0000u);
+            }
+            *reinterpret_cast<uint2*>(p.out + (long)t * p.D + col) = make_uint2(pack_bf16x2(y[j][0], y[j][1]), pack_bf16x2(y[j][2], y[j][3]));
+          }
         }
-        if (I8) {
-          const float* s = e == p.E ? p.shared_gate_up_scale : p.gate_up_scale + (long)e * 2 * p.F;
-          a *= s[f];
-          b *= s[p.F + f];
-        }
-        // rounded to bf16, the type of the next product's operands
-        p.act[(long)(first + j) * p.ld_act + f] = __float2bfloat16_rn(a / (1.f + expf(-a)) * b);
+        continue;
       }
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        atomicAdd(p.counters + 1 + it.a, 1);
+      const int e = it.e, first = it.first, n = s_first[it.a + 1] - first;
+      const bool shared = e == p.E;
+      const uint64_t mask = (uint64_t)s_mask[e][1] << 32 | s_mask[e][0];
+      // gate and up items: lanes of a warp hold eight columns of the gate, the same of the up product, and the next eight likewise
+      const int f = it.tile * MF_F + q * 16 + (lane >> 4) * 8 + (lane & 7), col = it.tile * MF_D + row;
+      float scale = 1.f;
+      if (I8) {
+        if (it.kind == GATE) scale = f < p.F ? (shared ? p.shared_gate_up_scale : p.gate_up_scale + (long)e * 2 * p.F)[f + (lane >> 3 & 1) * p.F] : 0.f;
+        else scale = col < p.D ? (shared ? p.shared_down_scale : p.down_scale + (long)e * p.D)[col] : 0.f;
       }
-    } else {
-      for (int i = tid; i < n * MF_D; i += THREADS) {
-        const int j = i / MF_D, c = i % MF_D, col = it.tile * MF_D + c;
-        if (col >= p.D) continue;
-        float a = 0.f;
+      auto activate = [&](float v, int slot) {             // rounded to bf16, the type of the next product's operands
+        v *= scale;
+        const float up = __shfl_down_sync(0xffffffffu, v, 8);
+        if (!(lane & 8) && f < p.F) p.act[(long)slot * p.ld_act + f] = __float2bfloat16_rn(v / (1.f + expf(-v)) * up);
+      };
+      if (!mbar_wait_warp(&acc_full[acc], accph, abort_flag, p.status, ERR_WAIT_TMEM_FULL)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + acc * TB + (uint32_t(q * 32) << 16);
+      float* to = p.sums + ((long)it.part * p.slots + first) * p.D + col;
+      int slot = 0;                                        // within the expert
+#pragma unroll 1
+      for (int c = 0; c < TB; c += 16) {
+        const uint32_t bits = it.kind == GATE ? (uint32_t)(mask >> c) & 0xffffu : c + 16 <= n ? 0xffffu : c < n ? (1u << (n - c)) - 1 : 0u;
+        if (bits == 0) continue;
+        uint32_t r[16];
+        tmem_ld_32x16(taddr + c, r);
+        tmem_ld_wait();
 #pragma unroll
-        for (int w = 0; w < MF_WARPS; ++w) a += mf_part[(w * NT * 8 + j) * MF_PL + c];
-        if (I8) a *= (e == p.E ? p.shared_down_scale : p.down_scale + (long)e * p.D)[col];
-        p.part[(long)(first + j) * p.D + col] = a;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        s_last = atomicAdd(p.counters + 1 + p.E + 1 + it.tile, 1) == n_active - 1;
-        __threadfence();
-      }
-      __syncthreads();
-      if (s_last) {
-        for (int i = tid; i < p.T * MF_D; i += THREADS) {
-          const int t = i / MF_D, col = it.tile * MF_D + i % MF_D;
-          if (col >= p.D) continue;
-          float y = p.residual == nullptr ? 0.f : __bfloat162float(p.residual[t * p.ldr + col]);
-          if (p.shared_gate_up != nullptr) y += __ldcg(p.part + (long)(chosen + t) * p.D + col);
-          for (int k = 0; k < p.top_k; ++k) y = fmaf(p.weight[t * p.top_k + k], __ldcg(p.part + (long)s_slot[t * p.top_k + k] * p.D + col), y);
-          p.out[(long)t * p.D + col] = __float2bfloat16_rn(y);
+        for (int j = 0; j < 16; ++j) {
+          if (!(bits >> j & 1)) continue;
+          const float v = __uint_as_float(r[j]);
+          if (it.kind == GATE) activate(v, first + slot);
+          else if (col < p.D) to[(long)slot * p.D] = v * scale;
+          ++slot;
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+      if (it.kind == GATE) mf_fence_proxy();               // activations are read by bulk copies
+      __syncwarp();
+      if (lane == 0) mf_release(it.kind == GATE ? &done[it.a] : &down_done[it.tile]);
     }
-    now = next;
-    next = s_next;
-    it = nx;
+  } else if constexpr (I8) {
+    // ---------------- conversions: groups of four warps take steps in turn, one buffer each ----------------
+    const int q = warp & 3, row = q * 32 + lane, group = (warp - S::CONVERT) >> 2;
+    int s = 0, qi = 0, cv = 0;
+    uint32_t ph = 0, qph = 0, cvph = 1;
+    bool ok = true;
+    while (ok) {
+      if (!mbar_wait_warp(&item_full[qi], qph, abort_flag, p.status, ERR_WAIT_MISC)) break;
+      const int kind = s_item[qi].kind, steps = s_item[qi].steps;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[qi]);
+      if (++qi == QUEUE) { qi = 0; qph ^= 1; }
+      if (kind == END) break;
+      if (kind == SUM) continue;
+      for (int j = 0; j < steps; ++j) {
+        if (cv == group) {
+          if (!mbar_wait_warp(&full_bar[s], ph, abort_flag, p.status, ERR_WAIT_FULL) ||
+              !mbar_wait_warp(&conv_empty[cv], cvph, abort_flag, p.status, ERR_WAIT_EMPTY)) { ok = false; break; }
+          tc_fence_after();
+          const uint8_t* from = sA + s * A_STAGE + row * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const uint4 v = *reinterpret_cast<const uint4*>(from + (((4 * h + c) ^ (row & 7)) << 4));
+              mf_widen(v.x, w[8 * c], w[8 * c + 1]);
+              mf_widen(v.y, w[8 * c + 2], w[8 * c + 3]);
+              mf_widen(v.z, w[8 * c + 4], w[8 * c + 5]);
+              mf_widen(v.w, w[8 * c + 6], w[8 * c + 7]);
+            }
+            tmem_st_32x32(tmem_base + ACC * TB + cv * 64 + h * 32 + (uint32_t(q * 32) << 16), w);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&conv_full[cv]);
+        }
+        if (++s == STAGES) { s = 0; ph ^= 1; }
+        if (++cv == CONV) { cv = 0; cvph ^= 1; }
+      }
+    }
+  }
+
+  __syncwarp();
+  __syncthreads();
+  if (s_abort) {                                           // let what is under way end before the memory it uses is given up
+    const uint64_t since = globaltimer_ns();
+    while (globaltimer_ns() - since < 2000000ull) __nanosleep(1000);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, S::TMEM);
   }
 }
 
-template <int NT, bool I8>
-static int launch_moe_few(const MoeFew& p, int items, int device, cudaStream_t st) {
-  constexpr int bytes = MF_WARPS * NT * 8 * MF_PL * 4;
+struct MoeFewMaps {
+  CUtensorMap x, act, gate, down, shared_gate, shared_down;
+};
+
+template <int TB, bool I8>
+static int launch_moe_few(const MoeFewMaps& m, const MoeFew& p, int grid, int device, cudaStream_t st) {
+  using S = mf::Shape<TB, I8>;
   static OncePerDevice once;
-  if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(moe_few_kernel<NT, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); })) return -e;
-  launch_early(moe_few_kernel<NT, I8>, dim3(items < 296 ? items : 296), MF_WARPS * 32, bytes, st, p);
+  if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(moe_few_kernel<TB, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); })) return -e;
+  launch_early(moe_few_kernel<TB, I8>, dim3(grid), S::THREADS, S::SMEM, st, m.x, m.act, m.gate, m.down, m.shared_gate, m.shared_down, p);
   return -(int)cudaGetLastError();
 }
 
@@ -448,41 +689,58 @@ static int launch_moe_few(const MoeFew& p, int items, int device, cudaStream_t s
 
 using namespace inv;
 
-extern "C" long inv_moe_few_bytes(long T, long D, long F, long E, long top_k, int shared) { return MoeFewPlan(T, D, F, E, top_k, shared != 0).bytes; }
+extern "C" long inv_moe_few_bytes(long T, long D, long F, long E, long top_k, int shared, int i8) {
+  return MoeFewPlan(T, D, F, E, top_k, shared != 0, i8 != 0).bytes;
+}
 
 extern "C" int inv_moe_few(const void* call) {
   const MoeFewCall& c = *static_cast<const MoeFewCall*>(call);
   if (c.T <= 0) return 0;
   const int grain = c.i8 ? 16 : 8;
-  const MoeFewPlan plan(c.T, c.D, c.F, c.E, c.top_k, c.shared_gate_up != nullptr);
-  if (c.T > MF_TOKENS || c.E < 1 || c.E > MF_EXPERTS || c.top_k < 1 || c.top_k > MF_TOP || c.top_k > c.E || c.D < grain || c.F < grain || c.D % grain || c.F % grain ||
-      c.ldx % 8 || c.work_bytes < plan.bytes || c.E * (2 * c.F / MF_F + c.D / MF_D + 4) > (1 << 30) ||
+  const bool shared = c.shared_gate_up != nullptr;
+  if (c.T > MF_TOKENS || c.E < 1 || c.E > MF_EXPERTS || c.top_k < 1 || c.top_k > MF_TOP || c.top_k > c.E || c.D < grain || c.F < grain || c.D % grain ||
+      c.F % grain || c.D > (1 << 24) || c.F > (1 << 24) || c.ldx % 8 || c.ldr % 4 ||
       (((uintptr_t)c.x | (uintptr_t)c.router | (uintptr_t)c.gate_up | (uintptr_t)c.down | (uintptr_t)c.shared_gate_up | (uintptr_t)c.shared_down |
-        (uintptr_t)c.work) & 15))
+        (uintptr_t)c.work | (uintptr_t)c.residual | (uintptr_t)c.out) & 15))
     return -ERR_BAD_ARG;
+  const MoeFewPlan plan(c.T, c.D, c.F, c.E, c.top_k, shared, c.i8 != 0);
+  const long items = (long)plan.experts * (plan.f_tiles + plan.d_tiles * plan.down_parts) + plan.d_tiles * ((c.T + MF_GROUP - 1) / MF_GROUP);
+  if (c.work_bytes < plan.bytes || items > (1 << 30)) return -ERR_BAD_ARG;
   cudaStream_t st = (cudaStream_t)c.stream;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;
   char* work = static_cast<char*>(c.work);
   MoeFew p;
-  p.x = c.x; p.residual = c.residual;
-  p.gate_up = (const uint8_t*)c.gate_up; p.down = (const uint8_t*)c.down;
-  p.shared_gate_up = (const uint8_t*)c.shared_gate_up; p.shared_down = (const uint8_t*)c.shared_down;
+  p.residual = c.residual;
   p.gate_up_scale = c.gate_up_scale; p.down_scale = c.down_scale;
   p.shared_gate_up_scale = c.shared_gate_up_scale; p.shared_down_scale = c.shared_down_scale;
   p.out = c.out; p.counts = c.counts; p.counters = (int*)(work + plan.counters); p.status = c.status;
   p.choice = (const int*)(work + plan.choice); p.weight = (const float*)(work + plan.weight);
-  p.act = (__nv_bfloat16*)(work + plan.act); p.part = (float*)(work + plan.part);
-  p.ldx = c.ldx; p.ldr = c.ldr;
-  p.T = (int)c.T; p.D = (int)c.D; p.F = (int)c.F; p.E = (int)c.E; p.top_k = (int)c.top_k; p.ld_act = plan.ld_act;
-  p.f_tiles = (p.F + MF_F - 1) / MF_F; p.d_tiles = (p.D + MF_D - 1) / MF_D;
-  p.inv_f = div_reciprocal(p.f_tiles); p.inv_d = div_reciprocal(p.d_tiles);
-  moe_few_router_kernel<<<(unsigned)p.T, 256, 0, st>>>(c.x, c.ldx, c.router, p.D, p.E, p.top_k, (int*)p.choice, (float*)p.weight, p.counters, plan.n_counters);
+  p.act = (__nv_bfloat16*)(work + plan.act); p.sums = (float*)(work + plan.sums);
+  p.ldr = c.ldr;
+  p.T = (int)c.T; p.D = (int)c.D; p.F = (int)c.F; p.E = (int)c.E; p.top_k = (int)c.top_k; p.shared = shared; p.ld_act = plan.ld_act; p.slots = plan.slots;
+  p.f_tiles = plan.f_tiles; p.d_tiles = plan.d_tiles; p.gate_steps = plan.gate_steps; p.down_steps = plan.down_steps; p.down_per = plan.down_per; p.down_parts = plan.down_parts; p.experts = plan.experts;
+  p.inv_k = div_reciprocal(p.top_k); p.inv_f = div_reciprocal(p.f_tiles);
+  p.inv_down = div_reciprocal(p.d_tiles * p.down_parts); p.inv_down_parts = div_reciprocal(p.down_parts); p.inv_d = div_reciprocal(p.d_tiles);
+  const int tb = p.T <= 16 ? 16 : p.T <= 32 ? 32 : 64;
+  const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, type = c.i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : bf16;
+  const uint64_t D = c.D, F = c.F, E = c.E, size = c.i8 ? 1 : 2, row = D * size;
+  const uint32_t wide = c.i8 ? 128 : 64;
+  MoeFewMaps m;
+  int rc = make_tmap(&m.x, bf16, 2, c.x, {D, (uint64_t)c.T}, {(uint64_t)c.ldx * 2}, {64, (uint32_t)tb});
+  if (rc == 0) rc = make_tmap(&m.act, bf16, 2, p.act, {F, (uint64_t)plan.slots}, {(uint64_t)plan.ld_act * 2}, {64, (uint32_t)tb});
+  if (rc == 0) rc = make_tmap(&m.gate, type, 5, c.gate_up, {D, 8, 2, F / 8, E}, {row, F * row, 8 * row, 2 * F * row}, {wide, 8, 2, MF_F / 8, 1});
+  if (rc == 0) rc = make_tmap(&m.down, type, 3, c.down, {F, D, E}, {F * size, D * F * size}, {wide, 128, 1});
+  m.shared_gate = m.gate;
+  m.shared_down = m.down;
+  if (rc == 0 && shared) rc = make_tmap(&m.shared_gate, type, 5, c.shared_gate_up, {D, 8, 2, F / 8, 1}, {row, F * row, 8 * row, 2 * F * row}, {wide, 8, 2, MF_F / 8, 1});
+  if (rc == 0 && shared) rc = make_tmap(&m.shared_down, type, 3, c.shared_down, {F, D, 1}, {F * size, D * F * size}, {wide, 128, 1});
+  if (rc) return rc;
+  const int slices = p.D >= 2048 ? 8 : p.D >= 1024 ? 4 : p.D >= 512 ? 2 : 1;
+  moe_few_router_kernel<<<(unsigned)p.T, 1024, 0, st>>>(c.x, c.ldx, c.router, p.D, p.E, p.top_k, slices, (int*)p.choice, (float*)p.weight, p.counters, plan.n_counters);
   if (const cudaError_t e = cudaGetLastError()) return -(int)e;
-  const long met = (c.T * c.top_k < c.E ? c.T * c.top_k : c.E) + (c.shared_gate_up != nullptr);     // experts at most
-  const long items = met * (p.f_tiles + p.d_tiles);
-  const int n = (int)(items < 296 ? items : 296);
-#define INV_MF(NT) (c.i8 ? launch_moe_few<NT, true>(p, n, device, st) : launch_moe_few<NT, false>(p, n, device, st))
-  return p.T <= 8 ? INV_MF(1) : p.T <= 16 ? INV_MF(2) : p.T <= 32 ? INV_MF(4) : INV_MF(8);
+  const int grid = (int)(items < 148 ? items : 148);
+#define INV_MF(TB) (c.i8 ? launch_moe_few<TB, true>(m, p, grid, device, st) : launch_moe_few<TB, false>(m, p, grid, device, st))
+  return tb == 16 ? INV_MF(16) : tb == 32 ? INV_MF(32) : INV_MF(64);
 #undef INV_MF
 }

@@ -33,7 +33,7 @@ _native.register_cuda_sigs({
     "inv_gemm_grouped": [_native.vp] * 3 + [_native.i32] * 9 + [_native.vp, _native.vp, _native.i32, _native.vp, _native.i32, _native.i32,
                                                                _native.i32, _native.i32, _native.vp, _native.vp, _native.i32, _native.i32,
                                                                _native.i64, _native.vp, _native.vp],
-    "inv_moe_few": [_native.vp], "inv_moe_few_bytes": [_native.i64] * 5 + [_native.i32],
+    "inv_moe_few": [_native.vp], "inv_moe_few_bytes": [_native.i64] * 5 + [_native.i32] * 2,
 })
 
 ALIGN = 128
@@ -310,7 +310,7 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
         router_w = router_w if router_w.is_contiguous() and router_w.data_ptr() % 16 == 0 else router_w.clone(memory_format=torch.contiguous_format)
         fn = rt.lib().inv_moe_few_bytes
         fn.restype = _native.i64
-        size = fn(T, D, inner, E, top_k, shared is not None)
+        size = fn(T, D, inner, E, top_k, shared is not None, stacks[0][1] is not None)
         work = torch.empty(size, dtype=torch.uint8, device=x.device)
         at = [(q.data_ptr(), rt.ptr(s)) for q, s in stacks] + [(0, 0)] * (4 - len(stacks))
         rt.check(rt.lib().inv_moe_few(_FEW(rows.data_ptr(), router_w.data_ptr(), rt.ptr(res), at[0][0], at[1][0], at[0][1], at[1][1], at[2][0], at[3][0], at[2][1],

@@ -1,7 +1,8 @@
 """The expert layer of a few tokens (ops.moe.moe_ffn_few) against its formula in 64 bits.
 
-Tolerances. A product of K terms is summed in chains of at most K / 128 + 16 steps (sixteen terms an instruction, eight warps, their sum), each off by at most
-2^-23 of the sum of the terms' sizes: (K / 128 + 16) 2^-23 |a| |b|. A router's logit is a chain of K / 32 + 6. silu' is at most 1.1 and exp and the quotient are off
+Tolerances. A product of K terms is summed sixteen terms an instruction, and parts of sixteen steps and more one after the other; a step of a chain is off by at most
+2^-23 of the sum of the terms' sizes: (K / 16 + K / 1024 + 16) 2^-23 |a| |b|. A router's logit is a chain of K / 256 + 21 (eight terms of every 2048, five steps
+among lanes, eight among warps). silu' is at most 1.1 and exp and the quotient are off
 by under 2^-20. The activations between the products are rounded to bf16, half a step 2^-8 of each. Those errors go through the second product by |w|, are
 weighted by the router's probabilities, which are off by twice the logits' error and 2^-20, and the result is rounded to bf16, 2^-8. On the CPU nothing is rounded
 between the products and chains are as long as K."""
@@ -63,10 +64,10 @@ def check(a, top_k, dev, chosen=None):
         rt.check_status()
     x = a["x"].reshape(-1, a["x"].shape[-1]).double()
     cpu = dev == "cpu"
-    chain = (lambda k: k + 16) if cpu else (lambda k: k / 128 + 16)
+    chain = (lambda k: k + 16) if cpu else (lambda k: k / 16 + k / 1024 + 16)
     half = 0.0 if cpu else 2.0 ** -8
     logits = x @ a["router_w"].double().t()
-    el = (x.abs() @ a["router_w"].double().abs().t()).amax(-1, keepdim=True) * ((x.shape[1] if cpu else x.shape[1] / 32) + 6) * 2.0 ** -24
+    el = (x.abs() @ a["router_w"].double().abs().t()).amax(-1, keepdim=True) * (x.shape[1] + 6 if cpu else x.shape[1] / 256 + 21) * 2.0 ** -24
     p = torch.softmax(logits, -1)
     if chosen is None:
         top, idx = p.topk(min(top_k + 1, p.shape[1]), -1)
