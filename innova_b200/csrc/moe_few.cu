@@ -25,7 +25,7 @@
 namespace inv {
 
 constexpr int MF_TOKENS = 64, MF_EXPERTS = 256, MF_TOP = 16;
-constexpr int MF_STEPS = 16;                       // of 128 bytes of K, of a down item at most
+constexpr int MF_STEPS = 12;                       // of 128 bytes of K, of a down item at most
 constexpr int MF_F = 64, MF_D = 128, MF_GROUP = 4; // columns of a gate and up item, of a down item; tokens of a sum
 
 // What the entry is given; sizes in elements.
@@ -186,14 +186,15 @@ struct MoeFew {
 };
 
 namespace mf {
-constexpr int A_STAGE = 128 * 128, QUEUE = 8, ACC = 4, CONV = 4;
+constexpr int A_STAGE = 128 * 128, QUEUE = 8;
 // Bytes of a weight row's step are 128: 64 or 128 values of K.
 template <int TB, bool I8>
 struct Shape {
-  static constexpr int STEP = I8 ? 128 : 64, B_STAGE = (I8 ? 2 : 1) * TB * 128, ROOM = (220 * 1024 - 1024) / (A_STAGE + B_STAGE),
-                       SETS = I8 ? 2 : 3;   // of four warps of sums; conversions take the threads of the third
-  static constexpr int STAGES = ROOM < 12 ? ROOM : 12, SUMS = 3, CONVERT = SUMS + 4 * SETS,
-                       THREADS = 32 * (CONVERT + (I8 ? 4 * CONV : 0));    // warps of loads, of products, of items, of sums, of conversions
+  static constexpr int STEP = I8 ? 128 : 64, B_STAGE = (I8 ? 2 : 1) * TB * 128;
+  static constexpr int PER_SM = I8 ? 1 : 2, ROOM = ((I8 ? 216 : 102) * 1024 - 1024) / (A_STAGE + B_STAGE), STAGES = ROOM < 12 ? ROOM : 12;
+  static constexpr int ACC = 4, CONV = 4, SETS = I8 ? 2 : 1;   // buffers of sums and of converted weights; sets of four warps of sums
+  // warps of loads, of products, of items, of sums, of conversions
+  static constexpr int SUMS = 3, CONVERT = SUMS + 4 * SETS, THREADS = 32 * (CONVERT + (I8 ? 4 * CONV : 0));
   static constexpr int SMEM = STAGES * (A_STAGE + B_STAGE) + 1024;
   static constexpr int COLS = ACC * TB + (I8 ? CONV * 64 : 0), TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
 };
@@ -260,18 +261,19 @@ __device__ __forceinline__ bool mf_wait(const int* p, int n, volatile int* abort
 }
 
 template <int TB, bool I8>
-__global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
+__global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>::PER_SM)
     moe_few_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_act, const __grid_constant__ CUtensorMap map_gate,
                    const __grid_constant__ CUtensorMap map_down, const __grid_constant__ CUtensorMap map_shared_gate,
                    const __grid_constant__ CUtensorMap map_shared_down, const __grid_constant__ MoeFew p) {
   using namespace mf;
   using S = Shape<TB, I8>;
-  constexpr int STAGES = S::STAGES, B_STAGE = S::B_STAGE, STEP = S::STEP;
+  constexpr int STAGES = S::STAGES, B_STAGE = S::B_STAGE, STEP = S::STEP, ACC = S::ACC, CONV = S::CONV;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full_bar[STAGES], empty_bar[STAGES], item_full[QUEUE], item_empty[QUEUE], acc_full[ACC], acc_empty[ACC], conv_full[CONV], conv_empty[CONV];
+  __shared__ uint64_t full_bar[STAGES], weights_bar[STAGES], empty_bar[STAGES], item_full[QUEUE], item_empty[QUEUE], acc_full[ACC], acc_empty[ACC], conv_full[CONV], conv_empty[CONV];
   __shared__ uint32_t s_mask[MF_EXPERTS + 1][2];                 // tokens of an expert; E: of the shared one
   __shared__ uint16_t s_index[MF_EXPERTS], s_expert[MF_EXPERTS + 1], s_first[MF_EXPERTS + 2], s_slot[MF_TOKENS * MF_TOP];
   __shared__ Item s_item[QUEUE];
+  __shared__ float s_weight[MF_TOKENS * MF_TOP];
   __shared__ int s_n;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_abort;
@@ -285,6 +287,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full_bar[i], 1);
+      mbar_init(&weights_bar[i], 1);
       mbar_init(&empty_bar[i], 1);
     }
     for (int i = 0; i < QUEUE; ++i) {
@@ -319,8 +322,10 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
 
   // Who goes where: the tokens of each expert, the experts that are met, and a slot for each choice, in the order of experts and of tokens within one.
   for (int i = tid; i < chosen; i += S::THREADS) {
-    const int t = div_by(i, p.top_k, p.inv_k);
-    atomicOr(&s_mask[p.choice[i]][t >> 5], 1u << (t & 31));
+    const int t = div_by(i, p.top_k, p.inv_k), e = p.choice[i];
+    s_slot[i] = (uint16_t)e;
+    s_weight[i] = p.weight[i];
+    atomicOr(&s_mask[e][t >> 5], 1u << (t & 31));
   }
   if (p.shared && tid == 0) {
     s_mask[p.E][0] = p.T >= 32 ? 0xffffffffu : (1u << p.T) - 1;
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
   }
   __syncthreads();
   for (int i = tid; i < chosen; i += S::THREADS) {
-    const int t = div_by(i, p.top_k, p.inv_k), e = p.choice[i];
+    const int t = div_by(i, p.top_k, p.inv_k), e = s_slot[i];
     const int below = t < 32 ? __popc(s_mask[e][0] & ((1u << t) - 1)) : __popc(s_mask[e][0]) + __popc(s_mask[e][1] & ((1u << (t - 32)) - 1));
     s_slot[i] = (uint16_t)(s_first[s_index[e]] + below);
   }
@@ -427,12 +432,14 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
         const bool shared = e == p.E;
         const CUtensorMap* map = it.kind == GATE ? (shared ? &map_shared_gate : &map_gate) : (shared ? &map_shared_down : &map_down);
         auto weights = [&](int i, int at) {
-          mbar_expect_tx(&full_bar[at], A_STAGE + B_STAGE);
+          uint64_t* bar = I8 ? &weights_bar[at] : &full_bar[at];               // conversions do not wait for the tokens
+          mbar_expect_tx(bar, I8 ? A_STAGE : A_STAGE + B_STAGE);
           const int k = (k0 + i) * STEP, plane = shared ? 0 : e;
-          if (it.kind == GATE) tma_load_5d(sA + at * A_STAGE, map, &full_bar[at], k, 0, 0, it.tile * (MF_F / 8), plane);
-          else tma_load_3d(sA + at * A_STAGE, map, &full_bar[at], k, it.tile * MF_D, plane);
+          if (it.kind == GATE) tma_load_5d(sA + at * A_STAGE, map, bar, k, 0, 0, it.tile * (MF_F / 8), plane);
+          else tma_load_3d(sA + at * A_STAGE, map, bar, k, it.tile * MF_D, plane);
         };
         auto tokens = [&](int i, int at) {
+          if (I8) mbar_expect_tx(&full_bar[at], B_STAGE);
 #pragma unroll
           for (int h = 0; h < (I8 ? 2 : 1); ++h) {
             if (it.kind == GATE) tma_load_2d(sB + at * B_STAGE + h * TB * 128, &map_x, &full_bar[at], (k0 + i) * STEP + 64 * h, 0);
@@ -508,7 +515,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
       }
     }
   } else if (warp < S::CONVERT) {
-    // ---------------- sums: sets of four warps take items in turn, since an item's fences and counters take longer than its products ----------------
+    // ---------------- sums: sets of four warps take items in turn ----------------
     const int q = warp & 3, row = q * 32 + lane;           // the lanes of tensor memory that this warp may read
     const int set = (warp - S::SUMS) >> 2;
     int qi = 0, turn = 0, next_acc = 0;
@@ -527,11 +534,13 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
       if (it.kind != SUM && ++next_acc == ACC) { next_acc = 0; next_accph ^= 1; }
       if (!mine) continue;
       if (it.kind == SUM) {
+        // eight lanes of a warp have 32 columns between them and add every fourth part; the four groups of lanes add up theirs
+        const int col = it.tile * MF_D + q * 32 + (lane & 7) * 4, t0 = it.part * MF_GROUP, mine_t = t0 + (lane >> 3);
+        uint2 residual = make_uint2(0, 0);
+        if (p.residual != nullptr && mine_t < p.T && col < p.D) residual = *reinterpret_cast<const uint2*>(p.residual + mine_t * p.ldr + col);
         bool there = true;
         if (lane == 0) there = mf_wait(&down_done[it.tile], n_active * p.down_parts * 4, abort_flag, p.status);
         if (!__shfl_sync(0xffffffffu, there, 0)) break;
-        // eight lanes of a warp have 32 columns between them and add every fourth part; the four groups of lanes add up theirs
-        const int col = it.tile * MF_D + q * 32 + (lane & 7) * 4, t0 = it.part * MF_GROUP;
         float y[MF_GROUP][4] = {};
         if (col < p.D) {
           for (int k = p.shared ? -1 : 0; k < p.top_k; ++k) {
@@ -540,7 +549,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
 #pragma unroll
             for (int j = 0; j < MF_GROUP; ++j) {
               const int t = min(t0 + j, p.T - 1), c = t * p.top_k + max(k, 0);
-              w[j] = k < 0 ? 1.f : p.weight[c];
+              w[j] = k < 0 ? 1.f : s_weight[c];
               from[j] = p.sums + (long)(k < 0 ? chosen + t : s_slot[c]) * p.D + col;
             }
 #pragma unroll 2
@@ -559,14 +568,10 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
             y[j][x] += __shfl_xor_sync(0xffffffffu, y[j][x], 8);
             y[j][x] += __shfl_xor_sync(0xffffffffu, y[j][x], 16);
           }
-          const int t = t0 + j;
-          if (lane >> 3 == j && t < p.T && col < p.D) {
-            if (p.residual != nullptr) {
-              const uint2 r = *reinterpret_cast<const uint2*>(p.residual + t * p.ldr + col);
-              y[j][0] += __uint_as_float(r.x << 16); y[j][1] += __uint_as_float(r.x & 0xffff0000u);
-              y[j][2] += __uint_as_float(r.y << 16); y[j][3] += __uint_as_float(r.y & 0xffff0000u);
-            }
-            *reinterpret_cast<uint2*>(p.out + (long)t * p.D + col) = make_uint2(pack_bf16x2(y[j][0], y[j][1]), pack_bf16x2(y[j][2], y[j][3]));
+          if (lane >> 3 == j && mine_t < p.T && col < p.D) {
+            y[j][0] += __uint_as_float(residual.x << 16); y[j][1] += __uint_as_float(residual.x & 0xffff0000u);
+            y[j][2] += __uint_as_float(residual.y << 16); y[j][3] += __uint_as_float(residual.y & 0xffff0000u);
+            *reinterpret_cast<uint2*>(p.out + (long)mine_t * p.D + col) = make_uint2(pack_bf16x2(y[j][0], y[j][1]), pack_bf16x2(y[j][2], y[j][3]));
           }
         }
         continue;
@@ -630,7 +635,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, 1)
       if (kind == SUM) continue;
       for (int j = 0; j < steps; ++j) {
         if (cv == group) {
-          if (!mbar_wait_warp(&full_bar[s], ph, abort_flag, p.status, ERR_WAIT_FULL) ||
+          if (!mbar_wait_warp(&weights_bar[s], ph, abort_flag, p.status, ERR_WAIT_FULL) ||
               !mbar_wait_warp(&conv_empty[cv], cvph, abort_flag, p.status, ERR_WAIT_EMPTY)) { ok = false; break; }
           tc_fence_after();
           const uint8_t* from = sA + s * A_STAGE + row * 128;
@@ -677,8 +682,9 @@ struct MoeFewMaps {
 };
 
 template <int TB, bool I8>
-static int launch_moe_few(const MoeFewMaps& m, const MoeFew& p, int grid, int device, cudaStream_t st) {
+static int launch_moe_few(const MoeFewMaps& m, const MoeFew& p, long items, int device, cudaStream_t st) {
   using S = mf::Shape<TB, I8>;
+  const int grid = (int)(items < 148 * S::PER_SM ? items : 148 * S::PER_SM);
   static OncePerDevice once;
   if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(moe_few_kernel<TB, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); })) return -e;
   launch_early(moe_few_kernel<TB, I8>, dim3(grid), S::THREADS, S::SMEM, st, m.x, m.act, m.gate, m.down, m.shared_gate, m.shared_down, p);
@@ -739,8 +745,7 @@ extern "C" int inv_moe_few(const void* call) {
   const int slices = p.D >= 2048 ? 8 : p.D >= 1024 ? 4 : p.D >= 512 ? 2 : 1;
   moe_few_router_kernel<<<(unsigned)p.T, 1024, 0, st>>>(c.x, c.ldx, c.router, p.D, p.E, p.top_k, slices, (int*)p.choice, (float*)p.weight, p.counters, plan.n_counters);
   if (const cudaError_t e = cudaGetLastError()) return -(int)e;
-  const int grid = (int)(items < 148 ? items : 148);
-#define INV_MF(TB) (c.i8 ? launch_moe_few<TB, true>(m, p, grid, device, st) : launch_moe_few<TB, false>(m, p, grid, device, st))
+#define INV_MF(TB) (c.i8 ? launch_moe_few<TB, true>(m, p, items, device, st) : launch_moe_few<TB, false>(m, p, items, device, st))
   return tb == 16 ? INV_MF(16) : tb == 32 ? INV_MF(32) : INV_MF(64);
 #undef INV_MF
 }

@@ -13,6 +13,7 @@ shift the reported loss value (src/moe_trainer.cpp:88-169), both carry gradients
 """
 from __future__ import annotations
 
+import functools
 import struct
 from typing import Optional, Tuple, Union
 
@@ -232,62 +233,86 @@ _FEW = struct.Struct("=16Q 9q").pack
 Weight = Union[torch.Tensor, Int8Weight]
 
 
-def moe_few_supported(x, router_w, w_gu, w_down, top_k=2) -> bool:
-    """Whether ``moe_ffn_few`` takes these tokens on their device: of at most 64, and on a GPU bf16 with sizes of its kernel."""
-    T, D = x.numel() // max(1, x.shape[-1]), x.shape[-1]
-    i8 = isinstance(w_gu, Int8Weight)
-    grain, E, inner = 16 if i8 else 8, router_w.shape[0], (w_down.q if i8 else w_down).shape[-1]
-    return T <= FEW_TOKENS and top_k <= min(E, FEW_TOP) and E <= FEW_EXPERTS and (not x.is_cuda or (x.dtype == torch.bfloat16 and D % grain == 0 and inner % grain == 0))
+def moe_few_supported(x, router_w, w_gate_up: Weight, w_down: Weight, top_k: int = 2) -> bool:
+    """Whether ``moe_ffn_few`` takes these tokens where they are: at most 64 of them, and on a GPU bf16 and sizes that its kernel has."""
+    D, E, i8 = x.shape[-1], router_w.shape[0], isinstance(w_down, Int8Weight)
+    inner, grain = (w_down.q if i8 else w_down).shape[-1], 16 if i8 else 8
+    return (x.numel() <= FEW_TOKENS * D and top_k <= min(E, FEW_TOP) and E <= FEW_EXPERTS
+            and (not x.is_cuda or x.dtype == torch.bfloat16 and D % grain == 0 and inner % grain == 0))
 
 
-def _plain(w: Weight) -> torch.Tensor:
-    return w.q if isinstance(w, Int8Weight) else w
+def _few_plain_weight(w, shape, dev, dtype) -> bool:
+    return isinstance(w, torch.Tensor) and w.shape == shape and w.dtype is dtype and w.get_device() == dev and w.is_contiguous() and w.data_ptr() % 16 == 0
 
 
-def _few_stack(w: Weight, dims: int, x, what: str):
-    """-> its values and scales, checked."""
-    if isinstance(w, Int8Weight):
-        check_weight(w, dims)
-        q, s = w
-        if x.is_cuda and not q.is_contiguous():
-            raise ValueError(f"{what} of {tuple(q.shape)} in 8 bits: rows one behind the other on a GPU")
-    else:
-        q, s = w, None
-        if q.dim() != dims or q.dtype != x.dtype or (x.is_cuda and (not q.is_contiguous() or q.data_ptr() % 16)):
-            raise ValueError(f"{what} of {q.dtype} {tuple(q.shape)}: contiguous {x.dtype} on 16-byte boundaries with {dims} dimensions, or an Int8Weight")
-    if q.device != x.device:
-        raise ValueError(f"{what} on {q.device}, x on {x.device}")
-    return q, s
+def _few_int8_weight(w, shape, dev) -> bool:
+    q, s = w
+    return (q.shape == shape and q.dtype is torch.int8 and s.shape == shape[:-1] and s.dtype is torch.float32 and q.get_device() == dev == s.get_device()
+            and q.is_contiguous() and s.is_contiguous() and q.data_ptr() % 16 == 0)
 
 
 def _few_check(x, router_w, w_gu, w_down, residual, top_k, shared):
-    """-> T, D, F, E and (values, scales) of the stacks and of the shared expert."""
+    """-> T, D, F, E, whether weights are in 8 bits. Asked in few expressions; what is wrong with arguments that fail is found by ``_few_refuse``."""
+    D, dev, dtype, i8 = x.shape[-1] if x.dim() else 0, x.get_device(), x.dtype, isinstance(w_down, Int8Weight)
+    T, down = x.numel() // max(1, D), w_down.q if i8 else w_down
+    if down.dim() == 3 and router_w.dim() == 2 and D > 0:
+        E, _, inner = down.shape
+        pairs = [(w_gu, (E, 2 * inner, D)), (w_down, (E, D, inner))]
+        if shared is not None and len(shared) == 2:
+            pairs += [(shared[0], (2 * inner, D)), (shared[1], (D, inner))]
+        grain = 16 if i8 else 8
+        if ((shared is None or len(shared) == 2) and router_w.shape == (E, D) and router_w.dtype is dtype and router_w.get_device() == dev
+                and 1 <= top_k <= min(E, FEW_TOP) and E <= FEW_EXPERTS and T <= FEW_TOKENS
+                and (residual is None or residual.shape == x.shape and residual.dtype is dtype and residual.get_device() == dev)
+                and (dtype is torch.bfloat16 or dtype is torch.float32 and dev < 0) and (dev < 0 or D % grain == 0 and inner % grain == 0 and inner > 0)
+                and all((isinstance(w, Int8Weight) and _few_int8_weight(w, s, dev)) if i8 else _few_plain_weight(w, s, dev, dtype)
+                        for w, s in pairs)):
+            return T, D, inner, E, i8
+    _few_refuse(x, router_w, w_gu, w_down, residual, top_k, shared)
+
+
+def _few_refuse(x, router_w, w_gu, w_down, residual, top_k, shared):
     if x.dim() < 1 or x.dtype not in (torch.bfloat16, torch.float32) or (x.is_cuda and x.dtype != torch.bfloat16):
         raise TypeError(f"x of {x.dtype} {tuple(x.shape)}: bf16 (fp32 too on the CPU)")
     D = x.shape[-1]
     T = x.numel() // max(1, D)
-    i8 = [isinstance(w, Int8Weight) for w in (w_gu, w_down, *(shared or ()))]
-    if any(i8) != all(i8) or (shared is not None and len(shared) != 2):
-        raise ValueError("experts and a shared one (gate_up, down): all in 8 bits or none")
+    if shared is not None and len(shared) != 2:
+        raise ValueError("a shared expert is a pair: gate_up, down")
+    named = [("w_gate_up", w_gu, 3), ("w_down", w_down, 3)] + ([] if shared is None else [("shared gate_up", shared[0], 2), ("shared down", shared[1], 2)])
+    i8 = [isinstance(w, Int8Weight) for _, w, _ in named]
+    if any(i8) != all(i8):
+        raise ValueError("weights of experts and of a shared one: all in 8 bits or none")
     if router_w.dim() != 2 or router_w.shape[1] != D or router_w.dtype != x.dtype or router_w.device != x.device:
         raise ValueError(f"router of {router_w.dtype} {tuple(router_w.shape)} on {router_w.device}: {x.dtype} [experts, {D}] on {x.device}")
-    E, inner = router_w.shape[0], _plain(w_down).shape[-1]
-    stacks = [_few_stack(w_gu, 3, x, "w_gate_up"), _few_stack(w_down, 3, x, "w_down")]
-    if shared is not None:
-        stacks += [_few_stack(shared[0], 2, x, "shared gate_up"), _few_stack(shared[1], 2, x, "shared down")]
-    for (q, _), shape in zip(stacks, ((E, 2 * inner, D), (E, D, inner), (2 * inner, D), (D, inner))):
-        if q.shape != shape:
-            raise ValueError(f"a weight of {tuple(q.shape)} where {shape} is needed for {E} experts of {inner} on {D}")
+    for what, w, dims in named:
+        q = w
+        if i8[0]:
+            check_weight(w, dims)
+            q = w.q
+        elif q.dim() != dims or q.dtype != x.dtype:
+            raise ValueError(f"{what} of {q.dtype} {tuple(q.shape)}: {x.dtype} with {dims} dimensions, or an Int8Weight")
+        if q.device != x.device:
+            raise ValueError(f"{what} on {q.device}, x on {x.device}")
+        if not q.is_contiguous() or q.data_ptr() % 16:
+            raise ValueError(f"{what} with strides {q.stride()}: contiguous, on 16-byte boundaries")
+    E, inner, grain = router_w.shape[0], (w_down.q if i8[0] else w_down).shape[-1], 16 if i8[0] else 8
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"residual of {residual.dtype} {tuple(residual.shape)} on {residual.device} for x of {x.dtype} {tuple(x.shape)}")
     if not 1 <= top_k <= E:
         raise ValueError(f"top_k {top_k} of {E} experts")
     if T > FEW_TOKENS or top_k > FEW_TOP or E > FEW_EXPERTS:
         raise ValueError(f"{T} tokens, {E} experts, top_k {top_k}: at most {FEW_TOKENS}, {FEW_EXPERTS} and {FEW_TOP} (moe_ffn takes more tokens)")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
-        raise ValueError(f"residual of {residual.dtype} {tuple(residual.shape)} on {residual.device} for x of {x.dtype} {tuple(x.shape)}")
-    grain = 16 if i8[0] else 8
-    if x.is_cuda and (D % grain or inner % grain or not D or not inner):
+    if x.is_cuda and (D % grain or inner % grain):
         raise ValueError(f"width {D} and expert width {inner}: multiples of {grain} on a GPU")
-    return T, D, inner, E, stacks
+    raise ValueError("weights of " + ", ".join(f"{tuple((w.q if i8[0] else w).shape)}" for _, w, _ in named) + f" for {E} experts of {inner} on {D}: "
+                     f"{(E, 2 * inner, D)}, {(E, D, inner)}" + (f", {(2 * inner, D)}, {(D, inner)}" if shared is not None else "") + " is needed, no width 0")
+
+
+@functools.lru_cache(maxsize=1024)
+def _few_bytes(*sizes):
+    fn = rt.lib().inv_moe_few_bytes
+    fn.restype = _native.i64
+    return fn(*sizes)
 
 
 def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Optional[torch.Tensor] = None, top_k: int = 2,
@@ -296,10 +321,11 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
     w_gate_up [E, 2F, D] (gate | up) and w_down [E, D, F] in bf16, or both as ``ops.int8.Int8Weight``; ``shared`` (gate_up [2F, D], down [D, F]): an expert that
     every token goes to with weight one. The routing weights are the raw probabilities; ties go to the lowest expert. Sums are kept in fp32, the activations
     between the products rounded to bf16, the result once. A token's result depends on no other. No gradient and no tangent passes through it."""
-    T, D, inner, E, stacks = _few_check(x, router_w, w_gate_up, w_down, residual, top_k, shared)
-    refuse_gradients("moe_ffn_few", x, router_w, residual, *(q for q, _ in stacks))
+    T, D, inner, E, i8 = _few_check(x, router_w, w_gate_up, w_down, residual, top_k, shared)
+    weights = (w_gate_up, w_down, *(shared or ()))
+    refuse_gradients("moe_ffn_few", x, router_w, residual, *(() if i8 else weights))
     if not x.is_cuda:
-        return _few_plain(x.reshape(T, D), router_w, stacks, residual, top_k, x.shape)
+        return _few_plain(x.reshape(T, D), router_w, weights, residual, top_k, x.shape)
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     counts = torch.empty(E, dtype=torch.int32, device=x.device)
     if T == 0:
@@ -307,25 +333,32 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
     with rt.device_of(x):
         rows, ldx = _dense_rows(x, D)
         res, ldr = (None, 0) if residual is None else _dense_rows(residual, D)
-        router_w = router_w if router_w.is_contiguous() and router_w.data_ptr() % 16 == 0 else router_w.clone(memory_format=torch.contiguous_format)
-        fn = rt.lib().inv_moe_few_bytes
-        fn.restype = _native.i64
-        size = fn(T, D, inner, E, top_k, shared is not None, stacks[0][1] is not None)
+        if not router_w.is_contiguous() or router_w.data_ptr() % 16:
+            router_w = router_w.clone(memory_format=torch.contiguous_format)
+        size = _few_bytes(T, D, inner, E, top_k, shared is not None, i8)
         work = torch.empty(size, dtype=torch.uint8, device=x.device)
-        at = [(q.data_ptr(), rt.ptr(s)) for q, s in stacks] + [(0, 0)] * (4 - len(stacks))
-        rt.check(rt.lib().inv_moe_few(_FEW(rows.data_ptr(), router_w.data_ptr(), rt.ptr(res), at[0][0], at[1][0], at[0][1], at[1][1], at[2][0], at[3][0], at[2][1],
-                                           at[3][1], out.data_ptr(), counts.data_ptr(), work.data_ptr(), rt.status_ptr(x), rt.stream_ptr(),
-                                           T, D, inner, E, top_k, ldx, ldr, stacks[0][1] is not None, size)), "inv_moe_few")
+        at = [w.q.data_ptr() if i8 else w.data_ptr() for w in weights]
+        scales = [w.scale.data_ptr() if i8 else 0 for w in weights]
+        if shared is None:
+            at += [0, 0]
+            scales += [0, 0]
+        rt.check(rt.lib().inv_moe_few(_FEW(rows.data_ptr(), router_w.data_ptr(), rt.ptr(res), *at[:2], *scales[:2], *at[2:], *scales[2:],
+                                           out.data_ptr(), counts.data_ptr(), work.data_ptr(), rt.status_ptr(x), rt.stream_ptr(),
+                                           T, D, inner, E, top_k, ldx, ldr, i8, size)), "inv_moe_few")
         rt.count_launches(1)
     return out, counts
 
 
-def _few_plain(x, router_w, stacks, residual, top_k, shape):
-    T, E = x.shape[0], router_w.shape[0]
+def _few_plain(x, router_w, weights, residual, top_k, shape):
+    E = router_w.shape[0]
+
+    def matrix(w, e):
+        if isinstance(w, Int8Weight):
+            return (w if e is None else Int8Weight(w.q[e], w.scale[e])).dequantize()
+        return (w if e is None else w[e]).float()
 
     def expert(h, pair, e=None):
-        gate_up, down = ((q if e is None else q[e], s if s is None or e is None else s[e]) for q, s in pair)
-        gate_up, down = (q.float() if s is None else q.float() * s.unsqueeze(-1) for q, s in (gate_up, down))
+        gate_up, down = (matrix(w, e) for w in pair)
         g, u = (h @ gate_up.t()).chunk(2, -1)
         return (F.silu(g) * u) @ down.t()
 
@@ -333,9 +366,9 @@ def _few_plain(x, router_w, stacks, residual, top_k, shape):
     probs = torch.softmax(h @ router_w.float().t(), -1)
     order = torch.sort(probs, dim=-1, descending=True, stable=True).indices[:, :top_k]
     y = torch.zeros_like(h) if residual is None else residual.reshape(h.shape).float()
-    if len(stacks) == 4:
-        y = y + expert(h, stacks[2:])
+    if len(weights) == 4:
+        y = y + expert(h, weights[2:])
     for e in order.unique().tolist():
         rows = (order == e).any(-1).nonzero().flatten()
-        y = y.index_add(0, rows, expert(h[rows], stacks[:2], e) * probs[rows, e].unsqueeze(-1))
+        y = y.index_add(0, rows, expert(h[rows], weights[:2], e) * probs[rows, e].unsqueeze(-1))
     return y.to(x.dtype).view(shape), torch.bincount(order.reshape(-1), minlength=E).int()
