@@ -277,7 +277,7 @@ def _few_refuse(x, router_w, w_gu, w_down, residual, top_k, shared):
     D = x.shape[-1]
     T = x.numel() // max(1, D)
     if shared is not None and len(shared) != 2:
-        raise ValueError("a shared expert is a pair: gate_up, down")
+        raise ValueError("a shared expert has 2 weights: gate_up, down")
     named = [("w_gate_up", w_gu, 3), ("w_down", w_down, 3)] + ([] if shared is None else [("shared gate_up", shared[0], 2), ("shared down", shared[1], 2)])
     i8 = [isinstance(w, Int8Weight) for _, w, _ in named]
     if any(i8) != all(i8):
