@@ -6,12 +6,12 @@
 // The sums are whole numbers below 2^31 (K <= 133144), so their order changes nothing; scales and bias are applied in fp32 and the result is rounded once.
 //
 // int8_rows_kernel      rows of activations into codes and scales
-// int8_few_kernel       up to 64 rows: weight bytes bound it; weights go from memory straight into the fragments of warp-level products
-// int8_tile_kernel      more rows: tiles of 256 x 256 on CTA pairs, tcgen05 kind::i8
+// int8_few_kernel       up to eight rows of weights of up to 32 MB: codes and product in one launch, warp-level products
+// int8_split_kernel     up to 128 rows, or results of few tiles: tcgen05 kind::i8, clusters that share K
+// int8_tile_kernel      the rest: tiles of 256 x 256 on CTA pairs, tcgen05 kind::i8
 #include "cta_pair.cuh"
 #include "gemm_common.cuh"
 #include "once_per_device.h"
-#include <cstdlib>
 
 namespace inv {
 
@@ -39,6 +39,20 @@ __device__ __forceinline__ int int8_code(float x, float s, float inv) {
   const float d = fmaf(-s, n + 0.5f, x);
   const int i = (int)n;
   return d > 0.f || (d == 0.f && (i & 1)) ? i + 1 : i;
+}
+
+// The scale of a row from the bits of its largest |x|: not a number is above infinity is above the rest. False where it is not finite.
+__device__ __forceinline__ bool int8_scale(uint32_t top, float& s, float& inv) {
+  const bool finite = top < 0x7f800000u;
+  s = finite ? __fdiv_rn(fmaxf(__uint_as_float(top), INT8_LEAST), 127.f) : __uint_as_float(0x7fc00000u);
+  inv = finite ? __frcp_rn(s) : 0.f;
+  return finite;
+}
+__device__ __forceinline__ uint2 int8_pack(const float* v, float s, float inv) {
+  uint32_t u[2] = {0u, 0u};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) u[j / 4] |= ((uint32_t)int8_code(v[j], s, inv) & 255u) << (8 * (j % 4));
+  return make_uint2(u[0], u[1]);
 }
 
 // Eight values from `row`, of which n exist; VEC: all of them, on a 16-byte boundary.
@@ -86,7 +100,7 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const T* __restrict__ x,
     const int i = tid + h * threads;
     if (i < eights) int8_eight<VEC>(row + i * 8, K - i * 8, v[h]);
   }
-  uint32_t top = 0;                                       // bits of the largest |x|: not a number is above infinity is above the rest
+  uint32_t top = 0;
 #pragma unroll
   for (int h = 0; h < HOLD; ++h)
     if (tid + h * threads < eights) {
@@ -105,17 +119,11 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const T* __restrict__ x,
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, (tid & 31) < threads / 32 ? sh[tid & 31] : 0u);
   }
-  const bool finite = top < 0x7f800000u;
-  const float s = finite ? __fdiv_rn(fmaxf(__uint_as_float(top), INT8_LEAST), 127.f) : __uint_as_float(0x7fc00000u);
-  const float inv = finite ? __frcp_rn(s) : 0.f;
+  float s, inv;
+  const bool finite = int8_scale(top, s, inv);
   if (tid == 0) sx[r] = s;
   auto store = [&](int i, const float* w) {
-    uint32_t u[2] = {0u, 0u};
-    if (finite) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) u[j / 4] |= ((uint32_t)int8_code(w[j], s, inv) & 255u) << (8 * (j % 4));
-    }
-    *reinterpret_cast<uint2*>(to + i * 8) = make_uint2(u[0], u[1]);
+    *reinterpret_cast<uint2*>(to + i * 8) = finite ? int8_pack(w, s, inv) : make_uint2(0u, 0u);
   };
 #pragma unroll
   for (int h = 0; h < HOLD; ++h)
@@ -127,9 +135,12 @@ __global__ void __launch_bounds__(512) int8_rows_kernel(const T* __restrict__ x,
   }
 }
 
+static bool int8_rows_vec(const Int8Call& c) {
+  return c.K % 8 == 0 && ((uintptr_t)c.x | (uintptr_t)(c.T > 1 ? c.ldx * (c.x_f32 ? 4 : 2) : 0)) % 16 == 0;
+}
+
 static int launch_int8_rows(const Int8Call& c, cudaStream_t st) {
-  const int size = c.x_f32 ? 4 : 2;
-  const bool vec = c.K % 8 == 0 && ((uintptr_t)c.x | (uintptr_t)(c.T > 1 ? c.ldx * size : 0)) % 16 == 0;
+  const bool vec = int8_rows_vec(c);
   const bool warps = c.K <= 1024 && c.T > 296;
   const int threads = warps ? 256 : c.K <= 512 ? 64 : c.K <= 1024 ? 128 : c.K <= 4096 ? 256 : 512;
   const unsigned grid = (unsigned)(warps ? (c.T + 7) / 8 : c.T);
@@ -155,13 +166,14 @@ __device__ __forceinline__ float int8_silu(float x) { return __fdividef(x, 1.f +
 
 // ---------------------------------------------------------------------------------------------- up to eight rows
 struct Int8Few {
+  const void* x;                   // bf16 or fp32, or null: codes and scales are given
   const int8_t *codes, *q;
   const float *sx, *sw;
   const void* bias;
   void* out;
-  long ldc, ldw, ldo;
-  int T, N, K, cols, tiles;        // cols: output columns
-  int bias_f32, out_f32;
+  long ldx, ldc, ldw, ldo;
+  int T, N, K, cols, tiles, pitch; // cols: output columns; pitch: between rows of codes in shared memory
+  int x_f32, x_vec, bias_f32, out_f32;
 };
 
 __device__ __forceinline__ void int8_mma(int* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -174,29 +186,37 @@ __device__ __forceinline__ uint4 int8_stream(const int8_t* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-// Sixteen codes of which only the first n exist.
-__device__ __forceinline__ uint4 int8_mask(uint4 v, int n) {
-  uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int b = n - 4 * j;
-    u[j] = b >= 4 ? u[j] : b <= 0 ? 0u : u[j] & (0xffffffffu >> (8 * (4 - b)));
-  }
-  return make_uint4(u[0], u[1], u[2], u[3]);
-}
 __device__ __forceinline__ float int8_bias(const void* b, int f32, int i) {
   return b == nullptr ? 0.f : f32 ? static_cast<const float*>(b)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
 }
+__device__ __forceinline__ void int8_eight_of(const Int8Few& p, int t, int i, float* v) {
+  const long at = t * p.ldx + i * 8;
+  const int n = p.K - i * 8;
+  if (p.x_f32) {
+    const float* row = static_cast<const float*>(p.x) + at;
+    if (p.x_vec) int8_eight<true>(row, n, v);
+    else int8_eight<false>(row, n, v);
+  } else {
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.x) + at;
+    if (p.x_vec) int8_eight<true>(row, n, v);
+    else int8_eight<false>(row, n, v);
+  }
+}
 
-// Weights go from memory straight into fragments, with none of a tile's set-up. A CTA takes 32 weight rows at a time (gated: 16 of the gate and their 16 of the up
-// product) as the 16-row operand, the activations as the other. Its eight warps take every eighth slice of K, 128 bytes of a row, and meet in shared memory. Both
-// operands read a lane's 32 consecutive bytes in the same order, which a sum over k does not notice. The warp-level product of 8-bit integers is slow on this GPU,
-// some 80 cycles an instruction and scheduler: sixteen rows took 27 us of 22016 x 4096, 64 rows 110, where the tiles below take 20 and 22.
-constexpr int FEW_WARPS = 8, FEW_SLICE = 128, FEW_PL = 36, FEW_ROWS = 8, FEW_RING = 2;
+// One launch: a CTA makes the codes of all rows for itself, in shared memory, while its first weights are on their way (every CTA reads x from L2, and with a kernel of
+// their own in front the codes cost 1.5 us on the device and 4 on the host). Weights go from memory straight into fragments, with none of a tile's set-up. A CTA
+// takes 32 weight rows at a time (gated: 16 of the gate and their 16 of the up product) as the 16-row operand, the activations as the other. Its eight warps
+// take every eighth slice of K, 128 bytes of a row, and meet in shared memory. Both operands read a lane's 32 consecutive bytes in the same order, which a sum over k does
+// not notice. The warp-level product of 8-bit integers is slow on this GPU, some 80 cycles an instruction and scheduler: sixteen rows took 27 us of 22016 x
+// 4096, 64 rows 110, where the tiles below take 20 and 22.
+constexpr int FEW_WARPS = 8, FEW_SLICE = 128, FEW_PL = 36, FEW_ROWS = 8, FEW_RING = 2, FEW_CODES = 88 * 1024;
 
 template <bool GATED>
 __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8Few p) {
+  extern __shared__ __align__(16) int8_t few_codes[];        // [T] rows of whole slices, pitch apart: 16 bytes off 128, so that eight lanes meet all banks
   __shared__ int part[FEW_WARPS * FEW_ROWS * FEW_PL];
+  __shared__ uint32_t tops[FEW_WARPS][FEW_ROWS];
+  __shared__ float scales[FEW_ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
   const int slices = (p.K + FEW_SLICE - 1) / FEW_SLICE;
   release_next();
@@ -215,8 +235,44 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
 #pragma unroll
   for (int u = 0; u < FEW_RING; ++u)
     if (warp + u * FEW_WARPS < slices) fetch(tile, warp + u * FEW_WARPS, ring[u]);
-  wait_previous();                                         // codes and scales of the activations
-  const int8_t* x = p.codes + (long)min(g, p.T - 1) * p.ldc + tig * 32;
+  const int eights = (p.K + 7) / 8, places = slices * (FEW_SLICE / 8);
+  if (p.x != nullptr) {
+    for (int t = 0; t < p.T; ++t) {
+      uint32_t top = 0;
+      for (int i = tid; i < eights; i += FEW_WARPS * 32) {
+        float v[8];
+        int8_eight_of(p, t, i, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) tops[warp][t] = top;
+    }
+    __syncthreads();
+    for (int t = 0; t < p.T; ++t) {
+      float s, inv;
+      const bool finite = int8_scale(__reduce_max_sync(0xffffffffu, lane < FEW_WARPS ? tops[lane][t] : 0u), s, inv);
+      if (tid == 0) scales[t] = s;
+      for (int i = tid; i < places; i += FEW_WARPS * 32) {
+        float v[8];
+        if (i < eights) int8_eight_of(p, t, i, v);
+        *reinterpret_cast<uint2*>(few_codes + t * p.pitch + i * 8) = i < eights && finite ? int8_pack(v, s, inv) : make_uint2(0u, 0u);
+      }
+    }
+  } else {
+    if (tid < p.T) scales[tid] = p.sx[tid];
+    for (int t = 0; t < p.T; ++t)
+      for (int i = tid; i < places; i += FEW_WARPS * 32) {
+        const int8_t* from = p.codes + t * p.ldc + i * 8;
+        uint2 v = make_uint2(0u, 0u);
+        if (i * 8 + 8 <= p.K) v = *reinterpret_cast<const uint2*>(from);
+        else
+          for (int j = 0; i * 8 + j < p.K; ++j) (j < 4 ? v.x : v.y) |= ((uint32_t)from[j] & 255u) << (8 * (j % 4));
+        *reinterpret_cast<uint2*>(few_codes + t * p.pitch + i * 8) = v;
+      }
+  }
+  __syncthreads();
+  const int8_t* x = few_codes + min(g, p.T - 1) * p.pitch + tig * 32;
   for (; tile < p.tiles; tile += gridDim.x) {
     int acc[2][4] = {};
     for (int s0 = warp; s0 < slices; s0 += FEW_RING * FEW_WARPS) {
@@ -224,14 +280,9 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
       for (int u = 0; u < FEW_RING; ++u) {
         const int s = s0 + u * FEW_WARPS;
         if (s >= slices) break;
-        const int left = p.K - s * FEW_SLICE - tig * 32;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint4 b = make_uint4(0, 0, 0, 0);
-          if (left > 16 * i) {
-            b = *reinterpret_cast<const uint4*>(x + s * FEW_SLICE + 16 * i);
-            if (left < 16 * i + 16) b = int8_mask(b, left - 16 * i);
-          }
+          const uint4 b = *reinterpret_cast<const uint4*>(x + s * FEW_SLICE + 16 * i);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             const uint4 lo = ring[u][2 * m][i], hi = ring[u][2 * m + 1][i];
@@ -262,7 +313,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
         a += part[(w * FEW_ROWS + t) * FEW_PL + c];
         if (GATED) b += part[(w * FEW_ROWS + t) * FEW_PL + 16 + c];
       }
-      const float s = p.sx[t];
+      const float s = scales[t];
       float y = fmaf((float)a * s, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
       if (GATED) y = int8_silu(y) * fmaf((float)b * s, p.sw[p.cols + col], int8_bias(p.bias, p.bias_f32, p.cols + col));
       if (p.out_f32) static_cast<float*>(p.out)[t * p.ldo + col] = y;
@@ -272,11 +323,16 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
   }
 }
 
+static int few_pitch(long K) { return (int)((K + FEW_SLICE - 1) / FEW_SLICE * FEW_SLICE + 16); }
+
 template <bool GATED>
-static int launch_int8_few(const Int8Call& c, bool early, cudaStream_t st) {
+static int launch_int8_few(const Int8Call& c, int device, cudaStream_t st) {
+  static OncePerDevice once;
+  if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(int8_few_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_CODES); })) return -e;
   const int cols = (int)(GATED ? c.N / 2 : c.N), per = GATED ? 16 : 32, tiles = (cols + per - 1) / per;
-  const Int8Few p = {c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, cols, tiles, (int)c.bias_f32, (int)c.out_f32};
-  launch_step(early, int8_few_kernel<GATED>, dim3(tiles < 296 ? tiles : 296), FEW_WARPS * 32, 0, st, p);
+  const Int8Few p = {c.x, c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldx, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, cols, tiles, few_pitch(c.K),
+                     (int)c.x_f32, int8_rows_vec(c), (int)c.bias_f32, (int)c.out_f32};
+  int8_few_kernel<GATED><<<tiles < 296 ? tiles : 296, FEW_WARPS * 32, c.T * p.pitch, st>>>(p);
   return -(int)cudaGetLastError();
 }
 
@@ -499,7 +555,6 @@ static int launch_int8_split(const Int8Call& c, bool early, int device, cudaStre
   auto fit = [&](int ctas) { const int n = ctas / tiles; return n < 1 ? 1 : n > 4 ? 4 : n; };
   int parts = fit(128);
   if (parts * tiles < 112) parts = fit(256);
-  if (const char* e = getenv("I8S")) parts = atoi(e);
   p.parts = parts > p.kb ? p.kb : parts;
   const int per_sm = tiles * p.parts <= 128 ? 1 : 2, most = stages(TB, per_sm), steps = (p.kb + p.parts - 1) / p.parts;
   p.stages = most < steps ? most : steps;
@@ -798,8 +853,7 @@ static int launch_int8_tiles(const Int8Call& c, bool early, int device, cudaStre
 
 enum Int8Route { INT8_FEW, INT8_SPLIT, INT8_TILES };
 static Int8Route int8_route(const Int8Call& c) {
-  if (const char* e = getenv("I8ROUTE")) return (Int8Route)atoi(e);
-  if (c.T <= FEW_ROWS && c.N * c.K <= (32l << 20)) return INT8_FEW;
+  if (c.T <= FEW_ROWS && c.N * c.K <= (32l << 20) && c.T * few_pitch(c.K) <= FEW_CODES) return INT8_FEW;
   const long tiles = (c.T + 127) / 128 * ((c.gated ? c.N / 2 + 63 : c.N + 127) / (c.gated ? 64 : 128));
   return c.T <= 128 || tiles <= 148 ? INT8_SPLIT : INT8_TILES;
 }
@@ -814,7 +868,14 @@ extern "C" int inv_int8_rows(const void* call) {
   return launch_int8_rows(c, (cudaStream_t)c.stream);
 }
 
-// Codes first where x is given, then the product, which starts while they are made: the kernel of the codes is launched plainly, so everything in front of it is
+// Whether a product makes the codes for itself and wants no place for them.
+extern "C" int inv_int8_alone(long T, long N, long K) {
+  Int8Call c = {};
+  c.T = T; c.N = N; c.K = K;
+  return int8_route(c) == INT8_FEW;
+}
+
+// Codes first where x is given and the product does not make them, then the product, which starts while they are made: the kernel of the codes is launched plainly, so everything in front of it is
 // complete when the product's first weights are read.
 extern "C" int inv_int8_linear(const void* call) {
   const Int8Call& c = *static_cast<const Int8Call*>(call);
@@ -825,16 +886,16 @@ extern "C" int inv_int8_linear(const void* call) {
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;
   const bool early = c.x != nullptr;
   const Int8Route route = int8_route(c);
+  if (route != INT8_FEW && (c.codes == nullptr || c.sx == nullptr)) return -ERR_BAD_ARG;
+  if (route == INT8_FEW) return c.gated ? launch_int8_few<true>(c, device, st) : launch_int8_few<false>(c, device, st);
   if (early)
     if (const int e = launch_int8_rows(c, st)) return e;
-  if (route == INT8_FEW) return c.gated ? launch_int8_few<true>(c, early, st) : launch_int8_few<false>(c, early, st);
   if (route == INT8_SPLIT) {
 #define INV_SPLIT(TB) (c.gated ? launch_int8_split<TB, true>(c, early, device, st) : launch_int8_split<TB, false>(c, early, device, st))
     const long col_tiles = (c.gated ? c.N / 2 + 63 : c.N + 127) / (c.gated ? 64 : 128);
     int tb = c.T <= 16 ? 16 : c.T <= 32 ? 32 : c.T <= 64 ? 64 : 128;
     if (c.T > 64)
       while (tb > 32 && (c.T + tb - 1) / tb * col_tiles < 100) tb /= 2;
-    if (const char* e = getenv("I8TB")) tb = atoi(e);
     return tb <= 16 ? INV_SPLIT(16) : tb <= 32 ? INV_SPLIT(32) : tb <= 64 ? INV_SPLIT(64) : INV_SPLIT(128);
 #undef INV_SPLIT
   }

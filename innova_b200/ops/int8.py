@@ -8,6 +8,7 @@ gives NaN. ``engines.int8_quantize_per_token`` and ``inference.serving.INT8Infer
 No gradient and no tangent passes through these."""
 from __future__ import annotations
 
+import functools
 import struct
 from typing import NamedTuple, Optional, Union
 
@@ -18,7 +19,8 @@ from torch.autograd import forward_ad
 from .. import _native
 from . import runtime as rt
 
-_native.register_cuda_sigs({"inv_int8_rows": [_native.vp], "inv_int8_linear": [_native.vp]})
+_native.register_cuda_sigs({"inv_int8_rows": [_native.vp], "inv_int8_linear": [_native.vp],
+                            "inv_int8_alone": [_native.i64] * 3})
 
 # What the entries are given: x, weights, their scales, bias, result, codes, their scales, status and stream; tokens, weight rows, K; strides of x, weights,
 # result and codes; whether x, the result and the bias are fp32; gated.
@@ -104,6 +106,11 @@ def check_weight(w: Int8Weight, dims: int):
         raise ValueError(f"weight rows with strides {q.stride()}: unit stride and 16-byte boundaries on a GPU (Int8Weight.quantize makes them so)")
 
 
+@functools.lru_cache(maxsize=1024)
+def _alone(T, N, K):
+    return rt.lib().inv_int8_alone(T, N, K) != 0
+
+
 def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
                 gated: bool = False) -> torch.Tensor:
     """x [..., K], in bf16 or fp32 or as ``quantize_rows`` gives it, times w [N, K] -> [..., N] in ``out_dtype`` (bf16 or fp32; that of x if not given, bf16
@@ -137,7 +144,10 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
     if T == 0 or cols == 0 or K == 0:
         return _without_products(out, bias, cols, gated)
     with rt.device_of(x):
-        if codes is None:
+        alone = codes is None and T <= 8 and _alone(T, N, K)
+        if alone:
+            from_x, from_codes, from_scale, ld_codes = rows.data_ptr(), 0, 0, 0
+        elif codes is None:
             wide = (K + 15) // 16 * 16
             work = torch.empty(T * (wide + 4), dtype=torch.uint8, device=x.device)
             from_x, from_codes, from_scale, ld_codes = rows.data_ptr(), work.data_ptr(), work.data_ptr() + T * wide, wide
@@ -151,7 +161,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
         rt.check(rt.lib().inv_int8_linear(_CALL(from_x, q.data_ptr(), sw.data_ptr(), rt.ptr(bias), out.data_ptr(), from_codes, from_scale, rt.status_ptr(x),
                                                 rt.stream_ptr(), T, N, K, ld, q.stride(0), cols, ld_codes, dtype is _fp32, out_dtype is _fp32,
                                                 bias is not None and bias.dtype is _fp32, gated)), "inv_int8_linear")
-        if codes is None:
+        if codes is None and not alone:
             rt.count_launches(1)
     return out
 
