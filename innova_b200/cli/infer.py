@@ -28,6 +28,7 @@ def main(argv=None):
     ap.add_argument("--greedy", action="store_true")
     ap.add_argument("--ref-layout", action="store_true", help="matrices stored [in, out] as the reference's Linear reads them")
     ap.add_argument("--kv-format", default="oil4")
+    ap.add_argument("--weights", default=None, choices=("int8",), help="projections and experts in 8-bit integers with a scale for each channel")
     ap.add_argument("--device", default="auto")
     ap.add_argument("--tokens", default="", help="comma-separated prompt token ids (no tokenizer needed)")
     a = ap.parse_args(argv)
@@ -43,7 +44,7 @@ def main(argv=None):
     model = export.load_model(path, dtype=torch.bfloat16 if dev.type == "cuda" else torch.float32, device=dev, ref_layout=a.ref_layout)
     vocab = os.path.join(a.model_dir, os.path.basename(path) + ".vocab") if a.model_dir else path + ".vocab"
     tok = load_tokenizer(vocab) if os.path.exists(vocab) else (ByteTokenizer() if model.cfg.vocab_size <= 256 else None)
-    gen = Generator(model, tok, kv_format=a.kv_format if dev.type == "cuda" else "bf16", max_batch=1)
+    gen = Generator(model, tok, kv_format=a.kv_format if dev.type == "cuda" else "bf16", max_batch=1, weight_format=a.weights)
     sp = SamplingParams() if a.greedy else SamplingParams(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p)
     if a.tokens:
         ids = [int(t) for t in a.tokens.split(",")]

@@ -6,6 +6,7 @@ InferenceEngine generate / stream / batch entry points (engines/inference/infere
 Prefill runs the flash-attention kernel on the whole prompt and appends K/V to the cache; every decode
 step runs the projections as skinny GEMMs and ``paged_decode`` attention over the (OIL4 or bf16) cache, or over an
 fp8 cache (``kv_format="fp8"``) one launch from the projection to the pages and one attention for any number of new tokens.
+``weight_format="int8"`` takes the blocks' projections and experts in 8-bit integers; mixture layers run up to 64 tokens in two launches.
 """
 from __future__ import annotations
 
@@ -16,6 +17,7 @@ from typing import Callable, List, Optional, Sequence
 import torch
 
 from .. import ops
+from ..ops.int8 import Int8Linears
 from .kv_cache import PagedKVCache
 from .sampler import Sampler, SamplingParams
 
@@ -38,7 +40,9 @@ class GenerationStats:
 
 class Generator:
     def __init__(self, model, tokenizer=None, kv_format: str = "oil4", max_batch: int = 1, max_seq: Optional[int] = None, linear_fn=None,
-                 num_pages: Optional[int] = None):
+                 num_pages: Optional[int] = None, weight_format: Optional[str] = None):
+        """``weight_format="int8"``: projections and experts of the blocks in 8-bit integers with a scale for each channel (``ops.int8``), made here from the
+        model's weights, which stay as they are."""
         self.model = model.eval()
         self.cfg = model.cfg
         self.tok = tokenizer
@@ -47,6 +51,8 @@ class Generator:
         self.stats = GenerationStats()
         # models of the registry bring their own cache and step function; the rest run the dense decoder's step below
         self.stepped = hasattr(model, "make_cache")
+        if weight_format not in (None, "int8") or (weight_format and (self.stepped or linear_fn is not None)):
+            raise ValueError(f"weight_format {weight_format!r}: 'int8', for decoders of this package's blocks and without a linear_fn")
         if self.stepped:
             self.cache = model.make_cache(max_batch, self.max_seq, self.device, num_pages)
             self._graphs, self._warm, self.use_graphs = {}, {}, self.device.type == "cuda"
@@ -54,6 +60,11 @@ class Generator:
         if self.device.type != "cuda" and kv_format == "oil4" and self.cfg.head_dim % 32:
             kv_format = "bf16"
         self.cache = PagedKVCache(self.cfg.num_layers, self.cfg.kv_heads, self.cfg.head_dim, max_batch, self.max_seq, self.device, kv_format)
+        self.int8_experts = {}
+        if weight_format == "int8":
+            linear_fn = Int8Linears(lin for blk in model.layers for part in (blk.attention, getattr(blk, "ffn", None)) if part is not None
+                                    for lin in part.children() if isinstance(lin, torch.nn.Linear))
+            self.int8_experts = {blk: blk.moe.int8_weights() for blk in model.layers if hasattr(blk, "moe") and blk.moe.ep is None}
         self.linear = linear_fn or (lambda x, lin: ops.linear(x, lin.weight, lin.bias))
 
     # ------------------------------------------------------------------ one forward over new tokens
@@ -216,6 +227,9 @@ class Generator:
     def _after_attention(self, blk, x, a):
         """The rest of a block behind its attention's output ``a``."""
         att = self.linear(a, blk.attention.o_proj)
+        if hasattr(blk, "moe"):
+            x = x + att
+            return blk.moe.serve(blk.ffn_norm(x), x, self.int8_experts.get(blk))
         if self.cfg.use_parallel_residual:
             return x + att + self._ffn(blk, blk.ffn_norm(x))
         x = x + att
@@ -223,6 +237,8 @@ class Generator:
 
     def _ffn(self, blk, h):
         f = blk.ffn
+        if f.gated and isinstance(self.linear, Int8Linears):
+            return self.linear(self.linear.gated(h, f.gate_up_proj), f.down_proj)
         if f.gated:
             return self.linear(ops.swiglu(self.linear(h, f.gate_up_proj)), f.down_proj)
         act = ops.gelu(self.linear(h, f.up_proj)) if self.cfg.activation == "gelu" else torch.relu(self.linear(h, f.up_proj))

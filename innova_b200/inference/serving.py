@@ -573,7 +573,8 @@ class InferenceEngine:
     """Load ``model.oil`` (+ ``.vocab``) and generate: plain, with statistics, streamed (pieces are flushed on
     punctuation or whitespace) or for a batch of prompts."""
 
-    def __init__(self, model_path: str, device: Optional[str] = None, dtype=None, kv_format: str = "oil4", max_batch: int = 1):
+    def __init__(self, model_path: str, device: Optional[str] = None, dtype=None, kv_format: str = "oil4", max_batch: int = 1,
+                 weight_format: Optional[str] = None):
         import os
         from ..formats import export
         from ..utils.tokenizer import load_tokenizer
@@ -582,7 +583,8 @@ class InferenceEngine:
         self.model = export.load_model(model_path, dtype=dtype, device=dev)
         vocab = model_path + ".vocab"
         self.tok = load_tokenizer(vocab) if os.path.exists(vocab) else None
-        self.gen = Generator(self.model, self.tok, kv_format=kv_format if dev.startswith("cuda") else "bf16", max_batch=max_batch)
+        self.gen = Generator(self.model, self.tok, kv_format=kv_format if dev.startswith("cuda") else "bf16", max_batch=max_batch,
+                             weight_format=weight_format)
 
     def generate(self, prompt: str, max_new_tokens: int = 64, sampling: Optional[SamplingParams] = None) -> str:
         return self.gen.generate(prompt, max_new_tokens, sampling)

@@ -14,7 +14,8 @@ import torch
 import torch.nn as nn
 
 from .. import ops
-from ..ops.moe import moe_ffn
+from ..ops.int8 import Int8Weight
+from ..ops.moe import moe_few_supported, moe_ffn, moe_ffn_few
 from .config import TransformerConfig
 from .dense import Attention, FFN, Norm, _ste, head_norm_state, load_head_norms
 
@@ -48,6 +49,29 @@ class MoELayer(nn.Module):
         if self.shared is not None:
             y = self.shared(h, y)
         return y, aux
+
+    def _plain_shared(self):
+        """Whether the shared expert is one that the layer of a few tokens takes along: SwiGLU without biases and adapters."""
+        s = self.shared
+        return s is not None and s.gated and s.gate_up_proj.bias is None and s.adapter is None
+
+    @torch.no_grad()
+    def int8_weights(self):
+        """Experts, and a shared one, in 8-bit integers, for ``serve``."""
+        shared = (Int8Weight.quantize(self.shared.gate_up_proj.weight), Int8Weight.quantize(self.shared.down_proj.weight)) if self._plain_shared() else None
+        return Int8Weight.quantize(self.w_gate_up), Int8Weight.quantize(self.w_down), shared
+
+    @torch.no_grad()
+    def serve(self, h, residual, int8=None):
+        """The layer for generation, without the auxiliary losses: up to 64 tokens in two launches (``ops.moe.moe_ffn_few``), with experts in 8 bits where
+        ``int8_weights`` are given. More tokens, experts on several ranks and what that form does not have run as in training, with the model's weights."""
+        if self.ep is None:
+            plain = self._plain_shared()
+            w_gate_up, w_down, shared = int8 or (self.w_gate_up, self.w_down, (self.shared.gate_up_proj.weight, self.shared.down_proj.weight) if plain else None)
+            if moe_few_supported(h, self.router.weight, w_gate_up, w_down, self.cfg.top_k):
+                y, self.last_counts = moe_ffn_few(h, self.router.weight, w_gate_up, w_down, residual, self.cfg.top_k, shared)
+                return y if plain or self.shared is None else self.shared(h, y)
+        return self(h, residual)[0]
 
 
 class MoEBlock(nn.Module):

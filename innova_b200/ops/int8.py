@@ -18,6 +18,8 @@ from torch.autograd import forward_ad
 
 from .. import _native
 from . import runtime as rt
+from .functional import swiglu
+from .gemm import linear
 
 _native.register_cuda_sigs({"inv_int8_rows": [_native.vp], "inv_int8_linear": [_native.vp],
                             "inv_int8_alone": [_native.i64] * 3})
@@ -144,7 +146,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
     if T == 0 or cols == 0 or K == 0:
         return _without_products(out, bias, cols, gated)
     with rt.device_of(x):
-        alone = codes is None and T <= 8 and _alone(T, N, K)
+        alone = codes is None and T <= 4 and _alone(T, N, K)
         if alone:
             from_x, from_codes, from_scale, ld_codes = rows.data_ptr(), 0, 0, 0
         elif codes is None:
@@ -164,6 +166,24 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
         if codes is None and not alone:
             rt.count_launches(1)
     return out
+
+
+class Int8Linears:
+    """A ``linear_fn`` of ``inference.Generator``: projections with their weights in 8-bit integers, laid out once; others as they are. The modules keep their
+    own weights, which later changes of them do not reach."""
+
+    def __init__(self, linears):
+        with torch.no_grad():
+            self.weights = {lin: Int8Weight.quantize(lin.weight) for lin in linears}
+
+    def __call__(self, x, lin):
+        w = self.weights.get(lin)
+        return linear(x, lin.weight, lin.bias) if w is None else int8_linear(x, w, lin.bias)
+
+    def gated(self, x, lin):
+        """silu(gate) * up of a projection that holds both."""
+        w = self.weights.get(lin)
+        return swiglu(linear(x, lin.weight, lin.bias)) if w is None else int8_linear(x, w, lin.bias, gated=True)
 
 
 def _without_products(out, bias, cols, gated):
