@@ -660,6 +660,7 @@ struct Int8Tiles {
   void* out;
   long ldo;
   int T, K, cols, m_tiles, n_tiles;
+  uint32_t inv_n;              // div_reciprocal
   int bias_f32, boxes;         // boxes: results leave through TMA stores
   int* status;
 };
@@ -725,7 +726,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
       int it = 0;
       bool ok = true;
       for (int w = pair; ok && w < total; w += npairs) {
-        const int m0 = w / p.n_tiles * BM + (int)cta * 128, n = w % p.n_tiles * TN;
+        const int mt = div_by(w, p.n_tiles, p.inv_n), m0 = mt * BM + (int)cta * 128, n = (w - mt * p.n_tiles) * TN;
         const int n0 = GATED ? n + (int)cta * p.cols : n + (int)cta * 128;
         for (int kb = 0; kb < kb_total; ++kb, ++it) {
           const int s = it % STAGES;
@@ -772,7 +773,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
     // scales and biases of a tile come from memory under the tile before it (3003 x 512 x 4096 gated: 16.2 us without, 15.1 with)
     float next_scale[4], next_bias[4], next_sx = 0.f;
     auto fetch = [&](int w) {
-      const int m0 = w / p.n_tiles * BM + (int)cta * 128 + q * 32, n0 = w % p.n_tiles * TN;
+      const int mt = div_by(w, p.n_tiles, p.inv_n), m0 = mt * BM + (int)cta * 128 + q * 32, n0 = (w - mt * p.n_tiles) * TN;
 #pragma unroll
       for (int x = 0; x < 4; ++x) {           // gated: CW columns of the gate, then those of the up product
         const int c = n0 + half * CW + (GATED ? (x & 1) : x) * 32 + lane, at = GATED && x >= 2 ? p.cols + c : c;
@@ -784,7 +785,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
     int i = 0;
     if (pair < total) fetch(pair);
     for (int w = pair; w < total; w += npairs, ++i) {
-      const int m0 = w / p.n_tiles * BM + (int)cta * 128 + q * 32, n0 = w % p.n_tiles * TN, acc = i & 1;
+      const int mt = div_by(w, p.n_tiles, p.inv_n), m0 = mt * BM + (int)cta * 128 + q * 32, n0 = (w - mt * p.n_tiles) * TN, acc = i & 1;
       const float sx = next_sx;
       __syncwarp();
 #pragma unroll
@@ -865,7 +866,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_remote(mapa_shared(smem_u32(&tmem_empty[acc]), 0));
+      if (lane == 0) mbar_arrive_remote_relaxed(mapa_shared(smem_u32(&tmem_empty[acc]), 0));
     }
     if (lane == 0) tma_store_wait_all();
   }
@@ -894,7 +895,7 @@ static int launch_int8_tiles(const Int8Call& c, bool early, int device, cudaStre
   Int8Tiles p;
   p.sx = c.sx; p.sw = c.sw; p.bias = c.bias; p.out = c.out; p.ldo = c.ldo; p.T = (int)c.T; p.K = (int)c.K; p.cols = cols;
   p.m_tiles = (int)((c.T + BM - 1) / BM); p.n_tiles = (cols + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
-  p.bias_f32 = (int)c.bias_f32; p.status = c.status;
+  p.inv_n = div_reciprocal(p.n_tiles); p.bias_f32 = (int)c.bias_f32; p.status = c.status;
   p.boxes = ((uintptr_t)c.out | (uintptr_t)(c.ldo * size)) % 16 == 0;
   CUtensorMap ta, tb, tc;
   int rc = make_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.codes, {(uint64_t)c.K, (uint64_t)c.T}, {(uint64_t)c.ldc}, {BK, 128});
