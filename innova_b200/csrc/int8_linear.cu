@@ -51,11 +51,14 @@ __device__ __forceinline__ uint64_t int8_fma2(uint64_t a, uint64_t b, uint64_t c
 // The scale of a row from the bits of its largest |x|: not a number is above infinity is above the rest. False where it is not finite.
 __device__ __forceinline__ bool int8_scale(uint32_t top, float& s, float& inv) {
   const bool finite = top < 0x7f800000u;
-  s = finite ? __fdiv_rn(fmaxf(__uint_as_float(top), INT8_LEAST), 127.f) : __uint_as_float(0x7fc00000u);
-  inv = finite ? __frcp_rn(s) : 0.f;
+  // a / 127 rounded to the nearest: the quotient by a product with 1 / 127, corrected by its remainder, which is exact
+  constexpr float PART = 1.f / 127.f;
+  const float a = finite ? fmaxf(__uint_as_float(top), INT8_LEAST) : 1.f, q = a * PART;
+  s = finite ? fmaf(fmaf(-127.f, q, a), PART, q) : __uint_as_float(0x7fc00000u);
+  inv = __fdividef(1.f, s);                                // within two units of the last place
   return finite;
 }
-// Codes of eight values. x * inv is off by under 1e-5 from the quotient, so the sum with MAGIC rounds as the quotient does unless that is as near to a half: there, one
+// Codes of eight values. x * inv is off by under 5e-5 from the quotient, so the sum with MAGIC rounds as the quotient does unless that is as near to a half: there, one
 // time in some thousands, the border decides. Packed arithmetic, two values an instruction: instructions bound the kernel of many rows.
 __device__ __forceinline__ uint2 int8_pack(const float2* v, float s, float inv) {
   constexpr float MAGIC = 12582912.f;
@@ -67,7 +70,7 @@ __device__ __forceinline__ uint2 int8_pack(const float2* v, float s, float inv) 
     const uint64_t x = int8_two(v[j]), m = int8_fma2(x, inv2, magic), r = int8_fma2(x, inv2, int8_fma2(m, minus, magic));
     u[2 * j] = (uint32_t)m;
     u[2 * j + 1] = (uint32_t)(m >> 32);
-    far = fmax3(far, fabsf(__uint_as_float((uint32_t)r)), fabsf(__uint_as_float((uint32_t)(r >> 32))));
+    far = fmaxf(fmaxf(far, fabsf(__uint_as_float((uint32_t)r))), fabsf(__uint_as_float((uint32_t)(r >> 32))));
   }
   if (far > 0.4999f) {
 #pragma unroll
@@ -119,13 +122,10 @@ struct Int8Eight {
   }
 };
 
-// A CTA takes a row, or (WARP) each of its eight warps one, a thread up to four times eight of its values, which it keeps between the maximum and the rounding; what a
+// A CTA takes a row, or (WARP) each of its eight warps one, a thread up to HOLD times eight of its values, which it keeps between the maximum and the rounding; what a
 // long row has beyond that is read twice. A row with a value that is not finite gets NaN for its scale. Codes are written in eights, zeros behind the row.
-// 8192 x 4096 in bf16: 28 us, 3.6 TB/s, bound by instructions (some 17 a value, the scale's division and the sum over the row among them); with conversions for
-// the rounding 30. CTAs that stay and load the next row under this one: 25.6, but 3003 x 512 3.8 for 2.8 and 301 x 1411 3.2 for 2.5.
-template <typename T, bool VEC, bool WARP>
+template <typename T, bool VEC, bool WARP, int HOLD>
 __global__ void __launch_bounds__(512) int8_rows_kernel(const T* __restrict__ x, long ldx, int rows, int K, int8_t* __restrict__ codes, long ldc, float* __restrict__ sx) {
-  constexpr int HOLD = 4;
   __shared__ uint32_t sh[16];
   release_next();
   const long r = WARP ? (long)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
@@ -174,14 +174,23 @@ static bool int8_rows_vec(const Int8Call& c) {
 
 static int launch_int8_rows(const Int8Call& c, cudaStream_t st) {
   const bool vec = int8_rows_vec(c);
-  const bool warps = c.K <= 1024 && c.T > 296;
-  const int threads = warps ? 256 : c.K <= 512 ? 64 : c.K <= 1024 ? 128 : c.K <= 4096 ? 256 : 512;
+  // Instructions bound many rows, and a row costs each of its warps some 150 besides its values: then few warps a row, 64 values a lane. 8192 x 4096 in bf16: 21 us
+  // (28 with eight warps a row and 16 values a lane); 2048 x 11008 17 (21). Fewer than two eights for each thread that the GPU holds: many warps, for the shortest
+  // chain (301 x 1411: 2.6 us, 5.3 as above); a warp for each of many short rows.
+  const long eights = (c.K + 7) / 8;
+  const bool many = c.T * eights >= 2l * 148 * 2048, warps = many ? eights <= 256 : c.T > 296 && eights <= 128;
+  const int hold = eights <= 64 ? 2 : eights <= 128 || !many ? 4 : 8;
+  const long want = many ? (eights + 7) / 8 : c.K <= 512 ? 64 : c.K <= 1024 ? 128 : c.K <= 4096 ? 256 : 512;
+  const int threads = (int)(warps ? 256 : want >= 512 ? 512 : (want + 31) / 32 * 32);
   const unsigned grid = (unsigned)(warps ? (c.T + 7) / 8 : c.T);
-#define INV_ROW(E, V, W) int8_rows_kernel<E, V, W><<<grid, threads, 0, st>>>((const E*)c.x, c.ldx, (int)c.T, (int)c.K, c.codes, c.ldc, c.sx)
-#define INV_ROWS(E, V)             \
-  do {                             \
-    if (warps) INV_ROW(E, V, true); \
-    else INV_ROW(E, V, false);     \
+#define INV_ROW(E, V, W, H) int8_rows_kernel<E, V, W, H><<<grid, threads, 0, st>>>((const E*)c.x, c.ldx, (int)c.T, (int)c.K, c.codes, c.ldc, c.sx)
+#define INV_ROWS(E, V)                                \
+  do {                                                \
+    if (!warps && hold <= 4) INV_ROW(E, V, false, 4); \
+    else if (!warps) INV_ROW(E, V, false, 8);         \
+    else if (hold == 2) INV_ROW(E, V, true, 2);       \
+    else if (hold == 4) INV_ROW(E, V, true, 4);       \
+    else INV_ROW(E, V, true, 8);                      \
   } while (0)
   if (c.x_f32) {
     if (vec) INV_ROWS(float, true);
@@ -190,8 +199,8 @@ static int launch_int8_rows(const Int8Call& c, cudaStream_t st) {
     if (vec) INV_ROWS(__nv_bfloat16, true);
     else INV_ROWS(__nv_bfloat16, false);
   }
-#undef INV_ROWS
 #undef INV_ROW
+#undef INV_ROWS
   return -(int)cudaGetLastError();
 }
 

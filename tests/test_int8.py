@@ -31,8 +31,8 @@ def weight(N, K, seed=1, device="cpu"):
 
 
 def definition(x):
-    """(codes, scales) of rows in 64 bits; the scale is rounded to fp32 as it is stored."""
-    s = (x.double().abs().amax(-1).clamp(min=1e-10) / 127).float()
+    """(codes, scales) of rows in 64 bits; 1e-10 is the fp32 number, and the scale is rounded to fp32 as it is stored."""
+    s = (x.float().abs().amax(-1).clamp(min=1e-10).double() / 127).float()
     return torch.round(x.double() / s.double().unsqueeze(-1)), s
 
 
@@ -153,6 +153,21 @@ def test_rows_gpu(dtype):
     x = torch.tensor([[0.0] * 40, [1e-12] * 40, [1] * 39 + [float("nan")], [float("-inf")] + [1] * 39], dtype=dtype)
     r, c = quantize_rows(x.cuda()), quantize_rows(x)
     assert torch.equal(r.q.cpu(), c.q) and torch.equal(r.scale.cpu().nan_to_num(7), c.scale.nan_to_num(7))
+
+
+@gpu
+def test_scales_and_codes_of_all_sizes_gpu():
+    """Scales are the nearest to a 127th over all exponents; codes of random and of nearly tied quotients are the definition's."""
+    g = torch.Generator().manual_seed(9)
+    x = torch.randn(1 << 20, 1, generator=g) * torch.exp2(torch.randint(-126, 127, (1 << 20, 1), generator=g).float())
+    r, (c, s) = quantize_rows(x.cuda()), definition(x)
+    assert torch.equal(r.scale.cpu(), s) and torch.equal(r.q.cpu().double(), c)
+    x = torch.randn(64, 8192, generator=g)
+    x[:, 0] = 127 * (1 + torch.rand(64, generator=g))                              # the largest: quotients n + 1/2 and their neighbours
+    x[:, 1:4096] = ((torch.randint(-120, 120, (64, 4095), generator=g) + 0.5) * (x[:, :1] / 127) * (1 + torch.randint(-3, 4, (64, 4095), generator=g) * 2.0 ** -23))
+    for rows_, many in ((x, False), (x.repeat(20, 1), True)):
+        r, (c, s) = quantize_rows(rows_.cuda()), definition(rows_)
+        assert torch.equal(r.scale.cpu(), s) and torch.equal(r.q.cpu().double(), c)
 
 
 FEW = [1, 2, 8, 9, 16, 17, 32, 33, 63, 64]
