@@ -193,8 +193,8 @@ struct Shape {
   static constexpr int STEP = I8 ? 128 : 64, B_STAGE = (I8 ? 2 : 1) * TB * 128;
   static constexpr int PER_SM = I8 ? 1 : 2, ROOM = ((I8 ? 216 : 102) * 1024 - 1024) / (A_STAGE + B_STAGE), STAGES = ROOM < 12 ? ROOM : 12;
   static constexpr int ACC = 4, CONV = 4, SETS = I8 ? 2 : 1;   // buffers of sums and of converted weights; sets of four warps of sums
-  // warps of loads, of products, of items, of sums, of conversions
-  static constexpr int SUMS = 3, CONVERT = SUMS + 4 * SETS, THREADS = 32 * (CONVERT + (I8 ? 4 * CONV : 0));
+  // warps of weights, of products, of items, of tokens, of sums, of conversions
+  static constexpr int SUMS = 4, CONVERT = SUMS + 4 * SETS, THREADS = 32 * (CONVERT + (I8 ? 4 * CONV : 0));
   static constexpr int SMEM = STAGES * (A_STAGE + B_STAGE) + 1024;
   static constexpr int COLS = ACC * TB + (I8 ? CONV * 64 : 0), TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
 };
@@ -228,20 +228,6 @@ __device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* m
       "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
       ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
       : "memory");
-}
-// Asks without waiting, which mbarrier.try_wait does for tens of microseconds.
-__device__ __forceinline__ bool mf_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n"
-      ".reg .pred p;\n"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      "selp.u32 %0, 1, 0, p;\n"
-      "}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
 }
 // Until *p reaches n. False where the limit runs out.
 __device__ __forceinline__ bool mf_wait(const int* p, int n, volatile int* abort_flag, int* status) {
@@ -286,13 +272,13 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
   release_next();
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&full_bar[i], 1);
+      mbar_init(&full_bar[i], I8 ? 1 : 2);       // tokens, and weights where nothing converts them
       mbar_init(&weights_bar[i], 1);
       mbar_init(&empty_bar[i], 1);
     }
     for (int i = 0; i < QUEUE; ++i) {
       mbar_init(&item_full[i], 1);
-      mbar_init(&item_empty[i], 2 + 4 * S::SETS + (I8 ? 4 * CONV : 0));
+      mbar_init(&item_empty[i], 3 + 4 * S::SETS + (I8 ? 4 * CONV : 0));
     }
     for (int i = 0; i < ACC; ++i) {
       mbar_init(&acc_full[i], 1);
@@ -416,7 +402,33 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
       }
     }
   } else if (warp == 0) {
-    // ---------------- loads ----------------
+    // ---------------- weights: as far ahead as there is room ----------------
+    if (elect_one_sync()) {
+      int s = 0, qi = 0;
+      uint32_t ph = 1, qph = 0;
+      bool ok = true;
+      while (ok) {
+        if (!mbar_wait(&item_full[qi], qph, abort_flag, p.status, ERR_WAIT_MISC)) break;
+        const Item it = s_item[qi];
+        mbar_arrive(&item_empty[qi]);
+        if (++qi == QUEUE) { qi = 0; qph ^= 1; }
+        if (it.kind == END) break;
+        if (it.kind == SUM) continue;
+        const bool shared = it.e == p.E;
+        const int plane = shared ? 0 : it.e, end = (it.k0 + it.steps) * STEP;
+        const CUtensorMap* map = it.kind == GATE ? (shared ? &map_shared_gate : &map_gate) : (shared ? &map_shared_down : &map_down);
+        for (int k = it.k0 * STEP; k < end; k += STEP) {
+          if (!mbar_wait(&empty_bar[s], ph, abort_flag, p.status, ERR_WAIT_EMPTY)) { ok = false; break; }
+          uint64_t* bar = I8 ? &weights_bar[s] : &full_bar[s];
+          mbar_expect_tx(bar, A_STAGE);
+          if (it.kind == GATE) tma_load_5d(sA + s * A_STAGE, map, bar, k, 0, 0, it.tile * (MF_F / 8), plane);
+          else tma_load_3d(sA + s * A_STAGE, map, bar, k, it.tile * MF_D, plane);
+          if (++s == STAGES) { s = 0; ph ^= 1; }
+        }
+      }
+    }
+  } else if (warp == 3) {
+    // ---------------- tokens ----------------
     if (elect_one_sync()) {
       int s = 0, qi = 0, ready = -1;               // experts up to `ready` have their activations
       uint32_t ph = 1, qph = 0;
@@ -428,46 +440,18 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
         if (++qi == QUEUE) { qi = 0; qph ^= 1; }
         if (it.kind == END) break;
         if (it.kind == SUM) continue;
-        const int e = it.e, k0 = it.k0, steps = it.steps;
-        const bool shared = e == p.E;
-        const CUtensorMap* map = it.kind == GATE ? (shared ? &map_shared_gate : &map_gate) : (shared ? &map_shared_down : &map_down);
-        auto weights = [&](int i, int at) {
-          uint64_t* bar = I8 ? &weights_bar[at] : &full_bar[at];               // conversions do not wait for the tokens
-          mbar_expect_tx(bar, I8 ? A_STAGE : A_STAGE + B_STAGE);
-          const int k = (k0 + i) * STEP, plane = shared ? 0 : e;
-          if (it.kind == GATE) tma_load_5d(sA + at * A_STAGE, map, bar, k, 0, 0, it.tile * (MF_F / 8), plane);
-          else tma_load_3d(sA + at * A_STAGE, map, bar, k, it.tile * MF_D, plane);
-        };
-        auto tokens = [&](int i, int at) {
-          if (I8) mbar_expect_tx(&full_bar[at], B_STAGE);
-#pragma unroll
-          for (int h = 0; h < (I8 ? 2 : 1); ++h) {
-            if (it.kind == GATE) tma_load_2d(sB + at * B_STAGE + h * TB * 128, &map_x, &full_bar[at], (k0 + i) * STEP + 64 * h, 0);
-            else tma_load_2d(sB + at * B_STAGE + h * TB * 128, &map_act, &full_bar[at], (k0 + i) * STEP + 64 * h, it.first);
-          }
-        };
-        int i = 0;
-        if (it.kind == DOWN && it.a > ready) {     // its weights may come before its activations are there
-          int at = s;
-          uint32_t aph = ph;
-          for (; i < steps && i < STAGES && mf_test(&empty_bar[at], aph); ++i) {
-            weights(i, at);
-            if (++at == STAGES) { at = 0; aph ^= 1; }
-          }
-          // a load whose other half never comes would be waited for in vain: it is sent in any case
-          ok = mf_wait(&done[it.a], p.f_tiles * 4, abort_flag, p.status);
+        if (it.kind == DOWN && it.a > ready) {
+          if (!mf_wait(&done[it.a], p.f_tiles * 4, abort_flag, p.status)) break;
           mf_fence_proxy();
           ready = it.a;
-          for (int j = 0; j < i; ++j) {
-            tokens(j, s);
-            if (++s == STAGES) { s = 0; ph ^= 1; }
-          }
-          if (!ok) break;
         }
-        for (; i < steps; ++i) {
+        const int row = it.kind == GATE ? 0 : it.first, end = (it.k0 + it.steps) * STEP;
+        const CUtensorMap* map = it.kind == GATE ? &map_x : &map_act;
+        for (int k = it.k0 * STEP; k < end; k += STEP) {
           if (!mbar_wait(&empty_bar[s], ph, abort_flag, p.status, ERR_WAIT_EMPTY)) { ok = false; break; }
-          weights(i, s);
-          tokens(i, s);
+          mbar_expect_tx(&full_bar[s], B_STAGE);
+#pragma unroll
+          for (int h = 0; h < (I8 ? 2 : 1); ++h) tma_load_2d(sB + s * B_STAGE + h * TB * 128, map, &full_bar[s], k + 64 * h, row);
           if (++s == STAGES) { s = 0; ph ^= 1; }
         }
       }
