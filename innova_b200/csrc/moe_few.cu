@@ -186,7 +186,7 @@ struct MoeFew {
 };
 
 namespace mf {
-constexpr int A_STAGE = 128 * 128, QUEUE = 8;
+constexpr int A_STAGE = 128 * 128, QUEUE = 2;
 // Bytes of a weight row's step are 128: 64 or 128 values of K.
 template <int TB, bool I8>
 struct Shape {
