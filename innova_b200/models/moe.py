@@ -55,22 +55,26 @@ class MoELayer(nn.Module):
         s = self.shared
         return s is not None and s.gated and s.gate_up_proj.bias is None and s.adapter is None
 
+    def _few_weights(self):
+        """Experts, and a shared one or None, as a forward pass takes them."""
+        s, cfg = self.shared, self.cfg
+        return (_ste(self.w_gate_up, cfg), _ste(self.w_down, cfg),
+                (_ste(s.gate_up_proj.weight, cfg), _ste(s.down_proj.weight, cfg)) if self._plain_shared() else None)
+
     @torch.no_grad()
     def int8_weights(self):
         """Experts, and a shared one, in 8-bit integers, for ``serve``."""
-        shared = (Int8Weight.quantize(self.shared.gate_up_proj.weight), Int8Weight.quantize(self.shared.down_proj.weight)) if self._plain_shared() else None
-        return Int8Weight.quantize(self.w_gate_up), Int8Weight.quantize(self.w_down), shared
+        w_gate_up, w_down, shared = self._few_weights()
+        return Int8Weight.quantize(w_gate_up), Int8Weight.quantize(w_down), shared and tuple(Int8Weight.quantize(w) for w in shared)
 
     @torch.no_grad()
     def serve(self, h, residual, int8=None):
         """The layer for generation, without the auxiliary losses: up to 64 tokens in two launches (``ops.moe.moe_ffn_few``), with experts in 8 bits where
         ``int8_weights`` are given. More tokens, experts on several ranks and what that form does not have run as in training, with the model's weights."""
-        if self.ep is None:
-            plain = self._plain_shared()
-            w_gate_up, w_down, shared = int8 or (self.w_gate_up, self.w_down, (self.shared.gate_up_proj.weight, self.shared.down_proj.weight) if plain else None)
-            if moe_few_supported(h, self.router.weight, w_gate_up, w_down, self.cfg.top_k):
-                y, self.last_counts = moe_ffn_few(h, self.router.weight, w_gate_up, w_down, residual, self.cfg.top_k, shared)
-                return y if plain or self.shared is None else self.shared(h, y)
+        if self.ep is None and moe_few_supported(h, self.router.weight, *(int8[:2] if int8 else (self.w_gate_up, self.w_down)), self.cfg.top_k):
+            w_gate_up, w_down, shared = int8 or self._few_weights()
+            y, self.last_counts = moe_ffn_few(h, self.router.weight, w_gate_up, w_down, residual, self.cfg.top_k, shared)
+            return y if shared is not None or self.shared is None else self.shared(h, y)
         return self(h, residual)[0]
 
 

@@ -104,8 +104,8 @@ def check_weight(w: Int8Weight, dims: int):
                          f"and contiguous fp32 for its rows on {q.device}")
     if q.shape[-1] > MAX_K:
         raise ValueError(f"K of {q.shape[-1]}: sums of more than {MAX_K} products do not fit in 32 bits")
-    if q.is_cuda and (q.data_ptr() % 16 or q.stride(-1) != 1 or any(d % 16 for d in q.stride()[:-1])):
-        raise ValueError(f"weight rows with strides {q.stride()}: unit stride and 16-byte boundaries on a GPU (Int8Weight.quantize makes them so)")
+    if q.is_cuda and (q.data_ptr() % 16 or q.stride(-1) != 1 or any(d % 16 for d in q.stride()[:-1]) or q.stride(-2) < q.shape[-1]):
+        raise ValueError(f"weight rows with strides {q.stride()}: unit stride, 16-byte boundaries and no overlap on a GPU (Int8Weight.quantize makes them so)")
 
 
 @functools.lru_cache(maxsize=1024)
@@ -130,7 +130,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
             and (codes is not None or dtype is _bf16 or dtype is _fp32) and (out_dtype is _bf16 or out_dtype is _fp32)
             and (bias is None or bias.shape == sw.shape and (bias.dtype is _bf16 or bias.dtype is _fp32) and bias.get_device() == dev)
             and (codes is None or dtype is _int8 and codes.scale.shape == x.shape[:-1] and codes.scale.dtype is _fp32 and codes.scale.get_device() == dev)
-            and (dev < 0 or q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.data_ptr() % 16 == 0)) or gated and q.shape[0] % 2:
+            and (dev < 0 or q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= q.shape[1] and q.data_ptr() % 16 == 0)) or gated and q.shape[0] % 2:
         _refuse(x, codes, w, bias, out_dtype, gated)
     refuse_gradients("int8_linear", x, bias)
     N, K = q.shape
@@ -154,7 +154,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
             work = torch.empty(T * (wide + 4), dtype=torch.uint8, device=x.device)
             from_x, from_codes, from_scale, ld_codes = rows.data_ptr(), work.data_ptr(), work.data_ptr() + T * wide, wide
         else:
-            if rows.data_ptr() % 16 or ld % 16:
+            if rows.data_ptr() % 16 or ld % 16 or ld < K:
                 aligned = _empty_rows(rows.shape, x.device)
                 rows, ld = aligned.copy_(rows), aligned.stride(0)
             scale = codes.scale.contiguous()

@@ -242,13 +242,14 @@ def moe_few_supported(x, router_w, w_gate_up: Weight, w_down: Weight, top_k: int
 
 
 def _few_plain_weight(w, shape, dev, dtype) -> bool:
-    return isinstance(w, torch.Tensor) and w.shape == shape and w.dtype is dtype and w.get_device() == dev and w.is_contiguous() and w.data_ptr() % 16 == 0
+    return (isinstance(w, torch.Tensor) and w.shape == shape and w.dtype is dtype and w.get_device() == dev
+            and (dev < 0 or w.is_contiguous() and w.data_ptr() % 16 == 0))
 
 
 def _few_int8_weight(w, shape, dev) -> bool:
     q, s = w
     return (q.shape == shape and q.dtype is torch.int8 and s.shape == shape[:-1] and s.dtype is torch.float32 and q.get_device() == dev == s.get_device()
-            and q.is_contiguous() and s.is_contiguous() and q.data_ptr() % 16 == 0)
+            and s.is_contiguous() and (dev < 0 or q.is_contiguous() and q.data_ptr() % 16 == 0))
 
 
 def _few_check(x, router_w, w_gu, w_down, residual, top_k, shared):
@@ -293,8 +294,8 @@ def _few_refuse(x, router_w, w_gu, w_down, residual, top_k, shared):
             raise ValueError(f"{what} of {q.dtype} {tuple(q.shape)}: {x.dtype} with {dims} dimensions, or an Int8Weight")
         if q.device != x.device:
             raise ValueError(f"{what} on {q.device}, x on {x.device}")
-        if not q.is_contiguous() or q.data_ptr() % 16:
-            raise ValueError(f"{what} with strides {q.stride()}: contiguous, on 16-byte boundaries")
+        if q.is_cuda and (not q.is_contiguous() or q.data_ptr() % 16):
+            raise ValueError(f"{what} with strides {q.stride()}: contiguous, on 16-byte boundaries on a GPU")
     E, inner, grain = router_w.shape[0], (w_down.q if i8[0] else w_down).shape[-1], 16 if i8[0] else 8
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"residual of {residual.dtype} {tuple(residual.shape)} on {residual.device} for x of {x.dtype} {tuple(x.shape)}")
@@ -332,6 +333,8 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
         return out, counts.zero_()
     with rt.device_of(x):
         rows, ldx = _dense_rows(x, D)
+        if ldx < D:                                 # one row for several tokens
+            rows, ldx = x.reshape(T, D).contiguous(), D
         res, ldr = (None, 0) if residual is None else _dense_rows(residual, D)
         if not router_w.is_contiguous() or router_w.data_ptr() % 16:
             router_w = router_w.clone(memory_format=torch.contiguous_format)

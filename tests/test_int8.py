@@ -254,6 +254,10 @@ def test_linear_views_and_leading_dimensions():
     assert torch.equal(int8_linear(x[5], w), want[5])
     r = quantize_rows(x)
     assert torch.equal(int8_linear(Int8Rows(r.q.contiguous(), r.scale), w), want)      # rows of codes off 16-byte boundaries
+    one = Int8Rows(r.q[3].expand(24, 101), r.scale[3].expand(24))                      # one row for all tokens
+    assert torch.equal(int8_linear(one, w), want[3].expand(24, 96)) and torch.equal(int8_linear(x[3].expand(24, 101), w), want[3].expand(24, 96))
+    with pytest.raises(ValueError, match="overlap"):
+        int8_linear(x, Int8Weight(w.q[:1].expand(96, 101), w.scale))
     with pytest.raises(ValueError, match="16-byte"):
         int8_linear(x, Int8Weight(w.q.contiguous(), w.scale))
     with pytest.raises(ValueError, match="x on"):

@@ -72,6 +72,16 @@ def test_mixture_with_biased_activation_of_the_shared_expert():
     assert Generator(m, kv_format="bf16", max_batch=1, max_seq=64).generate_tokens(ids, max_new_tokens=4) == greedy(m, ids, 4)
 
 
+def test_mixture_trained_in_a_format_is_served_in_it():
+    m = mixture(ste_format="oil8")
+    ids = torch.randint(0, 97, (2, 9), generator=torch.Generator().manual_seed(8))
+    x, h = torch.randn(4, 64), torch.randn(4, 64)
+    moe = m.layers[0].moe
+    with torch.no_grad():
+        assert torch.allclose(moe.serve(h, x), moe(h, x)[0], rtol=1e-5, atol=1e-6)
+    assert len(Generator(m, kv_format="bf16", max_batch=2, max_seq=64, weight_format="int8").generate_tokens(ids, max_new_tokens=3)[0]) == 3
+
+
 def test_int8_experts_are_their_values():
     """With experts alone in 8 bits a mixture says what the model with those values says: nothing else is rounded on the CPU."""
     m = mixture()

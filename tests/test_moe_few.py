@@ -218,6 +218,8 @@ def test_views():
     assert torch.equal(moe_ffn_few(**b)[0], y)
     b = dict(a, x=a["x"].view(3, 2, 2, 64), residual=a["residual"].view(3, 2, 2, 64))
     assert torch.equal(moe_ffn_few(**b)[0], y.view(3, 2, 2, 64))
+    b = dict(a, x=a["x"][5].expand(12, 64), residual=a["residual"][5].expand(12, 64))          # one row for all tokens
+    assert torch.equal(moe_ffn_few(**b)[0], y[5].expand(12, 64))
     b = dict(a, x=a["x"].t().contiguous().t(), router_w=a["router_w"].t().contiguous().t())
     assert torch.equal(moe_ffn_few(**b)[0], y)
 
