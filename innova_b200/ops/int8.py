@@ -56,7 +56,11 @@ class Int8Weight(NamedTuple):
 
 
 def refuse_gradients(what, *tensors):
-    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    grad = forward_ad._current_level >= 0
+    if torch.is_grad_enabled():
+        for t in tensors:
+            grad = grad or (t is not None and t.requires_grad)
+    if grad:
         raise RuntimeError(f"{what} serves: no gradient and no tangent passes through it (call it under torch.no_grad())")
 
 
@@ -140,7 +144,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
         y = F.linear(codes.q.double(), q.double()).float() * codes.scale.unsqueeze(-1) * sw
         y = y if bias is None else y + bias.float()
         return (F.silu(y[..., :cols]) * y[..., cols:] if gated else y).to(out_dtype)
-    out = torch.empty(*x.shape[:-1], cols, dtype=out_dtype, device=x.device)
+    out = x.new_empty((*x.shape[:-1], cols), dtype=out_dtype)
     rows, ld = _rows_of(x)
     T = rows.shape[0]
     if T == 0 or cols == 0 or K == 0:
@@ -151,8 +155,9 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
             from_x, from_codes, from_scale, ld_codes = rows.data_ptr(), 0, 0, 0
         elif codes is None:
             wide = (K + 15) // 16 * 16
-            work = torch.empty(T * (wide + 4), dtype=torch.uint8, device=x.device)
-            from_x, from_codes, from_scale, ld_codes = rows.data_ptr(), work.data_ptr(), work.data_ptr() + T * wide, wide
+            work = x.new_empty(T * (wide + 4), dtype=torch.uint8)
+            at = work.data_ptr()
+            from_x, from_codes, from_scale, ld_codes = rows.data_ptr(), at, at + T * wide, wide
         else:
             if rows.data_ptr() % 16 or ld % 16 or ld < K:
                 aligned = _empty_rows(rows.shape, x.device)

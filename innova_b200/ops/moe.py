@@ -241,33 +241,31 @@ def moe_few_supported(x, router_w, w_gate_up: Weight, w_down: Weight, top_k: int
             and (not x.is_cuda or x.dtype == torch.bfloat16 and D % grain == 0 and inner % grain == 0))
 
 
-def _few_plain_weight(w, shape, dev, dtype) -> bool:
-    return (isinstance(w, torch.Tensor) and w.shape == shape and w.dtype is dtype and w.get_device() == dev
-            and (dev < 0 or w.is_contiguous() and w.data_ptr() % 16 == 0))
-
-
-def _few_int8_weight(w, shape, dev) -> bool:
-    q, s = w
-    return (q.shape == shape and q.dtype is torch.int8 and s.shape == shape[:-1] and s.dtype is torch.float32 and q.get_device() == dev == s.get_device()
-            and s.is_contiguous() and (dev < 0 or q.is_contiguous() and q.data_ptr() % 16 == 0))
+def _few_weight(w, shape, dev, dtype, i8) -> bool:
+    q = w
+    if isinstance(w, Int8Weight):
+        q, s = w
+        if not (i8 and s.shape == shape[:-1] and s.dtype is torch.float32 and s.get_device() == dev and s.is_contiguous()):
+            return False
+        dtype = torch.int8
+    elif i8:
+        return False
+    return q.shape == shape and q.dtype is dtype and q.get_device() == dev and (dev < 0 or q.is_contiguous() and q.data_ptr() % 16 == 0)
 
 
 def _few_check(x, router_w, w_gu, w_down, residual, top_k, shared):
     """-> T, D, F, E, whether weights are in 8 bits. Asked in few expressions; what is wrong with arguments that fail is found by ``_few_refuse``."""
-    D, dev, dtype, i8 = x.shape[-1] if x.dim() else 0, x.get_device(), x.dtype, isinstance(w_down, Int8Weight)
-    T, down = x.numel() // max(1, D), w_down.q if i8 else w_down
-    if down.dim() == 3 and router_w.dim() == 2 and D > 0:
-        E, _, inner = down.shape
-        pairs = [(w_gu, (E, 2 * inner, D)), (w_down, (E, D, inner))]
-        if shared is not None and len(shared) == 2:
-            pairs += [(shared[0], (2 * inner, D)), (shared[1], (D, inner))]
+    shape, dev, dtype, i8 = x.shape, x.get_device(), x.dtype, isinstance(w_down, Int8Weight)
+    D, down = shape[-1] if shape else 0, w_down.q if i8 else w_down
+    if D > 0 and down.dim() == 3 and (shared is None or len(shared) == 2):
+        T, (E, _, inner) = x.numel() // D, down.shape
         grain = 16 if i8 else 8
-        if ((shared is None or len(shared) == 2) and router_w.shape == (E, D) and router_w.dtype is dtype and router_w.get_device() == dev
+        if (router_w.shape == (E, D) and router_w.dtype is dtype and router_w.get_device() == dev
                 and 1 <= top_k <= min(E, FEW_TOP) and E <= FEW_EXPERTS and T <= FEW_TOKENS
-                and (residual is None or residual.shape == x.shape and residual.dtype is dtype and residual.get_device() == dev)
+                and (residual is None or residual.shape == shape and residual.dtype is dtype and residual.get_device() == dev)
                 and (dtype is torch.bfloat16 or dtype is torch.float32 and dev < 0) and (dev < 0 or D % grain == 0 and inner % grain == 0 and inner > 0)
-                and all((isinstance(w, Int8Weight) and _few_int8_weight(w, s, dev)) if i8 else _few_plain_weight(w, s, dev, dtype)
-                        for w, s in pairs)):
+                and _few_weight(w_gu, (E, 2 * inner, D), dev, dtype, i8) and _few_weight(w_down, (E, D, inner), dev, dtype, i8)
+                and (shared is None or _few_weight(shared[0], (2 * inner, D), dev, dtype, i8) and _few_weight(shared[1], (D, inner), dev, dtype, i8))):
             return T, D, inner, E, i8
     _few_refuse(x, router_w, w_gu, w_down, residual, top_k, shared)
 
@@ -327,8 +325,7 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
     refuse_gradients("moe_ffn_few", x, router_w, residual, *(() if i8 else weights))
     if not x.is_cuda:
         return _few_plain(x.reshape(T, D), router_w, weights, residual, top_k, x.shape)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    counts = torch.empty(E, dtype=torch.int32, device=x.device)
+    out, counts = torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(E, dtype=torch.int32)
     if T == 0:
         return out, counts.zero_()
     with rt.device_of(x):
@@ -339,12 +336,11 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
         if not router_w.is_contiguous() or router_w.data_ptr() % 16:
             router_w = router_w.clone(memory_format=torch.contiguous_format)
         size = _few_bytes(T, D, inner, E, top_k, shared is not None, i8)
-        work = torch.empty(size, dtype=torch.uint8, device=x.device)
-        at = [w.q.data_ptr() if i8 else w.data_ptr() for w in weights]
-        scales = [w.scale.data_ptr() if i8 else 0 for w in weights]
+        work = x.new_empty(size, dtype=torch.uint8)
+        at = [w.q.data_ptr() for w in weights] if i8 else [w.data_ptr() for w in weights]
+        scales = [w.scale.data_ptr() for w in weights] if i8 else [0, 0, 0, 0]
         if shared is None:
-            at += [0, 0]
-            scales += [0, 0]
+            at, scales = [*at, 0, 0], [*scales[:2], 0, 0]
         rt.check(rt.lib().inv_moe_few(_FEW(rows.data_ptr(), router_w.data_ptr(), rt.ptr(res), *at[:2], *scales[:2], *at[2:], *scales[2:],
                                            out.data_ptr(), counts.data_ptr(), work.data_ptr(), rt.status_ptr(x), rt.stream_ptr(),
                                            T, D, inner, E, top_k, ldx, ldr, i8, size)), "inv_moe_few")
