@@ -192,7 +192,7 @@ template <int TB, bool I8>
 struct Shape {
   static constexpr int STEP = I8 ? 128 : 64, B_STAGE = (I8 ? 2 : 1) * TB * 128;
   static constexpr int PER_SM = I8 ? 1 : 2, ROOM = ((I8 ? 216 : 102) * 1024 - 1024) / (A_STAGE + B_STAGE), STAGES = ROOM < 12 ? ROOM : 12;
-  static constexpr int ACC = 4, CONV = 4, SETS = I8 ? 2 : 1;   // buffers of sums and of converted weights; sets of four warps of sums
+  static constexpr int ACC = 4, CONV = 4, SETS = I8 ? 2 : 1, SUM_AHEAD = I8 ? 2 : 4;   // buffers of sums and of converted weights; sets of four warps of sums
   // warps of weights, of products, of items, of tokens, of sums, of conversions
   static constexpr int SUMS = 4, CONVERT = SUMS + 4 * SETS, THREADS = 32 * (CONVERT + (I8 ? 4 * CONV : 0));
   static constexpr int SMEM = STAGES * (A_STAGE + B_STAGE) + 1024;
@@ -213,6 +213,9 @@ __device__ __forceinline__ void mf_widen(uint32_t v, uint32_t& lo, uint32_t& hi)
   const __nv_bfloat162 b = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m1), *reinterpret_cast<const __nv_bfloat162*>(&s1));
   lo = *reinterpret_cast<const uint32_t*>(&a);
   hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ void tmem_ld_32x1(uint32_t taddr, uint32_t& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
 }
 __device__ __forceinline__ int mf_acquire(const int* p) {
   int v;
@@ -260,6 +263,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
   __shared__ uint16_t s_index[MF_EXPERTS], s_expert[MF_EXPERTS + 1], s_first[MF_EXPERTS + 2], s_slot[MF_TOKENS * MF_TOP];
   __shared__ Item s_item[QUEUE];
   __shared__ float s_weight[MF_TOKENS * MF_TOP];
+  __shared__ uint8_t s_token[MF_TOKENS * (MF_TOP + 1)];          // of a slot
   __shared__ int s_n;
   __shared__ uint32_t tmem_slot;
   __shared__ int s_abort;
@@ -350,8 +354,11 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
   for (int i = tid; i < chosen; i += S::THREADS) {
     const int t = div_by(i, p.top_k, p.inv_k), e = s_slot[i];
     const int below = t < 32 ? __popc(s_mask[e][0] & ((1u << t) - 1)) : __popc(s_mask[e][0]) + __popc(s_mask[e][1] & ((1u << (t - 32)) - 1));
-    s_slot[i] = (uint16_t)(s_first[s_index[e]] + below);
+    const int slot = s_first[s_index[e]] + below;
+    s_slot[i] = (uint16_t)slot;
+    s_token[slot] = (uint8_t)t;
   }
+  if (p.shared && tid < p.T) s_token[chosen + tid] = (uint8_t)tid;
   __syncthreads();
 
   const int n_active = s_n, per_down = p.d_tiles * p.down_parts, n_gate = n_active * p.f_tiles, n_down = n_gate + n_active * per_down, n_items = n_down + p.d_tiles * ((p.T + MF_GROUP - 1) / MF_GROUP);
@@ -518,7 +525,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
       if (it.kind != SUM && ++next_acc == ACC) { next_acc = 0; next_accph ^= 1; }
       if (!mine) continue;
       if (it.kind == SUM) {
-        // eight lanes of a warp have 32 columns between them and add every fourth part; the four groups of lanes add up theirs
+        // eight lanes of a warp have 32 columns between them and add every fourth of a token's parts; the four groups of lanes add up theirs
         const int col = it.tile * MF_D + q * 32 + (lane & 7) * 4, t0 = it.part * MF_GROUP, mine_t = t0 + (lane >> 3);
         uint2 residual = make_uint2(0, 0);
         if (p.residual != nullptr && mine_t < p.T && col < p.D) residual = *reinterpret_cast<const uint2*>(p.residual + mine_t * p.ldr + col);
@@ -527,22 +534,17 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
         if (!__shfl_sync(0xffffffffu, there, 0)) break;
         float y[MF_GROUP][4] = {};
         if (col < p.D) {
-          for (int k = p.shared ? -1 : 0; k < p.top_k; ++k) {
-            float w[MF_GROUP];
-            const float* from[MF_GROUP];
+          const int terms = (p.top_k + p.shared) * p.down_parts;
+#pragma unroll S::SUM_AHEAD
+          for (int i = lane >> 3; i < terms; i += 4) {
+            const int k = div_by(i, p.down_parts, p.inv_down_parts), part = i - k * p.down_parts;
 #pragma unroll
             for (int j = 0; j < MF_GROUP; ++j) {
-              const int t = min(t0 + j, p.T - 1), c = t * p.top_k + max(k, 0);
-              w[j] = k < 0 ? 1.f : s_weight[c];
-              from[j] = p.sums + (long)(k < 0 ? chosen + t : s_slot[c]) * p.D + col;
+              const int t = min(t0 + j, p.T - 1), c = t * p.top_k + k;
+              const float w = k == p.top_k ? 1.f : s_weight[c];
+              const float4 u = __ldcg(reinterpret_cast<const float4*>(p.sums + ((long)part * p.slots + (k == p.top_k ? chosen + t : s_slot[c])) * p.D + col));
+              y[j][0] = fmaf(w, u.x, y[j][0]); y[j][1] = fmaf(w, u.y, y[j][1]); y[j][2] = fmaf(w, u.z, y[j][2]); y[j][3] = fmaf(w, u.w, y[j][3]);
             }
-#pragma unroll 2
-            for (int part = lane >> 3; part < p.down_parts; part += 4)
-#pragma unroll
-              for (int j = 0; j < MF_GROUP; ++j) {
-                const float4 u = __ldcg(reinterpret_cast<const float4*>(from[j] + (long)part * p.slots * p.D));
-                y[j][0] = fmaf(w[j], u.x, y[j][0]); y[j][1] = fmaf(w[j], u.y, y[j][1]); y[j][2] = fmaf(w[j], u.z, y[j][2]); y[j][3] = fmaf(w[j], u.w, y[j][3]);
-              }
           }
         }
 #pragma unroll
@@ -562,7 +564,6 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
       }
       const int e = it.e, first = it.first, n = s_first[it.a + 1] - first;
       const bool shared = e == p.E;
-      const uint64_t mask = (uint64_t)s_mask[e][1] << 32 | s_mask[e][0];
       // gate and up items: lanes of a warp hold eight columns of the gate, the same of the up product, and the next eight likewise
       const int f = it.tile * MF_F + q * 16 + (lane >> 4) * 8 + (lane & 7), col = it.tile * MF_D + row;
       float scale = 1.f;
@@ -570,30 +571,37 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
         if (it.kind == GATE) scale = f < p.F ? (shared ? p.shared_gate_up_scale : p.gate_up_scale + (long)e * 2 * p.F)[f + (lane >> 3 & 1) * p.F] : 0.f;
         else scale = col < p.D ? (shared ? p.shared_down_scale : p.down_scale + (long)e * p.D)[col] : 0.f;
       }
-      auto activate = [&](float v, int slot) {             // rounded to bf16, the type of the next product's operands
-        v *= scale;
-        const float up = __shfl_down_sync(0xffffffffu, v, 8);
-        if (!(lane & 8) && f < p.F) p.act[(long)slot * p.ld_act + f] = __float2bfloat16_rn(v / (1.f + expf(-v)) * up);
-      };
       if (!mbar_wait_warp(&acc_full[acc], accph, abort_flag, p.status, ERR_WAIT_TMEM_FULL)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + acc * TB + (uint32_t(q * 32) << 16);
-      float* to = p.sums + ((long)it.part * p.slots + first) * p.D + col;
-      int slot = 0;                                        // within the expert
+      if (it.kind == GATE) {
+        // Two tokens at a time: lanes with the gate take the first of them, those with the up product the second.
+        const bool second = lane & 8;
 #pragma unroll 1
-      for (int c = 0; c < TB; c += 16) {
-        const uint32_t bits = it.kind == GATE ? (uint32_t)(mask >> c) & 0xffffu : c + 16 <= n ? 0xffffu : c < n ? (1u << (n - c)) - 1 : 0u;
-        if (bits == 0) continue;
-        uint32_t r[16];
-        tmem_ld_32x16(taddr + c, r);
-        tmem_ld_wait();
+        for (int c = 0; c < n; c += 4) {
+          uint32_t r[4];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (!(bits >> j & 1)) continue;
-          const float v = __uint_as_float(r[j]);
-          if (it.kind == GATE) activate(v, first + slot);
-          else if (col < p.D) to[(long)slot * p.D] = v * scale;
-          ++slot;
+          for (int j = 0; j < 4; ++j) tmem_ld_32x1(taddr + s_token[first + min(c + j, n - 1)], r[j]);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const float u = __uint_as_float(r[j]) * scale, v = __uint_as_float(r[j + 1]) * scale, other = __shfl_xor_sync(0xffffffffu, second ? u : v, 8);
+            const float g = second ? other : u, up = second ? v : other;
+            const int slot = c + j + second;
+            // rounded to bf16, the type of the next product's operands
+            if (slot < n && f < p.F) p.act[(long)(first + slot) * p.ld_act + f] = __float2bfloat16_rn(g / (1.f + expf(-g)) * up);
+          }
+        }
+      } else {
+        float* to = p.sums + ((long)it.part * p.slots + first) * p.D + col;
+#pragma unroll 1
+        for (int c = 0; c < n; c += 16) {
+          uint32_t r[16];
+          tmem_ld_32x16(taddr + c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c + j < n && col < p.D) to[(long)(c + j) * p.D] = __uint_as_float(r[j]) * scale;
         }
       }
       tc_fence_before();
