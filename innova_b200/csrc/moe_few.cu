@@ -10,10 +10,11 @@
 //
 // The second kernel's work is a list of items: 128 weight rows of one expert's gate and up product (eight and eight in turn) by all of K; then 128 rows of its down
 // product by a part of K; then sums of 128 output columns for four tokens. CTAs draw items in order from a counter. Down items and sums wait for what they
-// read; that comes from items drawn earlier, by CTAs that run, so every wait ends, whatever else runs on the GPU. How K is cut depends on the layer's sizes alone, and
+// read; that comes from items drawn earlier, by CTAs that run, so every wait ends, whatever else runs on the GPU. An item is drawn when the one before it starts to load:
+// one further ahead, the last items were spread less evenly (4 tokens of 8 experts 72.3 us, 69.5 so). How K is cut depends on the layer's sizes alone, and
 // the parts are added in one order: a token's result depends on no order of arrival and on no other token. (Gate and up products in parts, added by
-// the warp that finished the last one, made the SMs more even and were slower, 145 us against 114 for 64 tokens of the 24-layer mixture: fences and counters take
-// microseconds in a loaded memory system.)
+// the warp that finished the last one, made the SMs more even and were slower, 145 us against 114 for 64 tokens of the 24-layer mixture when it was tried: fences and
+// counters take microseconds in a loaded memory system.)
 //
 // Weight rows are the 128-row operand of tcgen05 products, all tokens the other one, whichever experts they chose: columns that are not an expert's are computed
 // and not looked at, which costs nothing that counts (128 x 64 x 64 takes 200 cycles, its 16 KB of weights 700 from memory). Down products take an
@@ -205,14 +206,28 @@ struct __align__(16) Item {
 };
 }  // namespace mf
 
-// Four codes into bf16: 128 + (the lower seven bits), less 128, or 256 where the sign bit is set. Each is a number of eight bits, so nothing is rounded.
-__device__ __forceinline__ void mf_widen(uint32_t v, uint32_t& lo, uint32_t& hi) {
+// Four codes into bf16, in two ways; neither rounds anything. Selections and logic have half the rate of products: the first way is mostly those, the second mostly products,
+// and half the codes go each way (16 tokens of 8 experts of 2048 x 5632: 63.4 us; all the first way 66.5, all the second 64.5).
+// 128 + (the lower seven bits), less 128, or 256 where the sign bit is set.
+__device__ __forceinline__ void mf_widen_logic(uint32_t v, uint32_t& lo, uint32_t& hi) {
   const uint32_t m = v & 0x7f7f7f7fu, s = v & 0x80808080u, c = 0x43434343u;
   const uint32_t m0 = __byte_perm(m, c, 0x4140), m1 = __byte_perm(m, c, 0x4342), s0 = __byte_perm(s, c, 0x4140), s1 = __byte_perm(s, c, 0x4342);
   const __nv_bfloat162 a = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m0), *reinterpret_cast<const __nv_bfloat162*>(&s0));
   const __nv_bfloat162 b = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&m1), *reinterpret_cast<const __nv_bfloat162*>(&s1));
   lo = *reinterpret_cast<const uint32_t*>(&a);
   hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+// With the sign bit flipped, u = code + 128, the pattern 0x4300 | u is p = 256 + code (code < 0) or 256 + 2 code: code = t - max(t / 2, 0), t = p - 256.
+__device__ __forceinline__ uint32_t mf_widen_2(uint32_t p) {
+  const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&p);
+  const __nv_bfloat162 r = __hfma2_relu(v, __float2bfloat162_rn(0.5f), __float2bfloat162_rn(-128.f));
+  const __nv_bfloat162 w = __hsub2(__hadd2(v, __float2bfloat162_rn(-256.f)), r);
+  return *reinterpret_cast<const uint32_t*>(&w);
+}
+__device__ __forceinline__ void mf_widen_products(uint32_t v, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = v ^ 0x80808080u, c = 0x43434343u;
+  lo = mf_widen_2(__byte_perm(u, c, 0x4140));
+  hi = mf_widen_2(__byte_perm(u, c, 0x4342));
 }
 __device__ __forceinline__ void tmem_ld_32x1(uint32_t taddr, uint32_t& r) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
@@ -258,7 +273,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
   using S = Shape<TB, I8>;
   constexpr int STAGES = S::STAGES, B_STAGE = S::B_STAGE, STEP = S::STEP, ACC = S::ACC, CONV = S::CONV;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full_bar[STAGES], weights_bar[STAGES], empty_bar[STAGES], item_full[QUEUE], item_empty[QUEUE], acc_full[ACC], acc_empty[ACC], conv_full[CONV], conv_empty[CONV];
+  __shared__ uint64_t full_bar[STAGES], weights_bar[STAGES], empty_bar[STAGES], item_full[QUEUE], item_empty[QUEUE], acc_full[ACC], acc_empty[ACC], conv_full[CONV], conv_empty[CONV], taken;
   __shared__ uint32_t s_mask[MF_EXPERTS + 1][2];                 // tokens of an expert; E: of the shared one
   __shared__ uint16_t s_index[MF_EXPERTS], s_expert[MF_EXPERTS + 1], s_first[MF_EXPERTS + 2], s_slot[MF_TOKENS * MF_TOP];
   __shared__ Item s_item[QUEUE];
@@ -292,6 +307,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
       mbar_init(&conv_full[i], 4);
       mbar_init(&conv_empty[i], 1);
     }
+    mbar_init(&taken, 1);
     s_abort = 0;
     fence_barrier_init();
     tma_prefetch_desc(&map_gate);
@@ -322,43 +338,40 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
     s_mask[p.E][1] = p.T >= 64 ? 0xffffffffu : p.T > 32 ? (1u << (p.T - 32)) - 1 : 0u;
   }
   __syncthreads();
-  if (warp == 0) {
+  if (warp * 32 < p.E) {                           // a warp for 32 experts, which counts those before them as well
     int first = 0, active = 0;
-    for (int e0 = 0; e0 < p.E + p.shared; e0 += 32) {
-      const int e = e0 + lane, n = e < p.E + p.shared ? __popc(s_mask[e][0]) + __popc(s_mask[e][1]) : 0;
-      int sum = n;
+    for (int e = lane; e < warp * 32; e += 32) {
+      const int n = __popc(s_mask[e][0]) + __popc(s_mask[e][1]);
+      first += __reduce_add_sync(0xffffffffu, n);
+      active += __popc(__ballot_sync(0xffffffffu, n > 0));
+    }
+    const int e = warp * 32 + lane, n = e < p.E ? __popc(s_mask[e][0]) + __popc(s_mask[e][1]) : 0;
+    int sum = n;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-      }
-      const uint32_t has = __ballot_sync(0xffffffffu, n > 0);
-      const int a = active + __popc(has & ((1u << lane) - 1));
-      if (n > 0) {
-        s_expert[a] = (uint16_t)e;
-        s_first[a] = (uint16_t)(first + sum - n);
-      }
-      if (e < p.E) {
-        s_index[e] = (uint16_t)a;
-        if (blockIdx.x == 0) p.counts[e] = n;
-      }
-      first += __shfl_sync(0xffffffffu, sum, 31);
-      active += __popc(has);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += v;
     }
-    if (lane == 0) {
-      s_first[active] = (uint16_t)first;
-      s_n = active;
+    const uint32_t has = __ballot_sync(0xffffffffu, n > 0);
+    const int a = active + __popc(has & ((1u << lane) - 1));
+    if (n > 0) {
+      s_expert[a] = (uint16_t)e;
+      s_first[a] = (uint16_t)(first + sum - n);
+    }
+    if (e < p.E) {
+      s_index[e] = (uint16_t)a;
+      if (blockIdx.x == 0) p.counts[e] = n;
+    }
+    if (e == p.E - 1) {                            // behind them, the shared expert
+      const int all = active + __popc(has);
+      s_first[all] = (uint16_t)chosen;
+      if (p.shared) {
+        s_expert[all] = (uint16_t)p.E;
+        s_first[all + 1] = (uint16_t)(chosen + p.T);
+      }
+      s_n = all + p.shared;
     }
   }
-  __syncthreads();
-  for (int i = tid; i < chosen; i += S::THREADS) {
-    const int t = div_by(i, p.top_k, p.inv_k), e = s_slot[i];
-    const int below = t < 32 ? __popc(s_mask[e][0] & ((1u << t) - 1)) : __popc(s_mask[e][0]) + __popc(s_mask[e][1] & ((1u << (t - 32)) - 1));
-    const int slot = s_first[s_index[e]] + below;
-    s_slot[i] = (uint16_t)slot;
-    s_token[slot] = (uint8_t)t;
-  }
-  if (p.shared && tid < p.T) s_token[chosen + tid] = (uint8_t)tid;
   __syncthreads();
 
   const int n_active = s_n, per_down = p.d_tiles * p.down_parts, n_gate = n_active * p.f_tiles, n_down = n_gate + n_active * per_down, n_items = n_down + p.d_tiles * ((p.T + MF_GROUP - 1) / MF_GROUP);
@@ -369,9 +382,8 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
     // ---------------- items: drawn and described for the others ----------------
     if (lane == 0) {
       int qi = 0;
-      uint32_t qph = 1;
+      uint32_t qph = 1, tph = 0;
       while (true) {
-        const int next = ticket < n_items ? atomicAdd(p.counters, 1) : ticket;      // on its way while this one is described
         Item it;
         int i = ticket;
         it.a = it.e = it.first = it.k0 = it.steps = 0;
@@ -404,8 +416,9 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
         s_item[qi] = it;
         mbar_arrive(&item_full[qi]);
         if (++qi == QUEUE) { qi = 0; qph ^= 1; }
-        if (it.kind == END) break;
-        ticket = next;
+        if (it.kind == END || !mbar_wait(&taken, tph, abort_flag, p.status, ERR_WAIT_MISC)) break;
+        tph ^= 1;
+        ticket = atomicAdd(p.counters, 1);
       }
     }
   } else if (warp == 0) {
@@ -418,6 +431,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
         if (!mbar_wait(&item_full[qi], qph, abort_flag, p.status, ERR_WAIT_MISC)) break;
         const Item it = s_item[qi];
         mbar_arrive(&item_empty[qi]);
+        mbar_arrive(&taken);
         if (++qi == QUEUE) { qi = 0; qph ^= 1; }
         if (it.kind == END) break;
         if (it.kind == SUM) continue;
@@ -449,7 +463,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
         if (it.kind == SUM) continue;
         if (it.kind == DOWN && it.a > ready) {
           if (!mf_wait(&done[it.a], p.f_tiles * 4, abort_flag, p.status)) break;
-          mf_fence_proxy();
+          mf_fence_proxy();                          // activations were written by plain stores and are read by bulk copies
           ready = it.a;
         }
         const int row = it.kind == GATE ? 0 : it.first, end = (it.k0 + it.steps) * STEP;
@@ -509,6 +523,15 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
     // ---------------- sums: sets of four warps take items in turn ----------------
     const int q = warp & 3, row = q * 32 + lane;           // the lanes of tensor memory that this warp may read
     const int set = (warp - S::SUMS) >> 2;
+    for (int i = tid - S::SUMS * 32; i < chosen; i += 128 * S::SETS) {
+      const int t = div_by(i, p.top_k, p.inv_k), e = s_slot[i];
+      const int below = t < 32 ? __popc(s_mask[e][0] & ((1u << t) - 1)) : __popc(s_mask[e][0]) + __popc(s_mask[e][1] & ((1u << (t - 32)) - 1));
+      const int slot = s_first[s_index[e]] + below;
+      s_slot[i] = (uint16_t)slot;
+      s_token[slot] = (uint8_t)t;
+    }
+    if (p.shared && tid - S::SUMS * 32 < p.T) s_token[chosen + tid - S::SUMS * 32] = (uint8_t)(tid - S::SUMS * 32);
+    asm volatile("bar.sync 1, %0;" ::"r"(128 * S::SETS) : "memory");
     int qi = 0, turn = 0, next_acc = 0;
     uint32_t qph = 0, next_accph = 0;
     while (true) {
@@ -607,7 +630,6 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&acc_empty[acc]);
-      if (it.kind == GATE) mf_fence_proxy();               // activations are read by bulk copies
       __syncwarp();
       if (lane == 0) mf_release(it.kind == GATE ? &done[it.a] : &down_done[it.tile]);
     }
@@ -637,10 +659,10 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const uint4 v = *reinterpret_cast<const uint4*>(from + (((4 * h + c) ^ (row & 7)) << 4));
-              mf_widen(v.x, w[8 * c], w[8 * c + 1]);
-              mf_widen(v.y, w[8 * c + 2], w[8 * c + 3]);
-              mf_widen(v.z, w[8 * c + 4], w[8 * c + 5]);
-              mf_widen(v.w, w[8 * c + 6], w[8 * c + 7]);
+              mf_widen_logic(v.x, w[8 * c], w[8 * c + 1]);
+              mf_widen_products(v.y, w[8 * c + 2], w[8 * c + 3]);
+              mf_widen_logic(v.z, w[8 * c + 4], w[8 * c + 5]);
+              mf_widen_products(v.w, w[8 * c + 6], w[8 * c + 7]);
             }
             tmem_st_32x32(tmem_base + ACC * TB + cv * 64 + h * 32 + (uint32_t(q * 32) << 16), w);
           }

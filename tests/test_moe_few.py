@@ -263,3 +263,21 @@ def test_near_the_training_form():
         z, _, c = moe_ffn(a["x"], a["router_w"], a["w_gate_up"], a["w_down"], a["residual"], 2)
     assert torch.equal(counts, c)
     assert float((y.float() - z.float()).norm()) <= 4 * 2.0 ** -8 * float(z.float().norm())
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 17, 40])
+def test_every_code_is_widened_exactly(T):
+    # 256 columns hold each code once in every row. Codes are exact in bf16 and the scale is a power of two, so both forms add up the same terms, sixteen at a time.
+    D, F = 256, 64
+    g = torch.Generator().manual_seed(3)
+    codes = torch.stack([torch.arange(-128, 128).roll(37 * i) for i in range(2 * F)]).to(torch.int8)
+    down = torch.stack([torch.randperm(256, generator=g)[:F] - 128 for _ in range(D)]).to(torch.int8)
+    x = torch.randn(T, D, generator=g).to(BF)
+    out = []
+    for i8 in (True, False):
+        weights = [Int8Weight(q[None], torch.full((1, len(q)), 2.0 ** -6)) if i8 else (q[None].to(BF) * 2.0 ** -6) for q in (codes, down)]
+        a = to(dict(x=x, router_w=torch.zeros(1, D, dtype=BF), w_gate_up=weights[0], w_down=weights[1]), "cuda")
+        out.append(moe_ffn_few(**a, top_k=1)[0])
+    rt.check_status()
+    assert torch.equal(*out)
