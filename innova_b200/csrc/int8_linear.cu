@@ -6,7 +6,7 @@
 // The sums are whole numbers below 2^31 (K <= 133144), so their order changes nothing; scales and bias are applied in fp32 and the result is rounded once.
 //
 // int8_rows_kernel      rows of activations into codes and scales
-// int8_few_kernel       up to four rows, weights of up to 32 MB: codes and product in one launch, warp-level products
+// int8_few_kernel       one row, or up to four and weights of up to 32 MB: codes and product in one launch
 // int8_split_kernel     up to 128 rows, or results of few tiles: tcgen05 kind::i8, clusters that share K
 // int8_tile_kernel      the rest: tiles of 256 x 256 on CTA pairs, tcgen05 kind::i8
 #include "cta_pair.cuh"
@@ -214,7 +214,7 @@ struct Int8Few {
   const void* bias;
   void* out;
   long ldx, ldc, ldw, ldo;
-  int T, N, K, cols, tiles, pitch; // cols: output columns; pitch: between rows of codes in shared memory
+  int T, N, K, cols, per, tiles;   // cols: output columns; per: of a tile
   int x_f32, x_vec, bias_f32, out_f32;
 };
 
@@ -232,77 +232,66 @@ __device__ __forceinline__ float int8_bias(const void* b, int f32, int i) {
   return b == nullptr ? 0.f : f32 ? static_cast<const float*>(b)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(b)[i]);
 }
 // One launch: a CTA makes the codes of all rows for itself, in shared memory, while its first weights are on their way (every CTA reads x from L2, and with a kernel of
-// their own in front the codes cost 1.5 us on the device and 4 on the host). Weights go from memory straight into fragments, with none of a tile's set-up. A CTA
-// takes 32 weight rows at a time (gated: 16 of the gate and their 16 of the up product) as the 16-row operand, the activations as the other. Its eight warps
-// take every eighth slice of K, 128 bytes of a row, and meet in shared memory. Both operands read a lane's 32 consecutive bytes in the same order, which a sum over k does
-// not notice. The warp-level product of 8-bit integers is slow on this GPU, some 80 cycles an instruction and scheduler: sixteen rows took 27 us of 22016 x
-// 4096, 64 rows 110, where the tiles below take 20 and 22.
-constexpr int FEW_WARPS = 8, FEW_SLICE = 128, FEW_PL = 36, FEW_ROWS = 4, FEW_RING = 2, FEW_CODES = 88 * 1024;
+// their own in front the codes cost 1.5 us on the device and 4 on the host). Weights go from memory straight into registers and are multiplied there, with none of a
+// tile's set-up.
+//
+// int8_few_kernel, one and two rows: products of four codes a lane and instruction. A warp reads 512 bytes of four weight rows at a time. A tile's rows by the slices
+// of K are dealt out to the warps in equal runs, whose sums meet in shared memory, and tiles are as wide as spreads the weights over two CTAs an SM.
+// int8_few_mma_kernel, three and four rows: a CTA takes 32 weight rows at a time (gated: 16 of the gate and their 16 of the up product) as the 16-row operand of
+// warp-level matrix products, the activations as the other. Its eight warps take every eighth slice of K, 128 bytes of a row, and meet in shared memory. Both
+// operands read a lane's 32 consecutive bytes in the same order, which a sum over k does not notice.
+//
+// Neither kind of product is fast on this GPU: some 8 cycles a scheduler for 32 lanes' four codes, some 80 for 16 x 8 x 32. 6144 x 4096, us, in products of
+// codes and of matrices: one row 7.4, 8.7; two 8.7, 9.4; four 11.6, 10.2. Against codes in front and tcgen05 tiles: one row 12288 x 4096 11.4, 13.6, 22016 x 4096 17.4,
+// 18.8, 22016 x 11008 42.3, 42.8: any size. Two rows 12288 x 4096 12.5, 13.7, but 4096 x 11008 14.1, 12.9, four rows of the former 15.5, 13.8: weights of up to 32 MB.
+constexpr int FEW_WARPS = 8, FEW_ROWS = 4, FEW_SLICE = 512, FEW_RING = 4, FEW_CODES = 88 * 1024, FEW_WIDEST = 512;
+constexpr int MMA_SLICE = 128, MMA_PL = 36, MMA_RING = 2;
+static long few_room(long T, long K) { return T > 2 ? T * ((K + MMA_SLICE - 1) / MMA_SLICE * MMA_SLICE + 16) : T * ((K + FEW_SLICE - 1) / FEW_SLICE * FEW_SLICE); }
 
-template <bool GATED>
-__global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8Few p) {
-  extern __shared__ __align__(16) int8_t few_codes[];        // [T] rows of whole slices, pitch apart: 16 bytes off 128, so that eight lanes meet all banks
-  __shared__ int part[FEW_WARPS * 8 * FEW_PL];                // the product has eight rows of activations
-  __shared__ uint32_t tops[FEW_WARPS][FEW_ROWS];
-  __shared__ float scales[FEW_ROWS];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
-  const int slices = (p.K + FEW_SLICE - 1) / FEW_SLICE;
-  release_next();
-  uint4 ring[FEW_RING][4][2];
-  auto fetch = [&](int tile, int s, uint4 (&r)[4][2]) {
-    const int at = s * FEW_SLICE + tig * 32;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int row = GATED ? min(tile * 16 + (t & 1) * 8 + g, p.cols - 1) + (t >> 1) * p.cols : min(tile * 32 + t * 8 + g, p.N - 1);
-      const int8_t* from = p.q + (long)row * p.ldw + at;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) r[t][i] = at + 16 * i < p.K ? int8_stream(from + 16 * i) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  int tile = blockIdx.x;
-#pragma unroll
-  for (int u = 0; u < FEW_RING; ++u)
-    if (warp + u * FEW_WARPS < slices) fetch(tile, warp + u * FEW_WARPS, ring[u]);
-  const int eights = (p.K + 7) / 8, places = slices * (FEW_SLICE / 8);
+// Codes of all rows into shared memory, `pitch` apart, with zeros up to `width`, and their scales.
+template <int TT>
+__device__ __forceinline__ void int8_few_codes(const Int8Few& p, int8_t* few_codes, int pitch, int width, uint32_t (&tops)[FEW_WARPS][TT], float (&scales)[TT]) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int eights = (p.K + 7) / 8, places = width / 8;
   if (p.x != nullptr) {
     // all rows' loads of a place at once
     auto codes = [&](auto* x, auto vec) {
       using T = std::remove_const_t<std::remove_pointer_t<decltype(x)>>;
       using Eight = Int8Eight<T, decltype(vec)::value>;
-      uint32_t top[FEW_ROWS] = {};
+      uint32_t top[TT] = {};
       for (int i = tid; i < eights; i += FEW_WARPS * 32) {
-        Eight e[FEW_ROWS];
+        Eight e[TT];
 #pragma unroll
-        for (int t = 0; t < FEW_ROWS; ++t)
+        for (int t = 0; t < TT; ++t)
           if (t < p.T) e[t].load(x + t * p.ldx + i * 8, p.K - i * 8);
 #pragma unroll
-        for (int t = 0; t < FEW_ROWS; ++t)
+        for (int t = 0; t < TT; ++t)
           if (t < p.T) top[t] = e[t].largest(top[t]);
       }
 #pragma unroll
-      for (int t = 0; t < FEW_ROWS; ++t) {
+      for (int t = 0; t < TT; ++t) {
         top[t] = __reduce_max_sync(0xffffffffu, top[t]);
         if (lane == 0) tops[warp][t] = top[t];
       }
       __syncthreads();
-      float s[FEW_ROWS], inv[FEW_ROWS];
-      bool finite[FEW_ROWS];
+      float sx[TT], inv[TT];
+      bool finite[TT];
 #pragma unroll
-      for (int t = 0; t < FEW_ROWS; ++t) {
-        finite[t] = int8_scale(__reduce_max_sync(0xffffffffu, lane < FEW_WARPS ? tops[lane][t] : 0u), s[t], inv[t]);
-        if (tid == t) scales[t] = s[t];
+      for (int t = 0; t < TT; ++t) {
+        finite[t] = int8_scale(__reduce_max_sync(0xffffffffu, lane < FEW_WARPS ? tops[lane][t] : 0u), sx[t], inv[t]);
+        if (tid == t) scales[t] = sx[t];
       }
       for (int i = tid; i < places; i += FEW_WARPS * 32) {
-        Eight e[FEW_ROWS];
+        Eight e[TT];
 #pragma unroll
-        for (int t = 0; t < FEW_ROWS; ++t)
+        for (int t = 0; t < TT; ++t)
           if (t < p.T && i < eights) e[t].load(x + t * p.ldx + i * 8, p.K - i * 8);
 #pragma unroll
-        for (int t = 0; t < FEW_ROWS; ++t) {
+        for (int t = 0; t < TT; ++t) {
           if (t >= p.T) break;
           float2 v[4];
           e[t].values(v);
-          *reinterpret_cast<uint2*>(few_codes + t * p.pitch + i * 8) = i < eights && finite[t] ? int8_pack(v, s[t], inv[t]) : make_uint2(0u, 0u);
+          *reinterpret_cast<uint2*>(few_codes + t * pitch + i * 8) = i < eights && finite[t] ? int8_pack(v, sx[t], inv[t]) : make_uint2(0u, 0u);
         }
       }
     };
@@ -322,21 +311,154 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
         if (i * 8 + 8 <= p.K) v = *reinterpret_cast<const uint2*>(from);
         else
           for (int j = 0; i * 8 + j < p.K; ++j) (j < 4 ? v.x : v.y) |= ((uint32_t)from[j] & 255u) << (8 * (j % 4));
-        *reinterpret_cast<uint2*>(few_codes + t * p.pitch + i * 8) = v;
+        *reinterpret_cast<uint2*>(few_codes + t * pitch + i * 8) = v;
       }
   }
   __syncthreads();
-  const int8_t* x = few_codes + min(g, p.T - 1) * p.pitch + tig * 32;
-  for (; tile < p.tiles; tile += gridDim.x) {
-    int acc[2][4] = {};
-    for (int s0 = warp; s0 < slices; s0 += FEW_RING * FEW_WARPS) {
+}
+
+template <int TT, bool GATED>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8Few p) {
+  constexpr int UNIT = 4;                                    // rows that a warp takes a slice of at a time
+  extern __shared__ __align__(16) int8_t few_codes[];        // [T] rows of whole slices
+  __shared__ int part[TT * FEW_WIDEST];
+  __shared__ uint32_t tops[FEW_WARPS][TT];
+  __shared__ float scales[TT];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int slices = (p.K + FEW_SLICE - 1) / FEW_SLICE, pitch = slices * FEW_SLICE;
+  release_next();
+  for (int i = tid; i < TT * FEW_WIDEST; i += FEW_WARPS * 32) part[i] = 0;
+  uint4 ring[FEW_RING][UNIT];
+  int rows = 0, first = 0;                                   // of the tile; its first column
+  auto fetch = [&](int group, int s, uint4 (&r)[UNIT]) {
+#pragma unroll
+    for (int t = 0; t < UNIT; ++t) {
+      const int at = s * FEW_SLICE + lane * 16, i = group * UNIT + t, half = rows / 2;
+      const long row = GATED && i >= half ? first + i - half + p.cols : first + i;
+      r[t] = i < rows && at < p.K ? int8_stream(p.q + row * p.ldw + at) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  int tile = blockIdx.x, units = 0, unit = 0, end = 0, ahead = 0, group = 0, s = 0, next_group = 0, next_s = 0;
+  auto advance = [&](int& group, int& s) {
+    if (++s == slices) { s = 0; ++group; }
+  };
+  auto start = [&] {                                         // of a tile: this warp's run, and its first loads
+    first = tile * p.per;
+    rows = min(p.per, p.cols - first) * (GATED ? 2 : 1);
+    units = (rows + UNIT - 1) / UNIT * slices;
+    unit = ahead = units * warp / FEW_WARPS;
+    end = units * (warp + 1) / FEW_WARPS;
+    group = next_group = unit / slices;
+    s = next_s = unit - group * slices;
+#pragma unroll
+    for (int u = 0; u < FEW_RING; ++u) {
+      if (ahead == end) break;
+      fetch(next_group, next_s, ring[u]);
+      ++ahead;
+      advance(next_group, next_s);
+    }
+  };
+  start();
+  int8_few_codes<TT>(p, few_codes, pitch, pitch, tops, scales);
+  const int8_t* x = few_codes + lane * 16;
+  while (true) {
+    int acc[TT][UNIT] = {};
+    auto flush = [&] {                                       // whole numbers, in whatever order
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        int mine = 0;
+#pragma unroll
+        for (int r = 0; r < UNIT; ++r) {
+          const int all = __reduce_add_sync(0xffffffffu, acc[t][r]);
+          if (lane == r) mine = all;
+          acc[t][r] = 0;
+        }
+        if (lane < UNIT && group * UNIT + lane < rows) atomicAdd(&part[t * FEW_WIDEST + group * UNIT + lane], mine);
+      }
+    };
+    while (unit < end) {
 #pragma unroll
       for (int u = 0; u < FEW_RING; ++u) {
+        if (unit == end) break;
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          const uint4 b = *reinterpret_cast<const uint4*>(x + t * pitch + s * FEW_SLICE);
+#pragma unroll
+          for (int r = 0; r < UNIT; ++r) {
+            acc[t][r] = __dp4a((int)ring[u][r].x, (int)b.x, acc[t][r]);
+            acc[t][r] = __dp4a((int)ring[u][r].y, (int)b.y, acc[t][r]);
+            acc[t][r] = __dp4a((int)ring[u][r].z, (int)b.z, acc[t][r]);
+            acc[t][r] = __dp4a((int)ring[u][r].w, (int)b.w, acc[t][r]);
+          }
+        }
+        if (ahead < end) {
+          fetch(next_group, next_s, ring[u]);
+          ++ahead;
+          advance(next_group, next_s);
+        }
+        ++unit;
+        if (s + 1 == slices || unit == end) flush();
+        advance(group, s);
+      }
+    }
+    __syncthreads();
+    const int width = min(p.per, p.cols - first), now = first;
+    const bool more = tile + (int)gridDim.x < p.tiles;
+    if (more) {
+      tile += gridDim.x;
+      start();
+    }
+    for (int i = tid; i < width * TT; i += FEW_WARPS * 32) {
+      const int t = i / width, c = i - t * width, col = now + c;
+      const float sx = scales[t];
+      float y = fmaf((float)part[t * FEW_WIDEST + c] * sx, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
+      if (GATED) y = int8_silu(y) * fmaf((float)part[t * FEW_WIDEST + width + c] * sx, p.sw[p.cols + col], int8_bias(p.bias, p.bias_f32, p.cols + col));
+      if (p.out_f32) static_cast<float*>(p.out)[t * p.ldo + col] = y;
+      else static_cast<__nv_bfloat16*>(p.out)[t * p.ldo + col] = __float2bfloat16_rn(y);
+    }
+    if (!more) break;
+    __syncthreads();
+    for (int i = tid; i < TT * FEW_WIDEST; i += FEW_WARPS * 32) part[i] = 0;
+    __syncthreads();
+  }
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_mma_kernel(const Int8Few p) {
+  extern __shared__ __align__(16) int8_t few_codes[];        // [T] rows of whole slices, pitch apart: 16 bytes off 128, so that eight lanes meet all banks
+  __shared__ int part[FEW_WARPS * 8 * MMA_PL];                // the product has eight rows of activations
+  __shared__ uint32_t tops[FEW_WARPS][FEW_ROWS];
+  __shared__ float scales[FEW_ROWS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, tig = lane & 3;
+  const int slices = (p.K + MMA_SLICE - 1) / MMA_SLICE, pitch = slices * MMA_SLICE + 16;
+  release_next();
+  uint4 ring[MMA_RING][4][2];
+  auto fetch = [&](int tile, int s, uint4 (&r)[4][2]) {
+    const int at = s * MMA_SLICE + tig * 32;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = GATED ? min(tile * 16 + (t & 1) * 8 + g, p.cols - 1) + (t >> 1) * p.cols : min(tile * 32 + t * 8 + g, p.N - 1);
+      const int8_t* from = p.q + (long)row * p.ldw + at;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) r[t][i] = at + 16 * i < p.K ? int8_stream(from + 16 * i) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  int tile = blockIdx.x;
+#pragma unroll
+  for (int u = 0; u < MMA_RING; ++u)
+    if (warp + u * FEW_WARPS < slices) fetch(tile, warp + u * FEW_WARPS, ring[u]);
+  int8_few_codes<FEW_ROWS>(p, few_codes, pitch, slices * MMA_SLICE, tops, scales);
+  const int8_t* x = few_codes + min(g, p.T - 1) * pitch + tig * 32;
+  for (; tile < p.tiles; tile += gridDim.x) {
+    int acc[2][4] = {};
+    for (int s0 = warp; s0 < slices; s0 += MMA_RING * FEW_WARPS) {
+#pragma unroll
+      for (int u = 0; u < MMA_RING; ++u) {
         const int s = s0 + u * FEW_WARPS;
         if (s >= slices) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint4 b = *reinterpret_cast<const uint4*>(x + s * FEW_SLICE + 16 * i);
+          const uint4 b = *reinterpret_cast<const uint4*>(x + s * MMA_SLICE + 16 * i);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             const uint4 lo = ring[u][2 * m][i], hi = ring[u][2 * m + 1][i];
@@ -344,18 +466,18 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
             int8_mma(acc[m], lo.z, hi.z, lo.w, hi.w, b.z, b.w);
           }
         }
-        const int next = s + FEW_RING * FEW_WARPS;
+        const int next = s + MMA_RING * FEW_WARPS;
         if (next < slices) fetch(tile, next, ring[u]);
         else if (tile + (int)gridDim.x < p.tiles && warp + u * FEW_WARPS < slices) fetch(tile + gridDim.x, warp + u * FEW_WARPS, ring[u]);
       }
     }
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      int* to = part + (warp * 8 + 2 * tig) * FEW_PL + m * 16 + g;
+      int* to = part + (warp * 8 + 2 * tig) * MMA_PL + m * 16 + g;
       to[0] = acc[m][0];
-      to[FEW_PL] = acc[m][1];
+      to[MMA_PL] = acc[m][1];
       to[8] = acc[m][2];
-      to[FEW_PL + 8] = acc[m][3];
+      to[MMA_PL + 8] = acc[m][3];
     }
     __syncthreads();
     constexpr int COLS = GATED ? 16 : 32;
@@ -364,8 +486,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
       int a = 0, b = 0;
 #pragma unroll
       for (int w = 0; w < FEW_WARPS; ++w) {
-        a += part[(w * 8 + t) * FEW_PL + c];
-        if (GATED) b += part[(w * 8 + t) * FEW_PL + 16 + c];
+        a += part[(w * 8 + t) * MMA_PL + c];
+        if (GATED) b += part[(w * 8 + t) * MMA_PL + 16 + c];
       }
       const float s = scales[t];
       float y = fmaf((float)a * s, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
@@ -377,16 +499,22 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
   }
 }
 
-static int few_pitch(long K) { return (int)((K + FEW_SLICE - 1) / FEW_SLICE * FEW_SLICE + 16); }
-
-template <bool GATED>
+template <int TT, bool GATED>
 static int launch_int8_few(const Int8Call& c, int device, cudaStream_t st) {
+  constexpr bool MMA = TT > 2;
   static OncePerDevice once;
-  if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(int8_few_kernel<GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_CODES); })) return -e;
-  const int cols = (int)(GATED ? c.N / 2 : c.N), per = GATED ? 16 : 32, tiles = (cols + per - 1) / per;
-  const Int8Few p = {c.x, c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldx, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, cols, tiles, few_pitch(c.K),
+  const auto kernel = [] {
+    if constexpr (MMA) return int8_few_mma_kernel<GATED>;
+    else return int8_few_kernel<TT, GATED>;
+  }();
+  if (const int e = once.ask(device, [&] { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_CODES); })) return -e;
+  const int cols = (int)(GATED ? c.N / 2 : c.N), least = (MMA ? 32 : 4) / (GATED ? 2 : 1), most = MMA ? least : FEW_WIDEST / (GATED ? 2 : 1);
+  int per = (cols + 295) / 296;
+  per = per < least ? least : per > most ? most : per;
+  const int tiles = (cols + per - 1) / per;
+  const Int8Few p = {c.x, c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldx, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, cols, per, tiles,
                      (int)c.x_f32, int8_rows_vec(c), (int)c.bias_f32, (int)c.out_f32};
-  int8_few_kernel<GATED><<<tiles < 296 ? tiles : 296, FEW_WARPS * 32, c.T * p.pitch, st>>>(p);
+  kernel<<<tiles < 296 ? tiles : 296, FEW_WARPS * 32, few_room(c.T, c.K), st>>>(p);
   return -(int)cudaGetLastError();
 }
 
@@ -921,7 +1049,7 @@ static int launch_int8_tiles(const Int8Call& c, bool early, int device, cudaStre
 
 enum Int8Route { INT8_FEW, INT8_SPLIT, INT8_TILES };
 static Int8Route int8_route(const Int8Call& c) {
-  if (c.T <= FEW_ROWS && c.N * c.K <= (32l << 20) && c.T * few_pitch(c.K) <= FEW_CODES) return INT8_FEW;
+  if (c.T <= FEW_ROWS && (c.T == 1 || c.N * c.K <= (32l << 20)) && few_room(c.T, c.K) <= FEW_CODES) return INT8_FEW;
   const long tiles = (c.T + 127) / 128 * ((c.gated ? c.N / 2 + 63 : c.N + 127) / (c.gated ? 64 : 128));
   return c.T <= 128 || tiles <= 148 ? INT8_SPLIT : INT8_TILES;
 }
@@ -955,7 +1083,11 @@ extern "C" int inv_int8_linear(const void* call) {
   const bool early = c.x != nullptr;
   const Int8Route route = int8_route(c);
   if (route != INT8_FEW && (c.codes == nullptr || c.sx == nullptr)) return -ERR_BAD_ARG;
-  if (route == INT8_FEW) return c.gated ? launch_int8_few<true>(c, device, st) : launch_int8_few<false>(c, device, st);
+  if (route == INT8_FEW) {
+#define INV_FEW(TT) (c.gated ? launch_int8_few<TT, true>(c, device, st) : launch_int8_few<TT, false>(c, device, st))
+    return c.T == 1 ? INV_FEW(1) : c.T == 2 ? INV_FEW(2) : INV_FEW(4);
+#undef INV_FEW
+  }
   if (early)
     if (const int e = launch_int8_rows(c, st)) return e;
   if (route == INT8_SPLIT) {

@@ -289,3 +289,24 @@ def test_linear_streams_and_graphs():
     torch.cuda.synchronize()
     assert all(torch.equal(y, int8_linear(a, w[0])) for y, a in zip(ys, still))
     rt.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 2, 3, 4])
+def test_up_to_four_rows(T):
+    """Columns that do not fill the last CTA's share, slices of K that the warps share unevenly, more columns than one pass over the GPU takes."""
+    for i, (K, N) in enumerate([(511, 888), (513, 6146), (1030, 2050), (4100, 1186), (5632, 592), (48, 160002), (16, 320006)]):
+        product(T, K, N, (BF, F32)[i % 2], None, (None, F32, BF)[i % 3], False, i)
+        product(T, K, N, BF, F32, (BF, None)[i % 2], True, i + 20)
+    x, w = rows(4, 1030, BF).cuda(), weight(1200, 1030, device="cuda")
+    fine = int8_linear(x[:T], w)
+    assert torch.equal(int8_linear(quantize_rows(x[:T]), w), fine)
+    x[T - 1, 1029] = float("nan")
+    y = int8_linear(x[:T], w)
+    assert torch.isnan(y[-1]).all() and torch.equal(y[:-1], fine[:-1])
+
+
+@gpu
+def test_one_row_and_a_large_weight():
+    product(1, 4100, 9000, BF, None, BF, False)
+    product(1, 4100, 9000, BF, None, None, True)
