@@ -239,10 +239,10 @@ __device__ __forceinline__ float int8_bias(const void* b, int f32, int i) {
 // of K are dealt out to the warps in equal runs, whose sums meet in shared memory, and tiles are as wide as spreads the weights over two CTAs an SM.
 // int8_few_mma_kernel, three and four rows: a CTA takes 32 weight rows at a time (gated: 16 of the gate and their 16 of the up product) as the 16-row operand of
 // warp-level matrix products, the activations as the other. Its eight warps take every eighth slice of K, 128 bytes of a row, and meet in shared memory. Both
-// operands read a lane's 32 consecutive bytes in the same order, which a sum over k does not notice.
+// operands read a lane's bytes in the same order, which a sum over k does not notice.
 //
 // Neither kind of product is fast on this GPU: some 8 cycles a scheduler for 32 lanes' four codes, some 80 for 16 x 8 x 32. 6144 x 4096, us, in products of
-// codes and of matrices: one row 7.4, 8.7; two 8.7, 9.4; four 11.6, 10.2. Against codes in front and tcgen05 tiles: one row 12288 x 4096 11.4, 13.6, 22016 x 4096 17.4,
+// codes and of matrices: one row 7.4, 8.7; two 8.7, 9.4; four 11.6, 10.1. Against codes in front and tcgen05 tiles: one row 12288 x 4096 11.4, 13.6, 22016 x 4096 17.4,
 // 18.8, 22016 x 11008 42.3, 42.8: any size. Two rows 12288 x 4096 12.5, 13.7, but 4096 x 11008 14.1, 12.9, four rows of the former 15.5, 13.8: weights of up to 32 MB.
 constexpr int FEW_WARPS = 8, FEW_ROWS = 4, FEW_SLICE = 512, FEW_RING = 4, FEW_CODES = 88 * 1024, FEW_WIDEST = 512;
 constexpr int MMA_SLICE = 128, MMA_PL = 36, MMA_RING = 2;
@@ -434,13 +434,13 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_mma_kernel(const I
   release_next();
   uint4 ring[MMA_RING][4][2];
   auto fetch = [&](int tile, int s, uint4 (&r)[4][2]) {
-    const int at = s * MMA_SLICE + tig * 32;
+    const int at = s * MMA_SLICE + tig * 16;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const int row = GATED ? min(tile * 16 + (t & 1) * 8 + g, p.cols - 1) + (t >> 1) * p.cols : min(tile * 32 + t * 8 + g, p.N - 1);
       const int8_t* from = p.q + (long)row * p.ldw + at;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) r[t][i] = at + 16 * i < p.K ? int8_stream(from + 16 * i) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 2; ++i) r[t][i] = at + 64 * i < p.K ? int8_stream(from + 64 * i) : make_uint4(0, 0, 0, 0);
     }
   };
   int tile = blockIdx.x;
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_mma_kernel(const I
   for (int u = 0; u < MMA_RING; ++u)
     if (warp + u * FEW_WARPS < slices) fetch(tile, warp + u * FEW_WARPS, ring[u]);
   int8_few_codes<FEW_ROWS>(p, few_codes, pitch, slices * MMA_SLICE, tops, scales);
-  const int8_t* x = few_codes + min(g, p.T - 1) * pitch + tig * 32;
+  const int8_t* x = few_codes + min(g, p.T - 1) * pitch + tig * 16;
   for (; tile < p.tiles; tile += gridDim.x) {
     int acc[2][4] = {};
     for (int s0 = warp; s0 < slices; s0 += MMA_RING * FEW_WARPS) {
@@ -458,7 +458,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_mma_kernel(const I
         if (s >= slices) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const uint4 b = *reinterpret_cast<const uint4*>(x + s * MMA_SLICE + 16 * i);
+          const uint4 b = *reinterpret_cast<const uint4*>(x + s * MMA_SLICE + 64 * i);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
             const uint4 lo = ring[u][2 * m][i], hi = ring[u][2 * m + 1][i];
