@@ -126,27 +126,30 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
     if isinstance(x, Int8Rows):
         codes, x = x, x.q
     q, sw = w
-    dtype = x.dtype
+    dtype, shape, dev = x.dtype, x.shape, x.get_device()
     out_dtype = out_dtype or (_bf16 if codes is not None else dtype)
-    dev = x.get_device()
-    if not (q.dim() == 2 and q.dtype is _int8 and sw.dtype is _fp32 and sw.shape == q.shape[:1] and sw.is_contiguous() and x.dim() > 0
-            and x.shape[-1] == q.shape[1] and q.shape[1] <= MAX_K and dev == q.get_device() == sw.get_device()
-            and (codes is not None or dtype is _bf16 or dtype is _fp32) and (out_dtype is _bf16 or out_dtype is _fp32)
-            and (bias is None or bias.shape == sw.shape and (bias.dtype is _bf16 or bias.dtype is _fp32) and bias.get_device() == dev)
-            and (codes is None or dtype is _int8 and codes.scale.shape == x.shape[:-1] and codes.scale.dtype is _fp32 and codes.scale.get_device() == dev)
-            and (dev < 0 or q.stride(1) == 1 and q.stride(0) % 16 == 0 and q.stride(0) >= q.shape[1] and q.data_ptr() % 16 == 0)) or gated and q.shape[0] % 2:
+    N, K = q.shape if q.dim() == 2 else (0, -1)
+    ldw = K if K % 16 == 0 and q.is_contiguous() else q.stride(0) if K >= 0 and q.stride(1) == 1 else -1
+    if not (shape and shape[-1] == K <= MAX_K and q.dtype is _int8 and sw.dtype is _fp32 and sw.shape == (N,) and sw.is_contiguous()
+            and dev == q.get_device() == sw.get_device() and (codes is not None or dtype is _bf16 or dtype is _fp32) and (out_dtype is _bf16 or out_dtype is _fp32)
+            and (bias is None or bias.shape == (N,) and (bias.dtype is _bf16 or bias.dtype is _fp32) and bias.get_device() == dev)
+            and (codes is None or dtype is _int8 and codes.scale.shape == shape[:-1] and codes.scale.dtype is _fp32 and codes.scale.get_device() == dev)
+            and (dev < 0 or ldw % 16 == 0 and ldw >= K and q.data_ptr() % 16 == 0)) or gated and N % 2:
         _refuse(x, codes, w, bias, out_dtype, gated)
     refuse_gradients("int8_linear", x, bias)
-    N, K = q.shape
     cols = N // 2 if gated else N
     if dev < 0:
         codes = quantize_rows(x) if codes is None else codes
         y = F.linear(codes.q.double(), q.double()).float() * codes.scale.unsqueeze(-1) * sw
         y = y if bias is None else y + bias.float()
         return (F.silu(y[..., :cols]) * y[..., cols:] if gated else y).to(out_dtype)
-    out = x.new_empty((*x.shape[:-1], cols), dtype=out_dtype)
-    rows, ld = _rows_of(x)
-    T = rows.shape[0]
+    if len(shape) == 2 and x.is_contiguous():
+        rows, ld, T = x, K, shape[0]
+        out = x.new_empty((T, cols), dtype=out_dtype)
+    else:
+        out = x.new_empty((*shape[:-1], cols), dtype=out_dtype)
+        rows, ld = _rows_of(x)
+        T = rows.shape[0]
     if T == 0 or cols == 0 or K == 0:
         return _without_products(out, bias, cols, gated)
     with rt.device_of(x):
@@ -166,7 +169,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
             from_x, from_codes, from_scale, ld_codes = 0, rows.data_ptr(), scale.data_ptr(), ld
         bias = bias if bias is None else bias.contiguous()
         rt.check(rt.lib().inv_int8_linear(_CALL(from_x, q.data_ptr(), sw.data_ptr(), rt.ptr(bias), out.data_ptr(), from_codes, from_scale, rt.status_ptr(x),
-                                                rt.stream_ptr(), T, N, K, ld, q.stride(0), cols, ld_codes, dtype is _fp32, out_dtype is _fp32,
+                                                rt.stream_ptr(), T, N, K, ld, ldw, cols, ld_codes, dtype is _fp32, out_dtype is _fp32,
                                                 bias is not None and bias.dtype is _fp32, gated)), "inv_int8_linear")
         if codes is None and not alone:
             rt.count_launches(1)
