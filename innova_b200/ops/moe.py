@@ -321,10 +321,13 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
     every token goes to with weight one. The routing weights are the raw probabilities; ties go to the lowest expert. Sums are kept in fp32, the activations
     between the products rounded to bf16, the result once. A token's result depends on no other. No gradient and no tangent passes through it."""
     T, D, inner, E, i8 = _few_check(x, router_w, w_gate_up, w_down, residual, top_k, shared)
-    weights = (w_gate_up, w_down, *(shared or ()))
-    refuse_gradients("moe_ffn_few", x, router_w, residual, *(() if i8 else weights))
+    shared_up, shared_down = shared or (None, None)
+    if i8:
+        refuse_gradients("moe_ffn_few", x, router_w, residual)
+    else:
+        refuse_gradients("moe_ffn_few", x, router_w, residual, w_gate_up, w_down, shared_up, shared_down)
     if not x.is_cuda:
-        return _few_plain(x.reshape(T, D), router_w, weights, residual, top_k, x.shape)
+        return _few_plain(x.reshape(T, D), router_w, (w_gate_up, w_down, *(shared or ())), residual, top_k, x.shape)
     out, counts = torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(E, dtype=torch.int32)
     if T == 0:
         return out, counts.zero_()
@@ -337,11 +340,16 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
             router_w = router_w.clone(memory_format=torch.contiguous_format)
         size = _few_bytes(T, D, inner, E, top_k, shared is not None, i8)
         work = x.new_empty(size, dtype=torch.uint8)
-        at = [w.q.data_ptr() for w in weights] if i8 else [w.data_ptr() for w in weights]
-        scales = [w.scale.data_ptr() for w in weights] if i8 else [0, 0, 0, 0]
-        if shared is None:
-            at, scales = [*at, 0, 0], [*scales[:2], 0, 0]
-        rt.check(rt.lib().inv_moe_few(_FEW(rows.data_ptr(), router_w.data_ptr(), rt.ptr(res), *at[:2], *scales[:2], *at[2:], *scales[2:],
+        if i8:
+            w, w2, v, v2 = w_gate_up.q, w_down.q, w_gate_up.scale.data_ptr(), w_down.scale.data_ptr()
+        else:
+            w, w2, v, v2 = w_gate_up, w_down, 0, 0
+        s = s2 = u = u2 = 0
+        if shared is not None and i8:
+            s, s2, u, u2 = shared_up.q.data_ptr(), shared_down.q.data_ptr(), shared_up.scale.data_ptr(), shared_down.scale.data_ptr()
+        elif shared is not None:
+            s, s2 = shared_up.data_ptr(), shared_down.data_ptr()
+        rt.check(rt.lib().inv_moe_few(_FEW(rows.data_ptr(), router_w.data_ptr(), rt.ptr(res), w.data_ptr(), w2.data_ptr(), v, v2, s, s2, u, u2,
                                            out.data_ptr(), counts.data_ptr(), work.data_ptr(), rt.status_ptr(x), rt.stream_ptr(),
                                            T, D, inner, E, top_k, ldx, ldr, i8, size)), "inv_moe_few")
         rt.count_launches(1)
