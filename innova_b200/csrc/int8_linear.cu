@@ -520,7 +520,9 @@ static int launch_int8_few(const Int8Call& c, int device, cudaStream_t st) {
 
 // ---------------------------------------------------------------------------------------------- few tiles
 // Weight rows are the 128-row operand and TB activations the other one (tcgen05 kind::i8 on one SM), so that few activations fill an instruction. A cluster of up
-// to eight CTAs shares a tile: each has a part of K, leaves its sums in its shared memory and adds up its share of the tile's results from all of them.
+// to four CTAs shares a tile: each has a part of K, leaves its sums in its shared memory and adds up its share of the tile's results from all of them (sums that met in
+// global memory through atomics took 53 to 250 us of 64 x 4096 x 11008). Weight bytes bound it, but for its start and end: with the codes in front 16 rows of a gated
+// 22016 x 4096 take 19.9 us, 4.6 TB/s, 64 rows of 4096 x 11008 14.7, 3.1 TB/s (the codes 2.6 us of them, the cluster's join 1.5).
 namespace i8s {
 constexpr int THREADS = 192, BK = 128, A_STAGE = 128 * BK;  // warp 0 loads, warp 1 products, warps 2 to 5 sums
 constexpr int MAX_STAGES = 12, REST = 1024 + 256;
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(i8s::THREADS, 2)
     for (int t = rank + p.parts * (warp * SUB + (GATED ? lane >> 4 : 0)); t < left; t += p.parts * (THREADS / 32) * SUB) {
       int v[SUB][4] = {};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4; ++j) {
         if (j >= p.parts) break;
         const uint32_t there = mapa_shared(base + t * 512, j);
 #pragma unroll
@@ -803,7 +805,8 @@ struct Int8Tiles {
 };
 
 // The pair protocol of the bf16 product (csrc/gemm_tcgen05_2cta.cu). GATED: the leader's half of the weights' rows are of the gate, the other CTA's of the up
-// product, so a CTA finds both in its tensor memory.
+// product, so a CTA finds both in its tensor memory. Many tiles are bound by the tensor cores, 88 % of whose cycles are busy: 8192 x 4096 x 22016 gated 478 us alone
+// (3.1 POP/s), 600 with its codes call after call (2.5, the power limit). Few tiles by the last round of tiles: 2048 x 11008 x 4096 has 128 of them on 74 pairs, 34 us.
 template <bool GATED, bool F32>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
     int8_tile_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ CUtensorMap tmap_c,

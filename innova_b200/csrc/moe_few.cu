@@ -3,7 +3,10 @@
 //   p = softmax(R x);  y_t = r_t + [shared expert] + sum over the top_k largest p_te of p_te W2_e (silu(W1g_e x_t) * (W1u_e x_t))
 //
 // Such a layer reads every expert that some token goes to once and does little arithmetic, so weight bytes bound it. The training form (csrc/moe.cu) pads
-// every expert to 128 rows and takes seven launches.
+// every expert to 128 rows and takes seven launches. Device times with 8 experts of 2048 x 5632, two for a token (in brackets the weights' bytes at 6.54 TB/s): 1 token 38 us
+// (21), 4 tokens 69 (58), 16 tokens 92 (84), 64 tokens 102 (85), in 8 bits 31 (11), 50, 65 (42), 80 (43); 7 tokens, 6 of 64 experts of 1024 x 704 and a shared one 38 us
+// (22). While it streams the second kernel reads 6.4 to 7 TB/s; the rest is the router with the launch behind it, 5 us, the fall from gate to down products, 3 to 5, and
+// the sums with the end, 4. In 8 bits the conversions take two thirds of all issue slots.
 //
 // moe_few_router_kernel   a CTA a token: logits, softmax, the largest entries; clears the counters of the next kernel
 // moe_few_kernel          gate and up products, down products and their sum, one CTA an SM, without a launch between them
