@@ -310,3 +310,19 @@ def test_up_to_four_rows(T):
 def test_one_row_and_a_large_weight():
     product(1, 4100, 9000, BF, None, BF, False)
     product(1, 4100, 9000, BF, None, None, True)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 2, 4, 64, 300])
+def test_weights_beyond_two_to_the_31(T):
+    N, K = 66000, 32768
+    w = Int8Weight(torch.randint(-127, 128, (N, K), dtype=torch.int8, device="cuda"), torch.rand(N, device="cuda") / 1000)
+    x = rows(T, K, BF).cuda()
+    y = int8_linear(x, w)
+    g = int8_linear(x, w, gated=True)
+    for a, b in ((0, 200), (N - 300, N)):                      # results are exact up to one rounding, however the rows are cut
+        assert torch.equal(y[:, a:b], int8_linear(x, Int8Weight(w.q[a:b], w.scale[a:b])))
+    half = N // 2
+    few = Int8Weight(torch.cat([w.q[half - 100:half], w.q[N - 100:]]), torch.cat([w.scale[half - 100:half], w.scale[N - 100:]]))
+    assert torch.equal(g[:, half - 100:], int8_linear(x, few, gated=True))
+    rt.check_status()

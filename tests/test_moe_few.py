@@ -281,3 +281,21 @@ def test_every_code_is_widened_exactly(T):
         out.append(moe_ffn_few(**a, top_k=1)[0])
     rt.check_status()
     assert torch.equal(*out)
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 40])
+def test_experts_beyond_two_to_the_31(T):
+    """The last two of 72 experts, by themselves and behind the others: probabilities of the others are 0."""
+    E, D, F = 72, 4096, 4096
+    g = torch.Generator("cuda").manual_seed(1)
+    w = [Int8Weight(torch.randint(-127, 128, s, dtype=torch.int8, device="cuda", generator=g), torch.rand(s[:2], device="cuda", generator=g) * 1e-3)
+         for s in ((E, 2 * F, D), (E, D, F))]
+    x = torch.randn(T, D, device="cuda", generator=g).to(BF)
+    x[:, 0] = 8.0
+    router = torch.randn(E, D, device="cuda", generator=g).to(BF) * 0.02
+    router[:E - 2, 0], router[E - 2:, 0] = -60.0, 0.0
+    y, counts = moe_ffn_few(x, router, *w)
+    z, _ = moe_ffn_few(x, router[E - 2:], *(Int8Weight(v.q[E - 2:], v.scale[E - 2:]) for v in w))
+    assert counts.tolist() == [0] * (E - 2) + [T, T] and torch.equal(y, z)
+    rt.check_status()
