@@ -13,8 +13,9 @@
 //
 // The second kernel's work is a list of items: 128 weight rows of one expert's gate and up product (eight and eight in turn) by all of K; then 128 rows of its down
 // product by a part of K; then sums of 128 output columns for four tokens. CTAs draw items in order from a counter. Down items and sums wait for what they
-// read; that comes from items drawn earlier, by CTAs that run, so every wait ends, whatever else runs on the GPU. An item is drawn when the one before it starts to load:
-// one further ahead, the last items were spread less evenly (4 tokens of 8 experts 72.3 us, 69.5 so). How K is cut depends on the layer's sizes alone, and
+// read; that comes from items drawn earlier, by CTAs that have all they need: a CTA draws its first item once it holds its tensor memory, for which it may have to wait
+// for another stream's kernel on its SM. So every wait ends, whatever else runs on the GPU. An item is drawn when the one before it starts to load: one further ahead, the
+// last items were spread less evenly (4 tokens of 8 experts 72.3 us, 69.5 so). How K is cut depends on the layer's sizes alone, and
 // the parts are added in one order: a token's result depends on no order of arrival and on no other token. (Gate and up products in parts, added by
 // the warp that finished the last one, made the SMs more even and were slower, 145 us against 114 for 64 tokens of the 24-layer mixture when it was tried: fences and
 // counters take microseconds in a loaded memory system.)
@@ -291,7 +292,6 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
   uint8_t* sB = smem + STAGES * A_STAGE;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, chosen = p.T * p.top_k;
 
-  release_next();
   if (tid == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&full_bar[i], I8 ? 1 : 2);       // tokens, and weights where nothing converts them
@@ -322,12 +322,13 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
   }
   for (int i = tid; i < 2 * (MF_EXPERTS + 1); i += S::THREADS) (&s_mask[0][0])[i] = 0;
   tc_fence_before();
-  wait_previous();
-  int ticket = 0;
-  if (warp == 2 && lane == 0) ticket = atomicAdd(p.counters, 1);
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
+  release_next();                                  // with tensor memory in hand: a kernel that starts early and takes some waits for this one's end
+  wait_previous();
+  int ticket = 0;
+  if (warp == 2 && lane == 0) ticket = atomicAdd(p.counters, 1);
 
   // Who goes where: the tokens of each expert, the experts that are met, and a slot for each choice, in the order of experts and of tokens within one.
   for (int i = tid; i < chosen; i += S::THREADS) {

@@ -299,3 +299,26 @@ def test_experts_beyond_two_to_the_31(T):
     z, _ = moe_ffn_few(x, router[E - 2:], *(Int8Weight(v.q[E - 2:], v.scale[E - 2:]) for v in w))
     assert counts.tolist() == [0] * (E - 2) + [T, T] and torch.equal(y, z)
     rt.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("i8", [False, True])
+def test_beside_products_that_hold_tensor_memory(i8):
+    """Products whose clusters fit on an SM beside a CTA of the layer, on another stream: each side may find the tensor memory taken, and both end."""
+    from innova_b200.ops.int8 import int8_linear
+    a = to(inputs(40, 512, 256, 16, i8), "cuda")
+    g = torch.Generator().manual_seed(4)
+    w = Int8Weight(torch.randint(-127, 128, (4096, 512), dtype=torch.int8, generator=g).cuda(), torch.full((4096,), 1e-3).cuda())
+    h = torch.randn(9, 512, generator=g).to(BF).cuda()
+    want, other = moe_ffn_few(**a, top_k=4)[0], int8_linear(h, w)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(100):
+        with torch.cuda.stream(streams[0]):
+            got[0].append(moe_ffn_few(**a, top_k=4)[0])
+        with torch.cuda.stream(streams[1]):
+            got[1] += [int8_linear(h, w) for _ in range(3)]
+    torch.cuda.synchronize()
+    rt.check_status()
+    assert all(torch.equal(y, want) for y in got[0]) and all(torch.equal(y, other) for y in got[1])
