@@ -559,6 +559,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
         bool there = true;
         if (lane == 0) there = mf_wait(&down_done[it.tile], n_active * p.down_parts * 4, abort_flag, p.status);
         if (!__shfl_sync(0xffffffffu, there, 0)) break;
+        __syncwarp();                              // what lane 0 acquired is the other lanes' too; a shuffle orders no memory
         float y[MF_GROUP][4] = {};
         if (col < p.D) {
           const int terms = (p.top_k + p.shared) * p.down_parts;
@@ -607,6 +608,7 @@ __global__ void __launch_bounds__(mf::Shape<TB, I8>::THREADS, mf::Shape<TB, I8>:
 #pragma unroll 1
         for (int c = 0; c < n; c += 4) {
           uint32_t r[4];
+          __syncwarp();                            // the stores below part the lanes, the loads want the whole warp
 #pragma unroll
           for (int j = 0; j < 4; ++j) tmem_ld_32x1(taddr + s_token[first + min(c + j, n - 1)], r[j]);
           tmem_ld_wait();
