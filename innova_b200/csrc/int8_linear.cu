@@ -527,7 +527,13 @@ namespace i8s {
 constexpr int THREADS = 192, BK = 128, A_STAGE = 128 * BK;  // warp 0 loads, warp 1 products, warps 2 to 5 sums
 constexpr int MAX_STAGES = 12, REST = 1024 + 256;
 constexpr int stages(int tb, int ctas) { return (227 * 1024 / ctas - 1024 * (ctas - 1) - REST - 4 * tb) / (A_STAGE + tb * BK); }    // with so many CTAs an SM
-constexpr int smem_bytes(int tb, int n) { return n * (A_STAGE + tb * BK) + REST + 4 * tb; }
+// At least 48 KB: a CTA of fewer would fit on an SM beside one of a pair that holds all tensor memory (int8_tile_kernel leaves 25 KB, other pairs less). On two streams
+// a cluster could then hold what the pair's other CTA wants, and the pair what the cluster's.
+constexpr int LEAST = 48 * 1024;
+constexpr int smem_bytes(int tb, int n) {
+  const int bytes = n * (A_STAGE + tb * BK) + REST + 4 * tb;
+  return bytes < LEAST ? LEAST : bytes;
+}
 }  // namespace i8s
 
 struct Int8Split {
@@ -582,7 +588,6 @@ __global__ void __launch_bounds__(i8s::THREADS, 2)
   const int ct = div_by(tile, p.t_tiles, p.inv_t), t0 = (tile - ct * p.t_tiles) * TB, left = min(TB, p.T - t0), n0 = ct * COLS;
   const int k0 = rank * p.kb / p.parts, steps = (rank + 1) * p.kb / p.parts - k0;
 
-  release_next();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -600,6 +605,7 @@ __global__ void __launch_bounds__(i8s::THREADS, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  release_next();                                          // with tensor memory in hand: a kernel that starts early and takes some waits for this one's end
 
   if (warp == 0) {
     if (elect_one_sync()) {
@@ -834,7 +840,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
   const int pair = (int)blockIdx.x >> 1, npairs = (int)gridDim.x >> 1;
   const int kb_total = (p.K + BK - 1) / BK, total = p.m_tiles * p.n_tiles;
 
-  release_next();
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
@@ -859,6 +864,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  release_next();                             // as above
   wait_previous();
 
   if (warp == 0) {

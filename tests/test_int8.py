@@ -326,3 +326,22 @@ def test_weights_beyond_two_to_the_31(T):
     few = Int8Weight(torch.cat([w.q[half - 100:half], w.q[N - 100:]]), torch.cat([w.scale[half - 100:half], w.scale[N - 100:]]))
     assert torch.equal(g[:, half - 100:], int8_linear(x, few, gated=True))
     rt.check_status()
+
+
+@gpu
+def test_clusters_beside_pairs():
+    """Small clusters on one stream and tiles of CTA pairs on another: neither waits for tensor memory that the other holds."""
+    few, many = rows(9, 128, BF).cuda(), rows(3000, 200, BF).cuda()
+    w, v = weight(4096, 128, device="cuda"), weight(2050, 200, device="cuda")
+    want = int8_linear(few, w), int8_linear(many, v)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(50):
+        with torch.cuda.stream(streams[0]):
+            got[0] += [int8_linear(few, w) for _ in range(4)]
+        with torch.cuda.stream(streams[1]):
+            got[1].append(int8_linear(many, v))
+    torch.cuda.synchronize()
+    rt.check_status()
+    assert all(torch.equal(y, want[i]) for i in (0, 1) for y in got[i])
