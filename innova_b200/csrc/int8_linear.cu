@@ -30,6 +30,97 @@ struct Int8Call {
   int64_t T, N, K, ldx, ldw, ldo, ldc, x_f32, out_f32, bias_f32, gated;
 };
 
+// ---------------------------------------------------------------------------------------------- plans
+constexpr int FEW_WARPS = 8, FEW_ROWS = 4, FEW_SLICE = 512, FEW_RING = 4, FEW_CODES = 88 * 1024, FEW_WIDEST = 512;
+constexpr int MMA_SLICE = 128, MMA_PL = 36, MMA_RING = 2;
+static long few_room(long T, long K) { return T > 2 ? T * ((K + MMA_SLICE - 1) / MMA_SLICE * MMA_SLICE + 16) : T * ((K + FEW_SLICE - 1) / FEW_SLICE * FEW_SLICE); }
+
+namespace i8s {
+constexpr int THREADS = 192, BK = 128, A_STAGE = 128 * BK;  // warp 0 loads, warp 1 products, warps 2 to 5 sums
+constexpr int MAX_STAGES = 12, REST = 1024 + 256;
+constexpr int stages(int tb, int ctas) { return (227 * 1024 / ctas - 1024 * (ctas - 1) - REST - 4 * tb) / (A_STAGE + tb * BK); }    // with so many CTAs an SM
+// At least 48 KB: a CTA of fewer would fit on an SM beside one of a pair that holds all tensor memory (int8_tile_kernel leaves 25 KB, other pairs less). On two streams
+// a cluster could then hold what the pair's other CTA wants, and the pair what the cluster's.
+constexpr int LEAST = 48 * 1024;
+constexpr int smem_bytes(int tb, int n) {
+  const int bytes = n * (A_STAGE + tb * BK) + REST + 4 * tb;
+  return bytes < LEAST ? LEAST : bytes;
+}
+}  // namespace i8s
+namespace i8t {
+constexpr int BM = 256, BN = 256, BK = 128, STAGES = 5;    // BK in bytes: a swizzled row
+constexpr int A_STAGE = 128 * BK, B_STAGE = 128 * BK;      // of one CTA
+constexpr int THREADS = 320;                               // warp 0 loads, warp 1 products, warps 2 to 9 results
+constexpr int STAGING = 8 * 4096;                          // a box of 32 rows x 128 bytes a warp
+constexpr int TABLE = 8 * 2 * 128 * 4;                     // scales and biases of a warp's 128 columns of a tile
+constexpr int SMEM_BYTES = STAGES * (A_STAGE + B_STAGE) + STAGING + TABLE + 1024 + 256;
+constexpr int TMEM_COLS = 512;
+// 8-bit signed operands, 32-bit whole sums, both operands K-major
+constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((BM >> 4) << 24);
+}  // namespace i8t
+
+// How a product is cut and launched, from its sizes alone.
+enum Int8Route { INT8_FEW, INT8_SPLIT, INT8_TILES };
+struct Int8Plan {
+  int route, cols, grid, cluster, threads, smem;
+  int tiles, t_tiles, tb, per, kb, parts, stages;   // tiles in all and along the rows; rows and columns of one; steps of K, parts of it, stages of a ring
+};
+static Int8Route int8_route(long T, long N, long K, bool gated) {
+  if (T <= FEW_ROWS && (T == 1 || N * K <= (32l << 20)) && few_room(T, K) <= FEW_CODES) return INT8_FEW;
+  const long tiles = (T + 127) / 128 * ((gated ? N / 2 + 63 : N + 127) / (gated ? 64 : 128));
+  return T <= 128 || tiles <= 148 ? INT8_SPLIT : INT8_TILES;
+}
+static Int8Plan int8_plan(long T, long N, long K, bool gated) {
+  Int8Plan n = {};
+  n.route = int8_route(T, N, K, gated);
+  n.cols = (int)(gated ? N / 2 : N);
+  n.cluster = n.parts = 1;
+  if (n.route == INT8_FEW) {
+    const int least = (T > 2 ? 32 : 4) / (gated ? 2 : 1), most = T > 2 ? least : FEW_WIDEST / (gated ? 2 : 1), even = (n.cols + 295) / 296;
+    n.tb = (int)T;
+    n.per = even < least ? least : even > most ? most : even;
+    n.t_tiles = 1;
+    n.tiles = (n.cols + n.per - 1) / n.per;
+    n.grid = n.tiles < 296 ? n.tiles : 296;
+    n.threads = FEW_WARPS * 32;
+    n.smem = (int)few_room(T, K);
+  } else if (n.route == INT8_SPLIT) {
+    using namespace i8s;
+    n.per = gated ? 64 : 128;
+    const int col_tiles = (n.cols + n.per - 1) / n.per;
+    n.tb = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+    if (T > 64)
+      while (n.tb > 32 && (T + n.tb - 1) / n.tb * col_tiles < 100) n.tb /= 2;
+    n.kb = (int)((K + BK - 1) / BK);
+    n.t_tiles = (int)((T + n.tb - 1) / n.tb);
+    n.tiles = col_tiles * n.t_tiles;
+    auto fit = [&](int ctas) { const int k = ctas / n.tiles; return k < 1 ? 1 : k > 4 ? 4 : k; };
+    int parts = fit(128);
+    if (parts * n.tiles < 112) parts = fit(256);
+    n.parts = n.cluster = parts > n.kb ? n.kb : parts;
+    const int per_sm = n.tiles * n.parts <= 128 ? 1 : 2, most = stages(n.tb, per_sm), steps = (n.kb + n.parts - 1) / n.parts, stage = A_STAGE + n.tb * BK;
+    n.stages = most < steps ? most : steps;
+    if (n.stages > MAX_STAGES) n.stages = MAX_STAGES;
+    if (n.stages * stage < n.tb * 512) n.stages = (n.tb * 512 + stage - 1) / stage;   // the sums take their place
+    n.grid = n.tiles * n.parts;
+    n.threads = THREADS;
+    n.smem = smem_bytes(n.tb, n.stages);
+  } else {
+    using namespace i8t;
+    n.tb = BM;
+    n.per = gated ? BN / 2 : BN;
+    n.kb = (int)((K + BK - 1) / BK);
+    n.t_tiles = (int)((T + BM - 1) / BM);
+    n.tiles = (n.cols + n.per - 1) / n.per * n.t_tiles;
+    n.stages = STAGES;
+    n.cluster = 2;
+    n.grid = 2 * (n.tiles < 74 ? n.tiles : 74);
+    n.threads = THREADS;
+    n.smem = SMEM_BYTES;
+  }
+  return n;
+}
+
 // ---------------------------------------------------------------------------------------------- rows into codes
 constexpr float INT8_LEAST = 1e-10f;
 
@@ -244,9 +335,6 @@ __device__ __forceinline__ float int8_bias(const void* b, int f32, int i) {
 // Neither kind of product is fast on this GPU: some 8 cycles a scheduler for 32 lanes' four codes, some 80 for 16 x 8 x 32. 6144 x 4096, us, in products of
 // codes and of matrices: one row 7.4, 8.7; two 8.7, 9.4; four 11.6, 10.1. Against codes in front and tcgen05 tiles: one row 12288 x 4096 11.4, 13.6, 22016 x 4096 17.4,
 // 18.8, 22016 x 11008 42.3, 42.8: any size. Two rows 12288 x 4096 12.5, 13.7, but 4096 x 11008 14.1, 12.9, four rows of the former 15.5, 13.8: weights of up to 32 MB.
-constexpr int FEW_WARPS = 8, FEW_ROWS = 4, FEW_SLICE = 512, FEW_RING = 4, FEW_CODES = 88 * 1024, FEW_WIDEST = 512;
-constexpr int MMA_SLICE = 128, MMA_PL = 36, MMA_RING = 2;
-static long few_room(long T, long K) { return T > 2 ? T * ((K + MMA_SLICE - 1) / MMA_SLICE * MMA_SLICE + 16) : T * ((K + FEW_SLICE - 1) / FEW_SLICE * FEW_SLICE); }
 
 // Codes of all rows into shared memory, `pitch` apart, with zeros up to `width`, and their scales.
 template <int TT>
@@ -500,7 +588,7 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_mma_kernel(const I
 }
 
 template <int TT, bool GATED>
-static int launch_int8_few(const Int8Call& c, int device, cudaStream_t st) {
+static int launch_int8_few(const Int8Call& c, const Int8Plan& n, int device, cudaStream_t st) {
   constexpr bool MMA = TT > 2;
   static OncePerDevice once;
   const auto kernel = [] {
@@ -508,13 +596,9 @@ static int launch_int8_few(const Int8Call& c, int device, cudaStream_t st) {
     else return int8_few_kernel<TT, GATED>;
   }();
   if (const int e = once.ask(device, [&] { return (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_CODES); })) return -e;
-  const int cols = (int)(GATED ? c.N / 2 : c.N), least = (MMA ? 32 : 4) / (GATED ? 2 : 1), most = MMA ? least : FEW_WIDEST / (GATED ? 2 : 1);
-  int per = (cols + 295) / 296;
-  per = per < least ? least : per > most ? most : per;
-  const int tiles = (cols + per - 1) / per;
-  const Int8Few p = {c.x, c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldx, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, cols, per, tiles,
+  const Int8Few p = {c.x, c.codes, c.q, c.sx, c.sw, c.bias, c.out, c.ldx, c.ldc, c.ldw, c.ldo, (int)c.T, (int)c.N, (int)c.K, n.cols, n.per, n.tiles,
                      (int)c.x_f32, int8_rows_vec(c), (int)c.bias_f32, (int)c.out_f32};
-  kernel<<<tiles < 296 ? tiles : 296, FEW_WARPS * 32, few_room(c.T, c.K), st>>>(p);
+  kernel<<<n.grid, n.threads, n.smem, st>>>(p);
   return -(int)cudaGetLastError();
 }
 
@@ -523,19 +607,6 @@ static int launch_int8_few(const Int8Call& c, int device, cudaStream_t st) {
 // to four CTAs shares a tile: each has a part of K, leaves its sums in its shared memory and adds up its share of the tile's results from all of them (sums that met in
 // global memory through atomics took 53 to 250 us of 64 x 4096 x 11008). Weight bytes bound it, but for its start and end: with the codes in front 16 rows of a gated
 // 22016 x 4096 take 19.9 us, 4.6 TB/s, 64 rows of 4096 x 11008 14.7, 3.1 TB/s (the codes 2.6 us of them, the cluster's join 1.5).
-namespace i8s {
-constexpr int THREADS = 192, BK = 128, A_STAGE = 128 * BK;  // warp 0 loads, warp 1 products, warps 2 to 5 sums
-constexpr int MAX_STAGES = 12, REST = 1024 + 256;
-constexpr int stages(int tb, int ctas) { return (227 * 1024 / ctas - 1024 * (ctas - 1) - REST - 4 * tb) / (A_STAGE + tb * BK); }    // with so many CTAs an SM
-// At least 48 KB: a CTA of fewer would fit on an SM beside one of a pair that holds all tensor memory (int8_tile_kernel leaves 25 KB, other pairs less). On two streams
-// a cluster could then hold what the pair's other CTA wants, and the pair what the cluster's.
-constexpr int LEAST = 48 * 1024;
-constexpr int smem_bytes(int tb, int n) {
-  const int bytes = n * (A_STAGE + tb * BK) + REST + 4 * tb;
-  return bytes < LEAST ? LEAST : bytes;
-}
-}  // namespace i8s
-
 struct Int8Split {
   const float *sx, *sw;
   const void* bias;
@@ -732,24 +803,14 @@ __global__ void __launch_bounds__(i8s::THREADS, 2)
 }
 
 template <int TB, bool GATED>
-static int launch_int8_split(const Int8Call& c, bool early, int device, cudaStream_t st) {
+static int launch_int8_split(const Int8Call& c, const Int8Plan& n, bool early, int device, cudaStream_t st) {
   using namespace i8s;
   static OncePerDevice once;
   if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(int8_split_kernel<TB, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(TB, stages(TB, 1))); }))
     return -e;
-  const int cols = (int)(GATED ? c.N / 2 : c.N);
   Int8Split p;
-  p.sx = c.sx; p.sw = c.sw; p.bias = c.bias; p.out = c.out; p.ldo = c.ldo; p.T = (int)c.T; p.cols = cols; p.status = c.status;
-  p.kb = (int)((c.K + BK - 1) / BK); p.t_tiles = (int)((c.T + TB - 1) / TB);
-  const int tiles = (cols + (GATED ? 63 : 127)) / (GATED ? 64 : 128) * p.t_tiles;
-  auto fit = [&](int ctas) { const int n = ctas / tiles; return n < 1 ? 1 : n > 4 ? 4 : n; };
-  int parts = fit(128);
-  if (parts * tiles < 112) parts = fit(256);
-  p.parts = parts > p.kb ? p.kb : parts;
-  const int per_sm = tiles * p.parts <= 128 ? 1 : 2, most = stages(TB, per_sm), steps = (p.kb + p.parts - 1) / p.parts;
-  p.stages = most < steps ? most : steps;
-  if (p.stages > MAX_STAGES) p.stages = MAX_STAGES;
-  if (p.stages * (A_STAGE + TB * BK) < TB * 512) p.stages = (TB * 512 + A_STAGE + TB * BK - 1) / (A_STAGE + TB * BK);   // the sums take their place
+  p.sx = c.sx; p.sw = c.sw; p.bias = c.bias; p.out = c.out; p.ldo = c.ldo; p.T = (int)c.T; p.cols = n.cols; p.status = c.status;
+  p.kb = n.kb; p.t_tiles = n.t_tiles; p.parts = n.parts; p.stages = n.stages;
   p.inv_t = div_reciprocal(p.t_tiles); p.inv_parts = div_reciprocal(p.parts);
   p.bias_f32 = (int)c.bias_f32; p.out_f32 = (int)c.out_f32;
   p.fours = c.ldo % 4 == 0 && (uintptr_t)c.out % 16 == 0;
@@ -760,9 +821,9 @@ static int launch_int8_split(const Int8Call& c, bool early, int device, cudaStre
   if (rc == 0) rc = make_tmap(&tx, u8, 2, c.codes, {K, T}, {(uint64_t)c.ldc}, {BK, TB});
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(tiles * p.parts);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem_bytes(TB, p.stages);
+  cfg.gridDim = dim3(n.grid);
+  cfg.blockDim = dim3(n.threads);
+  cfg.dynamicSmemBytes = n.smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -776,18 +837,6 @@ static int launch_int8_split(const Int8Call& c, bool early, int device, cudaStre
 }
 
 // ---------------------------------------------------------------------------------------------- tiles
-namespace i8t {
-constexpr int BM = 256, BN = 256, BK = 128, STAGES = 5;    // BK in bytes: a swizzled row
-constexpr int A_STAGE = 128 * BK, B_STAGE = 128 * BK;      // of one CTA
-constexpr int THREADS = 320;                               // warp 0 loads, warp 1 products, warps 2 to 9 results
-constexpr int STAGING = 8 * 4096;                          // a box of 32 rows x 128 bytes a warp
-constexpr int TABLE = 8 * 2 * 128 * 4;                     // scales and biases of a warp's 128 columns of a tile
-constexpr int SMEM_BYTES = STAGES * (A_STAGE + B_STAGE) + STAGING + TABLE + 1024 + 256;
-constexpr int TMEM_COLS = 512;
-// 8-bit signed operands, 32-bit whole sums, both operands K-major
-constexpr uint32_t IDESC = (2u << 4) | (1u << 7) | (1u << 10) | ((BN >> 3) << 17) | ((BM >> 4) << 24);
-}  // namespace i8t
-
 __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n"
@@ -1032,35 +1081,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
 }
 
 template <bool GATED, bool F32>
-static int launch_int8_tiles(const Int8Call& c, bool early, int device, cudaStream_t st) {
+static int launch_int8_tiles(const Int8Call& c, const Int8Plan& n, bool early, int device, cudaStream_t st) {
   using namespace i8t;
   static OncePerDevice once;
   if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(int8_tile_kernel<GATED, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES); }))
     return -e;
-  const int cols = (int)(GATED ? c.N / 2 : c.N), size = F32 ? 4 : 2;
+  const int size = F32 ? 4 : 2;
   Int8Tiles p;
-  p.sx = c.sx; p.sw = c.sw; p.bias = c.bias; p.out = c.out; p.ldo = c.ldo; p.T = (int)c.T; p.K = (int)c.K; p.cols = cols;
-  p.m_tiles = (int)((c.T + BM - 1) / BM); p.n_tiles = (cols + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
+  p.sx = c.sx; p.sw = c.sw; p.bias = c.bias; p.out = c.out; p.ldo = c.ldo; p.T = (int)c.T; p.K = (int)c.K; p.cols = n.cols;
+  p.m_tiles = n.t_tiles; p.n_tiles = n.tiles / n.t_tiles;
   p.inv_n = div_reciprocal(p.n_tiles); p.bias_f32 = (int)c.bias_f32; p.status = c.status;
   p.boxes = ((uintptr_t)c.out | (uintptr_t)(c.ldo * size)) % 16 == 0;
   CUtensorMap ta, tb, tc;
   int rc = make_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.codes, {(uint64_t)c.K, (uint64_t)c.T}, {(uint64_t)c.ldc}, {BK, 128});
   if (rc == 0) rc = make_tmap(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, c.q, {(uint64_t)c.K, (uint64_t)c.N}, {(uint64_t)c.ldw}, {BK, 128});
   tc = ta;
-  if (rc == 0 && p.boxes) rc = F32 ? make_tmap_2d_f32(&tc, c.out, (uint64_t)cols, (uint64_t)c.T, (uint64_t)c.ldo, 32, 32)
-                                   : make_tmap_2d_bf16(&tc, c.out, (uint64_t)cols, (uint64_t)c.T, (uint64_t)c.ldo, 64, 32);
+  if (rc == 0 && p.boxes) rc = F32 ? make_tmap_2d_f32(&tc, c.out, (uint64_t)n.cols, (uint64_t)c.T, (uint64_t)c.ldo, 32, 32)
+                                   : make_tmap_2d_bf16(&tc, c.out, (uint64_t)n.cols, (uint64_t)c.T, (uint64_t)c.ldo, 64, 32);
   if (rc) return rc;
-  const long total = (long)p.m_tiles * p.n_tiles;
-  const int pairs = (int)(total < 74 ? total : 74);
-  launch_step(early, int8_tile_kernel<GATED, F32>, dim3(2 * pairs), THREADS, SMEM_BYTES, st, ta, tb, tc, p);
+  launch_step(early, int8_tile_kernel<GATED, F32>, dim3(n.grid), n.threads, n.smem, st, ta, tb, tc, p);
   return -(int)cudaGetLastError();
-}
-
-enum Int8Route { INT8_FEW, INT8_SPLIT, INT8_TILES };
-static Int8Route int8_route(const Int8Call& c) {
-  if (c.T <= FEW_ROWS && (c.T == 1 || c.N * c.K <= (32l << 20)) && few_room(c.T, c.K) <= FEW_CODES) return INT8_FEW;
-  const long tiles = (c.T + 127) / 128 * ((c.gated ? c.N / 2 + 63 : c.N + 127) / (c.gated ? 64 : 128));
-  return c.T <= 128 || tiles <= 148 ? INT8_SPLIT : INT8_TILES;
 }
 
 }  // namespace inv
@@ -1074,10 +1114,14 @@ extern "C" int inv_int8_rows(const void* call) {
 }
 
 // Whether a product makes the codes for itself and wants no place for them.
-extern "C" int inv_int8_alone(long T, long N, long K) {
-  Int8Call c = {};
-  c.T = T; c.N = N; c.K = K;
-  return int8_route(c) == INT8_FEW;
+extern "C" int inv_int8_alone(long T, long N, long K) { return int8_route(T, N, K, false) == INT8_FEW; }
+
+// The plan's numbers in their order, for who wants to look at them.
+extern "C" int inv_int8_plan(long T, long N, long K, int gated, int* out) {
+  if (T < 1 || N < 1 || K < 1 || (gated && N < 2)) return -ERR_BAD_ARG;
+  const Int8Plan n = int8_plan(T, N, K, gated != 0);
+  for (const int v : {n.route, n.cols, n.grid, n.cluster, n.threads, n.smem, n.tiles, n.t_tiles, n.tb, n.per, n.kb, n.parts, n.stages}) *out++ = v;
+  return 0;
 }
 
 // Codes first where x is given and the product does not make them, then the product, which starts while they are made: the kernel of the codes is launched plainly, so everything in front of it is
@@ -1090,24 +1134,21 @@ extern "C" int inv_int8_linear(const void* call) {
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;
   const bool early = c.x != nullptr;
-  const Int8Route route = int8_route(c);
+  const Int8Plan plan = int8_plan(c.T, c.N, c.K, c.gated != 0);
+  const int route = plan.route, tb = plan.tb;
   if (route != INT8_FEW && (c.codes == nullptr || c.sx == nullptr)) return -ERR_BAD_ARG;
   if (route == INT8_FEW) {
-#define INV_FEW(TT) (c.gated ? launch_int8_few<TT, true>(c, device, st) : launch_int8_few<TT, false>(c, device, st))
+#define INV_FEW(TT) (c.gated ? launch_int8_few<TT, true>(c, plan, device, st) : launch_int8_few<TT, false>(c, plan, device, st))
     return c.T == 1 ? INV_FEW(1) : c.T == 2 ? INV_FEW(2) : INV_FEW(4);
 #undef INV_FEW
   }
   if (early)
     if (const int e = launch_int8_rows(c, st)) return e;
   if (route == INT8_SPLIT) {
-#define INV_SPLIT(TB) (c.gated ? launch_int8_split<TB, true>(c, early, device, st) : launch_int8_split<TB, false>(c, early, device, st))
-    const long col_tiles = (c.gated ? c.N / 2 + 63 : c.N + 127) / (c.gated ? 64 : 128);
-    int tb = c.T <= 16 ? 16 : c.T <= 32 ? 32 : c.T <= 64 ? 64 : 128;
-    if (c.T > 64)
-      while (tb > 32 && (c.T + tb - 1) / tb * col_tiles < 100) tb /= 2;
+#define INV_SPLIT(TB) (c.gated ? launch_int8_split<TB, true>(c, plan, early, device, st) : launch_int8_split<TB, false>(c, plan, early, device, st))
     return tb <= 16 ? INV_SPLIT(16) : tb <= 32 ? INV_SPLIT(32) : tb <= 64 ? INV_SPLIT(64) : INV_SPLIT(128);
 #undef INV_SPLIT
   }
-  if (c.gated) return c.out_f32 ? launch_int8_tiles<true, true>(c, early, device, st) : launch_int8_tiles<true, false>(c, early, device, st);
-  return c.out_f32 ? launch_int8_tiles<false, true>(c, early, device, st) : launch_int8_tiles<false, false>(c, early, device, st);
+  if (c.gated) return c.out_f32 ? launch_int8_tiles<true, true>(c, plan, early, device, st) : launch_int8_tiles<true, false>(c, plan, early, device, st);
+  return c.out_f32 ? launch_int8_tiles<false, true>(c, plan, early, device, st) : launch_int8_tiles<false, false>(c, plan, early, device, st);
 }

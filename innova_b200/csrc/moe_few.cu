@@ -52,7 +52,8 @@ struct MoeFewCall {
 struct MoeFewPlan {
   int slots, ld_act, f_tiles, d_tiles, experts, n_counters;
   int gate_steps, down_steps, down_per, down_parts;    // of K: in all, of a part, parts
-  long choice, weight, counters, act, sums, bytes;
+  int tb, slices;                                      // tokens of a product's operand; slices of D in the router
+  long choice, weight, counters, act, sums, bytes, items;
   MoeFewPlan(long T, long D, long F, long E, long top_k, bool shared, bool i8) {
     auto up = [](long v) { return (v + 255) / 256 * 256; };
     const int step = i8 ? 128 : 64;
@@ -73,6 +74,9 @@ struct MoeFewPlan {
     act = up(counters + n_counters * 4L);
     sums = up(act + (long)slots * ld_act * 2);
     bytes = up(sums + (long)down_parts * slots * D * 4);
+    items = (long)experts * (f_tiles + d_tiles * down_parts) + d_tiles * ((T + MF_GROUP - 1) / MF_GROUP);
+    tb = T <= 16 ? 16 : T <= 32 ? 32 : 64;
+    slices = D >= 2048 ? 8 : D >= 1024 ? 4 : D >= 512 ? 2 : 1;
   }
 };
 
@@ -202,6 +206,7 @@ struct Shape {
   static constexpr int SUMS = 4, CONVERT = SUMS + 4 * SETS, THREADS = 32 * (CONVERT + (I8 ? 4 * CONV : 0));
   static constexpr int SMEM = STAGES * (A_STAGE + B_STAGE) + 1024;
   static constexpr int COLS = ACC * TB + (I8 ? CONV * 64 : 0), TMEM = COLS <= 64 ? 64 : COLS <= 128 ? 128 : COLS <= 256 ? 256 : 512;
+  static int grid(long items) { return (int)(items < 148 * PER_SM ? items : 148 * PER_SM); }
 };
 enum Kind { GATE, DOWN, SUM, END };
 struct __align__(16) Item {
@@ -704,10 +709,9 @@ struct MoeFewMaps {
 template <int TB, bool I8>
 static int launch_moe_few(const MoeFewMaps& m, const MoeFew& p, long items, int device, cudaStream_t st) {
   using S = mf::Shape<TB, I8>;
-  const int grid = (int)(items < 148 * S::PER_SM ? items : 148 * S::PER_SM);
   static OncePerDevice once;
   if (const int e = once.ask(device, [] { return (int)cudaFuncSetAttribute(moe_few_kernel<TB, I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); })) return -e;
-  launch_early(moe_few_kernel<TB, I8>, dim3(grid), S::THREADS, S::SMEM, st, m.x, m.act, m.gate, m.down, m.shared_gate, m.shared_down, p);
+  launch_early(moe_few_kernel<TB, I8>, dim3(S::grid(items)), S::THREADS, S::SMEM, st, m.x, m.act, m.gate, m.down, m.shared_gate, m.shared_down, p);
   return -(int)cudaGetLastError();
 }
 
@@ -717,6 +721,24 @@ using namespace inv;
 
 extern "C" long inv_moe_few_bytes(long T, long D, long F, long E, long top_k, int shared, int i8) {
   return MoeFewPlan(T, D, F, E, top_k, shared != 0, i8 != 0).bytes;
+}
+
+template <int TB, bool I8>
+static int* moe_few_shape(const MoeFewPlan& n, int* out) {
+  using S = mf::Shape<TB, I8>;
+  for (const int v : {S::grid(n.items), S::THREADS, S::SMEM, S::PER_SM, S::STAGES, S::STEP, S::COLS, S::TMEM}) *out++ = v;
+  return out;
+}
+// The plan's numbers in their order, and those of the launch, for who wants to look at them.
+extern "C" int inv_moe_few_plan(long T, long D, long F, long E, long top_k, int shared, int i8, int* out, long* places) {
+  if (T < 1 || T > MF_TOKENS || D < 1 || F < 1 || E < 1 || E > MF_EXPERTS || top_k < 1 || top_k > MF_TOP || top_k > E) return -ERR_BAD_ARG;
+  const MoeFewPlan n(T, D, F, E, top_k, shared != 0, i8 != 0);
+  for (const int v : {n.slots, n.ld_act, n.f_tiles, n.d_tiles, n.experts, n.n_counters, n.gate_steps, n.down_steps, n.down_per, n.down_parts, n.tb, n.slices}) *out++ = v;
+  for (const long v : {n.choice, n.weight, n.counters, n.act, n.sums, n.bytes, n.items}) *places++ = v;
+#define INV_MF(TB) (i8 ? moe_few_shape<TB, true>(n, out) : moe_few_shape<TB, false>(n, out))
+  n.tb == 16 ? INV_MF(16) : n.tb == 32 ? INV_MF(32) : INV_MF(64);
+#undef INV_MF
+  return 0;
 }
 
 extern "C" int inv_moe_few(const void* call) {
@@ -730,8 +752,7 @@ extern "C" int inv_moe_few(const void* call) {
         (uintptr_t)c.work | (uintptr_t)c.residual | (uintptr_t)c.out) & 15))
     return -ERR_BAD_ARG;
   const MoeFewPlan plan(c.T, c.D, c.F, c.E, c.top_k, shared, c.i8 != 0);
-  const long items = (long)plan.experts * (plan.f_tiles + plan.d_tiles * plan.down_parts) + plan.d_tiles * ((c.T + MF_GROUP - 1) / MF_GROUP);
-  if (c.work_bytes < plan.bytes || items > (1 << 30)) return -ERR_BAD_ARG;
+  if (c.work_bytes < plan.bytes || plan.items > (1 << 30)) return -ERR_BAD_ARG;
   cudaStream_t st = (cudaStream_t)c.stream;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;
@@ -748,7 +769,7 @@ extern "C" int inv_moe_few(const void* call) {
   p.f_tiles = plan.f_tiles; p.d_tiles = plan.d_tiles; p.gate_steps = plan.gate_steps; p.down_steps = plan.down_steps; p.down_per = plan.down_per; p.down_parts = plan.down_parts; p.experts = plan.experts;
   p.inv_k = div_reciprocal(p.top_k); p.inv_f = div_reciprocal(p.f_tiles);
   p.inv_down = div_reciprocal(p.d_tiles * p.down_parts); p.inv_down_parts = div_reciprocal(p.down_parts); p.inv_d = div_reciprocal(p.d_tiles);
-  const int tb = p.T <= 16 ? 16 : p.T <= 32 ? 32 : 64;
+  const int tb = plan.tb;
   const CUtensorMapDataType bf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, type = c.i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : bf16;
   const uint64_t D = c.D, F = c.F, E = c.E, size = c.i8 ? 1 : 2, row = D * size;
   const uint32_t wide = c.i8 ? 128 : 64;
@@ -762,10 +783,9 @@ extern "C" int inv_moe_few(const void* call) {
   if (rc == 0 && shared) rc = make_tmap(&m.shared_gate, type, 5, c.shared_gate_up, {D, 8, 2, F / 8, 1}, {row, F * row, 8 * row, 2 * F * row}, {wide, 8, 2, MF_F / 8, 1});
   if (rc == 0 && shared) rc = make_tmap(&m.shared_down, type, 3, c.shared_down, {F, D, 1}, {F * size, D * F * size}, {wide, 128, 1});
   if (rc) return rc;
-  const int slices = p.D >= 2048 ? 8 : p.D >= 1024 ? 4 : p.D >= 512 ? 2 : 1;
-  moe_few_router_kernel<<<(unsigned)p.T, 1024, 0, st>>>(c.x, c.ldx, c.router, p.D, p.E, p.top_k, slices, (int*)p.choice, (float*)p.weight, p.counters, plan.n_counters);
+  moe_few_router_kernel<<<(unsigned)p.T, 1024, 0, st>>>(c.x, c.ldx, c.router, p.D, p.E, p.top_k, plan.slices, (int*)p.choice, (float*)p.weight, p.counters, plan.n_counters);
   if (const cudaError_t e = cudaGetLastError()) return -(int)e;
-#define INV_MF(TB) (c.i8 ? launch_moe_few<TB, true>(m, p, items, device, st) : launch_moe_few<TB, false>(m, p, items, device, st))
+#define INV_MF(TB) (c.i8 ? launch_moe_few<TB, true>(m, p, plan.items, device, st) : launch_moe_few<TB, false>(m, p, plan.items, device, st))
   return tb == 16 ? INV_MF(16) : tb == 32 ? INV_MF(32) : INV_MF(64);
 #undef INV_MF
 }

@@ -22,7 +22,7 @@ from .functional import swiglu
 from .gemm import linear
 
 _native.register_cuda_sigs({"inv_int8_rows": [_native.vp], "inv_int8_linear": [_native.vp],
-                            "inv_int8_alone": [_native.i64] * 3})
+                            "inv_int8_alone": [_native.i64] * 3, "inv_int8_plan": [_native.i64] * 3 + [_native.i32, _native.vp]})
 
 # What the entries are given: x, weights, their scales, bias, result, codes, their scales, status and stream; tokens, weight rows, K; strides of x, weights,
 # result and codes; whether x, the result and the bias are fp32; gated.

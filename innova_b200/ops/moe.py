@@ -35,6 +35,7 @@ _native.register_cuda_sigs({
                                                                _native.i32, _native.i32, _native.vp, _native.vp, _native.i32, _native.i32,
                                                                _native.i64, _native.vp, _native.vp],
     "inv_moe_few": [_native.vp], "inv_moe_few_bytes": [_native.i64] * 5 + [_native.i32] * 2,
+    "inv_moe_few_plan": [_native.i64] * 5 + [_native.i32] * 2 + [_native.vp] * 2,
 })
 
 ALIGN = 128
