@@ -3,7 +3,7 @@
 //   s_t = max(|x_t|, 1e-10) / 127       c_tk = rint(x_tk / s_t), halves to even
 //   y_tn = s_t s_n sum_k c_tk q_nk + b_n            gated: silu(y_tn) y_t,n+F, n < F
 //
-// The sums are whole numbers below 2^31 (K <= 133144), so their order changes nothing; scales and bias are applied in fp32 and the result is rounded once.
+// The sums are whole numbers below 2^31 (K <= 131071, codes from -128), so their order changes nothing; scales and bias are applied in fp32 and the result is rounded once.
 //
 // int8_rows_kernel      rows of activations into codes and scales
 // int8_few_kernel       one row, or up to four and weights of up to 32 MB: codes and product in one launch
@@ -15,6 +15,8 @@
 #include <type_traits>
 
 namespace inv {
+
+constexpr long INT8_MAX_K = 131071;      // 128 * 128 K < 2^31
 
 // What the entry is given; sizes in elements.
 struct Int8Call {
@@ -1129,7 +1131,7 @@ extern "C" int inv_int8_plan(long T, long N, long K, int gated, int* out) {
 extern "C" int inv_int8_linear(const void* call) {
   const Int8Call& c = *static_cast<const Int8Call*>(call);
   if (c.T <= 0 || c.N <= 0 || c.K <= 0) return 0;
-  if (c.K > 133144 || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2) || (c.gated && c.N < 2)) return -ERR_BAD_ARG;
+  if (c.K > INT8_MAX_K || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2) || (c.gated && c.N < 2)) return -ERR_BAD_ARG;
   cudaStream_t st = (cudaStream_t)c.stream;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;

@@ -1,8 +1,8 @@
 """Products with weights and activations in 8-bit integers (``csrc/int8_linear.cu``), for serving.
 
 A row of activations is held as whole numbers c = rint(x / s) (halves to even) with s = max(|x|, 1e-10) / 127 in fp32, a scale for each token; a row of
-weights likewise, a scale for each output channel. Their sums of products are whole numbers that 32 bits hold up to K = 133144, so that a result depends on
-no order and not on how many tokens came with it; scales and bias are applied in fp32 and the result is rounded once. A row with a value that is not finite
+weights likewise, a scale for each output channel. Codes of the caller's own may be any int8, -128 among them. Sums of products are whole numbers that 32 bits hold up to
+K = 131071 (128 * 128 K < 2^31), so that a result depends on no order and not on how many tokens came with it; scales and bias are applied in fp32 and the result is rounded once. A row with a value that is not finite
 gives NaN. ``engines.int8_quantize_per_token`` and ``inference.serving.INT8Inference`` hold rows the same way; the product of the latter is of fp32.
 
 No gradient and no tangent passes through these."""
@@ -28,7 +28,7 @@ _native.register_cuda_sigs({"inv_int8_rows": [_native.vp], "inv_int8_linear": [_
 # result and codes; whether x, the result and the bias are fp32; gated.
 _CALL = struct.Struct("=9Q 11q").pack
 
-MAX_K, LEAST = 133144, 1e-10
+MAX_K, LEAST = 131071, 1e-10
 _int8, _fp32, _bf16 = torch.int8, torch.float32, torch.bfloat16
 
 

@@ -345,3 +345,24 @@ def test_clusters_beside_pairs():
     torch.cuda.synchronize()
     rt.check_status()
     assert all(torch.equal(y, want[i]) for i in (0, 1) for y in got[i])
+
+
+def test_the_longest_rows_hold_every_code():
+    """-128 in rows of the caller's own and in weights: the longest K that is taken has sums below 2^31, the next is refused."""
+    assert 128 * 128 * int8.MAX_K < 2 ** 31 <= 128 * 128 * (int8.MAX_K + 1)
+    K = 131200
+    with pytest.raises(ValueError, match="32 bits"):
+        int8_linear(torch.ones(1, K), Int8Weight(torch.full((1, K), -128, dtype=torch.int8), torch.ones(1)))
+
+
+@gpu
+@pytest.mark.parametrize("T", [1, 2, 4, 20, 70])
+def test_largest_sums_of_every_code(T):
+    K = int8.MAX_K // 16 * 16
+    w = Int8Weight(torch.full((4, K), -128, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda"))
+    w.q[1] = 127
+    x = Int8Rows(torch.full((T, K), -128, dtype=torch.int8, device="cuda"), torch.ones(T, device="cuda"))
+    y = int8_linear(x, w, out_dtype=F32).cpu().double()
+    want = 128.0 * K * torch.tensor([128, -127, 128, 128], dtype=torch.float64)
+    assert bool(((y - want).abs() <= 2 * E24 * want.abs()).all())            # one conversion to fp32; scales of one
+    rt.check_status()
