@@ -48,7 +48,7 @@ class Int8Weight(NamedTuple):
 
     @staticmethod
     def quantize(w: torch.Tensor) -> "Int8Weight":
-        """w [..., N, K] in bf16 or fp32. On a GPU stacks go one by one: nothing of the weight's size is held beside the result."""
+        """w [..., N, K] in bf16 or fp32. Nothing of the weight's size is held beside the result, unless w's rows have no even distance or no unit stride: then a copy."""
         return Int8Weight(*quantize_rows(w.detach()))
 
     def dequantize(self) -> torch.Tensor:
@@ -143,15 +143,11 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
         y = F.linear(codes.q.double(), q.double()).float() * codes.scale.unsqueeze(-1) * sw
         y = y if bias is None else y + bias.float()
         return (F.silu(y[..., :cols]) * y[..., cols:] if gated else y).to(out_dtype)
-    if len(shape) == 2 and x.is_contiguous():
-        rows, ld, T = x, K, shape[0]
-        out = x.new_empty((T, cols), dtype=out_dtype)
-    else:
-        out = x.new_empty((*shape[:-1], cols), dtype=out_dtype)
-        rows, ld = _rows_of(x)
-        T = rows.shape[0]
-    if T == 0 or cols == 0 or K == 0:
+    out = x.new_empty((*shape[:-1], cols), dtype=out_dtype)
+    if cols == 0 or K == 0 or x.numel() == 0:
         return _without_products(out, bias, cols, gated)
+    rows, ld = (x, K) if len(shape) == 2 and x.is_contiguous() else _rows_of(x)
+    T = rows.shape[0]
     with rt.device_of(x):
         alone = codes is None and T <= 4 and _alone(T, N, K)
         if alone:

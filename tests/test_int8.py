@@ -366,3 +366,16 @@ def test_largest_sums_of_every_code(T):
     want = 128.0 * K * torch.tensor([128, -127, 128, 128], dtype=torch.float64)
     assert bool(((y - want).abs() <= 2 * E24 * want.abs()).all())            # one conversion to fp32; scales of one
     rt.check_status()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_nothing_to_add_up_behind_leading_dimensions(device):
+    b = torch.arange(4.0, device=device)
+    w = Int8Weight(torch.zeros(4, 0, dtype=torch.int8, device=device), torch.ones(4, device=device))
+    x = torch.zeros(2, 3, 0, device=device)
+    assert torch.equal(int8_linear(x, w, b), b.expand(2, 3, 4)) and not int8_linear(x, w).any()
+    assert torch.equal(int8_linear(x, w, b, gated=True), (torch.nn.functional.silu(b[:2]) * b[2:]).expand(2, 3, 2))
+    assert torch.equal(int8_linear(quantize_rows(x), w, b, F32), b.expand(2, 3, 4))
+    v = weight(6, 32, device=device)
+    for shape in ((0, 5, 32), (3, 0, 32), (0, 32)):
+        assert int8_linear(torch.zeros(shape, device=device), v).shape == (*shape[:-1], 6)
