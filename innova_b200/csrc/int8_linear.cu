@@ -297,6 +297,9 @@ static int launch_int8_rows(const Int8Call& c, cudaStream_t st) {
   return -(int)cudaGetLastError();
 }
 
+// The scales are multiplied first: a sum of codes, up to 2^31, times the scale of a token of 1e32 and more would not fit. The conversion, the scales' product and the
+// whole are rounded, half a step each.
+__device__ __forceinline__ float int8_value(int sum, float sx, float sw, float bias) { return fmaf((float)sum, sx * sw, bias); }
 __device__ __forceinline__ float int8_silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
 // ---------------------------------------------------------------------------------------------- up to four rows
@@ -501,8 +504,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_kernel(const Int8F
     for (int i = tid; i < width * TT; i += FEW_WARPS * 32) {
       const int t = i / width, c = i - t * width, col = now + c;
       const float sx = scales[t];
-      float y = fmaf((float)part[t * FEW_WIDEST + c] * sx, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
-      if (GATED) y = int8_silu(y) * fmaf((float)part[t * FEW_WIDEST + width + c] * sx, p.sw[p.cols + col], int8_bias(p.bias, p.bias_f32, p.cols + col));
+      float y = int8_value(part[t * FEW_WIDEST + c], sx, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
+      if (GATED) y = int8_silu(y) * int8_value(part[t * FEW_WIDEST + width + c], sx, p.sw[p.cols + col], int8_bias(p.bias, p.bias_f32, p.cols + col));
       if (p.out_f32) static_cast<float*>(p.out)[t * p.ldo + col] = y;
       else static_cast<__nv_bfloat16*>(p.out)[t * p.ldo + col] = __float2bfloat16_rn(y);
     }
@@ -580,8 +583,8 @@ __global__ void __launch_bounds__(FEW_WARPS * 32, 2) int8_few_mma_kernel(const I
         if (GATED) b += part[(w * 8 + t) * MMA_PL + 16 + c];
       }
       const float s = scales[t];
-      float y = fmaf((float)a * s, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
-      if (GATED) y = int8_silu(y) * fmaf((float)b * s, p.sw[p.cols + col], int8_bias(p.bias, p.bias_f32, p.cols + col));
+      float y = int8_value(a, s, p.sw[col], int8_bias(p.bias, p.bias_f32, col));
+      if (GATED) y = int8_silu(y) * int8_value(b, s, p.sw[p.cols + col], int8_bias(p.bias, p.bias_f32, p.cols + col));
       if (p.out_f32) static_cast<float*>(p.out)[t * p.ldo + col] = y;
       else static_cast<__nv_bfloat16*>(p.out)[t * p.ldo + col] = __float2bfloat16_rn(y);
     }
@@ -777,8 +780,8 @@ __global__ void __launch_bounds__(i8s::THREADS, 2)
       float y[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        y[i] = fmaf((float)v[0][i] * sx, sw[0][i], bias[0][i]);
-        if (GATED) y[i] = int8_silu(y[i]) * fmaf((float)v[SUB - 1][i] * sx, sw[SUB - 1][i], bias[SUB - 1][i]);
+        y[i] = int8_value(v[0][i], sx, sw[0][i], bias[0][i]);
+        if (GATED) y[i] = int8_silu(y[i]) * int8_value(v[SUB - 1][i], sx, sw[SUB - 1][i], bias[SUB - 1][i]);
       }
       const long o = (long)(t0 + t) * p.ldo + col;
       if (p.fours && col + 3 < p.cols) {
@@ -1013,16 +1016,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(i8t::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 s4 = *reinterpret_cast<const float4*>(scale + c + x + j), b4 = *reinterpret_cast<const float4*>(bias + c + x + j);
-            y[j] = fmaf((float)(int)r[j] * sx, s4.x, b4.x);
-            y[j + 1] = fmaf((float)(int)r[j + 1] * sx, s4.y, b4.y);
-            y[j + 2] = fmaf((float)(int)r[j + 2] * sx, s4.z, b4.z);
-            y[j + 3] = fmaf((float)(int)r[j + 3] * sx, s4.w, b4.w);
+            y[j] = int8_value((int)r[j], sx, s4.x, b4.x);
+            y[j + 1] = int8_value((int)r[j + 1], sx, s4.y, b4.y);
+            y[j + 2] = int8_value((int)r[j + 2], sx, s4.z, b4.z);
+            y[j + 3] = int8_value((int)r[j + 3], sx, s4.w, b4.w);
             if constexpr (GATED) {
               const float4 s5 = *reinterpret_cast<const float4*>(scale + 64 + c + x + j), b5 = *reinterpret_cast<const float4*>(bias + 64 + c + x + j);
-              y[j] = int8_silu(y[j]) * fmaf((float)(int)r2[j] * sx, s5.x, b5.x);
-              y[j + 1] = int8_silu(y[j + 1]) * fmaf((float)(int)r2[j + 1] * sx, s5.y, b5.y);
-              y[j + 2] = int8_silu(y[j + 2]) * fmaf((float)(int)r2[j + 2] * sx, s5.z, b5.z);
-              y[j + 3] = int8_silu(y[j + 3]) * fmaf((float)(int)r2[j + 3] * sx, s5.w, b5.w);
+              y[j] = int8_silu(y[j]) * int8_value((int)r2[j], sx, s5.x, b5.x);
+              y[j + 1] = int8_silu(y[j + 1]) * int8_value((int)r2[j + 1], sx, s5.y, b5.y);
+              y[j + 2] = int8_silu(y[j + 2]) * int8_value((int)r2[j + 2], sx, s5.z, b5.z);
+              y[j + 3] = int8_silu(y[j + 3]) * int8_value((int)r2[j + 3], sx, s5.w, b5.w);
             }
           }
           if constexpr (F32) {

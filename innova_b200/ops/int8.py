@@ -140,7 +140,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
     cols = N // 2 if gated else N
     if dev < 0:
         codes = quantize_rows(x) if codes is None else codes
-        y = F.linear(codes.q.double(), q.double()).float() * codes.scale.unsqueeze(-1) * sw
+        y = F.linear(codes.q.double(), q.double()).float() * (codes.scale.unsqueeze(-1) * sw)      # in this order: sums times a large scale alone may not fit
         y = y if bias is None else y + bias.float()
         return (F.silu(y[..., :cols]) * y[..., cols:] if gated else y).to(out_dtype)
     out = x.new_empty((*shape[:-1], cols), dtype=out_dtype)

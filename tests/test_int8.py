@@ -379,3 +379,19 @@ def test_nothing_to_add_up_behind_leading_dimensions(device):
     v = weight(6, 32, device=device)
     for shape in ((0, 5, 32), (3, 0, 32), (0, 32)):
         assert int8_linear(torch.zeros(shape, device=device), v).shape == (*shape[:-1], 6)
+
+
+@pytest.mark.parametrize("size", [1e36, 1e-9])
+@pytest.mark.parametrize("T", [1, 3, 20, 200, 3000])
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_rows_of_any_size(size, T, device):
+    """Results that fp32 holds, though a sum of codes times the token's scale is beyond it."""
+    K, N = 64, (2050 if T == 3000 else 66)
+    x, w = rows(T, K, F32) * size, weight(N, K)
+    assert float((127 * 73 * K ** 0.5) * x.abs().amax() / 127) > (2.0 ** 128 if size > 1 else 0)
+    y = int8_linear(x.to(device), Int8Weight(weight(N, K, device=device).q, w.scale.to(device)))
+    if device == "cuda":
+        rt.check_status()
+    want, err = expected(*definition(x), w)
+    assert float(want.abs().max()) < 2.0 ** 127
+    close(y.cpu(), want, err)
