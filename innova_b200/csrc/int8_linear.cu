@@ -16,7 +16,8 @@
 
 namespace inv {
 
-constexpr long INT8_MAX_K = 131071;      // 128 * 128 K < 2^31
+constexpr long INT8_MOST_K = 131071;      // 128 * 128 K < 2^31
+constexpr long INT8_MOST = (1l << 31) - 1024;  // rows, columns and values of a row that is made into codes: counted in 32 bits
 
 // What the entry is given; sizes in elements.
 struct Int8Call {
@@ -1115,6 +1116,7 @@ using namespace inv;
 extern "C" int inv_int8_rows(const void* call) {
   const Int8Call& c = *static_cast<const Int8Call*>(call);
   if (c.T <= 0 || c.K <= 0) return 0;
+  if (c.T > INT8_MOST || c.K > INT8_MOST) return -ERR_BAD_ARG;
   return launch_int8_rows(c, (cudaStream_t)c.stream);
 }
 
@@ -1123,7 +1125,7 @@ extern "C" int inv_int8_alone(long T, long N, long K) { return int8_route(T, N, 
 
 // The plan's numbers in their order, for who wants to look at them.
 extern "C" int inv_int8_plan(long T, long N, long K, int gated, int* out) {
-  if (T < 1 || N < 1 || K < 1 || (gated && N < 2)) return -ERR_BAD_ARG;
+  if (T < 1 || T > INT8_MOST || N < 1 || N > INT8_MOST || K < 1 || K > INT8_MOST_K || (gated && N < 2)) return -ERR_BAD_ARG;
   const Int8Plan n = int8_plan(T, N, K, gated != 0);
   for (const int v : {n.route, n.cols, n.grid, n.cluster, n.threads, n.smem, n.tiles, n.t_tiles, n.tb, n.per, n.kb, n.parts, n.stages}) *out++ = v;
   return 0;
@@ -1134,7 +1136,7 @@ extern "C" int inv_int8_plan(long T, long N, long K, int gated, int* out) {
 extern "C" int inv_int8_linear(const void* call) {
   const Int8Call& c = *static_cast<const Int8Call*>(call);
   if (c.T <= 0 || c.N <= 0 || c.K <= 0) return 0;
-  if (c.K > INT8_MAX_K || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2) || (c.gated && c.N < 2)) return -ERR_BAD_ARG;
+  if (c.T > INT8_MOST || c.N > INT8_MOST || c.K > INT8_MOST_K || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2) || (c.gated && c.N < 2)) return -ERR_BAD_ARG;
   cudaStream_t st = (cudaStream_t)c.stream;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;

@@ -395,3 +395,14 @@ def test_rows_of_any_size(size, T, device):
     want, err = expected(*definition(x), w)
     assert float(want.abs().max()) < 2.0 ** 127
     close(y.cpu(), want, err)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """By the entries, before they ask for a device: no pointer is looked at."""
+    from innova_b200 import _native
+    lib, bad = _native.cuda(), -7
+    at = 1 << 20
+    call = lambda T, N, K: int8._CALL(at, at, at, 0, at, at, at, at, 0, T, N, K, K, (K + 15) // 16 * 16, N, (K + 15) // 16 * 16, 0, 0, 0, 0)  # noqa: E731
+    assert lib.inv_int8_rows(call(1, 0, 2 ** 32 + 5)) == bad and lib.inv_int8_rows(call(2 ** 31, 0, 8)) == bad
+    for T, N, K in ((2 ** 31, 16, 16), (16, 2 ** 31, 16), (16, 16, 131072), (2 ** 32 + 1, 16, 16)):
+        assert lib.inv_int8_linear(call(T, N, K)) == bad
