@@ -136,7 +136,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
             and (codes is None or dtype is _int8 and codes.scale.shape == shape[:-1] and codes.scale.dtype is _fp32 and codes.scale.get_device() == dev)
             and (dev < 0 or ldw % 16 == 0 and ldw >= K and q.data_ptr() % 16 == 0)) or gated and N % 2:
         _refuse(x, codes, w, bias, out_dtype, gated)
-    refuse_gradients("int8_linear", x, bias)
+    refuse_gradients("int8_linear", x, bias, sw, None if codes is None else codes.scale)
     cols = N // 2 if gated else N
     if dev < 0:
         codes = quantize_rows(x) if codes is None else codes

@@ -406,3 +406,12 @@ def test_sizes_beyond_32_bits_are_refused():
     assert lib.inv_int8_rows(call(1, 0, 2 ** 32 + 5)) == bad and lib.inv_int8_rows(call(2 ** 31, 0, 8)) == bad
     for T, N, K in ((2 ** 31, 16, 16), (16, 2 ** 31, 16), (16, 16, 131072), (2 ** 32 + 1, 16, 16)):
         assert lib.inv_int8_linear(call(T, N, K)) == bad
+
+
+def test_scales_that_ask_for_gradients_are_refused():
+    w, x = weight(6, 32), rows(2, 32, F32)
+    r = quantize_rows(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        int8_linear(x, Int8Weight(w.q, w.scale.clone().requires_grad_()))
+    with pytest.raises(RuntimeError, match="no gradient"):
+        int8_linear(Int8Rows(r.q, r.scale.clone().requires_grad_()), w)

@@ -322,3 +322,13 @@ def test_beside_products_that_hold_tensor_memory(i8):
     torch.cuda.synchronize()
     rt.check_status()
     assert all(torch.equal(y, want) for y in got[0]) and all(torch.equal(y, other) for y in got[1])
+
+
+def test_weights_and_scales_that_ask_for_gradients_are_refused():
+    a, b = inputs(4, 32, 16, 4, shared=True), inputs(4, 32, 16, 4, True, True)
+    ask = lambda w: Int8Weight(w.q, w.scale.clone().requires_grad_()) if isinstance(w, Int8Weight) else w.clone().requires_grad_()  # noqa: E731
+    for c in (a, b):
+        for bad in (dict(w_gate_up=ask(c["w_gate_up"])), dict(w_down=ask(c["w_down"])), dict(shared=(ask(c["shared"][0]), c["shared"][1])),
+                    dict(shared=(c["shared"][0], ask(c["shared"][1])))):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                moe_ffn_few(**{**c, **bad})
