@@ -28,7 +28,8 @@ def main(argv=None):
     ap.add_argument("--greedy", action="store_true")
     ap.add_argument("--ref-layout", action="store_true", help="matrices stored [in, out] as the reference's Linear reads them")
     ap.add_argument("--kv-format", default="oil4")
-    ap.add_argument("--weights", default=None, choices=("int8",), help="projections and experts in 8-bit integers with a scale for each channel")
+    ap.add_argument("--weights", default=None, choices=("int8",),
+                    help="projections and experts in 8-bit integers with a scale for each channel, beside the model's weights")
     ap.add_argument("--device", default="auto")
     ap.add_argument("--tokens", default="", help="comma-separated prompt token ids (no tokenizer needed)")
     a = ap.parse_args(argv)

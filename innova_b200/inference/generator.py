@@ -42,7 +42,8 @@ class Generator:
     def __init__(self, model, tokenizer=None, kv_format: str = "oil4", max_batch: int = 1, max_seq: Optional[int] = None, linear_fn=None,
                  num_pages: Optional[int] = None, weight_format: Optional[str] = None):
         """``weight_format="int8"``: projections and experts of the blocks in 8-bit integers with a scale for each channel (``ops.int8``), made here from the
-        model's weights, which stay as they are."""
+        model's weights, which stay as they are and where they are: the integers take half as much memory again. A mixture's shared expert with biases, adapters or
+        without a gate keeps the model's weights; experts that several ranks hold are refused."""
         self.model = model.eval()
         self.cfg = model.cfg
         self.tok = tokenizer
@@ -64,7 +65,7 @@ class Generator:
         if weight_format == "int8":
             linear_fn = Int8Linears(lin for blk in model.layers for part in (blk.attention, getattr(blk, "ffn", None)) if part is not None
                                     for lin in part.children() if isinstance(lin, torch.nn.Linear))
-            self.int8_experts = {blk: blk.moe.int8_weights() for blk in model.layers if hasattr(blk, "moe") and blk.moe.ep is None}
+            self.int8_experts = {blk: blk.moe.int8_weights() for blk in model.layers if hasattr(blk, "moe")}
         self.linear = linear_fn or (lambda x, lin: ops.linear(x, lin.weight, lin.bias))
 
     # ------------------------------------------------------------------ one forward over new tokens

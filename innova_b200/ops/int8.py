@@ -51,8 +51,9 @@ class Int8Weight(NamedTuple):
         """w [..., N, K] in bf16 or fp32. Nothing of the weight's size is held beside the result, unless w's rows have no even distance or no unit stride: then a copy."""
         return Int8Weight(*quantize_rows(w.detach()))
 
-    def dequantize(self) -> torch.Tensor:
-        return self.q.float() * self.scale.unsqueeze(-1)
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values that the codes stand for: products in fp32, rounded once to ``dtype``."""
+        return torch.mul(self.q, self.scale.unsqueeze(-1), out=torch.empty(self.q.shape, dtype=dtype, device=self.q.device))
 
 
 def refuse_gradients(what, *tensors):

@@ -157,3 +157,63 @@ def test_int8_generation_gpu(make):
     long = torch.randint(0, 97, (2, 100), generator=torch.Generator().manual_seed(7)).cuda()      # tiles, and mixtures as in training
     assert [len(o) for o in gen.generate_tokens(long, max_new_tokens=3)] == [3, 3]
     rt.check_status()
+
+
+def of_their_values(layer):
+    """The layer with its experts' weights as 8-bit integers stand for them."""
+    r = copy.deepcopy(layer)
+    with torch.no_grad():
+        for p in (r.w_gate_up, r.w_down) + ((r.shared.gate_up_proj.weight, r.shared.down_proj.weight) if r._plain_shared() else ()):
+            p.copy_(Int8Weight.quantize(p).dequantize())
+    return r
+
+
+@pytest.mark.parametrize("kw", [{}, dict(num_experts=260, moe_ffn_hidden_size=8), dict(num_experts=20, top_k=17, moe_ffn_hidden_size=8), dict(activation="gelu", bias=True)])
+@pytest.mark.parametrize("T", [1, 64, 65, 150, 600])
+def test_int8_experts_whatever_the_number_of_tokens(T, kw):
+    """Long prompts, many experts and many choices run on the 8-bit experts too, not on the weights that these were made from."""
+    m = mixture(**kw).layers[0].moe
+    g = torch.Generator().manual_seed(T)
+    h, x = torch.randn(2, T, 64, generator=g)[:, :T], torch.randn(2, T, 64, generator=g)
+    w = m.int8_weights()
+    with torch.no_grad():
+        y, want, plain = m.serve(h, x, w), of_their_values(m)(h, x)[0], m(h, x)[0]
+    assert y.shape == h.shape and int(m.last_counts.sum()) == 2 * T * m.cfg.top_k
+    # fp32 sums in another order: chains of 64 + 48 + 18 steps at most, each off by half a step of what is added up, which stays below the largest value; twice that
+    # for the activation between. The rounding of the weights to 8 bits is to be seen beyond it.
+    tol = 200 * 2.0 ** -24 * float(want.abs().max())
+    assert float((y - want).abs().max()) <= tol < 0.5 * float((y - plain).abs().max())
+    assert float((m.serve(h[:1, :1], x[:1, :1], w) - y[:1, :1]).abs().max()) <= tol
+
+
+def test_int8_experts_of_several_ranks_are_refused():
+    m = mixture()
+    m.layers[1].moe.ep = object()
+    with pytest.raises(ValueError, match="several ranks"):
+        Generator(m, kv_format="bf16", weight_format="int8")
+
+
+def test_dequantised_in_a_type():
+    w = Int8Weight.quantize(torch.randn(3, 5, 40))
+    assert torch.equal(w.dequantize(torch.bfloat16), w.dequantize().bfloat16()) and torch.equal(w.dequantize(), w.q.float() * w.scale.unsqueeze(-1))
+
+
+@gpu
+def test_int8_experts_whatever_the_number_of_tokens_gpu():
+    kw = dict(vocab_pad_to=128, hidden_size=256, num_heads=4, head_dim=64, moe_ffn_hidden_size=192, num_experts=8)
+    m = mixture(torch.bfloat16, "cuda", **kw).layers[0].moe
+    w, r = m.int8_weights(), of_their_values(m)
+    g = torch.Generator("cuda").manual_seed(1)
+    h, x = (torch.randn(1, 3000, 256, device="cuda", generator=g).bfloat16() for _ in range(2))
+    with torch.no_grad():
+        few = torch.cat([m.serve(h[:, i:i + 60], x[:, i:i + 60], w) for i in range(0, 3000, 60)], 1)
+        for T in (65, 130, 400, 512):
+            assert torch.equal(m.serve(h[:, :T], x[:, :T], w), few[:, :T])       # chunks: the same to the last bit
+        many, want = m.serve(h, x, w), r(h, x)[0]
+        assert torch.equal(many, want)                                            # the training form on the same rounded weights
+        # a handful of roundings to bf16 in each form
+        assert float((many.float() - few.float()).norm()) < 6 * 2.0 ** -8 * float(few.float().norm())
+        odd = mixture(torch.bfloat16, "cuda", **{**kw, "hidden_size": 248, "num_heads": 31, "num_kv_heads": 31, "head_dim": 8}).layers[0].moe      # no form in 8 bits for a few
+        for T in (3, 100):
+            assert torch.equal(odd.serve(h[:, :T, :248], x[:, :T, :248], odd.int8_weights()), of_their_values(odd)(h[:, :T, :248], x[:, :T, :248])[0])
+    rt.check_status()
