@@ -415,3 +415,33 @@ def test_scales_that_ask_for_gradients_are_refused():
         int8_linear(x, Int8Weight(w.q, w.scale.clone().requires_grad_()))
     with pytest.raises(RuntimeError, match="no gradient"):
         int8_linear(Int8Rows(r.q, r.scale.clone().requires_grad_()), w)
+
+
+def test_which_products_go_through_tiles():
+    """What the tests below mean to reach."""
+    import ctypes
+    from innova_b200 import _native
+    out = (ctypes.c_int * 13)()
+    for T, N, gated, route in ((3001, 2050, 0, 2), (2500, 2052, 1, 2), (2500, 896, 0, 1), (2500, 897, 0, 2), (2500, 896, 1, 1), (2500, 898, 1, 2), (128, 1 << 20, 0, 1), (129, 9473, 0, 2)):
+        assert _native.cuda().inv_int8_plan(T, N, 101, gated, ctypes.addressof(out)) == 0 and out[0] == route
+
+
+@gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype,out_dtype", [(BF, BF), (F32, F32), (BF, F32), (F32, BF)])
+def test_tiles(dtype, out_dtype, gated):
+    """Both results' boxes and rows off 16-byte boundaries, biases of both types, ends of K, of rows and of columns."""
+    for i, (T, K, N) in enumerate([(3001, 101, 2050), (2500, 129, 2052), (2561, 384, 4096), (2700, 257, 2064), (2400, 40, 3002)]):
+        product(T, K, N, dtype, out_dtype, (BF, F32, None)[(i + gated) % 3], gated, i)
+        product(T, K, N, dtype, out_dtype, (F32, None, BF)[(i + gated) % 3], gated, i + 10)
+
+
+@gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_on_both_sides_of_the_tiles_border(gated):
+    for T, N in ((2500, 896), (2500, 898), (129, 9472), (129, 9474), (300, 6272), (300, 6400)):
+        product(T, 200, N, BF, F32, F32, gated)
+        product(T, 77, N, F32, BF, None, gated, 3)
+    x, w = rows(2500, 200, BF).cuda(), weight(898, 200, device="cuda")
+    y = int8_linear(x, w)                                                    # tiles
+    assert torch.equal(int8_linear(x[:300], w), y[:300]) and torch.equal(int8_linear(x[-7:], w), y[-7:])      # a cluster's
