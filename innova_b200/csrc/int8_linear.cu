@@ -3,10 +3,12 @@
 //   s_t = max(|x_t|, 1e-10) / 127       c_tk = rint(x_tk / s_t), halves to even
 //   y_tn = s_t s_n sum_k c_tk q_nk + b_n            gated: silu(y_tn) y_t,n+F, n < F
 //
-// The sums are whole numbers below 2^31 (K <= 131071, codes from -128), so their order changes nothing; scales and bias are applied in fp32 and the result is rounded once.
+// The sums are whole numbers below 2^31 (K <= 131071, codes from -128), so their order changes nothing; scales and bias are applied in fp32 and the result is rounded
+// once.
 //
 // int8_rows_kernel      rows of activations into codes and scales
-// int8_few_kernel       one row, or up to four and weights of up to 32 MB: codes and product in one launch
+// int8_few_kernel       one row, or two and weights of up to 32 MB: codes and product in one launch
+// int8_few_mma_kernel   three or four rows, likewise
 // int8_split_kernel     up to 128 rows, or results of few tiles: tcgen05 kind::i8, clusters that share K
 // int8_tile_kernel      the rest: tiles of 256 x 256 on CTA pairs, tcgen05 kind::i8
 #include "cta_pair.cuh"
@@ -145,7 +147,7 @@ __device__ __forceinline__ uint64_t int8_fma2(uint64_t a, uint64_t b, uint64_t c
 // The scale of a row from the bits of its largest |x|: not a number is above infinity is above the rest. False where it is not finite.
 __device__ __forceinline__ bool int8_scale(uint32_t top, float& s, float& inv) {
   const bool finite = top < 0x7f800000u;
-  // a / 127 rounded to the nearest: the quotient by a product with 1 / 127, corrected by its remainder, which is exact
+  // a / 127 rounded to the nearest: a quotient corrected by its exact remainder (one step of Newton's method in rounded products and sums)
   constexpr float PART = 1.f / 127.f;
   const float a = finite ? fmaxf(__uint_as_float(top), INT8_LEAST) : 1.f, q = a * PART;
   s = finite ? fmaf(fmaf(-127.f, q, a), PART, q) : __uint_as_float(0x7fc00000u);
@@ -301,6 +303,8 @@ static int launch_int8_rows(const Int8Call& c, cudaStream_t st) {
 // The scales are multiplied first: a sum of codes, up to 2^31, times the scale of a token of 1e32 and more would not fit. The conversion, the scales' product and the
 // whole are rounded, half a step each.
 __device__ __forceinline__ float int8_value(int sum, float sx, float sw, float bias) { return fmaf((float)sum, sx * sw, bias); }
+// The quick exponential and quotient, as in the other products' epilogues (silu_f), for fp32 results too: off by 2 + 1.16 |x| and 2 units of 2^-23. Below -87 the quotient is 0
+// in place of -5e-37. Neither has a branch, so that a warp stays together between its loads from tensor memory.
 __device__ __forceinline__ float int8_silu(float x) { return __fdividef(x, 1.f + __expf(-x)); }
 
 // ---------------------------------------------------------------------------------------------- up to four rows
@@ -340,7 +344,9 @@ __device__ __forceinline__ float int8_bias(const void* b, int f32, int i) {
 //
 // Neither kind of product is fast on this GPU: some 8 cycles a scheduler for 32 lanes' four codes, some 80 for 16 x 8 x 32. 6144 x 4096, us, in products of
 // codes and of matrices: one row 7.4, 8.7; two 8.7, 9.4; four 11.6, 10.1. Against codes in front and tcgen05 tiles: one row 12288 x 4096 11.4, 13.6, 22016 x 4096 17.4,
-// 18.8, 22016 x 11008 42.3, 42.8: any size. Two rows 12288 x 4096 12.5, 13.7, but 4096 x 11008 14.1, 12.9, four rows of the former 15.5, 13.8: weights of up to 32 MB.
+// 18.8, 22016 x 11008 42.3, 42.8: any size. Two, three and four rows 7168 x 4096 9.7, 10.4, 10.8 against 10.7, 8192 x 4096 10.1, 11.1, 11.4 against 11.2, 12288 x 4096
+// 12.5, 14.6, 15.0 against 14.1, 32768 x 1024 9.4, 10.3, 10.4 against 10.5: weights of up to 32 MB, where three and four rows are even. Long rows of few weights lose on the
+// device, 2048 x 11008 11.3, 16.5, 17.4 against 9.9, and have the 4 us of a second launch on the host in return.
 
 // Codes of all rows into shared memory, `pitch` apart, with zeros up to `width`, and their scales.
 template <int TT>
@@ -1136,7 +1142,9 @@ extern "C" int inv_int8_plan(long T, long N, long K, int gated, int* out) {
 extern "C" int inv_int8_linear(const void* call) {
   const Int8Call& c = *static_cast<const Int8Call*>(call);
   if (c.T <= 0 || c.N <= 0 || c.K <= 0) return 0;
-  if (c.T > INT8_MOST || c.N > INT8_MOST || c.K > INT8_MOST_K || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2) || (c.gated && c.N < 2)) return -ERR_BAD_ARG;
+  if (c.T > INT8_MOST || c.N > INT8_MOST || c.K > INT8_MOST_K || c.ldw % 16 || c.ldc % 16 || (((uintptr_t)c.q | (uintptr_t)c.codes) & 15) || (c.gated && c.N % 2) ||
+      (c.gated && c.N < 2))
+    return -ERR_BAD_ARG;
   cudaStream_t st = (cudaStream_t)c.stream;
   int device = 0;
   if (const cudaError_t e = cudaGetDevice(&device)) return -(int)e;

@@ -6,7 +6,7 @@ InferenceEngine generate / stream / batch entry points (engines/inference/infere
 Prefill runs the flash-attention kernel on the whole prompt and appends K/V to the cache; every decode
 step runs the projections as skinny GEMMs and ``paged_decode`` attention over the (OIL4 or bf16) cache, or over an
 fp8 cache (``kv_format="fp8"``) one launch from the projection to the pages and one attention for any number of new tokens.
-``weight_format="int8"`` takes the blocks' projections and experts in 8-bit integers; mixture layers run up to 64 tokens in two launches.
+``weight_format="int8"`` takes the blocks' projections and experts in 8-bit integers, beside the model's weights; mixture layers run up to 64 tokens in two launches.
 """
 from __future__ import annotations
 

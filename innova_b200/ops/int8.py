@@ -3,7 +3,8 @@
 A row of activations is held as whole numbers c = rint(x / s) (halves to even) with s = max(|x|, 1e-10) / 127 in fp32, a scale for each token; a row of
 weights likewise, a scale for each output channel. Codes of the caller's own may be any int8, -128 among them. Sums of products are whole numbers that 32 bits hold up to
 K = 131071 (128 * 128 K < 2^31), so that a result depends on no order and not on how many tokens came with it; scales and bias are applied in fp32 and the result is rounded once. A row with a value that is not finite
-gives NaN. ``engines.int8_quantize_per_token`` and ``inference.serving.INT8Inference`` hold rows the same way; the product of the latter is of fp32.
+gives NaN. ``engines.int8_quantize_per_token`` and ``inference.serving.INT8Inference`` hold rows the same way but for quotients next to a half, which they take from rounded
+quotients; the product of the latter is of fp32.
 
 No gradient and no tangent passes through these."""
 from __future__ import annotations
@@ -175,7 +176,7 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], w: Int8Weight, bias: Optional[
 
 class Int8Linears:
     """A ``linear_fn`` of ``inference.Generator``: projections with their weights in 8-bit integers, laid out once; others as they are. The modules keep their
-    own weights, which later changes of them do not reach."""
+    own weights beside them, which later changes of them do not reach."""
 
     def __init__(self, linears):
         with torch.no_grad():
