@@ -1,9 +1,10 @@
 """Products with weights and activations in 8-bit integers (``csrc/int8_linear.cu``), for serving.
 
 A row of activations is held as whole numbers c = rint(x / s) (halves to even) with s = max(|x|, 1e-10) / 127 in fp32, a scale for each token; a row of
-weights likewise, a scale for each output channel. Codes of the caller's own may be any int8, -128 among them. Sums of products are whole numbers that 32 bits hold up to
-K = 131071 (128 * 128 K < 2^31), so that a result depends on no order and not on how many tokens came with it; scales and bias are applied in fp32 and the result is rounded once. A row with a value that is not finite
-gives NaN. ``engines.int8_quantize_per_token`` and ``inference.serving.INT8Inference`` hold rows the same way but for quotients next to a half, which they take from rounded
+weights likewise, a scale for each output channel. Codes of the caller's own may be any int8, -128 among them. Sums of products are whole numbers that 32 bits
+hold up to K = 131071 (128 * 128 K < 2^31), so that a result depends on no order and not on how many tokens came with it; scales and bias are applied in fp32 and the
+result is rounded once. A row with a value that is not finite gives NaN, and so does a sum of zero where a token's scale times a channel's is beyond fp32.
+``engines.int8_quantize_per_token`` and ``inference.serving.INT8Inference`` hold rows the same way but for quotients next to a half, which they take from rounded
 quotients; the product of the latter is of fp32.
 
 No gradient and no tangent passes through these."""
@@ -54,7 +55,10 @@ class Int8Weight(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the codes stand for: products in fp32, rounded once to ``dtype``."""
-        return torch.mul(self.q, self.scale.unsqueeze(-1), out=torch.empty(self.q.shape, dtype=dtype, device=self.q.device))
+        s = self.scale.unsqueeze(-1)
+        if dtype is _fp32 or s.requires_grad:
+            return (self.q * s).to(dtype)
+        return torch.mul(self.q, s, out=torch.empty(self.q.shape, dtype=dtype, device=self.q.device))      # nothing of fp32 held on the way
 
 
 def refuse_gradients(what, *tensors):

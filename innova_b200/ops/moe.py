@@ -323,7 +323,10 @@ def moe_ffn_few(x, router_w, w_gate_up: Weight, w_down: Weight, residual: Option
     between the products rounded to bf16, the result once. A token's result depends on no other. No gradient and no tangent passes through it."""
     T, D, inner, E, i8 = _few_check(x, router_w, w_gate_up, w_down, residual, top_k, shared)
     shared_up, shared_down = shared or (None, None)
-    refuse_gradients("moe_ffn_few", x, router_w, residual, *(w.scale if i8 else w for w in (w_gate_up, w_down, *(shared or ()))))
+    if i8:
+        refuse_gradients("moe_ffn_few", x, router_w, residual, w_gate_up.scale, w_down.scale, *(() if shared is None else (shared_up.scale, shared_down.scale)))
+    else:
+        refuse_gradients("moe_ffn_few", x, router_w, residual, w_gate_up, w_down, shared_up, shared_down)
     if not x.is_cuda:
         return _few_plain(x.reshape(T, D), router_w, (w_gate_up, w_down, *(shared or ())), residual, top_k, x.shape)
     out, counts = torch.empty_like(x, memory_format=torch.contiguous_format), x.new_empty(E, dtype=torch.int32)

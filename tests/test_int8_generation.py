@@ -196,6 +196,9 @@ def test_int8_experts_of_several_ranks_are_refused():
 def test_dequantised_in_a_type():
     w = Int8Weight.quantize(torch.randn(3, 5, 40))
     assert torch.equal(w.dequantize(torch.bfloat16), w.dequantize().bfloat16()) and torch.equal(w.dequantize(), w.q.float() * w.scale.unsqueeze(-1))
+    asked = Int8Weight(w.q, w.scale.clone().requires_grad_())
+    asked.dequantize(torch.bfloat16).sum().backward()
+    assert asked.scale.grad is not None
 
 
 @gpu
