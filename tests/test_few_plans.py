@@ -218,3 +218,34 @@ def test_layers_between_guards(seed):
             assert out.whole() and work.whole() and c.whole(), what
             assert torch.equal(out.view(BF, T, D), want) and torch.equal(c.view(torch.int32, E), counts), what
             assert int(counts.sum()) == T * k, what
+
+
+@gpu
+def test_back_to_back_over_changing_states():
+    """Hundreds of calls that nothing waits between, each form behind each other one, over inputs that change: what the last calls give is what they give alone."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    states = []
+    for T, K, N, dt, gated in ((1, 640, 1000, BF, False), (2, 333, 514, F32, True), (4, 640, 1000, BF, False), (16, 1024, 2048, BF, True), (64, 1411, 1002, F32, False),
+                               (200, 300, 900, BF, False), (2500, 128, 1026, F32, False), (2500, 200, 2052, BF, True)):
+        for _ in range(3):
+            x = torch.randn(T, K, device="cuda", generator=g).to(dt)
+            w = Int8Weight.quantize(torch.randn(N, K, device="cuda", generator=g))
+            states.append(lambda x=x, w=w, gated=gated: int8.int8_linear(x, w, gated=gated))
+    for T, D, F, E, k, i8 in ((1, 256, 512, 8, 2, True), (7, 512, 176, 64, 6, False), (30, 256, 320, 8, 2, True), (64, 512, 256, 16, 4, False)):
+        for _ in range(3):
+            x, router = (torch.randn(n, D, device="cuda", generator=g).to(BF) for n in (T, E))
+            w = [torch.randn(*s, device="cuda", generator=g) * s[-1] ** -0.5 for s in ((E, 2 * F, D), (E, D, F))]
+            w = [Int8Weight.quantize(v) if i8 else v.to(BF) for v in w]
+            states.append(lambda x=x, router=router, w=w, k=k: moe.moe_ffn_few(x, router, *w, x, k)[0])
+    alone = []
+    for run in states:
+        alone.append(run())
+        torch.cuda.synchronize()
+    rng = random.Random(3)
+    for _ in range(20):
+        order = list(range(len(states))) * 3
+        rng.shuffle(order)
+        last = {i: states[i]() for i in order}
+    torch.cuda.synchronize()
+    rt.check_status()
+    assert all(torch.equal(y, alone[i]) for i, y in last.items())
